@@ -20,6 +20,7 @@
 #include "kernels.h"
 #include "runtime.h"
 #include "bindings_hybrid.h"
+#include "bindings_vocab.h"
 #include "tma_host.h"
 
 namespace {
@@ -1756,4 +1757,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("allreduce_sum", &allreduce_sum);
   nrl::bind_runtime(m);
   nrl::bind_hybrid(m);
+  nrl::bind_vocab(m);
 }

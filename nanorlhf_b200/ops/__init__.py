@@ -150,6 +150,105 @@ class _LmHeadLogprobTorch(torch.autograd.Function):
         return dh if ctx.needs_input_grad[0] else None, dw, None, None, None
 
 
+# ---- a distribution over the vocabulary that another model gives, or that a sampler cuts -------------------------------------
+def _check_temperature(what, temperature):
+    if not 0.0 < float(temperature) < float("inf"):
+        raise ValueError(f"{what}: temperature must be positive and finite, got {temperature}")
+
+
+def top_logprobs(logits, k: int, temperature: float = 1.0):
+    """Log-probabilities of the ``k`` most probable tokens of every row of ``logits`` [T, V] (bf16 or float32) under softmax(logits / temperature):
+    (logp float32 [T, k], idx int32 [T, k]), most probable first, ties by the lower index.  Tokens without mass (logit -inf) are not listed: idx -1,
+    logp -inf in their places.  1 <= k <= min(V, 1024).  No gradient; a row with a NaN has NaN log-probabilities."""
+    _check_temperature("top_logprobs", temperature)
+    if logits.dim() != 2 or not 1 <= int(k) <= min(logits.shape[1], 1024):
+        raise ValueError(f"top_logprobs: logits [T, V] and 1 <= k <= min(V, 1024) are needed, got {tuple(logits.shape)} and k = {k}")
+    if use_native(logits):
+        return _nat().top_logprobs(logits, int(k), float(temperature))
+    return ref.top_logprobs(logits, int(k), float(temperature))
+
+
+def _check_teacher(what, rows, top_logp, top_idx, weights, temperature, beta, tail):
+    _check_temperature(what, temperature)
+    if top_logp.dim() != 2 or top_logp.shape != top_idx.shape or top_logp.shape[0] != rows or not 1 <= top_logp.shape[1] <= 1024:
+        raise ValueError(f"{what}: top_logp and top_idx must be [{rows}, K] with 1 <= K <= 1024, got {tuple(top_logp.shape)} and {tuple(top_idx.shape)}")
+    if top_idx.dtype not in (torch.int32, torch.int64) or not top_logp.is_floating_point():
+        raise TypeError(f"{what}: top_logp must be a floating-point tensor and top_idx int32 or int64")
+    if weights is not None and tuple(weights.shape) != (rows,):
+        raise ValueError(f"{what}: weights must be [{rows}], got {tuple(weights.shape)}")
+    if not 0.0 <= beta <= 1.0:
+        raise ValueError(f"{what}: beta must be between 0 and 1, got {beta}")
+    if not tail and beta != 0.0:
+        raise ValueError(f"{what}: tail=False goes with beta = 0 only")
+
+
+def distill_loss(logits, top_logp, top_idx, weights=None, temperature: float = 1.0, beta: float = 0.0, tail: bool = True):
+    """Divergence of a student, ``logits`` [T, V], from a teacher of whom the log-probabilities ``top_logp`` of ``top_idx`` [T, K] are known
+    (``top_logprobs``): (sum_t weights[t] * loss_t, loss_t float32 [T]).  The first has a gradient with respect to ``logits``, the second none.
+
+    With q = softmax(logits / temperature), P and Q are the teacher's and the student's probabilities of the K tokens and of *all others together*:
+    beta = 0: KL(P | Q); beta = 1: KL(Q | P); between: beta KL(P | M) + (1 - beta) KL(Q | M), M = beta P + (1 - beta) Q.  ``tail=False`` (beta = 0) scales
+    the teacher's K probabilities to a sum of 1 instead, and compares them with q as it is.
+    ``weights`` [T]: share of every token (a mask over its sum; None: 1 / T each); a row of weight 0 is not read, its loss and gradient are 0.  Put constant
+    factors (gradient accumulation) in there: the gradient is formed in the forward, and a backward from 1 hands it on as it is.
+    Entries of ``top_idx`` outside [0, V) are skipped, entries of one token add up; no entries and a tail: loss 0."""
+    if logits.dim() != 2:
+        raise ValueError(f"distill_loss: logits must be [T, V], got {tuple(logits.shape)}")
+    _check_teacher("distill_loss", logits.shape[0], top_logp, top_idx, weights, temperature, float(beta), tail)
+    if use_native(logits):
+        return _nat().distill_loss(logits, top_logp, top_idx, weights, float(temperature), float(beta), bool(tail))
+    return ref.distill_loss(logits, top_logp, top_idx, weights, float(temperature), float(beta), bool(tail))
+
+
+def lmhead_distill_loss(hidden, weight, top_logp, top_idx, weights=None, temperature: float = 1.0, beta: float = 0.0, tail: bool = True):
+    """``distill_loss`` of the logits ``hidden @ weight.T`` ([T, H], [V, H], bf16), which are formed in float32 and never handed over; gradients with
+    respect to ``hidden`` and ``weight``.  T may be any: what is held at a time does not grow with it."""
+    if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1]:
+        raise ValueError(f"lmhead_distill_loss: hidden [T, H] and weight [V, H] are needed, got {tuple(hidden.shape)} and {tuple(weight.shape)}")
+    _check_teacher("lmhead_distill_loss", hidden.shape[0], top_logp, top_idx, weights, temperature, float(beta), tail)
+    if use_native(hidden):
+        return _nat().lmhead_distill_loss(hidden, weight, top_logp, top_idx, weights, float(temperature), float(beta), bool(tail))
+    return ref.distill_loss(hidden @ weight.t(), top_logp, top_idx, weights, float(temperature), float(beta), bool(tail))
+
+
+def lmhead_top_logprobs(hidden, weight, k: int, temperature: float = 1.0):
+    """``top_logprobs`` of the logits ``hidden @ weight.T``, which are formed in float32 (bf16 on CUDA) a few thousand rows at a time.  No gradient."""
+    if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1]:
+        raise ValueError(f"lmhead_top_logprobs: hidden [T, H] and weight [V, H] are needed, got {tuple(hidden.shape)} and {tuple(weight.shape)}")
+    _check_temperature("lmhead_top_logprobs", temperature)
+    if not 1 <= int(k) <= min(weight.shape[0], 1024):
+        raise ValueError(f"lmhead_top_logprobs: 1 <= k <= min(V, 1024) is needed, got {k}")
+    if use_native(hidden):
+        return _nat().lmhead_top_logprobs(hidden, weight, int(k), float(temperature))
+    with torch.no_grad():
+        return ref.top_logprobs(hidden @ weight.t(), int(k), float(temperature))
+
+
+def sample_filtered(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """One token per row of ``logits`` [B, V] (bf16 or float32) from given random numbers: (tokens int32 [B], logp float32 [B]).
+
+    With w = exp((logit - largest) / temperature): tokens with w >= ``min_p`` are kept, of those the ``top_k`` first (largest logit first, ties by the lower
+    index), of those the fewest first whose mass is at least ``top_p`` of theirs.  The token is the first kept one, by index, up to which the kept mass
+    exceeds ``uniforms`` (float32 [B], in [0, 1)) times the whole; ``logp`` is its log-probability among the kept.  Masses are float64, so that the result is
+    that of the definition.  Every filter is a number or a tensor [B] (float32; ``top_k`` int32); 0 / 1 / 0 leave top_k / top_p / min_p out, temperature 0
+    takes the first token of the order (logp 0).  In tensors a value beyond its range counts as the nearest in it, NaN as left out (temperature: as 0).
+    NaN logits count as -inf; a row of nothing else has token -1, logp -inf."""
+    if logits.dim() != 2 or tuple(uniforms.shape) != (logits.shape[0],):
+        raise ValueError(f"sample_filtered: logits [B, V] and uniforms [B] are needed, got {tuple(logits.shape)} and {tuple(uniforms.shape)}")
+    if uniforms.dtype != torch.float32:
+        raise TypeError(f"sample_filtered: uniforms must be float32, got {uniforms.dtype}")
+    for name, x, hi in (("temperature", temperature, float("inf")), ("top_k", top_k, float("inf")), ("top_p", top_p, 1.0), ("min_p", min_p, 1.0)):
+        if torch.is_tensor(x) and x.dim() > 0:
+            want = torch.int32 if name == "top_k" else torch.float32
+            if tuple(x.shape) != (logits.shape[0],) or x.dtype != want:
+                raise ValueError(f"sample_filtered: {name} must be a number or a {want} tensor [{logits.shape[0]}], got {x.dtype} {tuple(x.shape)}")
+        elif not 0 <= x <= hi or x == float("inf"):
+            raise ValueError(f"sample_filtered: {name} is out of range: {x}")
+    if use_native(logits):
+        return _nat().sample_filtered(logits, uniforms, temperature, top_k, top_p, min_p)
+    return ref.sample_filtered(logits, uniforms, temperature, top_k, top_p, min_p)
+
+
 def discounted_suffix_sum(rewards, gamma=1.0):
     if use_native(rewards):
         return _nat().gae_scan(rewards, None, gamma, 1.0)[0]

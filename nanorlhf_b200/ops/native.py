@@ -236,6 +236,136 @@ def lmhead_logprob(hidden, weight, targets, temperature=1.0, want_entropy=True):
 
 
 # --------------------------------------------------------------------------------------------
+# a teacher's top log-probabilities and the divergence from them
+# --------------------------------------------------------------------------------------------
+def _row_major(logits):
+    return logits if logits.stride(1) == 1 or logits.shape[1] == 1 else logits.contiguous()
+
+
+@torch.no_grad()
+def top_logprobs(logits, k, temperature):
+    _count()
+    return ext().top_logprobs(_row_major(logits), k, 1.0 / temperature)
+
+
+def _teacher(logits_columns, top_logp, top_idx, weights):
+    if top_idx.dtype != torch.int32:
+        top_idx = top_idx.clamp(-1, logits_columns).to(torch.int32)          # what is no token stays none
+    return top_logp.detach().float().contiguous(), top_idx.contiguous(), None if weights is None else weights.detach().float().contiguous()
+
+
+def _scaled(grads, g, capture):
+    """``grads`` times the scalar ``g``; in place where this backward is the graph's only one, which frees them, and every replay of a captured one forms them again."""
+    keep = getattr(torch._C._autograd, "_get_current_graph_task_keep_graph", None)
+    if torch.is_grad_enabled() or keep is None or keep() or ext().capture_id() != capture or g.dtype != torch.float32:
+        return [None if x is None else x * g.to(x.dtype) if x.dtype == g.dtype else (x.float() * g).to(x.dtype) for x in grads]
+    for x in grads:
+        if x is not None:
+            _count()
+            ext().scale_(x, g)
+    return grads
+
+
+class _DistillFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, top_logp, top_idx, weights, temperature, beta, tail, need):
+        _count(2)
+        loss, token, grad = ext().distill_loss(logits, top_logp, top_idx, weights, 1.0 / temperature, beta, tail, need, False, True)
+        ctx.save_for_backward(grad)
+        ctx.capture = ext().capture_id()
+        ctx.mark_non_differentiable(token)
+        return loss, token
+
+    @staticmethod
+    def backward(ctx, g_loss, _g_token):
+        return (_scaled(ctx.saved_tensors, g_loss, ctx.capture)[0],) + (None,) * 7
+
+
+def distill_loss(logits, top_logp, top_idx, weights, temperature, beta, tail):
+    top_logp, top_idx, weights = _teacher(logits.shape[1], top_logp, top_idx, weights)
+    need = torch.is_grad_enabled() and logits.requires_grad
+    return _DistillFn.apply(_row_major(logits), top_logp, top_idx, weights, temperature, beta, tail, need)
+
+
+LOGITS_BYTES = 4 << 30      # float logits of a head that are held at a time
+
+
+def _row_ranges(rows, columns):
+    """as few equal ranges of rows as keep the float logits of one within LOGITS_BYTES"""
+    most = max(256, LOGITS_BYTES // (4 * columns) // 256 * 256)
+    n = max(1, -(-rows // most))
+    step = max(1, -(-rows // n))
+    return [(s, min(rows, s + step)) for s in range(0, rows, step)]
+
+
+class _LmHeadDistillFn(torch.autograd.Function):
+    """Logits, losses and the logits' gradients of a range of rows at a time, and with them at once the gradients of the hidden states and the head's, so that no
+    logits are formed twice: three GEMMs in all.  The backward only multiplies by the loss's own gradient."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, top_logp, top_idx, weights, temperature, beta, tail, need_h, need_w):
+        from . import gemm as _lin
+        h, rows, V = hidden.contiguous(), hidden.shape[0], weight.shape[0]
+        if weights is None:
+            weights = h.new_full((rows,), 1.0 / max(rows, 1), dtype=torch.float32)
+        ranges = _row_ranges(rows, V)
+        dh = torch.empty_like(h) if need_h else None
+        dw = torch.zeros(weight.shape, dtype=torch.float32, device=weight.device) if need_w and len(ranges) != 1 else None
+        tokens = []
+        for s, e in ranges:
+            z = torch.empty(e - s, V, dtype=torch.float32, device=h.device)
+            _lin.gemm(h[s:e], weight, out_f32=z)
+            _count()
+            _, token, dz = ext().distill_loss(z, top_logp[s:e], top_idx[s:e], weights[s:e], 1.0 / temperature, beta, tail, need_h or need_w, True, False)
+            tokens.append(token)
+            del z
+            if need_h:
+                _lin.gemm(dz, weight, b_mn=True, out=dh[s:e])
+            if need_w and len(ranges) == 1:
+                dw = _lin.gemm(dz, h, a_mn=True, b_mn=True, split_k=0)
+            elif need_w:
+                _lin.gemm(dz, h[s:e], a_mn=True, b_mn=True, out_f32=dw, accumulate=True)
+        token = tokens[0] if len(tokens) == 1 else torch.cat(tokens) if tokens else h.new_empty(0, dtype=torch.float32)
+        _count()
+        loss = ext().weighted_sum(token, weights)
+        ctx.save_for_backward(dh, None if dw is None else dw.to(weight.dtype))
+        ctx.capture = ext().capture_id()
+        ctx.mark_non_differentiable(token)
+        return loss, token
+
+    @staticmethod
+    def backward(ctx, g_loss, _g_token):
+        return tuple(_scaled(ctx.saved_tensors, g_loss, ctx.capture)) + (None,) * 8
+
+
+def lmhead_distill_loss(hidden, weight, top_logp, top_idx, weights, temperature, beta, tail):
+    from . import gemm as _lin
+    if not _lin.supported(hidden, weight):                 # other types and sizes than the GEMM's: their logits, in float32
+        return distill_loss(F.linear(hidden.float(), weight.float()), top_logp, top_idx, weights, temperature, beta, tail)
+    top_logp, top_idx, weights = _teacher(weight.shape[0], top_logp, top_idx, weights)
+    grad = torch.is_grad_enabled()
+    return _LmHeadDistillFn.apply(hidden, weight, top_logp, top_idx, weights, temperature, beta, tail, grad and hidden.requires_grad,
+                                  grad and weight.requires_grad)
+
+
+@torch.no_grad()
+def lmhead_top_logprobs(hidden, weight, k, temperature):
+    from . import gemm as _lin
+    rows, V = hidden.shape[0], weight.shape[0]
+    logp = torch.empty(rows, k, dtype=torch.float32, device=hidden.device)
+    idx = torch.empty(rows, k, dtype=torch.int32, device=hidden.device)
+    h = hidden.contiguous()
+    for s, e in _row_ranges(rows, V):
+        if _lin.supported(h, weight):
+            z = torch.empty(e - s, V, dtype=torch.float32, device=h.device)
+            _lin.gemm(h[s:e], weight, out_f32=z)
+        else:
+            z = F.linear(h[s:e].float(), weight.float())
+        logp[s:e], idx[s:e] = top_logprobs(z, k, temperature)
+    return logp, idx
+
+
+# --------------------------------------------------------------------------------------------
 # RL kernels
 # --------------------------------------------------------------------------------------------
 def gae_scan(rewards, values, gamma, lam):
@@ -299,6 +429,22 @@ def adamw_flat(param, grad, m, v, lr, beta1, beta2, eps, wd, step, scale=1.0, ma
 def sample(logits, temperature, top_p, seed, step, row_ids=None, row_steps=None, out=None, impl=0):
     _count()
     return ext().sample(logits, float(temperature), float(top_p), int(seed), int(step), row_ids, row_steps, out, int(impl))
+
+
+def row_uniforms(seed, step, row_ids, row_steps=None):
+    """float32 [rows] in [0, 1), functions of (seed, row_ids[i], step + row_steps[i]) alone."""
+    _count()
+    return ext().row_uniforms(int(seed), int(step), row_ids, row_steps)
+
+
+@torch.no_grad()
+def sample_filtered(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    _count()
+    args = []
+    for x, off in ((temperature, 1.0), (top_k, 0), (top_p, 1.0), (min_p, 0.0)):
+        each = torch.is_tensor(x) and x.dim() > 0
+        args += [x.contiguous(), off] if each else [None, type(off)(x)]
+    return ext().sample_filtered(_row_major(logits), uniforms.contiguous(), *args)
 
 
 def kv_cache_write(k, v, k_cache, v_cache, slot_mapping, src_index=None):

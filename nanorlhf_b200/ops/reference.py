@@ -326,6 +326,93 @@ def top_p_sample(logits: torch.Tensor, temperature: float, top_p: float,
     return torch.multinomial(probs, 1, generator=generator).squeeze(1)
 
 
+# --------------------------------------------------------------------------------------------
+# a teacher's top log-probabilities, the divergence from them, filtered sampling
+# --------------------------------------------------------------------------------------------
+@torch.no_grad()
+def top_logprobs(logits: torch.Tensor, k: int, temperature: float = 1.0):
+    z = logits.double()
+    v, i = torch.where(z.isnan(), -math.inf, z).sort(dim=-1, descending=True, stable=True)
+    best, v, i = v[:, :1], v[:, :k], i[:, :k]
+    log_sum = torch.where(z == best, 0.0, (z - best) / temperature).exp().sum(-1, keepdim=True).log()
+    none = v == -math.inf
+    return (torch.where(v == best, 0.0, (v - best) / temperature) - log_sum).masked_fill(none, -math.inf).float(), i.masked_fill(none, -1).int()
+
+
+def distill_loss(logits: torch.Tensor, top_logp: torch.Tensor, top_idx: torch.Tensor, weights: Optional[torch.Tensor], temperature: float, beta: float,
+                 tail: bool):
+    """``ops.distill_loss`` over dense [T, V] probabilities in float64, differentiable by autograd."""
+    T, V = logits.shape
+    w = torch.full((T,), 1.0 / max(T, 1), dtype=torch.float64, device=logits.device) if weights is None else weights.double()
+    live = (w != 0)[:, None]
+    lq = torch.log_softmax(torch.where(live, logits, 0).double() / temperature, -1)
+    at = torch.where((top_idx >= 0) & (top_idx < V), top_idx, V).long()
+    P = torch.zeros(T, V + 1, dtype=torch.float64, device=logits.device).scatter_add(1, at, top_logp.detach().double().exp())[:, :V]
+    K = torch.zeros(T, V + 1, dtype=torch.bool, device=logits.device).scatter(1, at, True)[:, :V]
+    total = P.sum(-1, keepdim=True)
+
+    def plogs(p, *logs):                      # p * (logs[0] - logs[1]) where p > 0, without a gradient through what is masked
+        ok = p > 0
+        return torch.where(ok, torch.where(ok, p, 1.0) * (torch.where(ok, logs[0], 0.0) - torch.where(ok, logs[1], 0.0)), 0.0)
+
+    if not tail:
+        P = P / torch.where(total > 0, total, 1.0)
+        token = plogs(P, P.log(), lq).sum(-1)
+    else:
+        r = 1.0 - total
+        r = torch.where(r > 2.0 ** -24, r, 0.0)
+        none = K.all(-1, keepdim=True) | (lq.masked_fill(K, -math.inf) == -math.inf).all(-1, keepdim=True)
+        ls = torch.logsumexp(torch.where(none, 0.0, lq.masked_fill(K, -math.inf)), -1, keepdim=True)
+        ls = torch.where(none, -math.inf, ls)
+        P, lQ = torch.cat([P, r], -1), torch.cat([lq, ls], -1)
+        on = torch.cat([K, torch.ones_like(r, dtype=torch.bool)], -1)
+        lP = torch.cat([P[:, :V].log(), r.clamp_min(2.0 ** -24).log()], -1)
+        Q = torch.where(on, lQ.exp(), 0.0)
+        P = torch.where(on, P, 0.0)
+        if beta == 0.0:
+            token = plogs(P, P.log(), lQ).sum(-1)
+        elif beta == 1.0:
+            token = plogs(Q, lQ, lP).sum(-1)
+        else:
+            M = (beta * P + (1.0 - beta) * Q)
+            lM = torch.where(M > 0, M, 1.0).log()
+            token = beta * plogs(P, P.log(), lM).sum(-1) + (1.0 - beta) * plogs(Q, lQ, lM).sum(-1)
+    token = torch.where(live[:, 0], token, 0.0)
+    return (token * w).sum().float(), token.detach().float()
+
+
+@torch.no_grad()
+def sample_filtered(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    B, V = logits.shape
+    if B == 0:
+        return torch.empty(0, dtype=torch.int32, device=logits.device), torch.empty(0, device=logits.device)
+
+    def row(x):
+        return (x.double() if torch.is_tensor(x) else torch.tensor(float(x), dtype=torch.float64, device=logits.device)).expand(B)[:, None]
+
+    T, K, P, M = row(temperature), row(top_k), row(top_p), row(min_p).clamp_max(1.0)
+    z = torch.where(logits.isnan(), -math.inf, logits.double())
+    vals, order = z.sort(dim=-1, descending=True, stable=True)
+    best = vals[:, :1]
+    hot = T > 0
+    x = torch.where(z == best, 0.0, (z - best) / torch.where(hot, T, 1.0))
+    w = x.exp().masked_fill(z == -math.inf, 0.0)
+    ws = w.gather(1, order)
+    rank = torch.arange(V, device=logits.device)
+    keep = ~(ws < M) & (ws > 0) & ((rank < K) | ~(K > 0))
+    cum = (ws * keep).cumsum(-1)
+    keep &= ((cum - ws * keep) < P * cum[:, -1:]) | ~(P < 1.0) | (rank == 0)
+    kept = torch.zeros_like(keep).scatter(1, order, keep)
+    cum = (w * kept).cumsum(-1)
+    over = cum > uniforms[:, None].double() * cum[:, -1:]
+    last = torch.where(kept & (w > 0), rank, -1).amax(-1)
+    token = torch.where(over.any(-1), over.byte().argmax(-1), last)
+    token = torch.where(hot[:, 0], token, order[:, 0])
+    logp = torch.where(hot[:, 0], x.gather(1, token.clamp_min(0)[:, None])[:, 0] - cum[:, -1].log(), 0.0)
+    empty = best[:, 0] == -math.inf
+    return torch.where(empty, -1, token).int(), torch.where(empty, -math.inf, logp).float()
+
+
 class _LoraLinearRef(torch.autograd.Function):
     """PyTorch oracle / CPU backend of ``ops.lora_linear``: the rank-r update folded into the base GEMM's output
     (``addmm_`` with beta = 1), autograd keeps only x and the [T, r] projection; the base weight is frozen."""
