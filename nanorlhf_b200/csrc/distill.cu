@@ -19,12 +19,6 @@
 
 namespace nrl {
 
-NRL_DEVICE float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
 template <typename T, typename G>
 __global__ void __launch_bounds__(kRowThreads) distill_kernel(const T* __restrict__ logits, long row_stride, int V, const float* __restrict__ top_logp,
                                                               const int* __restrict__ top_idx, int K, const float* __restrict__ weights, double inv_temp,

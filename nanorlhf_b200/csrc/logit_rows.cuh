@@ -19,28 +19,74 @@ constexpr uint32_t kKeyNone = 0x007fffffu;             // -infinity: no mass
 
 NRL_DEVICE float clean(float z) { return z == z ? z : -INFINITY; }
 
+// 32 bytes of logits as they lie in memory, and arithmetic on them in pairs
+struct RawVec { uint32_t w[8]; };
+NRL_DEVICE uint64_t pair_of(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+NRL_DEVICE uint64_t pair_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+NRL_DEVICE uint64_t pair_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+NRL_DEVICE float2 pair_parts(uint64_t a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+  return r;
+}
+NRL_DEVICE uint64_t pair_both(float x) { return pair_of(__float_as_uint(x), __float_as_uint(x)); }
+NRL_DEVICE float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 template <typename T>
 struct LogitRow {
-  static constexpr int N = 16 / sizeof(T);             // elements of a 16-byte vector
+  static constexpr int N = 32 / sizeof(T);             // elements of a 32-byte vector
   const T* p;
   int V, skew, nvec;                                   // vector v holds the elements v * N - skew ...; the row starts `skew` elements into the first
   NRL_DEVICE LogitRow(const T* row, int v) : p(row), V(v) {
-    skew = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    skew = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 31) / sizeof(T));
     nvec = (V + skew + N - 1) / N;
   }
   NRL_DEVICE static float value(T x);
+  NRL_DEVICE static uint32_t none();                   // a word of -infinity
+  NRL_DEVICE static void put(RawVec& a, int j, T x);   // element j of a vector
   // elements outside the row are -infinity and are not read
-  NRL_DEVICE void load(int v, float (&x)[N]) const {
+  NRL_DEVICE RawVec raw(int v) const {
+    RawVec a;
     const int e0 = v * N - skew;
     if (e0 >= 0 && e0 + N <= V) {
-      const uint4 a = ldg_nc_v4(p + e0);
-      unpack(a, x);
+      asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(a.w[0]), "=r"(a.w[1]), "=r"(a.w[2]), "=r"(a.w[3]), "=r"(a.w[4]), "=r"(a.w[5]), "=r"(a.w[6]), "=r"(a.w[7])
+                   : "l"(p + e0));
     } else {
 #pragma unroll
-      for (int j = 0; j < N; ++j) x[j] = e0 + j >= 0 && e0 + j < V ? value(p[e0 + j]) : -INFINITY;
+      for (int j = 0; j < 8; ++j) a.w[j] = none();
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (e0 + j >= 0 && e0 + j < V) put(a, j, p[e0 + j]);
     }
+    return a;
   }
-  NRL_DEVICE static void unpack(const uint4& a, float (&x)[N]);
+  NRL_DEVICE static RawVec no_vec() {
+    RawVec a;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a.w[j] = none();
+    return a;
+  }
+  NRL_DEVICE static void unpack(const RawVec& a, float (&x)[N]);
+  NRL_DEVICE static float largest(const RawVec& a);    // NaN left aside
+  NRL_DEVICE static uint64_t pair(const RawVec& a, int i);        // elements 2 i and 2 i + 1
+  NRL_DEVICE void load(int v, float (&x)[N]) const { unpack(raw(v), x); }
   NRL_DEVICE float at(int e) const { return value(p[e]); }
   // every element of this warp's range: the warps have consecutive ranges of the row, their lanes interleaved vectors; f(index, logit)
   template <class F>
@@ -61,17 +107,47 @@ NRL_DEVICE float LogitRow<float>::value(float x) { return x; }
 template <>
 NRL_DEVICE float LogitRow<__nv_bfloat16>::value(__nv_bfloat16 x) { return __bfloat162float(x); }
 template <>
-NRL_DEVICE void LogitRow<float>::unpack(const uint4& a, float (&x)[4]) {
-  x[0] = __uint_as_float(a.x); x[1] = __uint_as_float(a.y); x[2] = __uint_as_float(a.z); x[3] = __uint_as_float(a.w);
+NRL_DEVICE uint32_t LogitRow<float>::none() { return 0xff800000u; }
+template <>
+NRL_DEVICE uint32_t LogitRow<__nv_bfloat16>::none() { return 0xff80ff80u; }
+template <>
+NRL_DEVICE void LogitRow<float>::put(RawVec& a, int j, float x) { a.w[j] = __float_as_uint(x); }
+template <>
+NRL_DEVICE void LogitRow<__nv_bfloat16>::put(RawVec& a, int j, __nv_bfloat16 x) {
+  const uint32_t b = __bfloat16_as_ushort(x);
+  a.w[j / 2] = j % 2 ? (a.w[j / 2] & 0xffffu) | b << 16 : (a.w[j / 2] & 0xffff0000u) | b;
 }
 template <>
-NRL_DEVICE void LogitRow<__nv_bfloat16>::unpack(const uint4& a, float (&x)[8]) {
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+NRL_DEVICE uint64_t LogitRow<float>::pair(const RawVec& a, int i) { return pair_of(a.w[2 * i], a.w[2 * i + 1]); }
+template <>
+NRL_DEVICE uint64_t LogitRow<__nv_bfloat16>::pair(const RawVec& a, int i) { return pair_of(a.w[i] << 16, a.w[i] & 0xffff0000u); }
+template <>
+NRL_DEVICE void LogitRow<float>::unpack(const RawVec& a, float (&x)[8]) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    x[2 * j] = __uint_as_float(w[j] << 16);
-    x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+  for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(a.w[j]);
+}
+template <>
+NRL_DEVICE void LogitRow<__nv_bfloat16>::unpack(const RawVec& a, float (&x)[16]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    x[2 * j] = __uint_as_float(a.w[j] << 16);
+    x[2 * j + 1] = __uint_as_float(a.w[j] & 0xffff0000u);
   }
+}
+template <>
+NRL_DEVICE float LogitRow<float>::largest(const RawVec& a) {
+  float m = __uint_as_float(a.w[0]);
+#pragma unroll
+  for (int j = 1; j < 7; j += 2) asm("max.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(__uint_as_float(a.w[j])), "f"(__uint_as_float(a.w[j + 1])));
+  return fmaxf(m, __uint_as_float(a.w[7]));
+}
+template <>
+NRL_DEVICE float LogitRow<__nv_bfloat16>::largest(const RawVec& a) {
+  __nv_bfloat162 m = *reinterpret_cast<const __nv_bfloat162*>(&a.w[0]);
+#pragma unroll
+  for (int j = 1; j < 8; ++j) m = __hmax2(m, *reinterpret_cast<const __nv_bfloat162*>(&a.w[j]));
+  const float2 f = __bfloat1622float2(m);
+  return fmaxf(f.x, f.y);
 }
 
 // Reductions over the block, in one order; every thread gets the result.  `red`: kRowWarps entries that nobody else uses until the next barrier.
@@ -192,6 +268,286 @@ NRL_DEVICE Border find_border(const LogitRow<T>& row, uint32_t lo, uint32_t top,
   }
   __syncthreads();
   return {key, sh.cut};
+}
+
+// ---- a row shared by the blocks of a cluster, and read once ---------------------------------------------------------------------------------------
+NRL_DEVICE uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+NRL_DEVICE uint32_t cluster_blocks() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
+NRL_DEVICE void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+NRL_DEVICE void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// the address of `p` (a shared-memory object of this block) in the shared memory of the cluster's block `rank`
+NRL_DEVICE uint32_t in_block(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+NRL_DEVICE void st_block(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
+NRL_DEVICE void st_block(uint32_t addr, double v) { asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory"); }
+NRL_DEVICE void st_block(uint32_t addr, uint64_t v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory"); }
+NRL_DEVICE int add_block(uint32_t addr, int v) {
+  int r;
+  asm volatile("atom.relaxed.cluster.shared::cluster.add.s32 %0, [%1], %2;" : "=r"(r) : "r"(addr), "r"(v) : "memory");
+  return r;
+}
+
+constexpr int kRowClusterMax = 8;
+constexpr int kRowUnroll = 2;                          // vectors of a thread in flight
+constexpr int kRowChunks = 16;                         // of a thread's vectors, each with a maximum of its own
+
+// The vectors of this block: thread t has first + t, first + t + kRowThreads, ..., in `chunks` chunks of `len`.
+struct RowShare {
+  int first, end, len, chunks;
+  NRL_DEVICE RowShare(int nvec, int rank, int blocks) {
+    const int per = (nvec + blocks - 1) / blocks;
+    first = min(nvec, rank * per);
+    end = min(nvec, first + per);
+    const int steps = (end - first + kRowThreads - 1) / kRowThreads;
+    len = (steps + kRowChunks * kRowUnroll - 1) / (kRowChunks * kRowUnroll) * kRowUnroll;
+    chunks = len > 0 ? (steps + len - 1) / len : 0;
+  }
+};
+// chunks of any block of the cluster at most, wherever the row starts (host)
+inline int row_chunks(int V, int vec, int blocks) {
+  const long nvec = (static_cast<long>(V) + 2 * vec - 2) / vec, per = (nvec + blocks - 1) / blocks, steps = (per + kRowThreads - 1) / kRowThreads;
+  return steps < kRowChunks * kRowUnroll ? static_cast<int>((steps + kRowUnroll - 1) / kRowUnroll) : kRowChunks;
+}
+
+// Blocks of a row's cluster (host).  A row of its own block is fastest where the rows fill the SMs; of few rows the cluster shares the reading, until its barriers
+// cost more.  us with 1 / 2 / 4 / 8 blocks (top 20 to 64 of bf16 rows of 151 936): 1 row 15.8 / 11.9 / 10.1 / 10.1, 8 rows 20.8 / 14.7 / 12.0 / 11.2, 32 rows 23.3 / 17.2 /
+// 15.6 / 28.4, 100 rows 23.3 / 20.5 / 25.9 / 51, 300 rows 36.6 / 42.6 / 62 / 118; 64 rows of 32 000 10.1 / 10.3 / 16.3 / 34, of 4000 floats 6.6 / 7.7 / 10.0 / 18.7.
+inline int row_blocks(long rows, int V, int vec) {
+  constexpr int kSms = 148;
+  const long nvec = V / vec;
+  int blocks = rows <= kSms / 8 ? 8 : rows <= kSms / 4 ? 4 : rows <= kSms ? 2 : 1;
+  while (blocks > 1 && nvec < 1024L * blocks) blocks /= 2;
+  return blocks;
+}
+
+// One pass over the block's share: thread-wise maximum `best`, sum s of 2^((z - m) c), m = best or the lowest float, and the maximum of every chunk.  The sum's reference moves with the
+// maximum, once for the kRowUnroll vectors of a step.  z - m is formed before the multiplication: m c would round at the size of the logits.
+// skip(v, a) may take elements of vector v out of the sum by making them -infinity.
+template <typename T, class S>
+NRL_DEVICE void row_pass(const LogitRow<T>& row, const RowShare& sh, float c, float* chunk_max, float& best, float& m, float& s, S&& skip) {
+  m = -3.402823466e38f;                                // finite, so that -infinity is 0 in the sum
+  s = 0.f;
+  best = -INFINITY;
+  const uint64_t c2 = pair_both(c);
+  for (int i = 0; i < sh.chunks; ++i) {
+    float cm = -INFINITY;
+    const int v0 = sh.first + i * sh.len * kRowThreads + static_cast<int>(threadIdx.x);
+    for (int u = 0; u < sh.len; u += kRowUnroll) {
+      RawVec a[kRowUnroll];
+#pragma unroll
+      for (int j = 0; j < kRowUnroll; ++j) {
+        const int v = v0 + (u + j) * kRowThreads;
+        a[j] = v < sh.end ? row.raw(v) : LogitRow<T>::no_vec();
+      }
+      float l = LogitRow<T>::largest(a[0]);
+#pragma unroll
+      for (int j = 1; j < kRowUnroll; ++j) l = fmaxf(l, LogitRow<T>::largest(a[j]));
+      cm = fmaxf(cm, l);
+      const float mn = fmaxf(m, l);
+      const uint64_t neg = pair_both(-mn);
+      uint64_t sum = 0;
+#pragma unroll
+      for (int j = 0; j < kRowUnroll; ++j) {
+        skip(v0 + (u + j) * kRowThreads, a[j]);
+#pragma unroll
+        for (int q = 0; q < LogitRow<T>::N / 2; ++q) {
+          const float2 e = pair_parts(pair_mul(pair_add(LogitRow<T>::pair(a[j], q), neg), c2));
+          sum = pair_add(sum, pair_of(__float_as_uint(ex2(e.x)), __float_as_uint(ex2(e.y))));
+        }
+      }
+      const float2 p = pair_parts(sum);
+      s = s * ex2((m - mn) * c) + (p.x + p.y);
+      m = mn;
+    }
+    best = fmaxf(best, cm);
+    chunk_max[i * kRowThreads + threadIdx.x] = cm;
+  }
+}
+
+// The bound of a block's candidates: a key that at least `want` of the block's groups' maxima reach (`keys`: this thread's, `groups` of them) and few more, by
+// a histogram of 256 equal ranges of keys between the least and the largest, and one of the range that holds the want-th where it holds many;
+// kKeyNone + 1 where fewer groups have any mass.  600 cycles; bit by bit with counts of one warp 4000.
+struct BoundShared {
+  int bins[2][256];
+  uint32_t lo[kRowWarps], hi[kRowWarps];
+};
+constexpr int kGroupsMax = 4;
+// of `bins`, the highest b that has, with those above, at least `want` counts; every lane gets b, what lies above it and what it holds
+NRL_DEVICE int highest_bin(const int* bins, int want, int& above, int& holds) {
+  const int lane = static_cast<int>(lane_id());
+  int n[8], sum = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum += n[i] = bins[lane * 8 + i];
+  int incl = sum;                                      // of this lane's bins and those above
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_down_sync(0xffffffffu, incl, o);
+    if (lane + o < 32) incl += y;
+  }
+  const unsigned reach = __ballot_sync(0xffffffffu, incl >= want);
+  const int owner = reach ? 31 - __clz(reach) : 0;
+  int b = lane * 8 + 7, h = n[7], a = incl - sum;       // a: above bin b
+#pragma unroll
+  for (int i = 6; i >= 0; --i)
+    if (a + h < want) {
+      a += h;
+      b = lane * 8 + i;
+      h = n[i];
+    }
+  above = __shfl_sync(0xffffffffu, a, owner);
+  holds = __shfl_sync(0xffffffffu, h, owner);
+  return __shfl_sync(0xffffffffu, b, owner);
+}
+NRL_DEVICE uint32_t group_bound(const uint32_t (&keys)[kGroupsMax], int groups, int want, BoundShared& sh) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  uint32_t lo = 0xffffffffu, hi = 0;
+#pragma unroll
+  for (int g = 0; g < kGroupsMax; ++g)
+    if (g < groups && keys[g] > kKeyNone) {
+      lo = min(lo, keys[g]);
+      hi = max(hi, keys[g]);
+    }
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  if (lane == 0) {
+    sh.lo[tid >> 5] = lo;
+    sh.hi[tid >> 5] = hi;
+  }
+  sh.bins[tid >> 8][tid & 255] = 0;
+  static_assert(kRowThreads == 512, "a thread a bin");
+  __syncthreads();
+  lo = __reduce_min_sync(0xffffffffu, sh.lo[lane % kRowWarps]);
+  hi = __reduce_max_sync(0xffffffffu, sh.hi[lane % kRowWarps]);
+  if (hi == 0) return kKeyNone + 1;
+  int bits = 32 - __clz(hi - lo);                      // keys differ from lo in so many bits at most
+#pragma unroll 1
+  for (int level = 0;; ++level) {
+    const int shift = bits > 8 ? bits - 8 : 0;
+#pragma unroll
+    for (int g = 0; g < kGroupsMax; ++g)
+      if (g < groups && keys[g] > kKeyNone && keys[g] >= lo && (bits == 32 || (keys[g] - lo) >> bits == 0)) atomicAdd(&sh.bins[level][(keys[g] - lo) >> shift], 1);
+    __syncthreads();
+    int above, holds;
+    const int b = highest_bin(sh.bins[level], want, above, holds);
+    if (above + holds < want) return kKeyNone + 1;
+    lo += static_cast<uint32_t>(b) << shift;
+    if (level == 1 || shift == 0 || holds <= 8 + want / 4) return lo;
+    want -= above;
+    bits = shift;
+  }
+}
+
+// What a block has gathered of its share.
+constexpr int kCandidates = 2048;
+struct RowList {
+  uint64_t cand[kCandidates];                          // (key, ~index): unsigned numbers in the order; those that other blocks send from the end on
+  unsigned short hits[kCandidates];
+  int n, nhits, sent;
+};
+// Into `list` all elements of the share whose keys reach `bound`: the chunks that have any (by their maxima) are read again, a vector a thread.  list.n and
+// list.nhits are 0 before; above kCandidates they say that there is more than what the list holds.
+template <typename T>
+NRL_DEVICE void gather_candidates(const LogitRow<T>& row, const RowShare& share, const float* chunk_max, uint32_t bound, RowList& list) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  unsigned mine = 0;
+#pragma unroll 4
+  for (int i = 0; i < share.chunks; ++i) mine |= (order_key(chunk_max[i * kRowThreads + tid]) >= bound ? 1u : 0u) << i;
+  if (__any_sync(0xffffffffu, mine != 0)) {
+    int incl = __popc(mine), base = 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) base = atomicAdd(&list.nhits, incl);
+    base = __shfl_sync(0xffffffffu, base, 31) + incl - __popc(mine);
+    for (; mine != 0; mine &= mine - 1, ++base)
+      if (base < kCandidates) list.hits[base] = static_cast<unsigned short>((__ffs(mine) - 1) * kRowThreads + tid);
+  }
+  __syncthreads();
+  const int vecs = min(list.nhits, kCandidates) * share.len;
+  for (int i = tid; i < vecs; i += kRowThreads) {
+    const int hit = list.hits[i / share.len], v = share.first + (hit / kRowThreads * share.len + i % share.len) * kRowThreads + hit % kRowThreads;
+    if (v >= share.end) continue;
+    const RawVec a = row.raw(v);
+    if (order_key(LogitRow<T>::largest(a)) < bound) continue;
+    float x[LogitRow<T>::N];
+    LogitRow<T>::unpack(a, x);
+    unsigned in = 0;
+#pragma unroll
+    for (int j = 0; j < LogitRow<T>::N; ++j) in |= (order_key(clean(x[j])) >= bound ? 1u : 0u) << j;
+    for (int at = atomicAdd(&list.n, __popc(in)); in != 0 && at < kCandidates; in &= in - 1, ++at) {
+      const int e = v * LogitRow<T>::N - row.skew + __ffs(in) - 1;
+      list.cand[at] = static_cast<uint64_t>(order_key(row.at(e))) << 32 | static_cast<uint32_t>(~e);
+    }
+  }
+  __syncthreads();
+}
+// The list to the first block's; a cluster barrier in front, by which that block is known to run, and one behind.
+NRL_DEVICE void send_candidates(const RowList& list, int* s_base) {
+  const uint32_t there = in_block(list.cand, 0);
+  const int n = list.n > kCandidates || list.nhits > kCandidates ? kCandidates + 1 : list.n;
+  if (threadIdx.x == 0) *s_base = add_block(in_block(&list.sent, 0), n);
+  __syncthreads();
+  for (int i = threadIdx.x; i < min(n, kCandidates) && *s_base + i < kCandidates; i += kRowThreads)
+    st_block(there + (kCandidates - 1 - *s_base - i) * 8, list.cand[i]);
+}
+// Behind the barrier, the first block: what came to its own, side by side; returns how many there are, above kCandidates where they do not fit.
+NRL_DEVICE int join_candidates(RowList& list) {
+  const int own = list.nhits > kCandidates ? kCandidates + 1 : list.n, sent = list.sent, all = own + sent;
+  if (sent == 0 || all > kCandidates) return all;
+  uint64_t x[kCandidates / kRowThreads];
+#pragma unroll
+  for (int t = 0; t < kCandidates / kRowThreads; ++t) {
+    const int i = threadIdx.x + t * kRowThreads;
+    if (i < sent) x[t] = list.cand[kCandidates - 1 - i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int t = 0; t < kCandidates / kRowThreads; ++t) {
+    const int i = threadIdx.x + t * kRowThreads;
+    if (i < sent) list.cand[own + i] = x[t];
+  }
+  __syncthreads();
+  return all;
+}
+
+// Candidates in their order: f(place, candidate) for the first n of them, behind a barrier.  Up to one a thread each counts those before it; more are sorted.
+template <class F>
+NRL_DEVICE void in_order(uint64_t* x, int found, int n, F&& f) {
+  const int tid = threadIdx.x;
+  if (found <= kRowThreads) {
+    uint64_t mine = 0;
+    int before = n;
+    if (tid < found) {
+      mine = x[tid];
+      before = 0;
+#pragma unroll 4
+      for (int j = 0; j < found; ++j) before += x[j] > mine ? 1 : 0;
+    }
+    __syncthreads();
+    if (before < n) f(before, mine);
+    return;
+  }
+  int size = 2 * kRowThreads;
+  while (size < found) size *= 2;
+  for (int i = found + tid; i < size; i += kRowThreads) x[i] = 0;
+  __syncthreads();
+  for (int w = 2; w <= size; w *= 2)
+    for (int d = w / 2; d > 0; d /= 2) {
+      for (int i = tid; i < size; i += kRowThreads) {
+        const int j = i ^ d;
+        if (j > i) {
+          const uint64_t a = x[i], c = x[j];
+          if ((a < c) == ((i & w) == 0)) { x[i] = c; x[j] = a; }
+        }
+      }
+      __syncthreads();
+    }
+  for (int i = tid; i < n; i += kRowThreads) f(i, x[i]);
 }
 
 }  // namespace nrl

@@ -1,70 +1,145 @@
 // The k most probable tokens of every row of logits with their log-probabilities, as a teacher hands them to a student or a server to its user:
 //   logp_j = z_j / tau - log sum_v exp(z_v / tau),   j = the k first tokens in (logit descending, index ascending)
 // Tokens without mass (-infinity) are not listed: -1 and -infinity in their places.
+//
+// A row is read once.  Beside the sum every thread keeps the maxima of its chunks.  The k-th largest of the block's threads' maxima is a bound that at least k
+// tokens reach, and few more do (k of G groups: about G ln(G / (G - k)) tokens): the chunks whose maximum reaches it are read again, and what reaches it there
+// are the candidates.  Every block of a row's cluster sends its own to the first, which ranks them.  Rows with more candidates than fit (many ties, a sorted
+// vocabulary) and rows with an infinite logit are looked through for the border itself, eight ranges of keys a pass.
 #include "common.cuh"
 #include "logit_rows.cuh"
+#include "per_device.h"
 #include "vocab_rows.h"
 
 namespace nrl {
 
+struct TopShared {
+  BorderShared border;
+  RowList list;
+  float2 part[kRowClusterMax][kRowWarps];                // maximum and sum of every warp of the cluster
+  BoundShared bound;
+  int base;
+  float log_sum;
+};
+
+// by the border, with no use of what the pass found but NaN (in `sum`)
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) top_logprobs_kernel(const T* __restrict__ logits, long row_stride, int V, int k, double inv_temp,
-                                                                   float* __restrict__ logp, int* __restrict__ idx) {
-  extern __shared__ uint64_t s_top[];                    // (key, ~index): unsigned numbers in the order
-  __shared__ BorderShared sh;
-  __shared__ float red[kRowWarps];
-  __shared__ int s_n;
-  const LogitRow<T> row(logits + blockIdx.x * row_stride, V);
-  float mx = -INFINITY;
-  row.each([&](int, float z) { mx = fmaxf(mx, z); });
-  mx = block_max(mx, red);
-  double sum = 0.0, listed = 0.0;
+__device__ __noinline__ void top_by_border(const LogitRow<T>& row, int k, double inv_temp, float mx, TopShared& sh, double& sum, int& n) {
+  double add = 0.0, listed = 0.0;
   row.each([&](int, float z) {
-    if (z != z) sum += z;
+    if (z != z) add += z;
     if (order_key(clean(z)) > kKeyNone) {
-      sum += z == mx ? 1.0 : exp((static_cast<double>(z) - mx) * inv_temp);
+      add += z == mx ? 1.0 : exp((static_cast<double>(z) - mx) * inv_temp);
       listed += 1.0;
     }
   });
-  sum = block_sum(sum, sh.red);
-  listed = block_sum(listed, sh.red);
-  const int n = min(k, static_cast<int>(listed));
-  int size = 1;
-  while (size < n) size *= 2;
-  if (n > 0) {
-    const Border b = find_border(row, kKeyNone + 1, order_key(mx), static_cast<double>(n), [](float) { return 1.0; }, sh);
-    if (threadIdx.x == 0) s_n = 0;
-    for (int i = threadIdx.x; i < size; i += kRowThreads) s_top[i] = 0;
-    __syncthreads();
-    row.each([&](int e, float z) {
-      const uint32_t key = order_key(clean(z));
-      if (b.has(key, e)) s_top[atomicAdd(&s_n, 1)] = static_cast<uint64_t>(key) << 32 | static_cast<uint32_t>(~e);
-    });
-    __syncthreads();
-    for (int w = 2; w <= size; w *= 2)
-      for (int d = w / 2; d > 0; d /= 2) {
-        for (int i = threadIdx.x; i < size; i += kRowThreads) {
-          const int j = i ^ d;
-          if (j > i) {
-            const uint64_t a = s_top[i], c = s_top[j];
-            if ((a < c) == ((i & w) == 0)) { s_top[i] = c; s_top[j] = a; }
-          }
-        }
-        __syncthreads();
-      }
-  }
-  const double lz = log(sum);
-  for (int i = threadIdx.x; i < k; i += kRowThreads) {
-    const long o = static_cast<long>(blockIdx.x) * k + i;
-    if (i < n) {
-      const float z = key_logit(static_cast<uint32_t>(s_top[i] >> 32));
-      logp[o] = static_cast<float>((z == mx ? 0.0 : (static_cast<double>(z) - mx) * inv_temp) - lz);
-      idx[o] = static_cast<int>(~static_cast<uint32_t>(s_top[i]));
-    } else {
-      logp[o] = -INFINITY;
-      idx[o] = -1;
+  sum = block_sum(add, sh.border.red);
+  n = min(k, static_cast<int>(block_sum(listed, sh.border.red)));
+  const Border b = find_border(row, kKeyNone + 1, order_key(mx), static_cast<double>(n), [](float) { return 1.0; }, sh.border);
+  if (threadIdx.x == 0) sh.list.n = 0;
+  __syncthreads();
+  row.each([&](int e, float z) {
+    const uint32_t key = order_key(clean(z));
+    if (b.has(key, e)) sh.list.cand[atomicAdd(&sh.list.n, 1)] = static_cast<uint64_t>(key) << 32 | static_cast<uint32_t>(~e);
+  });
+  __syncthreads();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads, 3) top_logprobs_kernel(const T* __restrict__ logits, long row_stride, int V, int k, double inv_temp,
+                                                                      float* __restrict__ logp, int* __restrict__ idx) {
+  extern __shared__ float s_chunk[];                     // [chunks][kRowThreads]
+  __shared__ TopShared sh;
+  const int rank = static_cast<int>(cluster_rank()), blocks = static_cast<int>(cluster_blocks()), tid = threadIdx.x;
+  const long r = blockIdx.x / blocks;
+  if (tid == 0) sh.list.n = sh.list.nhits = sh.list.sent = 0;
+  if (blocks > 1) cluster_arrive();                      // the first block's memory may be written once it is known to run
+  const LogitRow<T> row(logits + r * row_stride, V);
+  const RowShare share(row.nvec, rank, blocks);
+  const float c = static_cast<float>(inv_temp * 1.4426950408889634);
+  float best, m, s;
+  row_pass(row, share, c, s_chunk, best, m, s, [](int, const RawVec&) {});
+  // a thread's chunks in one group up to k = 256, in up to four above
+  const int groups = k <= 256 ? 1 : k <= 512 ? 2 : 4;
+  uint32_t keys[kGroupsMax];
+  keys[0] = order_key(best);
+  if (groups > 1)
+#pragma unroll
+    for (int g = 0; g < kGroupsMax; ++g) {
+      float x = -INFINITY;
+      for (int i = g; i < share.chunks; i += groups) x = fmaxf(x, s_chunk[i * kRowThreads + tid]);
+      keys[g] = order_key(x);
     }
+  const float mw = warp_max(m);
+  const float sw = warp_sum(s * ex2((m - mw) * c));        // where an infinite logit makes this NaN, the row is looked through again
+  const uint32_t bound = group_bound(keys, groups, k, sh.bound);
+  gather_candidates(row, share, s_chunk, bound, sh.list);
+  if (blocks > 1) cluster_wait();
+  if (lane_id() == 0) {
+    const uint32_t there = in_block(&sh.part[rank][tid >> 5], 0);
+    st_block(there, mw);
+    st_block(there + 4, sw);
   }
+  if (rank != 0) send_candidates(sh.list, &sh.base);
+  __syncwarp();
+  if (blocks > 1) {
+    cluster_arrive();
+    cluster_wait();
+    if (rank != 0) return;
+  } else {
+    __syncthreads();
+  }
+
+  int found = join_candidates(sh.list), n = min(k, found);
+  bool infinite = false;
+  for (int i = tid; i < found && i < kCandidates; i += kRowThreads) infinite |= sh.list.cand[i] >> 32 == 0xff800000u;
+  float top = -INFINITY;
+  for (int i = tid & 31; i < blocks * kRowWarps; i += 32) top = fmaxf(top, sh.part[i / kRowWarps][i % kRowWarps].x);
+  top = warp_max(top);
+  if (found > kCandidates || __syncthreads_or(infinite)) {
+    double sum;
+    top_by_border(row, k, inv_temp, top, sh, sum, n);
+    found = n;
+    if (tid == 0) sh.log_sum = static_cast<float>(log(sum));
+    __syncthreads();
+  } else if (tid >= kRowThreads - 32) {                  // the last warp, while the others rank
+    double sum = 0.0;
+    for (int i = tid & 31; i < blocks * kRowWarps; i += 32) {
+      const float2 p = sh.part[i / kRowWarps][i % kRowWarps];
+      sum += p.y * ex2((p.x - top) * c);
+    }
+    sum = warp_sum(sum);
+    if ((tid & 31) == 0) sh.log_sum = logf(static_cast<float>(sum));       // half a step of it: 5e-7; the double one takes as long as the ranking
+  }
+  in_order(sh.list.cand, found, n, [&](int place, uint64_t x) {
+    const float z = key_logit(static_cast<uint32_t>(x >> 32));
+    logp[r * k + place] = static_cast<float>((z == top ? 0.0 : (static_cast<double>(z) - top) * inv_temp) - sh.log_sum);
+    idx[r * k + place] = static_cast<int>(~static_cast<uint32_t>(x));
+  });
+  for (int i = n + tid; i < k; i += kRowThreads) {
+    logp[r * k + i] = -INFINITY;
+    idx[r * k + i] = -1;
+  }
+}
+
+template <typename T>
+cudaError_t launch_top(const void* logits, long row_stride, int rows, int V, int k, double inv_temp, float* logp, int* idx, cudaStream_t s) {
+  int blocks = row_blocks(rows, V, LogitRow<T>::N);
+  while (blocks > 1 && blocks * k * 3 / 2 > kCandidates) blocks /= 2;        // every block of a row brings about k candidates
+  static PerDevice<bool> done;
+  if (const cudaError_t e = allow_smem(done, top_logprobs_kernel<T>, kRowChunks * kRowThreads * 4); e != cudaSuccess) return e;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = blocks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows) * blocks);
+  cfg.blockDim = dim3(kRowThreads);
+  cfg.dynamicSmemBytes = row_chunks(V, LogitRow<T>::N, blocks) * kRowThreads * 4;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, top_logprobs_kernel<T>, static_cast<const T*>(logits), row_stride, V, k, inv_temp, logp, idx);
 }
 
 }  // namespace nrl
@@ -74,11 +149,6 @@ using namespace nrl;
 extern "C" cudaError_t nrl_top_logprobs(const void* logits, int is_bf16, long row_stride, int rows, int V, int k, double inv_temp, float* logp, int* idx,
                                         cudaStream_t s) {
   if (rows == 0) return cudaSuccess;
-  int size = 1;
-  while (size < k) size *= 2;
-  if (is_bf16)
-    top_logprobs_kernel<<<rows, kRowThreads, size * 8, s>>>(static_cast<const __nv_bfloat16*>(logits), row_stride, V, k, inv_temp, logp, idx);
-  else
-    top_logprobs_kernel<<<rows, kRowThreads, size * 8, s>>>(static_cast<const float*>(logits), row_stride, V, k, inv_temp, logp, idx);
-  return cudaGetLastError();
+  return is_bf16 ? launch_top<__nv_bfloat16>(logits, row_stride, rows, V, k, inv_temp, logp, idx, s)
+                 : launch_top<float>(logits, row_stride, rows, V, k, inv_temp, logp, idx, s);
 }
