@@ -12,6 +12,8 @@
 // bit map in shared memory knows: taken as 1 - sum q_k it would have no digits left where the student is sure.  r below 2^-24, which float32 log-probabilities
 // cannot tell from 0, counts as 0, and as 2^-24 under a logarithm.
 // An entry whose index is not a token (-1) is skipped; entries of one token add up.
+#include <type_traits>
+
 #include "common.cuh"
 #include "logit_rows.cuh"
 #include "per_device.h"
@@ -19,130 +21,270 @@
 
 namespace nrl {
 
+// A row of gradients is written once and read by another kernel: it is the first to leave L2, where the logits wait for the second pass.
+NRL_DEVICE void store_words(float* at, const uint32_t (&w)[8]) {
+  asm volatile("st.global.L1::no_allocate.L2::evict_first.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"l"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+NRL_DEVICE void store_words(__nv_bfloat16* at, const uint32_t (&w)[8]) { store_words(reinterpret_cast<float*>(at), w); }
+NRL_DEVICE void store_words(__nv_bfloat16* at, const uint32_t (&w)[4]) { __stcs(reinterpret_cast<uint4*>(at), make_uint4(w[0], w[1], w[2], w[3])); }
+// N gradients in words, as elements e0 .. of a row: those inside it
+template <typename G, int W>
+NRL_DEVICE void store_grads(G* out, int e0, int V, const uint32_t (&w)[W]) {
+  constexpr int N = W * 4 / sizeof(G);
+  if (e0 >= 0 && e0 + N <= V && (reinterpret_cast<uintptr_t>(out + e0) & (4 * W - 1)) == 0) {
+    store_words(out + e0, w);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (e0 + j >= 0 && e0 + j < V) {
+        if constexpr (sizeof(G) == 4) out[e0 + j] = __uint_as_float(w[j]);
+        else reinterpret_cast<unsigned short*>(out)[e0 + j] = static_cast<unsigned short>(w[j / 2] >> (16 * (j % 2)));
+      }
+  }
+}
+
+struct DistillShared {
+  __align__(16) int idx[kTopMax];                          // -1: not a token
+  float z[kTopMax], a[kTopMax];
+  double p[kTopMax];                                       // of the token by all its entries; below 0: not a token, or an earlier entry has it
+  double q[kTopMax];                                       // beta > 0: D of the token's event
+  float2 part[kRowClusterMax][kRowWarps];                  // maximum and sum of every warp of the cluster
+  double red[2][kRowWarps];
+};
+
+NRL_DEVICE void block_sum_two(double& x, double& y, double (&red)[2][kRowWarps]) {
+  x = warp_sum(x);
+  y = warp_sum(y);
+  __syncthreads();
+  if (lane_id() == 0) {
+    red[0][threadIdx.x >> 5] = x;
+    red[1][threadIdx.x >> 5] = y;
+  }
+  __syncthreads();
+  x = warp_sum(lane_id() < kRowWarps ? red[0][lane_id()] : 0.0);
+  y = warp_sum(lane_id() < kRowWarps ? red[1][lane_id()] : 0.0);
+}
+
+constexpr double kNoTail = 5.9604644775390625e-8;          // 2^-24
+
+// Blocks of a cluster share a row.  Beside the two passes, what a row costs is latency -- entries, barriers, double-precision logarithms -- so that is kept off
+// the way from one pass to the other: with beta = 0 every warp finds the factor for itself behind the barrier, and the loss is left for the end.
 template <typename T, typename G>
-__global__ void __launch_bounds__(kRowThreads) distill_kernel(const T* __restrict__ logits, long row_stride, int V, const float* __restrict__ top_logp,
-                                                              const int* __restrict__ top_idx, int K, const float* __restrict__ weights, double inv_temp,
-                                                              double beta, int tail, float* __restrict__ token_loss, G* __restrict__ grad) {
-  extern __shared__ uint32_t s_map[];                      // a bit for every token: one of the teacher's
-  __shared__ double red[kRowWarps];
-  __shared__ float redf[kRowWarps];
-  __shared__ int s_idx[kTopMax];                           // -1: not a token, or one that an earlier entry has
-  __shared__ double s_p[kTopMax], s_q[kTopMax];
-  const long r = blockIdx.x;
+__global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __restrict__ logits, long row_stride, int V, const float* __restrict__ top_logp,
+                                                                 const int* __restrict__ top_idx, int K, const float* __restrict__ weights, double inv_temp,
+                                                                 double beta, int tail, float* __restrict__ token_loss, G* __restrict__ grad) {
+  constexpr int N = LogitRow<T>::N, W = N * sizeof(G) / 4;
+  extern __shared__ __align__(16) uint32_t s_map[];        // a bit for every element of the share's vectors: one of the teacher's tokens
+  __shared__ DistillShared sh;
+  const int rank = static_cast<int>(cluster_rank()), blocks = static_cast<int>(cluster_blocks()), tid = threadIdx.x, lane = tid & 31;
+  const long r = blockIdx.x / blocks, rows = gridDim.x / blocks;
   const LogitRow<T> row(logits + r * row_stride, V);
-  const double weight = weights ? static_cast<double>(weights[r]) : 1.0 / gridDim.x;
+  const RowShare share(row.nvec, rank, blocks);
+  const float weight = weights ? weights[r] : 1.f;
   G* out = grad ? grad + r * V : nullptr;
-  if (weight == 0.0) {                                     // the row is not read
-    if (threadIdx.x == 0) token_loss[r] = 0.f;
+  if (weight == 0.f) {                                     // the row is not read
+    if (tid == 0 && rank == 0) token_loss[r] = 0.f;
+    const uint32_t none[W] = {};
     if (out)
-      for (int v = threadIdx.x; v < V; v += kRowThreads) out[v] = static_cast<G>(0.f);
+      for (int v = share.first + tid; v < share.end; v += kRowThreads) store_grads(out, v * N - row.skew, V, none);
     return;
   }
-  for (int i = threadIdx.x; i < (V + 31) / 32; i += kRowThreads) s_map[i] = 0;
-  for (int i = threadIdx.x; i < K; i += kRowThreads) {
-    const int at = top_idx[r * K + i];
-    s_idx[i] = at >= 0 && at < V ? at : -1;
-  }
+  if (blocks > 1) cluster_arrive();                        // shared memory may be written by the others once it is known to run
+  // ---- the teacher's entries, and where they lie in the share ----
+  for (int i = tid; i < (share.end - share.first) * N / 32 + 1; i += kRowThreads) s_map[i] = 0;
   __syncthreads();
-  int twin[kTopMax / kRowThreads];
+  static_assert(kTopMax == 2 * kRowThreads, "two entries a thread at most");
+  float a_mine[2];
+  T z_mine[2];
 #pragma unroll
-  for (int t = 0; t < kTopMax / kRowThreads; ++t) {
-    const int i = threadIdx.x + t * kRowThreads;
-    twin[t] = 0;
-    if (i < K && s_idx[i] >= 0) {
-      double p = 0.0;
-      for (int j = 0; j < K; ++j)
-        if (s_idx[j] == s_idx[i]) {
-          p += exp(static_cast<double>(top_logp[r * K + j]));
-          if (j < i) twin[t] = 1;
-        }
-      s_p[i] = p;
-      atomicOr(&s_map[s_idx[i] >> 5], 1u << (s_idx[i] & 31));
+  for (int t = 0; t < 2; ++t) {
+    const int i = tid + t * kRowThreads;
+    if (i < (K + 3) / 4 * 4) {
+      const int e = i < K ? top_idx[r * K + i] : -1, at = e >= 0 && e < V ? e : -1, bit = at + row.skew - share.first * N;
+      sh.idx[i] = at;
+      if (i < K) a_mine[t] = top_logp[r * K + i];
+      z_mine[t] = row.p[max(at, 0)];
+      if (at >= 0 && bit >= 0 && bit < (share.end - share.first) * N) atomicOr(&s_map[bit >> 5], 1u << (bit & 31));
     }
   }
-  __syncthreads();
+  __syncthreads();                                         // the map is whole; the entries' logits may still be on their way
 #pragma unroll
-  for (int t = 0; t < kTopMax / kRowThreads; ++t)
-    if (twin[t]) s_idx[threadIdx.x + t * kRowThreads] = -1;
+  for (int t = 0; t < 2; ++t) {
+    const int i = tid + t * kRowThreads;
+    if (i < K) {
+      sh.a[i] = a_mine[t];
+      sh.z[i] = LogitRow<T>::value(z_mine[t]);
+    }
+  }
 
-  float mx = -INFINITY;
-  row.each([&](int, float z) { mx = fmaxf(mx, z); });
-  mx = block_max(mx, redf);
+  // ---- the row's maximum, and its mass off the teacher's tokens ----
   const float c = static_cast<float>(inv_temp * 1.4426950408889634);
-  float rest = 0.f;
-  row.each([&](int e, float z) {
-    if (!(s_map[e >> 5] >> (e & 31) & 1)) rest += ex2((z - mx) * c);
-  });
-  double others = block_sum(static_cast<double>(rest), red);
-  double top = 0.0, psum = 0.0;
-  for (int i = threadIdx.x; i < K; i += kRowThreads)
-    if (s_idx[i] >= 0) {
-      const double q = exp((static_cast<double>(row.at(s_idx[i])) - mx) * inv_temp);
-      s_q[i] = q;
-      top += q;
-      psum += s_p[i];
+  const auto* map = reinterpret_cast<const std::conditional_t<N == 16, uint16_t, uint8_t>*>(s_map);
+  float best, m, mass;
+  row_pass(row, share, c, static_cast<float*>(nullptr), best, m, mass, [&](int v, RawVec& a) {
+    if (v >= share.end) return;
+    const unsigned bits = map[v - share.first];
+    if (bits == 0) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if constexpr (N == 16) {
+        if (bits >> (2 * j) & 1) a.w[j] = (a.w[j] & 0xffff0000u) | 0xff80u;
+        if (bits >> (2 * j + 1) & 1) a.w[j] = (a.w[j] & 0xffffu) | 0xff800000u;
+      } else {
+        if (bits >> j & 1) a.w[j] = 0xff800000u;
+      }
     }
-  top = block_sum(top, red);
-  psum = block_sum(psum, red);
-  const double total = top + others, log_total = log(total), s = others / total;
-  double rr = 1.0 - psum;
-  if (!(rr > 5.9604644775390625e-8)) rr = 0.0;
-  const double r_log = rr > 0.0 ? rr : 5.9604644775390625e-8;
-  // losses, and D of every event
-  double loss = 0.0, mean = 0.0;
-  for (int i = threadIdx.x; i < K; i += kRowThreads) {
-    if (s_idx[i] < 0) continue;
-    const double log_q = (static_cast<double>(row.at(s_idx[i])) - mx) * inv_temp - log_total, q = s_q[i] / total;
-    double p = s_p[i];
-    if (!tail) p = psum > 0.0 ? p / psum : 0.0;
-    if (beta == 0.0) {
-      if (p > 0.0) loss += p * (log(p) - log_q);
-      s_p[i] = q - p;                                      // the gradient's entry
-    } else if (beta == 1.0) {
-      const double d = q > 0.0 ? log_q - log(p) : 0.0;
+  });
+  const float mw = warp_max(m);
+  mass = warp_sum(mass * ex2((m - mw) * c));
+  if (blocks > 1) cluster_wait();
+  if (lane < blocks) {
+    const uint32_t there = in_block(&sh.part[rank][tid >> 5], lane);
+    st_block(there, mw);
+    st_block(there + 4, mass);
+  }
+  __syncwarp();
+  if (blocks > 1) cluster_arrive();
+  for (int i = tid; i < K; i += kRowThreads) {             // probabilities of the teacher's tokens, while the other blocks come
+    const int at = sh.idx[i];
+    double p = -1.0;
+    if (at >= 0) {
+      int same = 0;
+      for (int j = 0; j < K; j += 4) {                     // entries behind the last are -1
+        const int4 x = *reinterpret_cast<const int4*>(&sh.idx[j]);
+        same += (x.x == at) + (x.y == at) + (x.z == at) + (x.w == at);
+      }
+      p = exp(static_cast<double>(sh.a[i]));
+      if (same > 1)
+        for (int j = 0; j < K; ++j)
+          if (sh.idx[j] == at && j != i) p = j < i || p < 0.0 ? -1.0 : p + exp(static_cast<double>(sh.a[j]));
+    }
+    sh.p[i] = p;
+  }
+  __syncwarp();
+  if (blocks > 1) cluster_wait();
+  __syncthreads();
+  float mx = -INFINITY;
+  for (int i = lane; i < blocks * kRowWarps; i += 32) mx = fmaxf(mx, sh.part[i / kRowWarps][i % kRowWarps].x);
+  mx = warp_max(mx);
+  double others = 0.0, psum = 0.0, top = 0.0;
+  for (int i = lane; i < blocks * kRowWarps; i += 32) {
+    const float2 p = sh.part[i / kRowWarps][i % kRowWarps];
+    others += p.y * ex2((p.x - mx) * c);
+  }
+  others = warp_sum(others);
+  for (int i = lane; i < K; i += 32)
+    if (sh.p[i] >= 0.0) {
+      psum += sh.p[i];
+      top += ex2((sh.z[i] - mx) * c);
+    }
+  psum = warp_sum(psum);
+  top = warp_sum(top);
+
+  // ---- the K + 1 events ----
+  double rr = 1.0 - psum, off = 1.0, mean = 0.0, total = top + others;         // off: factor of q off K
+  if (!(rr > kNoTail)) rr = 0.0;
+  const bool teacher = tail || psum > 0.0;
+  if (beta == 0.0) {
+    if (tail) off = others > 0.0 ? 1.0 - rr / others * total : 0.0;
+    else if (!teacher) off = 0.0;
+  } else {
+    double loss = 0.0, none = 0.0;
+    top = 0.0;
+    for (int i = tid; i < K; i += kRowThreads)
+      if (sh.p[i] >= 0.0) top += exp((static_cast<double>(sh.z[i]) - mx) * inv_temp);
+    block_sum_two(top, none, sh.red);
+    total = top + others;
+    const double log_total = log(total), s = others / total;
+    for (int i = tid; i < K; i += kRowThreads) {
+      const double p = sh.p[i];
+      if (p < 0.0) continue;
+      const double log_q = (static_cast<double>(sh.z[i]) - mx) * inv_temp - log_total, q = exp(log_q);
+      double d = 0.0;
+      if (beta == 1.0) {
+        if (q > 0.0) d = log_q - log(p);
+      } else {
+        const double mid = beta * p + (1.0 - beta) * q;
+        if (q > 0.0) d = (1.0 - beta) * log(q / mid);
+        if (p > 0.0) loss += beta * p * log(p / mid);
+      }
       loss += q * d;
       mean += q * d;
-      s_p[i] = d;
-    } else {
-      const double m = beta * p + (1.0 - beta) * q, d = q > 0.0 ? (1.0 - beta) * log(q / m) : 0.0;
-      loss += (p > 0.0 ? beta * p * log(p / m) : 0.0) + q * d;
-      mean += q * d;
-      s_p[i] = d;
+      sh.q[i] = d;
     }
-    s_q[i] = q;
-  }
-  loss = block_sum(loss, red);
-  mean = block_sum(mean, red);
-  double off = 1.0;                                        // factor of q off K
-  if (tail) {
-    if (beta == 0.0) {
-      if (rr > 0.0) loss += rr * (log(rr) - log(s));
-      off = s > 0.0 ? 1.0 - rr / s : 0.0;
-    } else if (beta == 1.0) {
-      const double d = s > 0.0 ? log(s) - log(r_log) : 0.0;
-      loss += s * d;
-      mean += s * d;
-      off = d - mean;
+    block_sum_two(loss, mean, sh.red);
+    double d = 0.0;
+    if (beta == 1.0) {
+      if (s > 0.0) d = log(s) - log(rr > 0.0 ? rr : kNoTail);
     } else {
-      const double m = beta * rr + (1.0 - beta) * s, d = s > 0.0 ? (1.0 - beta) * log(s / m) : 0.0;
-      loss += (rr > 0.0 ? beta * rr * log(rr / m) : 0.0) + s * d;
-      mean += s * d;
-      off = d - mean;
+      const double mid = beta * rr + (1.0 - beta) * s;
+      if (s > 0.0) d = (1.0 - beta) * log(s / mid);
+      if (rr > 0.0) loss += beta * rr * log(rr / mid);
     }
-  } else if (!(psum > 0.0)) {
-    off = 0.0;                                             // no teacher
+    loss += s * d;
+    mean += s * d;
+    off = d - mean;
+    if (tid == 0 && rank == 0) token_loss[r] = static_cast<float>(loss);
   }
-  if (threadIdx.x == 0) token_loss[r] = static_cast<float>(loss);
-  if (!out) return;
-  const double g = weight * inv_temp;
-  const float f = static_cast<float>(fmin(fmax(g * off / total, -3e38), 3e38));      // finite: 0 times it is 0
-  row.each([&](int e, float z) {
-    if (!(s_map[e >> 5] >> (e & 31) & 1)) out[e] = static_cast<G>(ex2((z - mx) * c) * f);
-  });
-  for (int i = threadIdx.x; i < K; i += kRowThreads) {
-    if (s_idx[i] < 0) continue;
-    const double u = beta == 0.0 ? (!tail && !(psum > 0.0) ? 0.0 : s_p[i]) : s_q[i] * (s_p[i] - mean);
-    out[s_idx[i]] = static_cast<G>(static_cast<float>(g * u));
+
+  // ---- the gradient: off K one factor a row; the teacher's tokens are put right behind the others ----
+  if (out) {
+    const double g = (weights ? static_cast<double>(weight) : 1.0 / rows) * inv_temp;
+    const float f = static_cast<float>(fmin(fmax(g * off / total, -3e38), 3e38));      // finite: 0 times it is 0
+    const uint64_t c2 = pair_both(c), neg = pair_both(-mx), f2 = pair_both(f);
+    // backwards: what the first pass read last is the likeliest to be in L2
+#pragma unroll 1
+    for (int v = share.first + (share.end - share.first - 1) / kRowThreads * kRowThreads + tid; v >= share.first; v -= kRowThreads) {
+      if (v >= share.end) continue;
+      const RawVec a = row.template raw<true>(v);
+      uint32_t w[W];
+#pragma unroll
+      for (int q = 0; q < N / 2; ++q) {
+        const float2 e = pair_parts(pair_mul(pair_add(LogitRow<T>::pair(a, q), neg), c2));
+        const float2 y = pair_parts(pair_mul(pair_of(__float_as_uint(ex2(e.x)), __float_as_uint(ex2(e.y))), f2));
+        if constexpr (sizeof(G) == 4) {
+          w[2 * q] = __float_as_uint(y.x);
+          w[2 * q + 1] = __float_as_uint(y.y);
+        } else {
+          w[q] = pack_bf16x2(y.x, y.y);
+        }
+      }
+      store_grads(out, v * N - row.skew, V, w);
+    }
+    __syncthreads();
+    for (int i = tid; i < K; i += kRowThreads) {
+      const double p = sh.p[i];
+      const int bit = sh.idx[i] + row.skew - share.first * N;
+      if (p < 0.0 || bit < 0 || bit >= (share.end - share.first) * N) continue;
+      const double q = exp((static_cast<double>(sh.z[i]) - mx) * inv_temp) / total;
+      const double u = !teacher ? 0.0 : beta == 0.0 ? q - (tail ? p : p / psum) : q > 0.0 ? q * (sh.q[i] - mean) : 0.0;
+      out[sh.idx[i]] = static_cast<G>(static_cast<float>(g * u));
+    }
+  }
+
+  // ---- beta = 0: sum p (log p - log q) over the events, log q = x - log total ----
+  if (beta != 0.0 || rank != 0) return;
+  double mass_top = 0.0, loss = 0.0;
+  for (int i = tid; i < K; i += kRowThreads) {
+    const double p = sh.p[i];
+    if (p < 0.0) continue;
+    const double x = (static_cast<double>(sh.z[i]) - mx) * inv_temp;
+    mass_top += exp(x);
+    if (p > 0.0) loss += p * (log(p) - x);
+  }
+  block_sum_two(mass_top, loss, sh.red);
+  if (tid < 32) {                                          // three logarithms in one
+    total = mass_top + others;
+    const double l = log(lane == 0 ? total : lane == 1 ? (tail ? rr : psum) : others);
+    const double log_total = __shfl_sync(0xffffffffu, l, 0), log_r = __shfl_sync(0xffffffffu, l, 1), log_o = __shfl_sync(0xffffffffu, l, 2);
+    if (tail) {
+      loss += psum * log_total;
+      if (rr > 0.0) loss += rr * (log_r - log_o + log_total);
+    } else {
+      loss = psum > 0.0 ? loss / psum - log_r + log_total : 0.0;
+    }
+    if (lane == 0) token_loss[r] = static_cast<float>(loss);
   }
 }
 
@@ -171,11 +313,26 @@ template <typename T, typename G>
 cudaError_t launch_distill(const void* logits, long row_stride, int rows, int V, const float* top_logp, const int* top_idx, int k, const float* weights,
                            double inv_temp, double beta, int tail, float* token_loss, void* grad, cudaStream_t s) {
   static PerDevice<bool> done;
-  const int bytes = (V + 31) / 32 * 4;
-  if (const cudaError_t e = allow_smem(done, distill_kernel<T, G>, kDistillVocabMax / 8); e != cudaSuccess) return e;
-  distill_kernel<T, G><<<rows, kRowThreads, bytes, s>>>(static_cast<const T*>(logits), row_stride, V, top_logp, top_idx, k, weights, inv_temp, beta, tail,
-                                                         token_loss, static_cast<G*>(grad));
-  return cudaGetLastError();
+  constexpr int N = LogitRow<T>::N;
+  // Rows that the second pass would not find in L2 any more (three blocks on 148 SMs hold 444 rows, and 126 MB is what L2 has) get four blocks, which is a
+  // quarter of them at a time: 2048 x 151 936 floats 580 / 559 / 535 us with 1 / 2 / 4, bf16 307 / 307 / 405, 1500 x 50 021 floats 150 / 157 / 211.
+  int blocks = row_blocks(rows, V, N);
+  if (grad != nullptr && V * sizeof(T) > 400 * 1024 && blocks < 4) blocks = 4;
+  const int vecs = ((V + 2 * N - 2) / N + blocks - 1) / blocks;
+  if (const cudaError_t e = allow_smem(done, distill_kernel<T, G>, kDistillVocabMax / 8 + 128); e != cudaSuccess) return e;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = blocks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows) * blocks);
+  cfg.blockDim = dim3(kRowThreads);
+  cfg.dynamicSmemBytes = (vecs * N / 32 + 1) * 4;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, distill_kernel<T, G>, static_cast<const T*>(logits), row_stride, V, top_logp, top_idx, k, weights, inv_temp, beta, tail,
+                            token_loss, static_cast<G*>(grad));
 }
 
 }  // namespace nrl

@@ -60,14 +60,20 @@ struct LogitRow {
   NRL_DEVICE static float value(T x);
   NRL_DEVICE static uint32_t none();                   // a word of -infinity
   NRL_DEVICE static void put(RawVec& a, int j, T x);   // element j of a vector
-  // elements outside the row are -infinity and are not read
+  // elements outside the row are -infinity and are not read; LAST: nobody reads them again
+  template <bool LAST = false>
   NRL_DEVICE RawVec raw(int v) const {
     RawVec a;
     const int e0 = v * N - skew;
     if (e0 >= 0 && e0 + N <= V) {
-      asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                   : "=r"(a.w[0]), "=r"(a.w[1]), "=r"(a.w[2]), "=r"(a.w[3]), "=r"(a.w[4]), "=r"(a.w[5]), "=r"(a.w[6]), "=r"(a.w[7])
-                   : "l"(p + e0));
+      if constexpr (LAST)
+        asm volatile("ld.global.nc.L1::no_allocate.L2::evict_first.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(a.w[0]), "=r"(a.w[1]), "=r"(a.w[2]), "=r"(a.w[3]), "=r"(a.w[4]), "=r"(a.w[5]), "=r"(a.w[6]), "=r"(a.w[7])
+                     : "l"(p + e0));
+      else
+        asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(a.w[0]), "=r"(a.w[1]), "=r"(a.w[2]), "=r"(a.w[3]), "=r"(a.w[4]), "=r"(a.w[5]), "=r"(a.w[6]), "=r"(a.w[7])
+                     : "l"(p + e0));
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) a.w[j] = none();
@@ -325,7 +331,7 @@ inline int row_blocks(long rows, int V, int vec) {
 
 // One pass over the block's share: thread-wise maximum `best`, sum s of 2^((z - m) c), m = best or the lowest float, and the maximum of every chunk.  The sum's reference moves with the
 // maximum, once for the kRowUnroll vectors of a step.  z - m is formed before the multiplication: m c would round at the size of the logits.
-// skip(v, a) may take elements of vector v out of the sum by making them -infinity.
+// skip(v, a) may take elements of vector v out of the sum by making them -infinity.  chunk_max may be null.
 template <typename T, class S>
 NRL_DEVICE void row_pass(const LogitRow<T>& row, const RowShare& sh, float c, float* chunk_max, float& best, float& m, float& s, S&& skip) {
   m = -3.402823466e38f;                                // finite, so that -infinity is 0 in the sum
@@ -363,7 +369,7 @@ NRL_DEVICE void row_pass(const LogitRow<T>& row, const RowShare& sh, float c, fl
       m = mn;
     }
     best = fmaxf(best, cm);
-    chunk_max[i * kRowThreads + threadIdx.x] = cm;
+    if (chunk_max != nullptr) chunk_max[i * kRowThreads + threadIdx.x] = cm;
   }
 }
 
