@@ -92,6 +92,7 @@ struct LogitRow {
   NRL_DEVICE static void unpack(const RawVec& a, float (&x)[N]);
   NRL_DEVICE static float largest(const RawVec& a);    // NaN left aside
   NRL_DEVICE static uint64_t pair(const RawVec& a, int i);        // elements 2 i and 2 i + 1
+  NRL_DEVICE static void drop_nan(RawVec& a);          // NaN become -infinity
   NRL_DEVICE void load(int v, float (&x)[N]) const { unpack(raw(v), x); }
   NRL_DEVICE float at(int e) const { return value(p[e]); }
   // every element of this warp's range: the warps have consecutive ranges of the row, their lanes interleaved vectors; f(index, logit)
@@ -154,6 +155,21 @@ NRL_DEVICE float LogitRow<__nv_bfloat16>::largest(const RawVec& a) {
   for (int j = 1; j < 8; ++j) m = __hmax2(m, *reinterpret_cast<const __nv_bfloat162*>(&a.w[j]));
   const float2 f = __bfloat1622float2(m);
   return fmaxf(f.x, f.y);
+}
+
+template <>
+NRL_DEVICE void LogitRow<float>::drop_nan(RawVec& a) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) a.w[j] = __float_as_uint(fmaxf(__uint_as_float(a.w[j]), -INFINITY));
+}
+template <>
+NRL_DEVICE void LogitRow<__nv_bfloat16>::drop_nan(RawVec& a) {
+  const __nv_bfloat162 lowest = __halves2bfloat162(__ushort_as_bfloat16(0xff80u), __ushort_as_bfloat16(0xff80u));
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a.w[j]), lowest);
+    a.w[j] = *reinterpret_cast<const uint32_t*>(&m);
+  }
 }
 
 // Reductions over the block, in one order; every thread gets the result.  `red`: kRowWarps entries that nobody else uses until the next barrier.
@@ -331,8 +347,8 @@ inline int row_blocks(long rows, int V, int vec) {
 
 // One pass over the block's share: thread-wise maximum `best`, sum s of 2^((z - m) c), m = best or the lowest float, and the maximum of every chunk.  The sum's reference moves with the
 // maximum, once for the kRowUnroll vectors of a step.  z - m is formed before the multiplication: m c would round at the size of the logits.
-// skip(v, a) may take elements of vector v out of the sum by making them -infinity.  chunk_max may be null.
-template <typename T, class S>
+// skip(v, a) may take elements of vector v out of the sum by making them -infinity.  chunk_max may be null.  SUM false: the maxima alone.
+template <bool SUM = true, typename T, class S>
 NRL_DEVICE void row_pass(const LogitRow<T>& row, const RowShare& sh, float c, float* chunk_max, float& best, float& m, float& s, S&& skip) {
   m = -3.402823466e38f;                                // finite, so that -infinity is 0 in the sum
   s = 0.f;
@@ -352,6 +368,7 @@ NRL_DEVICE void row_pass(const LogitRow<T>& row, const RowShare& sh, float c, fl
 #pragma unroll
       for (int j = 1; j < kRowUnroll; ++j) l = fmaxf(l, LogitRow<T>::largest(a[j]));
       cm = fmaxf(cm, l);
+      if constexpr (!SUM) continue;
       const float mn = fmaxf(m, l);
       const uint64_t neg = pair_both(-mn);
       uint64_t sum = 0;
@@ -457,7 +474,7 @@ struct RowList {
 // list.nhits are 0 before; above kCandidates they say that there is more than what the list holds.
 template <typename T>
 NRL_DEVICE void gather_candidates(const LogitRow<T>& row, const RowShare& share, const float* chunk_max, uint32_t bound, RowList& list) {
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
   unsigned mine = 0;
 #pragma unroll 4
   for (int i = 0; i < share.chunks; ++i) mine |= (order_key(chunk_max[i * kRowThreads + tid]) >= bound ? 1u : 0u) << i;
@@ -521,6 +538,32 @@ NRL_DEVICE int join_candidates(RowList& list) {
   return all;
 }
 
+// `size` (a power of 2 from 64 on) numbers in descending order.  A warp has 64 neighbours to itself, so that steps up to a distance of 32 need no barrier.
+NRL_DEVICE void sort_block(uint64_t* x, int size) {
+  const int tid = threadIdx.x;
+#pragma unroll 1
+  for (int w = 2; w <= size; w *= 2)
+#pragma unroll 1
+    for (int d = w / 2; d > 0; d /= 2) {
+      if (d >= 32) __syncthreads();
+      else __syncwarp();
+      for (int t = tid; t < size / 2; t += kRowThreads) {
+        const int i = 2 * t - (t & (d - 1)), j = i + d;
+        const uint64_t a = x[i], c = x[j];
+        if ((a < c) == ((i & w) == 0)) { x[i] = c; x[j] = a; }
+      }
+    }
+  __syncthreads();
+}
+// x[0 .. n) in descending order; entries behind them up to the next power of 2 from 64 on are overwritten by 0
+NRL_DEVICE void sort_front(uint64_t* x, int n) {
+  int size = 64;
+  while (size < n) size *= 2;
+  for (int i = n + threadIdx.x; i < size; i += kRowThreads) x[i] = 0;
+  __syncthreads();
+  sort_block(x, size);
+}
+
 // Candidates in their order: f(place, candidate) for the first n of them, behind a barrier.  Up to one a thread each counts those before it; more are sorted.
 template <class F>
 NRL_DEVICE void in_order(uint64_t* x, int found, int n, F&& f) {
@@ -538,21 +581,7 @@ NRL_DEVICE void in_order(uint64_t* x, int found, int n, F&& f) {
     if (before < n) f(before, mine);
     return;
   }
-  int size = 2 * kRowThreads;
-  while (size < found) size *= 2;
-  for (int i = found + tid; i < size; i += kRowThreads) x[i] = 0;
-  __syncthreads();
-  for (int w = 2; w <= size; w *= 2)
-    for (int d = w / 2; d > 0; d /= 2) {
-      for (int i = tid; i < size; i += kRowThreads) {
-        const int j = i ^ d;
-        if (j > i) {
-          const uint64_t a = x[i], c = x[j];
-          if ((a < c) == ((i & w) == 0)) { x[i] = c; x[j] = a; }
-        }
-      }
-      __syncthreads();
-    }
+  sort_front(x, found);
   for (int i = tid; i < n; i += kRowThreads) f(i, x[i]);
 }
 

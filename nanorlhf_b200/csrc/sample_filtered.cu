@@ -1,46 +1,91 @@
 // One token per row of logits under temperature, min-p, top-k and top-p, from a given uniform number:
 //   w_i = exp((z_i - max z) / T);  keep w_i >= min_p;  of those the top_k first in (logit descending, index ascending);  of those the shortest prefix whose
 //   mass is at least top_p of theirs;  token = the first kept i, by index, with sum_{j <= i, kept} w_j > u * (mass of the kept)
-// and its log-probability among the kept.  Each filter keeps a prefix of the order, so what is kept is one Border.  T <= 0: the first of the order.
+// and its log-probability among the kept.  Each filter keeps a prefix of the order.  T <= 0: the first of the order.
 // Masses are double: a token changes with the last bits of a sum, and the same numbers are to give the same token wherever they are added up.
+//
+// What a filter leaves is mostly few tokens.  A row is read once, every thread keeping the maxima of its chunks; a bound that all kept tokens reach -- the
+// top_k-th largest of the threads' maxima, or the largest logit + T ln min_p -- picks the chunks that are read again, and the candidates that they hold are sorted
+// and filtered exactly.  A nucleus without other filters needs the mass of the whole row as well: the pass adds it up in float, and where what is known of its error
+// leaves the nucleus' last token open, or the candidates do not reach it, the row takes the long way: the border of the order by ranges of keys, in double.
 #include <curand_kernel.h>
 
 #include "common.cuh"
 #include "logit_rows.cuh"
+#include "per_device.h"
 #include "vocab_rows.h"
 
 namespace nrl {
 
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads) sample_filtered_kernel(const T* __restrict__ logits, long row_stride, int V,
-                                                                      const float* __restrict__ uniforms, SampleFilters f, int* __restrict__ tokens,
-                                                                      float* __restrict__ logp) {
-  __shared__ BorderShared sh;
-  __shared__ float redf[kRowWarps];
-  __shared__ double s_mass[kRowWarps];
-  const int r = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const LogitRow<T> row(logits + r * row_stride, V);
-  const double temp = f.temperature ? f.temperature[r] : f.temperature_all, top_p = f.top_p ? f.top_p[r] : f.top_p_all,
-               min_p = f.min_p ? f.min_p[r] : f.min_p_all;
-  const int top_k = f.top_k ? f.top_k[r] : f.top_k_all;
-  float mx = -INFINITY;
-  row.each([&](int, float z) { mx = fmaxf(mx, z); });
-  mx = block_max(mx, redf);
-  if (mx == -INFINITY) {                                   // nothing to draw from
-    if (threadIdx.x == 0) { tokens[r] = -1; logp[r] = -INFINITY; }
-    return;
+struct RowFilter {
+  double temp, inv_temp, top_p, min_p;
+  int top_k;                                               // 0: none
+  NRL_DEVICE RowFilter(const SampleFilters& f, long r, int V) {
+    temp = f.temperature ? f.temperature[r] : f.temperature_all;
+    top_p = f.top_p ? f.top_p[r] : f.top_p_all;
+    min_p = f.min_p ? f.min_p[r] : f.min_p_all;
+    top_k = f.top_k ? f.top_k[r] : f.top_k_all;
+    if (!(temp > 0.0)) {                                   // the first of the order, which has log-probability 0 among itself
+      temp = 1.0;
+      top_k = 1;
+    }
+    if (top_k < 0 || top_k >= V) top_k = 0;
+    if (!(min_p > 0.0)) min_p = 0.0;
+    if (min_p > 1.0) min_p = 1.0;
+    if (!(top_p < 1.0)) top_p = 1.0;
+    inv_temp = 1.0 / temp;
   }
+  NRL_DEVICE double x(float z, float mx) const { return z == mx ? 0.0 : (static_cast<double>(z) - mx) * inv_temp; }
+  NRL_DEVICE double mass(float z, float mx) const { return z == mx ? 1.0 : exp((static_cast<double>(z) - mx) * inv_temp); }
+};
+
+struct SampleShared {
+  BorderShared border;
+  RowList list;
+  BoundShared bound;
+  double scan[kRowWarps];
+  float2 part[kRowClusterMax][kRowWarps];                  // maximum and sum of every warp of the cluster
+  uint32_t part_bound[kRowClusterMax];
+  double total;
+  int base, token;
+};
+
+// sums over the threads up to and with this one, and over all
+NRL_DEVICE double block_scan(double v, double& all, double* red) {
+  const int lane = static_cast<int>(lane_id()), warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
+  __syncthreads();
+  if (lane == 31) red[warp] = v;
+  __syncthreads();
+  double before = 0.0;
+  all = 0.0;
+#pragma unroll 1
+  for (int w = 0; w < kRowWarps; ++w) {
+    if (w == warp) before = all;
+    all += red[w];
+  }
+  return before + v;
+}
+
+// The long way: the border by ranges of keys, then the kept mass of every warp's range and a walk through the range that holds the drawn one.
+template <typename T>
+__device__ __noinline__ void sample_by_border(const LogitRow<T>& row, const RowFilter& f, float mx, double u, SampleShared& shared, int* out_token, float* out_logp) {
+  BorderShared& sh = shared.border;
+  double* masses = shared.scan;
+  const int V = row.V, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t top = order_key(mx);
-  const bool greedy = !(temp > 0.0);
-  const double inv_temp = greedy ? 1.0 : 1.0 / temp;
-  auto mass = [&](float z) { return z == mx ? 1.0 : exp((static_cast<double>(z) - mx) * inv_temp); };
+  auto mass = [&](float z) { return f.mass(z, mx); };
   auto one = [](float) { return 1.0; };
   uint32_t floor_key = mx == INFINITY ? top : kKeyNone + 1;
-  if (min_p > 0.0 && !greedy) {                            // smallest key whose mass is min_p: every lane tries one of 32 keys of a range, seven times
+  if (f.min_p > 0.0) {                            // smallest key whose mass is min_p: every lane tries one of 32 keys of a range, seven times
     uint64_t lo = floor_key, hi = top;                     // in [lo, hi]; the largest logit is in whatever min_p says
     while (lo < hi) {
       const uint64_t step = (hi - lo + 31) / 32, k = lo + lane * step;
-      const unsigned in = __ballot_sync(0xffffffffu, k >= hi || mass(key_logit(static_cast<uint32_t>(k))) >= min_p);
+      const unsigned in = __ballot_sync(0xffffffffu, k >= hi || mass(key_logit(static_cast<uint32_t>(k))) >= f.min_p);
       const int i = in ? __ffs(in) - 1 : 32;               // the border lies behind the key of lane i - 1
       const uint64_t up = lo + static_cast<uint64_t>(i) * step;
       if (i == 0) { hi = lo; break; }
@@ -57,31 +102,27 @@ __global__ void __launch_bounds__(kRowThreads) sample_filtered_kernel(const T* _
     });
     return block_sum(m, sh.red);
   };
-  if (greedy) {
-    b = find_border(row, top, top, 1.0, one, sh);
-  } else {
-    if (top_k > 0 && total_of(one) > top_k) b = find_border(row, floor_key, top, static_cast<double>(top_k), one, sh);
-    if (top_p < 1.0) b = find_border(row, b.key, top, top_p > 0.0 ? top_p * total_of(mass) : 1e-300, mass, sh);
-  }
+  if (f.top_k > 0 && total_of(one) > f.top_k) b = find_border(row, floor_key, top, static_cast<double>(f.top_k), one, sh);
+  if (f.top_p < 1.0) b = find_border(row, b.key, top, f.top_p > 0.0 ? f.top_p * total_of(mass) : 1e-300, mass, sh);
   // the kept mass of every warp's range, and the first range in which the drawn mass is passed
   double mine = 0.0;
   row.each([&](int e, float z) {
     if (b.has(order_key(clean(z)), e)) mine += mass(z);
   });
   mine = warp_sum(mine);
-  if (lane == 0) s_mass[warp] = mine;
+  if (lane == 0) masses[warp] = mine;
   __syncthreads();
   double total = 0.0;
-  for (int w = 0; w < kRowWarps; ++w) total += s_mass[w];
-  const double target = static_cast<double>(uniforms[r]) * total;
+  for (int w = 0; w < kRowWarps; ++w) total += masses[w];
+  const double target = u * total;
   int owner = -1;
   double before = 0.0, base = 0.0;
   bool found = false;
   for (int w = 0; w < kRowWarps && !found; ++w)
-    if (s_mass[w] > 0.0) {
+    if (masses[w] > 0.0) {
       owner = w;
       before = base;
-      base += s_mass[w];
+      base += masses[w];
       found = base > target;
     }
   if (warp != owner) return;
@@ -127,10 +168,204 @@ __global__ void __launch_bounds__(kRowThreads) sample_filtered_kernel(const T* _
     before += __shfl_sync(0xffffffffu, incl, 31);
   }
   if (lane == 0) {
-    tokens[r] = token;
     const float z = row.at(token);
-    logp[r] = greedy ? 0.f : static_cast<float>((z == mx ? 0.0 : (static_cast<double>(z) - mx) * inv_temp) - log(total));
+    *out_token = token;
+    *out_logp = static_cast<float>(f.x(z, mx) - log(total));
   }
+}
+
+// Float sums of 2^x are off by so much of themselves at most: 2^-22 for 2^x, three steps of 2^-24 of the exponents, whose mean over the mass is log2 V < 24 at most, and
+// sums of at most 300 terms a thread in float.
+constexpr double kSumError = 2e-5;
+constexpr int kNucleusGroups = 128;                        // groups whose maxima bound the candidates of a nucleus
+
+// Over the sorted candidates: how many of them are kept; 0: it is not known (nucleus of a whole row whose mass `whole` is only known to kSumError, or whose last token is
+// not among the `sure` first, beyond which others may come between).
+NRL_DEVICE int kept_of(const uint64_t* x, int found, int sure, const RowFilter& f, float mx, double whole, SampleShared& sh, double& total) {
+  const int tid = threadIdx.x;
+  double done = 0.0;
+  int n = 0, n1 = found;
+  bool open = false;
+  total = 0.0;
+  if (f.top_k > 0 && f.top_k < n1) n1 = f.top_k;
+  const bool nucleus = f.top_p < 1.0;
+  double limit = 1e300, low = 0.0;
+  for (int pass = nucleus && whole == 0.0 ? 0 : 1; pass < 2; ++pass) {        // the first for the mass that the nucleus is a share of
+    done = 0.0;
+    n = 0;
+    if (pass == 1 && nucleus) {
+      limit = f.top_p * (whole > 0.0 ? whole : total);
+      low = whole > 0.0 ? limit * (1.0 - kSumError) : limit;
+      if (whole > 0.0) limit *= 1.0 + kSumError;
+    }
+    total = 0.0;
+#pragma unroll 1
+    for (int i0 = 0; i0 < n1; i0 += kRowThreads) {
+      const int i = i0 + tid;
+      double w = i < n1 ? f.mass(key_logit(static_cast<uint32_t>(x[i] >> 32)), mx) : 0.0;
+      if (w < f.min_p) w = 0.0;
+      double all;
+      const double before = done + block_scan(w, all, sh.scan) - w;
+      bool in = i < n1 && w > 0.0;
+      if (pass == 1 && nucleus && i > 0) {
+        if (in && before >= low && before < limit && whole > 0.0) open = true;
+        in = in && before < low;
+      }
+      n += __syncthreads_count(in);
+      double kept;
+      block_scan(in ? w : 0.0, kept, sh.scan);
+      total += kept;
+      done += all;
+    }
+  }
+  open = __syncthreads_or(open);
+  if (whole > 0.0 && (open || n >= sure)) return 0;         // the token behind the last kept has to be a candidate
+  return n;
+}
+
+// from the n first candidates, which are sorted, by index
+NRL_DEVICE void draw_of(uint64_t* x, int n, const RowFilter& f, float mx, double u, double total, SampleShared& sh, int* out_token, float* out_logp) {
+  const int tid = threadIdx.x;
+  __syncthreads();
+  for (int i = tid; i < n; i += kRowThreads) x[i] = x[i] << 32 | x[i] >> 32;        // (~index, key)
+  sort_front(x, n);                                         // (its first barrier is behind the swap)
+  if (tid == 0) sh.token = 0x7fffffff;
+  const double target = u * total;
+  double done = 0.0;
+  int last = 0;
+#pragma unroll 1
+  for (int i0 = 0; i0 < n; i0 += kRowThreads) {
+    const int i = i0 + tid;
+    const double w = i < n ? f.mass(key_logit(static_cast<uint32_t>(x[i])), mx) : 0.0;
+    double all;
+    const double upto = done + block_scan(w, all, sh.scan);
+    if (i < n && w > 0.0 && upto > target) atomicMin(&sh.token, i);
+    done += all;
+    last = min(n, i0 + kRowThreads) - 1;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    const uint64_t y = x[min(sh.token, last)];
+    *out_token = static_cast<int>(~static_cast<uint32_t>(y >> 32));
+    *out_logp = static_cast<float>(f.x(key_logit(static_cast<uint32_t>(y)), mx) - log(total));
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads, 3) sample_filtered_kernel(const T* __restrict__ logits, long row_stride, int V,
+                                                                         const float* __restrict__ uniforms, SampleFilters filters, int* __restrict__ tokens,
+                                                                         float* __restrict__ logp) {
+  extern __shared__ float s_chunk[];                       // [chunks][kRowThreads]
+  __shared__ SampleShared sh;
+  const int rank = static_cast<int>(cluster_rank()), blocks = static_cast<int>(cluster_blocks()), tid = threadIdx.x, lane = tid & 31;
+  const long r = blockIdx.x / blocks;
+  if (tid == 0) sh.list.n = sh.list.nhits = sh.list.sent = 0;
+  if (blocks > 1) cluster_arrive();                        // the first block's memory may be written once it is known to run
+  const LogitRow<T> row(logits + r * row_stride, V);
+  const RowFilter f(filters, r, V);
+  const RowShare share(row.nvec, rank, blocks);
+  const bool few = (f.top_k > 0 && f.top_k <= kTopMax) || f.min_p > 0.0;        // what is kept is a matter of the candidates alone
+  const bool nucleus = !few && f.top_p < 1.0 && f.top_k == 0;
+  const float c = static_cast<float>(f.inv_temp * 1.4426950408889634);
+  float best, m = 0.f, s = 0.f;
+  if (nucleus)
+    row_pass<true>(row, share, c, s_chunk, best, m, s, [](int, RawVec& a) { LogitRow<T>::drop_nan(a); });
+  else
+    row_pass<false>(row, share, c, s_chunk, best, m, s, [](int, const RawVec&) {});
+  // a thread's chunks in one group up to 256 tokens, in up to four above
+  const int want = few ? (f.top_k > 0 && f.top_k <= kTopMax ? f.top_k : 0) : kNucleusGroups, groups = want <= 256 ? 1 : want <= 512 ? 2 : 4;
+  uint32_t bound = kKeyNone + 1;
+  if (few || nucleus) {
+    if (want > 0) {
+      uint32_t keys[kGroupsMax];
+      keys[0] = order_key(best);
+      if (groups > 1)
+#pragma unroll
+        for (int g = 0; g < kGroupsMax; ++g) {
+          float x = -INFINITY;
+          for (int i = g; i < share.chunks; i += groups) x = fmaxf(x, s_chunk[i * kRowThreads + tid]);
+          keys[g] = order_key(x);
+        }
+      bound = group_bound(keys, groups, want, sh.bound);
+    }
+    if (f.min_p > 0.0) {                                   // min_p of the block's largest logit or below: a little less than its border
+      const float mb = block_max(best, reinterpret_cast<float*>(sh.scan));
+      const double t = f.temp * log(f.min_p), z = mb + t - 1e-6 * (fabs(static_cast<double>(mb)) - t);
+      if (z > -3e38 && z < 3e38) bound = max(bound, order_key(static_cast<float>(z)));
+    }
+    gather_candidates(row, share, s_chunk, bound, sh.list);
+  }
+  const float mw = warp_max(nucleus ? m : best);
+  const float sw = nucleus ? warp_sum(s * ex2((m - mw) * c)) : 0.f;
+  if (blocks > 1) cluster_wait();
+  if (lane == 0) {
+    const uint32_t there = in_block(&sh.part[rank][tid >> 5], 0);
+    st_block(there, mw);
+    st_block(there + 4, sw);
+  }
+  if (tid == 0) st_block(in_block(&sh.part_bound[rank], 0), __uint_as_float(bound));
+  if (rank != 0) send_candidates(sh.list, &sh.base);
+  __syncwarp();
+  if (blocks > 1) {
+    cluster_arrive();
+    cluster_wait();
+    if (rank != 0) return;
+  } else {
+    __syncthreads();
+  }
+
+  float mx = -INFINITY;
+  for (int i = lane; i < blocks * kRowWarps; i += 32) mx = fmaxf(mx, sh.part[i / kRowWarps][i % kRowWarps].x);
+  mx = warp_max(mx);
+  const int found = join_candidates(sh.list);
+  const double u = uniforms[r];
+  bool done = false;
+  if ((few || nucleus) && found > 0 && found <= kCandidates) {
+    double whole = 0.0;
+    int sure = found;
+    if (nucleus) {
+      uint32_t least = 0;
+      for (int i = lane; i < blocks * kRowWarps; i += 32) {
+        const float2 p = sh.part[i / kRowWarps][i % kRowWarps];
+        whole += p.y * ex2((p.x - mx) * c);
+      }
+      whole = warp_sum(whole);
+      for (int i = 0; i < blocks; ++i) least = max(least, sh.part_bound[i]);
+      int n = 0;
+      for (int i = tid; i < found; i += kRowThreads) n += static_cast<uint32_t>(sh.list.cand[i] >> 32) >= least ? 1 : 0;
+      sure = static_cast<int>(block_sum(static_cast<double>(n), sh.border.red));
+    }
+    if (mx < INFINITY && (!nucleus || whole > 0.0)) {
+      sort_front(sh.list.cand, found);
+      double total;
+      const int n = kept_of(sh.list.cand, found, sure, f, mx, whole, sh, total);
+      if (n > 0) {
+        draw_of(sh.list.cand, n, f, mx, u, total, sh, tokens + r, logp + r);
+        done = true;
+      }
+    }
+  } else if ((few || nucleus) && found == 0) {             // nothing to draw from
+    if (tid == 0) {
+      tokens[r] = -1;
+      logp[r] = -INFINITY;
+    }
+    done = true;
+  }
+  if (done) return;
+  __syncthreads();
+  if (mx <= -3.4e38f) {                                    // by the pass's finite start: look again
+    float t = -INFINITY;
+    row.each([&](int, float z) { t = fmaxf(t, z); });
+    mx = block_max(t, reinterpret_cast<float*>(sh.scan));
+    if (mx == -INFINITY) {
+      if (tid == 0) {
+        tokens[r] = -1;
+        logp[r] = -INFINITY;
+      }
+      return;
+    }
+  }
+  sample_by_border(row, f, mx, u, sh, tokens + r, logp + r);
 }
 
 __global__ void row_uniforms_kernel(unsigned long long seed, unsigned long long step, const int* __restrict__ row_ids, const int* __restrict__ row_steps,
@@ -142,6 +377,26 @@ __global__ void row_uniforms_kernel(unsigned long long seed, unsigned long long 
   out[i] = 1.f - curand_uniform(&st);                      // (0, 1] -> [0, 1)
 }
 
+template <typename T>
+cudaError_t launch_sample(const void* logits, long row_stride, int rows, int V, const float* uniforms, const SampleFilters& f, int* tokens, float* logp,
+                          cudaStream_t s) {
+  const int blocks = row_blocks(rows, V, LogitRow<T>::N);
+  static PerDevice<bool> done;
+  if (const cudaError_t e = allow_smem(done, sample_filtered_kernel<T>, kRowChunks * kRowThreads * 4); e != cudaSuccess) return e;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = blocks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows) * blocks);
+  cfg.blockDim = dim3(kRowThreads);
+  cfg.dynamicSmemBytes = row_chunks(V, LogitRow<T>::N, blocks) * kRowThreads * 4;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, sample_filtered_kernel<T>, static_cast<const T*>(logits), row_stride, V, uniforms, f, tokens, logp);
+}
+
 }  // namespace nrl
 
 using namespace nrl;
@@ -149,11 +404,8 @@ using namespace nrl;
 extern "C" cudaError_t nrl_sample_filtered(const void* logits, int is_bf16, long row_stride, int rows, int V, const float* uniforms, const SampleFilters* f,
                                            int* tokens, float* logp, cudaStream_t s) {
   if (rows == 0) return cudaSuccess;
-  if (is_bf16)
-    sample_filtered_kernel<<<rows, kRowThreads, 0, s>>>(static_cast<const __nv_bfloat16*>(logits), row_stride, V, uniforms, *f, tokens, logp);
-  else
-    sample_filtered_kernel<<<rows, kRowThreads, 0, s>>>(static_cast<const float*>(logits), row_stride, V, uniforms, *f, tokens, logp);
-  return cudaGetLastError();
+  return is_bf16 ? launch_sample<__nv_bfloat16>(logits, row_stride, rows, V, uniforms, *f, tokens, logp, s)
+                 : launch_sample<float>(logits, row_stride, rows, V, uniforms, *f, tokens, logp, s);
 }
 
 extern "C" cudaError_t nrl_row_uniforms(unsigned long long seed, unsigned long long step, const int* row_ids, const int* row_steps, int rows, float* out,
