@@ -117,8 +117,10 @@ std::tuple<torch::Tensor, torch::Tensor> sample_filtered(const torch::Tensor& lo
   f.top_k_all = static_cast<int>(std::min<int64_t>(top_k_all, logits.size(1)));
   c10::cuda::CUDAGuard guard(logits.device());
   torch::Tensor tokens = torch::empty({rows}, logits.options().dtype(torch::kInt32)), logp = torch::empty({rows}, logits.options().dtype(torch::kFloat32));
+  torch::Tensor top;
+  if (!nrl_sample_is_short(&f, logits.size(1))) top = torch::empty({rows}, logp.options());
   check(nrl_sample_filtered(logits.data_ptr(), is_bf16(logits), logits.stride(0), rows, logits.size(1), uniforms.data_ptr<float>(), &f, tokens.data_ptr<int>(),
-                            logp.data_ptr<float>(), cur_stream()), "sample_filtered");
+                            logp.data_ptr<float>(), top.defined() ? top.data_ptr<float>() : nullptr, cur_stream()), "sample_filtered");
   return {tokens, logp};
 }
 

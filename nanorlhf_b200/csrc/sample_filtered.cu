@@ -7,7 +7,7 @@
 // What a filter leaves is mostly few tokens.  A row is read once, every thread keeping the maxima of its chunks; a bound that all kept tokens reach -- the
 // top_k-th largest of the threads' maxima, or the largest logit + T ln min_p -- picks the chunks that are read again, and the candidates that they hold are sorted
 // and filtered exactly.  A nucleus without other filters needs the mass of the whole row as well: the pass adds it up in float, and where what is known of its error
-// leaves the nucleus' last token open, or the candidates do not reach it, the row takes the long way: the border of the order by ranges of keys, in double.
+// leaves the nucleus' last token open, or the candidates do not reach it, the row is left to a second kernel, as are rows without filters.
 #include <curand_kernel.h>
 
 #include "common.cuh"
@@ -46,7 +46,18 @@ struct SampleShared {
   double scan[kRowWarps];
   float2 part[kRowClusterMax][kRowWarps];                  // maximum and sum of every warp of the cluster
   uint32_t part_bound[kRowClusterMax];
-  double total;
+  int base, token;
+};
+
+constexpr int kBins = 16;                                  // ranges of logits a pass of the long way
+struct LongShared {
+  BorderShared border;
+  RowList list;
+  double scan[kRowWarps];
+  double mass[kRowClusterMax][kRowWarps], whole[kRowClusterMax];         // kept for good and altogether, by ranges of the row
+  double powers[32];                                       // 2^(j / 32)
+  float bins[2][kRowClusterMax][kBins + 2];                // and what lies above them and below
+  unsigned short place[kCandidates];
   int base, token;
 };
 
@@ -71,11 +82,11 @@ NRL_DEVICE double block_scan(double v, double& all, double* red) {
   return before + v;
 }
 
-// The long way: the border by ranges of keys, then the kept mass of every warp's range and a walk through the range that holds the drawn one.
-template <typename T>
-__device__ __noinline__ void sample_by_border(const LogitRow<T>& row, const RowFilter& f, float mx, double u, SampleShared& shared, int* out_token, float* out_logp) {
-  BorderShared& sh = shared.border;
-  double* masses = shared.scan;
+// By the border alone: found by ranges of keys, all in double, then the kept mass of every warp's range and a walk through the range that holds the drawn one.
+// (A function of its own for every kernel: one that kernels of different register counts share ends ptxas 12.9.)
+template <int KERNEL, typename T>
+__device__ __noinline__ void sample_by_border(const LogitRow<T>& row, const RowFilter& f, float mx, double u, BorderShared& sh, double* masses, int* out_token,
+                                              float* out_logp) {
   const int V = row.V, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t top = order_key(mx);
   auto mass = [&](float z) { return f.mass(z, mx); };
@@ -174,6 +185,310 @@ __device__ __noinline__ void sample_by_border(const LogitRow<T>& row, const RowF
   }
 }
 
+// e^x, x <= 0, to a few steps of double, by a table and a short series (P. T. P. Tang, 1989): x = (32 i + j) ln 2 / 32 + f, |f| <= ln 2 / 64, and six
+// terms of e^f (the seventh is below 3e-15 of them).  12 operations in double, which are what a long row's masses cost.
+NRL_DEVICE double exp_mass(double x, const double* powers) {
+  if (!(x > -700.0)) return 0.0;
+  constexpr double kSteps = 46.16624130844683, kStep = 0x1.62e42fefa0000p-6, kStepLow = 5.145609244655338e-14, kMagic = 6755399441055744.0;       // 32 / ln 2, ln 2 / 32 in two parts, 1.5 * 2^52
+  const double t = fma(x, kSteps, kMagic);
+  const int n = __double2loint(t);
+  double f = fma(t - kMagic, -kStep, x);
+  f = fma(t - kMagic, -kStepLow, f);
+  double e = fma(f, 1.0 / 120, 1.0 / 24);
+  e = fma(f, e, 1.0 / 6);
+  e = fma(f, e, 0.5);
+  e = fma(f, e, 1.0);
+  e = fma(f, e, 1.0);
+  const double p = powers[n & 31];
+  return e * __hiloint2double(__double2hiint(p) + ((n >> 5) << 20), __double2loint(p));
+}
+
+// ---- the long way -------------------------------------------------------------------------------------------------------------------------------
+// Rows of which many tokens are kept: a nucleus of more than fit, or all.  The blocks of a cluster share a row.  (1) Where a nucleus ends is narrowed down by passes in
+// float that add up the mass of 16 ranges of logits, lane by lane in shared memory, until one range holds few tokens.  (2) One pass in double: what lies above
+// that range, for every warp's range of the row, and altogether; the tokens inside are gathered.  (3) The first block sorts those, finds the last kept token, and
+// walks through the range of the row that holds the drawn mass.  What does not work out (many tokens of one logit, a border next to a range's edge) is left to
+// sample_by_border: then false.
+template <typename T>
+NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx, double u, int rank, int blocks, float* s_bins, LongShared& sh, int* out_token,
+                            float* out_logp) {
+  constexpr int N = LogitRow<T>::N;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const RowShare share(row.nvec, rank, blocks);
+  const float c = static_cast<float>(f.inv_temp * 1.4426950408889634);
+  if (tid < 32) sh.powers[tid] = exp2(tid / 32.0);
+  if (tid == 0) sh.list.n = sh.list.nhits = sh.list.sent = 0;
+  // the least logit that min_p keeps: every lane tries one of 32 keys of a range, seven times
+  uint32_t floor_key = kKeyNone + 1;
+  if (f.min_p > 0.0) {
+    uint64_t lo = floor_key, hi = order_key(mx);            // in [lo, hi]; the largest logit is in whatever min_p says
+    while (lo < hi) {
+      const uint64_t step = (hi - lo + 31) / 32, k = lo + lane * step;
+      const unsigned in = __ballot_sync(0xffffffffu, k >= hi || f.mass(key_logit(static_cast<uint32_t>(k)), mx) >= f.min_p);
+      const int i = in ? __ffs(in) - 1 : 32;
+      const uint64_t up = lo + static_cast<uint64_t>(i) * step;
+      if (i == 0) { hi = lo; break; }
+      lo = lo + static_cast<uint64_t>(i - 1) * step + 1;
+      if (up < hi) hi = up;
+    }
+    floor_key = static_cast<uint32_t>(hi);
+  }
+  const float floor = key_logit(floor_key);
+  const bool nucleus = f.top_p < 1.0;
+  // kept for good: logits from `high` on; open: those from `low` on
+  float high = floor, low = floor;
+  __syncthreads();
+  if (nucleus) {
+    high = INFINITY;
+    // what lies below V / (1 - p) times less than the largest is less than 1 - p of the whole
+    const double reach = f.temp * (log(static_cast<double>(row.V)) - log1p(-f.top_p)) + 1e-3;
+    low = fmaxf(floor, static_cast<float>(mx - reach));
+    float edge = mx;                                       // where the ranges begin; above it only what earlier passes put there
+    bool enough = false;
+#pragma unroll 1
+    for (int pass = 0; pass < 8 && !enough; ++pass) {
+      for (int i = tid; i < kBins * kRowThreads; i += kRowThreads) s_bins[i] = 0.f;
+      __syncthreads();
+      const float scale = kBins / fmaxf(edge - low, 1e-30f);
+      float above = 0.f, below = 0.f;
+      float* mine = s_bins + warp * kBins * 32 + lane;
+#pragma unroll 1
+      for (int v = share.first + tid; v < share.end; v += kRowThreads) {
+        float x[N];
+        row.load(v, x);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const float z = clean(x[j]);
+          if (z < floor) continue;
+          const float e = ex2((z - mx) * c);
+          if (z >= high) above += e;
+          else if (z < low) below += e;
+          else {
+            const int b = min(kBins - 1, max(0, static_cast<int>((edge - z) * scale)));
+            mine[b * 32] += e;
+          }
+        }
+      }
+      __syncthreads();
+      float sum = 0.f;                                     // a warp a bin
+#pragma unroll 1
+      for (int w = 0; w < kRowWarps; ++w) sum += s_bins[(w * kBins + warp) * 32 + lane];
+      sum = warp_sum(sum);
+      const double up = block_sum(static_cast<double>(above), sh.scan), rest = block_sum(static_cast<double>(below), sh.scan);
+      static_assert(kBins == kRowWarps, "a warp a bin");
+      float(&slot)[kRowClusterMax][kBins + 2] = sh.bins[pass & 1];
+      if (lane < blocks) {
+        st_block(in_block(&slot[rank][warp], lane), sum);
+        if (warp == 0) {
+          st_block(in_block(&slot[rank][kBins], lane), static_cast<float>(up));
+          st_block(in_block(&slot[rank][kBins + 1], lane), static_cast<float>(rest));
+        }
+      }
+      __syncwarp();
+      cluster_arrive();
+      cluster_wait();
+      double cum = 0.0, all = 0.0;
+      for (int q = 0; q < blocks; ++q) {
+        cum += slot[q][kBins];
+        for (int b = 0; b < kBins + 2; ++b) all += slot[q][b];
+      }
+      const double target = f.top_p * all;
+      int b = 0;
+      double m = 0.0;
+      for (;; ++b) {
+        m = 0.0;
+        for (int q = 0; q < blocks; ++q) m += slot[q][b];
+        if (cum + m >= target || b == kBins - 1) break;
+        cum += m;
+      }
+      const float width = (edge - low) / kBins, over = width / 16;
+      const float e1 = b == 0 ? edge : edge - b * width + over, e0 = b == kBins - 1 ? low : edge - (b + 1) * width - over;
+      if (b > 0) high = e1;                                // else as before: what lies above the edge is known
+      edge = e1;
+      low = fmaxf(e0, low);
+      enough = m <= 1200.0 * ex2((low - mx) * c);
+      __syncthreads();
+    }
+  }
+  // ---- in double: every warp's range of the row ----
+  double kept = 0.0, all = 0.0;
+  const int per = (share.end - share.first + kRowWarps - 1) / kRowWarps, begin = min(share.end, share.first + warp * per), stop = min(share.end, begin + per);
+#pragma unroll 1
+  for (int v = begin + lane; v < stop; v += 32) {
+    float x[N];
+    row.load(v, x);
+#pragma unroll 4
+    for (int j = 0; j < N; ++j) {
+      const float z = clean(x[j]);
+      if (!(z >= floor)) continue;
+      const double w = exp_mass(f.x(z, mx), sh.powers);
+      all += w;
+      if (z >= high) {
+        kept += w;
+      } else if (z >= low) {
+        const int at = atomicAdd(&sh.list.n, 1);
+        if (at < kCandidates) sh.list.cand[at] = static_cast<uint64_t>(order_key(z)) << 32 | static_cast<uint32_t>(~(v * N - row.skew + j));
+      }
+    }
+  }
+  kept = warp_sum(kept);
+  all = block_sum(all, sh.scan);
+  if (lane == 0) st_block(in_block(&sh.mass[rank][warp], 0), kept);
+  if (tid == 0) st_block(in_block(&sh.whole[rank], 0), all);
+  __syncthreads();
+  if (rank != 0) send_candidates(sh.list, &sh.base);
+  __syncwarp();
+  cluster_arrive();
+  cluster_wait();
+  if (rank != 0) return true;
+
+  // ---- the last kept token ----
+  const int found = join_candidates(sh.list);
+  if (found > kCandidates) return false;
+  double above = 0.0, whole = 0.0;
+  for (int q = 0; q < blocks; ++q) {
+    whole += sh.whole[q];
+    for (int w = 0; w < kRowWarps; ++w) above += sh.mass[q][w];
+  }
+  Border last{floor_key, 0x7fffffff};
+  int n = 0;
+  if (nucleus) {
+    const double limit = f.top_p * whole;
+    last.key = 0xffffffffu;
+    if (found > 0) sort_front(sh.list.cand, found);
+    if (above > 0.0 && above >= limit) return false;     // the border is above the range
+    double done = above, inside = 0.0;
+#pragma unroll 1
+    for (int i0 = 0; i0 < found; i0 += kRowThreads) {
+      const int i = i0 + tid;
+      const double w = i < found ? exp_mass(f.x(key_logit(static_cast<uint32_t>(sh.list.cand[i] >> 32)), mx), sh.powers) : 0.0;
+      double sum;
+      const double before = done + block_scan(w, sum, sh.scan) - w;
+      const bool in = i < found && (before < limit || (i == 0 && above == 0.0));
+      n += __syncthreads_count(in);
+      double mine;
+      block_scan(in ? w : 0.0, mine, sh.scan);
+      inside += mine;
+      done += sum;
+    }
+    if (done < limit && low > floor) return false;       // or below it
+    if (n > 0) {
+      const uint64_t x = sh.list.cand[n - 1];
+      last.key = static_cast<uint32_t>(x >> 32);
+      last.cut = static_cast<int>(~static_cast<uint32_t>(x));
+    }
+    // kept candidates to their ranges of the row
+    const int step = (row.nvec + blocks - 1) / blocks;
+    for (int i = tid; i < n; i += kRowThreads) {
+      const int v = (static_cast<int>(~static_cast<uint32_t>(sh.list.cand[i])) + row.skew) / N, q = v / step, first = q * step;
+      const int share_per = (min(row.nvec, first + step) - first + kRowWarps - 1) / kRowWarps;
+      sh.place[i] = static_cast<unsigned short>(q * kRowWarps + (v - first) / share_per);
+    }
+    __syncthreads();
+    if (tid < blocks * kRowWarps) {
+      double m = sh.mass[tid / kRowWarps][tid % kRowWarps];
+      for (int i = 0; i < n; ++i)
+        if (sh.place[i] == tid) m += exp_mass(f.x(key_logit(static_cast<uint32_t>(sh.list.cand[i] >> 32)), mx), sh.powers);
+      sh.mass[tid / kRowWarps][tid % kRowWarps] = m;
+    }
+    __syncthreads();
+  }
+  // ---- the range that holds the drawn mass, and the token in it ----
+  double total = 0.0;
+  for (int i = 0; i < blocks * kRowWarps; ++i) total += sh.mass[i / kRowWarps][i % kRowWarps];
+  const double target = u * total;
+  double base = 0.0, before = 0.0;
+  int range = -1;
+  for (int i = 0; i < blocks * kRowWarps; ++i) {
+    const double m = sh.mass[i / kRowWarps][i % kRowWarps];
+    if (!(m > 0.0)) continue;
+    range = i;
+    before = base;
+    base += m;
+    if (base > target) break;
+  }
+  if (range < 0) return false;
+  const RowShare there(row.nvec, range / kRowWarps, blocks);
+  const int tper = (there.end - there.first + kRowWarps - 1) / kRowWarps, t0 = min(there.end, there.first + range % kRowWarps * tper), t1 = min(there.end, t0 + tper);
+  if (tid == 0) {
+    sh.token = -1;
+    sh.base = 0x7fffffff;                                  // the first thread up to whose tokens the mass passes
+  }
+  int lead = -1;                                           // of this thread: its last kept token
+  __syncthreads();
+#pragma unroll 1
+  for (int v0 = t0; v0 < t1; v0 += kRowThreads) {
+    const int v = v0 + tid, e0 = v * N - row.skew;
+    float x[N];
+    double sum = 0.0;
+    if (v < t1) {
+      row.load(v, x);
+#pragma unroll 1
+      for (int j = 0; j < N; ++j) {
+        const float z = clean(x[j]);
+        if (e0 + j >= 0 && e0 + j < row.V && z >= floor && (z >= high || last.has(order_key(z), e0 + j))) {
+          const double w = exp_mass(f.x(z, mx), sh.powers);
+          sum += w;
+          if (w > 0.0) lead = e0 + j;
+        }
+      }
+    }
+    double tile;
+    const double upto = before + block_scan(sum, tile, sh.scan);
+    if (sum > 0.0 && upto > target) atomicMin(&sh.base, tid);
+    __syncthreads();
+    if (sh.base == tid) {
+      double a = upto - sum;
+      int hit = lead;
+#pragma unroll 1
+      for (int j = 0; j < N; ++j) {
+        const float z = clean(x[j]);
+        if (e0 + j >= 0 && e0 + j < row.V && z >= floor && (z >= high || last.has(order_key(z), e0 + j))) {
+          const double w = exp_mass(f.x(z, mx), sh.powers);
+          a += w;
+          if (w > 0.0 && a > target) {
+            hit = e0 + j;
+            break;
+          }
+        }
+      }
+      sh.token = hit;
+    }
+    before += tile;
+    if (sh.base != 0x7fffffff) break;
+  }
+  if (sh.base == 0x7fffffff && lead >= 0) atomicMax(&sh.token, lead);      // rounding lets none pass: the range's last
+  __syncthreads();
+  if (tid == 0) {
+    *out_token = sh.token;
+    *out_logp = static_cast<float>(f.x(row.at(sh.token), mx) - log(total));
+  }
+  return true;
+}
+
+// rows whose largest logit the kernel in front has left in `top` (NaN: drawn already)
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads, 2) sample_long_kernel(const T* __restrict__ logits, long row_stride, int V, const float* __restrict__ uniforms,
+                                                                     SampleFilters filters, const float* __restrict__ top, int* __restrict__ tokens,
+                                                                     float* __restrict__ logp) {
+  extern __shared__ float s_bins[];                        // [warps][kBins][32]
+  __shared__ LongShared sh;
+  const int rank = static_cast<int>(cluster_rank()), blocks = static_cast<int>(cluster_blocks());
+  const long r = blockIdx.x / blocks;
+  const float mx = top[r];
+  if (mx != mx) return;
+  const LogitRow<T> row(logits + r * row_stride, V);
+  const RowFilter f(filters, r, V);
+  if (blocks > 1) {                                        // shared memory may be written by the others once it is known to run
+    cluster_arrive();
+    cluster_wait();
+  }
+  if (!sample_long(row, f, mx, uniforms[r], rank, blocks, s_bins, sh, tokens + r, logp + r)) {
+    __syncthreads();
+    sample_by_border<1>(row, f, mx, uniforms[r], sh.border, sh.scan, tokens + r, logp + r);
+  }
+}
+
 // Float sums of 2^x are off by so much of themselves at most: 2^-22 for 2^x, three steps of 2^-24 of the exponents, whose mean over the mass is log2 V < 24 at most, and
 // sums of at most 300 terms a thread in float.
 constexpr double kSumError = 2e-5;
@@ -254,7 +569,7 @@ NRL_DEVICE void draw_of(uint64_t* x, int n, const RowFilter& f, float mx, double
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads, 3) sample_filtered_kernel(const T* __restrict__ logits, long row_stride, int V,
                                                                          const float* __restrict__ uniforms, SampleFilters filters, int* __restrict__ tokens,
-                                                                         float* __restrict__ logp) {
+                                                                         float* __restrict__ logp, float* __restrict__ top) {
   extern __shared__ float s_chunk[];                       // [chunks][kRowThreads]
   __shared__ SampleShared sh;
   const int rank = static_cast<int>(cluster_rank()), blocks = static_cast<int>(cluster_blocks()), tid = threadIdx.x, lane = tid & 31;
@@ -319,8 +634,15 @@ __global__ void __launch_bounds__(kRowThreads, 3) sample_filtered_kernel(const T
   mx = warp_max(mx);
   const int found = join_candidates(sh.list);
   const double u = uniforms[r];
-  bool done = false;
-  if ((few || nucleus) && found > 0 && found <= kCandidates) {
+  float open = __int_as_float(0x7fffffff);                 // NaN: drawn
+  if (mx == -INFINITY || ((few || nucleus) && found == 0)) {        // nothing to draw from
+    if (tid == 0) {
+      tokens[r] = -1;
+      logp[r] = -INFINITY;
+    }
+  } else if (mx == INFINITY || (few && found > kCandidates && f.top_k > 0) || (!few && f.top_k > 0)) {
+    sample_by_border<0>(row, f, mx, u, sh.border, sh.scan, tokens + r, logp + r);
+  } else if ((few || nucleus) && found <= kCandidates) {
     double whole = 0.0;
     int sure = found;
     if (nucleus) {
@@ -335,37 +657,15 @@ __global__ void __launch_bounds__(kRowThreads, 3) sample_filtered_kernel(const T
       for (int i = tid; i < found; i += kRowThreads) n += static_cast<uint32_t>(sh.list.cand[i] >> 32) >= least ? 1 : 0;
       sure = static_cast<int>(block_sum(static_cast<double>(n), sh.border.red));
     }
-    if (mx < INFINITY && (!nucleus || whole > 0.0)) {
-      sort_front(sh.list.cand, found);
-      double total;
-      const int n = kept_of(sh.list.cand, found, sure, f, mx, whole, sh, total);
-      if (n > 0) {
-        draw_of(sh.list.cand, n, f, mx, u, total, sh, tokens + r, logp + r);
-        done = true;
-      }
-    }
-  } else if ((few || nucleus) && found == 0) {             // nothing to draw from
-    if (tid == 0) {
-      tokens[r] = -1;
-      logp[r] = -INFINITY;
-    }
-    done = true;
+    sort_front(sh.list.cand, found);
+    double total;
+    const int n = kept_of(sh.list.cand, found, sure, f, mx, whole, sh, total);
+    if (n > 0) draw_of(sh.list.cand, n, f, mx, u, total, sh, tokens + r, logp + r);
+    else open = mx;
+  } else {
+    open = mx;
   }
-  if (done) return;
-  __syncthreads();
-  if (mx <= -3.4e38f) {                                    // by the pass's finite start: look again
-    float t = -INFINITY;
-    row.each([&](int, float z) { t = fmaxf(t, z); });
-    mx = block_max(t, reinterpret_cast<float*>(sh.scan));
-    if (mx == -INFINITY) {
-      if (tid == 0) {
-        tokens[r] = -1;
-        logp[r] = -INFINITY;
-      }
-      return;
-    }
-  }
-  sample_by_border(row, f, mx, u, sh, tokens + r, logp + r);
+  if (tid == 0 && top != nullptr) top[r] = open;
 }
 
 __global__ void row_uniforms_kernel(unsigned long long seed, unsigned long long step, const int* __restrict__ row_ids, const int* __restrict__ row_steps,
@@ -379,10 +679,11 @@ __global__ void row_uniforms_kernel(unsigned long long seed, unsigned long long 
 
 template <typename T>
 cudaError_t launch_sample(const void* logits, long row_stride, int rows, int V, const float* uniforms, const SampleFilters& f, int* tokens, float* logp,
-                          cudaStream_t s) {
-  const int blocks = row_blocks(rows, V, LogitRow<T>::N);
-  static PerDevice<bool> done;
+                          float* top, cudaStream_t s) {
+  static PerDevice<bool> done, done_long;
   if (const cudaError_t e = allow_smem(done, sample_filtered_kernel<T>, kRowChunks * kRowThreads * 4); e != cudaSuccess) return e;
+  if (const cudaError_t e = allow_smem(done_long, sample_long_kernel<T>, kBins * kRowThreads * 4); e != cudaSuccess) return e;
+  const int blocks = row_blocks(rows, V, LogitRow<T>::N);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = blocks;
@@ -394,18 +695,29 @@ cudaError_t launch_sample(const void* logits, long row_stride, int rows, int V, 
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, sample_filtered_kernel<T>, static_cast<const T*>(logits), row_stride, V, uniforms, f, tokens, logp);
+  const T* z = static_cast<const T*>(logits);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_filtered_kernel<T>, z, row_stride, V, uniforms, f, tokens, logp, top);
+  if (e != cudaSuccess || top == nullptr) return e;
+  cfg.dynamicSmemBytes = kBins * kRowThreads * 4;
+  return cudaLaunchKernelEx(&cfg, sample_long_kernel<T>, z, row_stride, V, uniforms, f, static_cast<const float*>(top), tokens, logp);
 }
 
 }  // namespace nrl
 
 using namespace nrl;
 
+// Every row is settled by its candidates, or by its border in the first kernel: one top_k of 1 to kTopMax for all, or temperature 0.
+extern "C" int nrl_sample_is_short(const SampleFilters* f, int V) {
+  const bool greedy = f->temperature == nullptr && !(f->temperature_all > 0.0);
+  return greedy || (f->top_k == nullptr && f->top_k_all > 0 && f->top_k_all <= kTopMax && f->top_k_all < V);
+}
+
 extern "C" cudaError_t nrl_sample_filtered(const void* logits, int is_bf16, long row_stride, int rows, int V, const float* uniforms, const SampleFilters* f,
-                                           int* tokens, float* logp, cudaStream_t s) {
+                                           int* tokens, float* logp, float* top, cudaStream_t s) {
   if (rows == 0) return cudaSuccess;
-  return is_bf16 ? launch_sample<__nv_bfloat16>(logits, row_stride, rows, V, uniforms, *f, tokens, logp, s)
-                 : launch_sample<float>(logits, row_stride, rows, V, uniforms, *f, tokens, logp, s);
+  if (top == nullptr && !nrl_sample_is_short(f, V)) return cudaErrorInvalidValue;
+  return is_bf16 ? launch_sample<__nv_bfloat16>(logits, row_stride, rows, V, uniforms, *f, tokens, logp, top, s)
+                 : launch_sample<float>(logits, row_stride, rows, V, uniforms, *f, tokens, logp, top, s);
 }
 
 extern "C" cudaError_t nrl_row_uniforms(unsigned long long seed, unsigned long long step, const int* row_ids, const int* row_steps, int rows, float* out,

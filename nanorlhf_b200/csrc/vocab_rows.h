@@ -24,8 +24,10 @@ struct SampleFilters {
   double temperature_all, top_p_all, min_p_all;
   int top_k_all;
 };
+// top: [rows] of scratch; may be null where nrl_sample_is_short says so
 cudaError_t nrl_sample_filtered(const void* logits, int is_bf16, long row_stride, int rows, int V, const float* uniforms, const SampleFilters* f,
-                                int* tokens, float* logp, cudaStream_t s);
+                                int* tokens, float* logp, float* top, cudaStream_t s);
+int nrl_sample_is_short(const SampleFilters* f, int V);
 // uniforms[i] in [0, 1) of (seed, row_ids[i], step + row_steps[i])
 cudaError_t nrl_row_uniforms(unsigned long long seed, unsigned long long step, const int* row_ids, const int* row_steps, int rows, float* out,
                              cudaStream_t s);
