@@ -39,6 +39,10 @@ struct RowFilter {
   NRL_DEVICE double mass(float z, float mx) const { return z == mx ? 1.0 : exp((static_cast<double>(z) - mx) * inv_temp); }
 };
 
+// Float sums of 2^x are off by so much of themselves at most: 2^-22 for 2^x, three steps of 2^-24 of the exponents, whose mean over the mass is log2 V < 24 at most, and
+// sums of at most 300 terms a thread in float.
+constexpr double kSumError = 2e-5;
+
 struct SampleShared {
   BorderShared border;
   RowList list;
@@ -49,16 +53,17 @@ struct SampleShared {
   int base, token;
 };
 
-constexpr int kBins = 16;                                  // ranges of logits a pass of the long way
+constexpr int kBins = 32;                                  // ranges of logits a pass of the long way
 struct LongShared {
   BorderShared border;
   RowList list;
   double scan[kRowWarps];
   double mass[kRowClusterMax][kRowWarps], whole[kRowClusterMax];         // kept for good and altogether, by ranges of the row
-  double powers[32];                                       // 2^(j / 32)
-  float bins[2][kRowClusterMax][kBins + 2];                // and what lies above them and below
+  double powers[128];
+  float bins[kRowClusterMax][kBins + 2];                   // what lies above them, they, and what lies below
+  float edge, high, low;
   unsigned short place[kCandidates];
-  int base, token;
+  int base, token, enough;
 };
 
 // sums over the threads up to and with this one, and over all
@@ -185,38 +190,43 @@ __device__ __noinline__ void sample_by_border(const LogitRow<T>& row, const RowF
   }
 }
 
-// e^x, x <= 0, to a few steps of double, by a table and a short series (P. T. P. Tang, 1989): x = (32 i + j) ln 2 / 32 + f, |f| <= ln 2 / 64, and six
-// terms of e^f (the seventh is below 3e-15 of them).  12 operations in double, which are what a long row's masses cost.
-NRL_DEVICE double exp_mass(double x, const double* powers) {
-  if (!(x > -700.0)) return 0.0;
-  constexpr double kSteps = 46.16624130844683, kStep = 0x1.62e42fefa0000p-6, kStepLow = 5.145609244655338e-14, kMagic = 6755399441055744.0;       // 32 / ln 2, ln 2 / 32 in two parts, 1.5 * 2^52
-  const double t = fma(x, kSteps, kMagic);
-  const int n = __double2loint(t);
-  double f = fma(t - kMagic, -kStep, x);
-  f = fma(t - kMagic, -kStepLow, f);
-  double e = fma(f, 1.0 / 120, 1.0 / 24);
-  e = fma(f, e, 1.0 / 6);
-  e = fma(f, e, 0.5);
-  e = fma(f, e, 1.0);
-  e = fma(f, e, 1.0);
-  const double p = powers[n & 31];
-  return e * __hiloint2double(__double2hiint(p) + ((n >> 5) << 20), __double2loint(p));
-}
+// w = e^((z - mx) / T) of a row, to a few steps of double, by a table and a short series (P. T. P. Tang, 1989): (z - mx) / T = (n + r) ln 2 / 128, n whole, |r| <= 1/2, so that
+// w = 2^(n / 128) e^(r ln 2 / 128), the first from a table of 128 and an exponent, the second by five terms (the sixth is below 2e-15 of them).  Not for z below
+// mx - 690 T, which has no such power of 2 (nor a share of a sum).
+struct RowMass {
+  double a, mx;                                            // n + r = (z - mx) a
+  const double* powers;                                    // 2^(j / 128)
+  static constexpr double kLn2 = 0.69314718055994530942;
+  NRL_DEVICE RowMass(const RowFilter& f, float largest, const double* table) : a(f.inv_temp * (128.0 / kLn2)), mx(largest), powers(table) {}
+  NRL_DEVICE double operator()(float z) const {
+    constexpr double kMagic = 6755399441055744.0;          // 1.5 * 2^52: the sum's low bits are the whole number
+    constexpr double kStep = kLn2 / 128;
+    const double y = (static_cast<double>(z) - mx) * a, t = y + kMagic, r = y - (t - kMagic);
+    const int n = __double2loint(t);
+    double e = fma(r, kStep * kStep * kStep * kStep / 24, kStep * kStep * kStep / 6);
+    e = fma(r, e, kStep * kStep / 2);
+    e = fma(r, e, kStep);
+    e = fma(r, e, 1.0);
+    const double p = powers[n & 127];
+    return e * __hiloint2double(__double2hiint(p) + ((n >> 7) << 20), __double2loint(p));
+  }
+};
 
 // ---- the long way -------------------------------------------------------------------------------------------------------------------------------
 // Rows of which many tokens are kept: a nucleus of more than fit, or all.  The blocks of a cluster share a row.  (1) Where a nucleus ends is narrowed down by passes in
-// float that add up the mass of 16 ranges of logits, lane by lane in shared memory, until one range holds few tokens.  (2) One pass in double: what lies above
-// that range, for every warp's range of the row, and altogether; the tokens inside are gathered.  (3) The first block sorts those, finds the last kept token, and
-// walks through the range of the row that holds the drawn mass.  What does not work out (many tokens of one logit, a border next to a range's edge) is left to
-// sample_by_border: then false.
+// float that add up the mass of 32 ranges of logits, every lane for itself in shared memory, until one range holds few tokens: two passes for the logits of an untrained
+// model.  (2) One pass in double: what lies above that range, for every warp's range of the row, and altogether; the tokens inside are gathered.  (3) The first
+// block sorts those, finds the last kept token, and walks through the range of the row that holds the drawn mass.  What does not work out (many tokens of one
+// logit) is left to sample_by_border: then false.
 template <typename T>
-NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx, double u, int rank, int blocks, float* s_bins, LongShared& sh, int* out_token,
-                            float* out_logp) {
+NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx, double u, int rank, int blocks, uint32_t* s_hist, LongShared& sh,
+                            int* out_token, float* out_logp) {
   constexpr int N = LogitRow<T>::N;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const RowShare share(row.nvec, rank, blocks);
   const float c = static_cast<float>(f.inv_temp * 1.4426950408889634);
-  if (tid < 32) sh.powers[tid] = exp2(tid / 32.0);
+  if (tid < 128) sh.powers[tid] = exp2(tid / 128.0);
+  const RowMass mass(f, mx, sh.powers);
   if (tid == 0) sh.list.n = sh.list.nhits = sh.list.sent = 0;
   // the least logit that min_p keeps: every lane tries one of 32 keys of a range, seven times
   uint32_t floor_key = kKeyNone + 1;
@@ -233,113 +243,129 @@ NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx
     }
     floor_key = static_cast<uint32_t>(hi);
   }
-  const float floor = key_logit(floor_key);
+  const float floor = fmaxf(key_logit(floor_key), static_cast<float>(fmax(-3e38, mx - 690.0 * f.temp)));
   const bool nucleus = f.top_p < 1.0;
   // kept for good: logits from `high` on; open: those from `low` on
   float high = floor, low = floor;
   __syncthreads();
   if (nucleus) {
     high = INFINITY;
-    // what lies below V / (1 - p) times less than the largest is less than 1 - p of the whole
+    // what lies below V / (1 - p) times less than the largest is less than 1 - p of the whole; with min_p the ranges begin with what that keeps
     const double reach = f.temp * (log(static_cast<double>(row.V)) - log1p(-f.top_p)) + 1e-3;
-    low = fmaxf(floor, static_cast<float>(mx - reach));
-    float edge = mx;                                       // where the ranges begin; above it only what earlier passes put there
+    if (!(f.min_p > 0.0)) low = fmaxf(floor, static_cast<float>(mx - reach));
+    float edge = mx;                                       // where the ranges begin
+    uint32_t* const mine = s_hist + warp * (kBins + 2) * 32 + lane;
     bool enough = false;
 #pragma unroll 1
-    for (int pass = 0; pass < 8 && !enough; ++pass) {
-      for (int i = tid; i < kBins * kRowThreads; i += kRowThreads) s_bins[i] = 0.f;
-      __syncthreads();
-      const float scale = kBins / fmaxf(edge - low, 1e-30f);
-      float above = 0.f, below = 0.f;
-      float* mine = s_bins + warp * kBins * 32 + lane;
+    for (int pass = 0; pass < 6 && !enough; ++pass) {
+#pragma unroll 8
+      for (int i = 0; i < kBins + 2; ++i) mine[i * 32] = 0;
+      // 2^23 and, rounded to whole numbers there, the number of the range: 0 above them, 1 .. kBins, kBins + 1 below
+      const float scale = -kBins / fmaxf(edge - low, 1e-30f), zero = 8388608.f, half = edge - 0.5f / scale;
 #pragma unroll 1
       for (int v = share.first + tid; v < share.end; v += kRowThreads) {
         float x[N];
         row.load(v, x);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-          const float z = clean(x[j]);
-          if (z < floor) continue;
-          const float e = ex2((z - mx) * c);
-          if (z >= high) above += e;
-          else if (z < low) below += e;
-          else {
-            const int b = min(kBins - 1, max(0, static_cast<int>((edge - z) * scale)));
-            mine[b * 32] += e;
-          }
+          const float z = fmaxf(x[j], -3e38f);             // NaN have no mass
+          const float t = fminf(fmaxf(fmaf(z - half, scale, zero), zero), zero + (kBins + 1));
+          uint32_t* const bin = mine + (__float_as_uint(t) & 63u) * 32;
+          *bin = __float_as_uint(__uint_as_float(*bin) + ex2((z - mx) * c));
         }
       }
       __syncthreads();
-      float sum = 0.f;                                     // a warp a bin
 #pragma unroll 1
-      for (int w = 0; w < kRowWarps; ++w) sum += s_bins[(w * kBins + warp) * 32 + lane];
-      sum = warp_sum(sum);
-      const double up = block_sum(static_cast<double>(above), sh.scan), rest = block_sum(static_cast<double>(below), sh.scan);
-      static_assert(kBins == kRowWarps, "a warp a bin");
-      float(&slot)[kRowClusterMax][kBins + 2] = sh.bins[pass & 1];
-      if (lane < blocks) {
-        st_block(in_block(&slot[rank][warp], lane), sum);
-        if (warp == 0) {
-          st_block(in_block(&slot[rank][kBins], lane), static_cast<float>(up));
-          st_block(in_block(&slot[rank][kBins + 1], lane), static_cast<float>(rest));
-        }
+      for (int b = warp; b < kBins + 2; b += kRowWarps) {
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kRowWarps; ++w) sum += __uint_as_float(s_hist[(w * (kBins + 2) + b) * 32 + lane]);
+        sum = warp_sum(sum);
+        if (lane == 0) st_block(in_block(&sh.bins[rank][b], 0), sum);
       }
       __syncwarp();
-      cluster_arrive();
-      cluster_wait();
-      double cum = 0.0, all = 0.0;
-      for (int q = 0; q < blocks; ++q) {
-        cum += slot[q][kBins];
-        for (int b = 0; b < kBins + 2; ++b) all += slot[q][b];
+      if (blocks > 1) {
+        cluster_arrive();
+        cluster_wait();
+      } else {
+        __syncthreads();
       }
-      const double target = f.top_p * all;
-      int b = 0;
-      double m = 0.0;
-      for (;; ++b) {
-        m = 0.0;
-        for (int q = 0; q < blocks; ++q) m += slot[q][b];
-        if (cum + m >= target || b == kBins - 1) break;
-        cum += m;
+      if (rank == 0 && warp == 0) {                        // a lane a range
+        double m = 0.0, start = 0.0, rest = 0.0;
+        for (int q = 0; q < blocks; ++q) {
+          m += sh.bins[q][lane + 1];
+          start += sh.bins[q][0];
+          rest += f.min_p > 0.0 && low <= floor ? 0.0 : sh.bins[q][kBins + 1];
+        }
+        double upto = m;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double y = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += y;
+        }
+        upto += start;
+        const double whole = __shfl_sync(0xffffffffu, upto, 31) + rest;
+        // from the range in which the mass passes what the nucleus needs, less what float sums may be off by, to the one in which it passes that and as much more
+        const unsigned past0 = __ballot_sync(0xffffffffu, upto >= whole * (f.top_p - kSumError / 2)), past1 = __ballot_sync(0xffffffffu, upto >= whole * (f.top_p + kSumError / 2));
+        const int b0 = past0 ? __ffs(past0) - 1 : 31, b1 = past1 ? __ffs(past1) - 1 : 31;
+        const double open = __shfl_sync(0xffffffffu, upto, b1) - __shfl_sync(0xffffffffu, upto - m, b0);
+        const float width = (edge - low) / kBins, over = width / 8 + 1e-6f * (fabsf(edge) + fabsf(low));
+        const float e1 = b0 == 0 ? edge : edge - b0 * width + over, e0 = b1 == kBins - 1 ? low : edge - (b1 + 1) * width - over;
+        const float next_high = b0 > 0 ? e1 : high, next_low = fmaxf(e0, low);
+        const int ok = open <= 1900.0 * ex2((next_low - mx) * c);
+        if (lane < blocks) {
+          st_block(in_block(&sh.edge, lane), e1);
+          st_block(in_block(&sh.high, lane), next_high);
+          st_block(in_block(&sh.low, lane), next_low);
+          st_block(in_block(&sh.enough, lane), __int_as_float(ok));
+        }
+        __syncwarp();
       }
-      const float width = (edge - low) / kBins, over = width / 16;
-      const float e1 = b == 0 ? edge : edge - b * width + over, e0 = b == kBins - 1 ? low : edge - (b + 1) * width - over;
-      if (b > 0) high = e1;                                // else as before: what lies above the edge is known
-      edge = e1;
-      low = fmaxf(e0, low);
-      enough = m <= 1200.0 * ex2((low - mx) * c);
+      if (blocks > 1) {
+        cluster_arrive();
+        cluster_wait();
+      }
+      __syncthreads();
+      edge = sh.edge;
+      high = sh.high;
+      low = sh.low;
+      enough = sh.enough != 0;
       __syncthreads();
     }
   }
   // ---- in double: every warp's range of the row ----
-  double kept = 0.0, all = 0.0;
+  double kept = 0.0, other = 0.0;
   const int per = (share.end - share.first + kRowWarps - 1) / kRowWarps, begin = min(share.end, share.first + warp * per), stop = min(share.end, begin + per);
 #pragma unroll 1
   for (int v = begin + lane; v < stop; v += 32) {
     float x[N];
     row.load(v, x);
-#pragma unroll 4
+    unsigned open = 0;
+#pragma unroll
     for (int j = 0; j < N; ++j) {
-      const float z = clean(x[j]);
-      if (!(z >= floor)) continue;
-      const double w = exp_mass(f.x(z, mx), sh.powers);
-      all += w;
-      if (z >= high) {
-        kept += w;
-      } else if (z >= low) {
-        const int at = atomicAdd(&sh.list.n, 1);
-        if (at < kCandidates) sh.list.cand[at] = static_cast<uint64_t>(order_key(z)) << 32 | static_cast<uint32_t>(~(v * N - row.skew + j));
-      }
+      const float z = x[j];                                // (NaN is not above anything)
+      const double w = mass(z);
+      if (z >= high) kept += w;
+      else if (z >= floor) other += w;
+      open |= (z >= low && z < high ? 1u : 0u) << j;
+    }
+    for (; open != 0; open &= open - 1) {
+      const int e = v * N - row.skew + __ffs(open) - 1, at = atomicAdd(&sh.list.n, 1);
+      if (at < kCandidates) sh.list.cand[at] = static_cast<uint64_t>(order_key(row.at(e))) << 32 | static_cast<uint32_t>(~e);
     }
   }
+  const double all = block_sum(kept + other, sh.scan);
   kept = warp_sum(kept);
-  all = block_sum(all, sh.scan);
   if (lane == 0) st_block(in_block(&sh.mass[rank][warp], 0), kept);
   if (tid == 0) st_block(in_block(&sh.whole[rank], 0), all);
   __syncthreads();
   if (rank != 0) send_candidates(sh.list, &sh.base);
   __syncwarp();
-  cluster_arrive();
-  cluster_wait();
+  if (blocks > 1) {
+    cluster_arrive();
+    cluster_wait();
+  }
+  __syncthreads();
   if (rank != 0) return true;
 
   // ---- the last kept token ----
@@ -357,18 +383,16 @@ NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx
     last.key = 0xffffffffu;
     if (found > 0) sort_front(sh.list.cand, found);
     if (above > 0.0 && above >= limit) return false;     // the border is above the range
-    double done = above, inside = 0.0;
+    double done = above;
+    double* const masses = reinterpret_cast<double*>(s_hist);        // the ranges of logits are not needed any more
 #pragma unroll 1
     for (int i0 = 0; i0 < found; i0 += kRowThreads) {
       const int i = i0 + tid;
-      const double w = i < found ? exp_mass(f.x(key_logit(static_cast<uint32_t>(sh.list.cand[i] >> 32)), mx), sh.powers) : 0.0;
+      const double w = i < found ? mass(key_logit(static_cast<uint32_t>(sh.list.cand[i] >> 32))) : 0.0;
+      if (i < found) masses[i] = w;
       double sum;
       const double before = done + block_scan(w, sum, sh.scan) - w;
-      const bool in = i < found && (before < limit || (i == 0 && above == 0.0));
-      n += __syncthreads_count(in);
-      double mine;
-      block_scan(in ? w : 0.0, mine, sh.scan);
-      inside += mine;
+      n += __syncthreads_count(i < found && (before < limit || (i == 0 && above == 0.0)));
       done += sum;
     }
     if (done < limit && low > floor) return false;       // or below it
@@ -385,11 +409,11 @@ NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx
       sh.place[i] = static_cast<unsigned short>(q * kRowWarps + (v - first) / share_per);
     }
     __syncthreads();
-    if (tid < blocks * kRowWarps) {
-      double m = sh.mass[tid / kRowWarps][tid % kRowWarps];
-      for (int i = 0; i < n; ++i)
-        if (sh.place[i] == tid) m += exp_mass(f.x(key_logit(static_cast<uint32_t>(sh.list.cand[i] >> 32)), mx), sh.powers);
-      sh.mass[tid / kRowWarps][tid % kRowWarps] = m;
+    for (int q = warp; q < blocks * kRowWarps; q += kRowWarps) {
+      double m = 0.0;
+      for (int i = lane; i < n; i += 32) m += sh.place[i] == q ? masses[i] : 0.0;
+      m = warp_sum(m);
+      if (lane == 0) sh.mass[q / kRowWarps][q % kRowWarps] += m;
     }
     __syncthreads();
   }
@@ -427,7 +451,7 @@ NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx
       for (int j = 0; j < N; ++j) {
         const float z = clean(x[j]);
         if (e0 + j >= 0 && e0 + j < row.V && z >= floor && (z >= high || last.has(order_key(z), e0 + j))) {
-          const double w = exp_mass(f.x(z, mx), sh.powers);
+          const double w = mass(z);
           sum += w;
           if (w > 0.0) lead = e0 + j;
         }
@@ -444,7 +468,7 @@ NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx
       for (int j = 0; j < N; ++j) {
         const float z = clean(x[j]);
         if (e0 + j >= 0 && e0 + j < row.V && z >= floor && (z >= high || last.has(order_key(z), e0 + j))) {
-          const double w = exp_mass(f.x(z, mx), sh.powers);
+          const double w = mass(z);
           a += w;
           if (w > 0.0 && a > target) {
             hit = e0 + j;
@@ -471,7 +495,7 @@ template <typename T>
 __global__ void __launch_bounds__(kRowThreads, 2) sample_long_kernel(const T* __restrict__ logits, long row_stride, int V, const float* __restrict__ uniforms,
                                                                      SampleFilters filters, const float* __restrict__ top, int* __restrict__ tokens,
                                                                      float* __restrict__ logp) {
-  extern __shared__ float s_bins[];                        // [warps][kBins][32]
+  extern __shared__ __align__(16) uint32_t s_hist[];       // floats [warps][kBins + 2][32]
   __shared__ LongShared sh;
   const int rank = static_cast<int>(cluster_rank()), blocks = static_cast<int>(cluster_blocks());
   const long r = blockIdx.x / blocks;
@@ -483,86 +507,73 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_long_kernel(const T* __
     cluster_arrive();
     cluster_wait();
   }
-  if (!sample_long(row, f, mx, uniforms[r], rank, blocks, s_bins, sh, tokens + r, logp + r)) {
+  if (!sample_long(row, f, mx, uniforms[r], rank, blocks, s_hist, sh, tokens + r, logp + r)) {
     __syncthreads();
     sample_by_border<1>(row, f, mx, uniforms[r], sh.border, sh.scan, tokens + r, logp + r);
   }
 }
 
-// Float sums of 2^x are off by so much of themselves at most: 2^-22 for 2^x, three steps of 2^-24 of the exponents, whose mean over the mass is log2 V < 24 at most, and
-// sums of at most 300 terms a thread in float.
-constexpr double kSumError = 2e-5;
 constexpr int kNucleusGroups = 128;                        // groups whose maxima bound the candidates of a nucleus
 
 // Over the sorted candidates: how many of them are kept; 0: it is not known (nucleus of a whole row whose mass `whole` is only known to kSumError, or whose last token is
-// not among the `sure` first, beyond which others may come between).
-NRL_DEVICE int kept_of(const uint64_t* x, int found, int sure, const RowFilter& f, float mx, double whole, SampleShared& sh, double& total) {
-  const int tid = threadIdx.x;
+// not among the `sure` first, beyond which others may come between).  mass, upto: theirs, and the sums up to and with every one.
+NRL_DEVICE int kept_of(const uint64_t* x, int found, int sure, const RowFilter& f, float mx, double whole, double* mass, double* upto, SampleShared& sh) {
+  const int tid = threadIdx.x, n1 = f.top_k > 0 && f.top_k < found ? f.top_k : found;
   double done = 0.0;
-  int n = 0, n1 = found;
-  bool open = false;
-  total = 0.0;
-  if (f.top_k > 0 && f.top_k < n1) n1 = f.top_k;
-  const bool nucleus = f.top_p < 1.0;
-  double limit = 1e300, low = 0.0;
-  for (int pass = nucleus && whole == 0.0 ? 0 : 1; pass < 2; ++pass) {        // the first for the mass that the nucleus is a share of
-    done = 0.0;
-    n = 0;
-    if (pass == 1 && nucleus) {
-      limit = f.top_p * (whole > 0.0 ? whole : total);
-      low = whole > 0.0 ? limit * (1.0 - kSumError) : limit;
-      if (whole > 0.0) limit *= 1.0 + kSumError;
-    }
-    total = 0.0;
 #pragma unroll 1
-    for (int i0 = 0; i0 < n1; i0 += kRowThreads) {
-      const int i = i0 + tid;
-      double w = i < n1 ? f.mass(key_logit(static_cast<uint32_t>(x[i] >> 32)), mx) : 0.0;
-      if (w < f.min_p) w = 0.0;
-      double all;
-      const double before = done + block_scan(w, all, sh.scan) - w;
-      bool in = i < n1 && w > 0.0;
-      if (pass == 1 && nucleus && i > 0) {
-        if (in && before >= low && before < limit && whole > 0.0) open = true;
-        in = in && before < low;
-      }
-      n += __syncthreads_count(in);
-      double kept;
-      block_scan(in ? w : 0.0, kept, sh.scan);
-      total += kept;
-      done += all;
+  for (int i0 = 0; i0 < n1; i0 += kRowThreads) {
+    const int i = i0 + tid;
+    double w = i < n1 ? f.mass(key_logit(static_cast<uint32_t>(x[i] >> 32)), mx) : 0.0, all;
+    if (w < f.min_p) w = 0.0;
+    const double sum = done + block_scan(w, all, sh.scan);
+    if (i < n1) {
+      mass[i] = w;
+      upto[i] = sum;
     }
+    done += all;
   }
-  open = __syncthreads_or(open);
-  if (whole > 0.0 && (open || n >= sure)) return 0;         // the token behind the last kept has to be a candidate
+  __syncthreads();
+  double limit = f.top_p < 1.0 ? f.top_p * (whole > 0.0 ? whole : done) : 1e300, low = limit;
+  if (whole > 0.0) {
+    low *= 1.0 - kSumError;
+    limit *= 1.0 + kSumError;
+  }
+  int n = 0;
+  bool open = false;
+#pragma unroll 1
+  for (int i0 = 0; i0 < n1; i0 += kRowThreads) {
+    const int i = i0 + tid;
+    const bool some = i < n1 && mass[i] > 0.0;
+    const double before = some && i > 0 ? upto[i - 1] : -1.0;
+    open |= before >= low && before < limit;
+    n += __syncthreads_count(some && before < low);
+  }
+  if (whole > 0.0 && (__syncthreads_or(open) || n >= sure)) return 0;        // the token behind the last kept has to be a candidate
   return n;
 }
 
 // from the n first candidates, which are sorted, by index
-NRL_DEVICE void draw_of(uint64_t* x, int n, const RowFilter& f, float mx, double u, double total, SampleShared& sh, int* out_token, float* out_logp) {
+NRL_DEVICE void draw_of(uint64_t* x, int n, const double* mass, double total, double u, SampleShared& sh, int* out_token, float* out_logp) {
   const int tid = threadIdx.x;
-  __syncthreads();
-  for (int i = tid; i < n; i += kRowThreads) x[i] = x[i] << 32 | x[i] >> 32;        // (~index, key)
+  for (int i = tid; i < n; i += kRowThreads) x[i] = x[i] << 32 | static_cast<uint32_t>(i);        // (~index, place)
   sort_front(x, n);                                         // (its first barrier is behind the swap)
   if (tid == 0) sh.token = 0x7fffffff;
   const double target = u * total;
   double done = 0.0;
-  int last = 0;
 #pragma unroll 1
   for (int i0 = 0; i0 < n; i0 += kRowThreads) {
     const int i = i0 + tid;
-    const double w = i < n ? f.mass(key_logit(static_cast<uint32_t>(x[i])), mx) : 0.0;
+    const double w = i < n ? mass[static_cast<uint32_t>(x[i])] : 0.0;
     double all;
     const double upto = done + block_scan(w, all, sh.scan);
-    if (i < n && w > 0.0 && upto > target) atomicMin(&sh.token, i);
+    if (i < n && upto > target) atomicMin(&sh.token, i);
     done += all;
-    last = min(n, i0 + kRowThreads) - 1;
   }
   __syncthreads();
   if (tid == 0) {
-    const uint64_t y = x[min(sh.token, last)];
+    const uint64_t y = x[min(sh.token, n - 1)];
     *out_token = static_cast<int>(~static_cast<uint32_t>(y >> 32));
-    *out_logp = static_cast<float>(f.x(key_logit(static_cast<uint32_t>(y)), mx) - log(total));
+    *out_logp = logf(static_cast<float>(mass[static_cast<uint32_t>(y)] / total));        // one step of it, and 2^-24 of the quotient
   }
 }
 
@@ -570,7 +581,8 @@ template <typename T>
 __global__ void __launch_bounds__(kRowThreads, 3) sample_filtered_kernel(const T* __restrict__ logits, long row_stride, int V,
                                                                          const float* __restrict__ uniforms, SampleFilters filters, int* __restrict__ tokens,
                                                                          float* __restrict__ logp, float* __restrict__ top) {
-  extern __shared__ float s_chunk[];                       // [chunks][kRowThreads]
+  extern __shared__ __align__(16) float s_chunk[];         // [chunks][kRowThreads]
+  static_assert(kRowChunks * kRowThreads * 4 >= 2 * kCandidates * 8, "masses and sums of the candidates in their place");
   __shared__ SampleShared sh;
   const int rank = static_cast<int>(cluster_rank()), blocks = static_cast<int>(cluster_blocks()), tid = threadIdx.x, lane = tid & 31;
   const long r = blockIdx.x / blocks;
@@ -658,9 +670,10 @@ __global__ void __launch_bounds__(kRowThreads, 3) sample_filtered_kernel(const T
       sure = static_cast<int>(block_sum(static_cast<double>(n), sh.border.red));
     }
     sort_front(sh.list.cand, found);
-    double total;
-    const int n = kept_of(sh.list.cand, found, sure, f, mx, whole, sh, total);
-    if (n > 0) draw_of(sh.list.cand, n, f, mx, u, total, sh, tokens + r, logp + r);
+    double* mass = reinterpret_cast<double*>(s_chunk);     // the maxima are not needed any more
+    double* upto = mass + kCandidates;
+    const int n = kept_of(sh.list.cand, found, sure, f, mx, whole, mass, upto, sh);
+    if (n > 0) draw_of(sh.list.cand, n, mass, upto[n - 1], u, sh, tokens + r, logp + r);
     else open = mx;
   } else {
     open = mx;
@@ -682,7 +695,7 @@ cudaError_t launch_sample(const void* logits, long row_stride, int rows, int V, 
                           float* top, cudaStream_t s) {
   static PerDevice<bool> done, done_long;
   if (const cudaError_t e = allow_smem(done, sample_filtered_kernel<T>, kRowChunks * kRowThreads * 4); e != cudaSuccess) return e;
-  if (const cudaError_t e = allow_smem(done_long, sample_long_kernel<T>, kBins * kRowThreads * 4); e != cudaSuccess) return e;
+  if (const cudaError_t e = allow_smem(done_long, sample_long_kernel<T>, (kBins + 2) * kRowThreads * 4); e != cudaSuccess) return e;
   const int blocks = row_blocks(rows, V, LogitRow<T>::N);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -691,14 +704,14 @@ cudaError_t launch_sample(const void* logits, long row_stride, int rows, int V, 
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows) * blocks);
   cfg.blockDim = dim3(kRowThreads);
-  cfg.dynamicSmemBytes = row_chunks(V, LogitRow<T>::N, blocks) * kRowThreads * 4;
+  cfg.dynamicSmemBytes = kRowChunks * kRowThreads * 4;
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   const T* z = static_cast<const T*>(logits);
   const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_filtered_kernel<T>, z, row_stride, V, uniforms, f, tokens, logp, top);
   if (e != cudaSuccess || top == nullptr) return e;
-  cfg.dynamicSmemBytes = kBins * kRowThreads * 4;
+  cfg.dynamicSmemBytes = (kBins + 2) * kRowThreads * 4;
   return cudaLaunchKernelEx(&cfg, sample_long_kernel<T>, z, row_stride, V, uniforms, f, static_cast<const float*>(top), tokens, logp);
 }
 
