@@ -335,6 +335,14 @@ class Qwen2ForCausalLM(Qwen2PreTrained):
             return _ref.lmhead_logprob_top_p(hidden, self.lm_head.weight, targets, temperature, top_p)
         return ops.lmhead_logprob(hidden, self.lm_head.weight, targets, temperature, want_entropy)
 
+    def top_logprobs(self, hidden, k, temperature=1.0):
+        """(logp, idx) [rows, k] of the k most probable next tokens: what a teacher hands to a student."""
+        return ops.lmhead_top_logprobs(hidden, self.lm_head.weight, k, temperature)
+
+    def distill_loss(self, hidden, top_logp, top_idx, weights=None, temperature=1.0, beta=0.0, tail=True):
+        """(loss, token losses) against a teacher's ``top_logprobs``; ``ops.lmhead_distill_loss`` says of what."""
+        return ops.lmhead_distill_loss(hidden, self.lm_head.weight, top_logp, top_idx, weights, temperature, beta, tail)
+
     def forward(self, input_ids, cu_seqlens, position_ids, max_seqlen=None):
         return self.logits(self.hidden_states(input_ids, cu_seqlens, position_ids, max_seqlen))
 
@@ -471,3 +479,31 @@ def response_logprobs(lm, query_responses: torch.Tensor, context_length: int, pa
         out_v = out_v.index_put((row[vsel], col[vsel] + 1 - context_length), vals)
         result.append(out_v)
     return tuple(result)
+
+
+@torch.no_grad()
+def response_top_logprobs(lm, query_responses: torch.Tensor, context_length: int, pad_token_id: int, k: int, temperature: float = 1.0):
+    """A teacher's view of the response part: (logp [B, T_r, k], idx [B, T_r, k]), entry j of which are its k most probable tokens for position j of the response,
+    given everything before.  Slots that ``response_logprobs`` calls invalid have idx -1 and logp -inf."""
+    B, L = query_responses.shape
+    plan = build_logprob_plan(query_responses, context_length, pad_token_id)
+    hidden = lm.hidden_states(plan["ids"], plan["cu"], plan["pos"], plan["max_seqlen"])
+    logp, idx = lm.top_logprobs(hidden.index_select(0, plan["src"]), k, temperature)
+    out_lp = logp.new_full((B, L - context_length, k), -math.inf)
+    out_idx = idx.new_full((B, L - context_length, k), -1)
+    return out_lp.index_put((plan["r"], plan["c"]), logp), out_idx.index_put((plan["r"], plan["c"]), idx)
+
+
+def response_distill_loss(lm, query_responses: torch.Tensor, context_length: int, pad_token_id: int, top_logp: torch.Tensor, top_idx: torch.Tensor,
+                          weights: Optional[torch.Tensor] = None, temperature: float = 1.0, beta: float = 0.0, tail: bool = True):
+    """Divergence of ``lm`` from a teacher's ``response_top_logprobs`` over the response part: (sum of weights * token losses, token losses [B, T_r]).
+    ``weights`` [B, T_r]: share of every slot (None: the mean over the valid ones); invalid slots do not count whatever they say.  Only the loss has a gradient."""
+    B, L = query_responses.shape
+    T_r = L - context_length
+    if tuple(top_idx.shape[:2]) != (B, T_r) or (weights is not None and tuple(weights.shape) != (B, T_r)):
+        raise ValueError(f"response_distill_loss: the teacher's entries and the weights must be [{B}, {T_r}, ...], got {tuple(top_idx.shape)}")
+    plan = build_logprob_plan(query_responses, context_length, pad_token_id)
+    hidden = lm.hidden_states(plan["ids"], plan["cu"], plan["pos"], plan["max_seqlen"])
+    r, c = plan["r"], plan["c"]
+    loss, token = lm.distill_loss(hidden.index_select(0, plan["src"]), top_logp[r, c], top_idx[r, c], None if weights is None else weights[r, c], temperature, beta, tail)
+    return loss, token.new_zeros(B, T_r).index_put((r, c), token)

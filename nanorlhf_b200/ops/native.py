@@ -447,6 +447,15 @@ def sample_filtered(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p
     return ext().sample_filtered(_row_major(logits), uniforms.contiguous(), *args)
 
 
+def sample_tokens(logits, temperature, top_p, seed, row_ids, row_steps, top_k=0, min_p=0.0):
+    """A token per row for the rollout engines, a function of (seed, row id, tokens generated): ``sample``, or with ``top_k`` / ``min_p`` ``sample_filtered``
+    of one uniform number per row.  A row without a finite logit gives token 0."""
+    if temperature == 0.0 or (top_k <= 0 and min_p <= 0.0):
+        return sample(logits, temperature, top_p, seed, 0, row_ids, row_steps)
+    tokens, _ = sample_filtered(logits, row_uniforms(seed, 0, row_ids, row_steps), float(temperature), int(top_k), float(top_p), float(min_p))
+    return tokens.clamp_(min=0)
+
+
 def kv_cache_write(k, v, k_cache, v_cache, slot_mapping, src_index=None):
     _count()
     ext().kv_cache_write(k, v, k_cache, v_cache, slot_mapping, src_index)

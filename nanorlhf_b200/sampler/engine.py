@@ -9,7 +9,7 @@ and nothing touches the host or the filesystem.
 ``generate`` keeps the reference's call shape -- ``generate([n,] model, tokenizer, prompts,
 temperature, max_tokens)`` returning a right-padded ``LongTensor[len(prompts)*n, max_tokens]`` in
 prompt-major / sample-minor order -- but takes prompt *ids* (the reference round-trips ids ->
-strings -> ids) and exposes ``top_p`` / ``seed``.
+strings -> ids) and exposes ``top_p`` / ``top_k`` / ``min_p`` / ``seed`` (``ops.sample_filtered`` says what the filters keep).
 """
 from __future__ import annotations
 
@@ -84,7 +84,9 @@ def release_native_engine(model):
 
 def generate(n: int, model, tokenizer, prompts: Union[torch.Tensor, Sequence[Sequence[int]]], temperature: float,
              max_tokens: int, top_p: float = 0.95, seed: Optional[int] = None, backend: str = "auto",
-             eos_token_id: Optional[int] = None, rollout_dtype: str = "bf16", **engine_kw) -> torch.Tensor:
+             eos_token_id: Optional[int] = None, rollout_dtype: str = "bf16", top_k: int = 0, min_p: float = 0.0, **engine_kw) -> torch.Tensor:
+    if top_k < 0 or not 0.0 <= min_p <= 1.0:
+        raise ValueError(f"top_k must be 0 (off) or positive and min_p between 0 (off) and 1, got {top_k} and {min_p}")
     pad_id = tokenizer.pad_token_id
     eos_id = tokenizer.eos_token_id if eos_token_id is None else eos_token_id
     if isinstance(prompts, torch.Tensor):
@@ -95,8 +97,8 @@ def generate(n: int, model, tokenizer, prompts: Union[torch.Tensor, Sequence[Seq
     if which == "native":
         eng = get_native_engine(model, rollout_dtype=rollout_dtype, **engine_kw)
         eng.sync_weights()
-        return eng.generate(prompts, n, temperature, top_p, max_tokens, eos_id, pad_id, seed)
-    return torch_generate(model, prompts, n, temperature, top_p, max_tokens, eos_id, pad_id, seed)
+        return eng.generate(prompts, n, temperature, top_p, max_tokens, eos_id, pad_id, seed, top_k, min_p)
+    return torch_generate(model, prompts, n, temperature, top_p, max_tokens, eos_id, pad_id, seed, top_k=top_k, min_p=min_p)
 
 
 def vllm_generate(*args, **kwargs) -> torch.Tensor:

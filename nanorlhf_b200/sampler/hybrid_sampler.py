@@ -1154,7 +1154,7 @@ class HybridSampler:
     # ------------------------------------------------------------------------------------------
     @torch.no_grad()
     def generate(self, prompts: Sequence[Sequence[int]], n: int, temperature: float, top_p: float, max_tokens: int,
-                 eos_id: Optional[int], pad_id: int, seed: int) -> torch.Tensor:
+                 eos_id: Optional[int], pad_id: int, seed: int, top_k: int = 0, min_p: float = 0.0) -> torch.Tensor:
         dev = self.device
         total = len(prompts) * n
         out = torch.full((total, max_tokens), pad_id, dtype=torch.long)
@@ -1192,7 +1192,7 @@ class HybridSampler:
                 continue
             row_ids = torch.tensor([r - rid0 for r in sampled], dtype=torch.int32, device=dev)
             row_steps = torch.tensor([gen[r] for r in sampled], dtype=torch.int32, device=dev)
-            new = native.sample(logits, temperature, top_p, seed, 0, row_ids, row_steps).tolist()   # rows keep their padded stride
+            new = native.sample_tokens(logits, temperature, top_p, seed, row_ids, row_steps, top_k, min_p).tolist()   # rows keep their padded stride
             for rid, t in zip(sampled, new):
                 out[rid - rid0, gen[rid]] = t
                 gen[rid] += 1

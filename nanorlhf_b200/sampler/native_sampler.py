@@ -8,7 +8,7 @@
 * the decode step (28 layers x {fused add+RMSNorm, tcgen05 GEMM(+bias), RoPE, KV page write, paged
   decode attention, SwiGLU} + lm_head GEMM + top-p sampler + state update) is ONE CUDA graph per batch
   bucket; the host only looks at the ``finished`` flags every ``sync_every`` steps;
-* sampling semantics of the reference's ``vllm_generate``: temperature, top-p 0.95, n samples per
+* sampling semantics of the reference's ``vllm_generate``: temperature, top-p 0.95 (and, where asked for, min-p and top-k in front of it), n samples per
   prompt, seeded, stop at EOS (kept), right-pad with pad_id, prompt-major / sample-minor order
   (GRPO/grpo_trainer.py:122-166); temperature 0 = greedy (ReMax baseline / eval).
 """
@@ -60,6 +60,7 @@ class NativeSampler:
         self.use_cuda_graph = use_cuda_graph
         self.sharded_sync = None                        # parallel.weight_sync.ShardedWeightSync under fused data parallelism
         self.enable_compaction = True                   # drop finished rows at sync points (tests switch it off for A/B)
+        self._filters = (0, 0.0)                        # top_k, min_p of the generation under way
         self.layers: List[_LayerWeights] = []
         self._weights_version = None
         self.k_cache: List[torch.Tensor] = []
@@ -319,7 +320,7 @@ class NativeSampler:
         for li in range(cfg.num_hidden_layers):
             x, res = self._layer_decode(li, x, res, cos, sin, st)
         logits = self._final_logits(x, res)
-        tok = native.sample(logits, temperature, top_p, seed, 0, st["row_ids"], st["gen_count"])
+        tok = native.sample_tokens(logits, temperature, top_p, seed, st["row_ids"], st["gen_count"], *self._filters)
         fin = st["finished"]
         tok = torch.where(fin, torch.full_like(tok, pad_id), tok)
         col = st["gen_count"].clamp(max=max_tokens).long()
@@ -338,7 +339,7 @@ class NativeSampler:
         """Run up to ``steps`` decode iterations through a CUDA graph (one graph per batch bucket and
         sampling configuration)."""
         key = (st["S"], st["block_tables"].shape[1], float(temperature), float(top_p), int(seed), eos_id, pad_id,
-               max_tokens, st["splits"])
+               max_tokens, st["splits"], self._filters)
         if not self.use_cuda_graph:
             for _ in range(steps):
                 self._decode_step(st, temperature, top_p, seed, eos_id, pad_id, max_tokens)
@@ -376,8 +377,9 @@ class NativeSampler:
     # ------------------------------------------------------------------------------------------
     @torch.no_grad()
     def generate(self, prompts: Sequence[Sequence[int]], n: int, temperature: float, top_p: float, max_tokens: int,
-                 eos_id: Optional[int], pad_id: int, seed: int) -> torch.Tensor:
+                 eos_id: Optional[int], pad_id: int, seed: int, top_k: int = 0, min_p: float = 0.0) -> torch.Tensor:
         from .. import _C
+        self._filters = (int(top_k), float(min_p))
         dev, PAGE = self.device, self.PAGE
         was_training = self.lm.training
         self.lm.eval()
@@ -447,7 +449,7 @@ class NativeSampler:
                     cnt = len(groups) * n
                     rows = slice(r0, r0 + cnt)
                     lg = logits[rep]
-                    tok = native.sample(lg, temperature, top_p, seed, 0, st["row_ids"][rows], st["gen_count"][rows])
+                    tok = native.sample_tokens(lg, temperature, top_p, seed, st["row_ids"][rows], st["gen_count"][rows], *self._filters)
                     plen = torch.tensor([len(gid_to_prompt[g]) for g in groups], dtype=torch.int32, device=dev).repeat_interleave(n)
                     st["out"][rows, 0] = tok
                     st["tokens"][rows] = tok

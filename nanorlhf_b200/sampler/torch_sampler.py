@@ -27,7 +27,7 @@ def _unwrap(model):
 @torch.no_grad()
 def torch_generate(model, prompts: Sequence[Sequence[int]], n: int, temperature: float, top_p: float,
                    max_tokens: int, eos_token_id: Optional[int], pad_token_id: int, seed: int = 0,
-                   batch_size: int = 256) -> torch.Tensor:
+                   batch_size: int = 256, top_k: int = 0, min_p: float = 0.0) -> torch.Tensor:
     """Returns LongTensor [len(prompts)*n, max_tokens] (right-padded with ``pad_token_id``)."""
     lm = _unwrap(model)
     device = next(lm.parameters()).device
@@ -38,12 +38,12 @@ def torch_generate(model, prompts: Sequence[Sequence[int]], n: int, temperature:
     gen = torch.Generator(device=device).manual_seed(int(seed))
     for s in range(0, len(expanded), batch_size):
         out[s:s + batch_size] = _generate_batch(lm, expanded[s:s + batch_size], temperature, top_p, max_tokens,
-                                                eos_token_id, pad_token_id, gen, device)
+                                                eos_token_id, pad_token_id, gen, device, top_k, min_p)
     lm.train(was_training)
     return out
 
 
-def _generate_batch(lm, prompts, temperature, top_p, max_tokens, eos_id, pad_id, gen, device):
+def _generate_batch(lm, prompts, temperature, top_p, max_tokens, eos_id, pad_id, gen, device, top_k=0, min_p=0.0):
     cfg = lm.config
     B = len(prompts)
     Lp = max(len(p) for p in prompts)
@@ -94,7 +94,11 @@ def _generate_batch(lm, prompts, temperature, top_p, max_tokens, eos_id, pad_id,
     finished = torch.zeros(B, dtype=torch.bool, device=device)
     for t in range(max_tokens):
         logits = lm.lm_head(hidden).float()
-        nxt = ref.top_p_sample(logits, temperature, top_p, gen)
+        if temperature > 0.0 and (top_k > 0 or min_p > 0.0):
+            u = torch.rand(B, generator=gen, device=device)
+            nxt = ref.sample_filtered(logits, u, temperature, top_k, top_p, min_p)[0].long().clamp_min(0)
+        else:
+            nxt = ref.top_p_sample(logits, temperature, top_p, gen)
         nxt = torch.where(finished, torch.full_like(nxt, pad_id), nxt)
         out[:, t] = nxt
         if eos_id is not None:

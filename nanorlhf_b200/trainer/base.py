@@ -100,6 +100,8 @@ class RLTrainer:
         for m in (policy, ref_policy, value_model):
             if m is not None:
                 disable_dropout_in_model(m)
+        if args.logprob_top_p_consistent and (args.top_k > 0 or args.min_p > 0.0):
+            raise ValueError("logprob_top_p_consistent scores with the nucleus alone; it does not go with top_k or min_p")
         if args.logprob_top_p_consistent and args.top_p < 1.0:
             # experimental: policy and reference log-probs under the truncated softmax the sampler draws from
             for m in (policy, ref_policy):
@@ -212,7 +214,7 @@ class RLTrainer:
                                             a.temperature, a.response_length, top_p=a.top_p,
                                             seed=seed + self.comm.rank * 7919, backend=a.sampler,
                                             rollout_dtype=a.rollout_dtype, kv_block_size=a.kv_block_size,
-                                            kv_cache_dtype=a.kv_cache_dtype, **self._weight_sync_kw())
+                                            kv_cache_dtype=a.kv_cache_dtype, top_k=a.top_k, min_p=a.min_p, **self._weight_sync_kw())
         return {"responses": responses}
 
     def _weight_sync_kw(self) -> dict:

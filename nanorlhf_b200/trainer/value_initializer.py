@@ -67,7 +67,7 @@ def finetuned_value_model(value_model, policy, ref_policy, reward_func: Callable
     with torch.no_grad():
         responses = sampler_engine.generate(1, policy, tokenizer, queries, ppo_args.temperature, ppo_args.response_length,
                                             top_p=ppo_args.top_p, backend=ppo_args.sampler,
-                                            rollout_dtype=ppo_args.rollout_dtype)
+                                            rollout_dtype=ppo_args.rollout_dtype, top_k=ppo_args.top_k, min_p=ppo_args.min_p)
         q_str = [s.replace(tokenizer.pad_token, "") for s in tokenizer.batch_decode(queries)]
         r_str = tokenizer.batch_decode(responses)
         if getattr(reward_func, "accepts_ids", False):
