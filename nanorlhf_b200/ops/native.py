@@ -248,43 +248,26 @@ def top_logprobs(logits, k, temperature):
     return ext().top_logprobs(_row_major(logits), k, 1.0 / temperature)
 
 
-def _teacher(logits_columns, top_logp, top_idx, weights):
-    if top_idx.dtype != torch.int32:
-        top_idx = top_idx.clamp(-1, logits_columns).to(torch.int32)          # what is no token stays none
-    return top_logp.detach().float().contiguous(), top_idx.contiguous(), None if weights is None else weights.detach().float().contiguous()
+class _RecordedDistillFn(torch.autograd.Function):
+    """The loss in a form that a tracer records as one operation (see ``_RecordedLossFn``)."""
 
-
-def _scaled(grads, g, capture):
-    """``grads`` times the scalar ``g``; in place where this backward is the graph's only one, which frees them, and every replay of a captured one forms them again."""
-    keep = getattr(torch._C._autograd, "_get_current_graph_task_keep_graph", None)
-    if torch.is_grad_enabled() or keep is None or keep() or ext().capture_id() != capture or g.dtype != torch.float32:
-        return [None if x is None else x * g.to(x.dtype) if x.dtype == g.dtype else (x.float() * g).to(x.dtype) for x in grads]
-    for x in grads:
-        if x is not None:
-            _count()
-            ext().scale_(x, g)
-    return grads
-
-
-class _DistillFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, top_logp, top_idx, weights, temperature, beta, tail, need):
-        _count(2)
-        loss, token, grad = ext().distill_loss(logits, top_logp, top_idx, weights, 1.0 / temperature, beta, tail, need, False, True)
+    def forward(ctx, logits, top_logp, top_idx, weights, inv_temp, beta, tail):
+        loss, token, grad = ext().distill_loss_parts(logits, top_logp, top_idx, weights, inv_temp, beta, tail, True, False, True)
         ctx.save_for_backward(grad)
-        ctx.capture = ext().capture_id()
         ctx.mark_non_differentiable(token)
         return loss, token
 
     @staticmethod
     def backward(ctx, g_loss, _g_token):
-        return (_scaled(ctx.saved_tensors, g_loss, ctx.capture)[0],) + (None,) * 7
+        return (ctx.saved_tensors[0] * g_loss,) + (None,) * 6
 
 
 def distill_loss(logits, top_logp, top_idx, weights, temperature, beta, tail):
-    top_logp, top_idx, weights = _teacher(logits.shape[1], top_logp, top_idx, weights)
-    need = torch.is_grad_enabled() and logits.requires_grad
-    return _DistillFn.apply(_row_major(logits), top_logp, top_idx, weights, temperature, beta, tail, need)
+    _count(3 if logits.requires_grad and torch.is_grad_enabled() else 2)          # the rows, their sum and, later, a factor of the gradient
+    if torch._C._get_tracing_state():
+        return _RecordedDistillFn.apply(_row_major(logits), *ext().teacher_entries(top_logp, top_idx, weights, logits.shape[1]), 1.0 / temperature, beta, tail)
+    return ext().distill_loss(logits, top_logp, top_idx, weights, 1.0 / temperature, beta, tail)
 
 
 LOGITS_BYTES = 4 << 30      # float logits of a head that are held at a time
@@ -316,7 +299,8 @@ class _LmHeadDistillFn(torch.autograd.Function):
             z = torch.empty(e - s, V, dtype=torch.float32, device=h.device)
             _lin.gemm(h[s:e], weight, out_f32=z)
             _count()
-            _, token, dz = ext().distill_loss(z, top_logp[s:e], top_idx[s:e], weights[s:e], 1.0 / temperature, beta, tail, need_h or need_w, True, False)
+            _, token, dz = ext().distill_loss_parts(z, top_logp[s:e], top_idx[s:e], weights[s:e], 1.0 / temperature, beta, tail,
+                                                        need_h or need_w, True, False)
             tokens.append(token)
             del z
             if need_h:
@@ -335,14 +319,16 @@ class _LmHeadDistillFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g_loss, _g_token):
-        return tuple(_scaled(ctx.saved_tensors, g_loss, ctx.capture)) + (None,) * 8
+        dh, dw = ctx.saved_tensors
+        _count((dh is not None) + (dw is not None))
+        return tuple(None if x is None else ext().scaled(x, g_loss, ctx.capture) for x in (dh, dw)) + (None,) * 8
 
 
 def lmhead_distill_loss(hidden, weight, top_logp, top_idx, weights, temperature, beta, tail):
     from . import gemm as _lin
     if not _lin.supported(hidden, weight):                 # other types and sizes than the GEMM's: their logits, in float32
         return distill_loss(F.linear(hidden.float(), weight.float()), top_logp, top_idx, weights, temperature, beta, tail)
-    top_logp, top_idx, weights = _teacher(weight.shape[0], top_logp, top_idx, weights)
+    top_logp, top_idx, weights = ext().teacher_entries(top_logp, top_idx, weights, weight.shape[0])
     grad = torch.is_grad_enabled()
     return _LmHeadDistillFn.apply(hidden, weight, top_logp, top_idx, weights, temperature, beta, tail, grad and hidden.requires_grad,
                                   grad and weight.requires_grad)
