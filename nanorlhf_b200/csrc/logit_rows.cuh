@@ -466,7 +466,7 @@ NRL_DEVICE uint32_t group_bound(const uint32_t (&keys)[kGroupsMax], int groups, 
 // What a block has gathered of its share.
 constexpr int kCandidates = 2048;
 struct RowList {
-  uint64_t cand[kCandidates];                          // (key, ~index): unsigned numbers in the order; those that other blocks send from the end on
+  __align__(16) uint64_t cand[kCandidates];            // (key, ~index): unsigned numbers in the order; those that other blocks send from the end on
   unsigned short hits[kCandidates];
   int n, nhits, sent;
 };
@@ -555,9 +555,43 @@ NRL_DEVICE void sort_block(uint64_t* x, int size) {
     }
   __syncthreads();
 }
-// x[0 .. n) in descending order; entries behind them up to the next power of 2 from 64 on are overwritten by 0
+// How many of the different numbers x[0 .. n) are above this thread's one or two, `mine`; x lies on 16 bytes and x[n] .. x[n + 7] are 0
+template <int M>
+NRL_DEVICE void count_above(const uint64_t* x, int n, const uint64_t (&mine)[M], int (&above)[M]) {
+#pragma unroll
+  for (int m = 0; m < M; ++m) above[m] = 0;
+#pragma unroll 1
+  for (int j = 0; j < n; j += 8) {
+    ulonglong2 y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = *reinterpret_cast<const ulonglong2*>(x + j + 2 * i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int m = 0; m < M; ++m) above[m] += (y[i].x > mine[m] ? 1 : 0) + (y[i].y > mine[m] ? 1 : 0);
+  }
+}
+template <int M>
+NRL_DEVICE void sort_counting(uint64_t* x, int n) {
+  uint64_t mine[M];
+  int place[M];
+#pragma unroll
+  for (int m = 0; m < M; ++m) mine[m] = x[min(static_cast<int>(threadIdx.x) + m * kRowThreads, n)];
+  if (static_cast<int>(threadIdx.x) < n) count_above(x, n, mine, place);
+  __syncthreads();
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+    if (static_cast<int>(threadIdx.x) + m * kRowThreads < n) x[place[m]] = mine[m];
+  __syncthreads();
+}
+// x[0 .. n) in descending order, all different; x has room for eight more, and entries behind them up to the next power of 2 may be overwritten.  Up to two a thread, every
+// thread counts where its own belong: 75 numbers 700 cycles, by exchanges 7000.
 NRL_DEVICE void sort_front(uint64_t* x, int n) {
-  int size = 64;
+  if (threadIdx.x < 8 && n <= 2 * kRowThreads) x[n + threadIdx.x] = 0;
+  __syncthreads();
+  if (n <= kRowThreads) return sort_counting<1>(x, n);
+  if (n <= 2 * kRowThreads) return sort_counting<2>(x, n);
+  int size = 2 * kRowThreads;
   while (size < n) size *= 2;
   for (int i = n + threadIdx.x; i < size; i += kRowThreads) x[i] = 0;
   __syncthreads();
@@ -569,16 +603,13 @@ template <class F>
 NRL_DEVICE void in_order(uint64_t* x, int found, int n, F&& f) {
   const int tid = threadIdx.x;
   if (found <= kRowThreads) {
-    uint64_t mine = 0;
-    int before = n;
-    if (tid < found) {
-      mine = x[tid];
-      before = 0;
-#pragma unroll 4
-      for (int j = 0; j < found; ++j) before += x[j] > mine ? 1 : 0;
-    }
+    if (tid < 8) x[found + tid] = 0;
     __syncthreads();
-    if (before < n) f(before, mine);
+    const uint64_t mine[1] = {x[min(tid, found)]};
+    int before[1] = {n};
+    if (tid < found) count_above(x, found, mine, before);
+    __syncthreads();
+    if (before[0] < n) f(before[0], mine[0]);
     return;
   }
   sort_front(x, found);

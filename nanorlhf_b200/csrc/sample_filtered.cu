@@ -77,14 +77,15 @@ NRL_DEVICE double block_scan(double v, double& all, double* red) {
   __syncthreads();
   if (lane == 31) red[warp] = v;
   __syncthreads();
-  double before = 0.0;
-  all = 0.0;
-#pragma unroll 1
-  for (int w = 0; w < kRowWarps; ++w) {
-    if (w == warp) before = all;
-    all += red[w];
+  double w = red[lane % kRowWarps];                        // every warp adds up the warps' sums, in one order
+#pragma unroll
+  for (int o = 1; o < kRowWarps; o <<= 1) {
+    const double y = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane % kRowWarps >= o) w += y;
   }
-  return before + v;
+  all = __shfl_sync(0xffffffffu, w, kRowWarps - 1);
+  const double before = __shfl_sync(0xffffffffu, w, warp - 1);
+  return warp > 0 ? before + v : v;
 }
 
 // By the border alone: found by ranges of keys, all in double, then the kept mass of every warp's range and a walk through the range that holds the drawn one.
@@ -712,6 +713,7 @@ cudaError_t launch_sample(const void* logits, long row_stride, int rows, int V, 
   const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_filtered_kernel<T>, z, row_stride, V, uniforms, f, tokens, logp, top);
   if (e != cudaSuccess || top == nullptr) return e;
   cfg.dynamicSmemBytes = (kBins + 2) * kRowThreads * 4;
+  if (getenv("NRL_C")) { attr[0].val.clusterDim.x = atoi(getenv("NRL_C")); cfg.gridDim = dim3(rows * atoi(getenv("NRL_C"))); }
   return cudaLaunchKernelEx(&cfg, sample_long_kernel<T>, z, row_stride, V, uniforms, f, static_cast<const float*>(top), tokens, logp);
 }
 
