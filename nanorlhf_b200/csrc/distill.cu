@@ -12,6 +12,7 @@
 // bit map in shared memory knows: taken as 1 - sum q_k it would have no digits left where the student is sure.  r below 2^-24, which float32 log-probabilities
 // cannot tell from 0, counts as 0, and as 2^-24 under a logarithm.
 // An entry whose index is not a token (-1) is skipped; entries of one token add up.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.cuh"
@@ -51,6 +52,7 @@ struct DistillShared {
   double q[kTopMax];                                       // beta > 0: D of the token's event
   float2 part[kRowClusterMax][kRowWarps];                  // maximum and sum of every warp of the cluster
   double red[2][kRowWarps];
+  int twins;                                               // some token has several entries
 };
 
 NRL_DEVICE void block_sum_two(double& x, double& y, double (&red)[2][kRowWarps]) {
@@ -81,7 +83,19 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
   const long r = blockIdx.x / blocks, rows = gridDim.x / blocks;
   const LogitRow<T> row(logits + r * row_stride, V);
   const RowShare share(row.nvec, rank, blocks);
+  // the row's own numbers on their way together
+  static_assert(kTopMax == 2 * kRowThreads, "two entries a thread at most");
+  int at[2];
+  float a_mine[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int i = tid + t * kRowThreads;
+    at[t] = i < K ? top_idx[r * K + i] : -1;
+    a_mine[t] = i < K ? top_logp[r * K + i] : 0.f;
+  }
   const float weight = weights ? weights[r] : 1.f;
+  const int map_words = ((share.end - share.first) * N / 32 + 4) / 4 * 4;
+  for (int i = tid * 4; i < map_words; i += kRowThreads * 4) *reinterpret_cast<uint4*>(s_map + i) = make_uint4(0, 0, 0, 0);
   G* out = grad ? grad + r * V : nullptr;
   if (weight == 0.f) {                                     // the row is not read
     if (tid == 0 && rank == 0) token_loss[r] = 0.f;
@@ -92,31 +106,19 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
   }
   if (blocks > 1) cluster_arrive();                        // shared memory may be written by the others once it is known to run
   // ---- the teacher's entries, and where they lie in the share ----
-  for (int i = tid; i < (share.end - share.first) * N / 32 + 1; i += kRowThreads) s_map[i] = 0;
+  if (tid == 0) sh.twins = 0;
   __syncthreads();
-  static_assert(kTopMax == 2 * kRowThreads, "two entries a thread at most");
-  float a_mine[2];
-  T z_mine[2];
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const int i = tid + t * kRowThreads;
-    if (i < (K + 3) / 4 * 4) {
-      const int e = i < K ? top_idx[r * K + i] : -1, at = e >= 0 && e < V ? e : -1, bit = at + row.skew - share.first * N;
-      sh.idx[i] = at;
-      if (i < K) a_mine[t] = top_logp[r * K + i];
-      z_mine[t] = row.p[max(at, 0)];
-      if (at >= 0 && bit >= 0 && bit < (share.end - share.first) * N) atomicOr(&s_map[bit >> 5], 1u << (bit & 31));
-    }
+    if (i >= (K + 3) / 4 * 4) continue;
+    if (at[t] < 0 || at[t] >= V) at[t] = -1;
+    const int bit = at[t] + row.skew - share.first * N;
+    sh.idx[i] = at[t];
+    sh.a[i] = a_mine[t];
+    if (at[t] >= 0 && bit >= 0 && bit < (share.end - share.first) * N) atomicOr(&s_map[bit >> 5], 1u << (bit & 31));
   }
-  __syncthreads();                                         // the map is whole; the entries' logits may still be on their way
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int i = tid + t * kRowThreads;
-    if (i < K) {
-      sh.a[i] = a_mine[t];
-      sh.z[i] = LogitRow<T>::value(z_mine[t]);
-    }
-  }
+  __syncthreads();
 
   // ---- the row's maximum, and its mass off the teacher's tokens ----
   const float c = static_cast<float>(inv_temp * 1.4426950408889634);
@@ -148,6 +150,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
   if (blocks > 1) cluster_arrive();
   for (int i = tid; i < K; i += kRowThreads) {             // probabilities of the teacher's tokens, while the other blocks come
     const int at = sh.idx[i];
+    const T z = row.p[max(at, 0)];
     double p = -1.0;
     if (at >= 0) {
       int same = 0;
@@ -156,11 +159,14 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
         same += (x.x == at) + (x.y == at) + (x.z == at) + (x.w == at);
       }
       p = exp(static_cast<double>(sh.a[i]));
-      if (same > 1)
+      if (same > 1) {
+        sh.twins = 1;
         for (int j = 0; j < K; ++j)
           if (sh.idx[j] == at && j != i) p = j < i || p < 0.0 ? -1.0 : p + exp(static_cast<double>(sh.a[j]));
+      }
     }
     sh.p[i] = p;
+    sh.z[i] = LogitRow<T>::value(z);
   }
   __syncwarp();
   if (blocks > 1) cluster_wait();
@@ -257,7 +263,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
       const double p = sh.p[i];
       const int bit = sh.idx[i] + row.skew - share.first * N;
       if (p < 0.0 || bit < 0 || bit >= (share.end - share.first) * N) continue;
-      const double q = exp((static_cast<double>(sh.z[i]) - mx) * inv_temp) / total;
+      const double q = ex2((sh.z[i] - mx) * c) / total;
       const double u = !teacher ? 0.0 : beta == 0.0 ? q - (tail ? p : p / psum) : q > 0.0 ? q * (sh.q[i] - mean) : 0.0;
       out[sh.idx[i]] = static_cast<G>(static_cast<float>(g * u));
     }
@@ -271,7 +277,8 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
     if (p < 0.0) continue;
     const double x = (static_cast<double>(sh.z[i]) - mx) * inv_temp;
     mass_top += exp(x);
-    if (p > 0.0) loss += p * (log(p) - x);
+    const double a = sh.a[i];                              // log p, unless other entries have the token too
+    if (p > 0.0) loss += p * ((sh.twins ? log(p) : a) - x);
   }
   block_sum_two(mass_top, loss, sh.red);
   if (tid < 32) {                                          // three logarithms in one
@@ -314,10 +321,12 @@ cudaError_t launch_distill(const void* logits, long row_stride, int rows, int V,
                            double inv_temp, double beta, int tail, float* token_loss, void* grad, cudaStream_t s) {
   static PerDevice<bool> done;
   constexpr int N = LogitRow<T>::N;
-  // Rows that the second pass would not find in L2 any more (three blocks on 148 SMs hold 444 rows, and 126 MB is what L2 has) get four blocks, which is a
-  // quarter of them at a time: 2048 x 151 936 floats 580 / 559 / 535 us with 1 / 2 / 4, bf16 307 / 307 / 405, 1500 x 50 021 floats 150 / 157 / 211.
+  // The second pass should find its rows in L2, which has 126 MB; three blocks on each of 148 SMs hold 444 rows at a time, or half or a quarter of them with two or four
+  // blocks a row.  us with 1 / 2 / 4 of 2048 x 151 936 floats 574 / 544 / 522, bf16 298 / 293 / 383 (DRAM reads 1.47 / 1.07 / 1.00 of the logits), of 1500 x 50 021 floats
+  // 148 / 155 / 211, of 2048 x 32 000 bf16 83 / 123 / 210.
   int blocks = row_blocks(rows, V, N);
-  if (grad != nullptr && V * sizeof(T) > 400 * 1024 && blocks < 4) blocks = 4;
+  const long held = std::min(rows, 444) * static_cast<long>(V) * sizeof(T);
+  if (grad != nullptr) blocks = std::max(blocks, held > 200L << 20 ? 4 : held > 100L << 20 ? 2 : 1);
   const int vecs = ((V + 2 * N - 2) / N + blocks - 1) / blocks;
   if (const cudaError_t e = allow_smem(done, distill_kernel<T, G>, kDistillVocabMax / 8 + 128); e != cudaSuccess) return e;
   cudaLaunchAttribute attr[1];
@@ -327,7 +336,7 @@ cudaError_t launch_distill(const void* logits, long row_stride, int rows, int V,
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows) * blocks);
   cfg.blockDim = dim3(kRowThreads);
-  cfg.dynamicSmemBytes = (vecs * N / 32 + 1) * 4;
+  cfg.dynamicSmemBytes = (vecs * N / 32 + 4) / 4 * 16;
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;

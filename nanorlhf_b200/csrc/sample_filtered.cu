@@ -713,7 +713,6 @@ cudaError_t launch_sample(const void* logits, long row_stride, int rows, int V, 
   const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_filtered_kernel<T>, z, row_stride, V, uniforms, f, tokens, logp, top);
   if (e != cudaSuccess || top == nullptr) return e;
   cfg.dynamicSmemBytes = (kBins + 2) * kRowThreads * 4;
-  if (getenv("NRL_C")) { attr[0].val.clusterDim.x = atoi(getenv("NRL_C")); cfg.gridDim = dim3(rows * atoi(getenv("NRL_C"))); }
   return cudaLaunchKernelEx(&cfg, sample_long_kernel<T>, z, row_stride, V, uniforms, f, static_cast<const float*>(top), tokens, logp);
 }
 
