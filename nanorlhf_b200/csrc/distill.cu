@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
   __syncthreads();
 
   // ---- the row's maximum, and its mass off the teacher's tokens ----
-  const float c = static_cast<float>(inv_temp * 1.4426950408889634);
+  const float c = log2_scale(inv_temp);
   const auto* map = reinterpret_cast<const std::conditional_t<N == 16, uint16_t, uint8_t>*>(s_map);
   float best, m, mass;
   row_pass(row, share, c, static_cast<float*>(nullptr), best, m, mass, [&](int v, RawVec& a) {

@@ -48,6 +48,9 @@ NRL_DEVICE float ex2(float x) {
   return r;
 }
 
+// logits to exponents of 2; finite, so that 0 times it is 0 at any temperature
+NRL_DEVICE float log2_scale(double inv_temp) { return static_cast<float>(fmin(inv_temp * 1.4426950408889634, 3e38)); }
+
 template <typename T>
 struct LogitRow {
   static constexpr int N = 32 / sizeof(T);             // elements of a 32-byte vector

@@ -225,7 +225,7 @@ NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx
   constexpr int N = LogitRow<T>::N;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const RowShare share(row.nvec, rank, blocks);
-  const float c = static_cast<float>(f.inv_temp * 1.4426950408889634);
+  const float c = log2_scale(f.inv_temp);
   if (tid < 128) sh.powers[tid] = exp2(tid / 128.0);
   const RowMass mass(f, mx, sh.powers);
   if (tid == 0) sh.list.n = sh.list.nhits = sh.list.sent = 0;
@@ -594,7 +594,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) sample_filtered_kernel(const T
   const RowShare share(row.nvec, rank, blocks);
   const bool few = (f.top_k > 0 && f.top_k <= kTopMax) || f.min_p > 0.0;        // what is kept is a matter of the candidates alone
   const bool nucleus = !few && f.top_p < 1.0 && f.top_k == 0;
-  const float c = static_cast<float>(f.inv_temp * 1.4426950408889634);
+  const float c = log2_scale(f.inv_temp);
   float best, m = 0.f, s = 0.f;
   if (nucleus)
     row_pass<true>(row, share, c, s_chunk, best, m, s, [](int, RawVec& a) { LogitRow<T>::drop_nan(a); });

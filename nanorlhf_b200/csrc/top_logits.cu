@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) top_logprobs_kernel(const T* _
   if (blocks > 1) cluster_arrive();                      // the first block's memory may be written once it is known to run
   const LogitRow<T> row(logits + r * row_stride, V);
   const RowShare share(row.nvec, rank, blocks);
-  const float c = static_cast<float>(inv_temp * 1.4426950408889634);
+  const float c = log2_scale(inv_temp);
   float best, m, s;
   row_pass(row, share, c, s_chunk, best, m, s, [](int, const RawVec&) {});
   // a thread's chunks in one group up to k = 256, in up to four above

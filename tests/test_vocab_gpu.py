@@ -129,6 +129,20 @@ def test_sampling_with_filters_of_every_row(B, V, dtype):
     _same_draws(z, u, temperature=t, top_k=k, top_p=p, min_p=m)
 
 
+@pytest.mark.parametrize("temperature", [1e-300, 1e-42, 1e-30, 1e30])
+@pytest.mark.parametrize("pattern", ["normal", "ties"])
+def test_temperatures_far_from_one(pattern, temperature):
+    z = _logits(pattern, 4, 30000, F32)
+    u = torch.rand(4, generator=_gen(3), device=DEV)
+    for kw in (dict(), dict(top_p=0.9), dict(top_k=40), dict(top_k=40, top_p=0.3), dict(min_p=0.5)):
+        _same_draws(z, u, temperature=temperature, **kw)
+    if temperature >= 1e-42:
+        _same_draws(z, u, temperature=torch.full((4,), temperature, device=DEV), top_p=torch.full((4,), 0.7, device=DEV))
+    logp, idx = ops.top_logprobs(z, 9, temperature)
+    want, at = ref.top_logprobs(z, 9, temperature)
+    assert torch.equal(idx, at) and ((logp == want) | ((logp - want).abs() <= 5e-6 + 2.0 ** -23 * want.abs())).all()
+
+
 def test_sampling_edges():
     z = torch.tensor([[1.0, 3.0, 3.0, math.nan], [-INF, math.nan, -INF, -INF], [INF, 0.0, INF, 1.0], [-2.0, -2.0, -INF, -2.0]], device=DEV)
     for u in ([0.999, 0.5, 0.6, 0.34], [0.0, 0.0, 0.0, 0.0], [0.2, 0.2, 0.2, 0.67]):
