@@ -331,12 +331,6 @@ struct RowShare {
     chunks = len > 0 ? (steps + len - 1) / len : 0;
   }
 };
-// chunks of any block of the cluster at most, wherever the row starts (host)
-inline int row_chunks(int V, int vec, int blocks) {
-  const long nvec = (static_cast<long>(V) + 2 * vec - 2) / vec, per = (nvec + blocks - 1) / blocks, steps = (per + kRowThreads - 1) / kRowThreads;
-  return steps < kRowChunks * kRowUnroll ? static_cast<int>((steps + kRowUnroll - 1) / kRowUnroll) : kRowChunks;
-}
-
 // Blocks of a row's cluster (host).  A row of its own block is fastest where the rows fill the SMs; of few rows the cluster shares the reading, until its barriers
 // cost more.  us with 1 / 2 / 4 / 8 blocks (top 20 to 64 of bf16 rows of 151 936): 1 row 15.8 / 11.9 / 10.1 / 10.1, 8 rows 20.8 / 14.7 / 12.0 / 11.2, 32 rows 23.3 / 17.2 /
 // 15.6 / 28.4, 100 rows 23.3 / 20.5 / 25.9 / 51, 300 rows 36.6 / 42.6 / 62 / 118; 64 rows of 32 000 10.1 / 10.3 / 16.3 / 34, of 4000 floats 6.6 / 7.7 / 10.0 / 18.7.
@@ -468,9 +462,17 @@ NRL_DEVICE uint32_t group_bound(const uint32_t (&keys)[kGroupsMax], int groups, 
 
 // What a block has gathered of its share.
 constexpr int kCandidates = 2048;
+struct SortCounts {
+  int start[kRowThreads + 1], next[kRowThreads];           // of 512 buckets
+  uint32_t lo[kRowWarps], hi[kRowWarps];
+  int sums[kRowWarps];
+};
 struct RowList {
   __align__(16) uint64_t cand[kCandidates];            // (key, ~index): unsigned numbers in the order; those that other blocks send from the end on
-  unsigned short hits[kCandidates];
+  union {
+    unsigned short hits[kCandidates];
+    SortCounts counts;                                 // (when the hits are not needed any more)
+  };
   int n, nhits, sent;
 };
 // Into `list` all elements of the share whose keys reach `bound`: the chunks that have any (by their maxima) are read again, a vector a thread.  list.n and
@@ -541,81 +543,96 @@ NRL_DEVICE int join_candidates(RowList& list) {
   return all;
 }
 
-// `size` (a power of 2 from 64 on) numbers in descending order.  A warp has 64 neighbours to itself, so that steps up to a distance of 32 need no barrier.
-NRL_DEVICE void sort_block(uint64_t* x, int size) {
-  const int tid = threadIdx.x;
-#pragma unroll 1
-  for (int w = 2; w <= size; w *= 2)
-#pragma unroll 1
-    for (int d = w / 2; d > 0; d /= 2) {
-      if (d >= 32) __syncthreads();
-      else __syncwarp();
-      for (int t = tid; t < size / 2; t += kRowThreads) {
-        const int i = 2 * t - (t & (d - 1)), j = i + d;
-        const uint64_t a = x[i], c = x[j];
-        if ((a < c) == ((i & w) == 0)) { x[i] = c; x[j] = a; }
-      }
-    }
-  __syncthreads();
-}
-// How many of the different numbers x[0 .. n) are above this thread's one or two, `mine`; x lies on 16 bytes and x[n] .. x[n + 7] are 0
-template <int M>
-NRL_DEVICE void count_above(const uint64_t* x, int n, const uint64_t (&mine)[M], int (&above)[M]) {
-#pragma unroll
-  for (int m = 0; m < M; ++m) above[m] = 0;
+// How many of the different numbers x[0 .. n) are above `mine`; x lies on 16 bytes and x[n] .. x[n + 7] are 0
+NRL_DEVICE int count_above(const uint64_t* x, int n, uint64_t mine) {
+  int above = 0;
 #pragma unroll 1
   for (int j = 0; j < n; j += 8) {
     ulonglong2 y[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] = *reinterpret_cast<const ulonglong2*>(x + j + 2 * i);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int m = 0; m < M; ++m) above[m] += (y[i].x > mine[m] ? 1 : 0) + (y[i].y > mine[m] ? 1 : 0);
+    for (int i = 0; i < 4; ++i) above += (y[i].x > mine ? 1 : 0) + (y[i].y > mine ? 1 : 0);
   }
+  return above;
 }
-template <int M>
-NRL_DEVICE void sort_counting(uint64_t* x, int n) {
-  uint64_t mine[M];
-  int place[M];
+// x[0 .. n) in descending order, n <= kCandidates, all different (the 32 high bits need not be); the eight entries behind them may be overwritten; y: room for as many.  Up to one a thread, every
+// thread counts where its own belongs: 75 numbers 700 cycles, by exchanges 7000.  More go to 512 buckets by equal ranges of their high bits first, and are counted
+// within theirs: 1358 numbers of five logits 25 000 cycles, by exchanges 30 000, and 6000 where few are of one logit.
+NRL_DEVICE void sort_front(uint64_t* x, int n, uint64_t* y, SortCounts& sc) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (n <= kRowThreads) {
+    if (tid < 8) x[n + tid] = 0;
+    __syncthreads();
+    const uint64_t mine = x[min(tid, n)];
+    const int place = tid < n ? count_above(x, n, mine) : 0;
+    __syncthreads();
+    if (tid < n) x[place] = mine;
+    __syncthreads();
+    return;
+  }
+  __syncthreads();
+  uint32_t lo = 0xffffffffu, hi = 0;
+  for (int i = tid; i < n; i += kRowThreads) {
+    lo = min(lo, static_cast<uint32_t>(x[i] >> 32));
+    hi = max(hi, static_cast<uint32_t>(x[i] >> 32));
+  }
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  if (lane == 0) {
+    sc.lo[warp] = lo;
+    sc.hi[warp] = hi;
+  }
+  sc.start[tid] = 0;
+  __syncthreads();
+  lo = __reduce_min_sync(0xffffffffu, sc.lo[lane % kRowWarps]);
+  hi = __reduce_max_sync(0xffffffffu, sc.hi[lane % kRowWarps]);
+  const int shift = max(0, 23 - __clz(hi - lo));           // 512 ranges at most, the highest numbers first
+  static_assert(kRowThreads == 512, "a bucket a thread");
+  auto bucket = [&](uint64_t v) { return static_cast<int>((hi - static_cast<uint32_t>(v >> 32)) >> shift); };
+  for (int i = tid; i < n; i += kRowThreads) atomicAdd(&sc.start[bucket(x[i])], 1);
+  __syncthreads();
+  const int count = sc.start[tid];
+  int incl = count;
 #pragma unroll
-  for (int m = 0; m < M; ++m) mine[m] = x[min(static_cast<int>(threadIdx.x) + m * kRowThreads, n)];
-  if (static_cast<int>(threadIdx.x) < n) count_above(x, n, mine, place);
+  for (int o = 1; o < 32; o <<= 1) {
+    const int z = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += z;
+  }
+  if (lane == 31) sc.sums[warp] = incl;
   __syncthreads();
-#pragma unroll
-  for (int m = 0; m < M; ++m)
-    if (static_cast<int>(threadIdx.x) + m * kRowThreads < n) x[place[m]] = mine[m];
+  int before = incl - count;
+  for (int w = 0; w < warp; ++w) before += sc.sums[w];
+  sc.start[tid] = sc.next[tid] = before;
+  if (tid == 0) sc.start[kRowThreads] = n;
   __syncthreads();
-}
-// x[0 .. n) in descending order, all different; x has room for eight more, and entries behind them up to the next power of 2 may be overwritten.  Up to two a thread, every
-// thread counts where its own belong: 75 numbers 700 cycles, by exchanges 7000.
-NRL_DEVICE void sort_front(uint64_t* x, int n) {
-  if (threadIdx.x < 8 && n <= 2 * kRowThreads) x[n + threadIdx.x] = 0;
+  for (int i = tid; i < n; i += kRowThreads) y[atomicAdd(&sc.next[bucket(x[i])], 1)] = x[i];
   __syncthreads();
-  if (n <= kRowThreads) return sort_counting<1>(x, n);
-  if (n <= 2 * kRowThreads) return sort_counting<2>(x, n);
-  int size = 2 * kRowThreads;
-  while (size < n) size *= 2;
-  for (int i = n + threadIdx.x; i < size; i += kRowThreads) x[i] = 0;
+  for (int i = tid; i < n; i += kRowThreads) {
+    const uint64_t mine = y[i];
+    const int b = bucket(mine), end = sc.start[b + 1];
+    int place = sc.start[b];
+#pragma unroll 4
+    for (int j = sc.start[b]; j < end; ++j) place += y[j] > mine ? 1 : 0;
+    x[place] = mine;
+  }
   __syncthreads();
-  sort_block(x, size);
 }
 
-// Candidates in their order: f(place, candidate) for the first n of them, behind a barrier.  Up to one a thread each counts those before it; more are sorted.
+// Candidates in their order: f(place, candidate) for the first n of them, behind a barrier.
 template <class F>
-NRL_DEVICE void in_order(uint64_t* x, int found, int n, F&& f) {
+NRL_DEVICE void in_order(uint64_t* x, int found, int n, uint64_t* y, SortCounts& sc, F&& f) {
   const int tid = threadIdx.x;
   if (found <= kRowThreads) {
     if (tid < 8) x[found + tid] = 0;
     __syncthreads();
-    const uint64_t mine[1] = {x[min(tid, found)]};
-    int before[1] = {n};
-    if (tid < found) count_above(x, found, mine, before);
+    const uint64_t mine = x[min(tid, found)];
+    const int before = tid < found ? count_above(x, found, mine) : n;
     __syncthreads();
-    if (before[0] < n) f(before[0], mine[0]);
+    if (before < n) f(before, mine);
     return;
   }
-  sort_front(x, found);
+  sort_front(x, found, y, sc);
   for (int i = tid; i < n; i += kRowThreads) f(i, x[i]);
 }
 

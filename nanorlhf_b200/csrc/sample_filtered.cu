@@ -10,6 +10,8 @@
 // leaves the nucleus' last token open, or the candidates do not reach it, the row is left to a second kernel, as are rows without filters.
 #include <curand_kernel.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "logit_rows.cuh"
 #include "per_device.h"
@@ -382,10 +384,10 @@ NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx
   if (nucleus) {
     const double limit = f.top_p * whole;
     last.key = 0xffffffffu;
-    if (found > 0) sort_front(sh.list.cand, found);
+    if (found > 0) sort_front(sh.list.cand, found, reinterpret_cast<uint64_t*>(s_hist), sh.list.counts);        // the ranges of logits are not needed any more
     if (above > 0.0 && above >= limit) return false;     // the border is above the range
     double done = above;
-    double* const masses = reinterpret_cast<double*>(s_hist);        // the ranges of logits are not needed any more
+    double* const masses = reinterpret_cast<double*>(s_hist);
 #pragma unroll 1
     for (int i0 = 0; i0 < found; i0 += kRowThreads) {
       const int i = i0 + tid;
@@ -554,10 +556,10 @@ NRL_DEVICE int kept_of(const uint64_t* x, int found, int sure, const RowFilter& 
 }
 
 // from the n first candidates, which are sorted, by index
-NRL_DEVICE void draw_of(uint64_t* x, int n, const double* mass, double total, double u, SampleShared& sh, int* out_token, float* out_logp) {
+NRL_DEVICE void draw_of(uint64_t* x, int n, const double* mass, double total, double u, SampleShared& sh, uint64_t* y, int* out_token, float* out_logp) {
   const int tid = threadIdx.x;
   for (int i = tid; i < n; i += kRowThreads) x[i] = x[i] << 32 | static_cast<uint32_t>(i);        // (~index, place)
-  sort_front(x, n);                                         // (its first barrier is behind the swap)
+  sort_front(x, n, y, sh.list.counts);                               // (its first barrier is behind the swap)
   if (tid == 0) sh.token = 0x7fffffff;
   const double target = u * total;
   double done = 0.0;
@@ -670,11 +672,11 @@ __global__ void __launch_bounds__(kRowThreads, 3) sample_filtered_kernel(const T
       for (int i = tid; i < found; i += kRowThreads) n += static_cast<uint32_t>(sh.list.cand[i] >> 32) >= least ? 1 : 0;
       sure = static_cast<int>(block_sum(static_cast<double>(n), sh.border.red));
     }
-    sort_front(sh.list.cand, found);
-    double* mass = reinterpret_cast<double*>(s_chunk);     // the maxima are not needed any more
+    sort_front(sh.list.cand, found, reinterpret_cast<uint64_t*>(s_chunk), sh.list.counts);        // the maxima are not needed any more
+    double* mass = reinterpret_cast<double*>(s_chunk);
     double* upto = mass + kCandidates;
     const int n = kept_of(sh.list.cand, found, sure, f, mx, whole, mass, upto, sh);
-    if (n > 0) draw_of(sh.list.cand, n, mass, upto[n - 1], u, sh, tokens + r, logp + r);
+    if (n > 0) draw_of(sh.list.cand, n, mass, upto[n - 1], u, sh, reinterpret_cast<uint64_t*>(upto), tokens + r, logp + r);
     else open = mx;
   } else {
     open = mx;
@@ -713,6 +715,11 @@ cudaError_t launch_sample(const void* logits, long row_stride, int rows, int V, 
   const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_filtered_kernel<T>, z, row_stride, V, uniforms, f, tokens, logp, top);
   if (e != cudaSuccess || top == nullptr) return e;
   cfg.dynamicSmemBytes = (kBins + 2) * kRowThreads * 4;
+  // Filters of every row's own send a part of the rows on, which twice the blocks finish sooner: 250 x 50 021 floats, a third of them, 71 / 63 / 61 us in all with 1 / 2 / 4,
+  // 700 rows 118 / 105 / 118, 64 x 151 936 115 / 84 / 77; where all rows come, 256 x 151 936, 258 / 268 / 311.
+  const int more = f.top_k != nullptr || f.top_p != nullptr || f.min_p != nullptr || f.temperature != nullptr ? std::min(2 * blocks, kRowClusterMax) : blocks;
+  attr[0].val.clusterDim.x = more;
+  cfg.gridDim = dim3(static_cast<unsigned>(rows) * more);
   return cudaLaunchKernelEx(&cfg, sample_long_kernel<T>, z, row_stride, V, uniforms, f, static_cast<const float*>(top), tokens, logp);
 }
 

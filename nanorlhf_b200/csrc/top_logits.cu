@@ -48,7 +48,8 @@ __device__ __noinline__ void top_by_border(const LogitRow<T>& row, int k, double
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads, 3) top_logprobs_kernel(const T* __restrict__ logits, long row_stride, int V, int k, double inv_temp,
                                                                       float* __restrict__ logp, int* __restrict__ idx) {
-  extern __shared__ float s_chunk[];                     // [chunks][kRowThreads]
+  extern __shared__ __align__(16) float s_chunk[];       // [chunks][kRowThreads]; then what sorting takes
+  static_assert(kCandidates * 8 <= kRowChunks * kRowThreads * 4, "in the place of the maxima");
   __shared__ TopShared sh;
   const int rank = static_cast<int>(cluster_rank()), blocks = static_cast<int>(cluster_blocks()), tid = threadIdx.x;
   const long r = blockIdx.x / blocks;
@@ -111,7 +112,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) top_logprobs_kernel(const T* _
     sum = warp_sum(sum);
     if ((tid & 31) == 0) sh.log_sum = logf(static_cast<float>(sum));       // half a step of it: 5e-7; the double one takes as long as the ranking
   }
-  in_order(sh.list.cand, found, n, [&](int place, uint64_t x) {
+  in_order(sh.list.cand, found, n, reinterpret_cast<uint64_t*>(s_chunk), sh.list.counts, [&](int place, uint64_t x) {
     const float z = key_logit(static_cast<uint32_t>(x >> 32));
     logp[r * k + place] = static_cast<float>((z == top ? 0.0 : (static_cast<double>(z) - top) * inv_temp) - sh.log_sum);
     idx[r * k + place] = static_cast<int>(~static_cast<uint32_t>(x));
@@ -135,7 +136,7 @@ cudaError_t launch_top(const void* logits, long row_stride, int rows, int V, int
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows) * blocks);
   cfg.blockDim = dim3(kRowThreads);
-  cfg.dynamicSmemBytes = row_chunks(V, LogitRow<T>::N, blocks) * kRowThreads * 4;
+  cfg.dynamicSmemBytes = kRowChunks * kRowThreads * 4;
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
