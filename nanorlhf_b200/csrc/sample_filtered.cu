@@ -516,7 +516,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_long_kernel(const T* __
   }
 }
 
-constexpr int kNucleusGroups = 128;                        // groups whose maxima bound the candidates of a nucleus
+constexpr int kNucleusGroups = 256;                        // groups whose maxima bound the candidates of a nucleus (128: 1024 peaked rows with top-p 0.95 442 -> 422 us)
 
 // Over the sorted candidates: how many of them are kept; 0: it is not known (nucleus of a whole row whose mass `whole` is only known to kSumError, or whose last token is
 // not among the `sure` first, beyond which others may come between).  mass, upto: theirs, and the sums up to and with every one.
