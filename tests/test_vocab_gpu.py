@@ -129,6 +129,17 @@ def test_sampling_with_filters_of_every_row(B, V, dtype):
     _same_draws(z, u, temperature=t, top_k=k, top_p=p, min_p=m)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("B", [15, 30, 100, 200])          # eight, four, two blocks a row and one
+@pytest.mark.parametrize("pattern", ["normal", "peaked", "ties"])
+def test_sampling_of_many_kept_tokens(pattern, B, dtype):
+    """nuclei of most of the vocabulary, no filters, and more tokens above min_p than are sorted"""
+    z = _logits(pattern, B, 80000, dtype, seed=2)
+    u = torch.rand(B, generator=_gen(B), device=DEV)
+    for kw in (dict(), dict(top_p=0.97), dict(temperature=1.5, top_p=0.6), dict(min_p=0.05), dict(min_p=0.01, top_p=0.9)):
+        _same_draws(z, u, **kw)
+
+
 @pytest.mark.parametrize("temperature", [1e-300, 1e-42, 1e-30, 1e30])
 @pytest.mark.parametrize("pattern", ["normal", "ties"])
 def test_temperatures_far_from_one(pattern, temperature):
@@ -477,6 +488,32 @@ def test_backward_captured_without_its_forward():
     for _ in range(3):
         graph.replay()
     assert torch.equal(g, want)
+
+
+@pytest.mark.parametrize("beta", [0.0, 0.5])
+def test_traced_distillation_follows_its_inputs(beta):
+    x, y = (_logits("normal", 5, 300, F32, seed=s) for s in (1, 2))
+    logp, idx = _teacher(x, 9)
+    f = lambda z: ops.distill_loss(z, logp, idx, beta=beta)  # noqa: E731
+    traced = torch.jit.trace(f, x, check_trace=False)
+    p, q = (y.clone().requires_grad_() for _ in range(2))
+    got, want = traced(p), f(q)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    (2.0 * got[0]).backward()
+    (2.0 * want[0]).backward()
+    assert torch.equal(p.grad, q.grad)
+
+
+def test_saved_gradients_may_be_packed_away():
+    """hooks on saved tensors get the gradient that the forward has formed, and the backward takes what they give"""
+    z = _logits("normal", 4, 500, F32)
+    logp, idx = _teacher(z, 9)
+    x, y = z.clone().requires_grad_(), z.clone().requires_grad_()
+    with torch.autograd.graph.save_on_cpu():
+        loss, _ = ops.distill_loss(x, logp, idx)
+    (3.0 * loss).backward()
+    (3.0 * ops.distill_loss(y, logp, idx)[0]).backward()
+    assert torch.equal(x.grad, y.grad)
 
 
 def test_rows_beyond_32_bit_offsets():
