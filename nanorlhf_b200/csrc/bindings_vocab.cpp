@@ -29,6 +29,11 @@ void check_beside(const torch::Tensor& t, const torch::Tensor& logits, torch::Sc
   TORCH_CHECK(t.device() == logits.device() && t.scalar_type() == type && t.sizes() == sizes && t.is_contiguous(), what, ": ", name, " must be a contiguous ",
               type, " tensor of shape ", sizes, " on the logits' device");
 }
+// a call's scratch memory: of the current stream, on 512 bytes
+torch::Tensor scratch_of(size_t bytes, const torch::Tensor& logits) {
+  return bytes > 0 ? torch::empty({static_cast<int64_t>(bytes)}, logits.options().dtype(torch::kUInt8)) : torch::Tensor();
+}
+inline void* ptr_of(const torch::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 inline bool is_bf16(const torch::Tensor& t) { return t.scalar_type() == torch::kBFloat16; }
 
 std::tuple<torch::Tensor, torch::Tensor> top_logprobs(const torch::Tensor& logits, int64_t k, double inv_temp) {
@@ -37,8 +42,9 @@ std::tuple<torch::Tensor, torch::Tensor> top_logprobs(const torch::Tensor& logit
   c10::cuda::CUDAGuard guard(logits.device());
   torch::Tensor logp = torch::empty({logits.size(0), k}, logits.options().dtype(torch::kFloat32));
   torch::Tensor idx = torch::empty({logits.size(0), k}, logits.options().dtype(torch::kInt32));
+  const torch::Tensor scratch = scratch_of(nrl_top_scratch(is_bf16(logits), logits.size(0), logits.size(1), k), logits);
   check(nrl_top_logprobs(logits.data_ptr(), is_bf16(logits), logits.stride(0), logits.size(0), logits.size(1), k, inv_temp, logp.data_ptr<float>(),
-                         idx.data_ptr<int>(), cur_stream()), "top_logprobs");
+                         idx.data_ptr<int>(), ptr_of(scratch), cur_stream()), "top_logprobs");
   return {logp, idx};
 }
 
@@ -59,9 +65,10 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> distill_loss(const torch
   torch::Tensor token = torch::empty({rows}, f32), loss, grad;
   if (with_loss) loss = torch::empty({}, f32);
   if (want_grad) grad = torch::empty({rows, V}, logits.options().dtype(bf16_grad || is_bf16(logits) ? torch::kBFloat16 : torch::kFloat32));
+  const torch::Tensor scratch = scratch_of(nrl_distill_scratch(is_bf16(logits), rows, V, want_grad), logits);
   check(nrl_distill_loss(logits.data_ptr(), is_bf16(logits), logits.stride(0), rows, V, top_logp.data_ptr<float>(), top_idx.data_ptr<int>(), k,
                          weights.has_value() ? weights->data_ptr<float>() : nullptr, inv_temp, beta, tail, token.data_ptr<float>(),
-                         with_loss ? loss.data_ptr<float>() : nullptr, want_grad ? grad.data_ptr() : nullptr, want_grad && is_bf16(grad), cur_stream()),
+                         with_loss ? loss.data_ptr<float>() : nullptr, ptr_of(grad), want_grad && is_bf16(grad), ptr_of(scratch), cur_stream()),
         "distill_loss");
   return {loss, token, grad};
 }
@@ -162,8 +169,9 @@ std::tuple<torch::Tensor, torch::Tensor> sample_filtered(const torch::Tensor& lo
   torch::Tensor tokens = torch::empty({rows}, logits.options().dtype(torch::kInt32)), logp = torch::empty({rows}, logits.options().dtype(torch::kFloat32));
   torch::Tensor top;
   if (!nrl_sample_is_short(&f, logits.size(1))) top = torch::empty({rows}, logp.options());
+  const torch::Tensor scratch = scratch_of(nrl_sample_scratch(is_bf16(logits), rows, logits.size(1), &f), logits);
   check(nrl_sample_filtered(logits.data_ptr(), is_bf16(logits), logits.stride(0), rows, logits.size(1), uniforms.data_ptr<float>(), &f, tokens.data_ptr<int>(),
-                            logp.data_ptr<float>(), top.defined() ? top.data_ptr<float>() : nullptr, cur_stream()), "sample_filtered");
+                            logp.data_ptr<float>(), static_cast<float*>(ptr_of(top)), ptr_of(scratch), cur_stream()), "sample_filtered");
   return {tokens, logp};
 }
 

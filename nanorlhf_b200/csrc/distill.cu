@@ -50,7 +50,7 @@ struct DistillShared {
   float z[kTopMax], a[kTopMax];
   double p[kTopMax];                                       // of the token by all its entries; below 0: not a token, or an earlier entry has it
   double q[kTopMax];                                       // beta > 0: D of the token's event
-  float2 part[kRowClusterMax][kRowWarps];                  // maximum and sum of every warp of the cluster
+  float2 part[kRowWarps];                                  // maximum and sum of every warp
   double red[2][kRowWarps];
   int twins;                                               // some token has several entries
 };
@@ -75,7 +75,7 @@ constexpr double kNoTail = 5.9604644775390625e-8;          // 2^-24
 template <typename T, typename G>
 __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __restrict__ logits, long row_stride, int V, const float* __restrict__ top_logp,
                                                                  const int* __restrict__ top_idx, int K, const float* __restrict__ weights, double inv_temp,
-                                                                 double beta, int tail, float* __restrict__ token_loss, G* __restrict__ grad) {
+                                                                 double beta, int tail, float* __restrict__ token_loss, G* __restrict__ grad, float2* parts) {
   constexpr int N = LogitRow<T>::N, W = N * sizeof(G) / 4;
   extern __shared__ __align__(16) uint32_t s_map[];        // a bit for every element of the share's vectors: one of the teacher's tokens
   __shared__ DistillShared sh;
@@ -104,7 +104,6 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
       for (int v = share.first + tid; v < share.end; v += kRowThreads) store_grads(out, v * N - row.skew, V, none);
     return;
   }
-  if (blocks > 1) cluster_arrive();                        // shared memory may be written by the others once it is known to run
   // ---- the teacher's entries, and where they lie in the share ----
   if (tid == 0) sh.twins = 0;
   __syncthreads();
@@ -138,16 +137,12 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
       }
     }
   });
-  const float mw = warp_max(m);
-  mass = warp_sum(mass * ex2((m - mw) * c));
-  if (blocks > 1) cluster_wait();
-  if (lane < blocks) {
-    const uint32_t there = in_block(&sh.part[rank][tid >> 5], lane);
-    st_block(there, mw);
-    st_block(there + 4, mass);
+  const float2 state = block_state(m, mass, c, sh.part);
+  if (blocks > 1) {
+    if (tid == 0) parts[r * blocks + rank] = state;
+    __syncwarp();
+    cluster_arrive();
   }
-  __syncwarp();
-  if (blocks > 1) cluster_arrive();
   for (int i = tid; i < K; i += kRowThreads) {             // probabilities of the teacher's tokens, while the other blocks come
     const int at = sh.idx[i];
     const T z = row.p[max(at, 0)];
@@ -171,15 +166,13 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
   __syncwarp();
   if (blocks > 1) cluster_wait();
   __syncthreads();
-  float mx = -INFINITY;
-  for (int i = lane; i < blocks * kRowWarps; i += 32) mx = fmaxf(mx, sh.part[i / kRowWarps][i % kRowWarps].x);
-  mx = warp_max(mx);
-  double others = 0.0, psum = 0.0, top = 0.0;
-  for (int i = lane; i < blocks * kRowWarps; i += 32) {
-    const float2 p = sh.part[i / kRowWarps][i % kRowWarps];
-    others += p.y * ex2((p.x - mx) * c);
+  float mx = state.x;
+  double others = state.y, psum = 0.0, top = 0.0;
+  if (blocks > 1) {
+    const float2 p = lane < blocks ? __ldcg(&parts[r * blocks + lane]) : make_float2(-INFINITY, 0.f);
+    mx = warp_max(p.x);
+    others = warp_sum(static_cast<double>(lane < blocks ? p.y * ex2((p.x - mx) * c) : 0.f));
   }
-  others = warp_sum(others);
   for (int i = lane; i < K; i += 32)
     if (sh.p[i] >= 0.0) {
       psum += sh.p[i];
@@ -316,17 +309,23 @@ __global__ void scale_kernel(T* __restrict__ x, long n, const float* __restrict_
     x[i] = static_cast<T>(static_cast<float>(x[i]) * f);
 }
 
-template <typename T, typename G>
-cudaError_t launch_distill(const void* logits, long row_stride, int rows, int V, const float* top_logp, const int* top_idx, int k, const float* weights,
-                           double inv_temp, double beta, int tail, float* token_loss, void* grad, cudaStream_t s) {
-  static PerDevice<bool> done;
-  constexpr int N = LogitRow<T>::N;
+template <typename T>
+int distill_blocks(int rows, int V, bool with_grad) {
   // The second pass should find its rows in L2, which has 126 MB; three blocks on each of 148 SMs hold 444 rows at a time, or half or a quarter of them with two or four
   // blocks a row.  us with 1 / 2 / 4 of 2048 x 151 936 floats 574 / 544 / 522, bf16 298 / 293 / 383 (DRAM reads 1.47 / 1.07 / 1.00 of the logits), of 1500 x 50 021 floats
   // 148 / 155 / 211, of 2048 x 32 000 bf16 83 / 123 / 210.
-  int blocks = row_blocks(rows, V, N);
+  int blocks = row_blocks(rows, V, LogitRow<T>::N);
   const long held = std::min(rows, 444) * static_cast<long>(V) * sizeof(T);
-  if (grad != nullptr) blocks = std::max(blocks, held > 200L << 20 ? 4 : held > 100L << 20 ? 2 : 1);
+  if (with_grad) blocks = std::max(blocks, held > 200L << 20 ? 4 : held > 100L << 20 ? 2 : 1);
+  return blocks;
+}
+
+template <typename T, typename G>
+cudaError_t launch_distill(const void* logits, long row_stride, int rows, int V, const float* top_logp, const int* top_idx, int k, const float* weights,
+                           double inv_temp, double beta, int tail, float* token_loss, void* grad, void* parts, cudaStream_t s) {
+  static PerDevice<bool> done;
+  constexpr int N = LogitRow<T>::N;
+  const int blocks = distill_blocks<T>(rows, V, grad != nullptr);
   const int vecs = ((V + 2 * N - 2) / N + blocks - 1) / blocks;
   if (const cudaError_t e = allow_smem(done, distill_kernel<T, G>, kDistillVocabMax / 8 + 128); e != cudaSuccess) return e;
   cudaLaunchAttribute attr[1];
@@ -341,20 +340,25 @@ cudaError_t launch_distill(const void* logits, long row_stride, int rows, int V,
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, distill_kernel<T, G>, static_cast<const T*>(logits), row_stride, V, top_logp, top_idx, k, weights, inv_temp, beta, tail,
-                            token_loss, static_cast<G*>(grad));
+                            token_loss, static_cast<G*>(grad), static_cast<float2*>(parts));
 }
 
 }  // namespace nrl
 
 using namespace nrl;
 
+extern "C" size_t nrl_distill_scratch(int is_bf16, int rows, int V, int with_grad) {
+  const int blocks = is_bf16 ? distill_blocks<__nv_bfloat16>(rows, V, with_grad) : distill_blocks<float>(rows, V, with_grad);
+  return blocks > 1 ? static_cast<size_t>(rows) * blocks * sizeof(float2) : 0;
+}
+
 extern "C" cudaError_t nrl_distill_loss(const void* logits, int is_bf16, long row_stride, int rows, int V, const float* top_logp, const int* top_idx, int k,
                                         const float* weights, double inv_temp, double beta, int tail, float* token_loss, float* loss, void* grad,
-                                        int grad_bf16, cudaStream_t s) {
+                                        int grad_bf16, void* scratch, cudaStream_t s) {
   if (V > kDistillVocabMax || k > kTopMax || (is_bf16 && grad && !grad_bf16)) return cudaErrorInvalidValue;
   if (rows > 0) {
     const auto launch = is_bf16 ? launch_distill<__nv_bfloat16, __nv_bfloat16> : grad_bf16 ? launch_distill<float, __nv_bfloat16> : launch_distill<float, float>;
-    const cudaError_t e = launch(logits, row_stride, rows, V, top_logp, top_idx, k, weights, inv_temp, beta, tail, token_loss, grad, s);
+    const cudaError_t e = launch(logits, row_stride, rows, V, top_logp, top_idx, k, weights, inv_temp, beta, tail, token_loss, grad, scratch, s);
     if (e != cudaSuccess) return e;
   }
   return loss ? nrl_weighted_sum(token_loss, weights, rows, loss, s) : cudaSuccess;

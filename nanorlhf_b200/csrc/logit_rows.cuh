@@ -300,22 +300,8 @@ NRL_DEVICE uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%clu
 NRL_DEVICE uint32_t cluster_blocks() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
 NRL_DEVICE void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 NRL_DEVICE void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-// the address of `p` (a shared-memory object of this block) in the shared memory of the cluster's block `rank`
-NRL_DEVICE uint32_t in_block(const void* p, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
-  return r;
-}
-NRL_DEVICE void st_block(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
-NRL_DEVICE void st_block(uint32_t addr, double v) { asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory"); }
-NRL_DEVICE void st_block(uint32_t addr, uint64_t v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory"); }
-NRL_DEVICE int add_block(uint32_t addr, int v) {
-  int r;
-  asm volatile("atom.relaxed.cluster.shared::cluster.add.s32 %0, [%1], %2;" : "=r"(r) : "r"(addr), "r"(v) : "memory");
-  return r;
-}
-
-constexpr int kRowClusterMax = 8;
+// Blocks of a cluster tell each other what they found through memory of the call's own, written before a barrier at which all arrive and read behind it, past the L1.
+constexpr int kRowClusterMax = 4;
 constexpr int kRowUnroll = 2;                          // vectors of a thread in flight
 constexpr int kRowChunks = 16;                         // of a thread's vectors, each with a maximum of its own
 
@@ -331,14 +317,15 @@ struct RowShare {
     chunks = len > 0 ? (steps + len - 1) / len : 0;
   }
 };
-// Blocks of a row's cluster (host).  A row of its own block is fastest where the rows fill the SMs; of few rows the cluster shares the reading, until its barriers
-// cost more.  us with 1 / 2 / 4 / 8 blocks (top 20 to 64 of bf16 rows of 151 936): 1 row 15.8 / 11.9 / 10.1 / 10.1, 8 rows 20.8 / 14.7 / 12.0 / 11.2, 32 rows 23.3 / 17.2 /
-// 15.6 / 28.4, 100 rows 23.3 / 20.5 / 25.9 / 51, 300 rows 36.6 / 42.6 / 62 / 118; 64 rows of 32 000 10.1 / 10.3 / 16.3 / 34, of 4000 floats 6.6 / 7.7 / 10.0 / 18.7.
+// Blocks of a row's cluster (host).  A row of its own block is fastest where the rows fill the SMs; of few rows the cluster shares the reading, until its barrier and
+// the way through memory cost more.  us with 1 / 2 / 4 / 8 blocks of bf16 rows of 151 936, top 20: 1 row 15.4 / 12.4 / 11.1 / 10.9, 32 rows 16.1 / 13.5 / 11.6 / 14.1, 64
+// rows 16.3 / 13.8 / 14.7 / 23.2, 100 rows 16.6 / 17.5 / 18.2 / 30.6, 300 rows 34 / 40 / 50 / 79; sampling with top-k 50: 1 row 15.2 / 14.4 / 14.3 / 17.3, 64 rows
+// 16.0 / 16.0 / 19.2 / 35.  With 1 / 2 blocks, top 20 of 32 000 floats: 1 row 7.7 / 8.3, 64 rows 7.9 / 9.3.
 inline int row_blocks(long rows, int V, int vec) {
   constexpr int kSms = 148;
   const long nvec = V / vec;
-  int blocks = rows <= kSms / 8 ? 8 : rows <= kSms / 4 ? 4 : rows <= kSms ? 2 : 1;
-  while (blocks > 1 && nvec < 1024L * blocks) blocks /= 2;
+  int blocks = rows < kSms / 4 ? 4 : rows <= kSms / 2 ? 2 : 1;
+  while (blocks > 1 && nvec < 2048L * blocks) blocks /= 2;
   return blocks;
 }
 
@@ -468,12 +455,12 @@ struct SortCounts {
   int sums[kRowWarps];
 };
 struct RowList {
-  __align__(16) uint64_t cand[kCandidates];            // (key, ~index): unsigned numbers in the order; those that other blocks send from the end on
+  __align__(16) uint64_t cand[kCandidates];            // (key, ~index): unsigned numbers in the order
   union {
     unsigned short hits[kCandidates];
     SortCounts counts;                                 // (when the hits are not needed any more)
   };
-  int n, nhits, sent;
+  int n, nhits;
 };
 // Into `list` all elements of the share whose keys reach `bound`: the chunks that have any (by their maxima) are read again, a vector a thread.  list.n and
 // list.nhits are 0 before; above kCandidates they say that there is more than what the list holds.
@@ -514,33 +501,61 @@ NRL_DEVICE void gather_candidates(const LogitRow<T>& row, const RowShare& share,
   }
   __syncthreads();
 }
-// The list to the first block's; a cluster barrier in front, by which that block is known to run, and one behind.
-NRL_DEVICE void send_candidates(const RowList& list, int* s_base) {
-  const uint32_t there = in_block(list.cand, 0);
-  const int n = list.n > kCandidates || list.nhits > kCandidates ? kCandidates + 1 : list.n;
-  if (threadIdx.x == 0) *s_base = add_block(in_block(&list.sent, 0), n);
-  __syncthreads();
-  for (int i = threadIdx.x; i < min(n, kCandidates) && *s_base + i < kCandidates; i += kRowThreads)
-    st_block(there + (kCandidates - 1 - *s_base - i) * 8, list.cand[i]);
+
+// A row's memory where several blocks share it; behind it the candidates of all blocks but the first, kCandidates each.
+struct RowMail {
+  float2 part[kRowClusterMax];                         // a block's largest logit and its sum of 2^((z - m) c)
+  double whole[kRowClusterMax], mass[kRowClusterMax][kRowWarps];
+  float4 edges;
+  float bins[kRowClusterMax][36];
+  int n[kRowClusterMax];
+  uint32_t bound[kRowClusterMax];
+  NRL_DEVICE uint64_t* list(int rank) { return reinterpret_cast<uint64_t*>(this + 1) + (rank - 1) * kCandidates; }
+};
+static_assert(sizeof(RowMail) % 16 == 0, "lists on 16 bytes");
+inline size_t row_mail_bytes(int blocks) { return blocks > 1 ? sizeof(RowMail) + static_cast<size_t>(blocks - 1) * kCandidates * 8 : 0; }
+
+// In front of the barrier: this block's list for the first.
+NRL_DEVICE void send_candidates(const RowList& list, int rank, RowMail& mail) {
+  const int n = list.nhits > kCandidates ? kCandidates + 1 : list.n;
+  if (threadIdx.x == 0) mail.n[rank] = n;
+  uint64_t* to = mail.list(rank);
+  for (int i = threadIdx.x; i < min(n, kCandidates); i += kRowThreads) to[i] = list.cand[i];
 }
-// Behind the barrier, the first block: what came to its own, side by side; returns how many there are, above kCandidates where they do not fit.
-NRL_DEVICE int join_candidates(RowList& list) {
-  const int own = list.nhits > kCandidates ? kCandidates + 1 : list.n, sent = list.sent, all = own + sent;
-  if (sent == 0 || all > kCandidates) return all;
-  uint64_t x[kCandidates / kRowThreads];
+// Behind it, the first block: all lists in its own; returns how many there are, above kCandidates where they do not fit.
+NRL_DEVICE int join_candidates(RowList& list, int blocks, RowMail* mail) {
+  int all = list.nhits > kCandidates ? kCandidates + 1 : list.n;
+  if (blocks == 1) return all;
+  int n[kRowClusterMax];                               // up to and with a block's
 #pragma unroll
-  for (int t = 0; t < kCandidates / kRowThreads; ++t) {
-    const int i = threadIdx.x + t * kRowThreads;
-    if (i < sent) x[t] = list.cand[kCandidates - 1 - i];
-  }
-  __syncthreads();
+  for (int q = 1; q < kRowClusterMax; ++q) n[q] = q < blocks ? __ldcg(&mail->n[q]) : 0;
+  n[0] = all;
 #pragma unroll
-  for (int t = 0; t < kCandidates / kRowThreads; ++t) {
-    const int i = threadIdx.x + t * kRowThreads;
-    if (i < sent) list.cand[own + i] = x[t];
+  for (int q = 1; q < kRowClusterMax; ++q) n[q] = min(n[q], kCandidates + 1) + n[q - 1];
+  all = n[kRowClusterMax - 1];
+  if (all > kCandidates) return all;
+  for (int i = n[0] + threadIdx.x; i < all; i += kRowThreads) {        // of all blocks at once
+    int q = 1, first = n[0];
+#pragma unroll
+    for (int p = 1; p < kRowClusterMax - 1; ++p)
+      if (i >= n[p]) {
+        q = p + 1;
+        first = n[p];
+      }
+    list.cand[i] = __ldcg(reinterpret_cast<unsigned long long*>(mail->list(q) + (i - first)));
   }
   __syncthreads();
   return all;
+}
+
+// The block's largest logit and sum of 2^((z - m) c) from its threads'; every thread gets them.  `part`: kRowWarps entries that nobody else uses.
+NRL_DEVICE float2 block_state(float m, float s, float c, float2* part) {
+  const float mw = warp_max(m), sw = warp_sum(s * ex2((m - mw) * c));
+  if (lane_id() == 0) part[threadIdx.x >> 5] = make_float2(mw, sw);
+  __syncthreads();
+  const float2 p = part[lane_id() % kRowWarps];
+  const float mb = warp_max(p.x);
+  return make_float2(mb, warp_sum(lane_id() < kRowWarps ? p.y * ex2((p.x - mb) * c) : 0.f));
 }
 
 // How many of the different numbers x[0 .. n) are above `mine`; x lies on 16 bytes and x[n] .. x[n + 7] are 0

@@ -41,18 +41,18 @@ struct RowFilter {
   NRL_DEVICE double mass(float z, float mx) const { return z == mx ? 1.0 : exp((static_cast<double>(z) - mx) * inv_temp); }
 };
 
-// Float sums of 2^x are off by so much of themselves at most: 2^-22 for 2^x, three steps of 2^-24 of the exponents, whose mean over the mass is log2 V < 24 at most, and
-// sums of at most 300 terms a thread in float.
-constexpr double kSumError = 2e-5;
+// The float sum of 2^x of a row is off by so much of itself at most, in units of 2^-24: 30 for a step's terms and for joining threads, warps and blocks; for every step of a
+// thread, of 512 x 16 elements at least, 3 of its additions and 4 of 2^x where the reference moves; 4 of 2^x; 3 of every exponent, whose mean over the mass is
+// log2 V <= 31, times ln 2.
+NRL_DEVICE double sum_error(int V) { return (100.0 + V / 1100.0) * 0x1p-24; }
 
 struct SampleShared {
   BorderShared border;
   RowList list;
   BoundShared bound;
   double scan[kRowWarps];
-  float2 part[kRowClusterMax][kRowWarps];                  // maximum and sum of every warp of the cluster
-  uint32_t part_bound[kRowClusterMax];
-  int base, token;
+  float2 part[kRowWarps];                                  // maximum and sum of every warp
+  int token;
 };
 
 constexpr int kBins = 32;                                  // ranges of logits a pass of the long way
@@ -62,11 +62,12 @@ struct LongShared {
   double scan[kRowWarps];
   double mass[kRowClusterMax][kRowWarps], whole[kRowClusterMax];         // kept for good and altogether, by ranges of the row
   double powers[128];
-  float bins[kRowClusterMax][kBins + 2];                   // what lies above them, they, and what lies below
-  float edge, high, low;
+  float bins[kBins + 2];                                   // what lies above them, they, and what lies below
+  float4 edges;                                            // where the next ranges begin, kept for good from, open from, enough
   unsigned short place[kCandidates];
-  int base, token, enough;
+  int base, token;
 };
+constexpr double kRangeSlack = 1e-5;                       // of the mass: what float sums may be off by when ranges are picked; double ones check them
 
 // sums over the threads up to and with this one, and over all
 NRL_DEVICE double block_scan(double v, double& all, double* red) {
@@ -223,14 +224,14 @@ struct RowMass {
 // logit) is left to sample_by_border: then false.
 template <typename T>
 NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx, double u, int rank, int blocks, uint32_t* s_hist, LongShared& sh,
-                            int* out_token, float* out_logp) {
+                            RowMail* mail, int* out_token, float* out_logp) {
   constexpr int N = LogitRow<T>::N;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const RowShare share(row.nvec, rank, blocks);
   const float c = log2_scale(f.inv_temp);
   if (tid < 128) sh.powers[tid] = exp2(tid / 128.0);
   const RowMass mass(f, mx, sh.powers);
-  if (tid == 0) sh.list.n = sh.list.nhits = sh.list.sent = 0;
+  if (tid == 0) sh.list.n = sh.list.nhits = 0;
   // the least logit that min_p keeps: every lane tries one of 32 keys of a range, seven times
   uint32_t floor_key = kKeyNone + 1;
   if (f.min_p > 0.0) {
@@ -284,7 +285,7 @@ NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx
 #pragma unroll
         for (int w = 0; w < kRowWarps; ++w) sum += __uint_as_float(s_hist[(w * (kBins + 2) + b) * 32 + lane]);
         sum = warp_sum(sum);
-        if (lane == 0) st_block(in_block(&sh.bins[rank][b], 0), sum);
+        if (lane == 0) (blocks > 1 ? mail->bins[rank] : sh.bins)[b] = sum;
       }
       __syncwarp();
       if (blocks > 1) {
@@ -296,9 +297,9 @@ NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx
       if (rank == 0 && warp == 0) {                        // a lane a range
         double m = 0.0, start = 0.0, rest = 0.0;
         for (int q = 0; q < blocks; ++q) {
-          m += sh.bins[q][lane + 1];
-          start += sh.bins[q][0];
-          rest += f.min_p > 0.0 && low <= floor ? 0.0 : sh.bins[q][kBins + 1];
+          m += blocks > 1 ? __ldcg(&mail->bins[q][lane + 1]) : sh.bins[lane + 1];
+          start += blocks > 1 ? __ldcg(&mail->bins[q][0]) : sh.bins[0];
+          rest += f.min_p > 0.0 && low <= floor ? 0.0 : blocks > 1 ? __ldcg(&mail->bins[q][kBins + 1]) : sh.bins[kBins + 1];
         }
         double upto = m;
 #pragma unroll
@@ -309,31 +310,27 @@ NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx
         upto += start;
         const double whole = __shfl_sync(0xffffffffu, upto, 31) + rest;
         // from the range in which the mass passes what the nucleus needs, less what float sums may be off by, to the one in which it passes that and as much more
-        const unsigned past0 = __ballot_sync(0xffffffffu, upto >= whole * (f.top_p - kSumError / 2)), past1 = __ballot_sync(0xffffffffu, upto >= whole * (f.top_p + kSumError / 2));
+        const unsigned past0 = __ballot_sync(0xffffffffu, upto >= whole * (f.top_p - kRangeSlack)), past1 = __ballot_sync(0xffffffffu, upto >= whole * (f.top_p + kRangeSlack));
         const int b0 = past0 ? __ffs(past0) - 1 : 31, b1 = past1 ? __ffs(past1) - 1 : 31;
         const double open = __shfl_sync(0xffffffffu, upto, b1) - __shfl_sync(0xffffffffu, upto - m, b0);
-        const float width = (edge - low) / kBins, over = width / 8 + 1e-6f * (fabsf(edge) + fabsf(low));
+        const float width = (edge - low) / kBins, over = width / 1024 + 1e-6f * (fabsf(edge) + fabsf(low));        // for the edges' rounding
         const float e1 = b0 == 0 ? edge : edge - b0 * width + over, e0 = b1 == kBins - 1 ? low : edge - (b1 + 1) * width - over;
         const float next_high = b0 > 0 ? e1 : high, next_low = fmaxf(e0, low);
-        const int ok = open <= 1900.0 * ex2((next_low - mx) * c);
-        if (lane < blocks) {
-          st_block(in_block(&sh.edge, lane), e1);
-          st_block(in_block(&sh.high, lane), next_high);
-          st_block(in_block(&sh.low, lane), next_low);
-          st_block(in_block(&sh.enough, lane), __int_as_float(ok));
-        }
+        const bool ok = open <= 1700.0 * ex2((next_low - mx) * c);        // tokens, by the least of their masses; those on the edges come on top
+        if (lane == 0) (blocks > 1 ? mail->edges : sh.edges) = make_float4(e1, next_high, next_low, ok ? 1.f : 0.f);
         __syncwarp();
       }
       if (blocks > 1) {
         cluster_arrive();
         cluster_wait();
+      } else {
+        __syncthreads();
       }
-      __syncthreads();
-      edge = sh.edge;
-      high = sh.high;
-      low = sh.low;
-      enough = sh.enough != 0;
-      __syncthreads();
+      const float4 next = blocks > 1 ? __ldcg(&mail->edges) : sh.edges;
+      edge = next.x;
+      high = next.y;
+      low = next.z;
+      enough = next.w != 0.f;
     }
   }
   // ---- in double: every warp's range of the row ----
@@ -359,20 +356,24 @@ NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx
   }
   const double all = block_sum(kept + other, sh.scan);
   kept = warp_sum(kept);
-  if (lane == 0) st_block(in_block(&sh.mass[rank][warp], 0), kept);
-  if (tid == 0) st_block(in_block(&sh.whole[rank], 0), all);
+  if (lane == 0) sh.mass[rank][warp] = kept;
+  if (tid == 0) sh.whole[rank] = all;
   __syncthreads();
-  if (rank != 0) send_candidates(sh.list, &sh.base);
-  __syncwarp();
   if (blocks > 1) {
+    if (tid < kRowWarps) mail->mass[rank][tid] = sh.mass[rank][tid];
+    if (tid == 0) mail->whole[rank] = all;
+    if (rank != 0) send_candidates(sh.list, rank, *mail);
+    __syncwarp();
     cluster_arrive();
     cluster_wait();
+    if (rank != 0) return true;
+    if (tid < blocks * kRowWarps) sh.mass[tid / kRowWarps][tid % kRowWarps] = __ldcg(&mail->mass[tid / kRowWarps][tid % kRowWarps]);
+    if (tid < blocks) sh.whole[tid] = __ldcg(&mail->whole[tid]);
+    __syncthreads();
   }
-  __syncthreads();
-  if (rank != 0) return true;
 
   // ---- the last kept token ----
-  const int found = join_candidates(sh.list);
+  const int found = join_candidates(sh.list, blocks, mail);
   if (found > kCandidates) return false;
   double above = 0.0, whole = 0.0;
   for (int q = 0; q < blocks; ++q) {
@@ -497,7 +498,7 @@ NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads, 2) sample_long_kernel(const T* __restrict__ logits, long row_stride, int V, const float* __restrict__ uniforms,
                                                                      SampleFilters filters, const float* __restrict__ top, int* __restrict__ tokens,
-                                                                     float* __restrict__ logp) {
+                                                                     float* __restrict__ logp, unsigned char* mails, size_t mail_bytes) {
   extern __shared__ __align__(16) uint32_t s_hist[];       // floats [warps][kBins + 2][32]
   __shared__ LongShared sh;
   const int rank = static_cast<int>(cluster_rank()), blocks = static_cast<int>(cluster_blocks());
@@ -506,11 +507,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_long_kernel(const T* __
   if (mx != mx) return;
   const LogitRow<T> row(logits + r * row_stride, V);
   const RowFilter f(filters, r, V);
-  if (blocks > 1) {                                        // shared memory may be written by the others once it is known to run
-    cluster_arrive();
-    cluster_wait();
-  }
-  if (!sample_long(row, f, mx, uniforms[r], rank, blocks, s_hist, sh, tokens + r, logp + r)) {
+  if (!sample_long(row, f, mx, uniforms[r], rank, blocks, s_hist, sh, reinterpret_cast<RowMail*>(mails + r * mail_bytes), tokens + r, logp + r)) {
     __syncthreads();
     sample_by_border<1>(row, f, mx, uniforms[r], sh.border, sh.scan, tokens + r, logp + r);
   }
@@ -518,9 +515,9 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_long_kernel(const T* __
 
 constexpr int kNucleusGroups = 256;                        // groups whose maxima bound the candidates of a nucleus (128: 1024 peaked rows with top-p 0.95 442 -> 422 us)
 
-// Over the sorted candidates: how many of them are kept; 0: it is not known (nucleus of a whole row whose mass `whole` is only known to kSumError, or whose last token is
+// Over the sorted candidates: how many of them are kept; 0: it is not known (nucleus of a whole row whose mass `whole` is a float sum, or whose last token is
 // not among the `sure` first, beyond which others may come between).  mass, upto: theirs, and the sums up to and with every one.
-NRL_DEVICE int kept_of(const uint64_t* x, int found, int sure, const RowFilter& f, float mx, double whole, double* mass, double* upto, SampleShared& sh) {
+NRL_DEVICE int kept_of(const uint64_t* x, int found, int sure, const RowFilter& f, float mx, double whole, double off, double* mass, double* upto, SampleShared& sh) {
   const int tid = threadIdx.x, n1 = f.top_k > 0 && f.top_k < found ? f.top_k : found;
   double done = 0.0;
 #pragma unroll 1
@@ -538,8 +535,8 @@ NRL_DEVICE int kept_of(const uint64_t* x, int found, int sure, const RowFilter& 
   __syncthreads();
   double limit = f.top_p < 1.0 ? f.top_p * (whole > 0.0 ? whole : done) : 1e300, low = limit;
   if (whole > 0.0) {
-    low *= 1.0 - kSumError;
-    limit *= 1.0 + kSumError;
+    low *= 1.0 - off;
+    limit *= 1.0 + off;
   }
   int n = 0;
   bool open = false;
@@ -583,14 +580,14 @@ NRL_DEVICE void draw_of(uint64_t* x, int n, const double* mass, double total, do
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads, 3) sample_filtered_kernel(const T* __restrict__ logits, long row_stride, int V,
                                                                          const float* __restrict__ uniforms, SampleFilters filters, int* __restrict__ tokens,
-                                                                         float* __restrict__ logp, float* __restrict__ top) {
+                                                                         float* __restrict__ logp, float* __restrict__ top, unsigned char* mails, size_t mail_bytes) {
   extern __shared__ __align__(16) float s_chunk[];         // [chunks][kRowThreads]
   static_assert(kRowChunks * kRowThreads * 4 >= 2 * kCandidates * 8, "masses and sums of the candidates in their place");
   __shared__ SampleShared sh;
   const int rank = static_cast<int>(cluster_rank()), blocks = static_cast<int>(cluster_blocks()), tid = threadIdx.x, lane = tid & 31;
   const long r = blockIdx.x / blocks;
-  if (tid == 0) sh.list.n = sh.list.nhits = sh.list.sent = 0;
-  if (blocks > 1) cluster_arrive();                        // the first block's memory may be written once it is known to run
+  if (tid == 0) sh.list.n = sh.list.nhits = 0;
+  RowMail* const mail = reinterpret_cast<RowMail*>(mails + r * mail_bytes);        // of several blocks
   const LogitRow<T> row(logits + r * row_stride, V);
   const RowFilter f(filters, r, V);
   const RowShare share(row.nvec, rank, blocks);
@@ -625,29 +622,26 @@ __global__ void __launch_bounds__(kRowThreads, 3) sample_filtered_kernel(const T
     }
     gather_candidates(row, share, s_chunk, bound, sh.list);
   }
-  const float mw = warp_max(nucleus ? m : best);
-  const float sw = nucleus ? warp_sum(s * ex2((m - mw) * c)) : 0.f;
-  if (blocks > 1) cluster_wait();
-  if (lane == 0) {
-    const uint32_t there = in_block(&sh.part[rank][tid >> 5], 0);
-    st_block(there, mw);
-    st_block(there + 4, sw);
-  }
-  if (tid == 0) st_block(in_block(&sh.part_bound[rank], 0), __uint_as_float(bound));
-  if (rank != 0) send_candidates(sh.list, &sh.base);
-  __syncwarp();
+  const float2 state = block_state(nucleus ? m : best, s, c, sh.part);        // (without a nucleus the sum is 0)
+  float mx = state.x;
+  double whole = state.y;
+  uint32_t least = bound;
   if (blocks > 1) {
+    if (tid == 0) {
+      mail->part[rank] = state;
+      mail->bound[rank] = bound;
+    }
+    if (rank != 0) send_candidates(sh.list, rank, *mail);
+    __syncwarp();
     cluster_arrive();
     cluster_wait();
     if (rank != 0) return;
-  } else {
-    __syncthreads();
+    const float2 p = lane < blocks ? __ldcg(&mail->part[lane]) : make_float2(-INFINITY, 0.f);
+    mx = warp_max(p.x);
+    whole = warp_sum(static_cast<double>(lane < blocks ? p.y * ex2((p.x - mx) * c) : 0.f));
+    for (int i = 0; i < blocks; ++i) least = max(least, __ldcg(&mail->bound[i]));
   }
-
-  float mx = -INFINITY;
-  for (int i = lane; i < blocks * kRowWarps; i += 32) mx = fmaxf(mx, sh.part[i / kRowWarps][i % kRowWarps].x);
-  mx = warp_max(mx);
-  const int found = join_candidates(sh.list);
+  const int found = join_candidates(sh.list, blocks, mail);
   const double u = uniforms[r];
   float open = __int_as_float(0x7fffffff);                 // NaN: drawn
   if (mx == -INFINITY || ((few || nucleus) && found == 0)) {        // nothing to draw from
@@ -658,16 +652,8 @@ __global__ void __launch_bounds__(kRowThreads, 3) sample_filtered_kernel(const T
   } else if (mx == INFINITY || (few && found > kCandidates && f.top_k > 0) || (!few && f.top_k > 0)) {
     sample_by_border<0>(row, f, mx, u, sh.border, sh.scan, tokens + r, logp + r);
   } else if ((few || nucleus) && found <= kCandidates) {
-    double whole = 0.0;
     int sure = found;
     if (nucleus) {
-      uint32_t least = 0;
-      for (int i = lane; i < blocks * kRowWarps; i += 32) {
-        const float2 p = sh.part[i / kRowWarps][i % kRowWarps];
-        whole += p.y * ex2((p.x - mx) * c);
-      }
-      whole = warp_sum(whole);
-      for (int i = 0; i < blocks; ++i) least = max(least, sh.part_bound[i]);
       int n = 0;
       for (int i = tid; i < found; i += kRowThreads) n += static_cast<uint32_t>(sh.list.cand[i] >> 32) >= least ? 1 : 0;
       sure = static_cast<int>(block_sum(static_cast<double>(n), sh.border.red));
@@ -675,7 +661,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) sample_filtered_kernel(const T
     sort_front(sh.list.cand, found, reinterpret_cast<uint64_t*>(s_chunk), sh.list.counts);        // the maxima are not needed any more
     double* mass = reinterpret_cast<double*>(s_chunk);
     double* upto = mass + kCandidates;
-    const int n = kept_of(sh.list.cand, found, sure, f, mx, whole, mass, upto, sh);
+    const int n = kept_of(sh.list.cand, found, sure, f, mx, nucleus ? whole : 0.0, sum_error(V), mass, upto, sh);
     if (n > 0) draw_of(sh.list.cand, n, mass, upto[n - 1], u, sh, reinterpret_cast<uint64_t*>(upto), tokens + r, logp + r);
     else open = mx;
   } else {
@@ -693,13 +679,24 @@ __global__ void row_uniforms_kernel(unsigned long long seed, unsigned long long 
   out[i] = 1.f - curand_uniform(&st);                      // (0, 1] -> [0, 1)
 }
 
+// Filters of every row's own send a part of the rows on, which twice the blocks finish sooner: 250 x 50 021 floats, a third of them, 78 / 69 / 70 us in all with 1 / 2 / 4;
+// where all rows come, 256 x 151 936, 258 / 268 / 311.  Of more than 1024 rows a third fill the SMs, and
+// several blocks would want 19 KB of scratch a row.
+template <typename T>
+int long_blocks(int rows, int V, const SampleFilters& f) {
+  const int blocks = row_blocks(rows, V, LogitRow<T>::N);
+  const bool own = f.top_k != nullptr || f.top_p != nullptr || f.min_p != nullptr || f.temperature != nullptr;
+  return own && rows <= 1024 ? std::min(2 * blocks, kRowClusterMax) : blocks;
+}
+
 template <typename T>
 cudaError_t launch_sample(const void* logits, long row_stride, int rows, int V, const float* uniforms, const SampleFilters& f, int* tokens, float* logp,
-                          float* top, cudaStream_t s) {
+                          float* top, void* scratch, cudaStream_t s) {
   static PerDevice<bool> done, done_long;
   if (const cudaError_t e = allow_smem(done, sample_filtered_kernel<T>, kRowChunks * kRowThreads * 4); e != cudaSuccess) return e;
   if (const cudaError_t e = allow_smem(done_long, sample_long_kernel<T>, (kBins + 2) * kRowThreads * 4); e != cudaSuccess) return e;
-  const int blocks = row_blocks(rows, V, LogitRow<T>::N);
+  const int blocks = row_blocks(rows, V, LogitRow<T>::N), more = long_blocks<T>(rows, V, f);
+  unsigned char* const mails = static_cast<unsigned char*>(scratch);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = blocks;
@@ -712,15 +709,13 @@ cudaError_t launch_sample(const void* logits, long row_stride, int rows, int V, 
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   const T* z = static_cast<const T*>(logits);
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_filtered_kernel<T>, z, row_stride, V, uniforms, f, tokens, logp, top);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_filtered_kernel<T>, z, row_stride, V, uniforms, f, tokens, logp, top, mails, row_mail_bytes(blocks));
   if (e != cudaSuccess || top == nullptr) return e;
   cfg.dynamicSmemBytes = (kBins + 2) * kRowThreads * 4;
-  // Filters of every row's own send a part of the rows on, which twice the blocks finish sooner: 250 x 50 021 floats, a third of them, 71 / 63 / 61 us in all with 1 / 2 / 4,
-  // 700 rows 118 / 105 / 118, 64 x 151 936 115 / 84 / 77; where all rows come, 256 x 151 936, 258 / 268 / 311.
-  const int more = f.top_k != nullptr || f.top_p != nullptr || f.min_p != nullptr || f.temperature != nullptr ? std::min(2 * blocks, kRowClusterMax) : blocks;
   attr[0].val.clusterDim.x = more;
   cfg.gridDim = dim3(static_cast<unsigned>(rows) * more);
-  return cudaLaunchKernelEx(&cfg, sample_long_kernel<T>, z, row_stride, V, uniforms, f, static_cast<const float*>(top), tokens, logp);
+  return cudaLaunchKernelEx(&cfg, sample_long_kernel<T>, z, row_stride, V, uniforms, f, static_cast<const float*>(top), tokens, logp, mails,
+                            row_mail_bytes(more));
 }
 
 }  // namespace nrl
@@ -733,12 +728,18 @@ extern "C" int nrl_sample_is_short(const SampleFilters* f, int V) {
   return greedy || (f->top_k == nullptr && f->top_k_all > 0 && f->top_k_all <= kTopMax && f->top_k_all < V);
 }
 
+extern "C" size_t nrl_sample_scratch(int is_bf16, int rows, int V, const SampleFilters* f) {
+  const int blocks = row_blocks(rows, V, is_bf16 ? LogitRow<__nv_bfloat16>::N : LogitRow<float>::N);
+  const int more = nrl_sample_is_short(f, V) ? blocks : is_bf16 ? long_blocks<__nv_bfloat16>(rows, V, *f) : long_blocks<float>(rows, V, *f);
+  return rows * row_mail_bytes(std::max(blocks, more));    // one after the other
+}
+
 extern "C" cudaError_t nrl_sample_filtered(const void* logits, int is_bf16, long row_stride, int rows, int V, const float* uniforms, const SampleFilters* f,
-                                           int* tokens, float* logp, float* top, cudaStream_t s) {
+                                           int* tokens, float* logp, float* top, void* scratch, cudaStream_t s) {
   if (rows == 0) return cudaSuccess;
   if (top == nullptr && !nrl_sample_is_short(f, V)) return cudaErrorInvalidValue;
-  return is_bf16 ? launch_sample<__nv_bfloat16>(logits, row_stride, rows, V, uniforms, *f, tokens, logp, top, s)
-                 : launch_sample<float>(logits, row_stride, rows, V, uniforms, *f, tokens, logp, top, s);
+  return is_bf16 ? launch_sample<__nv_bfloat16>(logits, row_stride, rows, V, uniforms, *f, tokens, logp, top, scratch, s)
+                 : launch_sample<float>(logits, row_stride, rows, V, uniforms, *f, tokens, logp, top, scratch, s);
 }
 
 extern "C" cudaError_t nrl_row_uniforms(unsigned long long seed, unsigned long long step, const int* row_ids, const int* row_steps, int rows, float* out,

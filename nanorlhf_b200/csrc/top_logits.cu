@@ -16,9 +16,8 @@ namespace nrl {
 struct TopShared {
   BorderShared border;
   RowList list;
-  float2 part[kRowClusterMax][kRowWarps];                // maximum and sum of every warp of the cluster
+  float2 part[kRowWarps];                                // maximum and sum of every warp
   BoundShared bound;
-  int base;
   float log_sum;
 };
 
@@ -47,14 +46,14 @@ __device__ __noinline__ void top_by_border(const LogitRow<T>& row, int k, double
 
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads, 3) top_logprobs_kernel(const T* __restrict__ logits, long row_stride, int V, int k, double inv_temp,
-                                                                      float* __restrict__ logp, int* __restrict__ idx) {
+                                                                      float* __restrict__ logp, int* __restrict__ idx, unsigned char* mails, size_t mail_bytes) {
   extern __shared__ __align__(16) float s_chunk[];       // [chunks][kRowThreads]; then what sorting takes
   static_assert(kCandidates * 8 <= kRowChunks * kRowThreads * 4, "in the place of the maxima");
   __shared__ TopShared sh;
   const int rank = static_cast<int>(cluster_rank()), blocks = static_cast<int>(cluster_blocks()), tid = threadIdx.x;
   const long r = blockIdx.x / blocks;
-  if (tid == 0) sh.list.n = sh.list.nhits = sh.list.sent = 0;
-  if (blocks > 1) cluster_arrive();                      // the first block's memory may be written once it is known to run
+  RowMail* const mail = reinterpret_cast<RowMail*>(mails + r * mail_bytes);        // of several blocks
+  if (tid == 0) sh.list.n = sh.list.nhits = 0;
   const LogitRow<T> row(logits + r * row_stride, V);
   const RowShare share(row.nvec, rank, blocks);
   const float c = log2_scale(inv_temp);
@@ -71,46 +70,32 @@ __global__ void __launch_bounds__(kRowThreads, 3) top_logprobs_kernel(const T* _
       for (int i = g; i < share.chunks; i += groups) x = fmaxf(x, s_chunk[i * kRowThreads + tid]);
       keys[g] = order_key(x);
     }
-  const float mw = warp_max(m);
-  const float sw = warp_sum(s * ex2((m - mw) * c));        // where an infinite logit makes this NaN, the row is looked through again
+  const float2 state = block_state(m, s, c, sh.part);    // where an infinite logit makes this NaN, the row is looked through again
   const uint32_t bound = group_bound(keys, groups, k, sh.bound);
   gather_candidates(row, share, s_chunk, bound, sh.list);
-  if (blocks > 1) cluster_wait();
-  if (lane_id() == 0) {
-    const uint32_t there = in_block(&sh.part[rank][tid >> 5], 0);
-    st_block(there, mw);
-    st_block(there + 4, sw);
-  }
-  if (rank != 0) send_candidates(sh.list, &sh.base);
-  __syncwarp();
+  float top = state.x;
+  double sum = state.y;
   if (blocks > 1) {
+    if (tid == 0) mail->part[rank] = state;
+    if (rank != 0) send_candidates(sh.list, rank, *mail);
+    __syncwarp();
     cluster_arrive();
     cluster_wait();
     if (rank != 0) return;
-  } else {
-    __syncthreads();
+    const float2 p = (tid & 31) < blocks ? __ldcg(&mail->part[tid & 31]) : make_float2(-INFINITY, 0.f);
+    top = warp_max(p.x);
+    sum = warp_sum(static_cast<double>((tid & 31) < blocks ? p.y * ex2((p.x - top) * c) : 0.f));
   }
-
-  int found = join_candidates(sh.list), n = min(k, found);
+  int found = join_candidates(sh.list, blocks, mail), n = min(k, found);
   bool infinite = false;
   for (int i = tid; i < found && i < kCandidates; i += kRowThreads) infinite |= sh.list.cand[i] >> 32 == 0xff800000u;
-  float top = -INFINITY;
-  for (int i = tid & 31; i < blocks * kRowWarps; i += 32) top = fmaxf(top, sh.part[i / kRowWarps][i % kRowWarps].x);
-  top = warp_max(top);
   if (found > kCandidates || __syncthreads_or(infinite)) {
-    double sum;
     top_by_border(row, k, inv_temp, top, sh, sum, n);
     found = n;
     if (tid == 0) sh.log_sum = static_cast<float>(log(sum));
     __syncthreads();
-  } else if (tid >= kRowThreads - 32) {                  // the last warp, while the others rank
-    double sum = 0.0;
-    for (int i = tid & 31; i < blocks * kRowWarps; i += 32) {
-      const float2 p = sh.part[i / kRowWarps][i % kRowWarps];
-      sum += p.y * ex2((p.x - top) * c);
-    }
-    sum = warp_sum(sum);
-    if ((tid & 31) == 0) sh.log_sum = logf(static_cast<float>(sum));       // half a step of it: 5e-7; the double one takes as long as the ranking
+  } else if (tid == kRowThreads - 1) {                   // while the others rank
+    sh.log_sum = logf(static_cast<float>(sum));          // half a step of it: 5e-7; the double one takes as long as the ranking
   }
   in_order(sh.list.cand, found, n, reinterpret_cast<uint64_t*>(s_chunk), sh.list.counts, [&](int place, uint64_t x) {
     const float z = key_logit(static_cast<uint32_t>(x >> 32));
@@ -124,9 +109,15 @@ __global__ void __launch_bounds__(kRowThreads, 3) top_logprobs_kernel(const T* _
 }
 
 template <typename T>
-cudaError_t launch_top(const void* logits, long row_stride, int rows, int V, int k, double inv_temp, float* logp, int* idx, cudaStream_t s) {
+int top_blocks(int rows, int V, int k) {
   int blocks = row_blocks(rows, V, LogitRow<T>::N);
   while (blocks > 1 && blocks * k * 3 / 2 > kCandidates) blocks /= 2;        // every block of a row brings about k candidates
+  return blocks;
+}
+
+template <typename T>
+cudaError_t launch_top(const void* logits, long row_stride, int rows, int V, int k, double inv_temp, float* logp, int* idx, void* mails, cudaStream_t s) {
+  const int blocks = top_blocks<T>(rows, V, k);
   static PerDevice<bool> done;
   if (const cudaError_t e = allow_smem(done, top_logprobs_kernel<T>, kRowChunks * kRowThreads * 4); e != cudaSuccess) return e;
   cudaLaunchAttribute attr[1];
@@ -140,16 +131,21 @@ cudaError_t launch_top(const void* logits, long row_stride, int rows, int V, int
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, top_logprobs_kernel<T>, static_cast<const T*>(logits), row_stride, V, k, inv_temp, logp, idx);
+  return cudaLaunchKernelEx(&cfg, top_logprobs_kernel<T>, static_cast<const T*>(logits), row_stride, V, k, inv_temp, logp, idx, static_cast<unsigned char*>(mails),
+                            row_mail_bytes(blocks));
 }
 
 }  // namespace nrl
 
 using namespace nrl;
 
+extern "C" size_t nrl_top_scratch(int is_bf16, int rows, int V, int k) {
+  return rows * row_mail_bytes(is_bf16 ? top_blocks<__nv_bfloat16>(rows, V, k) : top_blocks<float>(rows, V, k));
+}
+
 extern "C" cudaError_t nrl_top_logprobs(const void* logits, int is_bf16, long row_stride, int rows, int V, int k, double inv_temp, float* logp, int* idx,
-                                        cudaStream_t s) {
+                                        void* scratch, cudaStream_t s) {
   if (rows == 0) return cudaSuccess;
-  return is_bf16 ? launch_top<__nv_bfloat16>(logits, row_stride, rows, V, k, inv_temp, logp, idx, s)
-                 : launch_top<float>(logits, row_stride, rows, V, k, inv_temp, logp, idx, s);
+  return is_bf16 ? launch_top<__nv_bfloat16>(logits, row_stride, rows, V, k, inv_temp, logp, idx, scratch, s)
+                 : launch_top<float>(logits, row_stride, rows, V, k, inv_temp, logp, idx, scratch, s);
 }
