@@ -170,8 +170,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
   double others = state.y, psum = 0.0, top = 0.0;
   if (blocks > 1) {
     const float2 p = lane < blocks ? __ldcg(&parts[r * blocks + lane]) : make_float2(-INFINITY, 0.f);
-    mx = warp_max(p.x);
-    others = warp_sum(static_cast<double>(lane < blocks ? p.y * ex2((p.x - mx) * c) : 0.f));
+    join_states(p.x, p.y, c, mx, others);
   }
   for (int i = lane; i < K; i += 32)
     if (sh.p[i] >= 0.0) {

@@ -504,35 +504,30 @@ NRL_DEVICE void gather_candidates(const LogitRow<T>& row, const RowShare& share,
 
 // A row's memory where several blocks share it; behind it the candidates of all blocks but the first, kCandidates each.
 struct RowMail {
-  float2 part[kRowClusterMax];                         // a block's largest logit and its sum of 2^((z - m) c)
+  uint4 part[kRowClusterMax];                          // a block's largest logit, its sum of 2^((z - m) c), how many candidates it brings, and their bound
   double whole[kRowClusterMax], mass[kRowClusterMax][kRowWarps];
   float4 edges;
   float bins[kRowClusterMax][36];
-  int n[kRowClusterMax];
-  uint32_t bound[kRowClusterMax];
   NRL_DEVICE uint64_t* list(int rank) { return reinterpret_cast<uint64_t*>(this + 1) + (rank - 1) * kCandidates; }
 };
 static_assert(sizeof(RowMail) % 16 == 0, "lists on 16 bytes");
 inline size_t row_mail_bytes(int blocks) { return blocks > 1 ? sizeof(RowMail) + static_cast<size_t>(blocks - 1) * kCandidates * 8 : 0; }
 
-// In front of the barrier: this block's list for the first.
-NRL_DEVICE void send_candidates(const RowList& list, int rank, RowMail& mail) {
-  const int n = list.nhits > kCandidates ? kCandidates + 1 : list.n;
-  if (threadIdx.x == 0) mail.n[rank] = n;
+// In front of the barrier: what this block has, and its list for the first.
+NRL_DEVICE void send_candidates(const RowList& list, int rank, float2 state, uint32_t bound, RowMail& mail) {
+  const int n = list.nhits > kCandidates || list.n > kCandidates ? kCandidates + 1 : list.n;
+  if (threadIdx.x == 0) mail.part[rank] = make_uint4(__float_as_uint(state.x), __float_as_uint(state.y), n, bound);
+  if (rank == 0) return;
   uint64_t* to = mail.list(rank);
   for (int i = threadIdx.x; i < min(n, kCandidates); i += kRowThreads) to[i] = list.cand[i];
 }
-// Behind it, the first block: all lists in its own; returns how many there are, above kCandidates where they do not fit.
-NRL_DEVICE int join_candidates(RowList& list, int blocks, RowMail* mail) {
-  int all = list.nhits > kCandidates ? kCandidates + 1 : list.n;
-  if (blocks == 1) return all;
+// Behind it, the first block: part[q] in lane q of every warp, all lists in its own; returns how many candidates there are, above kCandidates where they do not fit.
+NRL_DEVICE int join_candidates(RowList& list, int blocks, RowMail* mail, uint4& part) {
+  part = static_cast<int>(lane_id()) < blocks ? __ldcg(&mail->part[lane_id()]) : make_uint4(0xff800000u, 0, 0, 0);
   int n[kRowClusterMax];                               // up to and with a block's
 #pragma unroll
-  for (int q = 1; q < kRowClusterMax; ++q) n[q] = q < blocks ? __ldcg(&mail->n[q]) : 0;
-  n[0] = all;
-#pragma unroll
-  for (int q = 1; q < kRowClusterMax; ++q) n[q] = min(n[q], kCandidates + 1) + n[q - 1];
-  all = n[kRowClusterMax - 1];
+  for (int q = 0; q < kRowClusterMax; ++q) n[q] = (q > 0 ? n[q - 1] : 0) + __shfl_sync(0xffffffffu, static_cast<int>(part.z), q);
+  const int all = n[kRowClusterMax - 1];
   if (all > kCandidates) return all;
   for (int i = n[0] + threadIdx.x; i < all; i += kRowThreads) {        // of all blocks at once
     int q = 1, first = n[0];
@@ -547,6 +542,12 @@ NRL_DEVICE int join_candidates(RowList& list, int blocks, RowMail* mail) {
   __syncthreads();
   return all;
 }
+NRL_DEVICE int candidates_of(const RowList& list) { return list.nhits > kCandidates ? kCandidates + 1 : list.n; }
+// the row's largest logit and its sum of 2^((z - m) c), from those of its blocks
+NRL_DEVICE void join_states(float m, float s, float c, float& largest, double& sum) {
+  largest = warp_max(m);
+  sum = warp_sum(static_cast<double>(s > 0.f ? s * ex2((m - largest) * c) : s));        // (a NaN stays one)
+}
 
 // The block's largest logit and sum of 2^((z - m) c) from its threads'; every thread gets them.  `part`: kRowWarps entries that nobody else uses.
 NRL_DEVICE float2 block_state(float m, float s, float c, float2* part) {
@@ -558,31 +559,36 @@ NRL_DEVICE float2 block_state(float m, float s, float c, float2* part) {
   return make_float2(mb, warp_sum(lane_id() < kRowWarps ? p.y * ex2((p.x - mb) * c) : 0.f));
 }
 
-// How many of the different numbers x[0 .. n) are above `mine`; x lies on 16 bytes and x[n] .. x[n + 7] are 0
-NRL_DEVICE int count_above(const uint64_t* x, int n, uint64_t mine) {
+// The place of a number among the n <= kRowThreads different ones x[0 .. n) in descending order, by counting those above it: `mine` of a number that some threads count
+// together, up to eight each (55 numbers 2100 -> 1000 cycles); the first of them gets the place, the others n.  x lies on 16 bytes; x[n] .. x[n + 63] are overwritten.
+NRL_DEVICE int place_of(uint64_t* x, int n, uint64_t& mine) {
+  const int tid = threadIdx.x, lg = n <= kRowThreads / 8 ? 3 : n <= kRowThreads / 4 ? 2 : n <= kRowThreads / 2 ? 1 : 0, part = tid & ((1 << lg) - 1);
+  if (tid < 64) x[n + tid] = 0;
+  __syncthreads();
+  mine = x[min(tid >> lg, n)];
   int above = 0;
+  const int end = (tid & ~31) >> lg < n ? n : 0;           // (the warps that have none leave the others the time)
 #pragma unroll 1
-  for (int j = 0; j < n; j += 8) {
+  for (int j = 2 * part; j < end; j += 8 << lg) {
     ulonglong2 y[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = *reinterpret_cast<const ulonglong2*>(x + j + 2 * i);
+    for (int i = 0; i < 4; ++i) y[i] = *reinterpret_cast<const ulonglong2*>(x + j + (2 * i << lg));
 #pragma unroll
     for (int i = 0; i < 4; ++i) above += (y[i].x > mine ? 1 : 0) + (y[i].y > mine ? 1 : 0);
   }
-  return above;
+  for (int o = 1; o < 1 << lg; o <<= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+  __syncthreads();
+  return tid >> lg < n && part == 0 ? above : n;
 }
-// x[0 .. n) in descending order, n <= kCandidates, all different (the 32 high bits need not be); the eight entries behind them may be overwritten; y: room for as many.  Up to one a thread, every
-// thread counts where its own belongs: 75 numbers 700 cycles, by exchanges 7000.  More go to 512 buckets by equal ranges of their high bits first, and are counted
+// x[0 .. n) in descending order, n <= kCandidates, all different (the 32 high bits need not be); the 64 entries behind them may be overwritten; y: room for as many.  Up to one a thread, places are
+// counted: by exchanges 7000 cycles.  More go to 512 buckets by equal ranges of their high bits first, and are counted
 // within theirs: 1358 numbers of five logits 25 000 cycles, by exchanges 30 000, and 6000 where few are of one logit.
 NRL_DEVICE void sort_front(uint64_t* x, int n, uint64_t* y, SortCounts& sc) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (n <= kRowThreads) {
-    if (tid < 8) x[n + tid] = 0;
-    __syncthreads();
-    const uint64_t mine = x[min(tid, n)];
-    const int place = tid < n ? count_above(x, n, mine) : 0;
-    __syncthreads();
-    if (tid < n) x[place] = mine;
+    uint64_t mine;
+    const int place = place_of(x, n, mine);
+    if (place < n) x[place] = mine;
     __syncthreads();
     return;
   }
@@ -639,11 +645,8 @@ template <class F>
 NRL_DEVICE void in_order(uint64_t* x, int found, int n, uint64_t* y, SortCounts& sc, F&& f) {
   const int tid = threadIdx.x;
   if (found <= kRowThreads) {
-    if (tid < 8) x[found + tid] = 0;
-    __syncthreads();
-    const uint64_t mine = x[min(tid, found)];
-    const int before = tid < found ? count_above(x, found, mine) : n;
-    __syncthreads();
+    uint64_t mine;
+    const int before = place_of(x, found, mine);
     if (before < n) f(before, mine);
     return;
   }

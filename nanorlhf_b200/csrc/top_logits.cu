@@ -75,18 +75,18 @@ __global__ void __launch_bounds__(kRowThreads, 3) top_logprobs_kernel(const T* _
   gather_candidates(row, share, s_chunk, bound, sh.list);
   float top = state.x;
   double sum = state.y;
+  int found = candidates_of(sh.list);
   if (blocks > 1) {
-    if (tid == 0) mail->part[rank] = state;
-    if (rank != 0) send_candidates(sh.list, rank, *mail);
+    send_candidates(sh.list, rank, state, bound, *mail);
     __syncwarp();
     cluster_arrive();
     cluster_wait();
     if (rank != 0) return;
-    const float2 p = (tid & 31) < blocks ? __ldcg(&mail->part[tid & 31]) : make_float2(-INFINITY, 0.f);
-    top = warp_max(p.x);
-    sum = warp_sum(static_cast<double>((tid & 31) < blocks ? p.y * ex2((p.x - top) * c) : 0.f));
+    uint4 part;
+    found = join_candidates(sh.list, blocks, mail, part);
+    join_states(__uint_as_float(part.x), __uint_as_float(part.y), c, top, sum);
   }
-  int found = join_candidates(sh.list, blocks, mail), n = min(k, found);
+  int n = min(k, found);
   bool infinite = false;
   for (int i = tid; i < found && i < kCandidates; i += kRowThreads) infinite |= sh.list.cand[i] >> 32 == 0xff800000u;
   if (found > kCandidates || __syncthreads_or(infinite)) {
