@@ -130,13 +130,27 @@ def test_sampling_with_filters_of_every_row(B, V, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("B", [15, 30, 100, 200])          # eight, four, two blocks a row and one
+@pytest.mark.parametrize("B", [15, 30, 100, 200])          # four, two blocks a row and one
 @pytest.mark.parametrize("pattern", ["normal", "peaked", "ties"])
 def test_sampling_of_many_kept_tokens(pattern, B, dtype):
     """nuclei of most of the vocabulary, no filters, and more tokens above min_p than are sorted"""
     z = _logits(pattern, B, 80000, dtype, seed=2)
     u = torch.rand(B, generator=_gen(B), device=DEV)
     for kw in (dict(), dict(top_p=0.97), dict(temperature=1.5, top_p=0.6), dict(min_p=0.05), dict(min_p=0.01, top_p=0.9)):
+        _same_draws(z, u, **kw)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("B", [8, 100])
+@pytest.mark.parametrize("lift", [-8.0, 8.0, -math.inf])
+def test_nuclei_of_rows_whose_fourth_is_unlike_the_rest(lift, B, dtype):
+    """512 vectors of 32 bytes out of every 2048 lie elsewhere than the others, or have no mass: threads' chunks and warps' ranges of very different masses"""
+    V = 151936
+    z = _logits("normal", B, V, dtype, seed=3)
+    part = torch.arange(V, device=DEV) // (512 * 32 // z.element_size()) % 4 == 0
+    z = torch.where(part, z + lift, z)
+    u = torch.rand(B, generator=_gen(B), device=DEV)
+    for kw in (dict(top_p=0.95), dict(top_p=0.5), dict(top_p=1e-3), dict(top_p=0.9999), dict(min_p=1e-4, top_p=0.9)):
         _same_draws(z, u, **kw)
 
 
