@@ -12,6 +12,11 @@
 // bit map in shared memory knows: taken as 1 - sum q_k it would have no digits left where the student is sure.  r below 2^-24, which float32 log-probabilities
 // cannot tell from 0, counts as 0, and as 2^-24 under a logarithm.
 // An entry whose index is not a token (-1) is skipped; entries of one token add up.
+//
+// Bytes bound it: logits read, gradients written; the second pass reads from L2 what the first has brought there, and forms the exponentials again, since a row of
+// them would not fit beside two other rows.  2048 x 151 936 bf16, K = 64, forward and backward: 295 us, 4.2 TB/s, where a copy's rate would take 190; issue slots 66 %,
+// special functions 56 %.  4011 rows of floats with gradients in bf16: 844 us, 4.3 TB/s.  Tried without gain: two blocks an SM, vectors fetched a step ahead in
+// registers, the next row fetched into L2, rows that start one behind the other.
 #include <algorithm>
 #include <type_traits>
 

@@ -8,6 +8,10 @@
 // top_k-th largest of the threads' maxima, or the largest logit + T ln min_p -- picks the chunks that are read again, and the candidates that they hold are sorted
 // and filtered exactly.  A nucleus without other filters needs the mass of the whole row as well: the pass adds it up in float, and where what is known of its error
 // leaves the nucleus' last token open, or the candidates do not reach it, the row is left to a second kernel, as are rows without filters.
+//
+// 1024 x 151 936 bf16, top-k 50 and top-p 0.95: 98 us, 3.2 TB/s, where a copy's rate would take 48: of a row's 72 000 cycles on an SM that it shares with two others
+// the reads take 50 000, the wait for the last warp and the bound 6700, candidates 5200, sorting, filtering and drawing 5000; and 1024 rows are 2.3 rounds of three
+// on every SM (888 rows 78 us).  One row: 13 us by four blocks.
 #include <curand_kernel.h>
 
 #include <algorithm>
@@ -222,6 +226,8 @@ struct RowMass {
 // model.  (2) One pass in double: what lies above that range, for every warp's range of the row, and altogether; the tokens inside are gathered.  (3) The first
 // block sorts those, finds the last kept token, and walks through the range of the row that holds the drawn mass.  What does not work out (many tokens of one
 // logit) is left to sample_by_border: then false.
+// 256 x 151 936 bf16, top-p 0.95 of logits of deviation 0.6: 227 us, of which 45 the kernel in front; 25 instructions an element for each pass in float and 31 for the
+// one in double fill the issue slots to 67 %; 108 SMs have two rows and 40 one.  A first look at a fourth of the row in place of the first pass: 234.
 template <typename T>
 NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx, double u, int rank, int blocks, uint32_t* s_hist, LongShared& sh,
                             RowMail* mail, int* out_token, float* out_logp) {

@@ -6,6 +6,10 @@
 // tokens reach, and few more do (k of G groups: about G ln(G / (G - k)) tokens): the chunks whose maximum reaches it are read again, and what reaches it there
 // are the candidates.  Every block of a row's cluster sends its own to the first, which ranks them.  Rows with more candidates than fit (many ties, a sorted
 // vocabulary) and rows with an infinite logit are looked through for the border itself, eight ranges of keys a pass.
+//
+// 2048 x 151 936 bf16, k = 64: 166 us, 3.8 TB/s, where a copy's rate would take 95.  The pass alone takes 105 -- 8.4 instructions an element, one of them a special
+// function, fill the issue slots to 65 % -- and a row's chain behind it, of which two other rows on the SM hide a part, the rest: waiting for the last warp 3900 cycles,
+// the bound 2100, candidates 5000 (two reads, one behind the other), ranks 2300, of 63 000.  One row: 10.6 us by four blocks.
 #include "common.cuh"
 #include "logit_rows.cuh"
 #include "per_device.h"

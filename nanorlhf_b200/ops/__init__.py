@@ -191,7 +191,7 @@ def distill_loss(logits, top_logp, top_idx, weights=None, temperature: float = 1
     the teacher's K probabilities to a sum of 1 instead, and compares them with q as it is.
     ``weights`` [T]: share of every token (a mask over its sum; None: 1 / T each); a row of weight 0 is not read, its loss and gradient are 0.  Put constant
     factors (gradient accumulation) in there: the gradient is formed in the forward, and a backward from 1 hands it on as it is.
-    Entries of ``top_idx`` outside [0, V) are skipped, entries of one token add up; no entries and a tail: loss 0."""
+    Entries of ``top_idx`` outside [0, V) are skipped, entries of one token add up; no entries and a tail: loss 0.  V <= 2^20 on CUDA; no second derivative."""
     if logits.dim() != 2:
         raise ValueError(f"distill_loss: logits must be [T, V], got {tuple(logits.shape)}")
     _check_teacher("distill_loss", logits.shape[0], top_logp, top_idx, weights, temperature, float(beta), tail)
@@ -202,7 +202,7 @@ def distill_loss(logits, top_logp, top_idx, weights=None, temperature: float = 1
 
 def lmhead_distill_loss(hidden, weight, top_logp, top_idx, weights=None, temperature: float = 1.0, beta: float = 0.0, tail: bool = True):
     """``distill_loss`` of the logits ``hidden @ weight.T`` ([T, H], [V, H], bf16), which are formed in float32 and never handed over; gradients with
-    respect to ``hidden`` and ``weight``.  T may be any: what is held at a time does not grow with it."""
+    respect to ``hidden`` and ``weight``, formed in the forward.  T may be any: at most 4 GiB of logits and half as much of their gradients are held at a time."""
     if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1]:
         raise ValueError(f"lmhead_distill_loss: hidden [T, H] and weight [V, H] are needed, got {tuple(hidden.shape)} and {tuple(weight.shape)}")
     _check_teacher("lmhead_distill_loss", hidden.shape[0], top_logp, top_idx, weights, temperature, float(beta), tail)
