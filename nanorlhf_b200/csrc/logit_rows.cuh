@@ -462,6 +462,14 @@ struct RowList {
   };
   int n, nhits;
 };
+// x[j], out of registers
+template <int N>
+NRL_DEVICE float pick(const float (&x)[N], int j) {
+  float z = x[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) z = i == j ? x[i] : z;
+  return z;
+}
 // Into `list` all elements of the share whose keys reach `bound`: the chunks that have any (by their maxima) are read again, a vector a thread.  list.n and
 // list.nhits are 0 before; above kCandidates they say that there is more than what the list holds.
 template <typename T>
@@ -496,7 +504,7 @@ NRL_DEVICE void gather_candidates(const LogitRow<T>& row, const RowShare& share,
     for (int j = 0; j < LogitRow<T>::N; ++j) in |= (order_key(clean(x[j])) >= bound ? 1u : 0u) << j;
     for (int at = atomicAdd(&list.n, __popc(in)); in != 0 && at < kCandidates; in &= in - 1, ++at) {
       const int e = v * LogitRow<T>::N - row.skew + __ffs(in) - 1;
-      list.cand[at] = static_cast<uint64_t>(order_key(row.at(e))) << 32 | static_cast<uint32_t>(~e);
+      list.cand[at] = static_cast<uint64_t>(order_key(pick(x, __ffs(in) - 1))) << 32 | static_cast<uint32_t>(~e);
     }
   }
   __syncthreads();
