@@ -142,7 +142,9 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
       }
     }
   });
-  const float2 state = block_state(m, mass, c, sh.part);
+  put_state(m, mass, c, sh.part);
+  __syncthreads();
+  const float2 state = get_state(c, sh.part);
   if (blocks > 1) {
     if (tid == 0) parts[r * blocks + rank] = state;
     __syncwarp();

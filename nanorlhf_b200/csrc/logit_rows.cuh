@@ -557,11 +557,12 @@ NRL_DEVICE void join_states(float m, float s, float c, float& largest, double& s
   sum = warp_sum(static_cast<double>(s > 0.f ? s * ex2((m - largest) * c) : s));        // (a NaN stays one)
 }
 
-// The block's largest logit and sum of 2^((z - m) c) from its threads'; every thread gets them.  `part`: kRowWarps entries that nobody else uses.
-NRL_DEVICE float2 block_state(float m, float s, float c, float2* part) {
+// The block's largest logit and sum of 2^((z - m) c) from its threads': put_state, a barrier, get_state, which every thread may call.  `part`: kRowWarps entries.
+NRL_DEVICE void put_state(float m, float s, float c, float2* part) {
   const float mw = warp_max(m), sw = warp_sum(s * ex2((m - mw) * c));
   if (lane_id() == 0) part[threadIdx.x >> 5] = make_float2(mw, sw);
-  __syncthreads();
+}
+NRL_DEVICE float2 get_state(float c, const float2* part) {
   const float2 p = part[lane_id() % kRowWarps];
   const float mb = warp_max(p.x);
   return make_float2(mb, warp_sum(lane_id() < kRowWarps ? p.y * ex2((p.x - mb) * c) : 0.f));

@@ -661,6 +661,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) sample_filtered_kernel(const T
   // a thread's chunks in one group up to 256 tokens, in up to four above
   const int want = few ? (f.top_k > 0 && f.top_k <= kTopMax ? f.top_k : 0) : kNucleusGroups, groups = want <= 256 ? 1 : want <= 512 ? 2 : 4;
   uint32_t bound = kKeyNone + 1;
+  put_state(nucleus ? m : best, s, c, sh.part);            // (without a nucleus the sum is 0)
   if (few || nucleus) {
     if (want > 0) {
       uint32_t keys[kGroupsMax];
@@ -680,8 +681,10 @@ __global__ void __launch_bounds__(kRowThreads, 3) sample_filtered_kernel(const T
       if (z > -3e38 && z < 3e38) bound = max(bound, order_key(static_cast<float>(z)));
     }
     gather_candidates(row, share, s_chunk, bound, sh.list);
+  } else {
+    __syncthreads();
   }
-  const float2 state = block_state(nucleus ? m : best, s, c, sh.part);        // (without a nucleus the sum is 0)
+  const float2 state = get_state(c, sh.part);
   float mx = state.x;
   double whole = state.y;
   uint32_t least = bound;

@@ -74,9 +74,10 @@ __global__ void __launch_bounds__(kRowThreads, 3) top_logprobs_kernel(const T* _
       for (int i = g; i < share.chunks; i += groups) x = fmaxf(x, s_chunk[i * kRowThreads + tid]);
       keys[g] = order_key(x);
     }
-  const float2 state = block_state(m, s, c, sh.part);    // where an infinite logit makes this NaN, the row is looked through again
+  put_state(m, s, c, sh.part);                           // where an infinite logit makes this NaN, the row is looked through again
   const uint32_t bound = group_bound(keys, groups, k, sh.bound);
   gather_candidates(row, share, s_chunk, bound, sh.list);
+  const float2 state = get_state(c, sh.part);
   float top = state.x;
   double sum = state.y;
   int found = candidates_of(sh.list);
