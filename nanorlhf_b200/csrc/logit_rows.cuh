@@ -302,25 +302,29 @@ NRL_DEVICE void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.
 NRL_DEVICE void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // Blocks of a cluster tell each other what they found through memory of the call's own, written before a barrier at which all arrive and read behind it, past the L1.
 constexpr int kRowClusterMax = 4;
-constexpr int kRowUnroll = 2;                          // vectors of a thread in flight
+// Vectors of a thread in flight where two blocks share an SM (that what a block does behind its pass hides the other's reads needs many bytes under way).  us with 4, with 3 and
+// three blocks, with 2 and three: top 64 of 2048 x 151 936 bf16 136 / 141 / 160, of 148 rows 16.4 / 18.7 / 22.9, sampling with top-k 50 of 1024 rows 86 / 92 / 99, top 200 of 777
+// x 50 021 floats 58.3 / 61.1 / 57.9; with 6 and two blocks 157 / 18.8 / 88 / 64.
+constexpr int kFlight = 4;
 constexpr int kRowChunks = 16;                         // of a thread's vectors, each with a maximum of its own
 
 // The vectors of this block: thread t has first + t, first + t + kRowThreads, ..., in `chunks` chunks of `len`.
 struct RowShare {
   int first, end, len, chunks;
-  NRL_DEVICE RowShare(int nvec, int rank, int blocks) {
+  NRL_DEVICE RowShare(int nvec, int rank, int blocks, int flight) {       // flight: vectors of a thread in flight
     const int per = (nvec + blocks - 1) / blocks;
     first = min(nvec, rank * per);
     end = min(nvec, first + per);
     const int steps = (end - first + kRowThreads - 1) / kRowThreads;
-    len = (steps + kRowChunks * kRowUnroll - 1) / (kRowChunks * kRowUnroll) * kRowUnroll;
+    len = (steps + kRowChunks * flight - 1) / (kRowChunks * flight) * flight;
     chunks = len > 0 ? (steps + len - 1) / len : 0;
   }
 };
 // Blocks of a row's cluster (host).  A row of its own block is fastest where the rows fill the SMs; of few rows the cluster shares the reading, until its barrier and
-// the way through memory cost more.  us with 1 / 2 / 4 / 8 blocks of bf16 rows of 151 936, top 20: 1 row 15.4 / 12.4 / 11.1 / 10.9, 32 rows 16.1 / 13.5 / 11.6 / 14.1, 64
-// rows 16.3 / 13.8 / 14.7 / 23.2, 100 rows 16.6 / 17.5 / 18.2 / 30.6, 300 rows 34 / 40 / 50 / 79; sampling with top-k 50: 1 row 15.2 / 14.4 / 14.3 / 17.3, 64 rows
-// 16.0 / 16.0 / 19.2 / 35.  With 1 / 2 blocks, top 20 of 32 000 floats: 1 row 7.7 / 8.3, 64 rows 7.9 / 9.3.
+// the way through memory cost more.  us with 1 / 2 / 4 blocks of rows of 151 936, top 20 of bf16: 1 row 12.1 / 10.9 / 9.9, 32 rows 12.8 / 11.8 / 10.5, 64 rows 12.9 /
+// 12.1 / 14.0, 100 rows 13.2 / 16.6 / 20.6; sampling with top-k 50 of floats: 1 row 18.5 / 14.8 / 13.2, 64 rows 18.9 / 15.7 / 16.9, of bf16, where the reads are the
+// smaller part, 11.0 / 11.4 / 11.8 and 11.4 / 12.4 / 15.8; without filters 1 row of bf16 49 / 35 / 28, 64 rows 52 / 37 / 44.  Of 32 000 floats with 1 / 2, top 20: 1 row
+// 6.8 / 7.5, 64 rows 7.3 / 8.3.
 inline int row_blocks(long rows, int V, int vec) {
   constexpr int kSms = 148;
   const long nvec = V / vec;
@@ -330,9 +334,9 @@ inline int row_blocks(long rows, int V, int vec) {
 }
 
 // One pass over the block's share: thread-wise maximum `best`, sum s of 2^((z - m) c), m = best or the lowest float, and the maximum of every chunk.  The sum's reference moves with the
-// maximum, once for the kRowUnroll vectors of a step.  z - m is formed before the multiplication: m c would round at the size of the logits.
+// maximum, once for the FLIGHT vectors of a step.  z - m is formed before the multiplication: m c would round at the size of the logits.
 // skip(v, a) may take elements of vector v out of the sum by making them -infinity.  chunk_max may be null.  SUM false: the maxima alone.
-template <bool SUM = true, typename T, class S>
+template <int FLIGHT, bool SUM = true, typename T, class S>
 NRL_DEVICE void row_pass(const LogitRow<T>& row, const RowShare& sh, float c, float* chunk_max, float& best, float& m, float& s, S&& skip) {
   m = -3.402823466e38f;                                // finite, so that -infinity is 0 in the sum
   s = 0.f;
@@ -341,23 +345,23 @@ NRL_DEVICE void row_pass(const LogitRow<T>& row, const RowShare& sh, float c, fl
   for (int i = 0; i < sh.chunks; ++i) {
     float cm = -INFINITY;
     const int v0 = sh.first + i * sh.len * kRowThreads + static_cast<int>(threadIdx.x);
-    for (int u = 0; u < sh.len; u += kRowUnroll) {
-      RawVec a[kRowUnroll];
+    for (int u = 0; u < sh.len; u += FLIGHT) {
+      RawVec a[FLIGHT];
 #pragma unroll
-      for (int j = 0; j < kRowUnroll; ++j) {
+      for (int j = 0; j < FLIGHT; ++j) {
         const int v = v0 + (u + j) * kRowThreads;
         a[j] = v < sh.end ? row.raw(v) : LogitRow<T>::no_vec();
       }
       float l = LogitRow<T>::largest(a[0]);
 #pragma unroll
-      for (int j = 1; j < kRowUnroll; ++j) l = fmaxf(l, LogitRow<T>::largest(a[j]));
+      for (int j = 1; j < FLIGHT; ++j) l = fmaxf(l, LogitRow<T>::largest(a[j]));
       cm = fmaxf(cm, l);
       if constexpr (!SUM) continue;
       const float mn = fmaxf(m, l);
       const uint64_t neg = pair_both(-mn);
       uint64_t sum = 0;
 #pragma unroll
-      for (int j = 0; j < kRowUnroll; ++j) {
+      for (int j = 0; j < FLIGHT; ++j) {
         skip(v0 + (u + j) * kRowThreads, a[j]);
 #pragma unroll
         for (int q = 0; q < LogitRow<T>::N / 2; ++q) {

@@ -9,9 +9,9 @@
 // and filtered exactly.  A nucleus without other filters needs the mass of the whole row as well: the pass adds it up in float, and where what is known of its error
 // leaves the nucleus' last token open, or the candidates do not reach it, the row is left to a second kernel, as are rows without filters.
 //
-// 1024 x 151 936 bf16, top-k 50 and top-p 0.95: 98 us, 3.2 TB/s, where a copy's rate would take 48: of a row's 72 000 cycles on an SM that it shares with two others
-// the reads take 50 000, the wait for the last warp and the bound 6700, candidates 5200, sorting, filtering and drawing 5000; and 1024 rows are 2.3 rounds of three
-// on every SM (888 rows 78 us).  One row: 13 us by four blocks.
+// 1024 x 151 936 bf16, top-k 50 and top-p 0.95: 86 us, 3.6 TB/s, where a copy's rate would take 48: half of a row's time on an SM, which it shares with another, is the
+// chain behind its reads (the wait for the last warp and the bound, candidates by two reads, sorting, filtering, drawing: 5000 cycles each at most), and 1024 rows are
+// 3.5 rounds of 296 (2664 rows 198 us).  One row: 11.6 us by four blocks.
 #include <curand_kernel.h>
 
 #include <algorithm>
@@ -45,10 +45,10 @@ struct RowFilter {
   NRL_DEVICE double mass(float z, float mx) const { return z == mx ? 1.0 : exp((static_cast<double>(z) - mx) * inv_temp); }
 };
 
-// The float sum of 2^x of a row is off by so much of itself at most, in units of 2^-24: 30 for a step's terms and for joining threads, warps and blocks; for every step of a
-// thread, of 512 x 16 elements at least, 3 of its additions and 4 of 2^x where the reference moves; 4 of 2^x; 3 of every exponent, whose mean over the mass is
+// The float sum of 2^x of a row is off by so much of itself at most, in units of 2^-24: 50 for a step's terms and for joining threads, warps and blocks; for every step of a
+// thread, of 512 x 32 elements at least, 3 of its additions and 4 of 2^x where the reference moves; 4 of 2^x; 3 of every exponent, whose mean over the mass is
 // log2 V <= 31, times ln 2.
-NRL_DEVICE double sum_error(int V) { return (100.0 + V / 1100.0) * 0x1p-24; }
+NRL_DEVICE double sum_error(int V) { return (120.0 + V / 2300.0) * 0x1p-24; }
 
 struct SampleShared {
   BorderShared border;
@@ -226,14 +226,14 @@ struct RowMass {
 // model.  (2) One pass in double: what lies above that range, for every warp's range of the row, and altogether; the tokens inside are gathered.  (3) The first
 // block sorts those, finds the last kept token, and walks through the range of the row that holds the drawn mass.  What does not work out (many tokens of one
 // logit) is left to sample_by_border: then false.
-// 256 x 151 936 bf16, top-p 0.95 of logits of deviation 0.6: 227 us, of which 45 the kernel in front; 25 instructions an element for each pass in float and 31 for the
+// 256 x 151 936 bf16, top-p 0.95 of logits of deviation 0.6: 222 us, of which 40 the kernel in front; 25 instructions an element for each pass in float and 31 for the
 // one in double fill the issue slots to 67 %; 108 SMs have two rows and 40 one.  A first look at a fourth of the row in place of the first pass: 234.
 template <typename T>
 NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx, double u, int rank, int blocks, uint32_t* s_hist, LongShared& sh,
                             RowMail* mail, int* out_token, float* out_logp) {
   constexpr int N = LogitRow<T>::N;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const RowShare share(row.nvec, rank, blocks);
+  const RowShare share(row.nvec, rank, blocks, 1);
   const float c = log2_scale(f.inv_temp);
   if (tid < 128) sh.powers[tid] = exp2(tid / 128.0);
   const RowMass mass(f, mx, sh.powers);
@@ -446,7 +446,7 @@ NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx
     if (base > target) break;
   }
   if (range < 0) return false;
-  const RowShare there(row.nvec, range / kRowWarps, blocks);
+  const RowShare there(row.nvec, range / kRowWarps, blocks, 1);
   const int tper = (there.end - there.first + kRowWarps - 1) / kRowWarps, t0 = min(there.end, there.first + range % kRowWarps * tper), t1 = min(there.end, t0 + tper);
   if (tid == 0) {
     sh.token = -1;
@@ -588,7 +588,7 @@ NRL_DEVICE void draw_of(uint64_t* x, int n, const double* mass, double total, do
 }
 
 // Both in one warp, for up to 64 sorted candidates that hold all that is kept: 1024 x 151 936 with top-k 50 and top-p 0.95 102 us by
-// the block and 99 by a warp, one row 14.7 / 13.0.
+// the block and 99 by a warp, one row 14.7 / 13.0 (with two vectors a thread in flight).
 constexpr int kDrawWarp = 64;
 NRL_DEVICE void draw_in_warp(const uint64_t* x, int n1, const RowFilter& f, float mx, double u, double* mass, int* out_token, float* out_logp) {
   const int lane = threadIdx.x & 31;
@@ -637,7 +637,7 @@ NRL_DEVICE void draw_in_warp(const uint64_t* x, int n1, const RowFilter& f, floa
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads, 3) sample_filtered_kernel(const T* __restrict__ logits, long row_stride, int V,
+__global__ void __launch_bounds__(kRowThreads, 2) sample_filtered_kernel(const T* __restrict__ logits, long row_stride, int V,
                                                                          const float* __restrict__ uniforms, SampleFilters filters, int* __restrict__ tokens,
                                                                          float* __restrict__ logp, float* __restrict__ top, unsigned char* mails, size_t mail_bytes) {
   extern __shared__ __align__(16) float s_chunk[];         // [chunks][kRowThreads]
@@ -649,15 +649,15 @@ __global__ void __launch_bounds__(kRowThreads, 3) sample_filtered_kernel(const T
   RowMail* const mail = reinterpret_cast<RowMail*>(mails + r * mail_bytes);        // of several blocks
   const LogitRow<T> row(logits + r * row_stride, V);
   const RowFilter f(filters, r, V);
-  const RowShare share(row.nvec, rank, blocks);
+  const RowShare share(row.nvec, rank, blocks, kFlight);
   const bool few = (f.top_k > 0 && f.top_k <= kTopMax) || f.min_p > 0.0;        // what is kept is a matter of the candidates alone
   const bool nucleus = !few && f.top_p < 1.0 && f.top_k == 0;
   const float c = log2_scale(f.inv_temp);
   float best, m = 0.f, s = 0.f;
   if (nucleus)
-    row_pass<true>(row, share, c, s_chunk, best, m, s, [](int, RawVec& a) { LogitRow<T>::drop_nan(a); });
+    row_pass<kFlight, true>(row, share, c, s_chunk, best, m, s, [](int, RawVec& a) { LogitRow<T>::drop_nan(a); });
   else
-    row_pass<false>(row, share, c, s_chunk, best, m, s, [](int, const RawVec&) {});
+    row_pass<kFlight, false>(row, share, c, s_chunk, best, m, s, [](int, const RawVec&) {});
   // a thread's chunks in one group up to 256 tokens, in up to four above
   const int want = few ? (f.top_k > 0 && f.top_k <= kTopMax ? f.top_k : 0) : kNucleusGroups, groups = want <= 256 ? 1 : want <= 512 ? 2 : 4;
   uint32_t bound = kKeyNone + 1;

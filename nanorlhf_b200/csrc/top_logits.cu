@@ -7,9 +7,9 @@
 // are the candidates.  Every block of a row's cluster sends its own to the first, which ranks them.  Rows with more candidates than fit (many ties, a sorted
 // vocabulary) and rows with an infinite logit are looked through for the border itself, eight ranges of keys a pass.
 //
-// 2048 x 151 936 bf16, k = 64: 166 us, 3.8 TB/s, where a copy's rate would take 95.  The pass alone takes 105 -- 8.4 instructions an element, one of them a special
-// function, fill the issue slots to 65 % -- and a row's chain behind it, of which two other rows on the SM hide a part, the rest: waiting for the last warp 3900 cycles,
-// the bound 2100, candidates 5000 (two reads, one behind the other), ranks 2300, of 63 000.  One row: 10.6 us by four blocks.
+// 2048 x 151 936 bf16, k = 64: 140 us, 4.5 TB/s, where a copy's rate would take 95.  What keeps it from that is bytes under way: two blocks of an SM read four vectors a
+// thread at a time, and while one waits for its last warp, finds the bound, reads the candidates (two reads, one behind the other) and ranks them -- 13 000 cycles of
+// a row -- the other reads alone.  One row: 9.8 us by four blocks.
 #include "common.cuh"
 #include "logit_rows.cuh"
 #include "per_device.h"
@@ -49,7 +49,7 @@ __device__ __noinline__ void top_by_border(const LogitRow<T>& row, int k, double
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads, 3) top_logprobs_kernel(const T* __restrict__ logits, long row_stride, int V, int k, double inv_temp,
+__global__ void __launch_bounds__(kRowThreads, 2) top_logprobs_kernel(const T* __restrict__ logits, long row_stride, int V, int k, double inv_temp,
                                                                       float* __restrict__ logp, int* __restrict__ idx, unsigned char* mails, size_t mail_bytes) {
   extern __shared__ __align__(16) float s_chunk[];       // [chunks][kRowThreads]; then what sorting takes
   static_assert(kCandidates * 8 <= kRowChunks * kRowThreads * 4, "in the place of the maxima");
@@ -59,10 +59,10 @@ __global__ void __launch_bounds__(kRowThreads, 3) top_logprobs_kernel(const T* _
   RowMail* const mail = reinterpret_cast<RowMail*>(mails + r * mail_bytes);        // of several blocks
   if (tid == 0) sh.list.n = sh.list.nhits = 0;
   const LogitRow<T> row(logits + r * row_stride, V);
-  const RowShare share(row.nvec, rank, blocks);
+  const RowShare share(row.nvec, rank, blocks, kFlight);
   const float c = log2_scale(inv_temp);
   float best, m, s;
-  row_pass(row, share, c, s_chunk, best, m, s, [](int, const RawVec&) {});
+  row_pass<kFlight>(row, share, c, s_chunk, best, m, s, [](int, const RawVec&) {});
   // a thread's chunks in one group up to k = 256, in up to four above
   const int groups = k <= 256 ? 1 : k <= 512 ? 2 : 4;
   uint32_t keys[kGroupsMax];
