@@ -86,3 +86,22 @@ def test_settings():
     from nanorlhf_b200.config import RLConfig
     a = RLConfig()
     assert a.top_k == 0 and a.min_p == 0.0
+
+
+@pytest.mark.parametrize("kw", [dict(top_k=40), dict(min_p=0.05)])
+def test_trainer_does_not_score_with_the_nucleus_what_other_filters_cut(tmp_path, kw):
+    from nanorlhf_b200.config import RLConfig
+    from nanorlhf_b200.reward.api import LengthReward
+    from nanorlhf_b200.trainer import ReinforceTrainer
+    from nanorlhf_b200.utils.data import synthetic_hh_dataset
+    from nanorlhf_b200.utils.tokenizer import ByteTokenizer
+
+    tok = ByteTokenizer()
+    cfg = Qwen2Config.tiny(vocab_size=tok.vocab_size)
+    models = [Qwen2ForCausalLM.from_config(cfg, torch.float32, seed=1) for _ in range(2)]
+    base = dict(output_dir=str(tmp_path), response_length=4, per_device_train_batch_size=2, gradient_accumulation_steps=2, num_mini_batches=2, total_episodes=8,
+                learning_rate=1e-3, sampler="torch", report_to="none", **kw)
+    data = synthetic_hh_dataset(tok, 8, max_prompt_tokens=8)
+    ReinforceTrainer(RLConfig(**base), tok, *models, data, reward_func=LengthReward(3))
+    with pytest.raises(ValueError, match="logprob_top_p_consistent"):
+        ReinforceTrainer(RLConfig(**base, logprob_top_p_consistent=True), tok, *models, data, reward_func=LengthReward(3))
