@@ -220,6 +220,13 @@ struct RowMass {
   }
 };
 
+// *addr += x in shared memory that no other thread uses
+NRL_DEVICE void add_shared(uint32_t addr, float x) {
+  float y;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(y) : "r"(addr) : "memory");
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(y + x) : "memory");
+}
+
 // ---- the long way -------------------------------------------------------------------------------------------------------------------------------
 // Rows of which many tokens are kept: a nucleus of more than fit, or all.  The blocks of a cluster share a row.  (1) Where a nucleus ends is narrowed down by passes in
 // float that add up the mass of 32 ranges of logits, every lane for itself in shared memory, until one range holds few tokens: two passes for the logits of an untrained
@@ -270,18 +277,21 @@ NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx
     for (int pass = 0; pass < 6 && !enough; ++pass) {
 #pragma unroll 8
       for (int i = 0; i < kBins + 2; ++i) mine[i * 32] = 0;
-      // 2^23 and, rounded to whole numbers there, the number of the range: 0 above them, 1 .. kBins, kBins + 1 below
-      const float scale = -kBins / fmaxf(edge - low, 1e-30f), zero = 8388608.f, half = edge - 0.5f / scale;
+      // The number of a logit's range -- 0 above them, 1 .. kBins, kBins + 1 below -- is (edge + half a range - z) / (kBins + 1) ranges, held within 0 and 1, times kBins + 1 and
+      // rounded, which the addition of 2^23 does; its bits shifted to a range's 128 bytes, less 2^23's, which leave 2^31 there.
+      const float per = 1.f / fmaxf((edge - low) * ((kBins + 1.f) / kBins), 1e-30f), zero = (edge + (edge - low) * (0.5f / kBins)) * per;
+      const uint32_t bins = smem_u32(mine) - 0x80000000u;
+      const uint64_t neg2 = pair_both(-mx), c2 = pair_both(c);
 #pragma unroll 1
       for (int v = share.first + tid; v < share.end; v += kRowThreads) {
-        float x[N];
-        row.load(v, x);
+        RawVec a = row.raw(v);
+        LogitRow<T>::drop_nan(a);
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const float z = fmaxf(x[j], -3e38f);             // NaN have no mass
-          const float t = fminf(fmaxf(fmaf(z - half, scale, zero), zero), zero + (kBins + 1));
-          uint32_t* const bin = mine + (__float_as_uint(t) & 63u) * 32;
-          *bin = __float_as_uint(__uint_as_float(*bin) + ex2((z - mx) * c));
+        for (int q = 0; q < N / 2; ++q) {
+          const uint64_t z = LogitRow<T>::pair(a, q);
+          const float2 x = pair_parts(z), e = pair_parts(pair_mul(pair_add(z, neg2), c2));
+          add_shared(bins + (__float_as_uint(fmaf(__saturatef(fmaf(x.x, -per, zero)), kBins + 1.f, 8388608.f)) << 7), ex2(e.x));
+          add_shared(bins + (__float_as_uint(fmaf(__saturatef(fmaf(x.y, -per, zero)), kBins + 1.f, 8388608.f)) << 7), ex2(e.y));
         }
       }
       __syncthreads();
