@@ -233,8 +233,9 @@ NRL_DEVICE void add_shared(uint32_t addr, float x) {
 // model.  (2) One pass in double: what lies above that range, for every warp's range of the row, and altogether; the tokens inside are gathered.  (3) The first
 // block sorts those, finds the last kept token, and walks through the range of the row that holds the drawn mass.  What does not work out (many tokens of one
 // logit) is left to sample_by_border: then false.
-// 256 x 151 936 bf16, top-p 0.95 of logits of deviation 0.6: 222 us, of which 40 the kernel in front; 25 instructions an element for each pass in float and 31 for the
-// one in double fill the issue slots to 67 %; 108 SMs have two rows and 40 one.  A first look at a fourth of the row in place of the first pass: 234.
+// 256 x 151 936 bf16, top-p 0.95 of logits of deviation 0.6: 215 us, of which 40 the kernel in front; 19 instructions an element for each pass in float and 31 for the
+// one in double fill the issue slots to 62 %; 108 SMs have two rows and 40 one.  A first look at a fourth of the row in place of the first pass, and vectors fetched
+// one ahead, gave nothing.
 template <typename T>
 NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx, double u, int rank, int blocks, uint32_t* s_hist, LongShared& sh,
                             RowMail* mail, int* out_token, float* out_logp) {
@@ -752,7 +753,8 @@ __global__ void row_uniforms_kernel(unsigned long long seed, unsigned long long 
   out[i] = 1.f - curand_uniform(&st);                      // (0, 1] -> [0, 1)
 }
 
-// Filters of every row's own send a part of the rows on, which twice the blocks finish sooner: 250 x 50 021 floats, a third of them, 78 / 69 / 70 us in all with 1 / 2 / 4;
+// Filters of every row's own send a part of the rows on, which twice the blocks finish sooner: 250 x 50 021 floats, a third of them, 78 / 69 / 70 us in all with 1 / 2 / 4
+// (before ranges took 19 instructions);
 // where all rows come, 256 x 151 936, 258 / 268 / 311.  Of more than 1024 rows a third fill the SMs, and
 // several blocks would want 19 KB of scratch a row.
 template <typename T>
