@@ -31,11 +31,11 @@ struct RowFilter {
     top_p = f.top_p ? f.top_p[r] : f.top_p_all;
     min_p = f.min_p ? f.min_p[r] : f.min_p_all;
     top_k = f.top_k ? f.top_k[r] : f.top_k_all;
-    if (!(temp > 0.0)) {                                   // the first of the order, which has log-probability 0 among itself
-      temp = 1.0;
+    if (top_k < 0 || top_k >= V) top_k = 0;
+    if (!(temp > 0.0)) {                                   // the first of the order, which has log-probability 0 among itself; also of one column, or a call
+      temp = 1.0;                                          // that is greedy altogether would leave its rows to a second kernel which it does not launch
       top_k = 1;
     }
-    if (top_k < 0 || top_k >= V) top_k = 0;
     if (!(min_p > 0.0)) min_p = 0.0;
     if (min_p > 1.0) min_p = 1.0;
     if (!(top_p < 1.0)) top_p = 1.0;
