@@ -9,8 +9,10 @@
 // vocabulary: the factor is 1.
 //
 // A divergence is the small difference of large terms, so everything about the K + 1 events is in double.  s is summed over the tokens off K alone, which a
-// bit map in shared memory knows: taken as 1 - sum q_k it would have no digits left where the student is sure.  r below 2^-24, which float32 log-probabilities
-// cannot tell from 0, counts as 0, and as 2^-24 under a logarithm.
+// bit map in shared memory knows: taken as 1 - sum q_k it would have no digits left where the student is sure.  The sum is relative to the largest logit off K,
+// m, since relative to the row's it would be 0 in float from 87 temperatures between the two on: s = S exp((m - max z) / tau) / total, of which the logarithm is
+// taken in parts, and dL/dz_v tau = e_v (exp((m - max z) / tau) / total - r / S) off K with e_v = exp((z_v - m) / tau).
+// r below 2^-24, which float32 log-probabilities cannot tell from 0, counts as 0, and as 2^-24 under a logarithm.
 // An entry whose index is not a token (-1) is skipped; entries of one token add up.
 //
 // Bytes bound it: logits read, gradients written; the second pass reads from L2 what the first has brought there, and forms the exponentials again, since a row of
@@ -58,6 +60,7 @@ struct DistillShared {
   float2 part[kRowWarps];                                  // maximum and sum of every warp
   double red[2][kRowWarps];
   int twins;                                               // some token has several entries
+  uint32_t top;                                            // key of the tokens' largest logit
 };
 
 NRL_DEVICE void block_sum_two(double& x, double& y, double (&red)[2][kRowWarps]) {
@@ -114,7 +117,10 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
     return;
   }
   // ---- the teacher's entries, and where they lie in the share ----
-  if (tid == 0) sh.twins = 0;
+  if (tid == 0) {
+    sh.twins = 0;
+    sh.top = kKeyNone;
+  }
   __syncthreads();
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
@@ -128,7 +134,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
   }
   __syncthreads();
 
-  // ---- the row's maximum, and its mass off the teacher's tokens ----
+  // ---- off the teacher's tokens: the largest logit, and the mass relative to it ----
   const float c = log2_scale(inv_temp);
   const auto* map = reinterpret_cast<const std::conditional_t<N == 16, uint16_t, uint8_t>*>(s_map);
   float best, m, mass;
@@ -173,16 +179,18 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
     }
     sh.p[i] = p;
     sh.z[i] = LogitRow<T>::value(z);
+    if (at >= 0) atomicMax(&sh.top, order_key(clean(sh.z[i])));
   }
   __syncwarp();
   if (blocks > 1) cluster_wait();
   __syncthreads();
-  float mx = state.x;
-  double others = state.y, psum = 0.0, top = 0.0;
+  float high = state.x;                                    // the largest off K
+  double sum = state.y, psum = 0.0, top = 0.0;
   if (blocks > 1) {
     const float2 p = lane < blocks ? __ldcg(&parts[r * blocks + lane]) : make_float2(-INFINITY, 0.f);
-    join_states(p.x, p.y, c, mx, others);
+    join_states(p.x, p.y, c, high, sum);
   }
+  const float mx = fmaxf(high, key_logit(sh.top));         // the largest of all
   for (int i = lane; i < K; i += 32)
     if (sh.p[i] >= 0.0) {
       psum += sh.p[i];
@@ -190,22 +198,24 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
     }
   psum = warp_sum(psum);
   top = warp_sum(top);
+  const auto below = [&] { return high == mx ? 0.0 : (static_cast<double>(high) - mx) * inv_temp; };        // (formed where it is wanted: registers)
+  const double shrink = beta == 0.0 ? ex2((high - mx) * c) : exp(below());        // (float beside the float sum of `top`; the loss forms its own)
 
   // ---- the K + 1 events ----
-  double rr = 1.0 - psum, off = 1.0, mean = 0.0, total = top + others;         // off: factor of q off K
+  double rr = 1.0 - psum, mean = 0.0, total = top + sum * shrink, off;         // off: factor of e_v off K
   if (!(rr > kNoTail)) rr = 0.0;
   const bool teacher = tail || psum > 0.0;
   if (beta == 0.0) {
-    if (tail) off = others > 0.0 ? 1.0 - rr / others * total : 0.0;
-    else if (!teacher) off = 0.0;
+    off = !teacher ? 0.0 : shrink / total;
+    if (tail && sum != 0.0) off -= rr / sum;
   } else {
     double loss = 0.0, none = 0.0;
     top = 0.0;
     for (int i = tid; i < K; i += kRowThreads)
       if (sh.p[i] >= 0.0) top += exp((static_cast<double>(sh.z[i]) - mx) * inv_temp);
     block_sum_two(top, none, sh.red);
-    total = top + others;
-    const double log_total = log(total), s = others / total;
+    total = top + sum * shrink;
+    const double log_total = log(total), s = sum * shrink / total;
     for (int i = tid; i < K; i += kRowThreads) {
       const double p = sh.p[i];
       if (p < 0.0) continue;
@@ -225,7 +235,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
     block_sum_two(loss, mean, sh.red);
     double d = 0.0;
     if (beta == 1.0) {
-      if (s > 0.0) d = log(s) - log(rr > 0.0 ? rr : kNoTail);
+      if (s > 0.0) d = log(sum) + below() - log_total - log(rr > 0.0 ? rr : kNoTail);
     } else {
       const double mid = beta * rr + (1.0 - beta) * s;
       if (s > 0.0) d = (1.0 - beta) * log(s / mid);
@@ -233,15 +243,15 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
     }
     loss += s * d;
     mean += s * d;
-    off = d - mean;
+    off = (d - mean) * shrink / total;
     if (tid == 0 && rank == 0) token_loss[r] = static_cast<float>(loss);
   }
 
   // ---- the gradient: off K one factor a row; the teacher's tokens are put right behind the others ----
   if (out) {
     const double g = (weights ? static_cast<double>(weight) : 1.0 / rows) * inv_temp;
-    const float f = static_cast<float>(fmin(fmax(g * off / total, -3e38), 3e38));      // finite: 0 times it is 0
-    const uint64_t c2 = pair_both(c), neg = pair_both(-mx), f2 = pair_both(f);
+    const float f = static_cast<float>(fmin(fmax(g * off, -3e38), 3e38));      // finite: 0 times it is 0
+    const uint64_t c2 = pair_both(c), neg = pair_both(-high), f2 = pair_both(f);
     // backwards: what the first pass read last is the likeliest to be in L2
 #pragma unroll 1
     for (int v = share.first + (share.end - share.first - 1) / kRowThreads * kRowThreads + tid; v >= share.first; v -= kRowThreads) {
@@ -285,9 +295,9 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
   }
   block_sum_two(mass_top, loss, sh.red);
   if (tid < 32) {                                          // three logarithms in one
-    total = mass_top + others;
-    const double l = log(lane == 0 ? total : lane == 1 ? (tail ? rr : psum) : others);
-    const double log_total = __shfl_sync(0xffffffffu, l, 0), log_r = __shfl_sync(0xffffffffu, l, 1), log_o = __shfl_sync(0xffffffffu, l, 2);
+    total = mass_top + sum * exp(below());
+    const double l = log(lane == 0 ? total : lane == 1 ? (tail ? rr : psum) : sum);
+    const double log_total = __shfl_sync(0xffffffffu, l, 0), log_r = __shfl_sync(0xffffffffu, l, 1), log_o = __shfl_sync(0xffffffffu, l, 2) + below();
     if (tail) {
       loss += psum * log_total;
       if (rr > 0.0) loss += rr * (log_r - log_o + log_total);

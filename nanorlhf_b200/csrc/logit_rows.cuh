@@ -335,7 +335,7 @@ inline int row_blocks(long rows, int V, int vec) {
 
 // One pass over the block's share: thread-wise maximum `best`, sum s of 2^((z - m) c), m = best or the lowest float, and the maximum of every chunk.  The sum's reference moves with the
 // maximum, once for the FLIGHT vectors of a step.  z - m is formed before the multiplication: m c would round at the size of the logits.
-// skip(v, a) may take elements of vector v out of the sum by making them -infinity.  chunk_max may be null.  SUM false: the maxima alone.
+// skip(v, a) may take elements of vector v out of maxima and sum by making them -infinity.  chunk_max may be null.  SUM false: the maxima alone, of all elements.
 template <int FLIGHT, bool SUM = true, typename T, class S>
 NRL_DEVICE void row_pass(const LogitRow<T>& row, const RowShare& sh, float c, float* chunk_max, float& best, float& m, float& s, S&& skip) {
   m = -3.402823466e38f;                                // finite, so that -infinity is 0 in the sum
@@ -352,6 +352,9 @@ NRL_DEVICE void row_pass(const LogitRow<T>& row, const RowShare& sh, float c, fl
         const int v = v0 + (u + j) * kRowThreads;
         a[j] = v < sh.end ? row.raw(v) : LogitRow<T>::no_vec();
       }
+      if constexpr (SUM)
+#pragma unroll
+        for (int j = 0; j < FLIGHT; ++j) skip(v0 + (u + j) * kRowThreads, a[j]);
       float l = LogitRow<T>::largest(a[0]);
 #pragma unroll
       for (int j = 1; j < FLIGHT; ++j) l = fmaxf(l, LogitRow<T>::largest(a[j]));
@@ -361,14 +364,12 @@ NRL_DEVICE void row_pass(const LogitRow<T>& row, const RowShare& sh, float c, fl
       const uint64_t neg = pair_both(-mn);
       uint64_t sum = 0;
 #pragma unroll
-      for (int j = 0; j < FLIGHT; ++j) {
-        skip(v0 + (u + j) * kRowThreads, a[j]);
+      for (int j = 0; j < FLIGHT; ++j)
 #pragma unroll
         for (int q = 0; q < LogitRow<T>::N / 2; ++q) {
           const float2 e = pair_parts(pair_mul(pair_add(LogitRow<T>::pair(a[j], q), neg), c2));
           sum = pair_add(sum, pair_of(__float_as_uint(ex2(e.x)), __float_as_uint(ex2(e.y))));
         }
-      }
       const float2 p = pair_parts(sum);
       s = s * ex2((m - mn) * c) + (p.x + p.y);
       m = mn;

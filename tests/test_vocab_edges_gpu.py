@@ -5,12 +5,14 @@ import pytest
 import torch
 
 from nanorlhf_b200 import ops
+from nanorlhf_b200.ops import reference as ref
 
 pytestmark = pytest.mark.gpu
 
 INF = math.inf
 BF16, F32 = torch.bfloat16, torch.float32
 DEV = "cuda"
+BETAS = [(0.0, True), (0.0, False), (1.0, True), (0.4, True)]
 
 
 def _gen(seed):
@@ -39,3 +41,34 @@ def test_sampling_of_one_column_is_written(T, dtype):
         _spoil()
         tok, logp = ops.sample_filtered(none, u, **kw)
         assert tok.tolist() == [-1] * T and logp.tolist() == [-INF] * T, kw
+
+
+# ---- a student that is sure --------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("beta,tail", BETAS)
+@pytest.mark.parametrize("gap,temperature", [(60.0, 0.6), (26.0, 0.25), (100.0, 1.0), (1e4, 1.0), (1e4, 0.3), (-100.0, 1.0), (-1e4, 0.5)])
+@pytest.mark.parametrize("T,V", [(5, 1000), (3, 151936), (50, 151936)])          # one, four, two blocks a row
+def test_distillation_where_the_rest_lies_far_below(T, V, gap, temperature, beta, tail, dtype):
+    """the teacher's tokens `gap` above (or below) all others: what the rest has left, relative to the row's largest logit, is beyond float's range"""
+    z = torch.randn(T, V, generator=_gen(3), device=DEV)
+    at = torch.arange(8, device=DEV) * (V // 8) + 3
+    z[:, at] += gap
+    z = z.to(dtype)
+    idx = at.int().expand(T, 8).contiguous()
+    logp = torch.log_softmax(torch.randn(T, 8, generator=_gen(4), device=DEV), -1) + math.log(0.9)
+    x, y = z.clone().requires_grad_(), z.double().requires_grad_()
+    loss, token = ops.distill_loss(x, logp, idx, None, temperature, beta, tail)
+    want, tw = ref.distill_loss(y, logp, idx, None, temperature, beta, tail)
+    loss.backward()
+    want.backward()
+    # the rest's sum is off by 5e-6 of itself at most, of which the loss has a share below one; the result is rounded to float32, and so is the one it is held against
+    assert torch.isfinite(token).all() and ((token - tw).abs() <= 5e-6 + 2.0 ** -23 * tw.abs()).all()
+    assert abs(loss.item() - want.item()) <= 5e-6 + 2.0 ** -23 * abs(want.item())
+    # gradients: half a step of their type, 5e-6 of the sum, and exponents of 10 bits where a row has its mass, three steps of 2^-24 of them: 2e-6
+    tol = (2.0 ** -8 if dtype == BF16 else 0.0) + 1e-5
+    # and where they are next to nothing, differences of logarithms up to 4e4 that are rounded to 2^-53 of themselves on either side: 1e-11 of the probabilities, which
+    # sum to 1 (times 1 / (T temperature) <= 1)
+    on = torch.zeros(V, dtype=torch.bool, device=DEV).index_fill_(0, at, True)
+    for part in (on, ~on):
+        gx, gy = x.grad[:, part].double(), y.grad[:, part]
+        assert (gx - gy).norm() <= tol * gy.norm() + 1e-11
