@@ -81,6 +81,9 @@ NRL_DEVICE void block_sum_two(double& x, double& y, double (&red)[2][kRowWarps])
 constexpr int kDistillFlight = 2;
 
 constexpr double kNoTail = 5.9604644775390625e-8;          // 2^-24
+// What is left of 1 by K <= 1024 float32 log-probabilities that sum to 1: half a step of each, 2^-24 of sum p |log p| <= log 1024, and of the row's sum that they share
+// 5e-7.  Where the student has no mass off K at all -- all its tokens are listed, or teacher and student share a mask -- that is nobody's, and no infinite divergence.
+constexpr double kNobodys = 9.5367431640625e-7;            // 2^-20
 
 // Blocks of a cluster share a row.  Beside the two passes, what a row costs is latency -- entries, barriers, double-precision logarithms -- so that is kept off
 // the way from one pass to the other: with beta = 0 every warp finds the factor for itself behind the barrier, and the loss is left for the end.
@@ -203,7 +206,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
 
   // ---- the K + 1 events ----
   double rr = 1.0 - psum, mean = 0.0, total = top + sum * shrink, off;         // off: factor of e_v off K
-  if (!(rr > kNoTail)) rr = 0.0;
+  if (!(rr > kNoTail) || (sum == 0.0 && rr <= kNobodys)) rr = 0.0;
   const bool teacher = tail || psum > 0.0;
   if (beta == 0.0) {
     off = !teacher ? 0.0 : shrink / total;

@@ -359,9 +359,9 @@ def distill_loss(logits: torch.Tensor, top_logp: torch.Tensor, top_idx: torch.Te
         P = P / torch.where(total > 0, total, 1.0)
         token = plogs(P, P.log(), lq).sum(-1)
     else:
-        r = 1.0 - total
-        r = torch.where(r > 2.0 ** -24, r, 0.0)
         none = K.all(-1, keepdim=True) | (lq.masked_fill(K, -math.inf) == -math.inf).all(-1, keepdim=True)
+        r = 1.0 - total
+        r = torch.where(r > torch.where(none, 2.0 ** -20, 2.0 ** -24), r, 0.0)          # (what rounding of log-probabilities leaves of 1 is nobody's where nobody else is)
         ls = torch.logsumexp(torch.where(none, 0.0, lq.masked_fill(K, -math.inf)), -1, keepdim=True)
         ls = torch.where(none, -math.inf, ls)
         P, lQ = torch.cat([P, r], -1), torch.cat([lq, ls], -1)

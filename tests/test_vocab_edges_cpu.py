@@ -1,0 +1,33 @@
+"""Calls of the vocabulary operators at the ends of their ranges, in their plain forms."""
+import math
+
+import pytest
+import torch
+
+from nanorlhf_b200 import ops
+
+INF = math.inf
+BETAS = [(0.0, True), (0.0, False), (1.0, True), (0.4, True)]
+
+
+@pytest.mark.parametrize("beta,tail", BETAS)
+@pytest.mark.parametrize("K", [1, 2, 6, 300, 1024])
+def test_a_teacher_who_lists_all_that_the_student_may_use(K, beta, tail):
+    """what rounding of its log-probabilities leaves of 1 is no mass that nobody has"""
+    T, V = 400, K + 50
+    g = torch.Generator().manual_seed(K)
+    teacher, z = torch.randn(T, K, generator=g), torch.randn(T, K, generator=g).double()
+    logp, idx = ops.top_logprobs(teacher, K)
+    listed = torch.log_softmax(teacher, -1)                        # another rounding
+    every = torch.arange(K, dtype=torch.int32).expand(T, K)
+    masked = torch.cat([z, torch.full((T, V - K), -INF, dtype=torch.float64)], -1)
+    for a, i in ((logp, idx), (listed, every)):
+        for x in (z, masked):
+            x = x.clone().requires_grad_()
+            loss, token = ops.distill_loss(x, a, i, beta=beta, tail=tail)
+            loss.backward()
+            assert torch.isfinite(token).all() and torch.isfinite(x.grad).all()
+            # KL >= 0, of probabilities that sum to 1 within 2^-20
+            assert (token >= -2.0 ** -20).all()
+    if beta == 0.0 and tail:                                       # more than rounding: mass where the student has none
+        assert (ops.distill_loss(masked, logp - 1e-5, idx)[1] == INF).all()

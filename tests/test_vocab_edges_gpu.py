@@ -19,6 +19,10 @@ def _gen(seed):
     return torch.Generator(device=DEV).manual_seed(seed)
 
 
+def _rel(a, b):
+    return ((a.double() - b.double()).norm() / b.double().norm().clamp(min=1e-30)).item()
+
+
 # ---- one column ------------------------------------------------------------------------------------------------------------------
 def _spoil():
     """the allocator's small blocks, which the next results lie in, hold no result of an earlier call"""
@@ -72,3 +76,25 @@ def test_distillation_where_the_rest_lies_far_below(T, V, gap, temperature, beta
     for part in (on, ~on):
         gx, gy = x.grad[:, part].double(), y.grad[:, part]
         assert (gx - gy).norm() <= tol * gy.norm() + 1e-11
+
+
+# ---- a teacher who lists all tokens ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("beta,tail", BETAS)
+@pytest.mark.parametrize("T,V,K", [(300, 6, 6), (200, 1024, 1024), (100, 5000, 300), (40, 151936, 1000), (10, 151936, 7)])
+def test_a_teacher_who_lists_all_that_the_student_may_use(T, V, K, beta, tail, dtype):
+    """what rounding of its log-probabilities leaves of 1 is no mass that nobody has"""
+    at = torch.randperm(V, generator=_gen(1), device=DEV)[:K]
+    z, t = (torch.full((T, V), -INF, device=DEV).index_copy_(1, at, torch.randn(T, K, generator=_gen(s), device=DEV)) for s in (2, 3))
+    logp, idx = ops.top_logprobs(t, K)
+    assert (idx >= 0).all()
+    x, y = z.to(dtype).clone().requires_grad_(), z.to(dtype).double().requires_grad_()
+    loss, token = ops.distill_loss(x, logp, idx, None, 1.0, beta, tail)
+    want, tw = ref.distill_loss(y, logp, idx, None, 1.0, beta, tail)
+    loss.backward()
+    want.backward()
+    # no mass but the teacher's tokens', which is double: rounded to float32 on either side
+    assert torch.isfinite(token).all() and ((token - tw).abs() <= 2.0 ** -23 * (1.0 + tw.abs())).all()
+    assert torch.isfinite(x.grad).all() and _rel(x.grad, y.grad) <= (2.0 ** -8 if dtype == BF16 else 0.0) + 5e-6
+    if beta == 0.0 and tail and K < V:                     # more than rounding: mass where the student has none
+        assert (ops.distill_loss(x.detach(), logp - 1e-5, idx)[1] == INF).all()
