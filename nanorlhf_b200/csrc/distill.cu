@@ -253,7 +253,8 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
   // ---- the gradient: off K one factor a row; the teacher's tokens are put right behind the others ----
   if (out) {
     const double g = (weights ? static_cast<double>(weight) : 1.0 / rows) * inv_temp;
-    const float f = static_cast<float>(fmin(fmax(g * off, -3e38), 3e38));      // finite: 0 times it is 0
+    const double y = g * off;
+    const float f = y == y ? static_cast<float>(fmin(fmax(y, -3e38), 3e38)) : NAN;      // 0 times a finite one is 0; what is not a number makes the row none
     const uint64_t c2 = pair_both(c), neg = pair_both(-high), f2 = pair_both(f);
     // backwards: what the first pass read last is the likeliest to be in L2
 #pragma unroll 1
@@ -280,7 +281,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
       const int bit = sh.idx[i] + row.skew - share.first * N;
       if (p < 0.0 || bit < 0 || bit >= (share.end - share.first) * N) continue;
       const double q = ex2((sh.z[i] - mx) * c) / total;
-      const double u = !teacher ? 0.0 : beta == 0.0 ? q - (tail ? p : p / psum) : q > 0.0 ? q * (sh.q[i] - mean) : 0.0;
+      const double u = !teacher ? 0.0 : beta == 0.0 ? q - (tail ? p : p / psum) : q == 0.0 ? 0.0 : q * (sh.q[i] - mean);
       out[sh.idx[i]] = static_cast<G>(static_cast<float>(g * u));
     }
   }

@@ -351,8 +351,8 @@ def distill_loss(logits: torch.Tensor, top_logp: torch.Tensor, top_idx: torch.Te
     K = torch.zeros(T, V + 1, dtype=torch.bool, device=logits.device).scatter(1, at, True)[:, :V]
     total = P.sum(-1, keepdim=True)
 
-    def plogs(p, *logs):                      # p * (logs[0] - logs[1]) where p > 0, without a gradient through what is masked
-        ok = p > 0
+    def plogs(p, *logs):                      # p * (logs[0] - logs[1]) where p is not 0, without a gradient through what is masked
+        ok = p != 0
         return torch.where(ok, torch.where(ok, p, 1.0) * (torch.where(ok, logs[0], 0.0) - torch.where(ok, logs[1], 0.0)), 0.0)
 
     if not tail:

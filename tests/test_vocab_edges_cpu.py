@@ -31,3 +31,17 @@ def test_a_teacher_who_lists_all_that_the_student_may_use(K, beta, tail):
             assert (token >= -2.0 ** -20).all()
     if beta == 0.0 and tail:                                       # more than rounding: mass where the student has none
         assert (ops.distill_loss(masked, logp - 1e-5, idx)[1] == INF).all()
+
+
+@pytest.mark.parametrize("beta,tail", BETAS)
+@pytest.mark.parametrize("bad", [math.nan, INF])
+def test_a_row_that_is_not_a_number_has_no_loss(bad, beta, tail):
+    z = torch.randn(3, 40, generator=torch.Generator().manual_seed(1))
+    idx = torch.tensor([3, 30, 7], dtype=torch.int32).expand(3, 3)
+    logp = torch.full((3, 3), 0.25).log()
+    z[1, 20] = bad                                                 # off the teacher's tokens
+    z[2, 30] = bad                                                 # one of them
+    x = z.requires_grad_()
+    loss, token = ops.distill_loss(x, logp, idx, beta=beta, tail=tail)
+    loss.backward()
+    assert loss.isnan() and token.isnan().tolist() == [False, True, True] and x.grad[1:].isnan().all() and torch.isfinite(x.grad[0]).all()

@@ -98,3 +98,27 @@ def test_a_teacher_who_lists_all_that_the_student_may_use(T, V, K, beta, tail, d
     assert torch.isfinite(x.grad).all() and _rel(x.grad, y.grad) <= (2.0 ** -8 if dtype == BF16 else 0.0) + 5e-6
     if beta == 0.0 and tail and K < V:                     # more than rounding: mass where the student has none
         assert (ops.distill_loss(x.detach(), logp - 1e-5, idx)[1] == INF).all()
+
+
+# ---- what is not a number ----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("beta,tail", BETAS)
+@pytest.mark.parametrize("bad", [math.nan, INF])
+@pytest.mark.parametrize("V", [500, 151936])
+def test_gradients_of_a_row_that_is_not_a_number(V, bad, beta, tail, dtype):
+    """are not numbers either, and those of the other rows are what they are without it"""
+    z = torch.randn(4, V, generator=_gen(1), device=DEV)
+    idx = torch.tensor([3, 40, 7], dtype=torch.int32, device=DEV).expand(4, 3).contiguous()
+    logp = torch.full((4, 3), 0.25, device=DEV).log()
+    z[1, 100] = bad                                        # off the teacher's tokens
+    z[2, 40] = bad                                         # one of them
+    x = z.to(dtype).requires_grad_()
+    loss, token = ops.distill_loss(x, logp, idx, beta=beta, tail=tail)
+    loss.backward()
+    assert loss.isnan() and token[1:3].isnan().all() and x.grad[1:3].isnan().all()
+    clean = z.detach().clone()
+    clean[1:3] = 0.0
+    y = clean.to(dtype).requires_grad_()
+    loss, want = ops.distill_loss(y, logp, idx, beta=beta, tail=tail)
+    loss.backward()
+    assert torch.equal(token[[0, 3]], want[[0, 3]]) and torch.equal(x.grad[[0, 3]], y.grad[[0, 3]])
