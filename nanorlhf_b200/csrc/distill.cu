@@ -195,19 +195,20 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
   }
   const float mx = fmaxf(high, key_logit(sh.top));         // the largest of all
   for (int i = lane; i < K; i += 32)
-    if (sh.p[i] >= 0.0) {
+    if (!(sh.p[i] < 0.0)) {
       psum += sh.p[i];
       top += ex2((sh.z[i] - mx) * c);
     }
   psum = warp_sum(psum);
   top = warp_sum(top);
+  if (psum != psum) sum = NAN;                             // a token of the teacher's that is not a number makes the row none
   const auto below = [&] { return high == mx ? 0.0 : (static_cast<double>(high) - mx) * inv_temp; };        // (formed where it is wanted: registers)
   const double shrink = beta == 0.0 ? ex2((high - mx) * c) : exp(below());        // (float beside the float sum of `top`; the loss forms its own)
 
   // ---- the K + 1 events ----
   double rr = 1.0 - psum, mean = 0.0, total = top + sum * shrink, off;         // off: factor of e_v off K
   if (!(rr > kNoTail) || (sum == 0.0 && rr <= kNobodys)) rr = 0.0;
-  const bool teacher = tail || psum > 0.0;
+  const bool teacher = tail || psum != 0.0;
   if (beta == 0.0) {
     off = !teacher ? 0.0 : shrink / total;
     if (tail && sum != 0.0) off -= rr / sum;
@@ -306,7 +307,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
       loss += psum * log_total;
       if (rr > 0.0) loss += rr * (log_r - log_o + log_total);
     } else {
-      loss = psum > 0.0 ? loss / psum - log_r + log_total : 0.0;
+      loss = psum != 0.0 ? loss / psum - log_r + log_total : 0.0;
     }
     if (lane == 0) token_loss[r] = static_cast<float>(loss);
   }

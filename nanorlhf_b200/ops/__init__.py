@@ -190,8 +190,8 @@ def distill_loss(logits, top_logp, top_idx, weights=None, temperature: float = 1
     beta = 0: KL(P | Q); beta = 1: KL(Q | P); between: beta KL(P | M) + (1 - beta) KL(Q | M), M = beta P + (1 - beta) Q.  ``tail=False`` (beta = 0) scales
     the teacher's K probabilities to a sum of 1 instead, and compares them with q as it is.
     ``weights`` [T]: share of every token (a mask over its sum; None: 1 / T each); a row of weight 0 is not read, its loss and gradient are 0.  Put constant
-    factors (gradient accumulation) in there: the gradient is formed in the forward, and a backward from 1 hands it on as it is.  A row with a NaN or +inf has
-    NaN for its loss and its gradient.
+    factors (gradient accumulation) in there: the gradient is formed in the forward, and a backward from 1 hands it on as it is.  A row with a NaN or +inf, or
+    a token of the teacher's with a NaN, has NaN for its loss and no gradient that is a number.
     Entries of ``top_idx`` outside [0, V) are skipped, entries of one token add up; no entries and a tail: loss 0.  What the teacher leaves of 1 counts as 0 below
     2^-24, and below 2^-20 where the student gives all other tokens none (with more than that KL(P | Q) is infinite).  V <= 2^20 on CUDA; no second derivative."""
     if logits.dim() != 2:

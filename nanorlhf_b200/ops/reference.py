@@ -356,12 +356,12 @@ def distill_loss(logits: torch.Tensor, top_logp: torch.Tensor, top_idx: torch.Te
         return torch.where(ok, torch.where(ok, p, 1.0) * (torch.where(ok, logs[0], 0.0) - torch.where(ok, logs[1], 0.0)), 0.0)
 
     if not tail:
-        P = P / torch.where(total > 0, total, 1.0)
+        P = P / torch.where(total != 0, total, 1.0)
         token = plogs(P, P.log(), lq).sum(-1)
     else:
         none = K.all(-1, keepdim=True) | (lq.masked_fill(K, -math.inf) == -math.inf).all(-1, keepdim=True)
         r = 1.0 - total
-        r = torch.where(r > torch.where(none, 2.0 ** -20, 2.0 ** -24), r, 0.0)          # (what rounding of log-probabilities leaves of 1 is nobody's where nobody else is)
+        r = torch.where(r <= torch.where(none, 2.0 ** -20, 2.0 ** -24), 0.0, r)          # (what rounding of log-probabilities leaves of 1 is nobody's where nobody else is)
         ls = torch.logsumexp(torch.where(none, 0.0, lq.masked_fill(K, -math.inf)), -1, keepdim=True)
         ls = torch.where(none, -math.inf, ls)
         P, lQ = torch.cat([P, r], -1), torch.cat([lq, ls], -1)
@@ -375,7 +375,7 @@ def distill_loss(logits: torch.Tensor, top_logp: torch.Tensor, top_idx: torch.Te
             token = plogs(Q, lQ, lP).sum(-1)
         else:
             M = (beta * P + (1.0 - beta) * Q)
-            lM = torch.where(M > 0, M, 1.0).log()
+            lM = torch.where(M != 0, M, 1.0).log()
             token = beta * plogs(P, P.log(), lM).sum(-1) + (1.0 - beta) * plogs(Q, lQ, lM).sum(-1)
     token = torch.where(live[:, 0], token, 0.0)
     return (token * w).sum().float(), token.detach().float()

@@ -45,3 +45,16 @@ def test_a_row_that_is_not_a_number_has_no_loss(bad, beta, tail):
     loss, token = ops.distill_loss(x, logp, idx, beta=beta, tail=tail)
     loss.backward()
     assert loss.isnan() and token.isnan().tolist() == [False, True, True] and x.grad[1:].isnan().all() and torch.isfinite(x.grad[0]).all()
+
+
+@pytest.mark.parametrize("beta,tail", BETAS)
+def test_a_teacher_that_is_not_a_number_is_not_left_out(beta, tail):
+    z = torch.randn(3, 700, generator=torch.Generator().manual_seed(1), requires_grad=True)
+    idx = torch.tensor([3, 40, 7, -1], dtype=torch.int32).expand(3, 4).contiguous()
+    logp = torch.full((3, 4), 0.2).log()
+    logp[1, 2] = math.nan
+    logp[2, 3] = math.nan                                  # of no token: skipped
+    loss, token = ops.distill_loss(z, logp, idx, beta=beta, tail=tail)
+    loss.backward()
+    assert loss.isnan() and token.isnan().tolist() == [False, True, False]
+    assert z.grad[1].isnan().all() and torch.isfinite(z.grad[[0, 2]]).all()

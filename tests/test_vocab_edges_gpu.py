@@ -122,3 +122,16 @@ def test_gradients_of_a_row_that_is_not_a_number(V, bad, beta, tail, dtype):
     loss, want = ops.distill_loss(y, logp, idx, beta=beta, tail=tail)
     loss.backward()
     assert torch.equal(token[[0, 3]], want[[0, 3]]) and torch.equal(x.grad[[0, 3]], y.grad[[0, 3]])
+
+
+@pytest.mark.parametrize("beta,tail", BETAS)
+def test_a_teacher_that_is_not_a_number_is_not_left_out(beta, tail):
+    z = torch.randn(3, 700, generator=_gen(1), device=DEV, requires_grad=True)
+    idx = torch.tensor([3, 40, 7, -1], dtype=torch.int32, device=DEV).expand(3, 4).contiguous()
+    logp = torch.full((3, 4), 0.2, device=DEV).log()
+    logp[1, 2] = math.nan
+    logp[2, 3] = math.nan                                  # of no token: skipped
+    loss, token = ops.distill_loss(z, logp, idx, beta=beta, tail=tail)
+    loss.backward()
+    assert loss.isnan() and token.isnan().tolist() == [False, True, False]
+    assert z.grad[1].isnan().all() and torch.isfinite(z.grad[[0, 2]]).all()
