@@ -66,6 +66,7 @@ struct LongShared {
   double scan[kRowWarps];
   double mass[kRowClusterMax][kRowWarps], whole[kRowClusterMax];         // kept for good and altogether, by ranges of the row
   double powers[128];
+  double kept;                                             // what min_p keeps, by float sums
   float bins[kBins + 2];                                   // what lies above them, they, and what lies below
   float4 edges;                                            // where the next ranges begin, kept for good from, open from, enough
   unsigned short place[kCandidates];
@@ -280,7 +281,10 @@ NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx
       for (int i = 0; i < kBins + 2; ++i) mine[i * 32] = 0;
       // The number of a logit's range -- 0 above them, 1 .. kBins, kBins + 1 below -- is (edge + half a range - z) / (kBins + 1) ranges, held within 0 and 1, times kBins + 1 and
       // rounded, which the addition of 2^23 does; its bits shifted to a range's 128 bytes, less 2^23's, which leave 2^31 there.
-      const float per = 1.f / fmaxf((edge - low) * ((kBins + 1.f) / kBins), 1e-30f), zero = (edge + (edge - low) * (0.5f / kBins)) * per;
+      // With min_p the first ranges hold all that it keeps: what they sum up to is the whole, in later passes as well, whose bin below has tokens that count and others that
+      // do not.  They reach a little lower, or the least logit kept would lie on the last one's edge and rounding would put its tokens on either side.
+      const float least = f.min_p > 0.0 && pass == 0 ? low - (2e-6f * (edge - low) + 1e-6f * (fabsf(edge) + fabsf(low))) : low;
+      const float per = 1.f / fmaxf((edge - least) * ((kBins + 1.f) / kBins), 1e-30f), zero = (edge + (edge - least) * (0.5f / kBins)) * per;
       const uint32_t bins = smem_u32(mine) - 0x80000000u;
       const uint64_t neg2 = pair_both(-mx), c2 = pair_both(c);
 #pragma unroll 1
@@ -316,7 +320,7 @@ NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx
         for (int q = 0; q < blocks; ++q) {
           m += blocks > 1 ? __ldcg(&mail->bins[q][lane + 1]) : sh.bins[lane + 1];
           start += blocks > 1 ? __ldcg(&mail->bins[q][0]) : sh.bins[0];
-          rest += f.min_p > 0.0 && low <= floor ? 0.0 : blocks > 1 ? __ldcg(&mail->bins[q][kBins + 1]) : sh.bins[kBins + 1];
+          rest += f.min_p > 0.0 ? 0.0 : blocks > 1 ? __ldcg(&mail->bins[q][kBins + 1]) : sh.bins[kBins + 1];
         }
         double upto = m;
 #pragma unroll
@@ -325,12 +329,16 @@ NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx
           if (lane >= o) upto += y;
         }
         upto += start;
-        const double whole = __shfl_sync(0xffffffffu, upto, 31) + rest;
+        double whole = __shfl_sync(0xffffffffu, upto, 31) + rest;
+        if (f.min_p > 0.0) {
+          if (pass > 0) whole = sh.kept;
+          else if (lane == 0) sh.kept = whole;
+        }
         // from the range in which the mass passes what the nucleus needs, less what float sums may be off by, to the one in which it passes that and as much more
         const unsigned past0 = __ballot_sync(0xffffffffu, upto >= whole * (f.top_p - kRangeSlack)), past1 = __ballot_sync(0xffffffffu, upto >= whole * (f.top_p + kRangeSlack));
         const int b0 = past0 ? __ffs(past0) - 1 : 31, b1 = past1 ? __ffs(past1) - 1 : 31;
         const double open = __shfl_sync(0xffffffffu, upto, b1) - __shfl_sync(0xffffffffu, upto - m, b0);
-        const float width = (edge - low) / kBins, over = width / 1024 + 1e-6f * (fabsf(edge) + fabsf(low));        // for the edges' rounding
+        const float width = (edge - least) / kBins, over = width / 1024 + 1e-6f * (fabsf(edge) + fabsf(low));        // for the edges' rounding
         const float e1 = b0 == 0 ? edge : edge - b0 * width + over, e0 = b1 == kBins - 1 ? low : edge - (b1 + 1) * width - over;
         const float next_high = b0 > 0 ? e1 : high, next_low = fmaxf(e0, low);
         const bool ok = open <= 1700.0 * ex2((next_low - mx) * c);        // tokens, by the least of their masses; those on the edges come on top

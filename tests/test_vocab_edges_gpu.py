@@ -23,6 +23,14 @@ def _rel(a, b):
     return ((a.double() - b.double()).norm() / b.double().norm().clamp(min=1e-30)).item()
 
 
+def _same_draws(z, u, **kw):
+    tok, logp = ops.sample_filtered(z, u, **kw)
+    want, lw = ref.sample_filtered(z, u, **kw)
+    assert torch.equal(tok, want), (tok != want).nonzero()[:8]
+    # two roundings of float32, and 2e-7 where a mass's last bits move a sum
+    assert ((logp == lw) | ((logp - lw).abs() <= 2e-7 + 2.0 ** -23 * lw.abs())).all()
+
+
 # ---- one column ------------------------------------------------------------------------------------------------------------------
 def _spoil():
     """the allocator's small blocks, which the next results lie in, hold no result of an earlier call"""
@@ -135,3 +143,29 @@ def test_a_teacher_that_is_not_a_number_is_not_left_out(beta, tail):
     loss.backward()
     assert loss.isnan() and token.isnan().tolist() == [False, True, False]
     assert z.grad[1].isnan().all() and torch.isfinite(z.grad[[0, 2]]).all()
+
+
+# ---- min-p with a nucleus ----------------------------------------------------------------------------------------------------------
+def _fastest(f, n=12):
+    times = []
+    for _ in range(n):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        f()
+        b.record()
+        b.synchronize()
+        times.append(a.elapsed_time(b))
+    return min(times)
+
+
+@pytest.mark.parametrize("rows,dtype", [(200, BF16), (60, F32), (20, BF16)])             # one, two, four blocks a row
+@pytest.mark.parametrize("std,min_p", [(0.6, 0.02), (0.6, 0.05), (0.9, 0.01)])
+def test_a_nucleus_behind_min_p_costs_what_a_nucleus_costs(std, min_p, rows, dtype):
+    """thousands of tokens above min_p: where their nucleus ends is found by the ranges that find any other nucleus' end (0.2 ms; a row looked through for its border
+    takes 1 ms), and is the definition's"""
+    z = (torch.randn(rows, 151936, generator=_gen(7), device=DEV) * std).to(dtype)
+    u = torch.rand(rows, generator=_gen(8), device=DEV)
+    for p in (0.95, 0.7):
+        _same_draws(z, u, min_p=min_p, top_p=p)
+        plain, both = _fastest(lambda: ops.sample_filtered(z, u, top_p=p)), _fastest(lambda: ops.sample_filtered(z, u, top_p=p, min_p=min_p))
+        assert both <= 2.5 * plain, (plain, both)
