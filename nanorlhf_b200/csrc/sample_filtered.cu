@@ -581,8 +581,10 @@ NRL_DEVICE int kept_of(const uint64_t* x, int found, int sure, const RowFilter& 
   return n;
 }
 
-// from the n first candidates, which are sorted, by index
-NRL_DEVICE void draw_of(uint64_t* x, int n, const double* mass, double total, double u, SampleShared& sh, uint64_t* y, int* out_token, float* out_logp) {
+// from the n first candidates, which are sorted, by index; the log-probability from the logit: the quotient of a kept mass and the whole may be below float's range
+template <typename T>
+NRL_DEVICE void draw_of(const LogitRow<T>& row, uint64_t* x, int n, const RowFilter& f, float mx, const double* mass, double total, double u, SampleShared& sh, uint64_t* y,
+                        int* out_token, float* out_logp) {
   const int tid = threadIdx.x;
   for (int i = tid; i < n; i += kRowThreads) x[i] = x[i] << 32 | static_cast<uint32_t>(i);        // (~index, place)
   sort_front(x, n, y, sh.list.counts);                               // (its first barrier is behind the swap)
@@ -600,9 +602,9 @@ NRL_DEVICE void draw_of(uint64_t* x, int n, const double* mass, double total, do
   }
   __syncthreads();
   if (tid == 0) {
-    const uint64_t y = x[min(sh.token, n - 1)];
-    *out_token = static_cast<int>(~static_cast<uint32_t>(y >> 32));
-    *out_logp = logf(static_cast<float>(mass[static_cast<uint32_t>(y)] / total));        // one step of it, and 2^-24 of the quotient
+    const int token = static_cast<int>(~static_cast<uint32_t>(x[min(sh.token, n - 1)] >> 32));
+    *out_token = token;
+    *out_logp = static_cast<float>(f.x(row.at(token), mx) - log(total));
   }
 }
 
@@ -632,7 +634,7 @@ NRL_DEVICE void draw_in_warp(const uint64_t* x, int n1, const RowFilter& f, floa
   int n = 0;                                               // (the first is kept whatever top_p says)
 #pragma unroll
   for (int t = 0; t < 2; ++t) n += __popc(__ballot_sync(0xffffffffu, w[t] > 0.0 && (before[t] < limit || (t == 0 && lane == 0))));
-  const double total = __shfl_sync(0xffffffffu, n > 32 ? upto[1] : upto[0], (n - 1) & 31), target = u * total;
+  const double total = __shfl_sync(0xffffffffu, n > 32 ? upto[1] : upto[0], (n - 1) & 31), target = u * total, log_total = log(total);
   __syncwarp();
   const uint32_t at0 = static_cast<uint32_t>(x[lane]), at1 = static_cast<uint32_t>(x[lane + 32]);        // ~index
   double a0 = 0.0, a1 = 0.0;                               // mass of the kept ones up to and with it, by index
@@ -651,7 +653,7 @@ NRL_DEVICE void draw_in_warp(const uint64_t* x, int n1, const RowFilter& f, floa
   for (int t = 0; t < 2; ++t)
     if ((t == 0 ? in0 && at0 == token : in1 && at1 == token)) {
       *out_token = static_cast<int>(~token);
-      *out_logp = logf(static_cast<float>(w[t] / total));  // one step of it, and 2^-24 of the quotient
+      *out_logp = static_cast<float>(f.x(key_logit(static_cast<uint32_t>(x[lane + t * 32] >> 32)), mx) - log_total);
     }
 }
 
@@ -743,7 +745,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_filtered_kernel(const T
       if (tid < 32) draw_in_warp(sh.list.cand, n1, f, mx, u, mass, tokens + r, logp + r);
     } else {
       const int n = kept_of(sh.list.cand, found, sure, f, mx, nucleus ? whole : 0.0, sum_error(V), mass, upto, sh);
-      if (n > 0) draw_of(sh.list.cand, n, mass, upto[n - 1], u, sh, reinterpret_cast<uint64_t*>(upto), tokens + r, logp + r);
+      if (n > 0) draw_of(row, sh.list.cand, n, f, mx, mass, upto[n - 1], u, sh, reinterpret_cast<uint64_t*>(upto), tokens + r, logp + r);
       else open = mx;
     }
   } else {

@@ -169,3 +169,15 @@ def test_a_nucleus_behind_min_p_costs_what_a_nucleus_costs(std, min_p, rows, dty
         _same_draws(z, u, min_p=min_p, top_p=p)
         plain, both = _fastest(lambda: ops.sample_filtered(z, u, top_p=p)), _fastest(lambda: ops.sample_filtered(z, u, top_p=p, min_p=min_p))
         assert both <= 2.5 * plain, (plain, both)
+
+
+# ---- a log-probability beyond float32's quotients ----------------------------------------------------------------------------------
+@pytest.mark.parametrize("kept", [2, 60, 100, 600])
+@pytest.mark.parametrize("gap", [88.0, 100.0, 200.0, 600.0])
+def test_log_probability_of_a_kept_token_of_little_mass(gap, kept):
+    """a number of 0 draws the first kept token, however little it has"""
+    z = torch.full((2, 3000), -1e30, device=DEV)
+    z[0, 5], z[0, 10:9 + kept] = 0.0, gap
+    z[1, 5], z[1, 10:9 + kept] = -gap, torch.linspace(0.0, 3.0, kept - 1, device=DEV)
+    for kw in (dict(top_k=kept), dict(top_k=kept, min_p=1e-300), dict(min_p=1e-300), dict(top_k=kept, temperature=1.1)):
+        _same_draws(z, torch.zeros(2, device=DEV), **kw)
