@@ -760,7 +760,7 @@ __global__ void row_uniforms_kernel(unsigned long long seed, unsigned long long 
   if (i >= rows) return;
   curandStatePhilox4_32_10_t st;
   curand_init(seed, static_cast<unsigned long long>(row_ids ? row_ids[i] : i), step + (row_steps ? static_cast<unsigned long long>(row_steps[i]) : 0ull), &st);
-  out[i] = 1.f - curand_uniform(&st);                      // (0, 1] -> [0, 1)
+  out[i] = fminf(1.f - curand_uniform(&st), 0x1.fffffep-1f);        // (0, 1] -> [0, 1): the difference is rounded to 1 from 2^-25 down
 }
 
 // Filters of every row's own send a part of the rows on, which twice the blocks finish sooner: 250 x 50 021 floats, a third of them, 78 / 69 / 70 us in all with 1 / 2 / 4

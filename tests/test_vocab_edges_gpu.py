@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from nanorlhf_b200 import ops
+from nanorlhf_b200.ops import native
 from nanorlhf_b200.ops import reference as ref
 
 pytestmark = pytest.mark.gpu
@@ -181,3 +182,11 @@ def test_log_probability_of_a_kept_token_of_little_mass(gap, kept):
     z[1, 5], z[1, 10:9 + kept] = -gap, torch.linspace(0.0, 3.0, kept - 1, device=DEV)
     for kw in (dict(top_k=kept), dict(top_k=kept, min_p=1e-300), dict(min_p=1e-300), dict(top_k=kept, temperature=1.1)):
         _same_draws(z, torch.zeros(2, device=DEV), **kw)
+
+
+# ---- uniform numbers ---------------------------------------------------------------------------------------------------------------
+def test_uniform_numbers_stay_below_one():
+    """of these rows, the first of seed 0 whose number is next to 1 (one in 3 * 10^7 is)"""
+    ids = torch.tensor([40657998, 66330067, 84170650, 97987152, 137839096, 1068921965], dtype=torch.int32, device=DEV)
+    assert native.row_uniforms(0, 0, ids).tolist() == [1.0 - 2.0 ** -24] * 6          # the largest float32 below 1
+    assert torch.equal(native.row_uniforms(0, 0, ids + 1).lt(1.0 - 2.0 ** -20), torch.ones(6, dtype=torch.bool, device=DEV))
