@@ -48,8 +48,9 @@ NRL_DEVICE float ex2(float x) {
   return r;
 }
 
-// logits to exponents of 2; finite, so that 0 times it is 0 at any temperature
-NRL_DEVICE float log2_scale(double inv_temp) { return static_cast<float>(fmin(inv_temp * 1.4426950408889634, 3e38)); }
+// logits to exponents of 2; finite, so that 0 times it is 0, and above 0, so that -infinity times it is none, at any temperature (from 1e45 up, where it would be 0, a
+// difference of float32 logits has an exponent below 1e-6)
+NRL_DEVICE float log2_scale(double inv_temp) { return static_cast<float>(fmin(fmax(inv_temp * 1.4426950408889634, 0x1p-149), 3e38)); }
 
 template <typename T>
 struct LogitRow {

@@ -190,3 +190,45 @@ def test_uniform_numbers_stay_below_one():
     ids = torch.tensor([40657998, 66330067, 84170650, 97987152, 137839096, 1068921965], dtype=torch.int32, device=DEV)
     assert native.row_uniforms(0, 0, ids).tolist() == [1.0 - 2.0 ** -24] * 6          # the largest float32 below 1
     assert torch.equal(native.row_uniforms(0, 0, ids + 1).lt(1.0 - 2.0 ** -20), torch.ones(6, dtype=torch.bool, device=DEV))
+
+
+# ---- temperatures ------------------------------------------------------------------------------------------------------------------
+def _rows(pattern, T, V, dtype):
+    z = torch.randn(T, V, generator=_gen(V), device=DEV)
+    if pattern == "masked":
+        z = z.masked_fill(torch.rand(T, V, generator=_gen(2), device=DEV) > 0.5, -INF)
+    return z.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("pattern", ["normal", "masked"])
+@pytest.mark.parametrize("temperature", [1e44, 1e46, 1e100, 1e300])
+@pytest.mark.parametrize("T,V", [(2, 151936), (60, 50021)])
+def test_temperatures_whose_reciprocal_is_none_of_floats(T, V, temperature, pattern, dtype):
+    """every token with mass is as probable as any other"""
+    z = _rows(pattern, T, V, dtype)
+    logp, idx = ops.top_logprobs(z, 9, temperature)
+    want, at = ref.top_logprobs(z, 9, temperature)
+    assert torch.equal(idx, at) and ((logp - want).abs() <= 5e-6 + 2.0 ** -23 * want.abs()).all()
+    u = torch.rand(T, generator=_gen(5), device=DEV)
+    for kw in (dict(), dict(top_p=0.5), dict(top_p=0.01), dict(top_k=40, top_p=0.3), dict(min_p=0.5, top_p=0.6)):
+        _same_draws(z, u, temperature=temperature, **kw)
+    if pattern == "normal":
+        x, y = z.clone().requires_grad_(), z.double().requires_grad_()
+        loss, token = ops.distill_loss(x, logp, idx, None, temperature)
+        other, tw = ref.distill_loss(y, logp, idx, None, temperature, 0.0, True)
+        loss.backward()
+        other.backward()
+        assert ((token - tw).abs() <= 5e-6).all() and (x.grad == 0).all()        # 1 / temperature of anything is below float32's least number
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("pattern", ["normal", "masked"])
+def test_an_infinite_temperature_of_a_row_is_the_largest(pattern, dtype):
+    T, V = 20, 50021
+    z = _rows(pattern, T, V, dtype)
+    u = torch.rand(T, generator=_gen(6), device=DEV)
+    hot = torch.ones(T, device=DEV)
+    hot[::2] = INF
+    for kw in (dict(), dict(top_p=0.5), dict(top_p=0.01), dict(top_k=40), dict(min_p=0.5, top_p=0.6)):
+        _same_draws(z, u, temperature=hot, **kw)
