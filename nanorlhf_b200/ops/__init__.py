@@ -204,7 +204,8 @@ def distill_loss(logits, top_logp, top_idx, weights=None, temperature: float = 1
 
 def lmhead_distill_loss(hidden, weight, top_logp, top_idx, weights=None, temperature: float = 1.0, beta: float = 0.0, tail: bool = True):
     """``distill_loss`` of the logits ``hidden @ weight.T`` ([T, H], [V, H], bf16), which are formed in float32 and never handed over; gradients with
-    respect to ``hidden`` and ``weight``, formed in the forward.  T may be any: at most 4 GiB of logits and half as much of their gradients are held at a time."""
+    respect to ``hidden`` and ``weight``, formed in the forward.  T may be any: at most 4 GiB of logits and half as much of their gradients are held at a time.  Other types,
+    and sizes that are no multiples of 8, are multiplied by torch in float32."""
     if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1]:
         raise ValueError(f"lmhead_distill_loss: hidden [T, H] and weight [V, H] are needed, got {tuple(hidden.shape)} and {tuple(weight.shape)}")
     _check_teacher("lmhead_distill_loss", hidden.shape[0], top_logp, top_idx, weights, temperature, float(beta), tail)

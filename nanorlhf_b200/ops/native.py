@@ -273,6 +273,16 @@ def distill_loss(logits, top_logp, top_idx, weights, temperature, beta, tail):
 LOGITS_BYTES = 4 << 30      # float logits of a head that are held at a time
 
 
+def _head_logits(h, weight, fused):
+    """float logits of some rows"""
+    from . import gemm as _lin
+    if not fused:
+        return F.linear(h.float(), weight.float())
+    z = torch.empty(h.shape[0], weight.shape[0], dtype=torch.float32, device=h.device)
+    _lin.gemm(h, weight, out_f32=z)
+    return z
+
+
 def _row_ranges(rows, columns):
     """as few equal ranges of rows as keep the float logits of one within LOGITS_BYTES"""
     most = max(256, LOGITS_BYTES // (4 * columns) // 256 * 256)
@@ -283,32 +293,38 @@ def _row_ranges(rows, columns):
 
 class _LmHeadDistillFn(torch.autograd.Function):
     """Logits, losses and the logits' gradients of a range of rows at a time, and with them at once the gradients of the hidden states and the head's, so that no
-    logits are formed twice: three GEMMs in all.  The backward only multiplies by the loss's own gradient."""
+    logits are formed twice: three GEMMs in all, by torch in float32 for other types and sizes than the GEMM's.  The backward only multiplies by the loss's own gradient."""
 
     @staticmethod
     def forward(ctx, hidden, weight, top_logp, top_idx, weights, temperature, beta, tail, need_h, need_w):
         from . import gemm as _lin
         h, rows, V = hidden.contiguous(), hidden.shape[0], weight.shape[0]
+        fused = _lin.supported(h, weight)
         if weights is None:
             weights = h.new_full((rows,), 1.0 / max(rows, 1), dtype=torch.float32)
-        ranges = _row_ranges(rows, V)
+        ranges = _row_ranges(rows, V if fused else V + V // 3 + 1)         # (their logits' gradients are float: both together take what the others' do)
         dh = torch.empty_like(h) if need_h else None
-        dw = torch.zeros(weight.shape, dtype=torch.float32, device=weight.device) if need_w and len(ranges) != 1 else None
+        once = fused and len(ranges) == 1                                 # dW leaves the GEMM rounded once
+        dw = torch.zeros(weight.shape, dtype=torch.float32, device=weight.device) if need_w and not once else None
         tokens = []
         for s, e in ranges:
-            z = torch.empty(e - s, V, dtype=torch.float32, device=h.device)
-            _lin.gemm(h[s:e], weight, out_f32=z)
+            z = _head_logits(h[s:e], weight, fused)
             _count()
             _, token, dz = ext().distill_loss_parts(z, top_logp[s:e], top_idx[s:e], weights[s:e], 1.0 / temperature, beta, tail,
-                                                        need_h or need_w, True, False)
+                                                        need_h or need_w, fused, False)
             tokens.append(token)
             del z
-            if need_h:
+            if need_h and fused:
                 _lin.gemm(dz, weight, b_mn=True, out=dh[s:e])
-            if need_w and len(ranges) == 1:
+            elif need_h:
+                dh[s:e] = dz @ weight.float()
+            if need_w and once:
                 dw = _lin.gemm(dz, h, a_mn=True, b_mn=True, split_k=0)
-            elif need_w:
+            elif need_w and fused:
                 _lin.gemm(dz, h[s:e], a_mn=True, b_mn=True, out_f32=dw, accumulate=True)
+            elif need_w:
+                dw.addmm_(dz.t(), h[s:e].float())
+            del dz
         token = tokens[0] if len(tokens) == 1 else torch.cat(tokens) if tokens else h.new_empty(0, dtype=torch.float32)
         _count()
         loss = ext().weighted_sum(token, weights)
@@ -325,9 +341,6 @@ class _LmHeadDistillFn(torch.autograd.Function):
 
 
 def lmhead_distill_loss(hidden, weight, top_logp, top_idx, weights, temperature, beta, tail):
-    from . import gemm as _lin
-    if not _lin.supported(hidden, weight):                 # other types and sizes than the GEMM's: their logits, in float32
-        return distill_loss(F.linear(hidden.float(), weight.float()), top_logp, top_idx, weights, temperature, beta, tail)
     top_logp, top_idx, weights = ext().teacher_entries(top_logp, top_idx, weights, weight.shape[0])
     grad = torch.is_grad_enabled()
     return _LmHeadDistillFn.apply(hidden, weight, top_logp, top_idx, weights, temperature, beta, tail, grad and hidden.requires_grad,
@@ -342,12 +355,9 @@ def lmhead_top_logprobs(hidden, weight, k, temperature):
     idx = torch.empty(rows, k, dtype=torch.int32, device=hidden.device)
     h = hidden.contiguous()
     for s, e in _row_ranges(rows, V):
-        if _lin.supported(h, weight):
-            z = torch.empty(e - s, V, dtype=torch.float32, device=h.device)
-            _lin.gemm(h[s:e], weight, out_f32=z)
-        else:
-            z = F.linear(h[s:e].float(), weight.float())
+        z = _head_logits(h[s:e], weight, _lin.supported(h, weight))
         logp[s:e], idx[s:e] = top_logprobs(z, k, temperature)
+        del z
     return logp, idx
 
 

@@ -232,3 +232,62 @@ def test_an_infinite_temperature_of_a_row_is_the_largest(pattern, dtype):
     hot[::2] = INF
     for kw in (dict(), dict(top_p=0.5), dict(top_p=0.01), dict(top_k=40), dict(min_p=0.5, top_p=0.6)):
         _same_draws(z, u, temperature=hot, **kw)
+
+
+# ---- what a head holds -------------------------------------------------------------------------------------------------------------
+def _held(f):
+    torch.cuda.synchronize()
+    start = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out = f()
+    torch.cuda.synchronize()
+    return torch.cuda.max_memory_allocated() - start, out
+
+
+@pytest.mark.parametrize("dtype,H", [(BF16, 64), (F32, 64), (BF16, 36)])
+def test_a_head_holds_no_more_than_it_says(dtype, H, monkeypatch):
+    """the float logits of one range of rows and half as much of their gradients, beside inputs, results and a float sum of the weight's gradient"""
+    T, V = 16384, 4000
+    part = 4096 * 4 * V                                    # 66 MB; all rows' logits are 262
+    monkeypatch.setattr(native, "LOGITS_BYTES", part)
+    h = torch.randn(T, H, generator=_gen(1), device=DEV).to(dtype).requires_grad_()
+    w = (torch.randn(V, H, generator=_gen(2), device=DEV) * 0.2).to(dtype).requires_grad_()
+    top = torch.full((T, 8), 0.05, device=DEV).log()
+    idx = torch.arange(8, dtype=torch.int32, device=DEV).expand(T, 8).contiguous() * 400
+    ops.lmhead_distill_loss(h[:6000], w, top[:6000], idx[:6000])[0].backward()           # (workspaces that stay)
+    h.grad = w.grad = None
+    held, (loss, token) = _held(lambda: ops.lmhead_distill_loss(h, w, top, idx))
+    # beside them: both gradients, the weight's as a float sum as well; operands in float where the type asks for it; allocations of 2 MiB at most for small things
+    beside = h.nbytes + w.nbytes + 4 * w.numel() + 4 * (h.numel() + w.numel()) + (2 << 20)
+    assert held <= 1.5 * part + beside, (held, part, beside)
+    held, (logp, _) = _held(lambda: ops.lmhead_top_logprobs(h, w, 8))
+    assert held <= part + 2 * 32 * T + 4 * (h.numel() + w.numel()) + (2 << 20), (held, part)
+    loss.backward()
+    # the whole in one range gives the same up to the order of float sums
+    monkeypatch.setattr(native, "LOGITS_BYTES", 4 << 30)
+    a, b = h.detach().clone().requires_grad_(), w.detach().clone().requires_grad_()
+    one, each = ops.lmhead_distill_loss(a, b, top, idx)
+    one.backward()
+    # float32 products of T, V and H terms, 2^-24 of their sizes each; gradients to half a step of their type in front of and behind the products
+    tol = 2.0 ** -7 if dtype == BF16 else 1e-5
+    assert abs(one.item() - loss.item()) <= 1e-6 and (each - token).abs().max() <= 1e-5 and _rel(h.grad, a.grad) <= tol and _rel(w.grad, b.grad) <= tol
+    assert torch.allclose(logp, ops.lmhead_top_logprobs(h, w, 8)[0], rtol=0.0, atol=1e-5)
+
+
+@pytest.mark.parametrize("beta,tail", BETAS)
+@pytest.mark.parametrize("T,V,H,hd,wd", [(40, 1003, 64, BF16, BF16), (33, 512, 20, F32, F32), (33, 512, 64, F32, BF16), (600, 2001, 36, BF16, F32)])
+def test_a_head_of_other_types_and_sizes(T, V, H, hd, wd, beta, tail, monkeypatch):
+    monkeypatch.setattr(native, "LOGITS_BYTES", 256 * 4 * V)                             # 600 rows: three ranges
+    h = torch.randn(T, H, generator=_gen(1), device=DEV).to(hd).requires_grad_()
+    w = (torch.randn(V, H, generator=_gen(2), device=DEV) * 0.2).to(wd).requires_grad_()
+    h64, w64 = h.detach().double().requires_grad_(), w.detach().double().requires_grad_()
+    top, idx = ops.top_logprobs((h64 @ w64.t()).detach().float() + 0.3, 9)
+    wt = torch.rand(T, generator=_gen(3), device=DEV) / T
+    loss, token = ops.lmhead_distill_loss(h, w, top, idx, wt, 0.8, beta, tail)
+    (2.0 * loss).backward()
+    want, tw = ref.distill_loss(h64 @ w64.t(), top, idx, wt, 0.8, beta, tail)
+    (2.0 * want).backward()
+    # float32 logits of H <= 64 products: 64 * 2^-24 of their terms, of which the sums are below 4: 1.5e-5 at the very most; gradients the same, and half a step of their type
+    assert ((token - tw).abs() <= 1.5e-5 * (1.0 + tw.abs())).all() and abs(loss.item() - want.item()) <= 1.5e-5 * (1.0 + abs(want.item()))
+    for a, b in ((h, h64), (w, w64)):
+        assert a.grad.dtype == a.dtype and _rel(a.grad, b.grad) <= (2.0 ** -8 if a.dtype == BF16 else 0.0) + 1e-4
