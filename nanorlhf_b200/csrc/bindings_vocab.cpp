@@ -3,6 +3,8 @@
 
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/graph_task.h>
 #include <torch/extension.h>
 
@@ -99,9 +101,21 @@ int64_t capture_id() {
   return status == cudaStreamCaptureStatusActive ? static_cast<int64_t>(id) : 0;
 }
 
+// A gradient of the running backward, where it may be differentiated again: its own derivative with respect to that backward's inputs is refused, for it was formed in the
+// forward and is a constant here.
+torch::Tensor refuse_second(const torch::Tensor& grad) {
+  const auto node = torch::autograd::get_current_node();
+  if (!at::GradMode::is_enabled() || !node) return grad;
+  torch::Tensor out = grad.detach();
+  torch::autograd::edge_list inputs = node->next_edges();
+  torch::autograd::create_gradient_edge(out, std::make_shared<torch::autograd::Error>("distillation: there is no second derivative", std::move(inputs)));
+  return out;
+}
+
 // grads times g, in place where this backward is the graph's only one, which frees them, and every replay of a captured one forms them again
 torch::Tensor scaled(torch::Tensor grad, const torch::Tensor& g, int64_t capture) {
   if (!grad.defined()) return grad;
+  grad = refuse_second(grad);
   if (at::GradMode::is_enabled() || torch::autograd::get_current_graph_task_keep_graph() || g.scalar_type() != torch::kFloat32 || capture_id() != capture)
     return grad.scalar_type() == g.scalar_type() ? grad * g : (grad.to(torch::kFloat32) * g).to(grad.scalar_type());
   scale_(grad, g);
@@ -196,6 +210,7 @@ void bind_vocab(pybind11::module_& m) {
   m.def("distill_loss", &distill_loss_fn);
   m.def("teacher_entries", &teacher_entries);
   m.def("scaled", &scaled);
+  m.def("refuse_second", &refuse_second);
   m.def("distill_loss_parts", &distill_loss, py::arg("logits"), py::arg("top_logp"), py::arg("top_idx"), py::arg("weights"), py::arg("inv_temp"), py::arg("beta"),
         py::arg("tail"), py::arg("want_grad"), py::arg("bf16_grad"), py::arg("with_loss"));
   m.def("weighted_sum", &weighted_sum);

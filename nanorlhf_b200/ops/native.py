@@ -260,7 +260,7 @@ class _RecordedDistillFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g_loss, _g_token):
-        return (ctx.saved_tensors[0] * g_loss,) + (None,) * 6
+        return (ext().refuse_second(ctx.saved_tensors[0]) * g_loss,) + (None,) * 6
 
 
 def distill_loss(logits, top_logp, top_idx, weights, temperature, beta, tail):

@@ -291,3 +291,27 @@ def test_a_head_of_other_types_and_sizes(T, V, H, hd, wd, beta, tail, monkeypatc
     assert ((token - tw).abs() <= 1.5e-5 * (1.0 + tw.abs())).all() and abs(loss.item() - want.item()) <= 1.5e-5 * (1.0 + abs(want.item()))
     for a, b in ((h, h64), (w, w64)):
         assert a.grad.dtype == a.dtype and _rel(a.grad, b.grad) <= (2.0 ** -8 if a.dtype == BF16 else 0.0) + 1e-4
+
+
+# ---- derivatives -------------------------------------------------------------------------------------------------------------------
+def test_a_second_derivative_is_refused():
+    z = torch.randn(4, 300, generator=_gen(1), device=DEV, requires_grad=True)
+    logp, idx = ops.top_logprobs(z.detach() * 1.1, 8)
+    s = torch.ones((), device=DEV, requires_grad=True)
+    (want,) = torch.autograd.grad(ops.distill_loss(z, logp, idx)[0], z)
+    loss, _ = ops.distill_loss(z, logp, idx)
+    (g,) = torch.autograd.grad(loss * s, z, create_graph=True)
+    assert torch.equal(g, want)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad((g * g).sum(), z, allow_unused=True, retain_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        ((g * g).sum() + (z * z).sum()).backward(retain_graph=True)
+    (gs,) = torch.autograd.grad((g * g).sum(), s)          # of the factor there is one
+    assert torch.allclose(gs, 2 * (want * want).sum())
+    h = torch.randn(4, 64, generator=_gen(2), device=DEV).to(BF16).requires_grad_()
+    w = torch.randn(304, 64, generator=_gen(3), device=DEV).to(BF16).requires_grad_()
+    loss, _ = ops.lmhead_distill_loss(h, w, logp, idx)
+    gh, gw = torch.autograd.grad(loss, (h, w), create_graph=True)
+    for g, x in ((gh, h), (gw, w), (gh, w), (gw, h)):
+        with pytest.raises(RuntimeError, match="second derivative"):
+            torch.autograd.grad(g.float().square().sum(), x, allow_unused=True, retain_graph=True)
