@@ -245,7 +245,7 @@ def sample_filtered(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p
             want = torch.int32 if name == "top_k" else torch.float32
             if tuple(x.shape) != (logits.shape[0],) or x.dtype != want:
                 raise ValueError(f"sample_filtered: {name} must be a number or a {want} tensor [{logits.shape[0]}], got {x.dtype} {tuple(x.shape)}")
-        elif not 0 <= x <= hi or x == float("inf"):
+        elif not 0 <= x <= hi or x == float("inf") or (name == "top_k" and x != int(x)):
             raise ValueError(f"sample_filtered: {name} is out of range: {x}")
     if use_native(logits):
         return _nat().sample_filtered(logits, uniforms, temperature, top_k, top_p, min_p)

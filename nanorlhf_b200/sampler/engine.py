@@ -85,8 +85,8 @@ def release_native_engine(model):
 def generate(n: int, model, tokenizer, prompts: Union[torch.Tensor, Sequence[Sequence[int]]], temperature: float,
              max_tokens: int, top_p: float = 0.95, seed: Optional[int] = None, backend: str = "auto",
              eos_token_id: Optional[int] = None, rollout_dtype: str = "bf16", top_k: int = 0, min_p: float = 0.0, **engine_kw) -> torch.Tensor:
-    if top_k < 0 or not 0.0 <= min_p <= 1.0:
-        raise ValueError(f"top_k must be 0 (off) or positive and min_p between 0 (off) and 1, got {top_k} and {min_p}")
+    if top_k < 0 or top_k != int(top_k) or not 0.0 <= min_p <= 1.0:
+        raise ValueError(f"top_k must be 0 (off) or a positive whole number and min_p between 0 (off) and 1, got {top_k} and {min_p}")
     pad_id = tokenizer.pad_token_id
     eos_id = tokenizer.eos_token_id if eos_token_id is None else eos_token_id
     if isinstance(prompts, torch.Tensor):

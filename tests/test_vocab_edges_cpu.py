@@ -58,3 +58,15 @@ def test_a_teacher_that_is_not_a_number_is_not_left_out(beta, tail):
     loss.backward()
     assert loss.isnan() and token.isnan().tolist() == [False, True, False]
     assert z.grad[1].isnan().all() and torch.isfinite(z.grad[[0, 2]]).all()
+
+
+def test_a_number_of_tokens_is_whole():
+    z, u = torch.zeros(2, 8), torch.tensor([0.0, 0.99])
+    for k in (2.5, torch.tensor(0.5)):                             # (one kept 3 tokens here and 2 on the device)
+        with pytest.raises(ValueError):
+            ops.sample_filtered(z, u, top_k=k)
+    for k in (2, 2.0, torch.tensor(2)):
+        assert ops.sample_filtered(z, u, top_k=k)[0].tolist() == [0, 1]
+    from nanorlhf_b200.sampler.engine import generate
+    with pytest.raises(ValueError, match="whole"):
+        generate(1, None, None, [[1]], 1.0, 4, top_k=2.5)
