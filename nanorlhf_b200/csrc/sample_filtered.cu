@@ -262,7 +262,8 @@ NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx
     }
     floor_key = static_cast<uint32_t>(hi);
   }
-  const float floor = fmaxf(key_logit(floor_key), static_cast<float>(fmax(-3e38, mx - 690.0 * f.temp)));
+  // (rounded up: to nearest, the next float below mx would be in at up to 1380 temperatures, for which RowMass has no exponent)
+  const float floor = fmaxf(key_logit(floor_key), __double2float_ru(mx - 690.0 * f.temp));
   const bool nucleus = f.top_p < 1.0;
   // kept for good: logits from `high` on; open: those from `low` on
   float high = floor, low = floor;

@@ -315,3 +315,28 @@ def test_a_second_derivative_is_refused():
     for g, x in ((gh, h), (gw, w), (gh, w), (gw, h)):
         with pytest.raises(RuntimeError, match="second derivative"):
             torch.autograd.grad(g.float().square().sum(), x, allow_unused=True, retain_graph=True)
+
+
+# ---- logits a step of float32 apart at temperatures as small as that ---------------------------------------------------------------
+@pytest.mark.parametrize("apart", [600.0, 689.0, 691.0, 707.0, 709.0, 730.0, 760.0, 1000.0, 1300.0, 1500.0])
+@pytest.mark.parametrize("T", [3, 100])
+def test_neighbouring_logits_at_their_own_temperature(T, apart):
+    """the second largest logits are the next float32 number, `apart` temperatures below the largest: what they have is no share of a sum, and no garbage"""
+    z = torch.randn(T, 40000, generator=_gen(1), device=DEV).clamp(max=2.0)
+    top = torch.tensor(4.0, device=DEV)
+    z[:, 100:200] = torch.nextafter(top, torch.zeros_like(top))
+    z[:, [300, 9000]] = top
+    step = 4.0 - z[0, 100].item()
+    u = torch.linspace(1e-6, 1.0 - 2.0 ** -24, T, device=DEV)
+    for kw in (dict(), dict(top_p=0.9), dict(top_p=0.4), dict(min_p=1e-300)):
+        _same_draws(z, u, temperature=step / apart, **kw)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T", [3, 100])
+def test_a_row_of_nothing_but_the_lowest_number(T, dtype):
+    """a mask that leaves nothing: every token is as probable as any other, or as one that has twice its mass"""
+    z = torch.full((T, 40000), torch.finfo(dtype).min, device=DEV, dtype=dtype)
+    u = torch.rand(T, generator=_gen(2), device=DEV)
+    for kw in (dict(), dict(top_p=0.7), dict(min_p=0.5), dict(top_k=9), dict(min_p=0.5, top_p=0.3), dict(temperature=1e30)):
+        _same_draws(z, u, **kw)
