@@ -228,9 +228,9 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
       if (beta == 1.0) {
         if (q > 0.0) d = log_q - log(p);
       } else {
-        const double mid = beta * p + (1.0 - beta) * q;
-        if (q > 0.0) d = (1.0 - beta) * log(q / mid);
-        if (p > 0.0) loss += beta * p * log(p / mid);
+        const double mid = beta * p + (1.0 - beta) * q;    // (0 where p and q are next to it: they count nothing)
+        if (q > 0.0 && mid > 0.0) d = (1.0 - beta) * log(q / mid);
+        if (p > 0.0 && mid > 0.0) loss += beta * p * log(p / mid);
       }
       loss += q * d;
       mean += q * d;
@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
       if (s > 0.0) d = log(sum) + below() - log_total - log(rr > 0.0 ? rr : kNoTail);
     } else {
       const double mid = beta * rr + (1.0 - beta) * s;
-      if (s > 0.0) d = (1.0 - beta) * log(s / mid);
+      if (s > 0.0 && mid > 0.0) d = (1.0 - beta) * log(s / mid);
       if (rr > 0.0) loss += beta * rr * log(rr / mid);
     }
     loss += s * d;

@@ -340,3 +340,24 @@ def test_a_row_of_nothing_but_the_lowest_number(T, dtype):
     u = torch.rand(T, generator=_gen(2), device=DEV)
     for kw in (dict(), dict(top_p=0.7), dict(min_p=0.5), dict(top_k=9), dict(min_p=0.5, top_p=0.3), dict(temperature=1e30)):
         _same_draws(z, u, **kw)
+
+
+# ---- probabilities at the end of double's range ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("beta", [0.01, 0.2, 0.5, 0.8, 0.99])
+def test_divergences_of_probabilities_next_to_nothing(beta):
+    """tokens of which neither teacher nor student gives more than the least numbers of double: their mixture may be rounded to 0"""
+    V, far = 200, torch.arange(700.0, 760.0, 0.5, device=DEV)
+    n = far.numel()
+    z = torch.full((n, V), -2000.0, device=DEV)
+    z[:, 0] = 0.0
+    z[:, 7], z[:, 9], z[:, 150] = -far, -far.flip(0), -far  # 150 is not listed: all that others have
+    idx = torch.tensor([0, 7, 9], dtype=torch.int32, device=DEV).expand(n, 3).contiguous()
+    for p in (-far, torch.full_like(far, -INF), torch.full_like(far, -744.0)):
+        logp = torch.stack([torch.zeros_like(p), p, p], -1)
+        x, y = z.clone().requires_grad_(), z.double().requires_grad_()
+        loss, token = ops.distill_loss(x, logp, idx, None, 1.0, beta)
+        want, tw = ref.distill_loss(y, logp, idx, None, 1.0, beta, True)
+        loss.backward()
+        want.backward()
+        # both sides sum numbers below e^-700; the mean is 0 within float32's least
+        assert (token - tw).abs().max() <= 1e-38 and torch.isfinite(loss) and (x.grad - y.grad).abs().max() <= 1e-38
