@@ -96,6 +96,22 @@ NRL_DEVICE double block_scan(double v, double& all, double* red) {
   return warp > 0 ? before + v : v;
 }
 
+// The smallest key in [lo, top] whose mass is at least min_p -- the largest logit is in whatever min_p says -- by every lane of a warp: each tries one of 32 keys of a range,
+// seven times.
+NRL_DEVICE uint32_t least_key(const RowFilter& f, float mx, uint32_t lo0, uint32_t top) {
+  uint64_t lo = lo0, hi = top;                             // in [lo, hi]
+  while (lo < hi) {
+    const uint64_t step = (hi - lo + 31) / 32, k = lo + lane_id() * step;
+    const unsigned in = __ballot_sync(0xffffffffu, k >= hi || f.mass(key_logit(static_cast<uint32_t>(k)), mx) >= f.min_p);
+    const int i = in ? __ffs(in) - 1 : 32;                 // the border lies behind the key of lane i - 1
+    const uint64_t up = lo + static_cast<uint64_t>(i) * step;
+    if (i == 0) return static_cast<uint32_t>(lo);
+    lo = lo + static_cast<uint64_t>(i - 1) * step + 1;
+    if (up < hi) hi = up;
+  }
+  return static_cast<uint32_t>(hi);
+}
+
 // By the border alone: found by ranges of keys, all in double, then the kept mass of every warp's range and a walk through the range that holds the drawn one.
 // (A function of its own for every kernel: one that kernels of different register counts share ends ptxas 12.9.)
 template <int KERNEL, typename T>
@@ -106,19 +122,7 @@ __device__ __noinline__ void sample_by_border(const LogitRow<T>& row, const RowF
   auto mass = [&](float z) { return f.mass(z, mx); };
   auto one = [](float) { return 1.0; };
   uint32_t floor_key = mx == INFINITY ? top : kKeyNone + 1;
-  if (f.min_p > 0.0) {                            // smallest key whose mass is min_p: every lane tries one of 32 keys of a range, seven times
-    uint64_t lo = floor_key, hi = top;                     // in [lo, hi]; the largest logit is in whatever min_p says
-    while (lo < hi) {
-      const uint64_t step = (hi - lo + 31) / 32, k = lo + lane * step;
-      const unsigned in = __ballot_sync(0xffffffffu, k >= hi || mass(key_logit(static_cast<uint32_t>(k))) >= f.min_p);
-      const int i = in ? __ffs(in) - 1 : 32;               // the border lies behind the key of lane i - 1
-      const uint64_t up = lo + static_cast<uint64_t>(i) * step;
-      if (i == 0) { hi = lo; break; }
-      lo = lo + static_cast<uint64_t>(i - 1) * step + 1;
-      if (up < hi) hi = up;
-    }
-    floor_key = static_cast<uint32_t>(hi);
-  }
+  if (f.min_p > 0.0) floor_key = least_key(f, mx, floor_key, top);
   Border b{floor_key, 0x7fffffff};
   auto total_of = [&](auto&& measure) {
     double m = 0.0;
@@ -247,21 +251,8 @@ NRL_DEVICE bool sample_long(const LogitRow<T>& row, const RowFilter& f, float mx
   if (tid < 128) sh.powers[tid] = exp2(tid / 128.0);
   const RowMass mass(f, mx, sh.powers);
   if (tid == 0) sh.list.n = sh.list.nhits = 0;
-  // the least logit that min_p keeps: every lane tries one of 32 keys of a range, seven times
-  uint32_t floor_key = kKeyNone + 1;
-  if (f.min_p > 0.0) {
-    uint64_t lo = floor_key, hi = order_key(mx);            // in [lo, hi]; the largest logit is in whatever min_p says
-    while (lo < hi) {
-      const uint64_t step = (hi - lo + 31) / 32, k = lo + lane * step;
-      const unsigned in = __ballot_sync(0xffffffffu, k >= hi || f.mass(key_logit(static_cast<uint32_t>(k)), mx) >= f.min_p);
-      const int i = in ? __ffs(in) - 1 : 32;
-      const uint64_t up = lo + static_cast<uint64_t>(i) * step;
-      if (i == 0) { hi = lo; break; }
-      lo = lo + static_cast<uint64_t>(i - 1) * step + 1;
-      if (up < hi) hi = up;
-    }
-    floor_key = static_cast<uint32_t>(hi);
-  }
+  uint32_t floor_key = kKeyNone + 1;                       // of the least logit that min_p keeps
+  if (f.min_p > 0.0) floor_key = least_key(f, mx, floor_key, order_key(mx));
   // (rounded up: to nearest, the next float below mx would be in at up to 1380 temperatures, for which RowMass has no exponent)
   const float floor = fmaxf(key_logit(floor_key), __double2float_ru(mx - 690.0 * f.temp));
   const bool nucleus = f.top_p < 1.0;
