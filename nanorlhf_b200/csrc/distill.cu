@@ -52,6 +52,26 @@ NRL_DEVICE void store_grads(G* out, int e0, int V, const uint32_t (&w)[W]) {
   }
 }
 
+// Elements whose bits are set in a map of the vectors first .. end
+template <int N>
+struct SkipMapped {
+  const uint32_t* map;
+  int first, end;
+  NRL_DEVICE unsigned marks(int v) const { return v < end ? reinterpret_cast<const std::conditional_t<N == 16, uint16_t, uint8_t>*>(map)[v - first] : 0; }
+  NRL_DEVICE void operator()(unsigned bits, RawVec& a) const {
+    if (bits == 0) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if constexpr (N == 16) {
+        if (bits >> (2 * j) & 1) a.w[j] = (a.w[j] & 0xffff0000u) | 0xff80u;
+        if (bits >> (2 * j + 1) & 1) a.w[j] = (a.w[j] & 0xffffu) | 0xff800000u;
+      } else {
+        if (bits >> j & 1) a.w[j] = 0xff800000u;
+      }
+    }
+  }
+};
+
 struct DistillShared {
   __align__(16) int idx[kTopMax];                          // -1: not a token
   float z[kTopMax], a[kTopMax];
@@ -139,22 +159,8 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
 
   // ---- off the teacher's tokens: the largest logit, and the mass relative to it ----
   const float c = log2_scale(inv_temp);
-  const auto* map = reinterpret_cast<const std::conditional_t<N == 16, uint16_t, uint8_t>*>(s_map);
   float best, m, mass;
-  row_pass<kDistillFlight>(row, share, c, static_cast<float*>(nullptr), best, m, mass, [&](int v, RawVec& a) {
-    if (v >= share.end) return;
-    const unsigned bits = map[v - share.first];
-    if (bits == 0) return;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if constexpr (N == 16) {
-        if (bits >> (2 * j) & 1) a.w[j] = (a.w[j] & 0xffff0000u) | 0xff80u;
-        if (bits >> (2 * j + 1) & 1) a.w[j] = (a.w[j] & 0xffffu) | 0xff800000u;
-      } else {
-        if (bits >> j & 1) a.w[j] = 0xff800000u;
-      }
-    }
-  });
+  row_pass<kDistillFlight>(row, share, c, static_cast<float*>(nullptr), best, m, mass, SkipMapped<N>{s_map, share.first, share.end});
   put_state(m, mass, c, sh.part);
   __syncthreads();
   const float2 state = get_state(c, sh.part);

@@ -336,9 +336,19 @@ inline int row_blocks(long rows, int V, int vec) {
 
 // One pass over the block's share: thread-wise maximum `best`, sum s of 2^((z - m) c), m = best or the lowest float, and the maximum of every chunk.  The sum's reference moves with the
 // maximum, once for the FLIGHT vectors of a step.  z - m is formed before the multiplication: m c would round at the size of the logits.
-// skip(v, a) may take elements of vector v out of maxima and sum by making them -infinity.  chunk_max may be null.  SUM false: the maxima alone, of all elements.
+// Elements may be taken out of maxima and sum by making them -infinity: skip(skip.marks(v), a) of vector v, its marks looked up while the vector is on its way.  chunk_max may
+// be null.  SUM false: the maxima alone, of all elements.
+struct SkipNone {
+  NRL_DEVICE unsigned marks(int) const { return 0; }
+  NRL_DEVICE void operator()(unsigned, RawVec&) const {}
+};
+template <typename T>
+struct SkipNan {
+  NRL_DEVICE unsigned marks(int) const { return 0; }
+  NRL_DEVICE void operator()(unsigned, RawVec& a) const { LogitRow<T>::drop_nan(a); }
+};
 template <int FLIGHT, bool SUM = true, typename T, class S>
-NRL_DEVICE void row_pass(const LogitRow<T>& row, const RowShare& sh, float c, float* chunk_max, float& best, float& m, float& s, S&& skip) {
+NRL_DEVICE void row_pass(const LogitRow<T>& row, const RowShare& sh, float c, float* chunk_max, float& best, float& m, float& s, const S& skip) {
   m = -3.402823466e38f;                                // finite, so that -infinity is 0 in the sum
   s = 0.f;
   best = -INFINITY;
@@ -353,9 +363,13 @@ NRL_DEVICE void row_pass(const LogitRow<T>& row, const RowShare& sh, float c, fl
         const int v = v0 + (u + j) * kRowThreads;
         a[j] = v < sh.end ? row.raw(v) : LogitRow<T>::no_vec();
       }
-      if constexpr (SUM)
+      if constexpr (SUM) {
+        unsigned marks[FLIGHT];
 #pragma unroll
-        for (int j = 0; j < FLIGHT; ++j) skip(v0 + (u + j) * kRowThreads, a[j]);
+        for (int j = 0; j < FLIGHT; ++j) marks[j] = skip.marks(v0 + (u + j) * kRowThreads);
+#pragma unroll
+        for (int j = 0; j < FLIGHT; ++j) skip(marks[j], a[j]);
+      }
       float l = LogitRow<T>::largest(a[0]);
 #pragma unroll
       for (int j = 1; j < FLIGHT; ++j) l = fmaxf(l, LogitRow<T>::largest(a[j]));

@@ -668,9 +668,9 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_filtered_kernel(const T
   const float c = log2_scale(f.inv_temp);
   float best, m = 0.f, s = 0.f;
   if (nucleus)
-    row_pass<kFlight, true>(row, share, c, s_chunk, best, m, s, [](int, RawVec& a) { LogitRow<T>::drop_nan(a); });
+    row_pass<kFlight, true>(row, share, c, s_chunk, best, m, s, SkipNan<T>());
   else
-    row_pass<kFlight, false>(row, share, c, s_chunk, best, m, s, [](int, const RawVec&) {});
+    row_pass<kFlight, false>(row, share, c, s_chunk, best, m, s, SkipNone());
   // a thread's chunks in one group up to 256 tokens, in up to four above
   const int want = few ? (f.top_k > 0 && f.top_k <= kTopMax ? f.top_k : 0) : kNucleusGroups, groups = want <= 256 ? 1 : want <= 512 ? 2 : 4;
   uint32_t bound = kKeyNone + 1;

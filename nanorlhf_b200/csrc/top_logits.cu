@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) top_logprobs_kernel(const T* _
   const RowShare share(row.nvec, rank, blocks, kFlight);
   const float c = log2_scale(inv_temp);
   float best, m, s;
-  row_pass<kFlight>(row, share, c, s_chunk, best, m, s, [](int, const RawVec&) {});
+  row_pass<kFlight>(row, share, c, s_chunk, best, m, s, SkipNone());
   // a thread's chunks in one group up to k = 256, in up to four above
   const int groups = k <= 256 ? 1 : k <= 512 ? 2 : 4;
   uint32_t keys[kGroupsMax];
