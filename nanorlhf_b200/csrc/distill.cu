@@ -16,8 +16,8 @@
 // An entry whose index is not a token (-1) is skipped; entries of one token add up.
 //
 // Bytes bound it: logits read, gradients written; the second pass reads from L2 what the first has brought there, and forms the exponentials again, since a row of
-// them would not fit beside two other rows.  2048 x 151 936 bf16, K = 64, forward and backward: 295 us, 4.2 TB/s, where a copy's rate would take 190; issue slots 66 %,
-// special functions 56 %.  4011 rows of floats with gradients in bf16: 844 us, 4.3 TB/s.  Tried without gain: two blocks an SM, vectors fetched a step ahead in
+// them would not fit beside two other rows.  2048 x 151 936 bf16, K = 64, forward and backward: 283 us, 4.4 TB/s, where a copy's rate would take 190; issue slots 67 %,
+// special functions 57 %.  4011 rows of floats with gradients in bf16: 810-830 us, 4.5 TB/s, with beta 1 915.  Tried without gain: two blocks an SM, vectors fetched a step ahead in
 // registers, the next row fetched into L2, rows that start one behind the other.
 #include <algorithm>
 #include <type_traits>
@@ -96,8 +96,8 @@ NRL_DEVICE void block_sum_two(double& x, double& y, double (&red)[2][kRowWarps])
   y = warp_sum(lane_id() < kRowWarps ? red[1][lane_id()] : 0.0);
 }
 
-// Vectors of a thread in flight in the first pass, where three blocks share an SM: us with 2 / 3, and with 4 and two blocks, of 2048 x 151 936 bf16 297 / 302 / 323, of 1500 x 50 021
-// floats 160 / 162 / 180, of 2048 x 32 000 bf16 81 / 87 / 90.
+// Vectors of a thread in flight in the first pass, where three blocks share an SM: us with 2 / 3, and with 4 and two blocks, of 2048 x 151 936 bf16 284 / 293-302 / 317, of 1500 x 50 021
+// floats 154 / 157 / 172, of 2048 x 32 000 bf16 78 / 85 / 89.
 constexpr int kDistillFlight = 2;
 
 constexpr double kNoTail = 5.9604644775390625e-8;          // 2^-24
@@ -343,8 +343,8 @@ __global__ void scale_kernel(T* __restrict__ x, long n, const float* __restrict_
 template <typename T>
 int distill_blocks(int rows, int V, bool with_grad) {
   // The second pass should find its rows in L2, which has 126 MB; three blocks on each of 148 SMs hold 444 rows at a time, or half or a quarter of them with two or four
-  // blocks a row.  us with 1 / 2 / 4 of 2048 x 151 936 floats 574 / 544 / 522, bf16 298 / 293 / 383 (DRAM reads 1.47 / 1.07 / 1.00 of the logits), of 1500 x 50 021 floats
-  // 148 / 155 / 211, of 2048 x 32 000 bf16 83 / 123 / 210.
+  // blocks a row.  us with 1 / 2 / 4 of 2048 x 151 936 floats 575 / 555 / 528, bf16 290 / 284 / 363 (DRAM reads 1.47 / 1.07 / 1.00 of the logits), of 1500 x 50 021 floats
+  // 154 / 181 / 266, of 2048 x 32 000 bf16 76 / 113 / 191.
   int blocks = row_blocks(rows, V, LogitRow<T>::N);
   const long held = std::min(rows, 444) * static_cast<long>(V) * sizeof(T);
   if (with_grad) blocks = std::max(blocks, held > 200L << 20 ? 4 : held > 100L << 20 ? 2 : 1);

@@ -322,10 +322,10 @@ struct RowShare {
   }
 };
 // Blocks of a row's cluster (host).  A row of its own block is fastest where the rows fill the SMs; of few rows the cluster shares the reading, until its barrier and
-// the way through memory cost more.  us with 1 / 2 / 4 blocks of rows of 151 936, top 20 of bf16: 1 row 12.1 / 10.9 / 9.9, 32 rows 12.8 / 11.8 / 10.5, 64 rows 12.9 /
-// 12.1 / 14.0, 100 rows 13.2 / 16.6 / 20.6; sampling with top-k 50 of floats: 1 row 18.5 / 14.8 / 13.2, 64 rows 18.9 / 15.7 / 16.9, of bf16, where the reads are the
-// smaller part, 11.0 / 11.4 / 11.8 and 11.4 / 12.4 / 15.8; without filters 1 row of bf16 49 / 35 / 28, 64 rows 52 / 37 / 44.  Of 32 000 floats with 1 / 2, top 20: 1 row
-// 6.8 / 7.5, 64 rows 7.3 / 8.3.
+// the way through memory cost more.  us with 1 / 2 / 4 blocks of rows of 151 936, top 20 of bf16: 1 row 12.0 / 11.1 / 9.8, 32 rows 12.9 / 11.9 / 10.4, 64 rows 13.1 /
+// 12.0 / 14.0, 100 rows 13.2 / 16.6 / 20.5; sampling with top-k 50 of floats: 1 row 16.9 / 14.4 / 12.9, 64 rows 17.7 / 15.2 / 16.6, of bf16, where the reads are the
+// smaller part, 10.5 / 11.3 / 11.7 and 10.9 / 12.2 / 15.5; without filters 1 row of bf16 51 / 34 / 26, 64 rows 52 / 37 / 42.  Of 32 000 floats with 1 / 2, top 20: 1 row
+// 6.8 / 7.6, 64 rows 7.1 / 8.2.
 inline int row_blocks(long rows, int V, int vec) {
   constexpr int kSms = 148;
   const long nvec = V / vec;

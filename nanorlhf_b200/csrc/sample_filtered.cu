@@ -9,9 +9,9 @@
 // and filtered exactly.  A nucleus without other filters needs the mass of the whole row as well: the pass adds it up in float, and where what is known of its error
 // leaves the nucleus' last token open, or the candidates do not reach it, the row is left to a second kernel, as are rows without filters.
 //
-// 1024 x 151 936 bf16, top-k 50 and top-p 0.95: 86 us, 3.6 TB/s, where a copy's rate would take 48: half of a row's time on an SM, which it shares with another, is the
+// 1024 x 151 936 bf16, top-k 50 and top-p 0.95: 82 us, 3.8 TB/s, where a copy's rate would take 48: half of a row's time on an SM, which it shares with another, is the
 // chain behind its reads (the wait for the last warp and the bound, candidates by two reads, sorting, filtering, drawing: 5000 cycles each at most), and 1024 rows are
-// 3.5 rounds of 296 (2664 rows 198 us).  One row: 11.6 us by four blocks.
+// 3.5 rounds of 296 (2664 rows 185-193 us).  One row: 11.5 us by four blocks.
 #include <curand_kernel.h>
 
 #include <algorithm>
@@ -238,7 +238,7 @@ NRL_DEVICE void add_shared(uint32_t addr, float x) {
 // model.  (2) One pass in double: what lies above that range, for every warp's range of the row, and altogether; the tokens inside are gathered.  (3) The first
 // block sorts those, finds the last kept token, and walks through the range of the row that holds the drawn mass.  What does not work out (many tokens of one
 // logit) is left to sample_by_border: then false.
-// 256 x 151 936 bf16, top-p 0.95 of logits of deviation 0.6: 215 us, of which 40 the kernel in front; 19 instructions an element for each pass in float and 31 for the
+// 256 x 151 936 bf16, top-p 0.95 of logits of deviation 0.6: 187 us (behind min-p 0.02 175, without filters 88), of which 30 the kernel in front; 19 instructions an element for each pass in float and 31 for the
 // one in double fill the issue slots to 62 %; 108 SMs have two rows and 40 one.  A first look at a fourth of the row in place of the first pass, and vectors fetched
 // one ahead, gave nothing.
 template <typename T>
@@ -602,8 +602,8 @@ NRL_DEVICE void draw_of(const LogitRow<T>& row, uint64_t* x, int n, const RowFil
   }
 }
 
-// Both in one warp, for up to 64 sorted candidates that hold all that is kept: 1024 x 151 936 with top-k 50 and top-p 0.95 102 us by
-// the block and 99 by a warp, one row 14.7 / 13.0 (with two vectors a thread in flight).
+// Both in one warp, for up to 64 sorted candidates that hold all that is kept: 1024 x 151 936 with top-k 50 and top-p 0.95 87 us by
+// the block and 80 by a warp, one row 12.4 / 11.3.
 constexpr int kDrawWarp = 64;
 NRL_DEVICE void draw_in_warp(const uint64_t* x, int n1, const RowFilter& f, float mx, double u, double* mass, int* out_token, float* out_logp) {
   const int lane = threadIdx.x & 31;
@@ -757,9 +757,8 @@ __global__ void row_uniforms_kernel(unsigned long long seed, unsigned long long 
   out[i] = fminf(1.f - curand_uniform(&st), 0x1.fffffep-1f);        // (0, 1] -> [0, 1): the difference is rounded to 1 from 2^-25 down
 }
 
-// Filters of every row's own send a part of the rows on, which twice the blocks finish sooner: 250 x 50 021 floats, a third of them, 78 / 69 / 70 us in all with 1 / 2 / 4
-// (before ranges took 19 instructions);
-// where all rows come, 256 x 151 936, 258 / 268 / 311.  Of more than 1024 rows a third fill the SMs, and
+// Filters of every row's own send a part of the rows on, which twice the blocks finish sooner: 250 x 50 021 floats, a third of them, 70 / 63.5 / 62 us in all with 1 / 2 / 4;
+// where all rows come, 256 x 151 936, 194 / 229 / 284.  Of more than 1024 rows a third fill the SMs, and
 // several blocks would want 19 KB of scratch a row.
 template <typename T>
 int long_blocks(int rows, int V, const SampleFilters& f) {

@@ -5,9 +5,9 @@
 // A row is read once.  Beside the sum every thread keeps the maxima of its chunks.  The k-th largest of the block's threads' maxima is a bound that at least k
 // tokens reach, and few more do (k of G groups: about G ln(G / (G - k)) tokens): the chunks whose maximum reaches it are read again, and what reaches it there
 // are the candidates.  Every block of a row's cluster sends its own to the first, which ranks them.  Rows with more candidates than fit (many ties, a sorted
-// vocabulary) and rows with an infinite logit are looked through for the border itself, eight ranges of keys a pass.
+// vocabulary, a k next to the number of the chunks) and rows with an infinite logit are looked through for the border itself, eight ranges of keys a pass.
 //
-// 2048 x 151 936 bf16, k = 64: 140 us, 4.5 TB/s, where a copy's rate would take 95.  What keeps it from that is bytes under way: two blocks of an SM read four vectors a
+// 2048 x 151 936 bf16, k = 64: 135 us, 4.6 TB/s, where a copy's rate would take 95.  What keeps it from that is bytes under way: two blocks of an SM read four vectors a
 // thread at a time, and while one waits for its last warp, finds the bound, reads the candidates (two reads, one behind the other) and ranks them -- 13 000 cycles of
 // a row -- the other reads alone.  One row: 9.8 us by four blocks.
 #include "common.cuh"

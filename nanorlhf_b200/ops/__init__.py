@@ -234,9 +234,8 @@ def sample_filtered(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p
     index), of those the fewest first whose mass is at least ``top_p`` of theirs.  The token is the first kept one, by index, up to which the kept mass
     exceeds ``uniforms`` (float32 [B], in [0, 1)) times the whole; ``logp`` is its log-probability among the kept.  Masses are float64, so that the result is
     that of the definition.  Every filter is a number or a tensor [B] (float32; ``top_k`` int32); 0 / 1 / 0 leave top_k / top_p / min_p out, temperature 0
-    takes the first token of the order (logp 0).  Masses below
-    e^-690 may count as none.  In tensors a value beyond its range counts as the nearest in it, NaN as left out (temperature: as 0).
-    NaN logits count as -inf; a row of nothing else has token -1, logp -inf."""
+    takes the first token of the order (logp 0).  In tensors a value beyond its range counts as the nearest in it, NaN as left out (temperature: as 0).  Masses below
+    e^-690 of the largest logit's may count as none.  NaN logits count as -inf; a row of nothing else has token -1, logp -inf."""
     if logits.dim() != 2 or tuple(uniforms.shape) != (logits.shape[0],):
         raise ValueError(f"sample_filtered: logits [B, V] and uniforms [B] are needed, got {tuple(logits.shape)} and {tuple(uniforms.shape)}")
     if uniforms.dtype != torch.float32:
