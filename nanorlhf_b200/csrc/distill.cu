@@ -102,7 +102,8 @@ constexpr int kDistillFlight = 2;
 
 constexpr double kNoTail = 5.9604644775390625e-8;          // 2^-24
 // What is left of 1 by K <= 1024 float32 log-probabilities that sum to 1: half a step of each, 2^-24 of sum p |log p| <= log 1024, and of the row's sum that they share
-// 5e-7.  Where the student has no mass off K at all -- all its tokens are listed, or teacher and student share a mask -- that is nobody's, and no infinite divergence.
+// 5e-7.  Where the student has no mass off K that a double holds -- all its tokens are listed, or teacher and student share a mask, by -infinity or by a number that is low
+// enough -- that is nobody's, and no divergence, infinite or of the mask's size.
 constexpr double kNobodys = 9.5367431640625e-7;            // 2^-20
 
 // Blocks of a cluster share a row.  Beside the two passes, what a row costs is latency -- entries, barriers, double-precision logarithms -- so that is kept off
@@ -213,7 +214,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
 
   // ---- the K + 1 events ----
   double rr = 1.0 - psum, mean = 0.0, total = top + sum * shrink, off;         // off: factor of e_v off K
-  if (!(rr > kNoTail) || (sum == 0.0 && rr <= kNobodys)) rr = 0.0;
+  if (!(rr > kNoTail) || (rr <= kNobodys && (sum == 0.0 || below() < -745.0))) rr = 0.0;
   const bool teacher = tail || psum != 0.0;
   if (beta == 0.0) {
     off = !teacher ? 0.0 : shrink / total;

@@ -193,7 +193,7 @@ def distill_loss(logits, top_logp, top_idx, weights=None, temperature: float = 1
     factors (gradient accumulation) in there: the gradient is formed in the forward, and a backward from 1 hands it on as it is.  A row with a NaN or +inf, or
     a token of the teacher's with a NaN, has NaN for its loss and no gradient that is a number.
     Entries of ``top_idx`` outside [0, V) are skipped, entries of one token add up; no entries and a tail: loss 0.  What the teacher leaves of 1 counts as 0 below
-    2^-24, and below 2^-20 where the student gives all other tokens none (with more than that KL(P | Q) is infinite).  V <= 2^20 on CUDA, where a second derivative is refused."""
+    2^-24, and below 2^-20 where the student gives all other tokens less than e^-745 of its best (with more than that, KL(P | Q) is infinite where it gives them nothing).  V <= 2^20 on CUDA, where a second derivative is refused."""
     if logits.dim() != 2:
         raise ValueError(f"distill_loss: logits must be [T, V], got {tuple(logits.shape)}")
     _check_teacher("distill_loss", logits.shape[0], top_logp, top_idx, weights, temperature, float(beta), tail)

@@ -361,7 +361,8 @@ def distill_loss(logits: torch.Tensor, top_logp: torch.Tensor, top_idx: torch.Te
     else:
         none = K.all(-1, keepdim=True) | (lq.masked_fill(K, -math.inf) == -math.inf).all(-1, keepdim=True)
         r = 1.0 - total
-        r = torch.where(r <= torch.where(none, 2.0 ** -20, 2.0 ** -24), 0.0, r)          # (what rounding of log-probabilities leaves of 1 is nobody's where nobody else is)
+        far = none | (lq.masked_fill(K, -math.inf).amax(-1, keepdim=True) - lq.amax(-1, keepdim=True) < -745.0)
+        r = torch.where(r <= torch.where(far, 2.0 ** -20, 2.0 ** -24), 0.0, r)          # (what rounding of log-probabilities leaves of 1 is nobody's where nobody has any mass)
         ls = torch.logsumexp(torch.where(none, 0.0, lq.masked_fill(K, -math.inf)), -1, keepdim=True)
         ls = torch.where(none, -math.inf, ls)
         P, lQ = torch.cat([P, r], -1), torch.cat([lq, ls], -1)

@@ -70,3 +70,20 @@ def test_a_number_of_tokens_is_whole():
     from nanorlhf_b200.sampler.engine import generate
     with pytest.raises(ValueError, match="whole"):
         generate(1, None, None, [[1]], 1.0, 4, top_k=2.5)
+
+
+@pytest.mark.parametrize("beta,tail", BETAS)
+@pytest.mark.parametrize("low", [-1e4, torch.finfo(torch.bfloat16).min, torch.finfo(torch.float32).min])
+def test_a_mask_by_a_low_number_is_one(low, beta, tail):
+    """teacher and student share it: the loss is that of the tokens that are left, as by -infinity"""
+    T, V, K = 100, 2000, 300
+    g = torch.Generator().manual_seed(5)
+    at = torch.arange(K) * 6
+    z = torch.full((T, V), low).index_copy_(1, at, torch.randn(T, K, generator=g))
+    logp, idx = torch.log_softmax(torch.randn(T, K, generator=g), -1), at.int().expand(T, K)
+    x, y = z.double().requires_grad_(), z.masked_fill(z == low, -INF).double().requires_grad_()
+    loss, token = ops.distill_loss(x, logp, idx, beta=beta, tail=tail)
+    other, want = ops.distill_loss(y, logp, idx, beta=beta, tail=tail)
+    loss.backward()
+    other.backward()
+    assert torch.equal(token, want) and (x.grad - y.grad).abs().max() < 1e-12

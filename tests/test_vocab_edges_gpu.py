@@ -361,3 +361,24 @@ def test_divergences_of_probabilities_next_to_nothing(beta):
         want.backward()
         # both sides sum numbers below e^-700; the mean is 0 within float32's least
         assert (token - tw).abs().max() <= 1e-38 and torch.isfinite(loss) and (x.grad - y.grad).abs().max() <= 1e-38
+
+
+# ---- masks by a low number ---------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("beta,tail", BETAS)
+@pytest.mark.parametrize("T,V,K", [(300, 700, 20), (10, 151936, 300), (50, 151936, 1024)])
+def test_a_mask_by_a_low_number_is_one(T, V, K, beta, tail, dtype):
+    """teacher and student share it: the loss is that of the tokens that are left, as by -infinity"""
+    at = torch.randperm(V, generator=_gen(1), device=DEV)[:K]
+    for low in (-1e4, torch.finfo(dtype).min):
+        z, t = (torch.full((T, V), low, device=DEV).index_copy_(1, at, torch.randn(T, K, generator=_gen(s), device=DEV)) for s in (2, 3))
+        z = z.to(dtype)
+        logp, idx = ops.top_logprobs(t, K)
+        x, y = z.clone().requires_grad_(), z.masked_fill(z == z.min(), -INF).requires_grad_()
+        loss, token = ops.distill_loss(x, logp, idx, beta=beta, tail=tail)
+        other, want = ops.distill_loss(y, logp, idx, beta=beta, tail=tail)
+        loss.backward()
+        other.backward()
+        assert torch.equal(token, want) and torch.equal(loss, other) and torch.equal(x.grad, y.grad)
+        ref_loss, tw = ref.distill_loss(z.double(), logp, idx, None, 1.0, beta, tail)
+        assert ((token - tw).abs() <= 2.0 ** -23 * (1.0 + tw.abs())).all()
