@@ -363,8 +363,10 @@ def distill_loss(logits: torch.Tensor, top_logp: torch.Tensor, top_idx: torch.Te
         r = 1.0 - total
         far = none | (lq.masked_fill(K, -math.inf).amax(-1, keepdim=True) - lq.amax(-1, keepdim=True) < -745.0)
         r = torch.where(r <= torch.where(far, 2.0 ** -20, 2.0 ** -24), 0.0, r)          # (what rounding of log-probabilities leaves of 1 is nobody's where nobody has any mass)
-        ls = torch.logsumexp(torch.where(none, 0.0, lq.masked_fill(K, -math.inf)), -1, keepdim=True)
-        ls = torch.where(none, -math.inf, ls)
+        # relative to the largest: of numbers like -3e38 a sum of exponentials has no logarithm beside them, and each would have the whole gradient
+        rest = torch.where(none, 0.0, lq.masked_fill(K, -math.inf))
+        best = rest.detach().amax(-1, keepdim=True)
+        ls = torch.where(none, -math.inf, torch.logsumexp(rest - best, -1, keepdim=True) + best)
         P, lQ = torch.cat([P, r], -1), torch.cat([lq, ls], -1)
         on = torch.cat([K, torch.ones_like(r, dtype=torch.bool)], -1)
         lP = torch.cat([P[:, :V].log(), r.clamp_min(2.0 ** -24).log()], -1)

@@ -87,3 +87,15 @@ def test_a_mask_by_a_low_number_is_one(low, beta, tail):
     loss.backward()
     other.backward()
     assert torch.equal(token, want) and (x.grad - y.grad).abs().max() < 1e-12
+
+
+@pytest.mark.parametrize("low", [-1e4, -1e17, torch.finfo(torch.float32).min])
+def test_tokens_of_equally_low_logits_share_a_gradient(low):
+    """the teacher gives the others 0.1, the student next to nothing: the pull towards them is 0.1 altogether"""
+    z = torch.full((2, 50), low)
+    z[:, :3] = torch.tensor([1.0, 2.0, 0.5])
+    x = z.requires_grad_()
+    loss, _ = ops.distill_loss(x, torch.full((2, 3), 0.3).log(), torch.arange(3, dtype=torch.int32).expand(2, 3), torch.tensor([1.0, 2.0]))
+    loss.backward()
+    want = torch.tensor([[-0.1 / 47], [-0.2 / 47]]).expand(2, 47)
+    assert torch.allclose(x.grad[:, 3:], want, rtol=1e-5, atol=0.0)         # 0.1 = 1 - 3 exp(log 0.3), of float32 logarithms: 1e-6 of it
