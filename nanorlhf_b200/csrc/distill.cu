@@ -4,14 +4,15 @@
 // (r = 1 - sum p_k, s = sum of q off K).  With P, Q these K + 1 numbers and M = beta P + (1 - beta) Q the loss of a token is
 //   beta = 0: KL(P | Q)     beta = 1: KL(Q | P)     between: beta KL(P | M) + (1 - beta) KL(Q | M)
 // and with D_j = log(Q_j / P_j) (beta = 1) or (1 - beta) log(Q_j / M_j) its gradient is
-//   dL/dz_v tau = q_v (D_event(v) - sum_j Q_j D_j)            (beta = 0: q_k - p_k for the teacher's tokens, q_v (1 - r / s) for the others)
+//   dL/dz_v tau = q_v (D_event(v) - sum_j Q_j D_j)            (beta = 0: W q_k - p_k for the teacher's tokens, q_v (W - r / s) for the others, W = sum p_k + r,
+//                                                              which is 1 unless entries sum to more)
 // so that off K a row needs one factor.  Without the event for the others (tail = 0, beta = 0) the p_k are scaled to sum to 1, and q keeps the whole
 // vocabulary: the factor is 1.
 //
 // A divergence is the small difference of large terms, so everything about the K + 1 events is in double.  s is summed over the tokens off K alone, which a
 // bit map in shared memory knows: taken as 1 - sum q_k it would have no digits left where the student is sure.  The sum is relative to the largest logit off K,
 // m, since relative to the row's it would be 0 in float from 87 temperatures between the two on: s = S exp((m - max z) / tau) / total, of which the logarithm is
-// taken in parts, and dL/dz_v tau = e_v (exp((m - max z) / tau) / total - r / S) off K with e_v = exp((z_v - m) / tau).
+// taken in parts, and dL/dz_v tau = e_v (W exp((m - max z) / tau) / total - r / S) off K with e_v = exp((z_v - m) / tau).
 // r below 2^-24, which float32 log-probabilities cannot tell from 0, counts as 0, and as 2^-24 under a logarithm.
 // An entry whose index is not a token (-1) is skipped; entries of one token add up.
 //
@@ -217,7 +218,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
   if (!(rr > kNoTail) || (rr <= kNobodys && (sum == 0.0 || below() < -745.0))) rr = 0.0;
   const bool teacher = tail || psum != 0.0;
   if (beta == 0.0) {
-    off = !teacher ? 0.0 : shrink / total;
+    off = !teacher ? 0.0 : tail ? (psum + rr) * shrink / total : shrink / total;
     if (tail && sum != 0.0) off -= rr / sum;
   } else {
     double loss = 0.0, none = 0.0;
@@ -289,7 +290,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_kernel(const T* __rest
       const int bit = sh.idx[i] + row.skew - share.first * N;
       if (p < 0.0 || bit < 0 || bit >= (share.end - share.first) * N) continue;
       const double q = ex2((sh.z[i] - mx) * c) / total;
-      const double u = !teacher ? 0.0 : beta == 0.0 ? q - (tail ? p : p / psum) : q == 0.0 ? 0.0 : q * (sh.q[i] - mean);
+      const double u = !teacher ? 0.0 : beta == 0.0 ? (tail ? q * (psum + rr) - p : q - p / psum) : q == 0.0 ? 0.0 : q * (sh.q[i] - mean);
       out[sh.idx[i]] = static_cast<G>(static_cast<float>(g * u));
     }
   }

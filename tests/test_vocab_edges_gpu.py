@@ -382,3 +382,26 @@ def test_a_mask_by_a_low_number_is_one(T, V, K, beta, tail, dtype):
         assert torch.equal(token, want) and torch.equal(loss, other) and torch.equal(x.grad, y.grad)
         ref_loss, tw = ref.distill_loss(z.double(), logp, idx, None, 1.0, beta, tail)
         assert ((token - tw).abs() <= 2.0 ** -23 * (1.0 + tw.abs())).all()
+
+
+# ---- entries that sum to more than 1, and more of them than tokens -----------------------------------------------------------------
+@pytest.mark.parametrize("beta,tail", BETAS)
+@pytest.mark.parametrize("T,V,K", [(6, 2, 9), (5, 7, 1000), (4, 50, 333), (20, 5000, 64), (3, 151936, 1024)])
+def test_entries_that_sum_to_more_than_one(T, V, K, beta, tail):
+    """the gradient is the loss's own: entries of one token add up, whatever they add up to"""
+    g = _gen(V)
+    z = torch.randn(T, V, generator=g, device=DEV)
+    idx = torch.randint(-1, V + 1, (T, K), generator=g, device=DEV).int()
+    for more in (0.0, 0.4, -0.6):
+        logp = torch.log_softmax(torch.randn(T, K, generator=g, device=DEV), -1) + more
+        if V < K:
+            idx[:, :V] = torch.arange(V, device=DEV)       # all tokens: only sums above 1 leave nothing to others, who are none
+            logp = logp.clamp_min(-0.5)
+        x, y = z.clone().requires_grad_(), z.double().requires_grad_()
+        loss, token = ops.distill_loss(x, logp, idx, None, 0.9, beta, tail)
+        want, tw = ref.distill_loss(y, logp, idx, None, 0.9, beta, tail)
+        loss.backward()
+        want.backward()
+        # events to 5e-6 of themselves, of which there are as many as they sum up to
+        whole = 1.0 + logp.double().exp().sum(-1)
+        assert ((token - tw).abs() <= 5e-6 * whole * (1.0 + tw.abs())).all() and _rel(x.grad, y.grad) <= 1e-5
