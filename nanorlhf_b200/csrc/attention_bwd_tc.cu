@@ -24,6 +24,7 @@
 #include "attention_tc.cuh"
 #include "kernels.h"
 #include "launch.h"
+#include "per_device.h"
 
 namespace nrl {
 
@@ -35,36 +36,40 @@ constexpr int kT64 = 2 * kP64;       // 64 x 128 bf16 tile (16 KB)
 constexpr int kRing = 4;
 
 struct AttnBwdParams {
-  const int* cu_seqlens;
+  AttnSeqs seqs;
   const float* lse;           // [Hq, T]
   const float* delta;         // [Hq, T]
   __nv_bfloat16 *dq, *dk, *dv;
   long dq_stride_t, dkv_stride_t;
-  int num_seqs, total_tokens, Hq, G;
+  int total_tokens, Hq, G;
   float scale, scale_log2;
 };
 
-// The `rank`-th block of 128 rows in the order of descending work: `level` counts the blocks of its sequence on the side where its work
-// lies (behind it for keys, in front of it for queries).  Result through `info` (4 ints of shared memory).
-NRL_DEVICE bool bwd_locate(const int* cu, int num_seqs, int rank, int* info, int& level, int& blocks, int& seq_start, int& seq_len) {
+// The `rank`-th block of 128 rows in the order of descending work (attn_levels: of keys what lies behind them, of queries what lies in front).
+// Result through `info` (12 ints of shared memory).
+template <bool GROUPS, bool KEYS>
+NRL_DEVICE bool bwd_locate(const AttnSeqs& seqs, int rank, int* info, int& block, AttnSeq& seq) {
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
-    int hi = 0, above = 0;                                     // blocks of the longest sequence; blocks with a level >= hi
-    for (int s = lane; s < num_seqs; s += 32) hi = max(hi, (cu[s + 1] - cu[s] + 127) / 128);
-    hi = __reduce_max_sync(0xffffffffu, hi);
+    int hi = attn_most_levels<GROUPS, KEYS, 128>(seqs, lane), above = 0;       // blocks with a level >= hi
     int lo = 0;
-    bool found = rank < attn_blocks_from<128>(cu, num_seqs, 0, lane);
+    bool found = rank < attn_blocks_of<GROUPS, KEYS, 128>(seqs, 0, lane);
     while (found && hi - lo > 1) {
-      const int mid = (lo + hi) >> 1, n = attn_blocks_from<128>(cu, num_seqs, mid, lane);
+      const int mid = (lo + hi) >> 1, n = attn_blocks_of<GROUPS, KEYS, 128>(seqs, mid, lane);
       if (rank < n) { lo = mid; } else { hi = mid; above = n; }
     }
-    const int src = found ? attn_nth_sequence<128>(cu, num_seqs, lo, rank - above, lane) : 0;
-    if (lane == 0) { info[0] = found; info[1] = lo; info[2] = cu[src]; info[3] = cu[src + 1] - cu[src]; }
+    const int src = found ? attn_nth_of<GROUPS, KEYS, 128>(seqs, lo, rank - above, lane) : 0;
+    if (lane == 0) {
+      const AttnSeq q = attn_seq<GROUPS>(seqs, src);
+      const AttnLevels l = attn_levels<GROUPS, KEYS, 128>(seqs, src);
+      info[0] = found; info[1] = KEYS ? l.top - 1 - lo : lo - (l.top - l.blocks); info[2] = q.start; info[3] = q.len;
+      if (GROUPS) { info[4] = q.prefix_start; info[5] = q.prefix_len; info[6] = q.seen_by; }
+    }
   }
   __syncthreads();
   if (!info[0]) return false;
-  level = info[1]; seq_start = info[2]; seq_len = info[3];
-  blocks = (seq_len + 127) / 128;
+  block = info[1];
+  seq = {info[2], info[3], GROUPS ? info[4] : 0, GROUPS ? info[5] : 0, GROUPS ? info[6] : info[3]};
   return true;
 }
 
@@ -90,8 +95,10 @@ NRL_DEVICE void bwd_chunk(const uint32_t (&sv)[16], const uint32_t (&dv)[16], ui
 }
 
 // Half a warp per pair, sixteen bytes per lane, two pairs in flight: 12 011 tokens x 28 heads 51 -> 29 us (8 bytes per lane, one pair per warp before)
+// GROUPS: the gradients of rows behind the last sequence are cleared
+template <bool GROUPS>
 __global__ void attn_bwd_delta_tc_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ dout,
-                                         float* __restrict__ delta, long o_stride_t, int total, unsigned Hq, unsigned pairs) {
+                                         float* __restrict__ delta, long o_stride_t, int total, unsigned Hq, unsigned pairs, const AttnBwdParams p) {
   pdl_wait();
   pdl_launch_dependents();
   const int sub = threadIdx.x & 15;
@@ -117,6 +124,14 @@ __global__ void attn_bwd_delta_tc_kernel(const __nv_bfloat16* __restrict__ o, co
     for (int m = 8; m > 0; m >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, m);
     const unsigned idx = first + u, t = idx / Hq, h = idx - t * Hq;
     if (sub == 0 && idx < pairs) delta[static_cast<long>(h) * total + t] = acc;
+    if (GROUPS && idx < pairs && t >= static_cast<unsigned>(p.seqs.cu[p.seqs.num])) {
+      const uint4 zero = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(p.dq + t * p.dq_stride_t + h * 128 + sub * 8) = zero;
+      if (h < Hq / p.G) {
+        *reinterpret_cast<uint4*>(p.dk + t * p.dkv_stride_t + h * 128 + sub * 8) = zero;
+        *reinterpret_cast<uint4*>(p.dv + t * p.dkv_stride_t + h * 128 + sub * 8) = zero;
+      }
+    }
   }
 }
 
@@ -133,6 +148,7 @@ struct DkdvSmem {
   static constexpr int kTotal = kBar + 256;
 };
 
+template <bool GROUPS>
 NRL_DEVICE void bwd_dkdv(uint8_t* smem, unsigned block, const CUtensorMap& tmQ, const CUtensorMap& tmDO, const CUtensorMap& tmK,
                          const CUtensorMap& tmV, const AttnBwdParams& p) {
   using L = DkdvSmem;
@@ -145,14 +161,17 @@ NRL_DEVICE void bwd_dkdv(uint8_t* smem, unsigned block, const CUtensorMap& tmQ, 
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(done_bar + 1);
   int* info = reinterpret_cast<int*>(tmem_ptr + 4);      // its own 16-byte slot: tcgen05.alloc writes next to it
 
-  int behind, blocks, seq_start, seq_len;
+  int kb;
+  AttnSeq seq;
   const int rank = block / (p.Hq / p.G), kvh = block - rank * (p.Hq / p.G);
-  if (!bwd_locate(p.cu_seqlens, p.num_seqs, rank, info, behind, blocks, seq_start, seq_len)) return;
-  const int kb = blocks - 1 - behind;
+  if (!bwd_locate<GROUPS, true>(p.seqs, rank, info, kb, seq)) return;
+  const int seq_start = seq.start;
+  // a prefix's keys are seen by all rows behind them up to the end of the group: the rows of a block are counted from the prefix's start
+  const int rows = seq.seen_by;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int key0 = kb * 128;
   const int i_begin = key0 / 64;                                   // first 64-row query block that sees these keys
-  const int n_qb = (seq_len + 63) / 64 - i_begin;                  // >= 1
+  const int n_qb = (rows + 63) / 64 - i_begin;                     // >= 1
   const int n_iter = p.G * n_qb;
 
   if (warp == 0 && lane == 0) {
@@ -262,7 +281,7 @@ NRL_DEVICE void bwd_dkdv(uint8_t* smem, unsigned block, const CUtensorMap& tmQ, 
       // threads 0..31 fetch -lse (in log2 units), 32..63 fetch -delta, of the columns' query rows of block `it`
       if (it >= n_iter || t128 >= 64) return 0.f;
       const int qq = (i_begin + qi) * 64 + half * 32 + (t128 & 31);
-      if (qq >= seq_len) return t128 < 32 ? -INFINITY : 0.f;         // lse = +inf  =>  P = 0 for rows past the end
+      if (qq >= rows) return t128 < 32 ? -INFINITY : 0.f;         // lse = +inf  =>  P = 0 for rows past the end
       const long off = static_cast<long>(head) * p.total_tokens + seq_start + qq;
       return t128 < 32 ? p.lse[off] * -1.4426950408889634f : -p.delta[off];
     };
@@ -303,7 +322,7 @@ NRL_DEVICE void bwd_dkdv(uint8_t* smem, unsigned block, const CUtensorMap& tmQ, 
     // ---- epilogue: parity 0 writes dV, parity 1 writes dK, each warpgroup 64 columns ----
     mbar_wait(done_bar, 0);
     tc_fence_after();
-    const bool row_ok = kk < seq_len;
+    const bool row_ok = kk < seq.len;
     const float f = par == 0 ? 1.f : p.scale;
     __nv_bfloat16* dst = (par == 0 ? p.dv : p.dk) + static_cast<long>(seq_start + kk) * p.dkv_stride_t + kvh * 128 + half * 64;
 #pragma unroll 1
@@ -336,6 +355,7 @@ struct DqSmem {
   static constexpr int kTotal = kBar + 256;
 };
 
+template <bool GROUPS>
 NRL_DEVICE void bwd_dq(uint8_t* smem, unsigned block, const CUtensorMap& tmQ, const CUtensorMap& tmDO, const CUtensorMap& tmK,
                        const CUtensorMap& tmV, const AttnBwdParams& p) {
   using L = DqSmem;
@@ -348,12 +368,15 @@ NRL_DEVICE void bwd_dq(uint8_t* smem, unsigned block, const CUtensorMap& tmQ, co
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(done_bar + 1);
   int* info = reinterpret_cast<int*>(tmem_ptr + 4);      // its own 16-byte slot: tcgen05.alloc writes next to it
 
-  int mb, blocks, seq_start, seq_len;
+  int mb;
+  AttnSeq seq;
   const int rank = block / p.Hq, head = block - rank * p.Hq, kvh = head / p.G;
-  if (!bwd_locate(p.cu_seqlens, p.num_seqs, rank, info, mb, blocks, seq_start, seq_len)) return;
+  if (!bwd_locate<GROUPS, false>(p.seqs, rank, info, mb, seq)) return;
+  const int seq_start = seq.start, seq_len = seq.len;
+  const int n_pre = GROUPS ? (seq.prefix_len + 63) / 64 : 0;       // key blocks of the prefix, walked first
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int q0 = mb * 128;
-  const int n_kb = min((seq_len + 63) / 64, (q0 + 128 + 63) / 64);
+  const int n_kb = n_pre + min((seq_len + 63) / 64, (q0 + 128 + 63) / 64);
 
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmDO); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
@@ -387,7 +410,7 @@ NRL_DEVICE void bwd_dq(uint8_t* smem, unsigned block, const CUtensorMap& tmQ, co
         mbar_arrive_expect_tx(&kv_full[st], 2 * kT64);
         uint8_t* sk = smem + L::kK + st * kT64;
         uint8_t* sv = smem + L::kV + st * kT64;
-        const int row = seq_start + j * 64;
+        const int row = GROUPS && j < n_pre ? seq.prefix_start + j * 64 : seq_start + (j - n_pre) * 64;
         tma_load_2d(sk, &tmK, &kv_full[st], kvh * 128, row);
         tma_load_2d(sk + kP64, &tmK, &kv_full[st], kvh * 128 + 64, row);
         tma_load_2d(sv, &tmV, &kv_full[st], kvh * 128, row);
@@ -455,8 +478,10 @@ NRL_DEVICE void bwd_dq(uint8_t* smem, unsigned block, const CUtensorMap& tmQ, co
     auto nd = [&](int) { return nd2; };
     for (int j = par; j < n_kb; j += 2) {
       const int n = j >> 1;
-      const int key0 = j * 64 + half * 32;
-      const int hi = min(row, seq_len - 1) - key0;             // last visible key of these columns
+      const bool pre = GROUPS && j < n_pre;
+      const int key0 = (pre ? j : j - n_pre) * 64 + half * 32;
+      const int hi = (pre ? seq.prefix_len - 1 : min(row, seq_len - 1)) - key0;             // last visible key of these columns
+      const bool cut = pre ? key0 + 32 > seq.prefix_len : key0 + 31 > q0 || key0 + 32 > seq_len;
       mbar_wait(&s_full[par], n & 1);
       tc_fence_after();
       uint32_t dk[16];
@@ -466,7 +491,7 @@ NRL_DEVICE void bwd_dq(uint8_t* smem, unsigned block, const CUtensorMap& tmQ, co
         tmem_ld_32x32b_x16(t_s + c * 16, sv);
         tmem_ld_32x32b_x16(t_dp + c * 16, dv);
         tmem_ld_wait();
-        if (key0 + 31 > q0 || key0 + 32 > seq_len) bwd_chunk<true, false>(sv, dv, sc2, nl, nd, ~mask_from(hi + 1 - c * 16), nullptr, dk + c * 8);
+        if (cut) bwd_chunk<true, false>(sv, dv, sc2, nl, nd, ~mask_from(hi + 1 - c * 16), nullptr, dk + c * 8);
         else bwd_chunk<false, false>(sv, dv, sc2, nl, nd, 0u, nullptr, dk + c * 8);
       }
       tmem_st_32x32b_x16(t_dp, dk);
@@ -497,6 +522,7 @@ NRL_DEVICE void bwd_dq(uint8_t* smem, unsigned block, const CUtensorMap& tmQ, co
 // Both in one launch, dQ's blocks behind those of dK / dV: neither takes anything from the other, and with two key heads dK / dV has a block for two SMs in
 // three only, so that dQ starts on the SMs that it leaves idle.  us of the whole backward as launches one after the other / so: 4 sequences, 6601 tokens, 12
 // heads over 2 250 / 164; 6 of 500, 28 over 4 116 / 76; 2 of 6005 1755 / 1582 to 1688; 4 of 6000 3529 / 3400; one of 300, 12 over 2 58 / 40.
+template <bool GROUPS>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ64, const __grid_constant__ CUtensorMap tmDO64, const __grid_constant__ CUtensorMap tmK128,
                    const __grid_constant__ CUtensorMap tmV128, const __grid_constant__ CUtensorMap tmQ128, const __grid_constant__ CUtensorMap tmDO128,
@@ -504,38 +530,56 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ64, const __grid_const
                    const unsigned dkdv_blocks) {
   extern __shared__ __align__(1024) uint8_t smem[];
   pdl_wait();
-  if (blockIdx.x < dkdv_blocks) bwd_dkdv(smem, blockIdx.x, tmQ64, tmDO64, tmK128, tmV128, p);
-  else bwd_dq(smem, blockIdx.x - dkdv_blocks, tmQ128, tmDO128, tmK64, tmV64, p);
+  if (blockIdx.x < dkdv_blocks) bwd_dkdv<GROUPS>(smem, blockIdx.x, tmQ64, tmDO64, tmK128, tmV128, p);
+  else bwd_dq<GROUPS>(smem, blockIdx.x - dkdv_blocks, tmQ128, tmDO128, tmK64, tmV64, p);
 }
 
 }  // namespace nrl
 
 // maps: [0] Q box 64 rows, [1] dO box 64 rows, [2] K box 128 rows, [3] V box 128 rows  (dK / dV)
 //       [4] Q box 128 rows, [5] dO box 128 rows, [6] K box 64 rows, [7] V box 64 rows  (dQ)
+namespace nrl {
+namespace {
+
+template <bool GROUPS>
+cudaError_t attn_bwd_tc(const CUtensorMap* maps, const void* o, const void* dout, const float* lse,
+                        float* delta, void* dq, void* dk, void* dv, long o_stride_t, long dq_stride_t,
+                        long dkv_stride_t, const AttnSeqs& seqs, int total, int Hq, int Hkv,
+                        float scale, cudaStream_t s) {
+  if (total == 0) return cudaSuccess;
+  constexpr int smem = DkdvSmem::kTotal > DqSmem::kTotal ? DkdvSmem::kTotal : DqSmem::kTotal;
+  static PerDevice<bool> configured;
+  const cudaError_t e = allow_smem(configured, attn_bwd_tc_kernel<GROUPS>, smem);
+  if (e != cudaSuccess) return e;
+  const unsigned pairs = static_cast<unsigned>(total) * Hq;                   // O alone would be a terabyte at 2^32
+  AttnBwdParams p;
+  p.seqs = seqs; p.lse = lse; p.delta = delta;
+  p.dq = static_cast<__nv_bfloat16*>(dq); p.dk = static_cast<__nv_bfloat16*>(dk); p.dv = static_cast<__nv_bfloat16*>(dv);
+  p.dq_stride_t = dq_stride_t; p.dkv_stride_t = dkv_stride_t;
+  p.total_tokens = total; p.Hq = Hq; p.G = Hq / Hkv;
+  p.scale = scale; p.scale_log2 = scale * 1.4426950408889634f;
+  launch_dependent(attn_bwd_delta_tc_kernel<GROUPS>, (pairs + 31) / 32, 256, 0, s, static_cast<const __nv_bfloat16*>(o), static_cast<const __nv_bfloat16*>(dout), delta,
+                   o_stride_t, total, static_cast<unsigned>(Hq), pairs, p);
+  const unsigned most = total / 128 + seqs.num, grid_kv = most * Hkv, grid_q = most * Hq;
+  launch_dependent(attn_bwd_tc_kernel<GROUPS>, grid_kv + grid_q, kBwdThreads, smem, s, maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], maps[6], maps[7], p,
+                   grid_kv);
+  return cudaGetLastError();
+}
+
+}  // namespace
+}  // namespace nrl
+
 extern "C" cudaError_t nrl_attn_bwd_tc(const CUtensorMap* maps, const void* o, const void* dout, const float* lse,
                                        float* delta, void* dq, void* dk, void* dv, long o_stride_t, long dq_stride_t,
                                        long dkv_stride_t, const int* cu, int num_seqs, int total, int Hq, int Hkv,
                                        float scale, cudaStream_t s) {
-  using namespace nrl;
-  if (total == 0) return cudaSuccess;
-  constexpr int smem = DkdvSmem::kTotal > DqSmem::kTotal ? DkdvSmem::kTotal : DqSmem::kTotal;
-  static bool configured = false;
-  if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(attn_bwd_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    configured = true;
-  }
-  const unsigned pairs = static_cast<unsigned>(total) * Hq;                   // O alone would be a terabyte at 2^32
-  launch_dependent(attn_bwd_delta_tc_kernel, (pairs + 31) / 32, 256, 0, s, static_cast<const __nv_bfloat16*>(o), static_cast<const __nv_bfloat16*>(dout), delta,
-                   o_stride_t, total, Hq, pairs);
-  AttnBwdParams p;
-  p.cu_seqlens = cu; p.lse = lse; p.delta = delta;
-  p.dq = static_cast<__nv_bfloat16*>(dq); p.dk = static_cast<__nv_bfloat16*>(dk); p.dv = static_cast<__nv_bfloat16*>(dv);
-  p.dq_stride_t = dq_stride_t; p.dkv_stride_t = dkv_stride_t;
-  p.num_seqs = num_seqs; p.total_tokens = total; p.Hq = Hq; p.G = Hq / Hkv;
-  p.scale = scale; p.scale_log2 = scale * 1.4426950408889634f;
-  const unsigned most = total / 128 + num_seqs, grid_kv = most * Hkv, grid_q = most * Hq;
-  launch_dependent(attn_bwd_tc_kernel, grid_kv + grid_q, kBwdThreads, smem, s, maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], maps[6], maps[7], p,
-                   grid_kv);
-  return cudaGetLastError();
+  return nrl::attn_bwd_tc<false>(maps, o, dout, lse, delta, dq, dk, dv, o_stride_t, dq_stride_t, dkv_stride_t, {cu, nullptr, num_seqs}, total, Hq, Hkv, scale, s);
+}
+
+// table: attention_groups.cu
+extern "C" cudaError_t nrl_attn_groups_bwd_tc(const CUtensorMap* maps, const void* o, const void* dout, const float* lse, float* delta, void* dq, void* dk,
+                                              void* dv, long o_stride_t, long dq_stride_t, long dkv_stride_t, const int* cu, const int* table, int num_seqs,
+                                              int total, int Hq, int Hkv, float scale, cudaStream_t s) {
+  return nrl::attn_bwd_tc<true>(maps, o, dout, lse, delta, dq, dk, dv, o_stride_t, dq_stride_t, dkv_stride_t, {cu, reinterpret_cast<const int4*>(table), num_seqs},
+                                total, Hq, Hkv, scale, s);
 }

@@ -29,7 +29,11 @@
 #include "common.cuh"
 #include "kernels.h"
 #include "decode_merge.cuh"
+#include "decode_modes.cuh"
+#include "fp8_fragments.cuh"
+#include "group_kernels.h"
 #include "launch.h"
+#include "per_device.h"
 
 #include <type_traits>
 
@@ -42,36 +46,6 @@ constexpr int kStages8 = 4;
 constexpr int kRawPage = kPg * kHd;                 // 2048 bytes of e4m3 (K or V of one page, one kv head)
 constexpr int kStage8 = 2 * kRawPage + 2 * 64;      // K, V^T, k_scale[16], v_scale[16]
 constexpr float kPScale = 1024.f;
-
-NRL_DEVICE void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
-  // rows 8..15 of the A tile are padding (G <= 8 query heads): a1 = a3 = 0
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(0u), "r"(a2), "r"(0u), "r"(b0), "r"(b1));
-}
-NRL_DEVICE uint32_t e4m3x2_to_f16x2(uint32_t v16) {
-  uint32_t r;
-  asm volatile("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(v16)));
-  return r;
-}
-NRL_DEVICE uint32_t pack_f16x2(float lo, float hi) {
-  __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&h);
-}
-NRL_DEVICE uint32_t lds32(uint32_t addr) {
-  uint32_t r;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r) : "r"(addr));
-  return r;
-}
-NRL_DEVICE uint4 lds128(uint32_t addr) {
-  uint4 r;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(addr));
-  return r;
-}
-// K rows are 128 B = 8 chunks of 16 B; chunk c of token row r lives at chunk c ^ 4 (r & 1): the eight lanes that are served together read chunks t = 0..3
-// (or 4..7) of an even and an odd row, which are all eight chunks' banks.
-NRL_DEVICE int k_sigma(int r) { return (r & 1) << 2; }
 
 // ---- page writer: one warp per (token, kv head) ----------------------------------------------------------------
 // kq [num_blocks, Hkv, 16, 128]   vq [num_blocks, Hkv, 128, 16] (transposed)   ks, vs [num_blocks, Hkv, 16]
@@ -129,17 +103,21 @@ struct Decode8Params {
   float scale_log2;
 };
 
-__global__ void __launch_bounds__(kWarps8 * 32, 3) paged_decode_fp8_kernel(Decode8Params p) {
+// MODE: decode_modes.cuh
+template <int MODE>
+__global__ void __launch_bounds__(kWarps8 * 32, 3) paged_decode_fp8_kernel(Decode8Params p, DecodeExtra x) {
   pdl_wait();
   pdl_launch_dependents();
   extern __shared__ __align__(128) uint8_t smem[];
   const int seq = blockIdx.x, kvh = blockIdx.y, split = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t4 = lane & 3;
-  const int ctx = p.context_lens[seq];
+  const int ctx = MODE == kDecodePlain ? p.context_lens[seq] : min(p.context_lens[seq], p.max_blocks * kPg);
   const int n_pages = (ctx + kPg - 1) / kPg;
-  const int pages_per_split = (n_pages + p.splits - 1) / p.splits;
-  const int page_lo = split * pages_per_split;
+  const DecodeFirst from = decode_first<MODE>(x, seq, ctx, lane);
+  const int page_0 = MODE == kDecodeTail ? from.token / kPg : 0;
+  const int pages_per_split = (n_pages - page_0 + p.splits - 1) / p.splits;
+  const int page_lo = page_0 + split * pages_per_split;
   const int page_hi = min(n_pages, page_lo + pages_per_split);
   const int* bt = p.block_tables + static_cast<long>(seq) * p.max_blocks;
 
@@ -239,6 +217,25 @@ __global__ void __launch_bounds__(kWarps8 * 32, 3) paged_decode_fp8_kernel(Decod
           for (int e = 0; e < 2; ++e)
             if (tok0 + u * kWarps8 * kPg + t4 * 4 + 2 * j + e >= ctx) s[u][j][e] = -INFINITY;
       }
+      const int page0 = tok0 + u * kWarps8 * kPg;
+      if (MODE == kDecodeTail && page0 < from.token) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (page0 + t4 * 4 + 2 * j + e < from.token) s[u][j][e] = -INFINITY;
+      }
+      if (MODE != kDecodePlain && (page0 + kPg > ctx || (MODE == kDecodeTail && page0 < from.token))) {
+        // values and scales outside the row's own tokens, whatever they are, meet weights of 0 as zeros
+        const int lo = MODE == kDecodeTail ? from.token - page0 : 0, hi = ctx - page0;
+        fp8_clear_values(my_smem + ((it + u) % kStages8) * kStage8 + kRawPage, lo, hi, lane);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vscale[u][i] = t4 * 4 + i >= lo && t4 * 4 + i < hi ? vscale[u][i] : 0.f;
+      }
+      if (MODE == kDecodeScored && g < p.G) {
+        float* raw = x.raw + ((static_cast<long>(seq) * p.Hkv + kvh) * p.G + g) * x.raw_len + tok0 + u * kWarps8 * kPg + t4 * 4;
+        *reinterpret_cast<float4*>(raw) = make_float4(s[u][0][0], s[u][0][1], s[u][1][0], s[u][1][1]);
+      }
       tmax = fmaxf(tmax, fmaxf(fmaxf(s[u][0][0], s[u][0][1]), fmaxf(s[u][1][0], s[u][1][1])));
     }
     tmax = fmaxf(tmax, __shfl_xor_sync(0xffffffffu, tmax, 1));
@@ -311,11 +308,11 @@ __global__ void __launch_bounds__(kWarps8 * 32, 3) paged_decode_fp8_kernel(Decod
       acc += mo[(w * 8 + r) * kHd + d] * c;
     }
     acc *= (1.f / kPScale);
-    if (p.splits == 1) {
-      p.out[(static_cast<long>(seq) * p.Hq + kvh * p.G + r) * kHd + d] = __float2bfloat16(L > 0.f ? acc / L : 0.f);
-    } else {
-      const long base = ((static_cast<long>(seq) * p.Hkv + kvh) * p.splits + split) * 8 + r;
-      p.part_o[base * kHd + d] = acc;
+    decode_join_prefix<MODE>(x, from, p.splits, p.part_o, p.part_ml, static_cast<long>(seq) * p.Hkv + kvh, split, r, d, M, L, acc);
+    if (p.splits == 1) p.out[(static_cast<long>(seq) * p.Hq + kvh * p.G + r) * kHd + d] = __float2bfloat16(L > 0.f ? acc / L : 0.f);
+    if (p.splits > 1 || MODE == kDecodeScored) {
+      const long base = ((static_cast<long>(seq) * p.Hkv + kvh) * decode_parts<MODE>(x, p.splits) + decode_part<MODE>(x, split)) * 8 + r;
+      if (p.splits > 1) p.part_o[base * kHd + d] = acc;
       if (d == 0) {
         p.part_ml[base * 2] = M;
         p.part_ml[base * 2 + 1] = L;
@@ -345,10 +342,13 @@ extern "C" cudaError_t nrl_kv_cache_write_fp8(const void* k, const void* v, long
   return cudaGetLastError();
 }
 
-extern "C" cudaError_t nrl_paged_decode_fp8(const void* q, long q_stride_s, const void* kq, const void* vq, const float* ks,
-                                            const float* vs, const int* block_tables, const int* context_lens, void* out,
-                                            float* part_o, float* part_ml, int S, int Hq, int Hkv, int head_dim, int page,
-                                            int max_blocks, int splits, float scale, cudaStream_t s) {
+namespace {
+
+template <int MODE>
+cudaError_t paged_decode_fp8_mode(const void* q, long q_stride_s, const void* kq, const void* vq, const float* ks,
+                                  const float* vs, const int* block_tables, const int* context_lens, void* out,
+                                  float* part_o, float* part_ml, int S, int Hq, int Hkv, int head_dim, int page,
+                                  int max_blocks, int splits, float scale, const DecodeExtra& x, cudaStream_t s) {
   if (head_dim != kHd || page != kPg || Hq % Hkv != 0 || Hq / Hkv > 8) return cudaErrorInvalidValue;
   if (S == 0) return cudaSuccess;
   Decode8Params p;
@@ -363,19 +363,35 @@ extern "C" cudaError_t nrl_paged_decode_fp8(const void* q, long q_stride_s, cons
   p.max_blocks = max_blocks; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.splits = splits;
   p.scale_log2 = scale * 1.4426950408889634f;
   const int smem = kWarps8 * kStages8 * kStage8;          // 67,584 B (>= the 16.3 KB the warp merge needs)
-  static bool configured = false;
-  if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(paged_decode_fp8_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    configured = true;
-  }
-  launch_dependent(paged_decode_fp8_kernel, dim3(S, Hkv, splits), kWarps8 * 32, smem, s, p);
-  cudaError_t e = cudaGetLastError();
+  static PerDevice<bool> configured;
+  cudaError_t e = allow_smem(configured, paged_decode_fp8_kernel<MODE>, smem);
   if (e != cudaSuccess) return e;
-  if (splits > 1) {
-    const MergeParams m = {part_o, part_ml, static_cast<__nv_bfloat16*>(out), Hq, Hkv, Hq / Hkv, splits};
+  launch_dependent(paged_decode_fp8_kernel<MODE>, dim3(S, Hkv, splits), kWarps8 * 32, smem, s, p, x);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  if (splits > 1 && MODE != kDecodeScored) {       // (scores are added where their parts are merged)
+    const MergeParams m = {part_o, part_ml, static_cast<__nv_bfloat16*>(out), Hq, Hkv, Hq / Hkv, decode_parts<MODE>(x, splits)};
     launch_dependent(decode8_merge_splits_kernel, dim3(S, Hq), kMergeD, 0, s, m);
     e = cudaGetLastError();
   }
   return e;
+}
+
+}  // namespace
+
+extern "C" cudaError_t nrl_paged_decode_fp8(const void* q, long q_stride_s, const void* kq, const void* vq, const float* ks,
+                                            const float* vs, const int* block_tables, const int* context_lens, void* out,
+                                            float* part_o, float* part_ml, int S, int Hq, int Hkv, int head_dim, int page,
+                                            int max_blocks, int splits, float scale, cudaStream_t s) {
+  return paged_decode_fp8_mode<kDecodePlain>(q, q_stride_s, kq, vq, ks, vs, block_tables, context_lens, out, part_o, part_ml, S, Hq, Hkv, head_dim, page,
+                                             max_blocks, splits, scale, DecodeExtra{}, s);
+}
+
+cudaError_t nrl::paged_decode_tail_fp8(const DecodeCall& c, const DecodeExtra& x, cudaStream_t s) {
+  return paged_decode_fp8_mode<kDecodeTail>(c.q, c.q_stride_s, c.k_cache, c.v_cache, c.k_scale, c.v_scale, c.block_tables, c.context_lens, c.out, c.part_o, c.part_ml,
+                                            c.S, c.Hq, c.Hkv, c.D, c.page, c.max_blocks, c.splits, c.scale, x, s);
+}
+cudaError_t nrl::paged_decode_scored_fp8(const DecodeCall& c, const DecodeExtra& x, cudaStream_t s) {
+  return paged_decode_fp8_mode<kDecodeScored>(c.q, c.q_stride_s, c.k_cache, c.v_cache, c.k_scale, c.v_scale, c.block_tables, c.context_lens, c.out, c.part_o,
+                                              c.part_ml, c.S, c.Hq, c.Hkv, c.D, c.page, c.max_blocks, c.splits, c.scale, x, s);
 }

@@ -18,6 +18,7 @@
 #include "attention_tc.cuh"
 #include "kernels.h"
 #include "launch.h"
+#include "per_device.h"
 
 namespace nrl {
 
@@ -25,11 +26,11 @@ constexpr int kTcBM = 256;                 // query rows per item (two tiles of 
 constexpr int kTcSlots = 4;                // ring of K and V tiles
 
 struct AttnTcParams {
-  const int* cu_seqlens;
+  AttnSeqs seqs;
   __nv_bfloat16* out;
   float* lse;                 // [Hq, T_total]
   long o_stride_t;
-  int num_seqs, total_tokens, Hq, G;
+  int total_tokens, Hq, G;
   float scale_log2;
 };
 
@@ -37,22 +38,36 @@ struct AttnTcSmem {
   static constexpr int kQ = 0;                                   // 2 tiles
   static constexpr int kRing = 2 * kAtTile;                      // kTcSlots tiles
   static constexpr int kBar = kRing + kTcSlots * kAtTile;        // mbarriers, TMEM pointer
-  static constexpr int kTab = kBar + 256;                        // two items: head (-1: none left), q0, first token, length
-  static constexpr int kTotal = kTab + 2 * 16;
+  static constexpr int kTab = kBar + 256;                        // two items: head (-1: none left), q0, first token, length, prefix's first token, its length
+  static constexpr int kTotal = kTab + 2 * 32;
 };
 
+template <bool GROUPS>
 struct AttnItem {
-  int head, q0, start, len;
+  int head, q0, start, len, prefix_start, prefix_len;
+  NRL_DEVICE int prefix_blocks() const { return GROUPS ? (prefix_len + kAtBN - 1) / kAtBN : 0; }
   NRL_DEVICE int blocks(int x) const {     // key blocks that tile x walks; tile B may lie entirely behind the end of the sequence
-    return q0 + x * 128 < len ? q0 / 128 + 1 + x : 0;
+    return q0 + x * 128 < len ? prefix_blocks() + q0 / 128 + 1 + x : 0;
+  }
+  // of block j: the first token, and how many of its keys are the prefix's or the sequence's
+  NRL_DEVICE int block_row(int j) const {
+    const int own = j - prefix_blocks();
+    return GROUPS && own < 0 ? prefix_start + j * kAtBN : start + own * kAtBN;
+  }
+  NRL_DEVICE int block_keys(int j) const {
+    const int own = j - prefix_blocks();
+    return GROUPS && own < 0 ? prefix_len - j * kAtBN : len - own * kAtBN;
   }
 };
-NRL_DEVICE AttnItem attn_item(const uint8_t* smem, uint64_t* tab_full, uint32_t k) {
+template <bool GROUPS>
+NRL_DEVICE AttnItem<GROUPS> attn_item(const uint8_t* smem, uint64_t* tab_full, uint32_t k) {
   mbar_wait(&tab_full[k & 1], (k >> 1) & 1);
-  const volatile int* t = reinterpret_cast<const volatile int*>(smem + AttnTcSmem::kTab + (k & 1) * 16);
-  return {t[0], t[1], t[2], t[3]};
+  const volatile int* t = reinterpret_cast<const volatile int*>(smem + AttnTcSmem::kTab + (k & 1) * 32);
+  return {t[0], t[1], t[2], t[3], GROUPS ? t[4] : 0, GROUPS ? t[5] : 0};
 }
 
+// GROUPS: sequences may continue another one, whose keys they see as a whole in front of their own
+template <bool GROUPS>
 __global__ void __launch_bounds__(kAtThreads, 1)
 attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                    const __grid_constant__ CUtensorMap tmV, const AttnTcParams p) {
@@ -97,24 +112,25 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   }
   pdl_wait();
   // warp 2: the blocks of the longest sequence and the first item, while barriers and tensor memory are set up
-  const int* cu = p.cu_seqlens;
-  int level = 0, above = 0, upto = 0;                                // row blocks with an index > level, >= level
-  auto item_of = [&](uint32_t k) {
+  struct Item { int4 own; int2 prefix; };
+  int level = 0, above = 0, upto = 0;                                // row blocks of a level > level, >= level
+  auto item_of = [&](uint32_t k) -> Item {
     const int at = (k & 1) ? (k + 1) * gridDim.x - 1 - blockIdx.x : k * gridDim.x + blockIdx.x;
     const int rank = at / p.Hq;
     while (level > 0 && rank >= upto) {
       --level;
       above = upto;
-      upto = attn_blocks_from<kTcBM>(cu, p.num_seqs, level, lane);
+      upto = attn_blocks_of<GROUPS, false, kTcBM>(p.seqs, level, lane);
     }
-    if (rank >= upto) return make_int4(-1, 0, 0, 0);
-    const int src = attn_nth_sequence<kTcBM>(cu, p.num_seqs, level, rank - above, lane);
-    return make_int4(at - rank * p.Hq, level * kTcBM, cu[src], cu[src + 1] - cu[src]);
+    if (rank >= upto) return {make_int4(-1, 0, 0, 0), make_int2(0, 0)};
+    const int src = attn_nth_of<GROUPS, false, kTcBM>(p.seqs, level, rank - above, lane);
+    const AttnSeq q = attn_seq<GROUPS>(p.seqs, src);
+    const AttnLevels l = attn_levels<GROUPS, false, kTcBM>(p.seqs, src);
+    return {make_int4(at - rank * p.Hq, (level - (l.top - l.blocks)) * kTcBM, q.start, q.len), make_int2(q.prefix_start, q.prefix_len)};
   };
-  int4 next = make_int4(-1, 0, 0, 0);
+  Item next = {make_int4(-1, 0, 0, 0), make_int2(0, 0)};
   if (warp == 2) {
-    for (int s = lane; s < p.num_seqs; s += 32) level = max(level, (cu[s + 1] - cu[s] + kTcBM - 1) / kTcBM);
-    level = __reduce_max_sync(0xffffffffu, level);
+    level = attn_most_levels<GROUPS, false, kTcBM>(p.seqs, lane);
     next = item_of(0);
   }
   tc_fence_before();
@@ -139,7 +155,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           if (++slot == kTcSlots) { slot = 0; phase ^= 1; }
         };
         for (uint32_t k = 0;; ++k) {
-          const AttnItem it = attn_item(smem, tab_full, k);
+          const AttnItem<GROUPS> it = attn_item<GROUPS>(smem, tab_full, k);
           mbar_arrive(&tab_empty[k & 1]);
           if (it.head < 0) break;
           const int kvc = it.head / p.G * kAtD, n = max(it.blocks(0), it.blocks(1));
@@ -153,8 +169,8 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             tma_load_2d(dst + kAtPanel, &tmQ, &q_full[x], it.head * kAtD + 64, it.start + it.q0 + x * 128);
           }
           for (int j = 0; j < n; ++j) {
-            load(&tmK, kvc, it.start + j * kAtBN);
-            load(&tmV, kvc, it.start + j * kAtBN);
+            load(&tmK, kvc, it.block_row(j));
+            load(&tmV, kvc, it.block_row(j));
           }
         }
       }
@@ -171,7 +187,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         };
         const uint32_t q_addr = smem_u32(smem + L::kQ), ring = smem_u32(smem + L::kRing);
         for (uint32_t k = 0;; ++k) {
-          const AttnItem it = attn_item(smem, tab_full, k);
+          const AttnItem<GROUPS> it = attn_item<GROUPS>(smem, tab_full, k);
           mbar_arrive(&tab_empty[k & 1]);
           if (it.head < 0) break;
           const int nx[2] = {it.blocks(0), it.blocks(1)}, n = max(nx[0], nx[1]);
@@ -202,7 +218,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             }
             // keys behind the end of the sequence belong to another one: their P is 0, and groups of 16 of them stay out.  The last group
             // may hold up to 15 rows of the next sequence's V times 0: an infinity or NaN there reaches this block's rows
-            const int steps = min(8, (it.len - j * kAtBN + 15) / 16);
+            const int steps = min(8, (it.block_keys(j) + 15) / 16);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               if (j < nx[x]) {
@@ -223,14 +239,15 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     } else if (warp == 2) {
       // ============================== items ==============================
       for (uint32_t k = 0;; ++k) {
-        const int4 it = next;
+        const Item it = next;
         mbar_wait(&tab_empty[k & 1], ((k >> 1) & 1) ^ 1);
         if (lane == 0) {
-          *reinterpret_cast<int4*>(smem + L::kTab + (k & 1) * 16) = it;
+          *reinterpret_cast<int4*>(smem + L::kTab + (k & 1) * 32) = it.own;
+          if (GROUPS) *reinterpret_cast<int2*>(smem + L::kTab + (k & 1) * 32 + 16) = it.prefix;
           mbar_arrive(&tab_full[k & 1]);
         }
         __syncwarp();
-        if (it.x < 0) break;
+        if (it.own.x < 0) break;
         next = item_of(k + 1);
       }
     }
@@ -243,7 +260,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     const uint32_t t_s = tmem_base + x * kAtBN + lane_off, t_o = tmem_base + kAtTmemO + x * kAtD + lane_off;
     uint32_t n_s = 0, n_o = 0;
     for (uint32_t k = 0;; ++k) {
-      const AttnItem it = attn_item(smem, tab_full, k);
+      const AttnItem<GROUPS> it = attn_item<GROUPS>(smem, tab_full, k);
       __syncwarp();
       if (lane == 0) mbar_arrive(&tab_empty[k & 1]);
       if (it.head < 0) break;
@@ -258,10 +275,11 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(t_s + c * 32, sv[c]);
         tmem_ld_wait();
-        const int key0 = j * kAtBN;
-        // only the block on the diagonal needs a mask: the others end before the tile's first row
-        if (j == n - 1) attn_mask_block(sv, 0, min(row, it.len - 1) - key0, 0);
-        attn_softmax_block<false>(sv, p.scale_log2, t_s, t_o, j == 0, m_run, l_run, it.len - key0 <= 64);
+        const int keys = it.block_keys(j);
+        // only the block on the diagonal needs a mask (the others end before the tile's first row), and the prefix's last one where it ends inside
+        if (j == n - 1) attn_mask_block(sv, 0, min(row, it.len - 1) - (it.len - keys), 0);
+        else if (GROUPS && j == it.prefix_blocks() - 1 && keys < kAtBN) attn_mask_block(sv, 0, keys - 1, 0);
+        attn_softmax_block<false>(sv, p.scale_log2, t_s, t_o, j == 0, m_run, l_run, keys <= 64);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_ready[x]);
@@ -301,22 +319,37 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 
 }  // namespace nrl
 
+namespace nrl {
+namespace {
+
+template <bool GROUPS>
+cudaError_t attn_fwd_tc(const CUtensorMap* tmQ, const CUtensorMap* tmK, const CUtensorMap* tmV, void* out, float* lse, long o_stride_t, const AttnSeqs& seqs,
+                        int total, int Hq, int Hkv, float scale, int num_sms, cudaStream_t s) {
+  if (total == 0) return cudaSuccess;
+  AttnTcParams p;
+  p.seqs = seqs; p.out = static_cast<__nv_bfloat16*>(out); p.lse = lse; p.o_stride_t = o_stride_t;
+  p.total_tokens = total; p.Hq = Hq; p.G = Hq / Hkv;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  static PerDevice<bool> configured;
+  const cudaError_t e = allow_smem(configured, attn_fwd_tc_kernel<GROUPS>, AttnTcSmem::kTotal);
+  if (e != cudaSuccess) return e;
+  const long most = static_cast<long>(total / kTcBM + seqs.num) * Hq;
+  launch_dependent(attn_fwd_tc_kernel<GROUPS>, static_cast<int>(most < num_sms ? most : num_sms), kAtThreads, AttnTcSmem::kTotal, s, *tmQ, *tmK, *tmV, p);
+  return cudaGetLastError();
+}
+
+}  // namespace
+}  // namespace nrl
+
 extern "C" cudaError_t nrl_attn_fwd_tc(const CUtensorMap* tmQ, const CUtensorMap* tmK, const CUtensorMap* tmV, void* out,
                                        float* lse, long o_stride_t, const int* cu, int num_seqs, int total, int Hq, int Hkv,
                                        float scale, int num_sms, cudaStream_t s) {
-  using namespace nrl;
-  if (total == 0) return cudaSuccess;
-  AttnTcParams p;
-  p.cu_seqlens = cu; p.out = static_cast<__nv_bfloat16*>(out); p.lse = lse; p.o_stride_t = o_stride_t;
-  p.num_seqs = num_seqs; p.total_tokens = total; p.Hq = Hq; p.G = Hq / Hkv;
-  p.scale_log2 = scale * 1.4426950408889634f;
-  static bool configured = false;
-  if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(attn_fwd_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, AttnTcSmem::kTotal);
-    if (e != cudaSuccess) return e;
-    configured = true;
-  }
-  const long most = static_cast<long>(total / kTcBM + num_seqs) * Hq;
-  launch_dependent(attn_fwd_tc_kernel, static_cast<int>(most < num_sms ? most : num_sms), kAtThreads, AttnTcSmem::kTotal, s, *tmQ, *tmK, *tmV, p);
-  return cudaGetLastError();
+  return nrl::attn_fwd_tc<false>(tmQ, tmK, tmV, out, lse, o_stride_t, {cu, nullptr, num_seqs}, total, Hq, Hkv, scale, num_sms, s);
+}
+
+// table: attention_groups.cu
+extern "C" cudaError_t nrl_attn_groups_fwd_tc(const CUtensorMap* tmQ, const CUtensorMap* tmK, const CUtensorMap* tmV, void* out, float* lse, long o_stride_t,
+                                              const int* cu, const int* table, int num_seqs, int total, int Hq, int Hkv, float scale, int num_sms,
+                                              cudaStream_t s) {
+  return nrl::attn_fwd_tc<true>(tmQ, tmK, tmV, out, lse, o_stride_t, {cu, reinterpret_cast<const int4*>(table), num_seqs}, total, Hq, Hkv, scale, num_sms, s);
 }

@@ -48,19 +48,58 @@ NRL_DEVICE void add_bf16x2(uint32_t pair, float& lo, float& hi) {
   asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tadd.rn.f32.bf16 %0, a, %0;\n\tadd.rn.f32.bf16 %1, b, %1;\n\t}" : "+f"(lo), "+f"(hi) : "r"(pair));
 }
 
-// Packed sequences cut into blocks of BM rows, put in order by the number of blocks in front of (or behind) them: how many blocks have
-// `level` or more of them, and the n-th sequence that has more than `level` blocks (both by a whole warp).
-template <int BM>
-NRL_DEVICE int attn_blocks_from(const int* cu, int num_seqs, int level, int lane) {
+// A packed batch: sequences one after the other (cu_seqlens), and, with GROUPS, sequences that continue another one: `table` says for each of them where it
+// and its prefix lie, and how many rows from its start on see its keys (attention_groups.cu).
+struct AttnSeq { int start, len, prefix_start, prefix_len, seen_by; };
+struct AttnSeqs {
+  const int* cu;
+  const int4* table;                          // [num] x {start, length, prefix's start, its length}, {rows that see its keys, -, -, -}
+  int num;
+};
+template <bool GROUPS>
+NRL_DEVICE AttnSeq attn_seq(const AttnSeqs& b, int s) {
+  if (!GROUPS) {
+    const int start = b.cu[s], len = b.cu[s + 1] - start;
+    return {start, len, 0, 0, len};
+  }
+  const int4 a = b.table[2 * s];
+  return {a.x, a.y, a.z, a.w, b.table[2 * s + 1].x};
+}
+// A sequence's blocks of BM rows have levels, by how much work each has: of `top` levels in all, its `blocks` blocks are the last ones, [top - blocks, top).
+// Of queries (KEYS false) the level counts the blocks that they walk, prefix and what lies in front; of keys those that walk them, from the last one.
+struct AttnLevels { int top, blocks; };
+template <bool GROUPS, bool KEYS, int BM>
+NRL_DEVICE AttnLevels attn_levels(const AttnSeqs& b, int s) {
+  const AttnSeq q = attn_seq<GROUPS>(b, s);
+  const int n = (q.len + BM - 1) / BM;
+  if (!GROUPS) return {n, n};
+  return {KEYS ? (q.seen_by + BM - 1) / BM : n + (q.prefix_len + BM - 1) / BM, n};
+}
+template <bool GROUPS, bool KEYS, int BM>
+NRL_DEVICE int attn_most_levels(const AttnSeqs& b, int lane) {
   int n = 0;
-  for (int s = lane; s < num_seqs; s += 32) n += max(0, (cu[s + 1] - cu[s] + BM - 1) / BM - level);
+  for (int s = lane; s < b.num; s += 32) n = max(n, attn_levels<GROUPS, KEYS, BM>(b, s).top);
+  return __reduce_max_sync(0xffffffffu, n);
+}
+// how many blocks have `level` or a higher one, and the n-th sequence with a block of exactly that level (both by a whole warp)
+template <bool GROUPS, bool KEYS, int BM>
+NRL_DEVICE int attn_blocks_of(const AttnSeqs& b, int level, int lane) {
+  int n = 0;
+  for (int s = lane; s < b.num; s += 32) {
+    const AttnLevels l = attn_levels<GROUPS, KEYS, BM>(b, s);
+    n += min(l.blocks, max(0, l.top - level));
+  }
   return __reduce_add_sync(0xffffffffu, n);
 }
-template <int BM>
-NRL_DEVICE int attn_nth_sequence(const int* cu, int num_seqs, int level, int n, int lane) {
-  for (int s0 = 0; s0 < num_seqs; s0 += 32) {
+template <bool GROUPS, bool KEYS, int BM>
+NRL_DEVICE int attn_nth_of(const AttnSeqs& b, int level, int n, int lane) {
+  for (int s0 = 0; s0 < b.num; s0 += 32) {
     const int s = s0 + lane;
-    const bool has = s < num_seqs && (cu[s + 1] - cu[s] + BM - 1) / BM > level;
+    bool has = false;
+    if (s < b.num) {
+      const AttnLevels l = attn_levels<GROUPS, KEYS, BM>(b, s);
+      has = level < l.top && l.top - level <= l.blocks;
+    }
     const uint32_t m = __ballot_sync(0xffffffffu, has);
     const uint32_t hit = __ballot_sync(0xffffffffu, has && __popc(m & ((1u << lane) - 1)) == n);
     if (hit != 0) return s0 + __ffs(hit) - 1;

@@ -21,6 +21,7 @@
 #include "runtime.h"
 #include "bindings_hybrid.h"
 #include "bindings_vocab.h"
+#include "bindings_groups.h"
 #include "tma_host.h"
 
 namespace {
@@ -1758,4 +1759,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   nrl::bind_runtime(m);
   nrl::bind_hybrid(m);
   nrl::bind_vocab(m);
+  nrl::bind_groups(m);
 }

@@ -9,6 +9,7 @@ records which ``.so`` files were loaded).
 """
 from __future__ import annotations
 
+import math
 import os
 
 import torch
@@ -250,6 +251,137 @@ def sample_filtered(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p
     if use_native(logits):
         return _nat().sample_filtered(logits, uniforms, temperature, top_k, top_p, min_p)
     return ref.sample_filtered(logits, uniforms, temperature, top_k, top_p, min_p)
+
+
+# ---- many samples of one prompt, and a cache of bounded size ------------------------------------------------------------------
+def _check_int32(what, beside, **tensors):
+    for name, x in tensors.items():
+        if x.dtype != torch.int32 or x.device != beside.device:
+            raise TypeError(f"{what}: {name} must be int32 on {beside.device}, got {x.dtype} on {x.device}")
+
+
+def _scale_of(what, scale, q):
+    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"{what}: scale must be finite, got {scale}")
+    return scale
+
+
+def attention_shared_prefix(q, k, v, cu_seqlens, cu_groups, max_seqlen=None, scale=None):
+    """Causal attention of packed groups: ``q`` [T, Hq, D], ``k`` and ``v`` [T, Hkv, D], sequence s in rows cu_seqlens[s] .. cu_seqlens[s + 1], group g of the sequences
+    cu_groups[g] .. cu_groups[g + 1] (int32).  The first sequence of a group is the *prefix* of its others: their rows see all of it, then their own sequence up to
+    themselves, as if the prefix stood in front of each of them; it is computed once.  Lengths may be 0.  A sequence of no group, and one that is its group's only
+    one, is plain (``attention_varlen``).  Rows behind the last sequence are 0, and so are their gradients.  Differentiable once in q, k and v.
+    On CUDA bf16 and D = 128; q, k and v may be views of a projection.  ``max_seqlen`` is not needed.  A non-finite value in one sequence may reach the ones packed
+    beside it."""
+    what = "attention_shared_prefix"
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or k.shape[1] == 0 or q.shape[1] % k.shape[1]:
+        raise ValueError(f"{what}: q [T, Hq, D] and k, v [T, Hkv, D] with Hq a multiple of Hkv are needed, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if not q.dtype == k.dtype == v.dtype or not q.device == k.device == v.device:
+        raise TypeError(f"{what}: q, k and v must have one type and device")
+    if cu_seqlens.dim() != 1 or cu_groups.dim() != 1 or cu_seqlens.numel() < 1 or cu_groups.numel() < 1:
+        raise ValueError(f"{what}: cu_seqlens [sequences + 1] and cu_groups [groups + 1] are needed, got {tuple(cu_seqlens.shape)} and {tuple(cu_groups.shape)}")
+    _check_int32(what, q, cu_seqlens=cu_seqlens, cu_groups=cu_groups)
+    scale = _scale_of(what, scale, q)
+    if use_native(q):
+        if q.dtype != torch.bfloat16 or q.shape[2] != 128:
+            raise TypeError(f"{what}: on CUDA bf16 and a head size of 128 are needed, got {q.dtype} and {q.shape[2]}")
+        return _nat().attention_shared_prefix(q, k, v, cu_seqlens.contiguous(), cu_groups.contiguous(), scale)
+    return ref.attention_shared_prefix(q, k, v, cu_seqlens, cu_groups, scale)
+
+
+def _check_pages(what, q, k_cache, v_cache, block_tables, context_lens, k_scale, v_scale):
+    if k_cache.dim() != 4 or v_cache.dim() != 4 or k_cache.shape[:2] != v_cache.shape[:2] or k_cache.shape[2] != 16 or k_cache.numel() != v_cache.numel():
+        raise ValueError(f"{what}: k_cache and v_cache must be [blocks, Hkv, 16, D], got {tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
+    if (k_scale is None) != (v_scale is None):
+        raise ValueError(f"{what}: k_scale and v_scale go together")
+    if k_cache.dtype != v_cache.dtype or (k_scale is not None) != (k_cache.dtype == torch.uint8):
+        raise TypeError(f"{what}: pages are bf16, or uint8 (e4m3) with scales, got {k_cache.dtype} and {v_cache.dtype}")
+    for s in (k_scale, v_scale):
+        if s is not None and (s.dtype != torch.float32 or tuple(s.shape) != tuple(k_cache.shape[:3])):
+            raise ValueError(f"{what}: scales must be float32 {tuple(k_cache.shape[:3])}, got {s.dtype} {tuple(s.shape)}")
+    rows = context_lens.shape[0] if context_lens.dim() == 1 else -1
+    if block_tables.dim() != 2 or block_tables.shape[0] != rows or block_tables.shape[1] < 1:
+        raise ValueError(f"{what}: block_tables [rows, pages] and context_lens [rows] are needed, got {tuple(block_tables.shape)} and {tuple(context_lens.shape)}")
+    _check_int32(what, k_cache, block_tables=block_tables, context_lens=context_lens)
+    if q is not None and (q.dim() != 3 or q.shape[0] != rows or q.shape[2] != k_cache.shape[3] or q.shape[1] % k_cache.shape[1] or q.shape[1] // k_cache.shape[1] > 8):
+        raise ValueError(f"{what}: q must be [{rows}, Hq, {k_cache.shape[3]}] with Hq a multiple, at most 8 times, of {k_cache.shape[1]}, got {tuple(q.shape)}")
+
+
+def paged_decode_shared(q, k_cache, v_cache, block_tables, context_lens, cu_groups, shared_lens, max_group=None, k_scale=None, v_scale=None, scale=None, splits=0):
+    """Decode attention, one new token per row, of rows that share their first tokens: the keys and values of those are read once per group.
+
+    ``q`` bf16 [S, Hq, 128] (views of a projection will do); pages, tables and lengths as in ``native.paged_decode`` (``k_cache`` [blocks, Hkv, 16, 128] bf16, or with
+    ``k_scale`` and ``v_scale`` [blocks, Hkv, 16] the e4m3 pages of the sampler).  Group g has rows cu_groups[g] .. cu_groups[g + 1] (int32), ``max_group`` of them at
+    most (a host number; None: S), and shares its first shared_lens[g] tokens: they are read from the pages of its first row, whatever the tables of its others say of
+    whole pages among them.  A row sees its first context_lens tokens, the shared ones among them; with none its result is 0; rows of no group are plain.
+    ``splits``: parts that the tokens behind the prefix are cut into (0: chosen).  No gradient."""
+    what = "paged_decode_shared"
+    _check_pages(what, q, k_cache, v_cache, block_tables, context_lens, k_scale, v_scale)
+    if shared_lens.dim() != 1 or tuple(cu_groups.shape) != (shared_lens.shape[0] + 1,):
+        raise ValueError(f"{what}: cu_groups [groups + 1] and shared_lens [groups] are needed, got {tuple(cu_groups.shape)} and {tuple(shared_lens.shape)}")
+    _check_int32(what, k_cache, cu_groups=cu_groups, shared_lens=shared_lens)
+    if max_group is not None and max_group < 1:
+        raise ValueError(f"{what}: max_group must be positive, got {max_group}")
+    scale = _scale_of(what, scale, q)
+    if use_native(q):
+        return _nat().paged_decode_shared(q, k_cache, v_cache, block_tables.contiguous(), context_lens.contiguous(), cu_groups.contiguous(), shared_lens.contiguous(),
+                                          max(1, q.shape[0]) if max_group is None else int(max_group), k_scale, v_scale, scale, int(splits))
+    return ref.paged_decode_shared(q, k_cache, v_cache, block_tables, context_lens, cu_groups, shared_lens, k_scale, v_scale, scale)
+
+
+def _check_scores(what, scores, k_cache, rows, name="scores"):
+    if scores.dim() != 3 or tuple(scores.shape[:2]) != (rows, k_cache.shape[1]) or scores.shape[2] < 1:
+        raise ValueError(f"{what}: {name} must be [{rows}, {k_cache.shape[1]}, tokens], got {tuple(scores.shape)}")
+    if scores.dtype != torch.float32 or scores.device != k_cache.device or (scores.stride(2) != 1 and scores.shape[2] > 1):
+        raise TypeError(f"{what}: {name} must be float32 on {k_cache.device}, the tokens of a head side by side")
+
+
+def paged_decode_scored(q, k_cache, v_cache, block_tables, context_lens, scores, decay=1.0, k_scale=None, v_scale=None, scale=None, out_scores=None, splits=0):
+    """Decode attention that adds up what weight every cached token gets: (out [S, Hq, 128], scores).
+
+    Arguments as in ``paged_decode_shared``.  ``scores`` float32 [S, Hkv, L], a row's tokens in their order: with p the attention weights,
+    scores[s, h, t] = decay * scores[s, h, t] + sum of p[s, g, t] over the query heads of kv head h; the newest token (t = context_lens[s] - 1) takes the sum alone, so
+    that its place need not be cleared.  In place, or into ``out_scores``, strides free up to the last; places from context_lens[s] on stay as they are, tokens from L on
+    have no score.  No gradient."""
+    what = "paged_decode_scored"
+    _check_pages(what, q, k_cache, v_cache, block_tables, context_lens, k_scale, v_scale)
+    _check_scores(what, scores, k_cache, q.shape[0])
+    if out_scores is not None:
+        _check_scores(what, out_scores, k_cache, q.shape[0], "out_scores")
+        if out_scores.shape != scores.shape:
+            raise ValueError(f"{what}: out_scores must be like scores, got {tuple(out_scores.shape)} and {tuple(scores.shape)}")
+    if not math.isfinite(decay):
+        raise ValueError(f"{what}: decay must be finite, got {decay}")
+    scale = _scale_of(what, scale, q)
+    if use_native(q):
+        return _nat().paged_decode_scored(q, k_cache, v_cache, block_tables.contiguous(), context_lens.contiguous(), scores, float(decay), k_scale, v_scale, scale, out_scores,
+                                          int(splits))
+    return ref.paged_decode_scored(q, k_cache, v_cache, block_tables, context_lens, scores, decay, k_scale, v_scale, scale, out_scores)
+
+
+def kv_evict(k_cache, v_cache, block_tables, context_lens, scores, keep: int, sinks: int = 0, recent: int = 0, k_scale=None, v_scale=None, out_tables=None):
+    """Rows of a paged cache over ``keep`` tokens give up the ones of least score: (kept int32 [S, Hkv, keep], their scores, new lengths int32 [S]).
+
+    A row of n = context_lens[s] > keep tokens keeps its first ``sinks``, its last ``recent`` and, of the others, those with the largest ``scores`` [S, Hkv, L]
+    (``paged_decode_scored``; ties: the lower index; NaN below everything), each kv head its own.  They move together, in order, into the first ``keep`` places of
+    the row: within its pages, or into those of ``out_tables`` [S, pages], where rows of fewer tokens are copied too.  kept[s, h, j] is where the token of place j was, -1 (score 0) behind the
+    last.  Places that nothing moves to stay as they are.  Pages that are written to must be one row's alone and, with ``out_tables``, no row's source; no context may
+    be longer than L.  Rotated keys keep their rotation: positions go on from where they were, lengths from the new ones."""
+    what = "kv_evict"
+    _check_pages(what, None, k_cache, v_cache, block_tables, context_lens, k_scale, v_scale)
+    _check_scores(what, scores, k_cache, block_tables.shape[0])
+    if int(keep) != keep or keep < 1 or sinks < 0 or recent < 0 or sinks + recent > keep:
+        raise ValueError(f"{what}: keep must be positive and at least sinks + recent, got {keep}, {sinks} and {recent}")
+    if out_tables is not None:
+        if out_tables.dim() != 2 or out_tables.shape[0] != block_tables.shape[0] or 16 * out_tables.shape[1] < min(keep, scores.shape[2], 16 * block_tables.shape[1]):
+            raise ValueError(f"{what}: out_tables must be [{block_tables.shape[0]}, pages] with room for {keep} tokens, got {tuple(out_tables.shape)}")
+        _check_int32(what, k_cache, out_tables=out_tables)
+        out_tables = out_tables.contiguous()
+    if use_native(k_cache):
+        return _nat().kv_evict(k_cache, v_cache, block_tables.contiguous(), context_lens.contiguous(), scores, int(keep), int(sinks), int(recent), k_scale, v_scale,
+                               out_tables)
+    return ref.kv_evict(k_cache, v_cache, block_tables, context_lens, scores, int(keep), int(sinks), int(recent), k_scale, v_scale, out_tables)
 
 
 def discounted_suffix_sum(rewards, gamma=1.0):

@@ -76,6 +76,106 @@ def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     return out
 
 
+def attention_shared_prefix(q, k, v, cu_seqlens, cu_groups, scale: Optional[float] = None):
+    """q: [T, Hq, D], k/v: [T, Hkv, D]; the first sequence of a group is the prefix of its others.  fp32 softmax, output in q.dtype; rows of no sequence are 0."""
+    D, g = q.shape[-1], q.shape[1] // k.shape[1]
+    scale = scale if scale is not None else 1.0 / math.sqrt(D)
+    cs, prefix_of = cu_seqlens.tolist(), {}
+    for a, b in zip(cu_groups.tolist()[:-1], cu_groups.tolist()[1:]):
+        prefix_of.update({s: a for s in range(a + 1, b)})
+    dtype, rows = q.dtype, []
+    q, k, v = q.float(), k.float(), v.float()            # (gradients of a prefix are summed over its sequences in float, too)
+    for s, (lo, hi) in enumerate(zip(cs[:-1], cs[1:])):
+        p0, p1 = (cs[prefix_of[s]], cs[prefix_of[s] + 1]) if s in prefix_of else (lo, lo)
+        n, extra = hi - lo, p1 - p0
+        ks, vs = (torch.cat([x[p0:p1], x[lo:hi]]).transpose(0, 1).repeat_interleave(g, dim=0) for x in (k, v))
+        att = torch.matmul(q[lo:hi].transpose(0, 1), ks.transpose(1, 2)) * scale
+        hidden = torch.ones(n, n, dtype=torch.bool, device=q.device).triu(1)
+        att = att.masked_fill(torch.cat([hidden.new_zeros(n, extra), hidden], 1), float("-inf"))
+        rows.append(torch.matmul(att.softmax(-1), vs).transpose(0, 1))
+    return torch.cat(rows + [q.new_zeros(q.shape[0] - cs[-1], *q.shape[1:])]).to(dtype)
+
+
+def _page_tokens(k_cache, v_cache, table, n, k_scale=None, v_scale=None):
+    """float keys and values [Hkv, n, D] of the first n tokens of a page table; fp8 pages hold e4m3 bytes, values transposed"""
+    table = table[:(n + 15) // 16].long()
+    k, v = k_cache[table], v_cache[table]
+    if k_scale is not None:
+        k = k.view(torch.float8_e4m3fn).float() * k_scale[table][..., None]
+        v = v.reshape(*v.shape[:2], k.shape[-1], 16).view(torch.float8_e4m3fn).float().transpose(2, 3) * v_scale[table][..., None, :].transpose(2, 3)
+    return tuple(x.float().transpose(0, 1).flatten(1, 2)[:, :n] for x in (k, v))
+
+
+def _decode_row(q, k, v, scale):
+    """(out [Hq, D], weights [Hkv, G, n]) of one row over keys and values [Hkv, n, D]; nothing to see: zeros"""
+    qs = q.float().view(k.shape[0], -1, q.shape[-1])
+    if k.shape[1] == 0:
+        return torch.zeros_like(q), qs.new_zeros(*qs.shape[:2], 0)
+    p = (torch.matmul(qs, k.transpose(1, 2)) * scale).softmax(-1)
+    return torch.matmul(p, v).reshape(q.shape).to(q.dtype), p
+
+
+def paged_decode_shared(q, k_cache, v_cache, block_tables, context_lens, cu_groups, shared_lens, k_scale=None, v_scale=None, scale: Optional[float] = None):
+    """A row's first tokens are read from the pages of its group's first row."""
+    scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
+    head = {}
+    for a, b, n in zip(cu_groups.tolist()[:-1], cu_groups.tolist()[1:], shared_lens.tolist()):
+        head.update({r: (a, max(0, n)) for r in range(a, b)})
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    for r, n in enumerate(context_lens.tolist()):
+        first, common = head.get(r, (r, 0))
+        common = min(common, n)
+        parts = [_page_tokens(k_cache, v_cache, block_tables[first], common, k_scale, v_scale),
+                 tuple(x[:, common:] for x in _page_tokens(k_cache, v_cache, block_tables[r], n, k_scale, v_scale))]
+        out[r] = _decode_row(q[r], *(torch.cat(x, 1) for x in zip(*parts)), scale)[0]
+    return out
+
+
+def paged_decode_scored(q, k_cache, v_cache, block_tables, context_lens, scores, decay=1.0, k_scale=None, v_scale=None, scale: Optional[float] = None,
+                        out_scores=None):
+    scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
+    out, out_scores = torch.empty(q.shape, dtype=q.dtype, device=q.device), scores if out_scores is None else out_scores
+    for r, n in enumerate(context_lens.tolist()):
+        out[r], p = _decode_row(q[r], *_page_tokens(k_cache, v_cache, block_tables[r], n, k_scale, v_scale), scale)
+        w, m = p.sum(1), min(n, scores.shape[2])
+        old = scores[r, :, :m] * decay
+        if m == n and n > 0:
+            old[:, n - 1] = 0.0
+        out_scores[r, :, :m] = old + w[:, :m]
+    return out, out_scores
+
+
+def kv_evict(k_cache, v_cache, block_tables, context_lens, scores, keep, sinks=0, recent=0, k_scale=None, v_scale=None, out_tables=None):
+    S, Hkv, L = scores.shape
+    kept = torch.full((S, Hkv, keep), -1, dtype=torch.int32, device=scores.device)
+    kept_scores = torch.zeros(S, Hkv, keep, dtype=torch.float32, device=scores.device)
+    lens = context_lens.clamp(min=0, max=min(L, 16 * block_tables.shape[1])).tolist()
+    for r, n in enumerate(lens):
+        for h in range(Hkv):
+            chosen = torch.arange(min(n, keep), device=scores.device)
+            if n > keep:
+                x = scores[r, h, sinks:n - recent]
+                x = x.masked_fill(x.isnan(), float("-inf"))
+                # a NaN is below -inf: stably by score, then numbers in front of NaN
+                order = torch.sort(x, descending=True, stable=True).indices
+                order = order[torch.sort(scores[r, h, sinks:n - recent][order].isnan().int(), stable=True).indices]
+                middle = order[:keep - sinks - recent].sort().values + sinks
+                chosen = torch.cat([chosen[:sinks], middle, torch.arange(n - recent, n, device=scores.device)])
+            m = chosen.numel()
+            kept[r, h, :m], kept_scores[r, h, :m] = chosen.int(), scores[r, h, chosen]
+            if m == 0 or (out_tables is None and n <= keep):
+                continue
+            to = block_tables[r] if out_tables is None else out_tables[r]
+            j = torch.arange(m, device=scores.device)
+            src, dst = (block_tables[r][chosen // 16].long(), chosen % 16), (to[j // 16].long(), j % 16)
+            for x, transposed in ((k_cache, False), (v_cache, k_scale is not None), (k_scale, False), (v_scale, False)):
+                if x is None:
+                    continue
+                x = x.view(*x.shape[:2], k_cache.shape[-1], 16).transpose(2, 3) if transposed else x
+                x[dst[0], h, dst[1]] = x[src[0], h, src[1]].clone()
+    return kept, kept_scores, torch.tensor(lens, dtype=torch.int32, device=scores.device).clamp_(max=keep)
+
+
 def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                            block_tables: torch.Tensor, context_lens: torch.Tensor,
                            scale: Optional[float] = None) -> torch.Tensor:
