@@ -16,10 +16,7 @@
 #include "common.cuh"
 #include "kernels.h"
 #include "decode_merge.cuh"
-#include "decode_modes.cuh"
-#include "group_kernels.h"
 #include "launch.h"
-#include "per_device.h"
 
 namespace nrl {
 
@@ -87,9 +84,7 @@ struct DecodeParams {
   float scale_log2;              // softmax scale * log2(e)
 };
 
-// MODE: decode_modes.cuh
-template <int MODE>
-__global__ void __launch_bounds__(kDecWarps * 32, 2) paged_decode_kernel(DecodeParams p, DecodeExtra x) {
+__global__ void __launch_bounds__(kDecWarps * 32, 2) paged_decode_kernel(DecodeParams p) {
   pdl_wait();
   pdl_launch_dependents();
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -98,12 +93,10 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2) paged_decode_kernel(DecodeP
   const int seq = blockIdx.x, kvh = blockIdx.y, split = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t4 = lane & 3;
-  const int ctx = MODE == kDecodePlain ? p.context_lens[seq] : min(p.context_lens[seq], p.max_blocks * kPage);
+  const int ctx = p.context_lens[seq];
   const int n_pages = (ctx + kPage - 1) / kPage;
-  const DecodeFirst from = decode_first<MODE>(x, seq, ctx, lane);
-  const int page_0 = MODE == kDecodeTail ? from.token / kPage : 0;
-  const int pages_per_split = (n_pages - page_0 + p.splits - 1) / p.splits;
-  const int page_lo = page_0 + split * pages_per_split;
+  const int pages_per_split = (n_pages + p.splits - 1) / p.splits;
+  const int page_lo = split * pages_per_split;
   const int page_hi = min(n_pages, page_lo + pages_per_split);
   const int* bt = p.block_tables + static_cast<long>(seq) * p.max_blocks;
 
@@ -164,13 +157,6 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2) paged_decode_kernel(DecodeP
     const uint32_t kb = smem_u32(my_smem + (it % kDecStages) * 2 * kPageBytes);
     const uint32_t vb = kb + kPageBytes;
     const int tok0 = (my_first + it * kDecWarps) * kPage;
-    if (MODE != kDecodePlain && (tok0 + kPage > ctx || (MODE == kDecodeTail && tok0 < from.token))) {
-      // values outside the row's own tokens, whatever they are, meet weights of 0 as zeros
-      for (int i = lane; i < kPage * 16; i += 32)
-        if (tok0 + (i >> 4) >= ctx || (MODE == kDecodeTail && tok0 + (i >> 4) < from.token))
-          *reinterpret_cast<uint4*>(my_smem + (it % kDecStages) * 2 * kPageBytes + kPageBytes + i * 16) = make_uint4(0, 0, 0, 0);
-      __syncwarp();
-    }
 
     // ---- S = Q K^T : 16 x 16 ----
     float s[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
@@ -191,14 +177,9 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2) paged_decode_kernel(DecodeP
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int tok = tok0 + nt * 8 + t4 * 2 + j;
-        s[nt][j] = (tok >= ctx || (MODE == kDecodeTail && tok < from.token)) ? -INFINITY : s[nt][j] * p.scale_log2;
+        s[nt][j] = (tok >= ctx) ? -INFINITY : s[nt][j] * p.scale_log2;
         tmax = fmaxf(tmax, s[nt][j]);
       }
-    if (MODE == kDecodeScored && g < p.G) {
-      float* raw = x.raw + ((static_cast<long>(seq) * p.Hkv + kvh) * p.G + g) * x.raw_len + tok0 + t4 * 2;
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt) *reinterpret_cast<float2*>(raw + nt * 8) = make_float2(s[nt][0], s[nt][1]);
-    }
     tmax = fmaxf(tmax, __shfl_xor_sync(0xffffffffu, tmax, 1));
     tmax = fmaxf(tmax, __shfl_xor_sync(0xffffffffu, tmax, 2));
     const float m_new = fmaxf(m_run, tmax);
@@ -265,11 +246,11 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2) paged_decode_kernel(DecodeP
       L += mml[(w * 8 + r) * 2 + 1] * c;
       acc += mo[(w * 8 + r) * kHeadDim + d] * c;
     }
-    decode_join_prefix<MODE>(x, from, p.splits, p.part_o, p.part_ml, static_cast<long>(seq) * p.Hkv + kvh, split, r, d, M, L, acc);
-    if (p.splits == 1) p.out[(static_cast<long>(seq) * p.Hq + kvh * p.G + r) * kHeadDim + d] = __float2bfloat16(L > 0.f ? acc / L : 0.f);
-    if (p.splits > 1 || MODE == kDecodeScored) {
-      const long base = ((static_cast<long>(seq) * p.Hkv + kvh) * decode_parts<MODE>(x, p.splits) + decode_part<MODE>(x, split)) * 8 + r;
-      if (p.splits > 1) p.part_o[base * kHeadDim + d] = acc;
+    if (p.splits == 1) {
+      p.out[(static_cast<long>(seq) * p.Hq + kvh * p.G + r) * kHeadDim + d] = __float2bfloat16(L > 0.f ? acc / L : 0.f);
+    } else {
+      const long base = ((static_cast<long>(seq) * p.Hkv + kvh) * p.splits + split) * 8 + r;
+      p.part_o[base * kHeadDim + d] = acc;
       if (d == 0) {
         p.part_ml[base * 2] = M;
         p.part_ml[base * 2 + 1] = L;
@@ -301,13 +282,10 @@ extern "C" cudaError_t nrl_kv_cache_write(const void* k, const void* v, long k_s
   return cudaGetLastError();
 }
 
-namespace {
-
-template <int MODE>
-cudaError_t paged_decode_mode(const void* q, long q_stride_s, const void* k_cache, const void* v_cache,
-                              const int* block_tables, const int* context_lens, void* out, float* part_o,
-                              float* part_ml, int S, int Hq, int Hkv, int head_dim, int page,
-                              int max_blocks, int splits, float scale, const DecodeExtra& x, cudaStream_t s) {
+extern "C" cudaError_t nrl_paged_decode(const void* q, long q_stride_s, const void* k_cache, const void* v_cache,
+                                        const int* block_tables, const int* context_lens, void* out, float* part_o,
+                                        float* part_ml, int S, int Hq, int Hkv, int head_dim, int page,
+                                        int max_blocks, int splits, float scale, cudaStream_t s) {
   if (head_dim != kHeadDim || page != kPage || Hq % Hkv != 0 || Hq / Hkv > 8) return cudaErrorInvalidValue;
   if (S == 0) return cudaSuccess;
   DecodeParams p;
@@ -327,36 +305,20 @@ cudaError_t paged_decode_mode(const void* q, long q_stride_s, const void* k_cach
   p.splits = splits;
   p.scale_log2 = scale * 1.4426950408889634f;
   const int smem = kDecWarps * kDecStages * 2 * kPageBytes + 16 * kHeadDim * 2;
-  static PerDevice<bool> configured;
-  cudaError_t e = allow_smem(configured, paged_decode_kernel<MODE>, smem);
-  if (e != cudaSuccess) return e;
+  static bool configured = false;
+  if (!configured) {
+    cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    configured = true;
+  }
   dim3 grid(S, Hkv, splits);
-  launch_dependent(paged_decode_kernel<MODE>, grid, kDecWarps * 32, smem, s, p, x);
-  e = cudaGetLastError();
+  launch_dependent(paged_decode_kernel, grid, kDecWarps * 32, smem, s, p);
+  cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  if (splits > 1 && MODE != kDecodeScored) {       // (scores are added where their parts are merged)
-    const MergeParams m = {part_o, part_ml, static_cast<__nv_bfloat16*>(out), Hq, Hkv, Hq / Hkv, decode_parts<MODE>(x, splits)};
+  if (splits > 1) {
+    const MergeParams m = {part_o, part_ml, static_cast<__nv_bfloat16*>(out), Hq, Hkv, Hq / Hkv, splits};
     launch_dependent(decode_merge_splits_kernel, dim3(S, Hq), kMergeD, 0, s, m);
     e = cudaGetLastError();
   }
   return e;
-}
-
-}  // namespace
-
-extern "C" cudaError_t nrl_paged_decode(const void* q, long q_stride_s, const void* k_cache, const void* v_cache,
-                                        const int* block_tables, const int* context_lens, void* out, float* part_o,
-                                        float* part_ml, int S, int Hq, int Hkv, int head_dim, int page,
-                                        int max_blocks, int splits, float scale, cudaStream_t s) {
-  return paged_decode_mode<kDecodePlain>(q, q_stride_s, k_cache, v_cache, block_tables, context_lens, out, part_o, part_ml, S, Hq, Hkv, head_dim, page,
-                                         max_blocks, splits, scale, DecodeExtra{}, s);
-}
-
-cudaError_t nrl::paged_decode_tail_bf16(const DecodeCall& c, const DecodeExtra& x, cudaStream_t s) {
-  return paged_decode_mode<kDecodeTail>(c.q, c.q_stride_s, c.k_cache, c.v_cache, c.block_tables, c.context_lens, c.out, c.part_o, c.part_ml, c.S, c.Hq, c.Hkv, c.D,
-                                        c.page, c.max_blocks, c.splits, c.scale, x, s);
-}
-cudaError_t nrl::paged_decode_scored_bf16(const DecodeCall& c, const DecodeExtra& x, cudaStream_t s) {
-  return paged_decode_mode<kDecodeScored>(c.q, c.q_stride_s, c.k_cache, c.v_cache, c.block_tables, c.context_lens, c.out, c.part_o, c.part_ml, c.S, c.Hq, c.Hkv,
-                                          c.D, c.page, c.max_blocks, c.splits, c.scale, x, s);
 }

@@ -29,11 +29,8 @@
 #include "common.cuh"
 #include "kernels.h"
 #include "decode_merge.cuh"
-#include "decode_modes.cuh"
 #include "fp8_fragments.cuh"
-#include "group_kernels.h"
 #include "launch.h"
-#include "per_device.h"
 
 #include <type_traits>
 
@@ -103,21 +100,17 @@ struct Decode8Params {
   float scale_log2;
 };
 
-// MODE: decode_modes.cuh
-template <int MODE>
-__global__ void __launch_bounds__(kWarps8 * 32, 3) paged_decode_fp8_kernel(Decode8Params p, DecodeExtra x) {
+__global__ void __launch_bounds__(kWarps8 * 32, 3) paged_decode_fp8_kernel(Decode8Params p) {
   pdl_wait();
   pdl_launch_dependents();
   extern __shared__ __align__(128) uint8_t smem[];
   const int seq = blockIdx.x, kvh = blockIdx.y, split = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t4 = lane & 3;
-  const int ctx = MODE == kDecodePlain ? p.context_lens[seq] : min(p.context_lens[seq], p.max_blocks * kPg);
+  const int ctx = p.context_lens[seq];
   const int n_pages = (ctx + kPg - 1) / kPg;
-  const DecodeFirst from = decode_first<MODE>(x, seq, ctx, lane);
-  const int page_0 = MODE == kDecodeTail ? from.token / kPg : 0;
-  const int pages_per_split = (n_pages - page_0 + p.splits - 1) / p.splits;
-  const int page_lo = page_0 + split * pages_per_split;
+  const int pages_per_split = (n_pages + p.splits - 1) / p.splits;
+  const int page_lo = split * pages_per_split;
   const int page_hi = min(n_pages, page_lo + pages_per_split);
   const int* bt = p.block_tables + static_cast<long>(seq) * p.max_blocks;
 
@@ -217,25 +210,6 @@ __global__ void __launch_bounds__(kWarps8 * 32, 3) paged_decode_fp8_kernel(Decod
           for (int e = 0; e < 2; ++e)
             if (tok0 + u * kWarps8 * kPg + t4 * 4 + 2 * j + e >= ctx) s[u][j][e] = -INFINITY;
       }
-      const int page0 = tok0 + u * kWarps8 * kPg;
-      if (MODE == kDecodeTail && page0 < from.token) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (page0 + t4 * 4 + 2 * j + e < from.token) s[u][j][e] = -INFINITY;
-      }
-      if (MODE != kDecodePlain && (page0 + kPg > ctx || (MODE == kDecodeTail && page0 < from.token))) {
-        // values and scales outside the row's own tokens, whatever they are, meet weights of 0 as zeros
-        const int lo = MODE == kDecodeTail ? from.token - page0 : 0, hi = ctx - page0;
-        fp8_clear_values(my_smem + ((it + u) % kStages8) * kStage8 + kRawPage, lo, hi, lane);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) vscale[u][i] = t4 * 4 + i >= lo && t4 * 4 + i < hi ? vscale[u][i] : 0.f;
-      }
-      if (MODE == kDecodeScored && g < p.G) {
-        float* raw = x.raw + ((static_cast<long>(seq) * p.Hkv + kvh) * p.G + g) * x.raw_len + tok0 + u * kWarps8 * kPg + t4 * 4;
-        *reinterpret_cast<float4*>(raw) = make_float4(s[u][0][0], s[u][0][1], s[u][1][0], s[u][1][1]);
-      }
       tmax = fmaxf(tmax, fmaxf(fmaxf(s[u][0][0], s[u][0][1]), fmaxf(s[u][1][0], s[u][1][1])));
     }
     tmax = fmaxf(tmax, __shfl_xor_sync(0xffffffffu, tmax, 1));
@@ -308,11 +282,11 @@ __global__ void __launch_bounds__(kWarps8 * 32, 3) paged_decode_fp8_kernel(Decod
       acc += mo[(w * 8 + r) * kHd + d] * c;
     }
     acc *= (1.f / kPScale);
-    decode_join_prefix<MODE>(x, from, p.splits, p.part_o, p.part_ml, static_cast<long>(seq) * p.Hkv + kvh, split, r, d, M, L, acc);
-    if (p.splits == 1) p.out[(static_cast<long>(seq) * p.Hq + kvh * p.G + r) * kHd + d] = __float2bfloat16(L > 0.f ? acc / L : 0.f);
-    if (p.splits > 1 || MODE == kDecodeScored) {
-      const long base = ((static_cast<long>(seq) * p.Hkv + kvh) * decode_parts<MODE>(x, p.splits) + decode_part<MODE>(x, split)) * 8 + r;
-      if (p.splits > 1) p.part_o[base * kHd + d] = acc;
+    if (p.splits == 1) {
+      p.out[(static_cast<long>(seq) * p.Hq + kvh * p.G + r) * kHd + d] = __float2bfloat16(L > 0.f ? acc / L : 0.f);
+    } else {
+      const long base = ((static_cast<long>(seq) * p.Hkv + kvh) * p.splits + split) * 8 + r;
+      p.part_o[base * kHd + d] = acc;
       if (d == 0) {
         p.part_ml[base * 2] = M;
         p.part_ml[base * 2 + 1] = L;
@@ -342,13 +316,10 @@ extern "C" cudaError_t nrl_kv_cache_write_fp8(const void* k, const void* v, long
   return cudaGetLastError();
 }
 
-namespace {
-
-template <int MODE>
-cudaError_t paged_decode_fp8_mode(const void* q, long q_stride_s, const void* kq, const void* vq, const float* ks,
-                                  const float* vs, const int* block_tables, const int* context_lens, void* out,
-                                  float* part_o, float* part_ml, int S, int Hq, int Hkv, int head_dim, int page,
-                                  int max_blocks, int splits, float scale, const DecodeExtra& x, cudaStream_t s) {
+extern "C" cudaError_t nrl_paged_decode_fp8(const void* q, long q_stride_s, const void* kq, const void* vq, const float* ks,
+                                            const float* vs, const int* block_tables, const int* context_lens, void* out,
+                                            float* part_o, float* part_ml, int S, int Hq, int Hkv, int head_dim, int page,
+                                            int max_blocks, int splits, float scale, cudaStream_t s) {
   if (head_dim != kHd || page != kPg || Hq % Hkv != 0 || Hq / Hkv > 8) return cudaErrorInvalidValue;
   if (S == 0) return cudaSuccess;
   Decode8Params p;
@@ -363,35 +334,19 @@ cudaError_t paged_decode_fp8_mode(const void* q, long q_stride_s, const void* kq
   p.max_blocks = max_blocks; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.splits = splits;
   p.scale_log2 = scale * 1.4426950408889634f;
   const int smem = kWarps8 * kStages8 * kStage8;          // 67,584 B (>= the 16.3 KB the warp merge needs)
-  static PerDevice<bool> configured;
-  cudaError_t e = allow_smem(configured, paged_decode_fp8_kernel<MODE>, smem);
+  static bool configured = false;
+  if (!configured) {
+    cudaError_t e = cudaFuncSetAttribute(paged_decode_fp8_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    configured = true;
+  }
+  launch_dependent(paged_decode_fp8_kernel, dim3(S, Hkv, splits), kWarps8 * 32, smem, s, p);
+  cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  launch_dependent(paged_decode_fp8_kernel<MODE>, dim3(S, Hkv, splits), kWarps8 * 32, smem, s, p, x);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  if (splits > 1 && MODE != kDecodeScored) {       // (scores are added where their parts are merged)
-    const MergeParams m = {part_o, part_ml, static_cast<__nv_bfloat16*>(out), Hq, Hkv, Hq / Hkv, decode_parts<MODE>(x, splits)};
+  if (splits > 1) {
+    const MergeParams m = {part_o, part_ml, static_cast<__nv_bfloat16*>(out), Hq, Hkv, Hq / Hkv, splits};
     launch_dependent(decode8_merge_splits_kernel, dim3(S, Hq), kMergeD, 0, s, m);
     e = cudaGetLastError();
   }
   return e;
-}
-
-}  // namespace
-
-extern "C" cudaError_t nrl_paged_decode_fp8(const void* q, long q_stride_s, const void* kq, const void* vq, const float* ks,
-                                            const float* vs, const int* block_tables, const int* context_lens, void* out,
-                                            float* part_o, float* part_ml, int S, int Hq, int Hkv, int head_dim, int page,
-                                            int max_blocks, int splits, float scale, cudaStream_t s) {
-  return paged_decode_fp8_mode<kDecodePlain>(q, q_stride_s, kq, vq, ks, vs, block_tables, context_lens, out, part_o, part_ml, S, Hq, Hkv, head_dim, page,
-                                             max_blocks, splits, scale, DecodeExtra{}, s);
-}
-
-cudaError_t nrl::paged_decode_tail_fp8(const DecodeCall& c, const DecodeExtra& x, cudaStream_t s) {
-  return paged_decode_fp8_mode<kDecodeTail>(c.q, c.q_stride_s, c.k_cache, c.v_cache, c.k_scale, c.v_scale, c.block_tables, c.context_lens, c.out, c.part_o, c.part_ml,
-                                            c.S, c.Hq, c.Hkv, c.D, c.page, c.max_blocks, c.splits, c.scale, x, s);
-}
-cudaError_t nrl::paged_decode_scored_fp8(const DecodeCall& c, const DecodeExtra& x, cudaStream_t s) {
-  return paged_decode_fp8_mode<kDecodeScored>(c.q, c.q_stride_s, c.k_cache, c.v_cache, c.k_scale, c.v_scale, c.block_tables, c.context_lens, c.out, c.part_o,
-                                              c.part_ml, c.S, c.Hq, c.Hkv, c.D, c.page, c.max_blocks, c.splits, c.scale, x, s);
 }

@@ -110,22 +110,22 @@ Pages check_pages(const torch::Tensor& k, const torch::Tensor& v, const c10::opt
   return {fp8, k.size(0), k.size(1)};
 }
 
+// the call and its result
 struct DecodeTensors {
-  torch::Tensor out, part_o, part_ml;
+  torch::Tensor out;
   nrl::DecodeCall c;
 };
-// the call, its result and `more` parts a row beside its own
 DecodeTensors decode_call(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& tables, const torch::Tensor& context,
-                          const c10::optional<torch::Tensor>& ks, const c10::optional<torch::Tensor>& vs, double scale, int64_t splits, const char* what) {
+                          const c10::optional<torch::Tensor>& ks, const c10::optional<torch::Tensor>& vs, double scale, const char* what) {
   check_rows(q, what, "q");
   const Pages pages = check_pages(k, v, ks, vs, what);
   TORCH_CHECK(k.device() == q.device(), what, ": pages and q must be on one device");
   check_ints(tables, q, 2, what, "block_tables");
   check_ints(context, q, 1, what, "context_lens");
   const int64_t S = q.size(0), Hq = q.size(1);
-  TORCH_CHECK(tables.size(0) == S && context.size(0) == S && tables.size(1) >= 1 && tables.size(1) < kIntMax / 16, what, ": block_tables [rows, pages] and context_lens [rows]");
-  TORCH_CHECK(pages.kv > 0 && Hq % pages.kv == 0 && Hq / pages.kv <= 8 && pages.kv <= 65535, what, ": the query heads must be a multiple, at most 8 times, of the kv heads");
-  TORCH_CHECK(splits >= 0 && splits <= 64, what, ": splits must be between 0 (chosen) and 64");
+  TORCH_CHECK(tables.size(0) == S && context.size(0) == S && tables.size(1) >= 1, what, ": block_tables [rows, pages] and context_lens [rows]");
+  TORCH_CHECK(S * tables.size(1) * std::max<int64_t>(1, pages.kv) <= kIntMax / 16 && tables.size(1) <= kIntMax / 512, what, ": too many rows or pages");
+  TORCH_CHECK(pages.kv > 0 && Hq % pages.kv == 0 && Hq / pages.kv <= 8 && pages.kv <= 256, what, ": the query heads must be a multiple, at most 8 times, of the kv heads");
   DecodeTensors t;
   t.out = torch::empty({S, Hq, 128}, q.options());
   nrl::DecodeCall& c = t.c;
@@ -138,41 +138,34 @@ DecodeTensors decode_call(const torch::Tensor& q, const torch::Tensor& k, const 
   c.block_tables = tables.data_ptr<int>();
   c.context_lens = context.data_ptr<int>();
   c.out = t.out.data_ptr();
-  c.part_o = c.part_ml = nullptr;
   c.S = S; c.Hq = Hq; c.Hkv = pages.kv; c.D = 128; c.page = 16; c.max_blocks = tables.size(1);
   c.scale = static_cast<float>(scale);
-  const int64_t blocks = std::max<int64_t>(1, S * pages.kv);
-  // two blocks an SM; a part has a page at least
-  c.splits = splits > 0 ? splits : std::max<int64_t>(1, std::min<int64_t>({8, (2 * num_sms() + blocks - 1) / blocks, tables.size(1)}));
   return t;
 }
-void add_parts(DecodeTensors& t, const torch::Tensor& q, int64_t parts, bool results, const char* what) {
-  nrl::DecodeCall& c = t.c;
-  TORCH_CHECK(static_cast<int64_t>(c.S) * c.Hkv * parts * 8 <= kIntMax, what, ": too many rows");
-  const auto f32 = q.options().dtype(torch::kFloat32);
-  if (results) t.part_o = torch::empty({c.S, c.Hkv, parts, 8, 128}, f32);
-  t.part_ml = torch::empty({c.S, c.Hkv, parts, 8, 2}, f32);
-  c.part_o = results ? t.part_o.data_ptr<float>() : nullptr;
-  c.part_ml = t.part_ml.data_ptr<float>();
-}
+torch::Tensor scratch_of(size_t bytes, const torch::Tensor& q) { return torch::empty({static_cast<int64_t>(bytes)}, q.options().dtype(torch::kUInt8)); }
 
 torch::Tensor paged_decode_shared(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& tables, const torch::Tensor& context,
                                   const torch::Tensor& cu_groups, const torch::Tensor& shared, int64_t max_group, const c10::optional<torch::Tensor>& ks,
-                                  const c10::optional<torch::Tensor>& vs, double scale, int64_t splits) {
+                                  const c10::optional<torch::Tensor>& vs, double scale) {
   const char* what = "paged_decode_shared";
   TORCH_CHECK(q.is_cuda(), what, ": q must be a CUDA tensor");
   c10::cuda::CUDAGuard guard(q.device());
-  DecodeTensors t = decode_call(q, k, v, tables, context, ks, vs, scale, splits, what);
+  const DecodeTensors t = decode_call(q, k, v, tables, context, ks, vs, scale, what);
+  const nrl::DecodeCall& c = t.c;
   check_ints(cu_groups, q, 1, what, "cu_groups");
   check_ints(shared, q, 1, what, "shared_lens");
   const int64_t groups = shared.numel();
   TORCH_CHECK(cu_groups.numel() == groups + 1, what, ": cu_groups must be [groups + 1] and shared_lens [groups]");
   TORCH_CHECK(max_group >= 1, what, ": max_group must be positive");
-  if (t.c.S == 0) return t.out;
-  max_group = std::min<int64_t>(max_group, t.c.S);
-  const int parts = groups > 0 ? nrl_decode_prefix_parts(groups, max_group, t.c.Hq, t.c.Hkv, t.c.max_blocks, num_sms()) : 0;
-  add_parts(t, q, parts + t.c.splits, true, what);
-  check(nrl_paged_decode_shared(&t.c, cu_groups.data_ptr<int>(), shared.data_ptr<int>(), groups, max_group, parts, cur_stream()), what);
+  if (c.S == 0) return t.out;
+  max_group = std::min<int64_t>(max_group, c.S);
+  const int parts = groups > 0 ? nrl_decode_prefix_parts(groups, max_group, c.Hq, c.Hkv, c.max_blocks, num_sms()) : 0;
+  const int64_t lines = static_cast<int64_t>(c.S) * c.Hkv * parts * 8;
+  TORCH_CHECK(lines <= kIntMax, what, ": too many rows");
+  const torch::Tensor prefix = torch::empty({lines * 130}, q.options().dtype(torch::kFloat32)), scratch = scratch_of(nrl_decode_flat_scratch(&c, num_sms()), q);
+  float* prefix_o = parts > 0 ? prefix.data_ptr<float>() : nullptr;
+  check(nrl_paged_decode_shared(&c, cu_groups.data_ptr<int>(), shared.data_ptr<int>(), groups, max_group, parts, prefix_o, prefix_o + lines * 128, scratch.data_ptr(),
+                                num_sms(), cur_stream()), what);
   return t.out;
 }
 
@@ -184,20 +177,19 @@ void check_scores(const torch::Tensor& s, int64_t S, int64_t kv, const torch::Te
 
 torch::Tensor paged_decode_scored(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& tables, const torch::Tensor& context,
                                   const torch::Tensor& scores, torch::Tensor out_scores, double decay, const c10::optional<torch::Tensor>& ks,
-                                  const c10::optional<torch::Tensor>& vs, double scale, int64_t splits) {
+                                  const c10::optional<torch::Tensor>& vs, double scale) {
   const char* what = "paged_decode_scored";
   TORCH_CHECK(q.is_cuda(), what, ": q must be a CUDA tensor");
   c10::cuda::CUDAGuard guard(q.device());
-  DecodeTensors t = decode_call(q, k, v, tables, context, ks, vs, scale, splits, what);
+  const DecodeTensors t = decode_call(q, k, v, tables, context, ks, vs, scale, what);
   const nrl::DecodeCall& c = t.c;
   check_scores(scores, c.S, c.Hkv, q, what, "scores");
   check_scores(out_scores, c.S, c.Hkv, q, what, "out_scores");
   TORCH_CHECK(out_scores.size(2) == scores.size(2), what, ": out_scores must be like scores");
   if (c.S == 0) return t.out;
-  add_parts(t, q, c.splits, c.splits > 1, what);
-  const torch::Tensor raw = torch::empty({c.S, c.Hq, 16LL * c.max_blocks}, q.options().dtype(torch::kFloat32));
+  const torch::Tensor raw = torch::empty({c.S, c.Hq, 16LL * c.max_blocks}, q.options().dtype(torch::kFloat32)), scratch = scratch_of(nrl_decode_flat_scratch(&c, num_sms()), q);
   check(nrl_paged_decode_scored(&c, scores.data_ptr<float>(), scores.stride(0), scores.stride(1), out_scores.data_ptr<float>(), out_scores.stride(0), out_scores.stride(1),
-                                scores.size(2), static_cast<float>(decay), raw.data_ptr<float>(), cur_stream()), what);
+                                scores.size(2), static_cast<float>(decay), raw.data_ptr<float>(), scratch.data_ptr(), num_sms(), cur_stream()), what);
   return t.out;
 }
 
@@ -214,6 +206,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> kv_evict(torch::Tensor k
   TORCH_CHECK(context.size(0) == S && tables.size(1) >= 1 && pages.kv > 0 && pages.kv <= 65535, what, ": block_tables [rows, pages] and context_lens [rows]");
   check_scores(scores, S, pages.kv, k, what, "scores");
   TORCH_CHECK(keep >= 1 && keep <= kIntMax / 2 && sinks >= 0 && recent >= 0 && sinks + recent <= keep, what, ": keep must be positive and at least sinks + recent");
+  TORCH_CHECK(pages.blocks * pages.kv * 16 <= kIntMax && (std::min<int64_t>(keep, scores.size(2)) + 511) / 512 * pages.kv <= 65535, what, ": too many tokens");
   if (out_tables.has_value()) {
     check_ints(*out_tables, k, 2, what, "out_tables");
     TORCH_CHECK(out_tables->size(0) == S && out_tables->size(1) >= 1, what, ": out_tables must be [rows, pages]");
@@ -238,7 +231,9 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> kv_evict(torch::Tensor k
   // no token is looked for behind the scores or behind the tables
   c.max_tokens = std::min<int64_t>(scores.size(2), 16 * tables.size(1));
   c.keep = keep; c.sinks = sinks; c.recent = recent;
-  check(nrl_kv_evict(&c, cur_stream()), what);
+  const torch::Tensor bits = torch::empty({S, pages.kv, (c.max_tokens + 31) / 32}, tables.options());
+  c.bits = reinterpret_cast<unsigned*>(bits.data_ptr<int>());
+  check(nrl_kv_evict(&c, num_sms(), cur_stream()), what);
   return {kept, kept_scores, lens};
 }
 

@@ -1,0 +1,641 @@
+// Decode attention over the pages of rows whose contexts differ: behind a shared prefix (decode_prefix.cu) and with scores.
+//
+//   out = sum_parts 2^(m_p - M) O_p / sum_parts 2^(m_p - M) l_p,  a part being the (maximum, sum, unnormalised result) of some of the row's keys
+//   scores[s, h, t] = decay * scores[s, h, t] + sum over the G heads of kv head h of 2^(x - M) / L     (the newest token: the sum alone)
+//
+// The pages of all rows and kv heads, one behind the other, are dealt to the warps of the chip in equal runs: no block is longer than another, none starts
+// again for every row, and few long contexts are cut as finely as many short ones.
+//   decode_plan   (one block) adds up the rows' pages and finds where every warp's run begins
+//   decode_flat   a warp walks its run through its own ring of pages (cp.async); of every row that it meets it leaves a part.  Run w and row-head r meet
+//                 in part w + r: along the runs one of the two grows by one at a time
+//   decode_join   a warp a row and head joins the parts, the prefix's too, in their order; with scores, further blocks form the weights from the scores that the
+//                 walk left in scratch memory (4 G bytes a token beside the 512 or 264 of its keys and values; what fits L2 is not read from memory again)
+// The arithmetic is that of attention_decode.cu and attention_decode_fp8.cu.  Bound by memory.
+#include "common.cuh"
+#include "fp8_fragments.cuh"
+#include "group_kernels.h"
+#include "launch.h"
+#include "per_device.h"
+
+#include <type_traits>
+
+namespace nrl {
+
+constexpr int kFlatWarps = 4;
+constexpr int kFlatD = 128;
+constexpr int kPlanThreads = 1024;
+constexpr float kFlatScale = 1024.f;              // of fp8 weights, which are f16 (2^10: small ones stay normal)
+
+template <bool FP8>
+struct FlatSizes {
+  static constexpr int kHalf = FP8 ? 2048 : 4096;                    // K or V of a page
+  static constexpr int kStage = 2 * kHalf + (FP8 ? 128 : 0);         // K, V, k_scale[16], v_scale[16]
+  static constexpr int kStages = FP8 ? 4 : 3;
+  static constexpr int kBlocks = FP8 ? 3 : 2;                        // an SM
+  static constexpr int kTotal = kFlatWarps * kStages * kStage;
+};
+
+struct FlatParams {
+  const __nv_bfloat16* q;
+  const uint8_t *k, *v;
+  const float *ks, *vs;
+  const int *block_tables, *context_lens, *cu_groups, *shared;
+  int4* rows;                   // [S] first token that the row walks itself, pages of the rows in front (of one kv head), its own pages, whether it has a prefix;
+                                // [S]: -, pages of all rows, pages a run, -
+  int4* starts;                 // [runs] row, kv head, page of the row's own, -
+  float *part_o, *part_ml;      // [runs + S Hkv, 8, D], [.., 8, 2]
+  float* raw;                   // scores in log2 units [S, Hkv, G, 16 max_blocks] (null: none)
+  const float *prefix_o, *prefix_ml;   // [S, Hkv, prefix_parts, 8, D], [.., 2]
+  __nv_bfloat16* out;
+  const float* scores_in;
+  float* scores_out;
+  long q_stride_s, in_row, in_head, out_row, out_head;
+  int n_groups, prefix_parts, S, max_blocks, Hq, Hkv, G, runs, least, max_tokens, chunk, wide;
+  float scale_log2, decay;
+};
+
+NRL_DEVICE int flat_context(const FlatParams& p, int s) { return max(0, min(p.context_lens[s], p.max_blocks * 16)); }
+// the last group that begins at or in front of a row; it has the row if it does not end there
+NRL_DEVICE int group_search(const int* cu, int n, int row) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cu[mid] <= row) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) decode_plan_kernel(const FlatParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  __shared__ int warp_sums[32];
+  __shared__ int cu_near[kPlanThreads + 1];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int* cu = p.cu_groups;
+  if (p.n_groups > 0 && p.n_groups <= kPlanThreads) {
+    for (int i = tid; i <= p.n_groups; i += kPlanThreads) cu_near[i] = p.cu_groups[i];
+    cu = cu_near;
+    __syncthreads();
+  }
+  int before = 0, off = 0, n = 0;                                    // pages of the rows in front of this pass; of this thread's row in the last one
+  for (int s0 = 0; s0 < p.S; s0 += kPlanThreads) {
+    const int s = s0 + tid;
+    int first = 0, prefix = 0;
+    n = 0;
+    if (s < p.S) {
+      const int ctx = flat_context(p, s);
+      if (p.n_groups > 0) {
+        const int g = group_search(cu, p.n_groups, s);
+        if (cu[g] <= s && s < cu[g + 1]) {
+          const int shared = p.shared[g];
+          prefix = shared > 0;
+          first = max(0, min(shared, ctx));
+        }
+      }
+      n = (ctx + 15) / 16 - first / 16;
+    }
+    int upto = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += v;
+    }
+    if (lane == 31) warp_sums[warp] = upto;
+    __syncthreads();
+    const int mine = warp_sums[lane];
+    int sums = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, sums, d);
+      if (lane >= d) sums += v;
+    }
+    const int in_front = __shfl_sync(0xffffffffu, sums - mine, warp), all = __shfl_sync(0xffffffffu, sums, 31);
+    off = before + in_front + upto - n;
+    if (s < p.S) p.rows[s] = make_int4(first, off, n, prefix);
+    before += all;
+    __syncthreads();
+  }
+  const int run = max(p.least, (before * p.Hkv + p.runs - 1) / p.runs);
+  if (tid == 0) p.rows[p.S] = make_int4(0, before, run, 0);
+  // the beginnings of the runs that begin in a row
+  for (int s0 = 0; s0 < p.S; s0 += kPlanThreads) {
+    if (p.S > kPlanThreads) {                                        // (a block sees its own writes)
+      const int4 row = s0 + tid < p.S ? p.rows[s0 + tid] : make_int4(0, 0, 0, 0);
+      off = row.y;
+      n = row.z;
+    }
+    // (all positions are below 2^27: checked on the host)
+    const int s = s0 + tid, a = off * p.Hkv, w0 = s < p.S ? (a + run - 1) / run : 0, some = s < p.S && n > 0 ? max(0, (a + n * p.Hkv + run - 1) / run - w0) : 0;
+    auto begin = [&](int w, int row, int a_row, int n_row) {
+      const int at = w * run - a_row, h = at / n_row;
+      p.starts[w] = make_int4(row, h, at - h * n_row, 0);
+    };
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < some) begin(w0 + i, s, a, n);
+    for (uint32_t many = __ballot_sync(0xffffffffu, some > 4); many != 0; many &= many - 1) {        // few rows with many runs
+      const int l = __ffs(many) - 1, a_l = __shfl_sync(0xffffffffu, a, l), n_l = __shfl_sync(0xffffffffu, n, l), w_l = __shfl_sync(0xffffffffu, w0, l),
+                some_l = __shfl_sync(0xffffffffu, some, l);
+      for (int i = 4 + lane; i < some_l; i += 32) begin(w_l + i, s0 + warp * 32 + l, a_l, n_l);
+    }
+  }
+}
+
+NRL_DEVICE void flat_ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+NRL_DEVICE void flat_ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+// rows 8..15 of the A tile are padding (G <= 8 query heads)
+NRL_DEVICE void flat_mma_bf16(float (&d)[4], uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(0u), "r"(a2), "r"(0u), "r"(b0), "r"(b1));
+}
+
+// A place in the run: a row-head and a page of its own.
+struct FlatAt {
+  int s, h, page, pages;        // pages: of the row; page < pages
+  int first, ctx;               // the row's first token of its own, its context
+};
+NRL_DEVICE void flat_row(const FlatParams& p, FlatAt& a, int s) {
+  const int4 row = p.rows[s];
+  a.s = s;
+  a.first = row.x;
+  a.pages = row.z;
+  a.ctx = flat_context(p, s);
+}
+NRL_DEVICE bool flat_next(const FlatParams& p, FlatAt& a) {          // true: another row-head begins
+  if (++a.page < a.pages) return false;
+  a.page = 0;
+  if (++a.h == p.Hkv) {
+    a.h = 0;
+    do flat_row(p, a, a.s + 1); while (a.pages == 0 && a.s + 1 < p.S);
+  }
+  return true;
+}
+
+template <bool FP8, bool SCORES>
+__global__ void __launch_bounds__(kFlatWarps * 32, FlatSizes<FP8>::kBlocks) decode_flat_kernel(const FlatParams p) {
+  // Behind decode_prefix, whose blocks have all begun when this one's do, and with that found decode_plan ended: nothing is taken from it, and only the end waits for its.
+  const bool beside = p.prefix_parts > 0;
+  if (!beside) pdl_wait();
+  pdl_launch_dependents();
+  using Z = FlatSizes<FP8>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  const int w = blockIdx.x * kFlatWarps + warp, run = p.rows[p.S].z;
+  const int count = w < p.runs ? max(0, min(run, p.rows[p.S].y * p.Hkv - w * run)) : 0;
+  if (count == 0) {
+    if (beside) pdl_wait();
+    return;
+  }
+  FlatAt here, ahead;
+  {
+    const int4 start = p.starts[w];
+    flat_row(p, here, start.x);
+    here.h = start.y;
+    here.page = start.z;
+    ahead = here;
+  }
+  uint8_t* ring = smem + warp * Z::kStages * Z::kStage;
+
+  // page numbers wait in the lanes, 32 of a row-head at a time
+  int ids = 0, ids_from = -1, issued = 0;
+  auto issue = [&]() {
+    if (issued < count) {
+      if (ids_from < 0 || ahead.page - ids_from >= 32) {
+        ids_from = ahead.page;
+        ids = ids_from + lane < ahead.pages ? p.block_tables[static_cast<long>(ahead.s) * p.max_blocks + ahead.first / 16 + ids_from + lane] : 0;
+      }
+      const long pg = static_cast<long>(__shfl_sync(0xffffffffu, ids, ahead.page - ids_from)) * p.Hkv + ahead.h;
+      uint8_t *kd = ring + (issued % Z::kStages) * Z::kStage, *vd = kd + Z::kHalf;
+      const uint8_t *ksrc = p.k + pg * Z::kHalf, *vsrc = p.v + pg * Z::kHalf;
+      if (FP8) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int chunk = lane + j * 32, r = chunk >> 3, c = chunk & 7;
+          cp_async_16(kd + r * 128 + ((c ^ k_sigma(r)) << 4), ksrc + chunk * 16);
+          cp_async_16(vd + chunk * 16, vsrc + chunk * 16);
+        }
+        if (lane < 8) cp_async_16(vd + Z::kHalf + lane * 16, (lane < 4 ? p.ks : p.vs) + pg * 16 + (lane & 3) * 4);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int chunk = lane + j * 32, at = (chunk >> 4) * 256 + (((chunk & 15) ^ ((chunk >> 4) & 7)) << 4);
+          cp_async_16(kd + at, ksrc + chunk * 16);
+          cp_async_16(vd + at, vsrc + chunk * 16);
+        }
+      }
+      if (++issued < count && flat_next(p, ahead)) ids_from = -1;
+    }
+    cp_async_commit();
+  };
+#pragma unroll 1
+  for (int i = 0; i < (FP8 ? Z::kStages : Z::kStages - 1); ++i) issue();
+
+  uint32_t qa0[8], qa2[8];                                           // row g: query head g of the kv head
+  float o[16][4];
+  float m_run = 0.f, l_run = 0.f;
+  auto enter = [&]() {                                               // a row-head's queries, nothing seen
+    const bool real = g < p.G;
+    const __nv_bfloat16* qrow = p.q + here.s * p.q_stride_s + (here.h * p.G + (real ? g : 0)) * kFlatD;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) {
+      if (FP8) {
+        const uint2 x = *reinterpret_cast<const uint2*>(qrow + (ks >> 2) * 64 + t4 * 16 + (ks & 3) * 4);
+        const float2 a = unpack_bf16x2(x.x), b = unpack_bf16x2(x.y);
+        qa0[ks] = real ? pack_f16x2(a.x, a.y) : 0u;
+        qa2[ks] = real ? pack_f16x2(b.x, b.y) : 0u;
+      } else {
+        qa0[ks] = real ? *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + t4 * 2) : 0u;
+        qa2[ks] = real ? *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + 8 + t4 * 2) : 0u;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    m_run = -INFINITY;
+    l_run = 0.f;
+  };
+  auto leave = [&]() {                                               // its part
+    float l = l_run;
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (g < p.G) {
+      const long part = (static_cast<long>(w) + static_cast<long>(here.s) * p.Hkv + here.h) * 8 + g;
+      float* dst = p.part_o + part * kFlatD + t4 * 2;
+#pragma unroll
+      for (int nd = 0; nd < 16; ++nd)
+        *reinterpret_cast<float2*>(dst + nd * 8) = make_float2(o[nd][0] * (FP8 ? 1.f / kFlatScale : 1.f), o[nd][1] * (FP8 ? 1.f / kFlatScale : 1.f));
+      if (t4 == 0) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(m_run, l);
+    }
+  };
+
+  auto step = [&](auto number, int it) {                             // pages it and, of two, it + 1 of the run, both of this row-head: one rescaling of O
+    constexpr int U = decltype(number)::value;
+    cp_async_wait<FP8 ? Z::kStages - U : Z::kStages - 1>();
+    __syncwarp();
+    const int page = here.first / 16 + here.page;
+    float s[U][2][4], vscale[U][4];
+    float top = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      uint8_t* st = ring + ((it + u) % Z::kStages) * Z::kStage;
+      const uint32_t kb = smem_u32(st);
+      const int tok0 = (page + u) * 16;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) s[u][j][0] = s[u][j][1] = s[u][j][2] = s[u][j][3] = 0.f;
+      // ---- S = Q K^T.  Key of column (j, e): bf16 8 j + 2 t + e, fp8 4 t + 2 j + e ----
+      if constexpr (FP8) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int krow = ((g >> 1) << 2) + 2 * j + (g & 1);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint4 w4 = lds128(kb + krow * 128 + (((4 * h + t4) ^ k_sigma(g)) << 4));
+            const uint32_t x[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              mma_f16_16816(s[u][j], qa0[4 * h + i], qa2[4 * h + i], e4m3x2_to_f16x2(x[i] & 0xFFFFu), e4m3x2_to_f16x2(x[i] >> 16));
+          }
+        }
+        const uint4 kr = lds128(kb + 2 * Z::kHalf + t4 * 16), vr = lds128(kb + 2 * Z::kHalf + 64 + t4 * 16);
+        const float kscale[4] = {__uint_as_float(kr.x), __uint_as_float(kr.y), __uint_as_float(kr.z), __uint_as_float(kr.w)};
+        vscale[u][0] = __uint_as_float(vr.x); vscale[u][1] = __uint_as_float(vr.y); vscale[u][2] = __uint_as_float(vr.z); vscale[u][3] = __uint_as_float(vr.w);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) s[u][j][e] *= kscale[2 * j + e] * p.scale_log2;
+      } else {
+        const int mrow = (lane & 7) + (lane >> 4) * 8, mcol = (lane >> 3) & 1;
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+          uint32_t kf[4];
+          flat_ldmatrix_x4(kf, kb + mrow * 256 + (((ks * 2 + mcol) ^ (mrow & 7)) << 4));
+          flat_mma_bf16(s[u][0], qa0[ks], qa2[ks], kf[0], kf[1]);
+          flat_mma_bf16(s[u][1], qa0[ks], qa2[ks], kf[2], kf[3]);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) s[u][j][e] *= p.scale_log2;
+      }
+      // ---- mask; values and scales outside the row's own tokens, whatever they are, meet weights of 0 as zeros ----
+      const int lo = here.first - tok0, hi = here.ctx - tok0;
+      if (lo > 0 || hi < 16) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int t = FP8 ? t4 * 4 + 2 * j + e : j * 8 + t4 * 2 + e;
+            if (t < lo || t >= hi) s[u][j][e] = -INFINITY;
+            if (FP8 && (t < lo || t >= hi)) vscale[u][2 * j + e] = 0.f;
+          }
+        if (FP8) {
+          fp8_clear_values(st + Z::kHalf, lo, hi, lane);
+        } else {
+          for (int i = lane; i < 256; i += 32)
+            if ((i >> 4) < lo || (i >> 4) >= hi) *reinterpret_cast<uint4*>(st + Z::kHalf + i * 16) = make_uint4(0, 0, 0, 0);
+          __syncwarp();
+        }
+      }
+      if (SCORES && g < p.G) {
+        float* raw = p.raw + ((static_cast<long>(here.s) * p.Hkv + here.h) * p.G + g) * (16L * p.max_blocks) + tok0;
+        if (FP8) {
+          *reinterpret_cast<float4*>(raw + t4 * 4) = make_float4(s[u][0][0], s[u][0][1], s[u][1][0], s[u][1][1]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) *reinterpret_cast<float2*>(raw + j * 8 + t4 * 2) = make_float2(s[u][j][0], s[u][j][1]);
+        }
+      }
+      top = fmaxf(top, fmaxf(fmaxf(s[u][0][0], s[u][0][1]), fmaxf(s[u][1][0], s[u][1][1])));
+    }
+    // ---- online softmax on row g ----
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const float m_new = fmaxf(m_run, top), m_sub = m_new == -INFINITY ? 0.f : m_new;
+    const float corr = exp2f(m_run - m_sub);                         // 0 while nothing has been seen
+    uint32_t pa[U][2];
+    float sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float p0 = exp2f(s[u][j][0] - m_sub), p1 = exp2f(s[u][j][1] - m_sub);
+        sum += p0 + p1;
+        pa[u][j] = FP8 ? pack_f16x2(p0 * (vscale[u][2 * j] * kFlatScale), p1 * (vscale[u][2 * j + 1] * kFlatScale)) : pack_bf16x2(p0, p1);
+      }
+    l_run = l_run * corr + sum;
+    m_run = m_new;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) { o[i][0] *= corr; o[i][1] *= corr; }
+    // ---- O += P V ----
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t vb = smem_u32(ring + ((it + u) % Z::kStages) * Z::kStage) + Z::kHalf;
+      if constexpr (FP8) {
+#pragma unroll
+        for (int nd = 0; nd < 16; ++nd) {
+          const uint32_t x = lds32(vb + (nd * 8 + g) * 16 + t4 * 4);
+          mma_f16_16816(o[nd], pa[u][0], pa[u][1], e4m3x2_to_f16x2(x & 0xFFFFu), e4m3x2_to_f16x2(x >> 16));
+        }
+      } else {
+        const int mrow = (lane & 7) + ((lane >> 3) & 1) * 8, mcol = lane >> 4;
+#pragma unroll
+        for (int nd = 0; nd < 8; ++nd) {
+          uint32_t vf[4];
+          flat_ldmatrix_x4_trans(vf, vb + mrow * 256 + (((nd * 2 + mcol) ^ (mrow & 7)) << 4));
+          flat_mma_bf16(o[nd * 2], pa[u][0], pa[u][1], vf[0], vf[1]);
+          flat_mma_bf16(o[nd * 2 + 1], pa[u][0], pa[u][1], vf[2], vf[3]);
+        }
+      }
+    }
+    __syncwarp();
+  };
+
+  enter();
+  for (int it = 0; it < count;) {
+    const bool two = FP8 && it + 1 < count && here.page + 1 < here.pages;
+    if constexpr (FP8) {
+      if (two) step(std::integral_constant<int, 2>{}, it);
+      else step(std::integral_constant<int, 1>{}, it);
+#pragma unroll 1
+      for (int u = 0; u < (two ? 2 : 1); ++u) issue();
+    } else {
+      issue();
+      step(std::integral_constant<int, 1>{}, it);
+    }
+    it += two ? 2 : 1;
+    if (two) ++here.page;
+    if (it == count) break;
+    const FlatAt last = here;
+    if (flat_next(p, here)) {
+      const FlatAt now = here;
+      here = last;
+      leave();
+      here = now;
+      enter();
+    }
+  }
+  leave();
+  cp_async_wait<0>();
+  if (beside) pdl_wait();
+}
+
+// ---- parts to results, scores to weights ---------------------------------------------------------------------------------------------
+constexpr int kJoinU = 4;                // parts in flight
+
+struct FlatParts {
+  const float2* ml;                      // of the row-head's first part: [n][8]
+  const float4* o;                       // [n][8][32]
+  int n;
+};
+NRL_DEVICE FlatParts flat_parts(const FlatParams& p, int4 row, int s, int h) {
+  const int run = p.rows[p.S].z, a = row.y * p.Hkv + h * row.z, w0 = a / run;
+  const long at = (static_cast<long>(w0) + static_cast<long>(s) * p.Hkv + h) * 8;
+  return {reinterpret_cast<const float2*>(p.part_ml) + at, reinterpret_cast<const float4*>(p.part_o) + at * 32, row.z > 0 ? (a + row.z - 1) / run - w0 + 1 : 0};
+}
+// head r's parts; a lane has four elements
+NRL_DEVICE void join_parts(const FlatParts& x, int r, int lane, float& M, float& L, float4& acc) {
+  for (int i0 = 0; i0 < x.n; i0 += kJoinU) {
+    float2 e[kJoinU];
+    float4 o[kJoinU];
+#pragma unroll
+    for (int u = 0; u < kJoinU; ++u) {
+      const bool ok = i0 + u < x.n;
+      e[u] = ok ? x.ml[(i0 + u) * 8 + r] : make_float2(-INFINITY, 0.f);
+      o[u] = ok ? x.o[((i0 + u) * 8 + r) * 32 + lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int u = 0; u < kJoinU; ++u) {
+      if (e[u].x == -INFINITY) continue;
+      const float top = fmaxf(M, e[u].x), a = exp2f(M - top), b = exp2f(e[u].x - top);          // 2^-inf = 0
+      L = L * a + e[u].y * b;
+      acc.x = acc.x * a + o[u].x * b; acc.y = acc.y * a + o[u].y * b; acc.z = acc.z * a + o[u].z * b; acc.w = acc.w * a + o[u].w * b;
+      M = top;
+    }
+  }
+}
+
+// grid: rows x (kv heads x, with scores, chunks of tokens); a warp a query head for the results, which the first chunk's blocks form
+template <bool SCORES>
+__global__ void __launch_bounds__(256) decode_join_kernel(const FlatParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int s = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = blockIdx.y % p.Hkv, chunk = blockIdx.y / p.Hkv;
+  const int ctx = flat_context(p, s), t0 = chunk * p.chunk, n = SCORES ? min(min(ctx, p.max_tokens), t0 + p.chunk) : 0;
+  if (chunk > 0 && t0 >= n) return;
+  const int4 row = p.rows[s];
+  const FlatParts own = flat_parts(p, row, s, h);
+  __shared__ float top[8], inv[8];
+  if (warp < p.G) {
+    float M = -INFINITY, L = 0.f;
+    if (chunk == 0) {
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (!SCORES && row.w) {
+        const long at = (static_cast<long>(s) * p.Hkv + h) * p.prefix_parts * 8;
+        join_parts({reinterpret_cast<const float2*>(p.prefix_ml) + at, reinterpret_cast<const float4*>(p.prefix_o) + at * 32, p.prefix_parts}, warp, lane, M, L, acc);
+      }
+      join_parts(own, warp, lane, M, L, acc);
+      const float f = L > 0.f ? 1.f / L : 0.f;
+      uint2 v;
+      v.x = pack_bf16x2(acc.x * f, acc.y * f);
+      v.y = pack_bf16x2(acc.z * f, acc.w * f);
+      *reinterpret_cast<uint2*>(p.out + (static_cast<long>(s) * p.Hq + h * p.G + warp) * kFlatD + lane * 4) = v;
+    } else {
+      for (int i = lane; i < own.n; i += 32) {
+        const float2 e = own.ml[i * 8 + warp];
+        const float m = fmaxf(M, e.x);
+        if (m == -INFINITY) continue;
+        L = L * exp2f(M - m) + e.y * exp2f(e.x - m);
+        M = m;
+      }
+      const float all = warp_max(M);
+      L = warp_sum(M == -INFINITY ? 0.f : L * exp2f(M - all));
+      M = all;
+    }
+    if (SCORES && lane == 0) {
+      top[warp] = M == -INFINITY ? 0.f : M;
+      inv[warp] = L > 0.f ? 1.f / L : 0.f;
+    }
+  }
+  if (!SCORES) return;
+  __syncthreads();
+  const long len = 16L * p.max_blocks;
+  const float* raw = p.raw + (static_cast<long>(s) * p.Hkv + h) * p.G * len;
+  const float* in = p.scores_in + s * p.in_row + h * p.in_head;
+  float* out = p.scores_out + s * p.out_row + h * p.out_head;
+  // four tokens a thread (scratch rows are multiples of 16 long)
+  for (int t = t0 + threadIdx.x * 4; t < n; t += blockDim.x * 4) {
+    float4 x[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      if (r < p.G) x[r] = *reinterpret_cast<const float4*>(raw + r * len + t);
+    float w[4] = {0.f, 0.f, 0.f, 0.f}, old[4];
+    const bool whole = t + 4 < ctx;       // none of them is the newest, all are there
+    if (whole && p.wide && t + 4 <= n) {
+      const float4 v = *reinterpret_cast<const float4*>(in + t);
+      old[0] = v.x; old[1] = v.y; old[2] = v.z; old[3] = v.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) old[i] = t + i < n && t + i < ctx - 1 ? in[t + i] : 0.f;
+    }
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      if (r < p.G) {
+        const float m = top[r], f = inv[r];
+        w[0] += exp2f(x[r].x - m) * f; w[1] += exp2f(x[r].y - m) * f; w[2] += exp2f(x[r].z - m) * f; w[3] += exp2f(x[r].w - m) * f;
+      }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = whole || t + i < ctx - 1 ? fmaf(p.decay, old[i], w[i]) : w[i];
+    if (p.wide && t + 4 <= n) {
+      *reinterpret_cast<float4*>(out + t) = make_float4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (t + i < n) out[t + i] = w[i];
+    }
+  }
+}
+
+namespace {
+
+template <bool FP8, bool SCORES>
+cudaError_t launch_flat(const FlatParams& p, cudaStream_t s) {
+  static PerDevice<bool> configured;
+  const cudaError_t e = allow_smem(configured, decode_flat_kernel<FP8, SCORES>, FlatSizes<FP8>::kTotal);
+  if (e != cudaSuccess) return e;
+  launch_dependent(decode_flat_kernel<FP8, SCORES>, (p.runs + kFlatWarps - 1) / kFlatWarps, kFlatWarps * 32, FlatSizes<FP8>::kTotal, s, p);
+  return cudaGetLastError();
+}
+
+// 16-byte pieces of scratch, one behind the other
+struct Pieces {
+  uint8_t* at;
+  size_t used = 0;
+  template <class T>
+  T* take(size_t n) {
+    T* r = reinterpret_cast<T*>(at + used);
+    used += (n * sizeof(T) + 15) / 16 * 16;
+    return r;
+  }
+};
+
+// runs: as many as warps fit the chip, or as the longest contexts that the tables allow could fill
+struct FlatPlan { int runs, least; };
+FlatPlan flat_plan(const DecodeCall* c, int num_sms) {
+  const long most = static_cast<long>(c->S) * c->Hkv * c->max_blocks;
+  const int fit = num_sms * kFlatWarps * (c->k_scale != nullptr ? FlatSizes<true>::kBlocks : FlatSizes<false>::kBlocks);
+  const int least = 2;
+  const long runs = (most + least - 1) / least;
+  return {static_cast<int>(runs < fit ? runs : fit), least};
+}
+size_t lay_out(FlatParams& p, const DecodeCall* c, const FlatPlan& plan, void* scratch) {
+  Pieces pieces = {static_cast<uint8_t*>(scratch)};
+  const size_t parts = static_cast<size_t>(plan.runs) + static_cast<size_t>(c->S) * c->Hkv;
+  p.rows = pieces.take<int4>(c->S + 1);
+  p.starts = pieces.take<int4>(plan.runs);
+  p.part_ml = pieces.take<float>(parts * 16);
+  p.part_o = pieces.take<float>(parts * 8 * kFlatD);
+  return pieces.used;
+}
+FlatParams flat_params(const DecodeCall* c, const FlatPlan& plan, void* scratch) {
+  FlatParams p = {};
+  lay_out(p, c, plan, scratch);
+  p.q = static_cast<const __nv_bfloat16*>(c->q);
+  p.k = static_cast<const uint8_t*>(c->k_cache);
+  p.v = static_cast<const uint8_t*>(c->v_cache);
+  p.ks = c->k_scale; p.vs = c->v_scale;
+  p.block_tables = c->block_tables; p.context_lens = c->context_lens;
+  p.out = static_cast<__nv_bfloat16*>(c->out);
+  p.q_stride_s = c->q_stride_s;
+  p.S = c->S; p.max_blocks = c->max_blocks; p.Hq = c->Hq; p.Hkv = c->Hkv; p.G = c->Hq / c->Hkv;
+  p.runs = plan.runs; p.least = plan.least;
+  p.scale_log2 = c->scale * 1.4426950408889634f;
+  return p;
+}
+
+}  // namespace
+}  // namespace nrl
+
+using namespace nrl;
+
+extern "C" size_t nrl_decode_flat_scratch(const DecodeCall* c, int num_sms) {
+  FlatParams p = {};
+  return lay_out(p, c, flat_plan(c, num_sms), nullptr);
+}
+
+extern "C" cudaError_t nrl_paged_decode_shared(const DecodeCall* c, const int* cu_groups, const int* shared, int n_groups, int max_group, int prefix_parts,
+                                               float* prefix_o, float* prefix_ml, void* scratch, int num_sms, cudaStream_t s) {
+  if (c->S == 0) return cudaSuccess;
+  FlatParams p = flat_params(c, flat_plan(c, num_sms), scratch);
+  p.cu_groups = cu_groups; p.shared = shared; p.n_groups = n_groups;
+  p.prefix_parts = n_groups > 0 ? prefix_parts : 0;
+  p.prefix_o = prefix_o; p.prefix_ml = prefix_ml;
+  launch_dependent(decode_plan_kernel, 1, kPlanThreads, 0, s, p);
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess && n_groups > 0) e = nrl_decode_prefix(c, cu_groups, shared, n_groups, max_group, prefix_parts, prefix_o, prefix_ml, s);
+  if (e == cudaSuccess) e = c->k_scale != nullptr ? launch_flat<true, false>(p, s) : launch_flat<false, false>(p, s);
+  if (e != cudaSuccess) return e;
+  launch_dependent(decode_join_kernel<false>, dim3(c->S, c->Hkv), 32 * p.G, 0, s, p);
+  return cudaGetLastError();
+}
+
+extern "C" cudaError_t nrl_paged_decode_scored(const DecodeCall* c, const float* scores_in, long in_row, long in_head, float* scores_out, long out_row, long out_head,
+                                               int max_tokens, float decay, float* raw, void* scratch, int num_sms, cudaStream_t s) {
+  if (c->S == 0) return cudaSuccess;
+  FlatParams p = flat_params(c, flat_plan(c, num_sms), scratch);
+  p.raw = raw; p.scores_in = scores_in; p.scores_out = scores_out;
+  p.in_row = in_row; p.in_head = in_head; p.out_row = out_row; p.out_head = out_head;
+  p.max_tokens = max_tokens < 16 * c->max_blocks ? max_tokens : 16 * c->max_blocks;
+  p.decay = decay;
+  launch_dependent(decode_plan_kernel, 1, kPlanThreads, 0, s, p);
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) e = c->k_scale != nullptr ? launch_flat<true, true>(p, s) : launch_flat<false, true>(p, s);
+  if (e != cudaSuccess) return e;
+  p.wide = (reinterpret_cast<uintptr_t>(scores_in) | reinterpret_cast<uintptr_t>(scores_out)) % 16 == 0 && (in_row | in_head | out_row | out_head) % 4 == 0;
+  // tokens a block: rows' contexts whole where there are rows enough for the chip
+  p.chunk = static_cast<long>(c->S) * c->Hkv >= 2L * num_sms ? 4096 : 512;
+  launch_dependent(decode_join_kernel<true>, dim3(c->S, c->Hkv * ((p.max_tokens + p.chunk - 1) / p.chunk)), 256, 0, s, p);
+  return cudaGetLastError();
+}

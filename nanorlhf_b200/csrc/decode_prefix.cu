@@ -2,14 +2,12 @@
 //
 //   out = sum_parts 2^(m_p - M) O_p / sum_parts 2^(m_p - M) l_p,  a part being the (maximum, sum, unnormalised result) of some of the row's keys
 //
-// Parts [0, prefix_parts) of a row are cut out of its group's prefix and formed here: the query rows of a group (samples x G heads of a kv head) are up to
-// 64 rows of a tile, every key and value of the prefix is read from memory once for all of them.  The rest of a row's tokens are the paged decode
-// kernels' (attention_decode.cu, attention_decode_fp8.cu, mode kDecodeTail), which join the parts.
+// The prefix's parts are formed here: the query rows of a group (samples x G heads of a kv head) are up to 64 rows of a tile, every key and value of the prefix is
+// read from memory once for all of them.  The rest of a row's tokens are decode_flat.cu's, which joins the parts.
 //
 // Block = 4 warps of 16 rows; 64 keys (4 pages) a step through shared memory (cp.async, three stages), mma.sync m16n8k16.  fp8 pages are dequantised on the
 // operand fragments as in attention_decode_fp8.cu.
 #include "common.cuh"
-#include "decode_modes.cuh"
 #include "fp8_fragments.cuh"
 #include "group_kernels.h"
 #include "launch.h"
@@ -38,7 +36,7 @@ struct PrefixParams {
   const int *block_tables, *context_lens, *cu_groups, *shared;
   float *part_o, *part_ml;
   long q_stride_s;
-  int S, max_blocks, Hkv, G, parts, prefix_parts, tiles;
+  int S, max_blocks, Hkv, G, prefix_parts, tiles;
   float scale_log2;
 };
 
@@ -117,7 +115,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 2) decode_prefix_kernel(const 
       const int at = tile * kPreRows + warp * 16 + g + i * 8;
       real[i] = at < n_rows;
       const int seq = seq0 + (real[i] ? at / p.G : 0), r = real[i] ? at % p.G : 0;
-      row[i] = (seq * p.Hkv + kvh) * p.parts * 8 + r;                 // of the parts, without the part (S * Hkv * parts * 8 is below 2^31: checked on the host)
+      row[i] = (seq * p.Hkv + kvh) * p.prefix_parts * 8 + r;          // of the parts, without the part (S * Hkv * parts * 8 is below 2^31: checked on the host)
       limit[i] = real[i] ? min(shared, p.context_lens[seq]) : 0;
       qrow[i] = p.q + seq * p.q_stride_s + (kvh * p.G + r) * 128;
     }
@@ -309,29 +307,20 @@ extern "C" int nrl_decode_prefix_parts(int n_groups, int max_group, int Hq, int 
   return static_cast<int>(want < 1 ? 1 : want > 16 ? (steps < 16 ? steps : 16) : (want < steps ? want : steps < 1 ? 1 : steps));
 }
 
-extern "C" cudaError_t nrl_paged_decode_shared(const DecodeCall* c, const int* cu_groups, const int* shared, int n_groups, int max_group, int prefix_parts,
-                                               cudaStream_t s) {
-  if (c->D != 128 || c->page != 16 || c->Hq % c->Hkv != 0 || c->Hq / c->Hkv > 8) return cudaErrorInvalidValue;
-  if (c->S == 0) return cudaSuccess;
-  const bool fp8 = c->k_scale != nullptr;
+extern "C" cudaError_t nrl_decode_prefix(const DecodeCall* c, const int* cu_groups, const int* shared, int n_groups, int max_group, int prefix_parts, float* prefix_o,
+                                         float* prefix_ml, cudaStream_t s) {
   PrefixParams p;
   p.q = static_cast<const __nv_bfloat16*>(c->q);
   p.k = static_cast<const uint8_t*>(c->k_cache);
   p.v = static_cast<const uint8_t*>(c->v_cache);
   p.ks = c->k_scale; p.vs = c->v_scale;
   p.block_tables = c->block_tables; p.context_lens = c->context_lens; p.cu_groups = cu_groups; p.shared = shared;
-  p.part_o = c->part_o; p.part_ml = c->part_ml;
+  p.part_o = prefix_o; p.part_ml = prefix_ml;
   p.q_stride_s = c->q_stride_s;
   p.S = c->S; p.max_blocks = c->max_blocks; p.Hkv = c->Hkv; p.G = c->Hq / c->Hkv;
-  p.parts = prefix_parts + c->splits; p.prefix_parts = prefix_parts;
+  p.prefix_parts = prefix_parts;
   p.tiles = (max_group * p.G + kPreRows - 1) / kPreRows;
   p.scale_log2 = c->scale * 1.4426950408889634f;
-  if (n_groups > 0) {
-    const dim3 grid(n_groups, c->Hkv, prefix_parts * p.tiles);
-    const cudaError_t e = fp8 ? launch_prefix<true>(p, grid, s) : launch_prefix<false>(p, grid, s);
-    if (e != cudaSuccess) return e;
-  }
-  DecodeExtra x = {};
-  x.cu_groups = cu_groups; x.shared = shared; x.n_groups = n_groups; x.prefix_parts = prefix_parts;
-  return fp8 ? paged_decode_tail_fp8(*c, x, s) : paged_decode_tail_bf16(*c, x, s);
+  const dim3 grid(n_groups, c->Hkv, prefix_parts * p.tiles);
+  return c->k_scale != nullptr ? launch_prefix<true>(p, grid, s) : launch_prefix<false>(p, grid, s);
 }

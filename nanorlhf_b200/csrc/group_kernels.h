@@ -1,11 +1,9 @@
 // Launch API of the kernels around many samples of one prompt and a cache of bounded size: decode attention behind a shared prefix and with scores
-// (decode_prefix.cu, decode_scored.cu, modes of the paged decode kernels), eviction (kv_evict.cu).  Pages have 16 tokens, heads 128 elements.
+// (decode_prefix.cu, decode_flat.cu), eviction (kv_evict.cu).  Pages have 16 tokens, heads 128 elements.
 #pragma once
 #include <cuda_runtime.h>
 
 namespace nrl {
-
-struct DecodeExtra;                       // decode_modes.cuh
 
 struct DecodeCall {
   const void* q;                          // [S, Hq, D] bf16, rows q_stride_s elements apart
@@ -14,25 +12,24 @@ struct DecodeCall {
   const float *k_scale, *v_scale;         // their scales [blocks, Hkv, 16] (null: bf16)
   const int *block_tables, *context_lens; // [S, max_blocks], [S]
   void* out;                              // [S, Hq, D] bf16
-  float *part_o, *part_ml;                // parts of rows: [S, Hkv, parts, 8, D], [S, Hkv, parts, 8, 2]
-  int S, Hq, Hkv, D, page, max_blocks, splits;
+  int S, Hq, Hkv, D, page, max_blocks;
   float scale;
 };
-
-cudaError_t paged_decode_tail_bf16(const DecodeCall& c, const DecodeExtra& x, cudaStream_t s);
-cudaError_t paged_decode_tail_fp8(const DecodeCall& c, const DecodeExtra& x, cudaStream_t s);
-cudaError_t paged_decode_scored_bf16(const DecodeCall& c, const DecodeExtra& x, cudaStream_t s);
-cudaError_t paged_decode_scored_fp8(const DecodeCall& c, const DecodeExtra& x, cudaStream_t s);
 
 }  // namespace nrl
 
 extern "C" {
-// parts that the prefix of a group is cut into; with them c.part_o and c.part_ml hold prefix_parts + c.splits parts
+// parts that the prefix of a group is cut into
 int nrl_decode_prefix_parts(int n_groups, int max_group, int Hq, int Hkv, int max_blocks, int num_sms);
-cudaError_t nrl_paged_decode_shared(const nrl::DecodeCall* c, const int* cu_groups, const int* shared, int n_groups, int max_group, int prefix_parts, cudaStream_t s);
+// the prefixes' parts alone: prefix_o [S, Hkv, prefix_parts, 8, D], prefix_ml [S, Hkv, prefix_parts, 8, 2]
+cudaError_t nrl_decode_prefix(const nrl::DecodeCall* c, const int* cu_groups, const int* shared, int n_groups, int max_group, int prefix_parts, float* prefix_o,
+                              float* prefix_ml, cudaStream_t s);
+size_t nrl_decode_flat_scratch(const nrl::DecodeCall* c, int num_sms);       // bytes of `scratch` below, on 16, for one call at a time
+cudaError_t nrl_paged_decode_shared(const nrl::DecodeCall* c, const int* cu_groups, const int* shared, int n_groups, int max_group, int prefix_parts, float* prefix_o,
+                                    float* prefix_ml, void* scratch, int num_sms, cudaStream_t s);
 // scores_in, scores_out [S, Hkv, max_tokens], rows and heads their strides apart (they may be the same memory); raw: [S, Hkv, G, 16 max_blocks] floats of scratch
 cudaError_t nrl_paged_decode_scored(const nrl::DecodeCall* c, const float* scores_in, long in_row, long in_head, float* scores_out, long out_row, long out_head,
-                                    int max_tokens, float decay, float* raw, cudaStream_t s);
+                                    int max_tokens, float decay, float* raw, void* scratch, int num_sms, cudaStream_t s);
 
 struct EvictCall {
   void *k_cache, *v_cache;                // as above, written in place
@@ -44,7 +41,8 @@ struct EvictCall {
   int* kept;                              // [S, Hkv, keep]
   float* kept_scores;                     // [S, Hkv, keep]
   int* new_lens;                          // [S]
+  unsigned* bits;                         // [S, Hkv, ceil(max_tokens / 32)] of scratch: a bit a token that is kept
   int S, Hkv, max_blocks, out_blocks, max_tokens, keep, sinks, recent;
 };
-cudaError_t nrl_kv_evict(const EvictCall* c, cudaStream_t s);
+cudaError_t nrl_kv_evict(const EvictCall* c, int num_sms, cudaStream_t s);
 }

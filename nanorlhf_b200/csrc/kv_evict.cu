@@ -1,12 +1,17 @@
 // Eviction from a paged KV cache: rows over their budget of `keep` tokens keep the first `sinks`, the last `recent` and, of the others, those with the
 // largest scores (ties: the lower index), every kv head its own; what is kept moves together, in order, into the first `keep` places.
 //
-// kv_select: a block per (row, kv head).  The scores, as whole numbers whose order is theirs, wait in shared memory (in global memory above 48 K tokens); the smallest
-// kept one is found digit by digit (11, 11 and 10 bits) from counts of the digits of what still ties with it, then every thread counts what is kept of a run of
-// neighbouring tokens, the counts are summed over the block, and the indices are written in order.
-// kv_move: a block per (row, kv head, slice of a token's keys or values).  Token j of what is kept comes from a place >= j, so that a block that reads a
-// range of places before it writes them, ranges in order, may move in place; other slices' bytes are not touched.  Values of fp8 pages lie transposed: a thread
-// has one element of all tokens, reads it sixteen tokens at a time and packs what is kept.
+// kv_select: a cluster of blocks per (row, kv head), more blocks where there are few and their contexts long.  A block has a range of tokens; their scores, as whole
+// numbers whose order is theirs, wait in shared memory (above 48 K tokens a block in global memory).  The smallest kept one is found three bits at a time: how many are at
+// or above each of seven candidates, by votes of warps and sums over the block and the cluster, until as many are above one as are to be kept.  Then the tokens are counted
+// again, word by word of 32, and indices and a bit a token are written in order.  Bound by latency, up to eleven rounds of a barrier (and one of the cluster).
+// Counts of digits by atomics meet: a score's highest bits are a few exponents, and 3750 tokens a block took 120 us with eight bits a round, 20 with eleven.
+// kv_move: a block per (row, kv head, slice of a token's keys or values), and per range of places where sources and targets are apart.  In place, token j of what
+// is kept comes from a place >= j, so that a block that reads a range of places before it writes them, ranges in order and the next one on its way, may move it;
+// other slices' bytes are not touched.
+// kv_move_transposed, at the same time: values of fp8 pages lie transposed.  Sixteen pages at a time go through shared memory, rows of 16 bytes 20 apart (no bank
+// conflicts), and a thread puts together an element's bytes of a whole page.
+#include "cluster_read.h"
 #include "common.cuh"
 #include "group_kernels.h"
 #include "launch.h"
@@ -16,8 +21,8 @@ namespace nrl {
 
 constexpr int kSelThreads = 512;
 constexpr int kSelWarps = kSelThreads / 32;
-constexpr int kSelSmemTokens = 48 * 1024;
-constexpr int kSelBins = 2048;
+constexpr int kSelTokens = 48 * 1024;     // of a block, in shared memory
+constexpr int kSelCluster = 8;
 
 // larger scores have larger keys; -0 is 0, a NaN is below everything (0)
 NRL_DEVICE uint32_t order_key(float x) {
@@ -25,224 +30,359 @@ NRL_DEVICE uint32_t order_key(float x) {
   const uint32_t b = __float_as_uint(x + 0.f);
   return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
+NRL_DEVICE void evict_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 
-__global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const EvictCall p, const int in_smem) {
+__global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const EvictCall p, const int cluster, const int in_smem) {
   pdl_wait();
   pdl_launch_dependents();
   extern __shared__ uint32_t keys[];
-  __shared__ uint32_t bins[kSelBins];
+  __shared__ __align__(16) uint4 warp_counts[2][kSelWarps][2];        // of two rounds in turn: eight counts, the first one unused
+  __shared__ __align__(16) uint4 counts[2][2];                        // the block's; others may still read the last round's
+  __shared__ __align__(16) uint4 total;
   __shared__ uint2 warp_sums[kSelWarps];
-  __shared__ uint32_t found[2];                                       // a digit, and how many of it are kept
-  const int seq = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int n = min(p.context_lens[seq], p.max_tokens);
+  const int seq = blockIdx.x / cluster, rank = blockIdx.x - seq * cluster, kvh = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int n = max(0, min(p.context_lens[seq], p.max_tokens));
   const long row = static_cast<long>(seq) * p.Hkv + kvh;
   int* kept = p.kept + row * p.keep;
   float* kept_scores = p.kept_scores + row * p.keep;
   const float* sc = p.scores + seq * p.score_row + kvh * p.score_head;
-  if (kvh == 0 && tid == 0) p.new_lens[seq] = max(0, min(n, p.keep));
+  uint32_t* bits = p.bits + row * ((p.max_tokens + 31) / 32);
+  if (kvh == 0 && rank == 0 && tid == 0) p.new_lens[seq] = min(n, p.keep);
   if (n <= p.keep) {
-    for (int j = tid; j < p.keep; j += kSelThreads) {
+    const int at = rank * kSelThreads + tid, step = cluster * kSelThreads;
+    for (int j = at; j < p.keep; j += step) {
       kept[j] = j < n ? j : -1;
       kept_scores[j] = j < n ? sc[j] : 0.f;
     }
+    for (int w = at; w * 32 < n; w += step) bits[w] = n - w * 32 >= 32 ? 0xffffffffu : (1u << (n - w * 32)) - 1;
     return;
   }
-  const int lo = p.sinks, hi = n - p.recent, m = hi - lo;             // candidates [lo, hi)
-  uint32_t need = p.keep - p.sinks - p.recent;                        // < m
-  auto key_at = [&](int i) { return in_smem ? keys[i] : order_key(sc[lo + i]); };
-  if (in_smem) for (int i = tid; i < m; i += kSelThreads) keys[i] = order_key(sc[lo + i]);
-  uint32_t prefix = 0, mask = 0;                                      // digits found so far
-  if (need > 0) {
+  const int lo = p.sinks, hi = n - p.recent;                          // [lo, hi) may go
+  const int words = (n + 31) / 32, per_block = (words + cluster - 1) / cluster, b0 = min(words, rank * per_block), b1 = min(words, b0 + per_block);
+  const int t0 = b0 * 32, m0 = max(lo, t0), m1 = min(hi, b1 * 32);     // of this block
+  const uint32_t wanted = p.keep - p.sinks - p.recent;
+  const bool any = wanted > 0;
+  auto key_at = [&](int t) { return in_smem ? keys[t - t0] : t >= m0 && t < m1 ? order_key(sc[t]) : 0u; };        // 0: may not go
+  // a warp has a range of neighbouring words of 32 tokens
+  const int per = (b1 - b0 + kSelWarps - 1) / kSelWarps, w0 = min(b1, b0 + warp * per), w1 = min(b1, w0 + per);
+  uint32_t least = 0;                                                 // `wanted` keys or more are at or above it
+  bool exact = false;                                                 // no more than those
+  if (any) {
+    if (in_smem) {
+#pragma unroll 4
+      for (int w = w0; w < w1; ++w) {                                 // (a warp reads its own)
+        const int t = w * 32 + lane;
+        keys[t - t0] = t >= m0 && t < m1 ? order_key(sc[t]) : 0u;
+      }
+    }
 #pragma unroll 1
-    for (int pass = 0; pass < 3; ++pass) {
-      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, width = pass == 2 ? 10 : 11;
-      for (int i = tid; i < kSelBins; i += kSelThreads) bins[i] = 0;
-      __syncthreads();
-      for (int i = tid; i < m; i += kSelThreads) {
-        const uint32_t k = key_at(i);
-        if ((k & mask) == prefix) atomicAdd(&bins[(k >> shift) & ((1u << width) - 1)], 1u);
+    for (int round = 0; round < 11 && !exact; ++round) {
+      const int shift = max(0, 29 - 3 * round), most = round < 10 ? 7 : 3;
+      uint32_t n_at[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 2
+      for (int w = w0; w < w1; ++w) {
+        const uint32_t k = key_at(w * 32 + lane);
+#pragma unroll
+        for (int v = 1; v < 8; ++v) n_at[v] += __popc(__ballot_sync(0xffffffffu, k >= least + (static_cast<uint32_t>(v) << shift)));
       }
+      if (lane < 2) warp_counts[round & 1][warp][lane] = lane == 0 ? make_uint4(0, n_at[1], n_at[2], n_at[3]) : make_uint4(n_at[4], n_at[5], n_at[6], n_at[7]);
       __syncthreads();
-      // thread i sums bins [4 i, 4 i + 4) from the top; the digit is where the sum from the top reaches `need`
-      uint32_t c[4], mine = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) mine += c[e] = bins[kSelBins - 1 - (tid * 4 + e)];
-      uint32_t upto = mine;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xffffffffu, upto, d);
-        if (lane >= d) upto += v;
-      }
-      if (lane == 31) warp_sums[warp].x = upto;
-      __syncthreads();
-      for (int w = 0; w < warp; ++w) upto += warp_sums[w].x;
-      uint32_t above = upto - mine;
-      if (above < need && need <= upto) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (above < need && need <= above + c[e]) { found[0] = kSelBins - 1 - (tid * 4 + e); found[1] = need - above; }
-          above += c[e];
+      // lane 2 i + j: half j of warp i's counts, then of block i's
+      auto add = [&](uint4 c, int from) {
+        for (int d = from; d >= 2; d >>= 1) {
+          c.x += __shfl_xor_sync(0xffffffffu, c.x, d); c.y += __shfl_xor_sync(0xffffffffu, c.y, d);
+          c.z += __shfl_xor_sync(0xffffffffu, c.z, d); c.w += __shfl_xor_sync(0xffffffffu, c.w, d);
         }
+        return c;
+      };
+      uint4 c = add(warp_counts[round & 1][lane >> 1][lane & 1], 16);
+      if (cluster > 1) {
+        if (warp == 0 && lane < 2) counts[round & 1][lane] = c;
+        evict_cluster_sync();
+        c = make_uint4(0, 0, 0, 0);
+        if ((lane >> 1) < cluster) {
+          const float4 v = ld_cluster_f4(smem_u32(&counts[round & 1][lane & 1]), lane >> 1);
+          c = make_uint4(__float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w));
+        }
+        c = add(c, 16);
       }
-      __syncthreads();
-      prefix |= found[0] << shift;
-      mask |= ((1u << width) - 1) << shift;
-      need = found[1];
-    }
-  }
-  // larger than `prefix`: kept; equal: the first `need`
-  const int per = (m + kSelThreads - 1) / kSelThreads, i0 = min(m, tid * per), i1 = min(m, i0 + per);
-  const bool none = p.keep == p.sinks + p.recent;
-  __syncthreads();
-  uint32_t more = 0, same = 0;
-  for (int i = i0; i < i1; ++i) {
-    const uint32_t k = key_at(i);
-    more += k > prefix;
-    same += k == prefix;
-  }
-  uint32_t more_upto = more, same_upto = same;
+      // the highest candidate that enough keys reach
+      const uint32_t mine[4] = {c.x, c.y, c.z, c.w};
+      uint32_t best = 0, of_best = 0;
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const uint32_t a = __shfl_up_sync(0xffffffffu, more_upto, d), b = __shfl_up_sync(0xffffffffu, same_upto, d);
-    if (lane >= d) { more_upto += a; same_upto += b; }
-  }
-  if (lane == 31) warp_sums[warp] = make_uint2(more_upto, same_upto);
-  __syncthreads();
-  uint32_t more_at = more_upto - more, same_at = same_upto - same;
-  for (int w = 0; w < warp; ++w) { more_at += warp_sums[w].x; same_at += warp_sums[w].y; }
-  if (!none) {
-    for (int i = i0; i < i1; ++i) {
-      const uint32_t k = key_at(i);
-      if (k > prefix || (k == prefix && same_at < need)) {
-        const uint32_t j = p.sinks + more_at + min(same_at, need);
-        kept[j] = lo + i;
-        kept_scores[j] = sc[lo + i];
+      for (int v = 1; v < 8; ++v) {
+        const uint32_t reach = __shfl_sync(0xffffffffu, mine[v & 3], v >> 2);
+        if (v <= most && reach >= wanted) { best = v; of_best = reach; }
       }
-      more_at += k > prefix;
-      same_at += k == prefix;
+      least += best << shift;
+      exact = best > 0 && of_best == wanted;
     }
   }
-  for (int j = tid; j < p.sinks; j += kSelThreads) { kept[j] = j; kept_scores[j] = sc[j]; }
-  for (int j = tid; j < p.recent; j += kSelThreads) { kept[p.keep - p.recent + j] = hi + j; kept_scores[p.keep - p.recent + j] = sc[hi + j]; }
+  if (exact) --least;                                                 // all above it (a candidate is above 0)
+  // kept: the first, the last, keys above `least`, and of those equal to it as many as there is room for, the first ones
+  auto look = [&](int word, uint32_t& more, uint32_t& same) {
+    const int t = word * 32 + lane;
+    const bool middle = any && t >= lo && t < hi;
+    const uint32_t k = middle ? key_at(t) : 0u;
+    more = __ballot_sync(0xffffffffu, t < n && (t < lo || t >= hi || (middle && k > least)));
+    same = __ballot_sync(0xffffffffu, middle && k == least);
+  };
+  uint32_t more = 0, same = 0;
+  for (int w = w0; w < w1; ++w) {
+    uint32_t a, b;
+    look(w, a, b);
+    more += __popc(a);
+    same += __popc(b);
+  }
+  if (lane == 0) warp_sums[warp] = make_uint2(more, same);
+  __syncthreads();
+  if (tid == 0) {
+    uint4 all = make_uint4(0, 0, 0, 0);
+    for (int w = 0; w < kSelWarps; ++w) { all.x += warp_sums[w].x; all.y += warp_sums[w].y; }
+    total = all;
+  }
+  evict_cluster_sync();
+  uint32_t need = p.keep;
+  more = same = 0;
+  for (int r = 0; r < cluster; ++r) {
+    const float4 v = ld_cluster_f4(smem_u32(&total), r);
+    need -= __float_as_uint(v.x);
+    more += r < rank ? __float_as_uint(v.x) : 0u;
+    same += r < rank ? __float_as_uint(v.y) : 0u;
+  }
+  for (int w = 0; w < warp; ++w) { more += warp_sums[w].x; same += warp_sums[w].y; }
+  const uint32_t under = (1u << lane) - 1;
+  for (int w = w0; w < w1; ++w) {
+    uint32_t a, b;
+    look(w, a, b);
+    const bool is = (a >> lane & 1) || ((b >> lane & 1) && same + __popc(b & under) < need);
+    if (is) {
+      const uint32_t j = more + __popc(a & under) + min(same + __popc(b & under), need);
+      kept[j] = w * 32 + lane;
+      kept_scores[j] = sc[w * 32 + lane];
+    }
+    const uint32_t m = __ballot_sync(0xffffffffu, is);
+    if (lane == 0) bits[w] = m;
+    more += __popc(a);
+    same += __popc(b);
+  }
+  evict_cluster_sync();                                               // a block's shared memory is read up to here
 }
 
 // ---- tokens' rows: 16-byte pieces of keys (and of bf16 values), and their scales ---------------------------------------------------------------------
 constexpr int kMoveThreads = 256;
 constexpr int kMoveUnits = 8;             // pieces a thread holds
 constexpr int kMovePieces = 4;            // pieces of a token that a block moves (64 bytes)
+constexpr int kMoveRange = kMoveThreads / kMovePieces * kMoveUnits;   // places at a time
+constexpr int kSpanPages = 16;            // of transposed values at a time: their tokens are as many as the threads
+constexpr int kSpanRow = 5;               // words from an element's row to the next
 
 struct MoveParams {
   EvictCall e;
   const int* out_tables;
-  int out_blocks, key_slices, value_slices;   // grid.z: slices of keys, then of values, then (fp8) values transposed and the scales
+  int out_blocks, key_slices;             // grid.y: kv heads x ranges of places; grid.z: slices of keys, then of values (fp8: the scales)
 };
 
-// where token t of a row lies: its place among all tokens of kv head `kvh`
-NRL_DEVICE long token_place(const int* table, int t, int Hkv, int kvh) { return (static_cast<long>(table[t >> 4]) * Hkv + kvh) * 16 + (t & 15); }
+// where token t of a row lies: its place among all tokens (below 2^31: checked on the host)
+NRL_DEVICE int token_place(const int* table, int t, int Hkv, int kvh) { return (table[t >> 4] * Hkv + kvh) * 16 + (t & 15); }
 
-template <class T, int PIECES>
-NRL_DEVICE void move_rows(T* rows, int row_elems, int slice, const int* from, const int* to, const int* kept, int count, int Hkv, int kvh, bool in_place) {
-  const int piece = threadIdx.x % PIECES, lane_tok = threadIdx.x / PIECES;
-  constexpr int kTok = kMoveThreads / PIECES, kRange = kTok * kMoveUnits;
+template <bool IN_PLACE, class T, int PIECES>
+NRL_DEVICE void move_rows(T* rows, int row_elems, int slice, const int* from, const int* to, const int* kept, int j0, int j1, int Hkv, int kvh) {
+  const int piece = threadIdx.x % PIECES, first = threadIdx.x / PIECES;
+  constexpr int kTok = kMoveThreads / PIECES;
   T cur[kMoveUnits];
-  long src[kMoveUnits], dst[kMoveUnits];
-  for (int j0 = 0; j0 < count; j0 += kRange) {
+  int dst[kMoveUnits];
+  T* mine = rows + slice * PIECES + piece;
+  auto read = [&](int j_at) {
+    int src[kMoveUnits];
 #pragma unroll
     for (int u = 0; u < kMoveUnits; ++u) {
-      const int j = j0 + u * kTok + lane_tok;
-      const int t = j < count ? kept[j] : -1;
-      dst[u] = -1;
-      if (t < 0 || (in_place && t == j)) continue;
-      src[u] = token_place(from, t, Hkv, kvh);
-      dst[u] = token_place(to, j, Hkv, kvh);
+      const int j = j_at + u * kTok + first, t = j < j1 ? kept[j] : -1;
+      const bool moves = t >= 0 && !(IN_PLACE && t == j);
+      src[u] = moves ? token_place(from, t, Hkv, kvh) : -1;
+      dst[u] = moves ? token_place(to, j, Hkv, kvh) : -1;
     }
 #pragma unroll
     for (int u = 0; u < kMoveUnits; ++u)
-      if (dst[u] >= 0) cur[u] = rows[src[u] * row_elems + slice * PIECES + piece];
+      if (src[u] >= 0) cur[u] = mine[static_cast<long>(src[u]) * row_elems];
+  };
+  if (!IN_PLACE) {
+    for (int j = j0; j < j1; j += kTok * kMoveUnits) {
+      read(j);
+#pragma unroll
+      for (int u = 0; u < kMoveUnits; ++u)
+        if (dst[u] >= 0) mine[static_cast<long>(dst[u]) * row_elems] = cur[u];
+    }
+    return;
+  }
+  read(j0);
+  for (int j = j0; j < j1; j += kTok * kMoveUnits) {
     __syncthreads();                      // all of this range is read before any of it is written
+    T val[kMoveUnits];
+    int at[kMoveUnits];
+#pragma unroll
+    for (int u = 0; u < kMoveUnits; ++u) { val[u] = cur[u]; at[u] = dst[u]; }
+    if (j + kTok * kMoveUnits < j1) read(j + kTok * kMoveUnits);
 #pragma unroll
     for (int u = 0; u < kMoveUnits; ++u)
-      if (dst[u] >= 0) rows[dst[u] * row_elems + slice * PIECES + piece] = cur[u];
-    __syncthreads();
+      if (at[u] >= 0) mine[static_cast<long>(at[u]) * row_elems] = val[u];
   }
 }
 
-__global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const MoveParams p) {
-  pdl_wait();
-  pdl_launch_dependents();
-  const int seq = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x;
-  int z = blockIdx.z;
-  const EvictCall& e = p.e;
-  const bool in_place = e.out_tables == nullptr, fp8 = e.k_scale != nullptr;
-  const int n = min(e.context_lens[seq], e.max_tokens), count = max(0, min(n, e.keep));
-  if (in_place && n <= e.keep) return;
-  const int* from = e.block_tables + static_cast<long>(seq) * e.max_blocks;
-  const int* to = p.out_tables + static_cast<long>(seq) * p.out_blocks;
-  const int* kept = e.kept + (static_cast<long>(seq) * e.Hkv + kvh) * e.keep;
-  const int row_elems = fp8 ? 8 : 16;
-  if (z < p.key_slices) return move_rows<uint4, kMovePieces>(static_cast<uint4*>(e.k_cache), row_elems, z, from, to, kept, count, e.Hkv, kvh, in_place);
-  z -= p.key_slices;
-  if (!fp8) return move_rows<uint4, kMovePieces>(static_cast<uint4*>(e.v_cache), row_elems, z, from, to, kept, count, e.Hkv, kvh, in_place);
-  if (z == 1) return move_rows<float, 1>(e.k_scale, 1, 0, from, to, kept, count, e.Hkv, kvh, in_place);
-  if (z == 2) return move_rows<float, 1>(e.v_scale, 1, 0, from, to, kept, count, e.Hkv, kvh, in_place);
-  // values transposed: thread d of 128 packs element d of the kept tokens, page by page
-  if (tid >= 128) return;
-  const uint4* v = static_cast<const uint4*>(e.v_cache);
-  uint4* out = static_cast<uint4*>(e.v_cache);
-  uint32_t word[4] = {0, 0, 0, 0};
-  int page = -1;
-  uint4 cur = make_uint4(0, 0, 0, 0);
-  for (int j = 0; j < count; ++j) {
-    const int t = kept[j];
-    if ((t >> 4) != page) {
-      page = t >> 4;
-      cur = v[(static_cast<long>(from[page]) * e.Hkv + kvh) * 128 + tid];
-    }
-    const int b = t & 15;
-    const uint32_t w = b < 8 ? (b < 4 ? cur.x : cur.y) : (b < 12 ? cur.z : cur.w);
-    const uint32_t byte = (w >> ((b & 3) * 8)) & 0xffu;
-    const int c = j & 15;
+// places [j0, j1) of the values of fp8 pages, j0 a multiple of 16
+NRL_DEVICE void move_transposed(uint4* v, long step, const int* from, const int* to, const int* kept, const uint16_t* bits, int j0, int j1) {
+  __shared__ uint32_t span[kSpanPages * 128 * kSpanRow];
+  __shared__ uint32_t left[2][128 * kSpanRow];                        // places of a page that is not full yet: read by one span, written by it for the next
+  __shared__ __align__(8) uint16_t place[kMoveThreads + 16];          // of the span's kept tokens, from the first place of their page on: the byte of element 0
+  const int tid = threadIdx.x, d = tid & 127, warp_half = tid >> 7;
+  const int last = kept[j1 - 1] >> 4;
+  int page = kept[j0] >> 4, j = j0, turn = 0;
+  uint4 cur[kMoveUnits];
+  auto read = [&](int at) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if ((c >> 2) == i) word[i] |= byte << ((c & 3) * 8);
-    if (c == 15 || j == count - 1) {
-      const long at = (static_cast<long>(to[j >> 4]) * e.Hkv + kvh) * 128 + tid;
-      if (c < 15) {                        // places behind the last stay as they were
-        const uint4 old = out[at];
+    for (int u = 0; u < kMoveUnits; ++u) {
+      const int pg = at + u * 2 + warp_half;
+      if (pg <= last && bits[pg] != 0) cur[u] = v[from[pg] * step + d];
+    }
+  };
+  read(page);
+  for (; j < j1; page += kSpanPages, turn ^= 1) {
+    const int t = j + tid < j1 ? kept[j + tid] : -1;
+    const bool here = t >= 0 && (t >> 4) < page + kSpanPages;
+#pragma unroll
+    for (int u = 0; u < kMoveUnits; ++u) {
+      uint32_t* w = span + ((u * 2 + warp_half) * 128 + d) * kSpanRow;
+      w[0] = cur[u].x; w[1] = cur[u].y; w[2] = cur[u].z; w[3] = cur[u].w;
+    }
+    if (here) place[(j & 15) + tid] = static_cast<uint16_t>(((t >> 4) - page) * 128 * kSpanRow * 4 + (t & 15));
+    const int to_j = j + __syncthreads_count(here);                   // places [j, to_j) come from this span
+    if (to_j < j1) read(page + kSpanPages);
+    const uint8_t* bytes = reinterpret_cast<const uint8_t*>(span) + d * kSpanRow * 4;
+    for (int pg = (j >> 4) + warp_half; pg * 16 < to_j; pg += 2) {
+      uint32_t word[4];
+      const int k0 = max(0, j - pg * 16), k1 = min(16, to_j - pg * 16);          // places of this page that are put now
+      const uint16_t* at = place + (pg - (j >> 4)) * 16;
+      if (k0 == 0 && k1 == 16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint2 four = *reinterpret_cast<const uint2*>(at + 4 * i);
+          const uint32_t a = bytes[four.x & 0xffffu], b = bytes[four.x >> 16], c = bytes[four.y & 0xffffu], e = bytes[four.y >> 16];
+          word[i] = __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, e, 0x0040), 0x5410);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          word[i] = k0 > i * 4 ? left[turn][d * kSpanRow + i] : 0u;
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const int k = i * 4 + b;
+            if (k >= k0 && k < k1) word[i] = (word[i] & ~(0xffu << (8 * b))) | (static_cast<uint32_t>(bytes[at[k]]) << (8 * b));
+          }
+        }
+      }
+      if (k1 == 16) {
+        v[to[pg] * step + d] = make_uint4(word[0], word[1], word[2], word[3]);
+      } else if (to_j < j1) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) left[turn ^ 1][d * kSpanRow + i] = word[i];
+      } else {                                                        // places behind the last stay as they were
+        const uint4 old = v[to[pg] * step + d];
         const uint32_t ow[4] = {old.x, old.y, old.z, old.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int k = c + 1 - i * 4;                                  // bytes of this word that are new
+          const int k = k1 - i * 4;                                   // bytes of this word that are new
           if (k < 4) word[i] = k <= 0 ? ow[i] : (word[i] & (0xffffffffu >> (32 - 8 * k))) | (ow[i] & (0xffffffffu << (8 * k)));
         }
+        v[to[pg] * step + d] = make_uint4(word[0], word[1], word[2], word[3]);
       }
-      out[at] = make_uint4(word[0], word[1], word[2], word[3]);
-      word[0] = word[1] = word[2] = word[3] = 0;
     }
+    j = to_j;
+    __syncthreads();                                                  // `left` is written, span and places are read
   }
+}
+
+struct MoveRow {
+  const int *from, *to, *kept;
+  long row;
+  int kvh, j0, j1;                        // places [j0, j1) of a row-head
+};
+template <bool IN_PLACE>
+NRL_DEVICE MoveRow move_row(const MoveParams& p) {
+  const EvictCall& e = p.e;
+  const int seq = blockIdx.x, kvh = blockIdx.y % e.Hkv, range = blockIdx.y / e.Hkv, n = min(e.context_lens[seq], e.max_tokens), count = max(0, min(n, e.keep));
+  const long row = static_cast<long>(seq) * e.Hkv + kvh;
+  const int j0 = IN_PLACE ? 0 : range * kMoveRange, j1 = IN_PLACE ? (n > e.keep ? count : 0) : min(count, j0 + kMoveRange);
+  return {e.block_tables + static_cast<long>(seq) * e.max_blocks, p.out_tables + static_cast<long>(seq) * p.out_blocks, e.kept + row * e.keep, row, kvh, j0, j1};
+}
+
+template <bool IN_PLACE>
+__global__ void __launch_bounds__(kMoveThreads, IN_PLACE ? 2 : 4) kv_move_kernel(const MoveParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const EvictCall& e = p.e;
+  const MoveRow m = move_row<IN_PLACE>(p);
+  if (m.j0 >= m.j1) return;
+  const int z = blockIdx.z;
+  const bool keys = z < p.key_slices, fp8 = e.k_scale != nullptr;
+  if (fp8 && !keys) return move_rows<IN_PLACE, float, 1>(z == p.key_slices ? e.k_scale : e.v_scale, 1, 0, m.from, m.to, m.kept, m.j0, m.j1, e.Hkv, m.kvh);
+  move_rows<IN_PLACE, uint4, kMovePieces>(static_cast<uint4*>(keys ? e.k_cache : e.v_cache), fp8 ? 8 : 16, keys ? z : z - p.key_slices, m.from, m.to, m.kept, m.j0, m.j1,
+                                          e.Hkv, m.kvh);
+}
+
+// values of fp8 pages.  It takes nothing from kv_move, whose blocks had all begun when this one does; its end waits for theirs.
+template <bool IN_PLACE>
+__global__ void __launch_bounds__(kMoveThreads, 4) kv_move_transposed_kernel(const MoveParams p) {
+  const EvictCall& e = p.e;
+  const MoveRow m = move_row<IN_PLACE>(p);
+  if (m.j0 < m.j1) {
+    const uint16_t* bits = reinterpret_cast<const uint16_t*>(e.bits + m.row * ((e.max_tokens + 31) / 32));
+    move_transposed(static_cast<uint4*>(e.v_cache) + static_cast<long>(m.kvh) * 128, static_cast<long>(e.Hkv) * 128, m.from, m.to, m.kept, bits, m.j0, m.j1);
+  }
+  pdl_wait();
+  pdl_launch_dependents();
 }
 
 }  // namespace nrl
 
 using namespace nrl;
 
-extern "C" cudaError_t nrl_kv_evict(const EvictCall* c, cudaStream_t s) {
+namespace {
+
+template <bool IN_PLACE>
+cudaError_t launch_moves(const MoveParams& p, cudaStream_t s) {
+  const EvictCall& c = p.e;
+  const bool fp8 = c.k_scale != nullptr;
+  const int places = c.keep < c.max_tokens ? c.keep : c.max_tokens, ranges = IN_PLACE ? 1 : (places + kMoveRange - 1) / kMoveRange;
+  launch_dependent(kv_move_kernel<IN_PLACE>, dim3(c.S, c.Hkv * ranges, fp8 ? p.key_slices + 2 : 2 * p.key_slices), kMoveThreads, 0, s, p);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || !fp8) return e;
+  launch_dependent(kv_move_transposed_kernel<IN_PLACE>, dim3(c.S, c.Hkv * ranges), kMoveThreads, 0, s, p);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+extern "C" cudaError_t nrl_kv_evict(const EvictCall* c, int num_sms, cudaStream_t s) {
   if (c->S == 0) return cudaSuccess;
-  const int in_smem = c->max_tokens <= kSelSmemTokens;
-  const int smem = in_smem ? c->max_tokens * 4 : 0;
+  // blocks a row-head: as many as find an SM, but 2048 tokens each at least; and as many as hold its scores
+  int cluster = 1;
+  while (cluster < kSelCluster && ((static_cast<long>(c->S) * c->Hkv * cluster * 2 <= 2L * num_sms && c->max_tokens >= cluster * 2 * 2048) ||
+                                   c->max_tokens > static_cast<long>(cluster) * kSelTokens)) cluster *= 2;
+  const int tokens = ((c->max_tokens + 31) / 32 + cluster - 1) / cluster * 32;
+  const int in_smem = tokens <= kSelTokens;
   static PerDevice<bool> configured;
-  cudaError_t e = allow_smem(configured, kv_select_kernel, kSelSmemTokens * 4);
+  cudaError_t e = allow_smem(configured, kv_select_kernel, kSelTokens * 4);
   if (e != cudaSuccess) return e;
-  launch_dependent(kv_select_kernel, dim3(c->S, c->Hkv), kSelThreads, smem, s, *c, in_smem);
+  launch_dependent_clusters(kv_select_kernel, dim3(c->S * cluster, c->Hkv), kSelThreads, in_smem ? tokens * 4 : 0, s, cluster, *c, cluster, in_smem);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   MoveParams p;
   p.e = *c;
   p.out_tables = c->out_tables != nullptr ? c->out_tables : c->block_tables;
   p.out_blocks = c->out_tables != nullptr ? c->out_blocks : c->max_blocks;
-  const bool fp8 = c->k_scale != nullptr;
-  p.key_slices = (fp8 ? 8 : 16) / kMovePieces;
-  p.value_slices = fp8 ? 3 : 16 / kMovePieces;
-  launch_dependent(kv_move_kernel, dim3(c->S, c->Hkv, p.key_slices + p.value_slices), kMoveThreads, 0, s, p);
-  return cudaGetLastError();
+  p.key_slices = (c->k_scale != nullptr ? 8 : 16) / kMovePieces;
+  return c->out_tables != nullptr ? launch_moves<false>(p, s) : launch_moves<true>(p, s);
 }

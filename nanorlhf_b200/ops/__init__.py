@@ -308,14 +308,14 @@ def _check_pages(what, q, k_cache, v_cache, block_tables, context_lens, k_scale,
         raise ValueError(f"{what}: q must be [{rows}, Hq, {k_cache.shape[3]}] with Hq a multiple, at most 8 times, of {k_cache.shape[1]}, got {tuple(q.shape)}")
 
 
-def paged_decode_shared(q, k_cache, v_cache, block_tables, context_lens, cu_groups, shared_lens, max_group=None, k_scale=None, v_scale=None, scale=None, splits=0):
+def paged_decode_shared(q, k_cache, v_cache, block_tables, context_lens, cu_groups, shared_lens, max_group=None, k_scale=None, v_scale=None, scale=None):
     """Decode attention, one new token per row, of rows that share their first tokens: the keys and values of those are read once per group.
 
     ``q`` bf16 [S, Hq, 128] (views of a projection will do); pages, tables and lengths as in ``native.paged_decode`` (``k_cache`` [blocks, Hkv, 16, 128] bf16, or with
     ``k_scale`` and ``v_scale`` [blocks, Hkv, 16] the e4m3 pages of the sampler).  Group g has rows cu_groups[g] .. cu_groups[g + 1] (int32), ``max_group`` of them at
     most (a host number; None: S), and shares its first shared_lens[g] tokens: they are read from the pages of its first row, whatever the tables of its others say of
     whole pages among them.  A row sees its first context_lens tokens, the shared ones among them; with none its result is 0; rows of no group are plain.
-    ``splits``: parts that the tokens behind the prefix are cut into (0: chosen).  No gradient."""
+    No gradient."""
     what = "paged_decode_shared"
     _check_pages(what, q, k_cache, v_cache, block_tables, context_lens, k_scale, v_scale)
     if shared_lens.dim() != 1 or tuple(cu_groups.shape) != (shared_lens.shape[0] + 1,):
@@ -326,7 +326,7 @@ def paged_decode_shared(q, k_cache, v_cache, block_tables, context_lens, cu_grou
     scale = _scale_of(what, scale, q)
     if use_native(q):
         return _nat().paged_decode_shared(q, k_cache, v_cache, block_tables.contiguous(), context_lens.contiguous(), cu_groups.contiguous(), shared_lens.contiguous(),
-                                          max(1, q.shape[0]) if max_group is None else int(max_group), k_scale, v_scale, scale, int(splits))
+                                          max(1, q.shape[0]) if max_group is None else int(max_group), k_scale, v_scale, scale)
     return ref.paged_decode_shared(q, k_cache, v_cache, block_tables, context_lens, cu_groups, shared_lens, k_scale, v_scale, scale)
 
 
@@ -337,7 +337,7 @@ def _check_scores(what, scores, k_cache, rows, name="scores"):
         raise TypeError(f"{what}: {name} must be float32 on {k_cache.device}, the tokens of a head side by side")
 
 
-def paged_decode_scored(q, k_cache, v_cache, block_tables, context_lens, scores, decay=1.0, k_scale=None, v_scale=None, scale=None, out_scores=None, splits=0):
+def paged_decode_scored(q, k_cache, v_cache, block_tables, context_lens, scores, decay=1.0, k_scale=None, v_scale=None, scale=None, out_scores=None):
     """Decode attention that adds up what weight every cached token gets: (out [S, Hq, 128], scores).
 
     Arguments as in ``paged_decode_shared``.  ``scores`` float32 [S, Hkv, L], a row's tokens in their order: with p the attention weights,
@@ -355,8 +355,7 @@ def paged_decode_scored(q, k_cache, v_cache, block_tables, context_lens, scores,
         raise ValueError(f"{what}: decay must be finite, got {decay}")
     scale = _scale_of(what, scale, q)
     if use_native(q):
-        return _nat().paged_decode_scored(q, k_cache, v_cache, block_tables.contiguous(), context_lens.contiguous(), scores, float(decay), k_scale, v_scale, scale, out_scores,
-                                          int(splits))
+        return _nat().paged_decode_scored(q, k_cache, v_cache, block_tables.contiguous(), context_lens.contiguous(), scores, float(decay), k_scale, v_scale, scale, out_scores)
     return ref.paged_decode_scored(q, k_cache, v_cache, block_tables, context_lens, scores, decay, k_scale, v_scale, scale, out_scores)
 
 

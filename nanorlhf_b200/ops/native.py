@@ -497,19 +497,19 @@ def attention_shared_prefix(q, k, v, cu_seqlens, cu_groups, scale):
 
 
 @torch.no_grad()
-def paged_decode_shared(q, k_cache, v_cache, block_tables, context_lens, cu_groups, shared_lens, max_group, k_scale, v_scale, scale, splits):
-    _count(2)
-    return ext().paged_decode_shared(_head_rows(q), k_cache, v_cache, block_tables, context_lens, cu_groups, shared_lens, max_group, k_scale, v_scale, scale, splits)
+def paged_decode_shared(q, k_cache, v_cache, block_tables, context_lens, cu_groups, shared_lens, max_group, k_scale, v_scale, scale):
+    _count(4)
+    return ext().paged_decode_shared(_head_rows(q), k_cache, v_cache, block_tables, context_lens, cu_groups, shared_lens, max_group, k_scale, v_scale, scale)
 
 
 @torch.no_grad()
-def paged_decode_scored(q, k_cache, v_cache, block_tables, context_lens, scores, decay, k_scale, v_scale, scale, out_scores, splits):
-    _count(2)
+def paged_decode_scored(q, k_cache, v_cache, block_tables, context_lens, scores, decay, k_scale, v_scale, scale, out_scores):
+    _count(3)
     out_scores = scores if out_scores is None else out_scores
-    return ext().paged_decode_scored(_head_rows(q), k_cache, v_cache, block_tables, context_lens, scores, out_scores, decay, k_scale, v_scale, scale, splits), out_scores
+    return ext().paged_decode_scored(_head_rows(q), k_cache, v_cache, block_tables, context_lens, scores, out_scores, decay, k_scale, v_scale, scale), out_scores
 
 
 @torch.no_grad()
 def kv_evict(k_cache, v_cache, block_tables, context_lens, scores, keep, sinks, recent, k_scale, v_scale, out_tables):
-    _count(2)
+    _count(2 if k_scale is None else 3)
     return ext().kv_evict(k_cache, v_cache, block_tables, context_lens, scores, keep, sinks, recent, k_scale, v_scale, out_tables)

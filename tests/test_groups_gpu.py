@@ -236,8 +236,8 @@ def test_decode_over_shared_pages(name, heads, kv, fp8):
     q = torch.randn(S, heads + 3, 128, generator=gen(12), device=DEV).to(torch.bfloat16)[:, :heads]
     kw = {"k_scale": st["ks"], "v_scale": st["vs"]}
     largest = max(len(c) for _, c in groups)
-    outs = [ops.paged_decode_shared(q, st["k"], st["v"], st["tables"], st["context"], st["cu"], st["shared"], max_group=m, splits=s, **kw)
-            for m, s in ((largest, 0), (None, 1), (largest, 5), (1, 0))]
+    outs = [ops.paged_decode_shared(q, st["k"], st["v"], st["tables"], st["context"], st["cu"], st["shared"], max_group=m, **kw)
+            for m in (largest, None, 1)]
     row = 0
     for shared, ctxs in groups:
         first = row
@@ -299,10 +299,10 @@ def test_decode_with_scores(contexts, heads, kv, fp8):
     for s, n in enumerate(contexts):
         if n:
             before[s, :, n - 1] = float("nan")                                                  # the newest token's place holds anything
-    for decay, splits, in_place in ((1.0, 0, False), (0.75, 3, True), (1.0, 1, False)):
+    for decay, in_place in ((1.0, False), (0.75, True)):
         scores = before.clone()
         into = None if in_place else torch.full((S, kv, L), 7.0, device=DEV)
-        out, new = ops.paged_decode_scored(q, st["k"], st["v"], st["tables"], st["context"], scores, decay, st["ks"], st["vs"], out_scores=into, splits=splits)
+        out, new = ops.paged_decode_scored(q, st["k"], st["v"], st["tables"], st["context"], scores, decay, st["ks"], st["vs"], out_scores=into)
         assert new is (scores if in_place else into)
         for s, n in enumerate(contexts):
             want, bound, w, wb = oracle.decode_row(q[s], *oracle.page_rows(st, st["tables"][s], n), SCALE, fp8)
@@ -375,10 +375,28 @@ def test_evict_all_alike_keeps_the_first():
     assert kept[0, 0].tolist() == list(range(40)) + list(range(190, 200)) and lens.tolist() == [50]
 
 
-def test_evict_from_more_tokens_than_shared_memory_holds():
-    n = 50_001
-    st = shared_batch(37, [(0, [n])], 1, False)
-    evict_both(st, random_scores(38, 1, 1, n), 4097, 16, 100)
+@pytest.mark.parametrize("contexts,keep", [([5000, 4200], 700), ([9001], 8000), ([20_011, 7, 12_345], 4097), ([50_001], 4097), ([330_000], 1000)])
+def test_evict_by_several_blocks_a_row(contexts, keep):
+    """Clusters of two to eight blocks, and more tokens than their shared memory holds; scores that tie across blocks."""
+    fp8 = len(contexts) == 2
+    st = shared_batch(37, [(0, [c]) for c in contexts], 1, fp8)
+    evict_both(st, random_scores(38, len(contexts), 1, max(contexts)), keep, 16, 100)
+
+
+@pytest.mark.parametrize("apart", [False, True])
+def test_evict_from_far_apart(apart):
+    """What is kept lies many pages apart: values of fp8 pages that wait for a page to be full, over spans without any."""
+    n, keep = 4000, 61
+    st = shared_batch(39, [(0, [n])], 2, True)
+    scores = torch.zeros(1, 2, n, device=DEV)
+    scores[0, 0, 5::97], scores[0, 1, [3, 4, 1000, 3990]] = 1.0, 2.0
+    to = None
+    if apart:
+        m = st["k"].shape[0]
+        for name in ("k", "v", "ks", "vs"):
+            st[name] = torch.cat([st[name], torch.zeros_like(st[name][:4])])
+        to = torch.arange(m, m + 4, device=DEV).int()[None]
+    evict_both(st, scores, keep, 0, 3, to)
 
 
 @pytest.mark.parametrize("fp8", [False, True])
