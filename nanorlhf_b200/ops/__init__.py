@@ -274,6 +274,8 @@ def attention_shared_prefix(q, k, v, cu_seqlens, cu_groups, max_seqlen=None, sca
     one, is plain (``attention_varlen``).  Rows behind the last sequence are 0, and so are their gradients.  Differentiable once in q, k and v.
     On CUDA bf16 and D = 128; q, k and v may be views of a projection.  ``max_seqlen`` is not needed.  A non-finite value in one sequence may reach the ones packed
     beside it."""
+    if use_native(q):
+        return _nat().attention_shared_prefix(q, k, v, cu_seqlens, cu_groups, scale)          # (checked there, with the same errors)
     what = "attention_shared_prefix"
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or k.shape[1] == 0 or q.shape[1] % k.shape[1]:
         raise ValueError(f"{what}: q [T, Hq, D] and k, v [T, Hkv, D] with Hq a multiple of Hkv are needed, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
@@ -282,12 +284,7 @@ def attention_shared_prefix(q, k, v, cu_seqlens, cu_groups, max_seqlen=None, sca
     if cu_seqlens.dim() != 1 or cu_groups.dim() != 1 or cu_seqlens.numel() < 1 or cu_groups.numel() < 1:
         raise ValueError(f"{what}: cu_seqlens [sequences + 1] and cu_groups [groups + 1] are needed, got {tuple(cu_seqlens.shape)} and {tuple(cu_groups.shape)}")
     _check_int32(what, q, cu_seqlens=cu_seqlens, cu_groups=cu_groups)
-    scale = _scale_of(what, scale, q)
-    if use_native(q):
-        if q.dtype != torch.bfloat16 or q.shape[2] != 128:
-            raise TypeError(f"{what}: on CUDA bf16 and a head size of 128 are needed, got {q.dtype} and {q.shape[2]}")
-        return _nat().attention_shared_prefix(q, k, v, cu_seqlens.contiguous(), cu_groups.contiguous(), scale)
-    return ref.attention_shared_prefix(q, k, v, cu_seqlens, cu_groups, scale)
+    return ref.attention_shared_prefix(q, k, v, cu_seqlens, cu_groups, _scale_of(what, scale, q))
 
 
 def _check_pages(what, q, k_cache, v_cache, block_tables, context_lens, k_scale, v_scale):
@@ -316,6 +313,8 @@ def paged_decode_shared(q, k_cache, v_cache, block_tables, context_lens, cu_grou
     most (a host number; None: S), and shares its first shared_lens[g] tokens: they are read from the pages of its first row, whatever the tables of its others say of
     whole pages among them.  A row sees its first context_lens tokens, the shared ones among them; with none its result is 0; rows of no group are plain.
     No gradient."""
+    if use_native(k_cache):
+        return _nat().paged_decode_shared(q, k_cache, v_cache, block_tables, context_lens, cu_groups, shared_lens, max_group, k_scale, v_scale, scale)
     what = "paged_decode_shared"
     _check_pages(what, q, k_cache, v_cache, block_tables, context_lens, k_scale, v_scale)
     if shared_lens.dim() != 1 or tuple(cu_groups.shape) != (shared_lens.shape[0] + 1,):
@@ -323,11 +322,7 @@ def paged_decode_shared(q, k_cache, v_cache, block_tables, context_lens, cu_grou
     _check_int32(what, k_cache, cu_groups=cu_groups, shared_lens=shared_lens)
     if max_group is not None and max_group < 1:
         raise ValueError(f"{what}: max_group must be positive, got {max_group}")
-    scale = _scale_of(what, scale, q)
-    if use_native(q):
-        return _nat().paged_decode_shared(q, k_cache, v_cache, block_tables.contiguous(), context_lens.contiguous(), cu_groups.contiguous(), shared_lens.contiguous(),
-                                          max(1, q.shape[0]) if max_group is None else int(max_group), k_scale, v_scale, scale)
-    return ref.paged_decode_shared(q, k_cache, v_cache, block_tables, context_lens, cu_groups, shared_lens, k_scale, v_scale, scale)
+    return ref.paged_decode_shared(q, k_cache, v_cache, block_tables, context_lens, cu_groups, shared_lens, k_scale, v_scale, _scale_of(what, scale, q))
 
 
 def _check_scores(what, scores, k_cache, rows, name="scores"):
@@ -344,6 +339,8 @@ def paged_decode_scored(q, k_cache, v_cache, block_tables, context_lens, scores,
     scores[s, h, t] = decay * scores[s, h, t] + sum of p[s, g, t] over the query heads of kv head h; the newest token (t = context_lens[s] - 1) takes the sum alone, so
     that its place need not be cleared.  In place, or into ``out_scores``, strides free up to the last; places from context_lens[s] on stay as they are, tokens from L on
     have no score.  No gradient."""
+    if use_native(k_cache):
+        return _nat().paged_decode_scored(q, k_cache, v_cache, block_tables, context_lens, scores, decay, k_scale, v_scale, scale, out_scores)
     what = "paged_decode_scored"
     _check_pages(what, q, k_cache, v_cache, block_tables, context_lens, k_scale, v_scale)
     _check_scores(what, scores, k_cache, q.shape[0])
@@ -353,10 +350,7 @@ def paged_decode_scored(q, k_cache, v_cache, block_tables, context_lens, scores,
             raise ValueError(f"{what}: out_scores must be like scores, got {tuple(out_scores.shape)} and {tuple(scores.shape)}")
     if not math.isfinite(decay):
         raise ValueError(f"{what}: decay must be finite, got {decay}")
-    scale = _scale_of(what, scale, q)
-    if use_native(q):
-        return _nat().paged_decode_scored(q, k_cache, v_cache, block_tables.contiguous(), context_lens.contiguous(), scores, float(decay), k_scale, v_scale, scale, out_scores)
-    return ref.paged_decode_scored(q, k_cache, v_cache, block_tables, context_lens, scores, decay, k_scale, v_scale, scale, out_scores)
+    return ref.paged_decode_scored(q, k_cache, v_cache, block_tables, context_lens, scores, decay, k_scale, v_scale, _scale_of(what, scale, q), out_scores)
 
 
 def kv_evict(k_cache, v_cache, block_tables, context_lens, scores, keep: int, sinks: int = 0, recent: int = 0, k_scale=None, v_scale=None, out_tables=None):
@@ -367,19 +361,19 @@ def kv_evict(k_cache, v_cache, block_tables, context_lens, scores, keep: int, si
     the row: within its pages, or into those of ``out_tables`` [S, pages], where rows of fewer tokens are copied too.  kept[s, h, j] is where the token of place j was, -1 (score 0) behind the
     last.  Places that nothing moves to stay as they are.  Pages that are written to must be one row's alone and, with ``out_tables``, no row's source; no context may
     be longer than L.  Rotated keys keep their rotation: positions go on from where they were, lengths from the new ones."""
+    if int(keep) != keep:
+        raise ValueError(f"kv_evict: keep must be a whole number, got {keep}")
+    if use_native(k_cache):
+        return _nat().kv_evict(k_cache, v_cache, block_tables, context_lens, scores, int(keep), int(sinks), int(recent), k_scale, v_scale, out_tables)
     what = "kv_evict"
     _check_pages(what, None, k_cache, v_cache, block_tables, context_lens, k_scale, v_scale)
     _check_scores(what, scores, k_cache, block_tables.shape[0])
-    if int(keep) != keep or keep < 1 or sinks < 0 or recent < 0 or sinks + recent > keep:
+    if keep < 1 or sinks < 0 or recent < 0 or sinks + recent > keep:
         raise ValueError(f"{what}: keep must be positive and at least sinks + recent, got {keep}, {sinks} and {recent}")
     if out_tables is not None:
         if out_tables.dim() != 2 or out_tables.shape[0] != block_tables.shape[0] or 16 * out_tables.shape[1] < min(keep, scores.shape[2], 16 * block_tables.shape[1]):
             raise ValueError(f"{what}: out_tables must be [{block_tables.shape[0]}, pages] with room for {keep} tokens, got {tuple(out_tables.shape)}")
         _check_int32(what, k_cache, out_tables=out_tables)
-        out_tables = out_tables.contiguous()
-    if use_native(k_cache):
-        return _nat().kv_evict(k_cache, v_cache, block_tables.contiguous(), context_lens.contiguous(), scores, int(keep), int(sinks), int(recent), k_scale, v_scale,
-                               out_tables)
     return ref.kv_evict(k_cache, v_cache, block_tables, context_lens, scores, int(keep), int(sinks), int(recent), k_scale, v_scale, out_tables)
 
 

@@ -466,10 +466,11 @@ def paged_decode(q, k_cache, v_cache, block_tables, context_lens, scale=None, sp
 # --------------------------------------------------------------------------------------------
 # many samples of one prompt, and a cache of bounded size
 # --------------------------------------------------------------------------------------------
-class _SharedPrefixFn(torch.autograd.Function):
+class _RecordedSharedPrefixFn(torch.autograd.Function):
+    """The attention in a form that a tracer records as one operation (see ``_RecordedLossFn``)."""
+
     @staticmethod
     def forward(ctx, q, k, v, cu_seqlens, cu_groups, scale):
-        _count(2)
         o, lse, table = ext().attn_groups_fwd(q, k, v, cu_seqlens, cu_groups, scale)
         ctx.save_for_backward(q, k, v, o, lse, cu_seqlens, table)
         ctx.scale = scale
@@ -478,38 +479,26 @@ class _SharedPrefixFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do):
-        _count(2)
-        return (*ext().attn_groups_bwd(do.contiguous(), *ctx.saved_tensors, ctx.scale), None, None, None)
-
-
-def _head_rows(x):
-    """[rows, heads, 128] as the kernels read it: a view of a projection stays one"""
-    ok = x.stride(-1) == 1 and (x.stride(1) == x.shape[2] or x.shape[1] == 1) and (x.shape[0] <= 1 or x.stride(0) % 8 == 0) and x.data_ptr() % 16 == 0
-    return x if ok else x.contiguous()
+        return (*ext().attn_groups_bwd(do, *ctx.saved_tensors, ctx.scale), None, None, None)
 
 
 def attention_shared_prefix(q, k, v, cu_seqlens, cu_groups, scale):
-    q, k, v = (_head_rows(x) for x in (q, k, v))
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _SharedPrefixFn.apply(q, k, v, cu_seqlens, cu_groups, scale)
-    _count(2)
-    return ext().attn_groups_fwd(q, k, v, cu_seqlens, cu_groups, scale)[0]
+    _count(4 if torch.is_grad_enabled() and q.requires_grad else 2)          # forward and, later, backward
+    if torch._C._get_tracing_state():
+        return _RecordedSharedPrefixFn.apply(*ext().attn_groups_arguments(q, k, v, cu_seqlens, cu_groups, scale))
+    return ext().attention_shared_prefix(q, k, v, cu_seqlens, cu_groups, scale)
 
 
-@torch.no_grad()
-def paged_decode_shared(q, k_cache, v_cache, block_tables, context_lens, cu_groups, shared_lens, max_group, k_scale, v_scale, scale):
+def paged_decode_shared(*args):
     _count(4)
-    return ext().paged_decode_shared(_head_rows(q), k_cache, v_cache, block_tables, context_lens, cu_groups, shared_lens, max_group, k_scale, v_scale, scale)
+    return ext().paged_decode_shared(*args)
 
 
-@torch.no_grad()
-def paged_decode_scored(q, k_cache, v_cache, block_tables, context_lens, scores, decay, k_scale, v_scale, scale, out_scores):
+def paged_decode_scored(*args):
     _count(3)
-    out_scores = scores if out_scores is None else out_scores
-    return ext().paged_decode_scored(_head_rows(q), k_cache, v_cache, block_tables, context_lens, scores, out_scores, decay, k_scale, v_scale, scale), out_scores
+    return ext().paged_decode_scored(*args)
 
 
-@torch.no_grad()
-def kv_evict(k_cache, v_cache, block_tables, context_lens, scores, keep, sinks, recent, k_scale, v_scale, out_tables):
-    _count(2 if k_scale is None else 3)
-    return ext().kv_evict(k_cache, v_cache, block_tables, context_lens, scores, keep, sinks, recent, k_scale, v_scale, out_tables)
+def kv_evict(*args):
+    _count(3)
+    return ext().kv_evict(*args)

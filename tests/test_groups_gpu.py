@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import groups_oracle as oracle
+from groups_refusals import refused_calls
 from nanorlhf_b200 import ops
 from nanorlhf_b200.ops import reference as ref
 
@@ -26,6 +27,16 @@ def within(got, want, bound, what, rounded=oracle.BF16):
     off = (got.double() - want).abs() - bound - rounded * want.abs() - 1e-30
     assert torch.isfinite(got).all(), what
     assert off.max().item() <= 0, f"{what}: {off.max().item()} beyond its bound at {off.argmax().item()}"
+
+
+def test_refusals():
+    refused_calls(DEV)
+    q = torch.zeros(4, 2, 128, device=DEV)
+    cu = torch.tensor([0, 4], dtype=torch.int32, device=DEV)
+    with pytest.raises(TypeError):
+        ops.attention_shared_prefix(q, q, q, cu, cu)                                        # float32
+    with pytest.raises(TypeError):
+        ops.attention_shared_prefix(*(q[..., :64].to(torch.bfloat16),) * 3, cu, cu)         # another head size
 
 
 # ---- packed groups -------------------------------------------------------------------------------------------------------------------------
