@@ -161,7 +161,7 @@ void check_pages(const torch::Tensor& k, const torch::Tensor& v, const c10::opti
                     ": block_tables [rows, pages] and context_lens [rows] are needed, got ", tables.sizes(), " and ", context.sizes());
   check_ints(tables, k, what, "block_tables");
   check_ints(context, k, what, "context_lens");
-  TORCH_CHECK_VALUE(tables.size(0) * tables.size(1) * k.size(1) <= kIntMax / 16 && tables.size(1) <= kIntMax / 512 && k.size(1) <= 256, what, ": too many rows, pages or heads");
+  TORCH_CHECK_VALUE(tables.size(0) * tables.size(1) * k.size(1) <= kIntMax / 16 && tables.size(0) * k.size(1) <= kIntMax / 64 && tables.size(1) <= kIntMax / 512 && k.size(1) <= 256, what, ": too many rows, pages or heads");
 }
 
 // a decode call's arguments, its result and its scratch
@@ -215,12 +215,8 @@ torch::Tensor paged_decode_shared(const torch::Tensor& q, const torch::Tensor& k
   const torch::Tensor cu_groups = cu_groups_in.contiguous(), shared = shared_in.contiguous();
   const nrl::DecodeCall& c = t.c;
   const int64_t groups = shared.numel(), max_group = std::min<int64_t>(max_group_in.value_or(c.S), c.S);
-  const int parts = groups > 0 ? nrl_decode_prefix_parts(groups, max_group, c.Hq, c.Hkv, c.max_blocks, num_sms()) : 0;
-  const int64_t lines = static_cast<int64_t>(c.S) * c.Hkv * parts * 8;
-  TORCH_CHECK_VALUE(lines <= kIntMax, what, ": too many rows");
-  float* prefix_o = t.take(lines * 132, nrl_decode_flat_scratch(&c, num_sms()));
-  check(nrl_paged_decode_shared(&c, cu_groups.data_ptr<int>(), shared.data_ptr<int>(), groups, max_group, parts, prefix_o, prefix_o + lines * 128, prefix_o + lines * 132,
-                                num_sms(), cur_stream()), what);
+  float* scratch = t.take(0, nrl_decode_scratch(&c, groups, max_group, num_sms()));
+  check(nrl_paged_decode_shared(&c, cu_groups.data_ptr<int>(), shared.data_ptr<int>(), groups, max_group, scratch, num_sms(), cur_stream()), what);
   return t.out;
 }
 
@@ -249,7 +245,7 @@ std::tuple<torch::Tensor, torch::Tensor> paged_decode_scored(const torch::Tensor
   TORCH_CHECK_VALUE(std::isfinite(decay), what, ": decay must be finite, got ", decay);
   if (t.empty()) return {t.out, into};
   const int64_t raws = 16LL * c.max_blocks * c.S * c.Hq;
-  float* raw = t.take(raws, nrl_decode_flat_scratch(&c, num_sms()));
+  float* raw = t.take(raws, nrl_decode_scratch(&c, 0, 0, num_sms()));
   check(nrl_paged_decode_scored(&c, scores.data_ptr<float>(), scores.stride(0), scores.stride(1), into.data_ptr<float>(), into.stride(0), into.stride(1), scores.size(2),
                                 static_cast<float>(decay), raw, raw + raws, num_sms(), cur_stream()), what);
   return {t.out, into};

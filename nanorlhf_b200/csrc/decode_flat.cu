@@ -12,6 +12,7 @@
 //                 walk left in scratch memory (4 G bytes a token beside the 512 or 264 of its keys and values; what fits L2 is not read from memory again)
 // The arithmetic is that of attention_decode.cu and attention_decode_fp8.cu.  Bound by memory.
 #include "common.cuh"
+#include "decode_runs.cuh"
 #include "fp8_fragments.cuh"
 #include "group_kernels.h"
 #include "launch.h"
@@ -24,6 +25,7 @@ namespace nrl {
 constexpr int kFlatWarps = 4;
 constexpr int kFlatD = 128;
 constexpr int kPlanThreads = 1024;
+constexpr int kPrefixLeast = 2;                   // steps of the prefixes a run
 constexpr float kFlatScale = 1024.f;              // of fp8 weights, which are f16 (2^10: small ones stay normal)
 
 template <bool FP8>
@@ -35,26 +37,6 @@ struct FlatSizes {
   static constexpr int kTotal = kFlatWarps * kStages * kStage;
 };
 
-struct FlatParams {
-  const __nv_bfloat16* q;
-  const uint8_t *k, *v;
-  const float *ks, *vs;
-  const int *block_tables, *context_lens, *cu_groups, *shared;
-  int4* rows;                   // [S] first token that the row walks itself, pages of the rows in front (of one kv head), its own pages, whether it has a prefix;
-                                // [S]: -, pages of all rows, pages a run, -
-  int4* starts;                 // [runs] row, kv head, page of the row's own, -
-  float *part_o, *part_ml;      // [runs + S Hkv, 8, D], [.., 8, 2]
-  float* raw;                   // scores in log2 units [S, Hkv, G, 16 max_blocks] (null: none)
-  const float *prefix_o, *prefix_ml;   // [S, Hkv, prefix_parts, 8, D], [.., 2]
-  __nv_bfloat16* out;
-  const float* scores_in;
-  float* scores_out;
-  long q_stride_s, in_row, in_head, out_row, out_head;
-  int n_groups, prefix_parts, S, max_blocks, Hq, Hkv, G, runs, least, max_tokens, chunk, wide;
-  float scale_log2, decay;
-};
-
-NRL_DEVICE int flat_context(const FlatParams& p, int s) { return max(0, min(p.context_lens[s], p.max_blocks * 16)); }
 // the last group that begins at or in front of a row; it has the row if it does not end there
 NRL_DEVICE int group_search(const int* cu, int n, int row) {
   int lo = 0, hi = n;
@@ -65,80 +47,105 @@ NRL_DEVICE int group_search(const int* cu, int n, int row) {
   return lo;
 }
 
+// the sum of `n` over the threads in front, and over all (a whole block)
+NRL_DEVICE int plan_scan(int n, int* warp_sums, int& all) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int upto = n;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += v;
+  }
+  if (lane == 31) warp_sums[warp] = upto;
+  __syncthreads();
+  const int mine = warp_sums[lane];
+  int sums = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, sums, d);
+    if (lane >= d) sums += v;
+  }
+  const int in_front = __shfl_sync(0xffffffffu, sums - mine, warp);
+  all = __shfl_sync(0xffffffffu, sums, 31);
+  __syncthreads();
+  return in_front + upto - n;
+}
+// Where runs begin: in which owner's stretch, and there, as quotient and remainder by its divisor.  `from`: the first position of every owner (by index), `total` behind the last.
+template <class From, class Divisor>
+NRL_DEVICE void plan_starts(int4* starts, int owners, int total, int run, From from, Divisor divisor) {
+  for (int w = threadIdx.x; w * run < total; w += kPlanThreads) {
+    int lo = 0, hi = owners;                                         // the last owner that begins at or in front: one that has something
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (from(mid) <= w * run) lo = mid; else hi = mid;
+    }
+    const int at = w * run - from(lo), d = divisor(lo), q = at / d;
+    starts[w] = make_int4(lo, q, at - q * d, 0);
+  }
+}
+
+// (all positions are below 2^27: checked on the host)
 __global__ void __launch_bounds__(kPlanThreads) decode_plan_kernel(const FlatParams p) {
   pdl_wait();
   pdl_launch_dependents();
   __shared__ int warp_sums[32];
-  __shared__ int cu_near[kPlanThreads + 1];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  __shared__ int cu_near[kPlanThreads + 1], from_near[kPlanThreads];
+  const int tid = threadIdx.x;
   const int* cu = p.cu_groups;
   if (p.n_groups > 0 && p.n_groups <= kPlanThreads) {
     for (int i = tid; i <= p.n_groups; i += kPlanThreads) cu_near[i] = p.cu_groups[i];
     cu = cu_near;
     __syncthreads();
   }
-  int before = 0, off = 0, n = 0;                                    // pages of the rows in front of this pass; of this thread's row in the last one
+  auto group_ok = [&](int g) { return cu[g] >= 0 && cu[g] < cu[g + 1] && cu[g + 1] <= p.S; };
+  // ---- rows ----
+  int before = 0, off, all;                                          // pages of the rows in front of this pass
   for (int s0 = 0; s0 < p.S; s0 += kPlanThreads) {
     const int s = s0 + tid;
-    int first = 0, prefix = 0;
-    n = 0;
+    int first = 0, prefix = 0, n = 0;
     if (s < p.S) {
       const int ctx = flat_context(p, s);
       if (p.n_groups > 0) {
         const int g = group_search(cu, p.n_groups, s);
-        if (cu[g] <= s && s < cu[g + 1]) {
+        if (cu[g] <= s && s < cu[g + 1] && group_ok(g)) {
           const int shared = p.shared[g];
-          prefix = shared > 0;
+          prefix = shared > 0 ? g + 1 : 0;
           first = max(0, min(shared, ctx));
         }
       }
-      n = (ctx + 15) / 16 - first / 16;
+      n = (ctx + 15) / 16 - first / 16 + (p.prefix_runs == 0 ? (first + 15) / 16 : 0);
     }
-    int upto = n;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, upto, d);
-      if (lane >= d) upto += v;
-    }
-    if (lane == 31) warp_sums[warp] = upto;
-    __syncthreads();
-    const int mine = warp_sums[lane];
-    int sums = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, sums, d);
-      if (lane >= d) sums += v;
-    }
-    const int in_front = __shfl_sync(0xffffffffu, sums - mine, warp), all = __shfl_sync(0xffffffffu, sums, 31);
-    off = before + in_front + upto - n;
+    off = before + plan_scan(n, warp_sums, all);
     if (s < p.S) p.rows[s] = make_int4(first, off, n, prefix);
+    from_near[tid] = off;
     before += all;
-    __syncthreads();
   }
   const int run = max(p.least, (before * p.Hkv + p.runs - 1) / p.runs);
   if (tid == 0) p.rows[p.S] = make_int4(0, before, run, 0);
-  // the beginnings of the runs that begin in a row
-  for (int s0 = 0; s0 < p.S; s0 += kPlanThreads) {
-    if (p.S > kPlanThreads) {                                        // (a block sees its own writes)
-      const int4 row = s0 + tid < p.S ? p.rows[s0 + tid] : make_int4(0, 0, 0, 0);
-      off = row.y;
-      n = row.z;
+  __syncthreads();                                                   // (a block sees its own writes)
+  plan_starts(p.starts, p.S, before * p.Hkv, run, [&](int s) { return (p.S <= kPlanThreads ? from_near[s] : p.rows[s].y) * p.Hkv; }, [&](int s) { return p.rows[s].z; });
+  if (p.prefix_runs == 0) return;
+  // ---- prefixes ----
+  before = 0;
+  __syncthreads();
+  for (int g0 = 0; g0 < p.n_groups; g0 += kPlanThreads) {
+    const int g = g0 + tid;
+    int rows = 0, tiles = 0, steps = 0;
+    if (g < p.n_groups && group_ok(g)) {
+      rows = (cu[g + 1] - cu[g]) * p.G;
+      tiles = (rows + kPrefixRows - 1) / kPrefixRows;
+      steps = (max(0, min(p.shared[g], p.max_blocks * 16)) + kPrefixKeys - 1) / kPrefixKeys;
     }
-    // (all positions are below 2^27: checked on the host)
-    const int s = s0 + tid, a = off * p.Hkv, w0 = s < p.S ? (a + run - 1) / run : 0, some = s < p.S && n > 0 ? max(0, (a + n * p.Hkv + run - 1) / run - w0) : 0;
-    auto begin = [&](int w, int row, int a_row, int n_row) {
-      const int at = w * run - a_row, h = at / n_row;
-      p.starts[w] = make_int4(row, h, at - h * n_row, 0);
-    };
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < some) begin(w0 + i, s, a, n);
-    for (uint32_t many = __ballot_sync(0xffffffffu, some > 4); many != 0; many &= many - 1) {        // few rows with many runs
-      const int l = __ffs(many) - 1, a_l = __shfl_sync(0xffffffffu, a, l), n_l = __shfl_sync(0xffffffffu, n, l), w_l = __shfl_sync(0xffffffffu, w0, l),
-                some_l = __shfl_sync(0xffffffffu, some, l);
-      for (int i = 4 + lane; i < some_l; i += 32) begin(w_l + i, s0 + warp * 32 + l, a_l, n_l);
-    }
+    off = before + plan_scan(steps * tiles * p.Hkv, warp_sums, all);
+    if (g < p.n_groups) p.groups[g] = make_int4(off, steps, tiles, rows);
+    from_near[tid] = off;
+    before += all;
   }
+  const int prefix_run = max(kPrefixLeast, (before + p.prefix_runs - 1) / p.prefix_runs);
+  if (tid == 0) p.groups[p.n_groups] = make_int4(before, prefix_run, 0, 0);
+  __syncthreads();
+  plan_starts(p.prefix_starts, p.n_groups, before, prefix_run, [&](int g) { return p.n_groups <= kPlanThreads ? from_near[g] : p.groups[g].x; },
+              [&](int g) { return p.groups[g].y; });
 }
 
 NRL_DEVICE void flat_ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
@@ -155,30 +162,39 @@ NRL_DEVICE void flat_mma_bf16(float (&d)[4], uint32_t a0, uint32_t a2, uint32_t 
 
 // A place in the run: a row-head and a page of its own.
 struct FlatAt {
-  int s, h, page, pages;        // pages: of the row; page < pages
+  int s, h, page, pages;        // pages: that the row walks; page < pages
   int first, ctx;               // the row's first token of its own, its context
+  int lead, lead_row;           // pages of a prefix that the row walks itself, in front, and the row whose they are
 };
+template <bool LEAD>
 NRL_DEVICE void flat_row(const FlatParams& p, FlatAt& a, int s) {
   const int4 row = p.rows[s];
   a.s = s;
   a.first = row.x;
   a.pages = row.z;
   a.ctx = flat_context(p, s);
+  a.lead = LEAD && p.prefix_runs == 0 ? (a.first + 15) / 16 : 0;
+  a.lead_row = a.lead > 0 ? p.cu_groups[row.w - 1] : 0;
 }
+template <bool LEAD>
 NRL_DEVICE bool flat_next(const FlatParams& p, FlatAt& a) {          // true: another row-head begins
   if (++a.page < a.pages) return false;
   a.page = 0;
   if (++a.h == p.Hkv) {
     a.h = 0;
-    do flat_row(p, a, a.s + 1); while (a.pages == 0 && a.s + 1 < p.S);
+    do flat_row<LEAD>(p, a, a.s + 1); while (a.pages == 0 && a.s + 1 < p.S);
   }
   return true;
+}
+// the page table's entry of page i that the row walks
+NRL_DEVICE long flat_entry(const FlatParams& p, const FlatAt& a, int i) {
+  return i < a.lead ? static_cast<long>(a.lead_row) * p.max_blocks + i : static_cast<long>(a.s) * p.max_blocks + a.first / 16 + i - a.lead;
 }
 
 template <bool FP8, bool SCORES>
 __global__ void __launch_bounds__(kFlatWarps * 32, FlatSizes<FP8>::kBlocks) decode_flat_kernel(const FlatParams p) {
   // Behind decode_prefix, whose blocks have all begun when this one's do, and with that found decode_plan ended: nothing is taken from it, and only the end waits for its.
-  const bool beside = p.prefix_parts > 0;
+  const bool beside = p.prefix_runs > 0;
   if (!beside) pdl_wait();
   pdl_launch_dependents();
   using Z = FlatSizes<FP8>;
@@ -193,7 +209,7 @@ __global__ void __launch_bounds__(kFlatWarps * 32, FlatSizes<FP8>::kBlocks) deco
   FlatAt here, ahead;
   {
     const int4 start = p.starts[w];
-    flat_row(p, here, start.x);
+    flat_row<!SCORES>(p, here, start.x);
     here.h = start.y;
     here.page = start.z;
     ahead = here;
@@ -206,7 +222,7 @@ __global__ void __launch_bounds__(kFlatWarps * 32, FlatSizes<FP8>::kBlocks) deco
     if (issued < count) {
       if (ids_from < 0 || ahead.page - ids_from >= 32) {
         ids_from = ahead.page;
-        ids = ids_from + lane < ahead.pages ? p.block_tables[static_cast<long>(ahead.s) * p.max_blocks + ahead.first / 16 + ids_from + lane] : 0;
+        ids = ids_from + lane < ahead.pages ? p.block_tables[flat_entry(p, ahead, ids_from + lane)] : 0;
       }
       const long pg = static_cast<long>(__shfl_sync(0xffffffffu, ids, ahead.page - ids_from)) * p.Hkv + ahead.h;
       uint8_t *kd = ring + (issued % Z::kStages) * Z::kStage, *vd = kd + Z::kHalf;
@@ -227,7 +243,7 @@ __global__ void __launch_bounds__(kFlatWarps * 32, FlatSizes<FP8>::kBlocks) deco
           cp_async_16(vd + at, vsrc + chunk * 16);
         }
       }
-      if (++issued < count && flat_next(p, ahead)) ids_from = -1;
+      if (++issued < count && flat_next<!SCORES>(p, ahead)) ids_from = -1;
     }
     cp_async_commit();
   };
@@ -275,14 +291,15 @@ __global__ void __launch_bounds__(kFlatWarps * 32, FlatSizes<FP8>::kBlocks) deco
     constexpr int U = decltype(number)::value;
     cp_async_wait<FP8 ? Z::kStages - U : Z::kStages - 1>();
     __syncwarp();
-    const int page = here.first / 16 + here.page;
     float s[U][2][4], vscale[U][4];
     float top = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       uint8_t* st = ring + ((it + u) % Z::kStages) * Z::kStage;
       const uint32_t kb = smem_u32(st);
-      const int tok0 = (page + u) * 16;
+      const int page = here.page + u;
+      const bool lead = !SCORES && page < here.lead;
+      const int tok0 = lead ? page * 16 : (here.first / 16 + page - here.lead) * 16;
 #pragma unroll
       for (int j = 0; j < 2; ++j) s[u][j][0] = s[u][j][1] = s[u][j][2] = s[u][j][3] = 0.f;
       // ---- S = Q K^T.  Key of column (j, e): bf16 8 j + 2 t + e, fp8 4 t + 2 j + e ----
@@ -321,7 +338,7 @@ __global__ void __launch_bounds__(kFlatWarps * 32, FlatSizes<FP8>::kBlocks) deco
           for (int e = 0; e < 2; ++e) s[u][j][e] *= p.scale_log2;
       }
       // ---- mask; values and scales outside the row's own tokens, whatever they are, meet weights of 0 as zeros ----
-      const int lo = here.first - tok0, hi = here.ctx - tok0;
+      const int lo = lead ? 0 : here.first - tok0, hi = (lead ? here.first : here.ctx) - tok0;
       if (lo > 0 || hi < 16) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -409,7 +426,7 @@ __global__ void __launch_bounds__(kFlatWarps * 32, FlatSizes<FP8>::kBlocks) deco
     if (two) ++here.page;
     if (it == count) break;
     const FlatAt last = here;
-    if (flat_next(p, here)) {
+    if (flat_next<!SCORES>(p, here)) {
       const FlatAt now = here;
       here = last;
       leave();
@@ -426,25 +443,35 @@ __global__ void __launch_bounds__(kFlatWarps * 32, FlatSizes<FP8>::kBlocks) deco
 constexpr int kJoinU = 4;                // parts in flight
 
 struct FlatParts {
-  const float2* ml;                      // of the row-head's first part: [n][8]
-  const float4* o;                       // [n][8][32]
+  const float2* ml;                      // of the first part of a row
+  const float4* o;
   int n;
 };
-NRL_DEVICE FlatParts flat_parts(const FlatParams& p, int4 row, int s, int h) {
+// head r's parts of a row's own tokens
+NRL_DEVICE FlatParts flat_parts(const FlatParams& p, int4 row, int s, int h, int r) {
   const int run = p.rows[p.S].z, a = row.y * p.Hkv + h * row.z, w0 = a / run;
-  const long at = (static_cast<long>(w0) + static_cast<long>(s) * p.Hkv + h) * 8;
+  const long at = (static_cast<long>(w0) + static_cast<long>(s) * p.Hkv + h) * 8 + r;
   return {reinterpret_cast<const float2*>(p.part_ml) + at, reinterpret_cast<const float4*>(p.part_o) + at * 32, row.z > 0 ? (a + row.z - 1) / run - w0 + 1 : 0};
 }
-// head r's parts; a lane has four elements
-NRL_DEVICE void join_parts(const FlatParts& x, int r, int lane, float& M, float& L, float4& acc) {
+// and of the prefix's, one a run
+NRL_DEVICE FlatParts prefix_parts(const FlatParams& p, int g, int s, int h, int r) {
+  const int4 group = p.groups[g];
+  const int first = p.cu_groups[g], row = (s - first) * p.G + r, run = p.groups[p.n_groups].y, a = group.x + (h * group.z + row / kPrefixRows) * group.y, c0 = a / run;
+  const long at = prefix_part_row(p, first, h, group.w, row) + static_cast<long>(kPrefixRows) * c0;
+  return {reinterpret_cast<const float2*>(p.prefix_ml) + at, reinterpret_cast<const float4*>(p.prefix_o) + at * 32, (a + group.y - 1) / run - c0 + 1};
+}
+// a lane has four elements; a row's parts lie 8 rows apart, a prefix's 64
+template <bool PREFIX>
+NRL_DEVICE void join_parts(const FlatParts& x, int lane, float& M, float& L, float4& acc) {
   for (int i0 = 0; i0 < x.n; i0 += kJoinU) {
     float2 e[kJoinU];
     float4 o[kJoinU];
 #pragma unroll
     for (int u = 0; u < kJoinU; ++u) {
       const bool ok = i0 + u < x.n;
-      e[u] = ok ? x.ml[(i0 + u) * 8 + r] : make_float2(-INFINITY, 0.f);
-      o[u] = ok ? x.o[((i0 + u) * 8 + r) * 32 + lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+      const long at = (i0 + u) * (PREFIX ? static_cast<long>(kPrefixRows) : 8L);
+      e[u] = ok ? x.ml[at] : make_float2(-INFINITY, 0.f);
+      o[u] = ok ? x.o[at * 32 + lane] : make_float4(0.f, 0.f, 0.f, 0.f);
     }
 #pragma unroll
     for (int u = 0; u < kJoinU; ++u) {
@@ -466,17 +493,14 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const FlatParams p) {
   const int ctx = flat_context(p, s), t0 = chunk * p.chunk, n = SCORES ? min(min(ctx, p.max_tokens), t0 + p.chunk) : 0;
   if (chunk > 0 && t0 >= n) return;
   const int4 row = p.rows[s];
-  const FlatParts own = flat_parts(p, row, s, h);
   __shared__ float top[8], inv[8];
   if (warp < p.G) {
+    const FlatParts own = flat_parts(p, row, s, h, warp);
     float M = -INFINITY, L = 0.f;
     if (chunk == 0) {
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (!SCORES && row.w) {
-        const long at = (static_cast<long>(s) * p.Hkv + h) * p.prefix_parts * 8;
-        join_parts({reinterpret_cast<const float2*>(p.prefix_ml) + at, reinterpret_cast<const float4*>(p.prefix_o) + at * 32, p.prefix_parts}, warp, lane, M, L, acc);
-      }
-      join_parts(own, warp, lane, M, L, acc);
+      if (!SCORES && row.w > 0 && p.prefix_runs > 0) join_parts<true>(prefix_parts(p, row.w - 1, s, h, warp), lane, M, L, acc);
+      join_parts<false>(own, lane, M, L, acc);
       const float f = L > 0.f ? 1.f / L : 0.f;
       uint2 v;
       v.x = pack_bf16x2(acc.x * f, acc.y * f);
@@ -484,7 +508,7 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const FlatParams p) {
       *reinterpret_cast<uint2*>(p.out + (static_cast<long>(s) * p.Hq + h * p.G + warp) * kFlatD + lane * 4) = v;
     } else {
       for (int i = lane; i < own.n; i += 32) {
-        const float2 e = own.ml[i * 8 + warp];
+        const float2 e = own.ml[i * 8];
         const float m = fmaxf(M, e.x);
         if (m == -INFINITY) continue;
         L = L * exp2f(M - m) + e.y * exp2f(e.x - m);
@@ -549,26 +573,33 @@ cudaError_t launch_flat(const FlatParams& p, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-// 16-byte pieces of scratch, one behind the other
+// pieces of scratch, one behind the other, on 64 bytes
 struct Pieces {
   uint8_t* at;
   size_t used = 0;
   template <class T>
   T* take(size_t n) {
     T* r = reinterpret_cast<T*>(at + used);
-    used += (n * sizeof(T) + 15) / 16 * 16;
+    used += (n * sizeof(T) + 63) / 64 * 64;
     return r;
   }
 };
 
-// runs: as many as warps fit the chip, or as the longest contexts that the tables allow could fill
-struct FlatPlan { int runs, least; };
-FlatPlan flat_plan(const DecodeCall* c, int num_sms) {
+// Runs: as many as warps (prefixes: blocks) fit the chip, or as the longest contexts that the tables allow could fill.
+// Where those contexts are few bytes, rows walk their prefixes themselves: the prefixes' kernel takes 8 us, in which decode_flat reads 40 MB.
+constexpr long kPrefixBytes = 40L << 20;
+struct FlatPlan { int runs, least, n_groups, prefix_runs; };
+FlatPlan flat_plan(const DecodeCall* c, int n_groups, int max_group, int num_sms) {
   const long most = static_cast<long>(c->S) * c->Hkv * c->max_blocks;
-  const int fit = num_sms * kFlatWarps * (c->k_scale != nullptr ? FlatSizes<true>::kBlocks : FlatSizes<false>::kBlocks);
-  const int least = 2;
+  const int fit = num_sms * kFlatWarps * (c->k_scale != nullptr ? FlatSizes<true>::kBlocks : FlatSizes<false>::kBlocks), least = 2;
   const long runs = (most + least - 1) / least;
-  return {static_cast<int>(runs < fit ? runs : fit), least};
+  FlatPlan plan = {static_cast<int>(runs < fit ? runs : fit), least, n_groups, 0};
+  if (n_groups > 0 && most * (c->k_scale != nullptr ? FlatSizes<true>::kStage : FlatSizes<false>::kStage) > kPrefixBytes) {
+    const long tiles = (static_cast<long>(max_group) * (c->Hq / c->Hkv) + kPrefixRows - 1) / kPrefixRows;
+    const long most_runs = (n_groups * tiles * c->Hkv * ((c->max_blocks * 16L + kPrefixKeys - 1) / kPrefixKeys) + kPrefixLeast - 1) / kPrefixLeast;
+    plan.prefix_runs = static_cast<int>(most_runs < 2L * num_sms ? most_runs : 2L * num_sms);
+  }
+  return plan;
 }
 size_t lay_out(FlatParams& p, const DecodeCall* c, const FlatPlan& plan, void* scratch) {
   Pieces pieces = {static_cast<uint8_t*>(scratch)};
@@ -577,6 +608,13 @@ size_t lay_out(FlatParams& p, const DecodeCall* c, const FlatPlan& plan, void* s
   p.starts = pieces.take<int4>(plan.runs);
   p.part_ml = pieces.take<float>(parts * 16);
   p.part_o = pieces.take<float>(parts * 8 * kFlatD);
+  if (plan.prefix_runs > 0) {
+    const size_t rows = static_cast<size_t>(c->S) * c->Hq + kPrefixRows * static_cast<size_t>(plan.prefix_runs);
+    p.groups = pieces.take<int4>(plan.n_groups + 1);
+    p.prefix_starts = pieces.take<int4>(plan.prefix_runs);
+    p.prefix_ml = pieces.take<float>(rows * 2);
+    p.prefix_o = pieces.take<float>(rows * kFlatD);
+  }
   return pieces.used;
 }
 FlatParams flat_params(const DecodeCall* c, const FlatPlan& plan, void* scratch) {
@@ -590,7 +628,7 @@ FlatParams flat_params(const DecodeCall* c, const FlatPlan& plan, void* scratch)
   p.out = static_cast<__nv_bfloat16*>(c->out);
   p.q_stride_s = c->q_stride_s;
   p.S = c->S; p.max_blocks = c->max_blocks; p.Hq = c->Hq; p.Hkv = c->Hkv; p.G = c->Hq / c->Hkv;
-  p.runs = plan.runs; p.least = plan.least;
+  p.runs = plan.runs; p.least = plan.least; p.n_groups = plan.n_groups; p.prefix_runs = plan.prefix_runs;
   p.scale_log2 = c->scale * 1.4426950408889634f;
   return p;
 }
@@ -600,21 +638,19 @@ FlatParams flat_params(const DecodeCall* c, const FlatPlan& plan, void* scratch)
 
 using namespace nrl;
 
-extern "C" size_t nrl_decode_flat_scratch(const DecodeCall* c, int num_sms) {
+extern "C" size_t nrl_decode_scratch(const DecodeCall* c, int n_groups, int max_group, int num_sms) {
   FlatParams p = {};
-  return lay_out(p, c, flat_plan(c, num_sms), nullptr);
+  return lay_out(p, c, flat_plan(c, n_groups, max_group, num_sms), nullptr);
 }
 
-extern "C" cudaError_t nrl_paged_decode_shared(const DecodeCall* c, const int* cu_groups, const int* shared, int n_groups, int max_group, int prefix_parts,
-                                               float* prefix_o, float* prefix_ml, void* scratch, int num_sms, cudaStream_t s) {
+extern "C" cudaError_t nrl_paged_decode_shared(const DecodeCall* c, const int* cu_groups, const int* shared, int n_groups, int max_group, void* scratch, int num_sms,
+                                               cudaStream_t s) {
   if (c->S == 0) return cudaSuccess;
-  FlatParams p = flat_params(c, flat_plan(c, num_sms), scratch);
-  p.cu_groups = cu_groups; p.shared = shared; p.n_groups = n_groups;
-  p.prefix_parts = n_groups > 0 ? prefix_parts : 0;
-  p.prefix_o = prefix_o; p.prefix_ml = prefix_ml;
+  FlatParams p = flat_params(c, flat_plan(c, n_groups, max_group, num_sms), scratch);
+  p.cu_groups = cu_groups; p.shared = shared;
   launch_dependent(decode_plan_kernel, 1, kPlanThreads, 0, s, p);
   cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess && n_groups > 0) e = nrl_decode_prefix(c, cu_groups, shared, n_groups, max_group, prefix_parts, prefix_o, prefix_ml, s);
+  if (e == cudaSuccess && p.prefix_runs > 0) e = launch_decode_prefix(p, s);
   if (e == cudaSuccess) e = c->k_scale != nullptr ? launch_flat<true, false>(p, s) : launch_flat<false, false>(p, s);
   if (e != cudaSuccess) return e;
   launch_dependent(decode_join_kernel<false>, dim3(c->S, c->Hkv), 32 * p.G, 0, s, p);
@@ -624,7 +660,7 @@ extern "C" cudaError_t nrl_paged_decode_shared(const DecodeCall* c, const int* c
 extern "C" cudaError_t nrl_paged_decode_scored(const DecodeCall* c, const float* scores_in, long in_row, long in_head, float* scores_out, long out_row, long out_head,
                                                int max_tokens, float decay, float* raw, void* scratch, int num_sms, cudaStream_t s) {
   if (c->S == 0) return cudaSuccess;
-  FlatParams p = flat_params(c, flat_plan(c, num_sms), scratch);
+  FlatParams p = flat_params(c, flat_plan(c, 0, 0, num_sms), scratch);
   p.raw = raw; p.scores_in = scores_in; p.scores_out = scores_out;
   p.in_row = in_row; p.in_head = in_head; p.out_row = out_row; p.out_head = out_head;
   p.max_tokens = max_tokens < 16 * c->max_blocks ? max_tokens : 16 * c->max_blocks;

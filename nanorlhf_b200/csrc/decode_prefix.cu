@@ -1,24 +1,25 @@
-// Decode attention of rows that share their first tokens: the prefix once per group, the rest per row.
+// Decode attention of rows that share their first tokens: the prefix's part.
 //
-//   out = sum_parts 2^(m_p - M) O_p / sum_parts 2^(m_p - M) l_p,  a part being the (maximum, sum, unnormalised result) of some of the row's keys
+// The query rows of a group (samples x G heads of a kv head) are tiles of up to 64; every key and value of the prefix is read from memory once for a tile.
+// The prefixes' steps of 64 tokens, of all tiles one behind the other, are dealt to the blocks in equal runs (decode_flat.cu: decode_plan), two blocks an SM; a run
+// that meets a tile leaves a part of it, (maximum, sum, unnormalised result), which is decode_join's.
 //
-// The prefix's parts are formed here: the query rows of a group (samples x G heads of a kv head) are up to 64 rows of a tile, every key and value of the prefix is
-// read from memory once for all of them.  The rest of a row's tokens are decode_flat.cu's, which joins the parts.
-//
-// Block = 4 warps of 16 rows; 64 keys (4 pages) a step through shared memory (cp.async, three stages), mma.sync m16n8k16.  fp8 pages are dequantised on the
-// operand fragments as in attention_decode_fp8.cu.
+// Block = 4 warps of 16 rows; 4 pages a step through shared memory (cp.async, three stages), mma.sync m16n8k16.  fp8 pages are dequantised on the operand
+// fragments as in attention_decode_fp8.cu.  Bound by issue slots (fp8, 112 rows: 720 instructions a warp and step), with few rows by memory.
+// On tcgen05, tiles of 128 rows against blocks of 128 keys with two streams of scores and a warpgroup each for their softmax, 13 groups x 4 kv heads x 4096 fp8
+// tokens of 112 rows took 44 us and 64 x 2 x 390 bf16 tokens of 48 rows 21: a tile of few rows costs the tensor pipe as much as a full one, and fp8 pages' way
+// through registers into its tiles competes with the softmax for issue slots.
 #include "common.cuh"
+#include "decode_runs.cuh"
 #include "fp8_fragments.cuh"
-#include "group_kernels.h"
 #include "launch.h"
 #include "per_device.h"
 
 namespace nrl {
 
-constexpr int kPreWarps = 4;
-constexpr int kPreRows = kPreWarps * 16;          // query rows of a block
+constexpr int kPreWarps = kPrefixRows / 16;
 constexpr int kPreStages = 3;
-constexpr int kPreStep = 4;                       // pages a step
+constexpr int kPreStep = kPrefixKeys / 16;        // pages a step
 constexpr float kPreScale = 1024.f;               // of fp8 weights, which are f16 (2^10: small ones stay normal)
 
 template <bool FP8>
@@ -29,15 +30,37 @@ struct PreSmem {
   static constexpr int kTotal = kPreStages * kStage;
 };
 
-struct PrefixParams {
-  const __nv_bfloat16* q;
-  const uint8_t *k, *v;
-  const float *ks, *vs;
-  const int *block_tables, *context_lens, *cu_groups, *shared;
-  float *part_o, *part_ml;
-  long q_stride_s;
-  int S, max_blocks, Hkv, G, prefix_parts, tiles;
-  float scale_log2;
+// Where a run stands: steps [step, step + n) of a tile
+struct PreWalk {
+  int g, h, tile, step, n;
+  int first, rows;                                 // the group's first row; query rows of a kv head
+  int shared, tiles, steps;                        // tokens; the group's tiles and steps
+  int left, at;                                    // steps of the run from this segment on; kv head x tiles + tile
+  NRL_DEVICE explicit PreWalk(const FlatParams& p) {
+    const int4 all = p.groups[p.n_groups], start = p.prefix_starts[blockIdx.x];        // all steps, steps a run
+    left = min(all.y, all.x - static_cast<int>(blockIdx.x) * all.y);
+    at = start.y;
+    if (left > 0) enter(p, start.x, start.z);
+  }
+  NRL_DEVICE void enter(const FlatParams& p, int group, int from) {
+    const int4 x = p.groups[group];
+    g = group; step = from;
+    first = p.cu_groups[g];
+    shared = min(p.shared[g], p.max_blocks * 16);
+    steps = x.y; tiles = x.z; rows = x.w;
+    h = at / tiles; tile = at - h * tiles;
+    n = min(left, steps - step);
+  }
+  NRL_DEVICE void next(const FlatParams& p) {
+    left -= n;
+    if (left <= 0) return;
+    int group = g;
+    if (++at == p.Hkv * tiles) {
+      at = 0;
+      do ++group; while (p.groups[group].y == 0);
+    }
+    enter(p, group, 0);
+  }
 };
 
 NRL_DEVICE void pre_ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
@@ -57,33 +80,28 @@ NRL_DEVICE void pre_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint
 }
 
 template <bool FP8>
-__global__ void __launch_bounds__(kPreWarps * 32, 2) decode_prefix_kernel(const PrefixParams p) {
+__global__ void __launch_bounds__(kPreWarps * 32, 2) decode_prefix_kernel(const FlatParams p) {
   pdl_wait();
   pdl_launch_dependents();
   using L = PreSmem<FP8>;
   extern __shared__ __align__(128) uint8_t smem[];
-  const int group = blockIdx.x, kvh = blockIdx.y, part = blockIdx.z / p.tiles;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
-  const int seq0 = p.cu_groups[group], n_rows = (min(p.cu_groups[group + 1], p.S) - seq0) * p.G;
-  const int shared = min(p.shared[group], p.max_blocks * 16);
-  if (shared <= 0) return;
-  const int n_steps = (shared + 16 * kPreStep - 1) / (16 * kPreStep), per_part = (n_steps + p.prefix_parts - 1) / p.prefix_parts;
-  const int step_lo = part * per_part, step_hi = min(n_steps, step_lo + per_part);
-  const int n_pages = (shared + 15) / 16;
-  const int* bt = p.block_tables + static_cast<long>(seq0) * p.max_blocks;
 
-  int ids[kPreStep];                                                 // pages of the step that is copied next
-  auto look_up = [&](int step) {
-#pragma unroll
-    for (int u = 0; u < kPreStep; ++u) ids[u] = step < step_hi && step * kPreStep + u < n_pages ? bt[step * kPreStep + u] : 0;
+  PreWalk in(p);                                                     // what is copied next: step in.step + in_j
+  const int total = max(0, in.left);
+  int in_j = 0, n_in = 0, id = 0;                                    // its page numbers, in the lanes
+  auto look_up = [&]() {
+    const int page = (in.step + in_j) * kPreStep + lane;
+    id = in.left > 0 && lane < kPreStep && page * 16 < in.shared ? p.block_tables[static_cast<long>(in.first) * p.max_blocks + page] : 0;
   };
-  auto issue = [&](int step) {
-    if (step < step_hi) {
-      uint8_t* st = smem + ((step - step_lo) % kPreStages) * L::kStage;
+  look_up();
+  auto issue = [&]() {
+    if (n_in < total) {
+      uint8_t* st = smem + (n_in % kPreStages) * L::kStage;
 #pragma unroll
       for (int u = 0; u < kPreStep; ++u) {
-        if (step * kPreStep + u >= n_pages) break;
-        const long pg = static_cast<long>(ids[u]) * p.Hkv + kvh;
+        const long pg = static_cast<long>(__shfl_sync(0xffffffffu, id, u)) * p.Hkv + in.h;
+        if (((in.step + in_j) * kPreStep + u) * 16 >= in.shared) break;
         const uint8_t *ksrc = p.k + pg * L::kHalf, *vsrc = p.v + pg * L::kHalf;
         uint8_t *kd = st + u * L::kPageSize, *vd = kd + L::kHalf;
         if (FP8) {
@@ -99,31 +117,38 @@ __global__ void __launch_bounds__(kPreWarps * 32, 2) decode_prefix_kernel(const 
           }
         }
       }
+      ++n_in;
+      if (++in_j == in.n) {
+        in_j = 0;
+        in.next(p);
+      }
+      look_up();
     }
     cp_async_commit();
-    look_up(step + 1);
   };
+  issue();
+  issue();
 
-  // (one tile a block; more only where a group is larger than was said)
-  for (int tile = blockIdx.z - part * p.tiles; tile * kPreRows < n_rows; tile += p.tiles) {
+  int n_out = 0;
+  for (PreWalk w(p); w.left > 0; w.next(p)) {
+    const int shared = w.shared;
     // this thread's rows: g and g + 8 of the warp's sixteen
-    int row[2], limit[2];
+    int limit[2];
     bool real[2];
     const __nv_bfloat16* qrow[2];
-  #pragma unroll
+#pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int at = tile * kPreRows + warp * 16 + g + i * 8;
-      real[i] = at < n_rows;
-      const int seq = seq0 + (real[i] ? at / p.G : 0), r = real[i] ? at % p.G : 0;
-      row[i] = (seq * p.Hkv + kvh) * p.prefix_parts * 8 + r;          // of the parts, without the part (S * Hkv * parts * 8 is below 2^31: checked on the host)
+      const int at = w.tile * kPrefixRows + warp * 16 + g + i * 8;
+      real[i] = at < w.rows;
+      const int seq = w.first + (real[i] ? at / p.G : 0), r = real[i] ? at % p.G : 0;
       limit[i] = real[i] ? min(shared, p.context_lens[seq]) : 0;
-      qrow[i] = p.q + seq * p.q_stride_s + (kvh * p.G + r) * 128;
+      qrow[i] = p.q + seq * p.q_stride_s + (w.h * p.G + r) * 128;
     }
-    const bool busy = tile * kPreRows + warp * 16 < n_rows;            // a warp without rows only copies
+    const bool busy = w.tile * kPrefixRows + warp * 16 < w.rows;     // a warp without rows only copies
     uint32_t qf[8][4];
-  #pragma unroll
+#pragma unroll
     for (int ks = 0; ks < 8; ++ks)
-  #pragma unroll
+#pragma unroll
       for (int i = 0; i < 2; ++i) {
         if (FP8) {
           const uint2 raw = *reinterpret_cast<const uint2*>(qrow[i] + (ks >> 2) * 64 + t4 * 16 + (ks & 3) * 4);
@@ -135,30 +160,26 @@ __global__ void __launch_bounds__(kPreWarps * 32, 2) decode_prefix_kernel(const 
           qf[ks][2 + i] = real[i] ? *reinterpret_cast<const uint32_t*>(qrow[i] + ks * 16 + 8 + t4 * 2) : 0u;
         }
       }
-
     float o[16][4];
-  #pragma unroll
+#pragma unroll
     for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
 
-    look_up(step_lo);
-    issue(step_lo);
-    issue(step_lo + 1);
-    for (int step = step_lo; step < step_hi; ++step) {
+    for (int step = w.step; step < w.step + w.n; ++step, ++n_out) {
       cp_async_wait<1>();
       __syncthreads();
-      uint8_t* st = smem + ((step - step_lo) % kPreStages) * L::kStage;
-      const int key0 = step * kPreStep * 16, pages = min(kPreStep, n_pages - step * kPreStep);
-      if (pages < kPreStep || key0 + kPreStep * 16 > shared) {
+      uint8_t* st = smem + (n_out % kPreStages) * L::kStage;
+      const int key0 = step * kPrefixKeys;
+      if (key0 + kPrefixKeys > shared) {
         // values (and scales) behind the prefix, whatever they are, meet weights of 0 as zeros; so do pages that were not fetched
         for (int u = 0; u < kPreStep; ++u) {
           uint8_t* vd = st + u * L::kPageSize + L::kHalf;
           const int n = max(0, min(16, shared - key0 - u * 16));
           if (FP8) {
-            uint32_t* w = reinterpret_cast<uint32_t*>(vd + tid * 16);
-  #pragma unroll
+            uint32_t* x = reinterpret_cast<uint32_t*>(vd + tid * 16);
+#pragma unroll
             for (int c = 0; c < 4; ++c)
-              if (n < c * 4 + 4) w[c] = n <= c * 4 ? 0u : w[c] & (0xffffffffu >> (32 - 8 * (n - c * 4)));
+              if (n < c * 4 + 4) x[c] = n <= c * 4 ? 0u : x[c] & (0xffffffffu >> (32 - 8 * (n - c * 4)));
             if (tid < 16 && tid >= n) reinterpret_cast<float*>(vd + L::kHalf)[16 + tid] = 0.f;
           } else {
             for (int i = n * 16 + tid; i < 256; i += kPreWarps * 32) *reinterpret_cast<uint4*>(vd + i * 16) = make_uint4(0, 0, 0, 0);
@@ -166,30 +187,30 @@ __global__ void __launch_bounds__(kPreWarps * 32, 2) decode_prefix_kernel(const 
         }
         __syncthreads();
       }
-      issue(step + 2);
+      issue();                                                       // into the stage that all have left
       if (!busy) continue;
       // ---- S = Q K^T ----
       float s[kPreStep * 2][4];
-  #pragma unroll
+#pragma unroll
       for (int u = 0; u < kPreStep; ++u) {
         const uint32_t kb = smem_u32(st + u * L::kPageSize);
-  #pragma unroll
+#pragma unroll
         for (int j = 0; j < 2; ++j) s[2 * u + j][0] = s[2 * u + j][1] = s[2 * u + j][2] = s[2 * u + j][3] = 0.f;
         if (FP8) {
-  #pragma unroll
+#pragma unroll
           for (int j = 0; j < 2; ++j) {
             const int krow = ((g >> 1) << 2) + 2 * j + (g & 1);
-  #pragma unroll
+#pragma unroll
             for (int h = 0; h < 2; ++h) {
               const uint4 w4 = lds128(kb + krow * 128 + (((4 * h + t4) ^ k_sigma(g)) << 4));
               const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-  #pragma unroll
+#pragma unroll
               for (int i = 0; i < 4; ++i) pre_mma<true>(s[2 * u + j], qf[4 * h + i], e4m3x2_to_f16x2(w[i] & 0xFFFFu), e4m3x2_to_f16x2(w[i] >> 16));
             }
           }
         } else {
           const int mrow = (lane & 7) + (lane >> 4) * 8, mcol = (lane >> 3) & 1;
-  #pragma unroll
+#pragma unroll
           for (int ks = 0; ks < 8; ++ks) {
             uint32_t kf[4];
             pre_ldmatrix_x4(kf, kb + mrow * 256 + (((ks * 2 + mcol) ^ (mrow & 7)) << 4));
@@ -201,7 +222,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 2) decode_prefix_kernel(const 
       // ---- scale, mask, online softmax on rows g and g + 8.  Key of column (u, j, e): bf16 16 u + 8 j + 2 t + e, fp8 16 u + 4 t + 2 j + e ----
       float vsc[kPreStep][4];
       float top[2] = {-INFINITY, -INFINITY};
-  #pragma unroll
+#pragma unroll
       for (int u = 0; u < kPreStep; ++u) {
         float ksc[4] = {1.f, 1.f, 1.f, 1.f};
         if (FP8) {
@@ -210,9 +231,9 @@ __global__ void __launch_bounds__(kPreWarps * 32, 2) decode_prefix_kernel(const 
           ksc[0] = __uint_as_float(kr.x); ksc[1] = __uint_as_float(kr.y); ksc[2] = __uint_as_float(kr.z); ksc[3] = __uint_as_float(kr.w);
           vsc[u][0] = __uint_as_float(vr.x); vsc[u][1] = __uint_as_float(vr.y); vsc[u][2] = __uint_as_float(vr.z); vsc[u][3] = __uint_as_float(vr.w);
         }
-  #pragma unroll
+#pragma unroll
         for (int j = 0; j < 2; ++j)
-  #pragma unroll
+#pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int key = key0 + u * 16 + (FP8 ? t4 * 4 + 2 * j + (e & 1) : j * 8 + t4 * 2 + (e & 1));
             float& x = s[2 * u + j][e];
@@ -221,7 +242,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 2) decode_prefix_kernel(const 
           }
       }
       float m_sub[2], corr[2], sum[2] = {0.f, 0.f};
-  #pragma unroll
+#pragma unroll
       for (int i = 0; i < 2; ++i) {
         top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
         top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
@@ -231,33 +252,33 @@ __global__ void __launch_bounds__(kPreWarps * 32, 2) decode_prefix_kernel(const 
         m_run[i] = m_new;
       }
       uint32_t pa[kPreStep][4];
-  #pragma unroll
+#pragma unroll
       for (int u = 0; u < kPreStep; ++u)
-  #pragma unroll
+#pragma unroll
         for (int j = 0; j < 2; ++j)
-  #pragma unroll
+#pragma unroll
           for (int i = 0; i < 2; ++i) {
             const float p0 = exp2f(s[2 * u + j][2 * i] - m_sub[i]), p1 = exp2f(s[2 * u + j][2 * i + 1] - m_sub[i]);
             sum[i] += p0 + p1;
             pa[u][2 * j + i] = FP8 ? pack_f16x2(p0 * (vsc[u][2 * j] * kPreScale), p1 * (vsc[u][2 * j + 1] * kPreScale)) : pack_bf16x2(p0, p1);
           }
-  #pragma unroll
+#pragma unroll
       for (int i = 0; i < 2; ++i) l_run[i] = l_run[i] * corr[i] + sum[i];
-  #pragma unroll
+#pragma unroll
       for (int i = 0; i < 16; ++i) { o[i][0] *= corr[0]; o[i][1] *= corr[0]; o[i][2] *= corr[1]; o[i][3] *= corr[1]; }
       // ---- O += P V ----
-  #pragma unroll
+#pragma unroll
       for (int u = 0; u < kPreStep; ++u) {
         const uint32_t vb = smem_u32(st + u * L::kPageSize + L::kHalf);
         if (FP8) {
-  #pragma unroll
+#pragma unroll
           for (int nd = 0; nd < 16; ++nd) {
             const uint32_t w = lds32(vb + (nd * 8 + g) * 16 + t4 * 4);
             pre_mma<true>(o[nd], pa[u], e4m3x2_to_f16x2(w & 0xFFFFu), e4m3x2_to_f16x2(w >> 16));
           }
         } else {
           const int mrow = (lane & 7) + ((lane >> 3) & 1) * 8, mcol = lane >> 4;
-  #pragma unroll
+#pragma unroll
           for (int nd = 0; nd < 8; ++nd) {
             uint32_t vf[4];
             pre_ldmatrix_x4_trans(vf, vb + mrow * 256 + (((nd * 2 + mcol) ^ (mrow & 7)) << 4));
@@ -267,60 +288,36 @@ __global__ void __launch_bounds__(kPreWarps * 32, 2) decode_prefix_kernel(const 
         }
       }
     }
-    cp_async_wait<0>();
     // ---- the part of every row; one without keys is (-inf, 0, 0) ----
-  #pragma unroll
+#pragma unroll
     for (int i = 0; i < 2; ++i) {
       l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 1);
       l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 2);
       if (!real[i]) continue;
-      const long base = row[i] + part * 8;
-      float* dst = p.part_o + base * 128 + t4 * 2;
-  #pragma unroll
+      const long at = prefix_part_row(p, w.first, w.h, w.rows, w.tile * kPrefixRows + warp * 16 + g + i * 8) + static_cast<long>(kPrefixRows) * blockIdx.x;
+      float* dst = p.prefix_o + at * 128 + t4 * 2;
+#pragma unroll
       for (int nd = 0; nd < 16; ++nd)
         *reinterpret_cast<float2*>(dst + nd * 8) = make_float2(o[nd][2 * i] * (FP8 ? 1.f / kPreScale : 1.f), o[nd][2 * i + 1] * (FP8 ? 1.f / kPreScale : 1.f));
-      if (t4 == 0) *reinterpret_cast<float2*>(p.part_ml + base * 2) = make_float2(m_run[i], l_run[i]);
+      if (t4 == 0) *reinterpret_cast<float2*>(p.prefix_ml + at * 2) = make_float2(m_run[i], l_run[i]);
     }
-    __syncthreads();                                                 // the next tile's copies go where this one's were read
   }
+  cp_async_wait<0>();
 }
 
 namespace {
 
 template <bool FP8>
-cudaError_t launch_prefix(const PrefixParams& p, dim3 grid, cudaStream_t s) {
+cudaError_t launch_prefix(const FlatParams& p, cudaStream_t s) {
   static PerDevice<bool> configured;
   const cudaError_t e = allow_smem(configured, decode_prefix_kernel<FP8>, PreSmem<FP8>::kTotal);
   if (e != cudaSuccess) return e;
-  launch_dependent(decode_prefix_kernel<FP8>, grid, kPreWarps * 32, PreSmem<FP8>::kTotal, s, p);
+  launch_dependent(decode_prefix_kernel<FP8>, p.prefix_runs, kPreWarps * 32, PreSmem<FP8>::kTotal, s, p);
   return cudaGetLastError();
 }
 
 }  // namespace
+
+cudaError_t launch_decode_prefix(const FlatParams& p, cudaStream_t s) { return p.ks != nullptr ? launch_prefix<true>(p, s) : launch_prefix<false>(p, s); }
+
 }  // namespace nrl
-
-using namespace nrl;
-
-extern "C" int nrl_decode_prefix_parts(int n_groups, int max_group, int Hq, int Hkv, int max_blocks, int num_sms) {
-  const long blocks = static_cast<long>(n_groups) * Hkv * ((static_cast<long>(max_group) * (Hq / Hkv) + kPreRows - 1) / kPreRows);
-  const long want = blocks > 0 ? (2L * num_sms + blocks - 1) / blocks : 1, steps = (max_blocks + kPreStep - 1) / kPreStep;
-  return static_cast<int>(want < 1 ? 1 : want > 16 ? (steps < 16 ? steps : 16) : (want < steps ? want : steps < 1 ? 1 : steps));
-}
-
-extern "C" cudaError_t nrl_decode_prefix(const DecodeCall* c, const int* cu_groups, const int* shared, int n_groups, int max_group, int prefix_parts, float* prefix_o,
-                                         float* prefix_ml, cudaStream_t s) {
-  PrefixParams p;
-  p.q = static_cast<const __nv_bfloat16*>(c->q);
-  p.k = static_cast<const uint8_t*>(c->k_cache);
-  p.v = static_cast<const uint8_t*>(c->v_cache);
-  p.ks = c->k_scale; p.vs = c->v_scale;
-  p.block_tables = c->block_tables; p.context_lens = c->context_lens; p.cu_groups = cu_groups; p.shared = shared;
-  p.part_o = prefix_o; p.part_ml = prefix_ml;
-  p.q_stride_s = c->q_stride_s;
-  p.S = c->S; p.max_blocks = c->max_blocks; p.Hkv = c->Hkv; p.G = c->Hq / c->Hkv;
-  p.prefix_parts = prefix_parts;
-  p.tiles = (max_group * p.G + kPreRows - 1) / kPreRows;
-  p.scale_log2 = c->scale * 1.4426950408889634f;
-  const dim3 grid(n_groups, c->Hkv, prefix_parts * p.tiles);
-  return c->k_scale != nullptr ? launch_prefix<true>(p, grid, s) : launch_prefix<false>(p, grid, s);
-}

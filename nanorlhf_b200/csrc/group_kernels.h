@@ -19,14 +19,11 @@ struct DecodeCall {
 }  // namespace nrl
 
 extern "C" {
-// parts that the prefix of a group is cut into
-int nrl_decode_prefix_parts(int n_groups, int max_group, int Hq, int Hkv, int max_blocks, int num_sms);
-// the prefixes' parts alone: prefix_o [S, Hkv, prefix_parts, 8, D], prefix_ml [S, Hkv, prefix_parts, 8, 2]
-cudaError_t nrl_decode_prefix(const nrl::DecodeCall* c, const int* cu_groups, const int* shared, int n_groups, int max_group, int prefix_parts, float* prefix_o,
-                              float* prefix_ml, cudaStream_t s);
-size_t nrl_decode_flat_scratch(const nrl::DecodeCall* c, int num_sms);       // bytes of `scratch` below, on 16, for one call at a time
-cudaError_t nrl_paged_decode_shared(const nrl::DecodeCall* c, const int* cu_groups, const int* shared, int n_groups, int max_group, int prefix_parts, float* prefix_o,
-                                    float* prefix_ml, void* scratch, int num_sms, cudaStream_t s);
+// bytes of `scratch` below, on 64, for one call at a time (scored: no groups)
+size_t nrl_decode_scratch(const nrl::DecodeCall* c, int n_groups, int max_group, int num_sms);
+// max_group: rows of a group at most; it bounds how many blocks the prefixes get, not what they do
+cudaError_t nrl_paged_decode_shared(const nrl::DecodeCall* c, const int* cu_groups, const int* shared, int n_groups, int max_group, void* scratch, int num_sms,
+                                    cudaStream_t s);
 // scores_in, scores_out [S, Hkv, max_tokens], rows and heads their strides apart (they may be the same memory); raw: [S, Hkv, G, 16 max_blocks] floats of scratch
 cudaError_t nrl_paged_decode_scored(const nrl::DecodeCall* c, const float* scores_in, long in_row, long in_head, float* scores_out, long out_row, long out_head,
                                     int max_tokens, float decay, float* raw, void* scratch, int num_sms, cudaStream_t s);

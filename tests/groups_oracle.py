@@ -76,7 +76,7 @@ def decode_row(q, k, v, scale, fp8):
         return torch.zeros(q.shape[0] * q.shape[1], q.shape[2], dtype=torch.float64, device=q.device), 0.0, q.new_zeros(k.shape[0], 0), q.new_zeros(k.shape[0], 0)
     p = torch.softmax(q @ k.transpose(1, 2) * scale, -1)
     o, a = p @ v, p @ v.abs()
-    # weights in bf16; or, times the values' scales and 2^10, in f16, whose steps are 2^-24 where it is denormal
-    bound = (F16 + F32) * a + BF16 * o.abs() + n * 2.0 ** -25 * 448.0 / 1024.0 if fp8 else (BF16 + F32) * (a + o.abs())
+    # weights in bf16; or, times the values' scales and at least 2^8, in f16, whose steps are 2^-24 where it is denormal
+    bound = (F16 + F32) * a + BF16 * o.abs() + n * 2.0 ** -25 * 448.0 / 256.0 if fp8 else (BF16 + F32) * (a + o.abs())
     worst = (q.abs() @ k.abs().transpose(1, 2)).amax() * scale * 128 * 2.0 ** -24 * 2 + 2.0 ** -20
     return o.flatten(0, 1), bound.flatten(0, 1), p.sum(1), p.sum(1) * worst

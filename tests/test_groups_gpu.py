@@ -237,12 +237,22 @@ BATCHES = {
 }
 
 
+def widen(st):
+    """Page tables of 50 MB of pages and more: prefixes are attended to for all rows of a group, instead of by each row."""
+    S, width = st["tables"].shape
+    more = 50_000_000 // (S * st["k"].shape[1] * 4096) + 1
+    st["tables"] = torch.cat([st["tables"], torch.full((S, more), st["k"].shape[0] - 1, dtype=torch.int32, device=DEV)], 1)
+
+
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("heads,kv", [(12, 2), (7, 1), (16, 2), (4, 4)])
 @pytest.mark.parametrize("name", list(BATCHES))
-def test_decode_over_shared_pages(name, heads, kv, fp8):
+def test_decode_over_shared_pages(name, heads, kv, fp8, wide):
     groups = BATCHES[name]
     st = shared_batch(11, groups, kv, fp8)
+    if wide:
+        widen(st)
     S = st["context"].numel()
     q = torch.randn(S, heads + 3, 128, generator=gen(12), device=DEV).to(torch.bfloat16)[:, :heads]
     kw = {"k_scale": st["ks"], "v_scale": st["vs"]}
@@ -261,9 +271,13 @@ def test_decode_over_shared_pages(name, heads, kv, fp8):
             row += 1
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("fp8", [False, True])
-def test_rows_of_no_group_are_plain(fp8):
+def test_rows_of_no_group_are_plain(fp8, wide):
+    """... and so are those of groups that do not follow one another."""
     st = shared_batch(13, [(48, [100, 77]), (0, [130, 5, 64])], 2, fp8)
+    if wide:
+        widen(st)
     q = torch.randn(5, 12, 128, generator=gen(14), device=DEV).to(torch.bfloat16)
     args = (q, st["k"], st["v"], st["tables"], st["context"])
     a = ops.paged_decode_shared(*args, st["cu"][:2].contiguous(), st["shared"][:1].contiguous(), max_group=2, k_scale=st["ks"], v_scale=st["vs"])
@@ -271,15 +285,42 @@ def test_rows_of_no_group_are_plain(fp8):
     assert torch.equal(a[2:], b[2:])
     none = torch.zeros(1, dtype=torch.int32, device=DEV)
     c = ops.paged_decode_shared(*args, none, none[:0], k_scale=st["ks"], v_scale=st["vs"])
-    assert torch.equal(a[2:], c[2:])
+    d = ops.paged_decode_shared(*args, torch.tensor([-3, 7, 2], dtype=torch.int32, device=DEV), torch.tensor([48, 48], dtype=torch.int32, device=DEV), k_scale=st["ks"],
+                                v_scale=st["vs"])
+    assert torch.equal(a[2:], c[2:]) and torch.equal(c, d)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_many_groups_and_long_prefixes(fp8):
+    """More groups and rows than decode_plan has threads, runs that meet several tiles, groups of more than one tile of query rows."""
+    few = [(300 + 16 * i, [320 + 16 * i + j for j in range(33)]) for i in range(3)] + [(1500, [1501 + j for j in range(70)])]
+    many = [(16 * (i % 5), [16 * (i % 5) + 1 + i % 3] * (1 + i % 2)) for i in range(1100)]
+    for seed, groups in ((70, few), (71, many)):
+        st = shared_batch(seed, groups, 2, fp8)
+        widen(st)
+        S = st["context"].numel()
+        q = torch.randn(S, 12, 128, generator=gen(seed), device=DEV).to(torch.bfloat16)
+        out = ops.paged_decode_shared(q, st["k"], st["v"], st["tables"], st["context"], st["cu"], st["shared"], max_group=70, k_scale=st["ks"], v_scale=st["vs"])
+        row = 0
+        for i, (shared, ctxs) in enumerate(groups):
+            first = row
+            for c in ctxs:
+                if len(groups) < 10 or i % 37 < 2:
+                    n = min(shared, c)
+                    parts = zip(oracle.page_rows(st, st["tables"][first], n), (x[:, n:] for x in oracle.page_rows(st, st["tables"][row], c)))
+                    want, bound, _, _ = oracle.decode_row(q[row], *(torch.cat(x, 1) for x in parts), SCALE, fp8)
+                    within(out[row], want, bound, f"row {row}")
+                row += 1
 
 
 @pytest.mark.parametrize("fp8", [False, True])
 def test_decode_over_shared_pages_in_two_graphs(fp8):
     """Two captured calls of other batches, replayed in turn and with other inputs."""
     calls = []
-    for seed, name in ((15, "a few"), (16, "many rows")):
+    for seed, name in ((15, "a few"), (16, "many rows"), (19, "long")):
         st = shared_batch(seed, BATCHES[name], 2, fp8)
+        if seed > 15:
+            widen(st)
         q = torch.randn(st["context"].numel(), 12, 128, generator=gen(seed), device=DEV).to(torch.bfloat16)
         f = lambda st=st, q=q: ops.paged_decode_shared(q, st["k"], st["v"], st["tables"], st["context"], st["cu"], st["shared"], max_group=37, k_scale=st["ks"],  # noqa: E731
                                                        v_scale=st["vs"])
