@@ -274,6 +274,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> kv_evict(torch::Tensor k
     to = out_tables->contiguous();
   }
   TORCH_CHECK_VALUE(k.size(0) * Hkv * 16 <= kIntMax && (std::min<int64_t>(keep, c.max_tokens) + 511) / 512 * Hkv <= 65535 && S <= kIntMax / 8, what, ": too many tokens");
+  TORCH_CHECK_VALUE(c.max_tokens <= 8 * 48 * 1024, what, ": scores and tables of at most 393 216 tokens a row, got ", c.max_tokens);
   torch::Tensor kept = torch::empty({S, Hkv, keep}, tables.options()), kept_scores = torch::empty({S, Hkv, keep}, scores.options());
   torch::Tensor lens = torch::empty({S}, tables.options());
   const torch::Tensor bits = torch::empty({S, Hkv, (c.max_tokens + 31) / 32}, tables.options());

@@ -200,242 +200,245 @@ __global__ void __launch_bounds__(kFlatWarps * 32, FlatSizes<FP8>::kBlocks) deco
   using Z = FlatSizes<FP8>;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-  const int w = blockIdx.x * kFlatWarps + warp, run = p.rows[p.S].z;
-  const int count = w < p.runs ? max(0, min(run, p.rows[p.S].y * p.Hkv - w * run)) : 0;
-  if (count == 0) {
-    if (beside) pdl_wait();
-    return;
-  }
-  FlatAt here, ahead;
-  {
-    const int4 start = p.starts[w];
-    flat_row<!SCORES>(p, here, start.x);
-    here.h = start.y;
-    here.page = start.z;
-    ahead = here;
-  }
-  uint8_t* ring = smem + warp * Z::kStages * Z::kStage;
-
-  // page numbers wait in the lanes, 32 of a row-head at a time
-  int ids = 0, ids_from = -1, issued = 0;
-  auto issue = [&]() {
-    if (issued < count) {
-      if (ids_from < 0 || ahead.page - ids_from >= 32) {
-        ids_from = ahead.page;
-        ids = ids_from + lane < ahead.pages ? p.block_tables[flat_entry(p, ahead, ids_from + lane)] : 0;
-      }
-      const long pg = static_cast<long>(__shfl_sync(0xffffffffu, ids, ahead.page - ids_from)) * p.Hkv + ahead.h;
-      uint8_t *kd = ring + (issued % Z::kStages) * Z::kStage, *vd = kd + Z::kHalf;
-      const uint8_t *ksrc = p.k + pg * Z::kHalf, *vsrc = p.v + pg * Z::kHalf;
-      if (FP8) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int chunk = lane + j * 32, r = chunk >> 3, c = chunk & 7;
-          cp_async_16(kd + r * 128 + ((c ^ k_sigma(r)) << 4), ksrc + chunk * 16);
-          cp_async_16(vd + chunk * 16, vsrc + chunk * 16);
-        }
-        if (lane < 8) cp_async_16(vd + Z::kHalf + lane * 16, (lane < 4 ? p.ks : p.vs) + pg * 16 + (lane & 3) * 4);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int chunk = lane + j * 32, at = (chunk >> 4) * 256 + (((chunk & 15) ^ ((chunk >> 4) & 7)) << 4);
-          cp_async_16(kd + at, ksrc + chunk * 16);
-          cp_async_16(vd + at, vsrc + chunk * 16);
-        }
-      }
-      if (++issued < count && flat_next<!SCORES>(p, ahead)) ids_from = -1;
+  const int run = p.rows[p.S].z, all = p.rows[p.S].y * p.Hkv;
+  // The next run that nobody has: blocks that find no room beside decode_prefix's begin late.
+  for (;;) {
+    int w = 0;
+    if (lane == 0) w = atomicAdd(&p.rows[p.S].w, 1);
+    w = __shfl_sync(0xffffffffu, w, 0);
+    const int count = w < p.runs ? min(run, all - w * run) : 0;
+    if (count <= 0) break;
+    FlatAt here, ahead;
+    {
+      const int4 start = p.starts[w];
+      flat_row<!SCORES>(p, here, start.x);
+      here.h = start.y;
+      here.page = start.z;
+      ahead = here;
     }
-    cp_async_commit();
-  };
+    uint8_t* ring = smem + warp * Z::kStages * Z::kStage;
+
+    // page numbers wait in the lanes, 32 of a row-head at a time
+    int ids = 0, ids_from = -1, issued = 0;
+    auto issue = [&]() {
+      if (issued < count) {
+        if (ids_from < 0 || ahead.page - ids_from >= 32) {
+          ids_from = ahead.page;
+          ids = ids_from + lane < ahead.pages ? p.block_tables[flat_entry(p, ahead, ids_from + lane)] : 0;
+        }
+        const long pg = static_cast<long>(__shfl_sync(0xffffffffu, ids, ahead.page - ids_from)) * p.Hkv + ahead.h;
+        uint8_t *kd = ring + (issued % Z::kStages) * Z::kStage, *vd = kd + Z::kHalf;
+        const uint8_t *ksrc = p.k + pg * Z::kHalf, *vsrc = p.v + pg * Z::kHalf;
+        if (FP8) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int chunk = lane + j * 32, r = chunk >> 3, c = chunk & 7;
+            cp_async_16(kd + r * 128 + ((c ^ k_sigma(r)) << 4), ksrc + chunk * 16);
+            cp_async_16(vd + chunk * 16, vsrc + chunk * 16);
+          }
+          if (lane < 8) cp_async_16(vd + Z::kHalf + lane * 16, (lane < 4 ? p.ks : p.vs) + pg * 16 + (lane & 3) * 4);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int chunk = lane + j * 32, at = (chunk >> 4) * 256 + (((chunk & 15) ^ ((chunk >> 4) & 7)) << 4);
+            cp_async_16(kd + at, ksrc + chunk * 16);
+            cp_async_16(vd + at, vsrc + chunk * 16);
+          }
+        }
+        if (++issued < count && flat_next<!SCORES>(p, ahead)) ids_from = -1;
+      }
+      cp_async_commit();
+    };
 #pragma unroll 1
-  for (int i = 0; i < (FP8 ? Z::kStages : Z::kStages - 1); ++i) issue();
+    for (int i = 0; i < (FP8 ? Z::kStages : Z::kStages - 1); ++i) issue();
 
-  uint32_t qa0[8], qa2[8];                                           // row g: query head g of the kv head
-  float o[16][4];
-  float m_run = 0.f, l_run = 0.f;
-  auto enter = [&]() {                                               // a row-head's queries, nothing seen
-    const bool real = g < p.G;
-    const __nv_bfloat16* qrow = p.q + here.s * p.q_stride_s + (here.h * p.G + (real ? g : 0)) * kFlatD;
+    uint32_t qa0[8], qa2[8];                                           // row g: query head g of the kv head
+    float o[16][4];
+    float m_run = 0.f, l_run = 0.f;
+    auto enter = [&]() {                                               // a row-head's queries, nothing seen
+      const bool real = g < p.G;
+      const __nv_bfloat16* qrow = p.q + here.s * p.q_stride_s + (here.h * p.G + (real ? g : 0)) * kFlatD;
 #pragma unroll
-    for (int ks = 0; ks < 8; ++ks) {
-      if (FP8) {
-        const uint2 x = *reinterpret_cast<const uint2*>(qrow + (ks >> 2) * 64 + t4 * 16 + (ks & 3) * 4);
-        const float2 a = unpack_bf16x2(x.x), b = unpack_bf16x2(x.y);
-        qa0[ks] = real ? pack_f16x2(a.x, a.y) : 0u;
-        qa2[ks] = real ? pack_f16x2(b.x, b.y) : 0u;
-      } else {
-        qa0[ks] = real ? *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + t4 * 2) : 0u;
-        qa2[ks] = real ? *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + 8 + t4 * 2) : 0u;
+      for (int ks = 0; ks < 8; ++ks) {
+        if (FP8) {
+          const uint2 x = *reinterpret_cast<const uint2*>(qrow + (ks >> 2) * 64 + t4 * 16 + (ks & 3) * 4);
+          const float2 a = unpack_bf16x2(x.x), b = unpack_bf16x2(x.y);
+          qa0[ks] = real ? pack_f16x2(a.x, a.y) : 0u;
+          qa2[ks] = real ? pack_f16x2(b.x, b.y) : 0u;
+        } else {
+          qa0[ks] = real ? *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + t4 * 2) : 0u;
+          qa2[ks] = real ? *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + 8 + t4 * 2) : 0u;
+        }
       }
-    }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    m_run = -INFINITY;
-    l_run = 0.f;
-  };
-  auto leave = [&]() {                                               // its part
-    float l = l_run;
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-    if (g < p.G) {
-      const long part = (static_cast<long>(w) + static_cast<long>(here.s) * p.Hkv + here.h) * 8 + g;
-      float* dst = p.part_o + part * kFlatD + t4 * 2;
+      for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+      m_run = -INFINITY;
+      l_run = 0.f;
+    };
+    auto leave = [&]() {                                               // its part
+      float l = l_run;
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      if (g < p.G) {
+        const long part = (static_cast<long>(w) + static_cast<long>(here.s) * p.Hkv + here.h) * 8 + g;
+        float* dst = p.part_o + part * kFlatD + t4 * 2;
 #pragma unroll
-      for (int nd = 0; nd < 16; ++nd)
-        *reinterpret_cast<float2*>(dst + nd * 8) = make_float2(o[nd][0] * (FP8 ? 1.f / kFlatScale : 1.f), o[nd][1] * (FP8 ? 1.f / kFlatScale : 1.f));
-      if (t4 == 0) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(m_run, l);
-    }
-  };
+        for (int nd = 0; nd < 16; ++nd)
+          *reinterpret_cast<float2*>(dst + nd * 8) = make_float2(o[nd][0] * (FP8 ? 1.f / kFlatScale : 1.f), o[nd][1] * (FP8 ? 1.f / kFlatScale : 1.f));
+        if (t4 == 0) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(m_run, l);
+      }
+    };
 
-  auto step = [&](auto number, int it) {                             // pages it and, of two, it + 1 of the run, both of this row-head: one rescaling of O
-    constexpr int U = decltype(number)::value;
-    cp_async_wait<FP8 ? Z::kStages - U : Z::kStages - 1>();
-    __syncwarp();
-    float s[U][2][4], vscale[U][4];
-    float top = -INFINITY;
+    auto step = [&](auto number, int it) {                             // pages it and, of two, it + 1 of the run, both of this row-head: one rescaling of O
+      constexpr int U = decltype(number)::value;
+      cp_async_wait<FP8 ? Z::kStages - U : Z::kStages - 1>();
+      __syncwarp();
+      float s[U][2][4], vscale[U][4];
+      float top = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      uint8_t* st = ring + ((it + u) % Z::kStages) * Z::kStage;
-      const uint32_t kb = smem_u32(st);
-      const int page = here.page + u;
-      const bool lead = !SCORES && page < here.lead;
-      const int tok0 = lead ? page * 16 : (here.first / 16 + page - here.lead) * 16;
+      for (int u = 0; u < U; ++u) {
+        uint8_t* st = ring + ((it + u) % Z::kStages) * Z::kStage;
+        const uint32_t kb = smem_u32(st);
+        const int page = here.page + u;
+        const bool lead = !SCORES && page < here.lead;
+        const int tok0 = lead ? page * 16 : (here.first / 16 + page - here.lead) * 16;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) s[u][j][0] = s[u][j][1] = s[u][j][2] = s[u][j][3] = 0.f;
-      // ---- S = Q K^T.  Key of column (j, e): bf16 8 j + 2 t + e, fp8 4 t + 2 j + e ----
-      if constexpr (FP8) {
+        for (int j = 0; j < 2; ++j) s[u][j][0] = s[u][j][1] = s[u][j][2] = s[u][j][3] = 0.f;
+        // ---- S = Q K^T.  Key of column (j, e): bf16 8 j + 2 t + e, fp8 4 t + 2 j + e ----
+        if constexpr (FP8) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int krow = ((g >> 1) << 2) + 2 * j + (g & 1);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint4 w4 = lds128(kb + krow * 128 + (((4 * h + t4) ^ k_sigma(g)) << 4));
+              const uint32_t x[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                mma_f16_16816(s[u][j], qa0[4 * h + i], qa2[4 * h + i], e4m3x2_to_f16x2(x[i] & 0xFFFFu), e4m3x2_to_f16x2(x[i] >> 16));
+            }
+          }
+          const uint4 kr = lds128(kb + 2 * Z::kHalf + t4 * 16), vr = lds128(kb + 2 * Z::kHalf + 64 + t4 * 16);
+          const float kscale[4] = {__uint_as_float(kr.x), __uint_as_float(kr.y), __uint_as_float(kr.z), __uint_as_float(kr.w)};
+          vscale[u][0] = __uint_as_float(vr.x); vscale[u][1] = __uint_as_float(vr.y); vscale[u][2] = __uint_as_float(vr.z); vscale[u][3] = __uint_as_float(vr.w);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) s[u][j][e] *= kscale[2 * j + e] * p.scale_log2;
+        } else {
+          const int mrow = (lane & 7) + (lane >> 4) * 8, mcol = (lane >> 3) & 1;
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks) {
+            uint32_t kf[4];
+            flat_ldmatrix_x4(kf, kb + mrow * 256 + (((ks * 2 + mcol) ^ (mrow & 7)) << 4));
+            flat_mma_bf16(s[u][0], qa0[ks], qa2[ks], kf[0], kf[1]);
+            flat_mma_bf16(s[u][1], qa0[ks], qa2[ks], kf[2], kf[3]);
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) s[u][j][e] *= p.scale_log2;
+        }
+        // ---- mask; values and scales outside the row's own tokens, whatever they are, meet weights of 0 as zeros ----
+        const int lo = lead ? 0 : here.first - tok0, hi = (lead ? here.first : here.ctx) - tok0;
+        if (lo > 0 || hi < 16) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int t = FP8 ? t4 * 4 + 2 * j + e : j * 8 + t4 * 2 + e;
+              if (t < lo || t >= hi) s[u][j][e] = -INFINITY;
+              if (FP8 && (t < lo || t >= hi)) vscale[u][2 * j + e] = 0.f;
+            }
+          if (FP8) {
+            fp8_clear_values(st + Z::kHalf, lo, hi, lane);
+          } else {
+            for (int i = lane; i < 256; i += 32)
+              if ((i >> 4) < lo || (i >> 4) >= hi) *reinterpret_cast<uint4*>(st + Z::kHalf + i * 16) = make_uint4(0, 0, 0, 0);
+            __syncwarp();
+          }
+        }
+        if (SCORES && g < p.G) {
+          float* raw = p.raw + ((static_cast<long>(here.s) * p.Hkv + here.h) * p.G + g) * (16L * p.max_blocks) + tok0;
+          if (FP8) {
+            *reinterpret_cast<float4*>(raw + t4 * 4) = make_float4(s[u][0][0], s[u][0][1], s[u][1][0], s[u][1][1]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) *reinterpret_cast<float2*>(raw + j * 8 + t4 * 2) = make_float2(s[u][j][0], s[u][j][1]);
+          }
+        }
+        top = fmaxf(top, fmaxf(fmaxf(s[u][0][0], s[u][0][1]), fmaxf(s[u][1][0], s[u][1][1])));
+      }
+      // ---- online softmax on row g ----
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const float m_new = fmaxf(m_run, top), m_sub = m_new == -INFINITY ? 0.f : m_new;
+      const float corr = exp2f(m_run - m_sub);                         // 0 while nothing has been seen
+      uint32_t pa[U][2];
+      float sum = 0.f;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const int krow = ((g >> 1) << 2) + 2 * j + (g & 1);
+          const float p0 = exp2f(s[u][j][0] - m_sub), p1 = exp2f(s[u][j][1] - m_sub);
+          sum += p0 + p1;
+          pa[u][j] = FP8 ? pack_f16x2(p0 * (vscale[u][2 * j] * kFlatScale), p1 * (vscale[u][2 * j + 1] * kFlatScale)) : pack_bf16x2(p0, p1);
+        }
+      l_run = l_run * corr + sum;
+      m_run = m_new;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint4 w4 = lds128(kb + krow * 128 + (((4 * h + t4) ^ k_sigma(g)) << 4));
-            const uint32_t x[4] = {w4.x, w4.y, w4.z, w4.w};
+      for (int i = 0; i < 16; ++i) { o[i][0] *= corr; o[i][1] *= corr; }
+      // ---- O += P V ----
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              mma_f16_16816(s[u][j], qa0[4 * h + i], qa2[4 * h + i], e4m3x2_to_f16x2(x[i] & 0xFFFFu), e4m3x2_to_f16x2(x[i] >> 16));
+      for (int u = 0; u < U; ++u) {
+        const uint32_t vb = smem_u32(ring + ((it + u) % Z::kStages) * Z::kStage) + Z::kHalf;
+        if constexpr (FP8) {
+#pragma unroll
+          for (int nd = 0; nd < 16; ++nd) {
+            const uint32_t x = lds32(vb + (nd * 8 + g) * 16 + t4 * 4);
+            mma_f16_16816(o[nd], pa[u][0], pa[u][1], e4m3x2_to_f16x2(x & 0xFFFFu), e4m3x2_to_f16x2(x >> 16));
+          }
+        } else {
+          const int mrow = (lane & 7) + ((lane >> 3) & 1) * 8, mcol = lane >> 4;
+#pragma unroll
+          for (int nd = 0; nd < 8; ++nd) {
+            uint32_t vf[4];
+            flat_ldmatrix_x4_trans(vf, vb + mrow * 256 + (((nd * 2 + mcol) ^ (mrow & 7)) << 4));
+            flat_mma_bf16(o[nd * 2], pa[u][0], pa[u][1], vf[0], vf[1]);
+            flat_mma_bf16(o[nd * 2 + 1], pa[u][0], pa[u][1], vf[2], vf[3]);
           }
         }
-        const uint4 kr = lds128(kb + 2 * Z::kHalf + t4 * 16), vr = lds128(kb + 2 * Z::kHalf + 64 + t4 * 16);
-        const float kscale[4] = {__uint_as_float(kr.x), __uint_as_float(kr.y), __uint_as_float(kr.z), __uint_as_float(kr.w)};
-        vscale[u][0] = __uint_as_float(vr.x); vscale[u][1] = __uint_as_float(vr.y); vscale[u][2] = __uint_as_float(vr.z); vscale[u][3] = __uint_as_float(vr.w);
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) s[u][j][e] *= kscale[2 * j + e] * p.scale_log2;
-      } else {
-        const int mrow = (lane & 7) + (lane >> 4) * 8, mcol = (lane >> 3) & 1;
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-          uint32_t kf[4];
-          flat_ldmatrix_x4(kf, kb + mrow * 256 + (((ks * 2 + mcol) ^ (mrow & 7)) << 4));
-          flat_mma_bf16(s[u][0], qa0[ks], qa2[ks], kf[0], kf[1]);
-          flat_mma_bf16(s[u][1], qa0[ks], qa2[ks], kf[2], kf[3]);
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) s[u][j][e] *= p.scale_log2;
       }
-      // ---- mask; values and scales outside the row's own tokens, whatever they are, meet weights of 0 as zeros ----
-      const int lo = lead ? 0 : here.first - tok0, hi = (lead ? here.first : here.ctx) - tok0;
-      if (lo > 0 || hi < 16) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int t = FP8 ? t4 * 4 + 2 * j + e : j * 8 + t4 * 2 + e;
-            if (t < lo || t >= hi) s[u][j][e] = -INFINITY;
-            if (FP8 && (t < lo || t >= hi)) vscale[u][2 * j + e] = 0.f;
-          }
-        if (FP8) {
-          fp8_clear_values(st + Z::kHalf, lo, hi, lane);
-        } else {
-          for (int i = lane; i < 256; i += 32)
-            if ((i >> 4) < lo || (i >> 4) >= hi) *reinterpret_cast<uint4*>(st + Z::kHalf + i * 16) = make_uint4(0, 0, 0, 0);
-          __syncwarp();
-        }
-      }
-      if (SCORES && g < p.G) {
-        float* raw = p.raw + ((static_cast<long>(here.s) * p.Hkv + here.h) * p.G + g) * (16L * p.max_blocks) + tok0;
-        if (FP8) {
-          *reinterpret_cast<float4*>(raw + t4 * 4) = make_float4(s[u][0][0], s[u][0][1], s[u][1][0], s[u][1][1]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) *reinterpret_cast<float2*>(raw + j * 8 + t4 * 2) = make_float2(s[u][j][0], s[u][j][1]);
-        }
-      }
-      top = fmaxf(top, fmaxf(fmaxf(s[u][0][0], s[u][0][1]), fmaxf(s[u][1][0], s[u][1][1])));
-    }
-    // ---- online softmax on row g ----
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const float m_new = fmaxf(m_run, top), m_sub = m_new == -INFINITY ? 0.f : m_new;
-    const float corr = exp2f(m_run - m_sub);                         // 0 while nothing has been seen
-    uint32_t pa[U][2];
-    float sum = 0.f;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float p0 = exp2f(s[u][j][0] - m_sub), p1 = exp2f(s[u][j][1] - m_sub);
-        sum += p0 + p1;
-        pa[u][j] = FP8 ? pack_f16x2(p0 * (vscale[u][2 * j] * kFlatScale), p1 * (vscale[u][2 * j + 1] * kFlatScale)) : pack_bf16x2(p0, p1);
-      }
-    l_run = l_run * corr + sum;
-    m_run = m_new;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) { o[i][0] *= corr; o[i][1] *= corr; }
-    // ---- O += P V ----
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint32_t vb = smem_u32(ring + ((it + u) % Z::kStages) * Z::kStage) + Z::kHalf;
-      if constexpr (FP8) {
-#pragma unroll
-        for (int nd = 0; nd < 16; ++nd) {
-          const uint32_t x = lds32(vb + (nd * 8 + g) * 16 + t4 * 4);
-          mma_f16_16816(o[nd], pa[u][0], pa[u][1], e4m3x2_to_f16x2(x & 0xFFFFu), e4m3x2_to_f16x2(x >> 16));
-        }
-      } else {
-        const int mrow = (lane & 7) + ((lane >> 3) & 1) * 8, mcol = lane >> 4;
-#pragma unroll
-        for (int nd = 0; nd < 8; ++nd) {
-          uint32_t vf[4];
-          flat_ldmatrix_x4_trans(vf, vb + mrow * 256 + (((nd * 2 + mcol) ^ (mrow & 7)) << 4));
-          flat_mma_bf16(o[nd * 2], pa[u][0], pa[u][1], vf[0], vf[1]);
-          flat_mma_bf16(o[nd * 2 + 1], pa[u][0], pa[u][1], vf[2], vf[3]);
-        }
-      }
-    }
-    __syncwarp();
-  };
+      __syncwarp();
+    };
 
-  enter();
-  for (int it = 0; it < count;) {
-    const bool two = FP8 && it + 1 < count && here.page + 1 < here.pages;
-    if constexpr (FP8) {
-      if (two) step(std::integral_constant<int, 2>{}, it);
-      else step(std::integral_constant<int, 1>{}, it);
+    enter();
+    for (int it = 0; it < count;) {
+      const bool two = FP8 && it + 1 < count && here.page + 1 < here.pages;
+      if constexpr (FP8) {
+        if (two) step(std::integral_constant<int, 2>{}, it);
+        else step(std::integral_constant<int, 1>{}, it);
 #pragma unroll 1
-      for (int u = 0; u < (two ? 2 : 1); ++u) issue();
-    } else {
-      issue();
-      step(std::integral_constant<int, 1>{}, it);
+        for (int u = 0; u < (two ? 2 : 1); ++u) issue();
+      } else {
+        issue();
+        step(std::integral_constant<int, 1>{}, it);
+      }
+      it += two ? 2 : 1;
+      if (two) ++here.page;
+      if (it == count) break;
+      const FlatAt last = here;
+      if (flat_next<!SCORES>(p, here)) {
+        const FlatAt now = here;
+        here = last;
+        leave();
+        here = now;
+        enter();
+      }
     }
-    it += two ? 2 : 1;
-    if (two) ++here.page;
-    if (it == count) break;
-    const FlatAt last = here;
-    if (flat_next<!SCORES>(p, here)) {
-      const FlatAt now = here;
-      here = last;
-      leave();
-      here = now;
-      enter();
-    }
+    leave();
+    cp_async_wait<0>();
   }
-  leave();
-  cp_async_wait<0>();
   if (beside) pdl_wait();
 }
 
@@ -569,7 +572,7 @@ cudaError_t launch_flat(const FlatParams& p, cudaStream_t s) {
   static PerDevice<bool> configured;
   const cudaError_t e = allow_smem(configured, decode_flat_kernel<FP8, SCORES>, FlatSizes<FP8>::kTotal);
   if (e != cudaSuccess) return e;
-  launch_dependent(decode_flat_kernel<FP8, SCORES>, (p.runs + kFlatWarps - 1) / kFlatWarps, kFlatWarps * 32, FlatSizes<FP8>::kTotal, s, p);
+  launch_dependent(decode_flat_kernel<FP8, SCORES>, p.blocks, kFlatWarps * 32, FlatSizes<FP8>::kTotal, s, p);
   return cudaGetLastError();
 }
 
@@ -588,17 +591,23 @@ struct Pieces {
 // Runs: as many as warps (prefixes: blocks) fit the chip, or as the longest contexts that the tables allow could fill.
 // Where those contexts are few bytes, rows walk their prefixes themselves: the prefixes' kernel takes 8 us, in which decode_flat reads 40 MB.
 constexpr long kPrefixBytes = 40L << 20;
-struct FlatPlan { int runs, least, n_groups, prefix_runs; };
+// One block of bf16 prefixes an SM, beside which blocks of decode_flat have room; those take their runs, shorter ones, as they come (64 groups of 8 rows, 390 + 750 tokens 93 ->
+// 88 us).  fp8 prefixes are bound by issue slots and get two: 13 groups of 16 rows, 4100 + 560 tokens, 92 us, with one 107.
+constexpr long kBesideRuns = 2;
+struct FlatPlan { int runs, least, n_groups, prefix_runs, blocks; };
 FlatPlan flat_plan(const DecodeCall* c, int n_groups, int max_group, int num_sms) {
   const long most = static_cast<long>(c->S) * c->Hkv * c->max_blocks;
   const int fit = num_sms * kFlatWarps * (c->k_scale != nullptr ? FlatSizes<true>::kBlocks : FlatSizes<false>::kBlocks), least = 2;
   const long runs = (most + least - 1) / least;
-  FlatPlan plan = {static_cast<int>(runs < fit ? runs : fit), least, n_groups, 0};
+  FlatPlan plan = {static_cast<int>(runs < fit ? runs : fit), least, n_groups, 0, 0};
   if (n_groups > 0 && most * (c->k_scale != nullptr ? FlatSizes<true>::kStage : FlatSizes<false>::kStage) > kPrefixBytes) {
     const long tiles = (static_cast<long>(max_group) * (c->Hq / c->Hkv) + kPrefixRows - 1) / kPrefixRows;
     const long most_runs = (n_groups * tiles * c->Hkv * ((c->max_blocks * 16L + kPrefixKeys - 1) / kPrefixKeys) + kPrefixLeast - 1) / kPrefixLeast;
-    plan.prefix_runs = static_cast<int>(most_runs < 2L * num_sms ? most_runs : 2L * num_sms);
+    const long prefix_fit = num_sms * (c->k_scale != nullptr ? 2L : 1L);
+    plan.prefix_runs = static_cast<int>(most_runs < prefix_fit ? most_runs : prefix_fit);
+    plan.runs = static_cast<int>(runs < kBesideRuns * fit ? runs : kBesideRuns * fit);
   }
+  plan.blocks = (plan.runs < fit ? plan.runs + kFlatWarps - 1 : fit) / kFlatWarps;
   return plan;
 }
 size_t lay_out(FlatParams& p, const DecodeCall* c, const FlatPlan& plan, void* scratch) {
@@ -628,7 +637,7 @@ FlatParams flat_params(const DecodeCall* c, const FlatPlan& plan, void* scratch)
   p.out = static_cast<__nv_bfloat16*>(c->out);
   p.q_stride_s = c->q_stride_s;
   p.S = c->S; p.max_blocks = c->max_blocks; p.Hq = c->Hq; p.Hkv = c->Hkv; p.G = c->Hq / c->Hkv;
-  p.runs = plan.runs; p.least = plan.least; p.n_groups = plan.n_groups; p.prefix_runs = plan.prefix_runs;
+  p.runs = plan.runs; p.least = plan.least; p.n_groups = plan.n_groups; p.prefix_runs = plan.prefix_runs; p.blocks = plan.blocks;
   p.scale_log2 = c->scale * 1.4426950408889634f;
   return p;
 }
@@ -671,7 +680,7 @@ extern "C" cudaError_t nrl_paged_decode_scored(const DecodeCall* c, const float*
   if (e != cudaSuccess) return e;
   p.wide = (reinterpret_cast<uintptr_t>(scores_in) | reinterpret_cast<uintptr_t>(scores_out)) % 16 == 0 && (in_row | in_head | out_row | out_head) % 4 == 0;
   // tokens a block: rows' contexts whole where there are rows enough for the chip
-  p.chunk = static_cast<long>(c->S) * c->Hkv >= 2L * num_sms ? 4096 : 512;
+  p.chunk = static_cast<long>(c->S) * c->Hkv >= 2L * num_sms ? 4096 : 1024;
   launch_dependent(decode_join_kernel<true>, dim3(c->S, c->Hkv * ((p.max_tokens + p.chunk - 1) / p.chunk)), 256, 0, s, p);
   return cudaGetLastError();
 }

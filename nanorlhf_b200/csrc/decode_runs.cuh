@@ -13,7 +13,7 @@ struct FlatParams {
   const int *block_tables, *context_lens, *cu_groups, *shared;
   // what decode_plan finds
   int4* rows;                   // [S] first token that the row walks itself, pages of the rows in front (of one kv head), its own pages, its prefix's group + 1 (0: none);
-                                // [S]: -, pages of all rows, pages a run, -
+                                // [S]: -, pages of all rows, pages a run, runs that have been taken
   int4* starts;                 // [runs] row, kv head, page of the row's own, -
   int4* groups;                 // [n_groups] steps of 64 tokens, of all heads and tiles, of the groups in front, the group's own (of a tile), its tiles of 64 query rows, its
                                 // query rows (of one kv head); [n_groups]: all steps, steps a run, -, -
@@ -25,7 +25,7 @@ struct FlatParams {
   const float* scores_in;
   float* scores_out;
   long q_stride_s, in_row, in_head, out_row, out_head;
-  int n_groups, prefix_runs, S, max_blocks, Hq, Hkv, G, runs, least, max_tokens, chunk, wide;
+  int n_groups, prefix_runs, blocks, S, max_blocks, Hq, Hkv, G, runs, least, max_tokens, chunk, wide;
   float scale_log2, decay;
 };
 

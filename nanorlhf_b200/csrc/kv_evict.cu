@@ -2,14 +2,15 @@
 // largest scores (ties: the lower index), every kv head its own; what is kept moves together, in order, into the first `keep` places.
 //
 // kv_select: a cluster of blocks per (row, kv head), more blocks where there are few and their contexts long.  A block has a range of tokens; their scores, as whole
-// numbers whose order is theirs, wait in shared memory (above 48 K tokens a block in global memory).  The smallest kept one is found three bits at a time: how many are at
-// or above each of seven candidates, by votes of warps and sums over the block and the cluster, until as many are above one as are to be kept.  Then the tokens are counted
-// again, word by word of 32, and indices and a bit a token are written in order.  Bound by latency, up to eleven rounds of a barrier (and one of the cluster).
-// Counts of digits by atomics meet: a score's highest bits are a few exponents, and 3750 tokens a block took 120 us with eight bits a round, 20 with eleven.
+// numbers whose order is theirs, wait in shared memory.  The smallest kept one is found three bits at a time: a thread counts the eight digits of the keys that may still be it
+// in the bytes of two words, warps, the block and the cluster add up, until as many keys are at or above a digit as are to be kept.  Then the tokens are
+// counted again, word by word of 32, and indices and a bit a token are written in order.  Bound by latency, up to eleven rounds of a barrier (and one of the cluster).
+// (Counts of digits by atomics in shared memory meet: a score's highest bits are a few exponents, and 3750 tokens a block took 120 us with eight bits a round, 20 with eleven;
+// seven votes a word and round 20.)
 // kv_move: a block per (row, kv head, slice of a token's keys or values), and per range of places where sources and targets are apart.  In place, token j of what
 // is kept comes from a place >= j, so that a block that reads a range of places before it writes them, ranges in order and the next one on its way, may move it;
 // other slices' bytes are not touched.
-// kv_move_transposed, at the same time: values of fp8 pages lie transposed.  Sixteen pages at a time go through shared memory, rows of 16 bytes 20 apart (no bank
+// kv_move_transposed, beside it: values of fp8 pages lie transposed.  Sixteen pages at a time go through shared memory, rows of 16 bytes 20 apart (no bank
 // conflicts), and a thread puts together an element's bytes of a whole page.
 #include "cluster_read.h"
 #include "common.cuh"
@@ -19,9 +20,7 @@
 
 namespace nrl {
 
-constexpr int kSelThreads = 512;
-constexpr int kSelWarps = kSelThreads / 32;
-constexpr int kSelTokens = 48 * 1024;     // of a block, in shared memory
+constexpr int kSelTokens = 48 * 1024;     // of a block, in shared memory; kSelCluster times as many of a row at the most (checked on the host)
 constexpr int kSelCluster = 8;
 
 // larger scores have larger keys; -0 is 0, a NaN is below everything (0)
@@ -30,16 +29,25 @@ NRL_DEVICE uint32_t order_key(float x) {
   const uint32_t b = __float_as_uint(x + 0.f);
   return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
+// 0 from 32 places on
+NRL_DEVICE uint32_t shl(uint32_t x, uint32_t by) {
+  uint32_t r;
+  asm("shl.b32 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(by));
+  return r;
+}
 NRL_DEVICE void evict_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-__global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const EvictCall p, const int cluster, const int in_smem) {
+// WARPS: 4 for up to 2048 tokens a block, where sums over more warps cost more than their share of the words saves
+template <int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) kv_select_kernel(const EvictCall p, const int cluster) {
+  constexpr int kSelWarps = WARPS, kSelThreads = WARPS * 32;
   pdl_wait();
   pdl_launch_dependents();
   extern __shared__ uint32_t keys[];
-  __shared__ __align__(16) uint4 warp_counts[2][kSelWarps][2];        // of two rounds in turn: eight counts, the first one unused
+  __shared__ __align__(16) uint4 warp_counts[2][kSelWarps];           // of two rounds in turn: eight counts of 16 bits
   __shared__ __align__(16) uint4 counts[2][2];                        // the block's; others may still read the last round's
   __shared__ __align__(16) uint4 total;
   __shared__ uint2 warp_sums[kSelWarps];
@@ -47,16 +55,12 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const EvictCall 
   const int n = max(0, min(p.context_lens[seq], p.max_tokens));
   const long row = static_cast<long>(seq) * p.Hkv + kvh;
   int* kept = p.kept + row * p.keep;
-  float* kept_scores = p.kept_scores + row * p.keep;
   const float* sc = p.scores + seq * p.score_row + kvh * p.score_head;
   uint32_t* bits = p.bits + row * ((p.max_tokens + 31) / 32);
   if (kvh == 0 && rank == 0 && tid == 0) p.new_lens[seq] = min(n, p.keep);
   if (n <= p.keep) {
     const int at = rank * kSelThreads + tid, step = cluster * kSelThreads;
-    for (int j = at; j < p.keep; j += step) {
-      kept[j] = j < n ? j : -1;
-      kept_scores[j] = j < n ? sc[j] : 0.f;
-    }
+    for (int j = at; j < p.keep; j += step) kept[j] = j < n ? j : -1;
     for (int w = at; w * 32 < n; w += step) bits[w] = n - w * 32 >= 32 ? 0xffffffffu : (1u << (n - w * 32)) - 1;
     return;
   }
@@ -65,60 +69,68 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const EvictCall 
   const int t0 = b0 * 32, m0 = max(lo, t0), m1 = min(hi, b1 * 32);     // of this block
   const uint32_t wanted = p.keep - p.sinks - p.recent;
   const bool any = wanted > 0;
-  auto key_at = [&](int t) { return in_smem ? keys[t - t0] : t >= m0 && t < m1 ? order_key(sc[t]) : 0u; };        // 0: may not go
   // a warp has a range of neighbouring words of 32 tokens
   const int per = (b1 - b0 + kSelWarps - 1) / kSelWarps, w0 = min(b1, b0 + warp * per), w1 = min(b1, w0 + per);
   uint32_t least = 0;                                                 // `wanted` keys or more are at or above it
   bool exact = false;                                                 // no more than those
   if (any) {
-    if (in_smem) {
-#pragma unroll 4
-      for (int w = w0; w < w1; ++w) {                                 // (a warp reads its own)
-        const int t = w * 32 + lane;
-        keys[t - t0] = t >= m0 && t < m1 ? order_key(sc[t]) : 0u;
-      }
+#pragma unroll 8
+    for (int w = w0; w < w1; ++w) {                                   // (a warp reads its own)
+      const int t = w * 32 + lane;
+      keys[t - t0] = t >= m0 && t < m1 ? order_key(sc[t]) : 0u;       // 0: may not go
     }
+    uint32_t over = 0;                                                // keys behind the eight digits
 #pragma unroll 1
     for (int round = 0; round < 11 && !exact; ++round) {
-      const int shift = max(0, 29 - 3 * round), most = round < 10 ? 7 : 3;
-      uint32_t n_at[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll 2
+      const int shift = max(0, 29 - 3 * round);                       // (the last round has the last two bits; four more digits have been counted)
+      uint32_t lo = 0, hi = 0;                                        // a lane has 96 words at the most
+#pragma unroll 4
       for (int w = w0; w < w1; ++w) {
-        const uint32_t k = key_at(w * 32 + lane);
-#pragma unroll
-        for (int v = 1; v < 8; ++v) n_at[v] += __popc(__ballot_sync(0xffffffffu, k >= least + (static_cast<uint32_t>(v) << shift)));
+        const uint32_t d = 8 * min((keys[w * 32 + lane - t0] - least) >> shift, 8u);
+        lo += shl(1u, d);
+        hi += shl(1u, d - 32u);
       }
-      if (lane < 2) warp_counts[round & 1][warp][lane] = lane == 0 ? make_uint4(0, n_at[1], n_at[2], n_at[3]) : make_uint4(n_at[4], n_at[5], n_at[6], n_at[7]);
-      __syncthreads();
-      // lane 2 i + j: half j of warp i's counts, then of block i's
-      auto add = [&](uint4 c, int from) {
-        for (int d = from; d >= 2; d >>= 1) {
-          c.x += __shfl_xor_sync(0xffffffffu, c.x, d); c.y += __shfl_xor_sync(0xffffffffu, c.y, d);
-          c.z += __shfl_xor_sync(0xffffffffu, c.z, d); c.w += __shfl_xor_sync(0xffffffffu, c.w, d);
+      uint4 c = make_uint4(lo & 0x00ff00ffu, (lo >> 8) & 0x00ff00ffu, hi & 0x00ff00ffu, (hi >> 8) & 0x00ff00ffu);       // digits 0 2, 1 3, 4 6, 5 7
+      auto add = [&](uint4 x, int from) {
+        for (int m = from; m > 0; m >>= 1) {
+          x.x += __shfl_xor_sync(0xffffffffu, x.x, m); x.y += __shfl_xor_sync(0xffffffffu, x.y, m);
+          x.z += __shfl_xor_sync(0xffffffffu, x.z, m); x.w += __shfl_xor_sync(0xffffffffu, x.w, m);
         }
-        return c;
+        return x;
       };
-      uint4 c = add(warp_counts[round & 1][lane >> 1][lane & 1], 16);
+      c = add(c, 16);
+      if (lane == 0) warp_counts[round & 1][warp] = c;
+      __syncthreads();
+      c = add(lane < kSelWarps ? warp_counts[round & 1][lane] : make_uint4(0, 0, 0, 0), kSelWarps / 2);
+      uint32_t n_of[8] = {c.x & 0xffffu, c.y & 0xffffu, c.x >> 16, c.y >> 16, c.z & 0xffffu, c.w & 0xffffu, c.z >> 16, c.w >> 16};
       if (cluster > 1) {
-        if (warp == 0 && lane < 2) counts[round & 1][lane] = c;
+        if (tid < 2) counts[round & 1][tid] = tid == 0 ? make_uint4(n_of[0], n_of[1], n_of[2], n_of[3]) : make_uint4(n_of[4], n_of[5], n_of[6], n_of[7]);
         evict_cluster_sync();
-        c = make_uint4(0, 0, 0, 0);
-        if ((lane >> 1) < cluster) {
-          const float4 v = ld_cluster_f4(smem_u32(&counts[round & 1][lane & 1]), lane >> 1);
-          c = make_uint4(__float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w));
+        uint4 x = make_uint4(0, 0, 0, 0);                             // lane i + 8 j: half j of block i's
+        if ((lane & 7) < cluster && lane < 16) {
+          const float4 v = ld_cluster_f4(smem_u32(&counts[round & 1][lane >> 3]), lane & 7);
+          x = make_uint4(__float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w));
         }
-        c = add(c, 16);
-      }
-      // the highest candidate that enough keys reach
-      const uint32_t mine[4] = {c.x, c.y, c.z, c.w};
-      uint32_t best = 0, of_best = 0;
+        x = add(x, kSelCluster / 2);
+        const uint32_t mine[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-      for (int v = 1; v < 8; ++v) {
-        const uint32_t reach = __shfl_sync(0xffffffffu, mine[v & 3], v >> 2);
-        if (v <= most && reach >= wanted) { best = v; of_best = reach; }
+        for (int v = 0; v < 8; ++v) n_of[v] = __shfl_sync(0xffffffffu, mine[v & 3], (v >> 2) * 8);
+      } else {
+#pragma unroll
+        for (int v = 0; v < 8; ++v) n_of[v] = __shfl_sync(0xffffffffu, n_of[v], 0);
+      }
+      // the highest digit that enough keys reach
+      uint32_t best = 0, of_best = 0, behind = over, reach = over;
+      bool found = false;
+#pragma unroll
+      for (int v = 7; v >= 0; --v) {
+        const uint32_t with = reach + (v < 4 || round < 10 ? n_of[v] : 0u);
+        if (!found && with >= wanted) { found = true; best = v; of_best = with; behind = reach; }
+        reach = with;
       }
       least += best << shift;
-      exact = best > 0 && of_best == wanted;
+      over = behind;
+      exact = of_best == wanted && least > 0;
     }
   }
   if (exact) --least;                                                 // all above it (a candidate is above 0)
@@ -126,11 +138,12 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const EvictCall 
   auto look = [&](int word, uint32_t& more, uint32_t& same) {
     const int t = word * 32 + lane;
     const bool middle = any && t >= lo && t < hi;
-    const uint32_t k = middle ? key_at(t) : 0u;
+    const uint32_t k = middle ? keys[t - t0] : 0u;
     more = __ballot_sync(0xffffffffu, t < n && (t < lo || t >= hi || (middle && k > least)));
     same = __ballot_sync(0xffffffffu, middle && k == least);
   };
   uint32_t more = 0, same = 0;
+#pragma unroll 4
   for (int w = w0; w < w1; ++w) {
     uint32_t a, b;
     look(w, a, b);
@@ -155,6 +168,7 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const EvictCall 
   }
   for (int w = 0; w < warp; ++w) { more += warp_sums[w].x; same += warp_sums[w].y; }
   const uint32_t under = (1u << lane) - 1;
+#pragma unroll 4
   for (int w = w0; w < w1; ++w) {
     uint32_t a, b;
     look(w, a, b);
@@ -162,7 +176,6 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const EvictCall 
     if (is) {
       const uint32_t j = more + __popc(a & under) + min(same + __popc(b & under), need);
       kept[j] = w * 32 + lane;
-      kept_scores[j] = sc[w * 32 + lane];
     }
     const uint32_t m = __ballot_sync(0xffffffffu, is);
     if (lane == 0) bits[w] = m;
@@ -183,7 +196,7 @@ constexpr int kSpanRow = 5;               // words from an element's row to the 
 struct MoveParams {
   EvictCall e;
   const int* out_tables;
-  int out_blocks, key_slices;             // grid.y: kv heads x ranges of places; grid.z: slices of keys, then of values (fp8: the scales)
+  int out_blocks, key_slices;             // grid.y: kv heads x ranges of places; grid.z: slices of keys, then of values (fp8: the scales), then the scores
 };
 
 // where token t of a row lies: its place among all tokens (below 2^31: checked on the host)
@@ -236,7 +249,7 @@ NRL_DEVICE void move_rows(T* rows, int row_elems, int slice, const int* from, co
 NRL_DEVICE void move_transposed(uint4* v, long step, const int* from, const int* to, const int* kept, const uint16_t* bits, int j0, int j1) {
   __shared__ uint32_t span[kSpanPages * 128 * kSpanRow];
   __shared__ uint32_t left[2][128 * kSpanRow];                        // places of a page that is not full yet: read by one span, written by it for the next
-  __shared__ __align__(8) uint16_t place[kMoveThreads + 16];          // of the span's kept tokens, from the first place of their page on: the byte of element 0
+  __shared__ __align__(16) uint32_t place[kMoveThreads + 16];         // of the span's kept tokens, from the first place of their page on: the byte of element 0
   const int tid = threadIdx.x, d = tid & 127, warp_half = tid >> 7;
   const int last = kept[j1 - 1] >> 4;
   int page = kept[j0] >> 4, j = j0, turn = 0;
@@ -257,19 +270,19 @@ NRL_DEVICE void move_transposed(uint4* v, long step, const int* from, const int*
       uint32_t* w = span + ((u * 2 + warp_half) * 128 + d) * kSpanRow;
       w[0] = cur[u].x; w[1] = cur[u].y; w[2] = cur[u].z; w[3] = cur[u].w;
     }
-    if (here) place[(j & 15) + tid] = static_cast<uint16_t>(((t >> 4) - page) * 128 * kSpanRow * 4 + (t & 15));
+    if (here) place[(j & 15) + tid] = ((t >> 4) - page) * 128 * kSpanRow * 4 + (t & 15);
     const int to_j = j + __syncthreads_count(here);                   // places [j, to_j) come from this span
     if (to_j < j1) read(page + kSpanPages);
     const uint8_t* bytes = reinterpret_cast<const uint8_t*>(span) + d * kSpanRow * 4;
     for (int pg = (j >> 4) + warp_half; pg * 16 < to_j; pg += 2) {
       uint32_t word[4];
       const int k0 = max(0, j - pg * 16), k1 = min(16, to_j - pg * 16);          // places of this page that are put now
-      const uint16_t* at = place + (pg - (j >> 4)) * 16;
+      const uint32_t* at = place + (pg - (j >> 4)) * 16;
       if (k0 == 0 && k1 == 16) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint2 four = *reinterpret_cast<const uint2*>(at + 4 * i);
-          const uint32_t a = bytes[four.x & 0xffffu], b = bytes[four.x >> 16], c = bytes[four.y & 0xffffu], e = bytes[four.y >> 16];
+          const uint4 four = *reinterpret_cast<const uint4*>(at + 4 * i);
+          const uint32_t a = bytes[four.x], b = bytes[four.y], c = bytes[four.z], e = bytes[four.w];
           word[i] = __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, e, 0x0040), 0x5410);
         }
       } else {
@@ -318,31 +331,46 @@ NRL_DEVICE MoveRow move_row(const MoveParams& p) {
   return {e.block_tables + static_cast<long>(seq) * e.max_blocks, p.out_tables + static_cast<long>(seq) * p.out_blocks, e.kept + row * e.keep, row, kvh, j0, j1};
 }
 
+// keys and bf16 values, the scales of fp8 ones, and the scores of what is kept.  It takes nothing from kv_move_transposed, whose blocks had all begun when this one does;
+// its end waits for theirs.
 template <bool IN_PLACE>
 __global__ void __launch_bounds__(kMoveThreads, IN_PLACE ? 2 : 4) kv_move_kernel(const MoveParams p) {
+  const EvictCall& e = p.e;
+  const bool fp8 = e.k_scale != nullptr;
+  if (!fp8) pdl_wait();
+  pdl_launch_dependents();
+  const MoveRow m = move_row<IN_PLACE>(p);
+  const int z = blockIdx.z, last = fp8 ? p.key_slices + 2 : 2 * p.key_slices;
+  if (z == last) {
+    float* to = e.kept_scores + m.row * e.keep;
+    const float* sc = e.scores + static_cast<long>(blockIdx.x) * e.score_row + m.kvh * e.score_head;
+    const int j0 = IN_PLACE ? 0 : blockIdx.y / e.Hkv * kMoveRange, j1 = IN_PLACE || (blockIdx.y / e.Hkv + 1) * e.Hkv == gridDim.y ? e.keep : min(e.keep, j0 + kMoveRange);
+#pragma unroll 4
+    for (int j = j0 + threadIdx.x; j < j1; j += kMoveThreads) {
+      const int t = m.kept[j];
+      to[j] = t >= 0 ? sc[t] : 0.f;
+    }
+  } else if (m.j0 < m.j1) {
+    const bool keys = z < p.key_slices;
+    if (fp8 && !keys)
+      move_rows<IN_PLACE, float, 1>(z == p.key_slices ? e.k_scale : e.v_scale, 1, 0, m.from, m.to, m.kept, m.j0, m.j1, e.Hkv, m.kvh);
+    else
+      move_rows<IN_PLACE, uint4, kMovePieces>(static_cast<uint4*>(keys ? e.k_cache : e.v_cache), fp8 ? 8 : 16, keys ? z : z - p.key_slices, m.from, m.to, m.kept, m.j0, m.j1,
+                                              e.Hkv, m.kvh);
+  }
+  if (fp8) pdl_wait();
+}
+
+// values of fp8 pages
+template <bool IN_PLACE>
+__global__ void __launch_bounds__(kMoveThreads, 4) kv_move_transposed_kernel(const MoveParams p) {
   pdl_wait();
   pdl_launch_dependents();
   const EvictCall& e = p.e;
   const MoveRow m = move_row<IN_PLACE>(p);
   if (m.j0 >= m.j1) return;
-  const int z = blockIdx.z;
-  const bool keys = z < p.key_slices, fp8 = e.k_scale != nullptr;
-  if (fp8 && !keys) return move_rows<IN_PLACE, float, 1>(z == p.key_slices ? e.k_scale : e.v_scale, 1, 0, m.from, m.to, m.kept, m.j0, m.j1, e.Hkv, m.kvh);
-  move_rows<IN_PLACE, uint4, kMovePieces>(static_cast<uint4*>(keys ? e.k_cache : e.v_cache), fp8 ? 8 : 16, keys ? z : z - p.key_slices, m.from, m.to, m.kept, m.j0, m.j1,
-                                          e.Hkv, m.kvh);
-}
-
-// values of fp8 pages.  It takes nothing from kv_move, whose blocks had all begun when this one does; its end waits for theirs.
-template <bool IN_PLACE>
-__global__ void __launch_bounds__(kMoveThreads, 4) kv_move_transposed_kernel(const MoveParams p) {
-  const EvictCall& e = p.e;
-  const MoveRow m = move_row<IN_PLACE>(p);
-  if (m.j0 < m.j1) {
-    const uint16_t* bits = reinterpret_cast<const uint16_t*>(e.bits + m.row * ((e.max_tokens + 31) / 32));
-    move_transposed(static_cast<uint4*>(e.v_cache) + static_cast<long>(m.kvh) * 128, static_cast<long>(e.Hkv) * 128, m.from, m.to, m.kept, bits, m.j0, m.j1);
-  }
-  pdl_wait();
-  pdl_launch_dependents();
+  const uint16_t* bits = reinterpret_cast<const uint16_t*>(e.bits + m.row * ((e.max_tokens + 31) / 32));
+  move_transposed(static_cast<uint4*>(e.v_cache) + static_cast<long>(m.kvh) * 128, static_cast<long>(e.Hkv) * 128, m.from, m.to, m.kept, bits, m.j0, m.j1);
 }
 
 }  // namespace nrl
@@ -351,15 +379,26 @@ using namespace nrl;
 
 namespace {
 
+template <int WARPS>
+cudaError_t launch_select(const EvictCall& c, int cluster, int tokens, cudaStream_t s) {
+  static PerDevice<bool> configured;
+  const cudaError_t e = allow_smem(configured, kv_select_kernel<WARPS>, kSelTokens * 4);
+  if (e != cudaSuccess) return e;
+  launch_dependent_clusters(kv_select_kernel<WARPS>, dim3(c.S * cluster, c.Hkv), WARPS * 32, tokens * 4, s, cluster, c, cluster);
+  return cudaGetLastError();
+}
+
 template <bool IN_PLACE>
 cudaError_t launch_moves(const MoveParams& p, cudaStream_t s) {
   const EvictCall& c = p.e;
   const bool fp8 = c.k_scale != nullptr;
   const int places = c.keep < c.max_tokens ? c.keep : c.max_tokens, ranges = IN_PLACE ? 1 : (places + kMoveRange - 1) / kMoveRange;
-  launch_dependent(kv_move_kernel<IN_PLACE>, dim3(c.S, c.Hkv * ranges, fp8 ? p.key_slices + 2 : 2 * p.key_slices), kMoveThreads, 0, s, p);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || !fp8) return e;
-  launch_dependent(kv_move_transposed_kernel<IN_PLACE>, dim3(c.S, c.Hkv * ranges), kMoveThreads, 0, s, p);
+  if (fp8) {
+    launch_dependent(kv_move_transposed_kernel<IN_PLACE>, dim3(c.S, c.Hkv * ranges), kMoveThreads, 0, s, p);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
+  launch_dependent(kv_move_kernel<IN_PLACE>, dim3(c.S, c.Hkv * ranges, (fp8 ? p.key_slices + 2 : 2 * p.key_slices) + 1), kMoveThreads, 0, s, p);
   return cudaGetLastError();
 }
 
@@ -372,12 +411,8 @@ extern "C" cudaError_t nrl_kv_evict(const EvictCall* c, int num_sms, cudaStream_
   while (cluster < kSelCluster && ((static_cast<long>(c->S) * c->Hkv * cluster * 2 <= 2L * num_sms && c->max_tokens >= cluster * 2 * 2048) ||
                                    c->max_tokens > static_cast<long>(cluster) * kSelTokens)) cluster *= 2;
   const int tokens = ((c->max_tokens + 31) / 32 + cluster - 1) / cluster * 32;
-  const int in_smem = tokens <= kSelTokens;
-  static PerDevice<bool> configured;
-  cudaError_t e = allow_smem(configured, kv_select_kernel, kSelTokens * 4);
-  if (e != cudaSuccess) return e;
-  launch_dependent_clusters(kv_select_kernel, dim3(c->S * cluster, c->Hkv), kSelThreads, in_smem ? tokens * 4 : 0, s, cluster, *c, cluster, in_smem);
-  e = cudaGetLastError();
+  if (tokens > kSelTokens) return cudaErrorInvalidValue;
+  cudaError_t e = tokens <= 2048 ? launch_select<4>(*c, cluster, tokens, s) : launch_select<16>(*c, cluster, tokens, s);
   if (e != cudaSuccess) return e;
   MoveParams p;
   p.e = *c;
