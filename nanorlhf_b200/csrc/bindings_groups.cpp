@@ -277,7 +277,8 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> kv_evict(torch::Tensor k
   TORCH_CHECK_VALUE(c.max_tokens <= 8 * 48 * 1024, what, ": scores and tables of at most 393 216 tokens a row, got ", c.max_tokens);
   torch::Tensor kept = torch::empty({S, Hkv, keep}, tables.options()), kept_scores = torch::empty({S, Hkv, keep}, scores.options());
   torch::Tensor lens = torch::empty({S}, tables.options());
-  const torch::Tensor bits = torch::empty({S, Hkv, (c.max_tokens + 31) / 32}, tables.options());
+  // 512 bytes a row-head of counts, then the bits
+  const torch::Tensor scratch = torch::empty({S * Hkv * (128 + (c.max_tokens + 31) / 32)}, tables.options());
   c.k_cache = k.data_ptr();
   c.v_cache = v.data_ptr();
   c.k_scale = ks.has_value() ? ks->data_ptr<float>() : nullptr;
@@ -291,7 +292,8 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> kv_evict(torch::Tensor k
   c.kept = kept.data_ptr<int>();
   c.kept_scores = kept_scores.data_ptr<float>();
   c.new_lens = lens.data_ptr<int>();
-  c.bits = reinterpret_cast<unsigned*>(bits.data_ptr<int>());
+  c.bits = reinterpret_cast<unsigned*>(scratch.data_ptr<int>()) + S * Hkv * 128;
+  c.told = reinterpret_cast<uint4*>(scratch.data_ptr<int>());
   c.S = S; c.Hkv = Hkv; c.max_blocks = tables.size(1); c.out_blocks = to.defined() ? to.size(1) : 0;
   c.keep = keep; c.sinks = sinks; c.recent = recent;
   check(nrl_kv_evict(&c, num_sms(), cur_stream()), what);

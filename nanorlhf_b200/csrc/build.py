@@ -22,7 +22,7 @@ OBJ = os.path.join(HERE, "build")
 CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 
 CU_SOURCES = ["gemm_sm100.cu", "gemm_sm100_2cta.cu", "gemm_tc.cu", "elementwise.cu", "rl_kernels.cu", "sampling.cu", "attention_decode.cu", "attention_decode_fp8.cu", "rope_kv.cu", "attention_fwd_tc.cu", "attention_bwd_tc.cu",
-              "attention_varlen.cu", "attention_deberta_tc.cu", "comm.cu", "quant.cu", "stream_ops.cu", "recurrent.cu", "delta_chunk_tc.cu", "attention_window.cu", "attention_window_mma.cu", "attention_window_tc.cu", "attention_latent_mma.cu", "moe.cu", "lightning.cu", "top_logits.cu", "distill.cu", "sample_filtered.cu", "attention_groups.cu", "decode_prefix.cu", "decode_flat.cu", "kv_evict.cu"]
+              "attention_varlen.cu", "attention_deberta_tc.cu", "comm.cu", "quant.cu", "stream_ops.cu", "recurrent.cu", "delta_chunk_tc.cu", "attention_window.cu", "attention_window_mma.cu", "attention_window_tc.cu", "attention_latent_mma.cu", "moe.cu", "lightning.cu", "top_logits.cu", "distill.cu", "sample_filtered.cu", "attention_groups.cu", "decode_flat.cu", "kv_evict.cu"]
 CPP_SOURCES = ["bindings.cpp", "runtime.cpp", "bindings_hybrid.cpp", "bindings_vocab.cpp", "bindings_groups.cpp"]
 # kernels of the float32 serving mode, and those that order logits or add them up to the last bit: IEEE division / sqrt / exp (no --use_fast_math)
 PRECISE_SOURCES = {"stream_ops.cu", "recurrent.cu", "delta_chunk_tc.cu", "attention_window.cu", "attention_window_mma.cu", "attention_window_tc.cu", "attention_latent_mma.cu", "moe.cu", "lightning.cu", "top_logits.cu", "distill.cu",

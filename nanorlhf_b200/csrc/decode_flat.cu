@@ -1,17 +1,19 @@
-// Decode attention over the pages of rows whose contexts differ: behind a shared prefix (decode_prefix.cu) and with scores.
+// Decode attention over the pages of rows whose contexts differ: behind a shared prefix (decode_prefix.cuh) and with scores.
 //
 //   out = sum_parts 2^(m_p - M) O_p / sum_parts 2^(m_p - M) l_p,  a part being the (maximum, sum, unnormalised result) of some of the row's keys
 //   scores[s, h, t] = decay * scores[s, h, t] + sum over the G heads of kv head h of 2^(x - M) / L     (the newest token: the sum alone)
 //
 // The pages of all rows and kv heads, one behind the other, are dealt to the warps of the chip in equal runs: no block is longer than another, none starts
 // again for every row, and few long contexts are cut as finely as many short ones.
-//   decode_plan   (one block) adds up the rows' pages and finds where every warp's run begins
-//   decode_flat   a warp walks its run through its own ring of pages (cp.async); of every row that it meets it leaves a part.  Run w and row-head r meet
-//                 in part w + r: along the runs one of the two grows by one at a time
+//   decode_plan   (one block) adds up the rows' pages and finds where every warp's run begins; few rows without prefixes' runs do without it: every block of
+//                 decode_flat makes the plan (4 rows of 330 tokens 10.1 -> 7.4 us, 64 rows of a 100-token prefix 17.9 -> 17.8)
+//   decode_flat   the first blocks walk the prefixes (decode_prefix.cuh), then all of them the rows: a warp walks a run through its own ring of pages (cp.async);
+//                 of every row that it meets it leaves a part.  Run w and row-head r meet in part w + r: along the runs one of the two grows by one at a time
 //   decode_join   a warp a row and head joins the parts, the prefix's too, in their order; with scores, further blocks form the weights from the scores that the
 //                 walk left in scratch memory (4 G bytes a token beside the 512 or 264 of its keys and values; what fits L2 is not read from memory again)
 // The arithmetic is that of attention_decode.cu and attention_decode_fp8.cu.  Bound by memory.
 #include "common.cuh"
+#include "decode_prefix.cuh"
 #include "decode_runs.cuh"
 #include "fp8_fragments.cuh"
 #include "group_kernels.h"
@@ -25,6 +27,7 @@ namespace nrl {
 constexpr int kFlatWarps = 4;
 constexpr int kFlatD = 128;
 constexpr int kPlanThreads = 1024;
+constexpr int kNearRows = kFlatWarps * 32;
 constexpr int kPrefixLeast = 2;                   // steps of the prefixes a run
 constexpr float kFlatScale = 1024.f;              // of fp8 weights, which are f16 (2^10: small ones stay normal)
 
@@ -35,6 +38,7 @@ struct FlatSizes {
   static constexpr int kStages = FP8 ? 4 : 3;
   static constexpr int kBlocks = FP8 ? 3 : 2;                        // an SM
   static constexpr int kTotal = kFlatWarps * kStages * kStage;
+  static_assert(kTotal >= PreSmem<FP8>::kTotal && kFlatWarps == kPreWarps);
 };
 
 // the last group that begins at or in front of a row; it has the row if it does not end there
@@ -84,6 +88,49 @@ NRL_DEVICE void plan_starts(int4* starts, int owners, int total, int run, From f
   }
 }
 
+NRL_DEVICE int flat_pages(const FlatParams& p, int ctx, int first) {     // that a row walks itself
+  return (ctx + 15) / 16 - first / 16 + (p.prefix_runs == 0 ? (first + 15) / 16 : 0);
+}
+// The plan of few rows and no prefixes' runs, by every block for itself, a thread a row: no kernel in front.
+NRL_DEVICE const int4* plan_near(const FlatParams& p) {
+  __shared__ struct { int4 rows[kNearRows + 1]; int group[kNearRows], sums[kNearRows / 32]; } near;
+  const int s = threadIdx.x, warp = s >> 5, lane = s & 31, ctx = s < p.S ? flat_context(p, s) : 0;
+  near.group[s] = 0;
+  if (p.n_groups > 0) {
+    __syncthreads();
+    for (int g = s; g < p.n_groups; g += kNearRows) {
+      const int a = p.cu_groups[g], b = p.cu_groups[g + 1];
+      if (a >= 0 && b <= p.S && p.shared[g] > 0)
+        for (int r = a; r < b; ++r) near.group[r] = g + 1;
+    }
+    __syncthreads();
+  }
+  const int prefix = near.group[s], first = prefix > 0 ? min(p.shared[prefix - 1], ctx) : 0, n = flat_pages(p, ctx, first);
+  int upto = n;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += v;
+  }
+  if (lane == 31) near.sums[warp] = upto;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kNearRows / 32; ++w) {
+    before += w < warp ? near.sums[w] : 0;
+    all += near.sums[w];
+  }
+  const int4 row = make_int4(first, before + upto - n, n, prefix), total = make_int4(0, all, max(p.least, (all * p.Hkv + p.runs - 1) / p.runs), 0);
+  near.rows[s] = row;
+  if (s == 0) near.rows[kNearRows] = total;
+  if (blockIdx.x == 0) {                                              // for decode_join
+    if (s < p.S) p.rows[s] = row;
+    if (s == 0) p.rows[p.S] = total;
+  }
+  __syncthreads();
+  return near.rows;
+}
+
 // (all positions are below 2^27: checked on the host)
 __global__ void __launch_bounds__(kPlanThreads) decode_plan_kernel(const FlatParams p) {
   pdl_wait();
@@ -113,7 +160,7 @@ __global__ void __launch_bounds__(kPlanThreads) decode_plan_kernel(const FlatPar
           first = max(0, min(shared, ctx));
         }
       }
-      n = (ctx + 15) / 16 - first / 16 + (p.prefix_runs == 0 ? (first + 15) / 16 : 0);
+      n = flat_pages(p, ctx, first);
     }
     off = before + plan_scan(n, warp_sums, all);
     if (s < p.S) p.rows[s] = make_int4(first, off, n, prefix);
@@ -126,6 +173,7 @@ __global__ void __launch_bounds__(kPlanThreads) decode_plan_kernel(const FlatPar
   plan_starts(p.starts, p.S, before * p.Hkv, run, [&](int s) { return (p.S <= kPlanThreads ? from_near[s] : p.rows[s].y) * p.Hkv; }, [&](int s) { return p.rows[s].z; });
   if (p.prefix_runs == 0) return;
   // ---- prefixes ----
+  const long own_work = static_cast<long>(before) * p.Hkv;
   before = 0;
   __syncthreads();
   for (int g0 = 0; g0 < p.n_groups; g0 += kPlanThreads) {
@@ -141,7 +189,11 @@ __global__ void __launch_bounds__(kPlanThreads) decode_plan_kernel(const FlatPar
     from_near[tid] = off;
     before += all;
   }
-  const int prefix_run = max(kPrefixLeast, (before + p.prefix_runs - 1) / p.prefix_runs);
+  // as many blocks as the prefixes' share of the work, one an SM at the least; they take rows' pages afterwards
+  const long work = static_cast<long>(before) * p.step_cost;
+  const long share = (p.blocks * work + own_work + work - 1) / max(1L, own_work + work), sms = p.num_sms;
+  const long many = min(max(1L, (share + sms - 1) / sms) * sms, static_cast<long>(p.prefix_runs));
+  const int prefix_run = max(kPrefixLeast, static_cast<int>((before + many - 1) / many));
   if (tid == 0) p.groups[p.n_groups] = make_int4(before, prefix_run, 0, 0);
   __syncthreads();
   plan_starts(p.prefix_starts, p.n_groups, before, prefix_run, [&](int g) { return p.n_groups <= kPlanThreads ? from_near[g] : p.groups[g].x; },
@@ -167,8 +219,8 @@ struct FlatAt {
   int lead, lead_row;           // pages of a prefix that the row walks itself, in front, and the row whose they are
 };
 template <bool LEAD>
-NRL_DEVICE void flat_row(const FlatParams& p, FlatAt& a, int s) {
-  const int4 row = p.rows[s];
+NRL_DEVICE void flat_row(const FlatParams& p, const int4* rows, FlatAt& a, int s) {
+  const int4 row = rows[s];
   a.s = s;
   a.first = row.x;
   a.pages = row.z;
@@ -177,12 +229,12 @@ NRL_DEVICE void flat_row(const FlatParams& p, FlatAt& a, int s) {
   a.lead_row = a.lead > 0 ? p.cu_groups[row.w - 1] : 0;
 }
 template <bool LEAD>
-NRL_DEVICE bool flat_next(const FlatParams& p, FlatAt& a) {          // true: another row-head begins
+NRL_DEVICE bool flat_next(const FlatParams& p, const int4* rows, FlatAt& a) {          // true: another row-head begins
   if (++a.page < a.pages) return false;
   a.page = 0;
   if (++a.h == p.Hkv) {
     a.h = 0;
-    do flat_row<LEAD>(p, a, a.s + 1); while (a.pages == 0 && a.s + 1 < p.S);
+    do flat_row<LEAD>(p, rows, a, a.s + 1); while (a.pages == 0 && a.s + 1 < p.S);
   }
   return true;
 }
@@ -191,27 +243,51 @@ NRL_DEVICE long flat_entry(const FlatParams& p, const FlatAt& a, int i) {
   return i < a.lead ? static_cast<long>(a.lead_row) * p.max_blocks + i : static_cast<long>(a.s) * p.max_blocks + a.first / 16 + i - a.lead;
 }
 
-template <bool FP8, bool SCORES>
+// NEAR: few rows, whose plan every block makes for itself; no prefixes' runs
+template <bool FP8, bool SCORES, bool NEAR>
 __global__ void __launch_bounds__(kFlatWarps * 32, FlatSizes<FP8>::kBlocks) decode_flat_kernel(const FlatParams p) {
-  // Behind decode_prefix, whose blocks have all begun when this one's do, and with that found decode_plan ended: nothing is taken from it, and only the end waits for its.
-  const bool beside = p.prefix_runs > 0;
-  if (!beside) pdl_wait();
+  pdl_wait();
   pdl_launch_dependents();
   using Z = FlatSizes<FP8>;
   extern __shared__ __align__(128) uint8_t smem[];
+  if constexpr (!SCORES && !NEAR) {
+    if (static_cast<int>(blockIdx.x) < p.prefix_runs) {
+      decode_prefix_run<FP8>(p, smem, blockIdx.x);
+      __syncthreads();
+    }
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-  const int run = p.rows[p.S].z, all = p.rows[p.S].y * p.Hkv;
-  // The next run that nobody has: blocks that find no room beside decode_prefix's begin late.
-  for (;;) {
+  const int4* rows = p.rows;
+  if constexpr (NEAR) rows = plan_near(p);
+  const int4 total = rows[NEAR ? kNearRows : p.S];
+  const int run = total.z, all = total.y * p.Hkv;
+  // The next run that nobody has: blocks that have walked a prefix come late.  Of few rows, one a warp.
+  for (bool more = true; more;) {
     int w = 0;
-    if (lane == 0) w = atomicAdd(&p.rows[p.S].w, 1);
-    w = __shfl_sync(0xffffffffu, w, 0);
+    if (NEAR) {
+      w = blockIdx.x * kFlatWarps + warp;
+      more = false;
+    } else {
+      if (lane == 0) w = atomicAdd(&p.rows[p.S].w, 1);
+      w = __shfl_sync(0xffffffffu, w, 0);
+    }
     const int count = w < p.runs ? min(run, all - w * run) : 0;
     if (count <= 0) break;
     FlatAt here, ahead;
     {
-      const int4 start = p.starts[w];
-      flat_row<!SCORES>(p, here, start.x);
+      int4 start;
+      if (NEAR) {
+        int lo = 0, hi = p.S;                                          // the last row that begins at or in front
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (rows[mid].y * p.Hkv <= w * run) lo = mid; else hi = mid;
+        }
+        const int at = w * run - rows[lo].y * p.Hkv, d = rows[lo].z;
+        start = make_int4(lo, at / d, at % d, 0);
+      } else {
+        start = p.starts[w];
+      }
+      flat_row<!SCORES>(p, rows, here, start.x);
       here.h = start.y;
       here.page = start.z;
       ahead = here;
@@ -245,7 +321,7 @@ __global__ void __launch_bounds__(kFlatWarps * 32, FlatSizes<FP8>::kBlocks) deco
             cp_async_16(vd + at, vsrc + chunk * 16);
           }
         }
-        if (++issued < count && flat_next<!SCORES>(p, ahead)) ids_from = -1;
+        if (++issued < count && flat_next<!SCORES>(p, rows, ahead)) ids_from = -1;
       }
       cp_async_commit();
     };
@@ -428,7 +504,7 @@ __global__ void __launch_bounds__(kFlatWarps * 32, FlatSizes<FP8>::kBlocks) deco
       if (two) ++here.page;
       if (it == count) break;
       const FlatAt last = here;
-      if (flat_next<!SCORES>(p, here)) {
+      if (flat_next<!SCORES>(p, rows, here)) {
         const FlatAt now = here;
         here = last;
         leave();
@@ -439,11 +515,9 @@ __global__ void __launch_bounds__(kFlatWarps * 32, FlatSizes<FP8>::kBlocks) deco
     leave();
     cp_async_wait<0>();
   }
-  if (beside) pdl_wait();
 }
 
 // ---- parts to results, scores to weights ---------------------------------------------------------------------------------------------
-constexpr int kJoinU = 4;                // parts in flight
 
 struct FlatParts {
   const float2* ml;                      // of the first part of a row
@@ -464,7 +538,7 @@ NRL_DEVICE FlatParts prefix_parts(const FlatParams& p, int g, int s, int h, int 
   return {reinterpret_cast<const float2*>(p.prefix_ml) + at, reinterpret_cast<const float4*>(p.prefix_o) + at * 32, (a + group.y - 1) / run - c0 + 1};
 }
 // a lane has four elements; a row's parts lie 8 rows apart, a prefix's 64
-template <bool PREFIX>
+template <bool PREFIX, int kJoinU>
 NRL_DEVICE void join_parts(const FlatParts& x, int lane, float& M, float& L, float4& acc) {
   for (int i0 = 0; i0 < x.n; i0 += kJoinU) {
     float2 e[kJoinU];
@@ -487,8 +561,9 @@ NRL_DEVICE void join_parts(const FlatParts& x, int lane, float& M, float& L, flo
   }
 }
 
-// grid: rows x (kv heads x, with scores, chunks of tokens); a warp a query head for the results, which the first chunk's blocks form
-template <bool SCORES>
+// grid: rows x (kv heads x, with scores, chunks of tokens); a warp a query head for the results, which the first chunk's blocks form.
+// U parts in flight: 8 for the many parts of few rows (8 rows of 30 k tokens 55 -> 53 us, 4 of 330 7.4 -> 6.8), else 4 (253 rows of 2 k tokens 71, with 8 73)
+template <bool SCORES, int U>
 __global__ void __launch_bounds__(256) decode_join_kernel(const FlatParams p) {
   pdl_wait();
   pdl_launch_dependents();
@@ -502,8 +577,8 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const FlatParams p) {
     float M = -INFINITY, L = 0.f;
     if (chunk == 0) {
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (!SCORES && row.w > 0 && p.prefix_runs > 0) join_parts<true>(prefix_parts(p, row.w - 1, s, h, warp), lane, M, L, acc);
-      join_parts<false>(own, lane, M, L, acc);
+      if (!SCORES && row.w > 0 && p.prefix_runs > 0) join_parts<true, U>(prefix_parts(p, row.w - 1, s, h, warp), lane, M, L, acc);
+      join_parts<false, U>(own, lane, M, L, acc);
       const float f = L > 0.f ? 1.f / L : 0.f;
       uint2 v;
       v.x = pack_bf16x2(acc.x * f, acc.y * f);
@@ -567,12 +642,30 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const FlatParams p) {
 
 namespace {
 
+cudaError_t launch_plan(const FlatParams& p, cudaStream_t s) {
+  if (p.near) return cudaSuccess;
+  launch_dependent(decode_plan_kernel, 1, kPlanThreads, 0, s, p);
+  return cudaGetLastError();
+}
+template <bool FP8, bool SCORES, bool NEAR>
+cudaError_t launch_walk(const FlatParams& p, cudaStream_t s) {
+  static PerDevice<bool> configured;
+  const cudaError_t e = allow_smem(configured, decode_flat_kernel<FP8, SCORES, NEAR>, FlatSizes<FP8>::kTotal);
+  if (e != cudaSuccess) return e;
+  launch_dependent(decode_flat_kernel<FP8, SCORES, NEAR>, p.blocks, kFlatWarps * 32, FlatSizes<FP8>::kTotal, s, p);
+  return cudaGetLastError();
+}
+
 template <bool FP8, bool SCORES>
 cudaError_t launch_flat(const FlatParams& p, cudaStream_t s) {
-  static PerDevice<bool> configured;
-  const cudaError_t e = allow_smem(configured, decode_flat_kernel<FP8, SCORES>, FlatSizes<FP8>::kTotal);
-  if (e != cudaSuccess) return e;
-  launch_dependent(decode_flat_kernel<FP8, SCORES>, p.blocks, kFlatWarps * 32, FlatSizes<FP8>::kTotal, s, p);
+  return p.near ? launch_walk<FP8, SCORES, true>(p, s) : launch_walk<FP8, SCORES, false>(p, s);
+}
+
+template <bool SCORES>
+cudaError_t launch_join(const FlatParams& p, int chunks, int threads, cudaStream_t s) {
+  const dim3 grid(p.S, p.Hkv * chunks);
+  if (p.near) launch_dependent(decode_join_kernel<SCORES, 8>, grid, threads, 0, s, p);
+  else launch_dependent(decode_join_kernel<SCORES, 4>, grid, threads, 0, s, p);
   return cudaGetLastError();
 }
 
@@ -591,9 +684,10 @@ struct Pieces {
 // Runs: as many as warps (prefixes: blocks) fit the chip, or as the longest contexts that the tables allow could fill.
 // Where those contexts are few bytes, rows walk their prefixes themselves: the prefixes' kernel takes 8 us, in which decode_flat reads 40 MB.
 constexpr long kPrefixBytes = 40L << 20;
-// One block of bf16 prefixes an SM, beside which blocks of decode_flat have room; those take their runs, shorter ones, as they come (64 groups of 8 rows, 390 + 750 tokens 93 ->
-// 88 us).  fp8 prefixes are bound by issue slots and get two: 13 groups of 16 rows, 4100 + 560 tokens, 92 us, with one 107.
-constexpr long kBesideRuns = 2;
+// A prefix's step of 64 tokens takes a block as long as this many pages of rows: blocks that begin with prefixes are as many SMs' worth as their share of the work.
+// Rows of 12 heads, 2 kv heads, all on one block an SM, two, three: bf16 64 x 8 of 512 + 256 tokens 48, 51, 58 us, 32 x 16 of 2000 + 128 77, 61, 75;
+// fp8 42, 42, 43 and 90, 67, 57; 13 x 16 of 28 heads, 4100 + 560 tokens 116, 86, 89.
+constexpr int kStepCost = 5, kStepCostFp8 = 8;
 struct FlatPlan { int runs, least, n_groups, prefix_runs, blocks; };
 FlatPlan flat_plan(const DecodeCall* c, int n_groups, int max_group, int num_sms) {
   const long most = static_cast<long>(c->S) * c->Hkv * c->max_blocks;
@@ -603,11 +697,11 @@ FlatPlan flat_plan(const DecodeCall* c, int n_groups, int max_group, int num_sms
   if (n_groups > 0 && most * (c->k_scale != nullptr ? FlatSizes<true>::kStage : FlatSizes<false>::kStage) > kPrefixBytes) {
     const long tiles = (static_cast<long>(max_group) * (c->Hq / c->Hkv) + kPrefixRows - 1) / kPrefixRows;
     const long most_runs = (n_groups * tiles * c->Hkv * ((c->max_blocks * 16L + kPrefixKeys - 1) / kPrefixKeys) + kPrefixLeast - 1) / kPrefixLeast;
-    const long prefix_fit = num_sms * (c->k_scale != nullptr ? 2L : 1L);
+    const long prefix_fit = fit / kFlatWarps;
     plan.prefix_runs = static_cast<int>(most_runs < prefix_fit ? most_runs : prefix_fit);
-    plan.runs = static_cast<int>(runs < kBesideRuns * fit ? runs : kBesideRuns * fit);
   }
   plan.blocks = (plan.runs < fit ? plan.runs + kFlatWarps - 1 : fit) / kFlatWarps;
+  if (plan.blocks < plan.prefix_runs) plan.blocks = plan.prefix_runs;
   return plan;
 }
 size_t lay_out(FlatParams& p, const DecodeCall* c, const FlatPlan& plan, void* scratch) {
@@ -626,7 +720,7 @@ size_t lay_out(FlatParams& p, const DecodeCall* c, const FlatPlan& plan, void* s
   }
   return pieces.used;
 }
-FlatParams flat_params(const DecodeCall* c, const FlatPlan& plan, void* scratch) {
+FlatParams flat_params(const DecodeCall* c, const FlatPlan& plan, void* scratch, int num_sms) {
   FlatParams p = {};
   lay_out(p, c, plan, scratch);
   p.q = static_cast<const __nv_bfloat16*>(c->q);
@@ -637,7 +731,9 @@ FlatParams flat_params(const DecodeCall* c, const FlatPlan& plan, void* scratch)
   p.out = static_cast<__nv_bfloat16*>(c->out);
   p.q_stride_s = c->q_stride_s;
   p.S = c->S; p.max_blocks = c->max_blocks; p.Hq = c->Hq; p.Hkv = c->Hkv; p.G = c->Hq / c->Hkv;
-  p.runs = plan.runs; p.least = plan.least; p.n_groups = plan.n_groups; p.prefix_runs = plan.prefix_runs; p.blocks = plan.blocks;
+  p.runs = plan.runs; p.least = plan.least; p.n_groups = plan.n_groups; p.prefix_runs = plan.prefix_runs; p.blocks = plan.blocks; p.num_sms = num_sms;
+  p.near = plan.prefix_runs == 0 && c->S <= kNearRows;
+  p.step_cost = c->k_scale != nullptr ? kStepCostFp8 : kStepCost;
   p.scale_log2 = c->scale * 1.4426950408889634f;
   return p;
 }
@@ -655,32 +751,27 @@ extern "C" size_t nrl_decode_scratch(const DecodeCall* c, int n_groups, int max_
 extern "C" cudaError_t nrl_paged_decode_shared(const DecodeCall* c, const int* cu_groups, const int* shared, int n_groups, int max_group, void* scratch, int num_sms,
                                                cudaStream_t s) {
   if (c->S == 0) return cudaSuccess;
-  FlatParams p = flat_params(c, flat_plan(c, n_groups, max_group, num_sms), scratch);
+  FlatParams p = flat_params(c, flat_plan(c, n_groups, max_group, num_sms), scratch, num_sms);
   p.cu_groups = cu_groups; p.shared = shared;
-  launch_dependent(decode_plan_kernel, 1, kPlanThreads, 0, s, p);
-  cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess && p.prefix_runs > 0) e = launch_decode_prefix(p, s);
+  cudaError_t e = launch_plan(p, s);
   if (e == cudaSuccess) e = c->k_scale != nullptr ? launch_flat<true, false>(p, s) : launch_flat<false, false>(p, s);
   if (e != cudaSuccess) return e;
-  launch_dependent(decode_join_kernel<false>, dim3(c->S, c->Hkv), 32 * p.G, 0, s, p);
-  return cudaGetLastError();
+  return launch_join<false>(p, 1, 32 * p.G, s);
 }
 
 extern "C" cudaError_t nrl_paged_decode_scored(const DecodeCall* c, const float* scores_in, long in_row, long in_head, float* scores_out, long out_row, long out_head,
                                                int max_tokens, float decay, float* raw, void* scratch, int num_sms, cudaStream_t s) {
   if (c->S == 0) return cudaSuccess;
-  FlatParams p = flat_params(c, flat_plan(c, 0, 0, num_sms), scratch);
+  FlatParams p = flat_params(c, flat_plan(c, 0, 0, num_sms), scratch, num_sms);
   p.raw = raw; p.scores_in = scores_in; p.scores_out = scores_out;
   p.in_row = in_row; p.in_head = in_head; p.out_row = out_row; p.out_head = out_head;
   p.max_tokens = max_tokens < 16 * c->max_blocks ? max_tokens : 16 * c->max_blocks;
   p.decay = decay;
-  launch_dependent(decode_plan_kernel, 1, kPlanThreads, 0, s, p);
-  cudaError_t e = cudaGetLastError();
+  cudaError_t e = launch_plan(p, s);
   if (e == cudaSuccess) e = c->k_scale != nullptr ? launch_flat<true, true>(p, s) : launch_flat<false, true>(p, s);
   if (e != cudaSuccess) return e;
   p.wide = (reinterpret_cast<uintptr_t>(scores_in) | reinterpret_cast<uintptr_t>(scores_out)) % 16 == 0 && (in_row | in_head | out_row | out_head) % 4 == 0;
   // tokens a block: rows' contexts whole where there are rows enough for the chip
   p.chunk = static_cast<long>(c->S) * c->Hkv >= 2L * num_sms ? 4096 : 1024;
-  launch_dependent(decode_join_kernel<true>, dim3(c->S, c->Hkv * ((p.max_tokens + p.chunk - 1) / p.chunk)), 256, 0, s, p);
-  return cudaGetLastError();
+  return launch_join<true>(p, (p.max_tokens + p.chunk - 1) / p.chunk, 256, s);
 }

@@ -1,19 +1,20 @@
 // Decode attention of rows that share their first tokens: the prefix's part.
 //
 // The query rows of a group (samples x G heads of a kv head) are tiles of up to 64; every key and value of the prefix is read from memory once for a tile.
-// The prefixes' steps of 64 tokens, of all tiles one behind the other, are dealt to the blocks in equal runs (decode_flat.cu: decode_plan), two blocks an SM; a run
-// that meets a tile leaves a part of it, (maximum, sum, unnormalised result), which is decode_join's.
+// The prefixes' steps of 64 tokens, of all tiles one behind the other, are dealt to blocks in equal runs (decode_flat.cu: decode_plan); a run that meets a tile leaves a
+// part of it, (maximum, sum, unnormalised result), which is decode_join's.
 //
-// Block = 4 warps of 16 rows; 4 pages a step through shared memory (cp.async, three stages), mma.sync m16n8k16.  fp8 pages are dequantised on the operand
-// fragments as in attention_decode_fp8.cu.  Bound by issue slots (fp8, 112 rows: 720 instructions a warp and step), with few rows by memory.
+// Block = 4 warps of 16 rows; 4 pages a step through shared memory (cp.async, three stages), mma.sync m16n8k16.  fp8 pages are dequantised on the operand fragments as in
+// attention_decode_fp8.cu.  Bound by the latency of a step (fp8, 96 rows: 2 warps a scheduler, of which one issues in 31 % of the cycles, the tensor pipe 25 %): so an
+// fp8 warp holds the scores of two pages at a time and its queries in shared memory, in 167 registers, for three blocks an SM (32 x 2 x 2000 tokens of 96 rows 46 -> 41 us).
+// Pages turned into f16 tiles once for the block, in place of once for every warp, took as long: what it saves in conversions it waits at one more barrier.
 // On tcgen05, tiles of 128 rows against blocks of 128 keys with two streams of scores and a warpgroup each for their softmax, 13 groups x 4 kv heads x 4096 fp8
 // tokens of 112 rows took 44 us and 64 x 2 x 390 bf16 tokens of 48 rows 21: a tile of few rows costs the tensor pipe as much as a full one, and fp8 pages' way
 // through registers into its tiles competes with the softmax for issue slots.
+#pragma once
 #include "common.cuh"
 #include "decode_runs.cuh"
 #include "fp8_fragments.cuh"
-#include "launch.h"
-#include "per_device.h"
 
 namespace nrl {
 
@@ -27,7 +28,8 @@ struct PreSmem {
   static constexpr int kHalf = FP8 ? 2048 : 4096;                    // K or V of a page
   static constexpr int kPageSize = 2 * kHalf + (FP8 ? 128 : 0);      // K, V, k_scale[16], v_scale[16]
   static constexpr int kStage = kPreStep * kPageSize;
-  static constexpr int kTotal = kPreStages * kStage;
+  static constexpr int kTotal = kPreStages * kStage + (FP8 ? kPrefixRows * 128 * 2 : 0);      // and the tile's queries
+  static constexpr int kPages = FP8 ? 2 : 4;                         // whose scores a warp holds at a time
 };
 
 // Where a run stands: steps [step, step + n) of a tile
@@ -36,9 +38,9 @@ struct PreWalk {
   int first, rows;                                 // the group's first row; query rows of a kv head
   int shared, tiles, steps;                        // tokens; the group's tiles and steps
   int left, at;                                    // steps of the run from this segment on; kv head x tiles + tile
-  NRL_DEVICE explicit PreWalk(const FlatParams& p) {
-    const int4 all = p.groups[p.n_groups], start = p.prefix_starts[blockIdx.x];        // all steps, steps a run
-    left = min(all.y, all.x - static_cast<int>(blockIdx.x) * all.y);
+  NRL_DEVICE PreWalk(const FlatParams& p, int run) {
+    const int4 all = p.groups[p.n_groups], start = p.prefix_starts[run];               // all steps, steps a run
+    left = min(all.y, all.x - run * all.y);
     at = start.y;
     if (left > 0) enter(p, start.x, start.z);
   }
@@ -79,15 +81,13 @@ NRL_DEVICE void pre_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// run `run` of the prefixes, by a whole block
 template <bool FP8>
-__global__ void __launch_bounds__(kPreWarps * 32, 2) decode_prefix_kernel(const FlatParams p) {
-  pdl_wait();
-  pdl_launch_dependents();
+NRL_DEVICE void decode_prefix_run(const FlatParams& p, uint8_t* smem, int run) {
   using L = PreSmem<FP8>;
-  extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
 
-  PreWalk in(p);                                                     // what is copied next: step in.step + in_j
+  PreWalk in(p, run);                                                   // what is copied next: step in.step + in_j
   const int total = max(0, in.left);
   int in_j = 0, n_in = 0, id = 0;                                    // its page numbers, in the lanes
   auto look_up = [&]() {
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 2) decode_prefix_kernel(const 
   issue();
 
   int n_out = 0;
-  for (PreWalk w(p); w.left > 0; w.next(p)) {
+  for (PreWalk w(p, run); w.left > 0; w.next(p)) {
     const int shared = w.shared;
     // this thread's rows: g and g + 8 of the warp's sixteen
     int limit[2];
@@ -144,22 +144,29 @@ __global__ void __launch_bounds__(kPreWarps * 32, 2) decode_prefix_kernel(const 
       limit[i] = real[i] ? min(shared, p.context_lens[seq]) : 0;
       qrow[i] = p.q + seq * p.q_stride_s + (w.h * p.G + r) * 128;
     }
+    int all_see = real[1] ? min(limit[0], limit[1]) : real[0] ? limit[0] : shared;          // what all rows of the warp see
+    all_see = __reduce_min_sync(0xffffffffu, all_see);
     const bool busy = w.tile * kPrefixRows + warp * 16 < w.rows;     // a warp without rows only copies
-    uint32_t qf[8][4];
+    uint32_t qf[FP8 ? 1 : 8][4];                                     // fp8: in shared memory, as the lanes hold them
+    uint4* const q_frags = reinterpret_cast<uint4*>(smem + kPreStages * L::kStage) + warp * 256 + lane;
 #pragma unroll
-    for (int ks = 0; ks < 8; ++ks)
+    for (int ks = 0; ks < 8; ++ks) {
+      uint32_t f[4];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if (FP8) {
           const uint2 raw = *reinterpret_cast<const uint2*>(qrow[i] + (ks >> 2) * 64 + t4 * 16 + (ks & 3) * 4);
           const float2 a = unpack_bf16x2(raw.x), b = unpack_bf16x2(raw.y);
-          qf[ks][i] = real[i] ? pack_f16x2(a.x, a.y) : 0u;
-          qf[ks][2 + i] = real[i] ? pack_f16x2(b.x, b.y) : 0u;
+          f[i] = real[i] ? pack_f16x2(a.x, a.y) : 0u;
+          f[2 + i] = real[i] ? pack_f16x2(b.x, b.y) : 0u;
         } else {
-          qf[ks][i] = real[i] ? *reinterpret_cast<const uint32_t*>(qrow[i] + ks * 16 + t4 * 2) : 0u;
-          qf[ks][2 + i] = real[i] ? *reinterpret_cast<const uint32_t*>(qrow[i] + ks * 16 + 8 + t4 * 2) : 0u;
+          f[i] = real[i] ? *reinterpret_cast<const uint32_t*>(qrow[i] + ks * 16 + t4 * 2) : 0u;
+          f[2 + i] = real[i] ? *reinterpret_cast<const uint32_t*>(qrow[i] + ks * 16 + 8 + t4 * 2) : 0u;
         }
       }
+      if (FP8) q_frags[ks * 32] = make_uint4(f[0], f[1], f[2], f[3]);
+      else qf[FP8 ? 0 : ks][0] = f[0], qf[FP8 ? 0 : ks][1] = f[1], qf[FP8 ? 0 : ks][2] = f[2], qf[FP8 ? 0 : ks][3] = f[3];
+    }
     float o[16][4];
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
@@ -189,26 +196,36 @@ __global__ void __launch_bounds__(kPreWarps * 32, 2) decode_prefix_kernel(const 
       }
       issue();                                                       // into the stage that all have left
       if (!busy) continue;
+#pragma unroll 1
+      for (int u0 = 0; u0 < kPreStep; u0 += L::kPages) {
       // ---- S = Q K^T ----
-      float s[kPreStep * 2][4];
+      float s[L::kPages * 2][4];
 #pragma unroll
-      for (int u = 0; u < kPreStep; ++u) {
-        const uint32_t kb = smem_u32(st + u * L::kPageSize);
+      for (int n = 0; n < 2 * L::kPages; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+      if constexpr (FP8) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) s[2 * u + j][0] = s[2 * u + j][1] = s[2 * u + j][2] = s[2 * u + j][3] = 0.f;
-        if (FP8) {
+        for (int h = 0; h < 2; ++h) {
+          uint4 q[4];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int krow = ((g >> 1) << 2) + 2 * j + (g & 1);
+          for (int i = 0; i < 4; ++i) q[i] = q_frags[(4 * h + i) * 32];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint4 w4 = lds128(kb + krow * 128 + (((4 * h + t4) ^ k_sigma(g)) << 4));
+          for (int u = 0; u < L::kPages; ++u)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int krow = ((g >> 1) << 2) + 2 * j + (g & 1);
+              const uint4 w4 = lds128(smem_u32(st + (u0 + u) * L::kPageSize) + krow * 128 + (((4 * h + t4) ^ k_sigma(g)) << 4));
               const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
-              for (int i = 0; i < 4; ++i) pre_mma<true>(s[2 * u + j], qf[4 * h + i], e4m3x2_to_f16x2(w[i] & 0xFFFFu), e4m3x2_to_f16x2(w[i] >> 16));
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t a[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+                pre_mma<true>(s[2 * u + j], a, e4m3x2_to_f16x2(w[i] & 0xFFFFu), e4m3x2_to_f16x2(w[i] >> 16));
+              }
             }
-          }
-        } else {
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < L::kPages; ++u) {
+          const uint32_t kb = smem_u32(st + (u0 + u) * L::kPageSize);
           const int mrow = (lane & 7) + (lane >> 4) * 8, mcol = (lane >> 3) & 1;
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks) {
@@ -220,24 +237,28 @@ __global__ void __launch_bounds__(kPreWarps * 32, 2) decode_prefix_kernel(const 
         }
       }
       // ---- scale, mask, online softmax on rows g and g + 8.  Key of column (u, j, e): bf16 16 u + 8 j + 2 t + e, fp8 16 u + 4 t + 2 j + e ----
-      float vsc[kPreStep][4];
+      float vsc[L::kPages][4];
       float top[2] = {-INFINITY, -INFINITY};
+      const bool whole = key0 + kPrefixKeys <= all_see;
 #pragma unroll
-      for (int u = 0; u < kPreStep; ++u) {
+      for (int u = 0; u < L::kPages; ++u) {
         float ksc[4] = {1.f, 1.f, 1.f, 1.f};
         if (FP8) {
-          const uint32_t sb = smem_u32(st + u * L::kPageSize + 2 * L::kHalf);
+          const uint32_t sb = smem_u32(st + (u0 + u) * L::kPageSize + 2 * L::kHalf);
           const uint4 kr = lds128(sb + t4 * 16), vr = lds128(sb + 64 + t4 * 16);
-          ksc[0] = __uint_as_float(kr.x); ksc[1] = __uint_as_float(kr.y); ksc[2] = __uint_as_float(kr.z); ksc[3] = __uint_as_float(kr.w);
-          vsc[u][0] = __uint_as_float(vr.x); vsc[u][1] = __uint_as_float(vr.y); vsc[u][2] = __uint_as_float(vr.z); vsc[u][3] = __uint_as_float(vr.w);
+          ksc[0] = __uint_as_float(kr.x) * p.scale_log2; ksc[1] = __uint_as_float(kr.y) * p.scale_log2;
+          ksc[2] = __uint_as_float(kr.z) * p.scale_log2; ksc[3] = __uint_as_float(kr.w) * p.scale_log2;
+          vsc[u][0] = __uint_as_float(vr.x) * kPreScale; vsc[u][1] = __uint_as_float(vr.y) * kPreScale;
+          vsc[u][2] = __uint_as_float(vr.z) * kPreScale; vsc[u][3] = __uint_as_float(vr.w) * kPreScale;
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int key = key0 + u * 16 + (FP8 ? t4 * 4 + 2 * j + (e & 1) : j * 8 + t4 * 2 + (e & 1));
+            const int key = key0 + (u0 + u) * 16 + (FP8 ? t4 * 4 + 2 * j + (e & 1) : j * 8 + t4 * 2 + (e & 1));
             float& x = s[2 * u + j][e];
-            x = key < limit[e >> 1] ? x * (ksc[2 * j + (e & 1)] * p.scale_log2) : -INFINITY;
+            x *= FP8 ? ksc[2 * j + (e & 1)] : p.scale_log2;
+            if (!whole && key >= limit[e >> 1]) x = -INFINITY;
             top[e >> 1] = fmaxf(top[e >> 1], x);
           }
       }
@@ -251,25 +272,27 @@ __global__ void __launch_bounds__(kPreWarps * 32, 2) decode_prefix_kernel(const 
         corr[i] = exp2f(m_run[i] - m_sub[i]);                          // 0 while nothing has been seen
         m_run[i] = m_new;
       }
-      uint32_t pa[kPreStep][4];
+      uint32_t pa[L::kPages][4];
 #pragma unroll
-      for (int u = 0; u < kPreStep; ++u)
+      for (int u = 0; u < L::kPages; ++u)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const float p0 = exp2f(s[2 * u + j][2 * i] - m_sub[i]), p1 = exp2f(s[2 * u + j][2 * i + 1] - m_sub[i]);
             sum[i] += p0 + p1;
-            pa[u][2 * j + i] = FP8 ? pack_f16x2(p0 * (vsc[u][2 * j] * kPreScale), p1 * (vsc[u][2 * j + 1] * kPreScale)) : pack_bf16x2(p0, p1);
+            pa[u][2 * j + i] = FP8 ? pack_f16x2(p0 * vsc[u][2 * j], p1 * vsc[u][2 * j + 1]) : pack_bf16x2(p0, p1);
           }
 #pragma unroll
       for (int i = 0; i < 2; ++i) l_run[i] = l_run[i] * corr[i] + sum[i];
+      if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) { o[i][0] *= corr[0]; o[i][1] *= corr[0]; o[i][2] *= corr[1]; o[i][3] *= corr[1]; }
+        for (int i = 0; i < 16; ++i) { o[i][0] *= corr[0]; o[i][1] *= corr[0]; o[i][2] *= corr[1]; o[i][3] *= corr[1]; }
+      }
       // ---- O += P V ----
 #pragma unroll
-      for (int u = 0; u < kPreStep; ++u) {
-        const uint32_t vb = smem_u32(st + u * L::kPageSize + L::kHalf);
+      for (int u = 0; u < L::kPages; ++u) {
+        const uint32_t vb = smem_u32(st + (u0 + u) * L::kPageSize + L::kHalf);
         if (FP8) {
 #pragma unroll
           for (int nd = 0; nd < 16; ++nd) {
@@ -287,6 +310,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 2) decode_prefix_kernel(const 
           }
         }
       }
+      }
     }
     // ---- the part of every row; one without keys is (-inf, 0, 0) ----
 #pragma unroll
@@ -294,7 +318,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 2) decode_prefix_kernel(const 
       l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 1);
       l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 2);
       if (!real[i]) continue;
-      const long at = prefix_part_row(p, w.first, w.h, w.rows, w.tile * kPrefixRows + warp * 16 + g + i * 8) + static_cast<long>(kPrefixRows) * blockIdx.x;
+      const long at = prefix_part_row(p, w.first, w.h, w.rows, w.tile * kPrefixRows + warp * 16 + g + i * 8) + static_cast<long>(kPrefixRows) * run;
       float* dst = p.prefix_o + at * 128 + t4 * 2;
 #pragma unroll
       for (int nd = 0; nd < 16; ++nd)
@@ -304,20 +328,5 @@ __global__ void __launch_bounds__(kPreWarps * 32, 2) decode_prefix_kernel(const 
   }
   cp_async_wait<0>();
 }
-
-namespace {
-
-template <bool FP8>
-cudaError_t launch_prefix(const FlatParams& p, cudaStream_t s) {
-  static PerDevice<bool> configured;
-  const cudaError_t e = allow_smem(configured, decode_prefix_kernel<FP8>, PreSmem<FP8>::kTotal);
-  if (e != cudaSuccess) return e;
-  launch_dependent(decode_prefix_kernel<FP8>, p.prefix_runs, kPreWarps * 32, PreSmem<FP8>::kTotal, s, p);
-  return cudaGetLastError();
-}
-
-}  // namespace
-
-cudaError_t launch_decode_prefix(const FlatParams& p, cudaStream_t s) { return p.ks != nullptr ? launch_prefix<true>(p, s) : launch_prefix<false>(p, s); }
 
 }  // namespace nrl

@@ -1,4 +1,4 @@
-// What decode_flat.cu and decode_prefix.cu share: the parameters of a decode call, and where parts lie.
+// What decode_flat.cu and decode_prefix.cuh share: the parameters of a decode call, and where parts lie.
 #pragma once
 #include "common.cuh"
 
@@ -25,7 +25,8 @@ struct FlatParams {
   const float* scores_in;
   float* scores_out;
   long q_stride_s, in_row, in_head, out_row, out_head;
-  int n_groups, prefix_runs, blocks, S, max_blocks, Hq, Hkv, G, runs, least, max_tokens, chunk, wide;
+  int n_groups, prefix_runs, blocks, S, max_blocks, Hq, Hkv, G, runs, least, max_tokens, chunk, wide, num_sms, near;
+  int step_cost;                // of a step of a prefix, in pages of a row
   float scale_log2, decay;
 };
 
@@ -34,8 +35,5 @@ NRL_DEVICE int flat_context(const FlatParams& p, int s) { return max(0, min(p.co
 NRL_DEVICE long prefix_part_row(const FlatParams& p, int first, int h, int rows, int row) {
   return static_cast<long>(first) * p.G * p.Hkv + static_cast<long>(h) * rows + row;
 }
-
-// the prefixes' parts (decode_prefix.cu)
-cudaError_t launch_decode_prefix(const FlatParams& p, cudaStream_t s);
 
 }  // namespace nrl

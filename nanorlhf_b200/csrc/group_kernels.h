@@ -39,6 +39,7 @@ struct EvictCall {
   float* kept_scores;                     // [S, Hkv, keep]
   int* new_lens;                          // [S]
   unsigned* bits;                         // [S, Hkv, ceil(max_tokens / 32)] of scratch: a bit a token that is kept
+  uint4* told;                            // [S, Hkv, 32] of scratch: what the blocks of a row-head tell one another
   int S, Hkv, max_blocks, out_blocks, max_tokens, keep, sinks, recent;
 };
 cudaError_t nrl_kv_evict(const EvictCall* c, int num_sms, cudaStream_t s);

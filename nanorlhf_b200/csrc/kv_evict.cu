@@ -3,16 +3,15 @@
 //
 // kv_select: a cluster of blocks per (row, kv head), more blocks where there are few and their contexts long.  A block has a range of tokens; their scores, as whole
 // numbers whose order is theirs, wait in shared memory.  The smallest kept one is found three bits at a time: a thread counts the eight digits of the keys that may still be it
-// in the bytes of two words, warps, the block and the cluster add up, until as many keys are at or above a digit as are to be kept.  Then the tokens are
+// in the bytes of two words, warps, the block and (through memory) the cluster add up, until as many keys are at or above a digit as are to be kept.  Then the tokens are
 // counted again, word by word of 32, and indices and a bit a token are written in order.  Bound by latency, up to eleven rounds of a barrier (and one of the cluster).
 // (Counts of digits by atomics in shared memory meet: a score's highest bits are a few exponents, and 3750 tokens a block took 120 us with eight bits a round, 20 with eleven;
 // seven votes a word and round 20.)
 // kv_move: a block per (row, kv head, slice of a token's keys or values), and per range of places where sources and targets are apart.  In place, token j of what
 // is kept comes from a place >= j, so that a block that reads a range of places before it writes them, ranges in order and the next one on its way, may move it;
 // other slices' bytes are not touched.
-// kv_move_transposed, beside it: values of fp8 pages lie transposed.  Sixteen pages at a time go through shared memory, rows of 16 bytes 20 apart (no bank
+// Values of fp8 pages lie transposed, and their blocks come first, for they take longest (in a launch in front of the others' 69 us, in one 60).  Sixteen pages at a time go through shared memory, rows of 16 bytes 20 apart (no bank
 // conflicts), and a thread puts together an element's bytes of a whole page.
-#include "cluster_read.h"
 #include "common.cuh"
 #include "group_kernels.h"
 #include "launch.h"
@@ -48,8 +47,6 @@ __global__ void __launch_bounds__(WARPS * 32) kv_select_kernel(const EvictCall p
   pdl_launch_dependents();
   extern __shared__ uint32_t keys[];
   __shared__ __align__(16) uint4 warp_counts[2][kSelWarps];           // of two rounds in turn: eight counts of 16 bits
-  __shared__ __align__(16) uint4 counts[2][2];                        // the block's; others may still read the last round's
-  __shared__ __align__(16) uint4 total;
   __shared__ uint2 warp_sums[kSelWarps];
   const int seq = blockIdx.x / cluster, rank = blockIdx.x - seq * cluster, kvh = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int n = max(0, min(p.context_lens[seq], p.max_tokens));
@@ -57,6 +54,8 @@ __global__ void __launch_bounds__(WARPS * 32) kv_select_kernel(const EvictCall p
   int* kept = p.kept + row * p.keep;
   const float* sc = p.scores + seq * p.score_row + kvh * p.score_head;
   uint32_t* bits = p.bits + row * ((p.max_tokens + 31) / 32);
+  // a cluster's blocks tell one another their counts, 32 bytes a block; of two rounds in turn: others may still read the last one's
+  uint4* const told = p.told + row * (4 * kSelCluster);
   if (kvh == 0 && rank == 0 && tid == 0) p.new_lens[seq] = min(n, p.keep);
   if (n <= p.keep) {
     const int at = rank * kSelThreads + tid, step = cluster * kSelThreads;
@@ -104,13 +103,11 @@ __global__ void __launch_bounds__(WARPS * 32) kv_select_kernel(const EvictCall p
       c = add(lane < kSelWarps ? warp_counts[round & 1][lane] : make_uint4(0, 0, 0, 0), kSelWarps / 2);
       uint32_t n_of[8] = {c.x & 0xffffu, c.y & 0xffffu, c.x >> 16, c.y >> 16, c.z & 0xffffu, c.w & 0xffffu, c.z >> 16, c.w >> 16};
       if (cluster > 1) {
-        if (tid < 2) counts[round & 1][tid] = tid == 0 ? make_uint4(n_of[0], n_of[1], n_of[2], n_of[3]) : make_uint4(n_of[4], n_of[5], n_of[6], n_of[7]);
+        uint4* const here = told + (round & 1) * 2 * kSelCluster;
+        if (tid < 2) here[rank * 2 + tid] = tid == 0 ? make_uint4(n_of[0], n_of[1], n_of[2], n_of[3]) : make_uint4(n_of[4], n_of[5], n_of[6], n_of[7]);
         evict_cluster_sync();
         uint4 x = make_uint4(0, 0, 0, 0);                             // lane i + 8 j: half j of block i's
-        if ((lane & 7) < cluster && lane < 16) {
-          const float4 v = ld_cluster_f4(smem_u32(&counts[round & 1][lane >> 3]), lane & 7);
-          x = make_uint4(__float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w));
-        }
+        if ((lane & 7) < cluster && lane < 16) x = __ldcg(here + (lane & 7) * 2 + (lane >> 3));
         x = add(x, kSelCluster / 2);
         const uint32_t mine[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -152,19 +149,22 @@ __global__ void __launch_bounds__(WARPS * 32) kv_select_kernel(const EvictCall p
   }
   if (lane == 0) warp_sums[warp] = make_uint2(more, same);
   __syncthreads();
-  if (tid == 0) {
-    uint4 all = make_uint4(0, 0, 0, 0);
-    for (int w = 0; w < kSelWarps; ++w) { all.x += warp_sums[w].x; all.y += warp_sums[w].y; }
-    total = all;
-  }
-  evict_cluster_sync();
+  uint2 all = make_uint2(0, 0);
+  for (int w = 0; w < kSelWarps; ++w) { all.x += warp_sums[w].x; all.y += warp_sums[w].y; }
   uint32_t need = p.keep;
   more = same = 0;
-  for (int r = 0; r < cluster; ++r) {
-    const float4 v = ld_cluster_f4(smem_u32(&total), r);
-    need -= __float_as_uint(v.x);
-    more += r < rank ? __float_as_uint(v.x) : 0u;
-    same += r < rank ? __float_as_uint(v.y) : 0u;
+  if (cluster > 1) {
+    evict_cluster_sync();                                             // (both rounds' counts have been read)
+    if (tid == 0) told[rank] = make_uint4(all.x, all.y, 0, 0);
+    evict_cluster_sync();
+    for (int r = 0; r < cluster; ++r) {
+      const uint4 v = __ldcg(told + r);
+      need -= v.x;
+      more += r < rank ? v.x : 0u;
+      same += r < rank ? v.y : 0u;
+    }
+  } else {
+    need -= all.x;
   }
   for (int w = 0; w < warp; ++w) { more += warp_sums[w].x; same += warp_sums[w].y; }
   const uint32_t under = (1u << lane) - 1;
@@ -182,7 +182,6 @@ __global__ void __launch_bounds__(WARPS * 32) kv_select_kernel(const EvictCall p
     more += __popc(a);
     same += __popc(b);
   }
-  evict_cluster_sync();                                               // a block's shared memory is read up to here
 }
 
 // ---- tokens' rows: 16-byte pieces of keys (and of bf16 values), and their scales ---------------------------------------------------------------------
@@ -331,16 +330,14 @@ NRL_DEVICE MoveRow move_row(const MoveParams& p) {
   return {e.block_tables + static_cast<long>(seq) * e.max_blocks, p.out_tables + static_cast<long>(seq) * p.out_blocks, e.kept + row * e.keep, row, kvh, j0, j1};
 }
 
-// keys and bf16 values, the scales of fp8 ones, and the scores of what is kept.  It takes nothing from kv_move_transposed, whose blocks had all begun when this one does;
-// its end waits for theirs.
-template <bool IN_PLACE>
+// A block has, by z: the values of fp8 pages, which take longest; a slice of the keys; of bf16 values; fp8 scales; the scores of what is kept.
+template <bool IN_PLACE, bool FP8>
 __global__ void __launch_bounds__(kMoveThreads, IN_PLACE ? 2 : 4) kv_move_kernel(const MoveParams p) {
-  const EvictCall& e = p.e;
-  const bool fp8 = e.k_scale != nullptr;
-  if (!fp8) pdl_wait();
+  pdl_wait();
   pdl_launch_dependents();
+  const EvictCall& e = p.e;
   const MoveRow m = move_row<IN_PLACE>(p);
-  const int z = blockIdx.z, last = fp8 ? p.key_slices + 2 : 2 * p.key_slices;
+  const int z = static_cast<int>(blockIdx.z) - (FP8 ? 1 : 0), last = FP8 ? p.key_slices + 2 : 2 * p.key_slices;
   if (z == last) {
     float* to = e.kept_scores + m.row * e.keep;
     const float* sc = e.scores + static_cast<long>(blockIdx.x) * e.score_row + m.kvh * e.score_head;
@@ -350,27 +347,22 @@ __global__ void __launch_bounds__(kMoveThreads, IN_PLACE ? 2 : 4) kv_move_kernel
       const int t = m.kept[j];
       to[j] = t >= 0 ? sc[t] : 0.f;
     }
-  } else if (m.j0 < m.j1) {
-    const bool keys = z < p.key_slices;
-    if (fp8 && !keys)
-      move_rows<IN_PLACE, float, 1>(z == p.key_slices ? e.k_scale : e.v_scale, 1, 0, m.from, m.to, m.kept, m.j0, m.j1, e.Hkv, m.kvh);
-    else
-      move_rows<IN_PLACE, uint4, kMovePieces>(static_cast<uint4*>(keys ? e.k_cache : e.v_cache), fp8 ? 8 : 16, keys ? z : z - p.key_slices, m.from, m.to, m.kept, m.j0, m.j1,
-                                              e.Hkv, m.kvh);
+    return;
   }
-  if (fp8) pdl_wait();
-}
-
-// values of fp8 pages
-template <bool IN_PLACE>
-__global__ void __launch_bounds__(kMoveThreads, 4) kv_move_transposed_kernel(const MoveParams p) {
-  pdl_wait();
-  pdl_launch_dependents();
-  const EvictCall& e = p.e;
-  const MoveRow m = move_row<IN_PLACE>(p);
   if (m.j0 >= m.j1) return;
-  const uint16_t* bits = reinterpret_cast<const uint16_t*>(e.bits + m.row * ((e.max_tokens + 31) / 32));
-  move_transposed(static_cast<uint4*>(e.v_cache) + static_cast<long>(m.kvh) * 128, static_cast<long>(e.Hkv) * 128, m.from, m.to, m.kept, bits, m.j0, m.j1);
+  if constexpr (FP8) {
+    if (z < 0) {
+      const uint16_t* bits = reinterpret_cast<const uint16_t*>(e.bits + m.row * ((e.max_tokens + 31) / 32));
+      move_transposed(static_cast<uint4*>(e.v_cache) + static_cast<long>(m.kvh) * 128, static_cast<long>(e.Hkv) * 128, m.from, m.to, m.kept, bits, m.j0, m.j1);
+      return;
+    }
+  }
+  const bool keys = z < p.key_slices;
+  if (FP8 && !keys)
+    move_rows<IN_PLACE, float, 1>(z == p.key_slices ? e.k_scale : e.v_scale, 1, 0, m.from, m.to, m.kept, m.j0, m.j1, e.Hkv, m.kvh);
+  else
+    move_rows<IN_PLACE, uint4, kMovePieces>(static_cast<uint4*>(keys ? e.k_cache : e.v_cache), FP8 ? 8 : 16, keys ? z : z - p.key_slices, m.from, m.to, m.kept, m.j0, m.j1,
+                                            e.Hkv, m.kvh);
 }
 
 }  // namespace nrl
@@ -393,12 +385,9 @@ cudaError_t launch_moves(const MoveParams& p, cudaStream_t s) {
   const EvictCall& c = p.e;
   const bool fp8 = c.k_scale != nullptr;
   const int places = c.keep < c.max_tokens ? c.keep : c.max_tokens, ranges = IN_PLACE ? 1 : (places + kMoveRange - 1) / kMoveRange;
-  if (fp8) {
-    launch_dependent(kv_move_transposed_kernel<IN_PLACE>, dim3(c.S, c.Hkv * ranges), kMoveThreads, 0, s, p);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-  }
-  launch_dependent(kv_move_kernel<IN_PLACE>, dim3(c.S, c.Hkv * ranges, (fp8 ? p.key_slices + 2 : 2 * p.key_slices) + 1), kMoveThreads, 0, s, p);
+  const dim3 grid(c.S, c.Hkv * ranges, (fp8 ? p.key_slices + 3 : 2 * p.key_slices) + 1);
+  if (fp8) launch_dependent(kv_move_kernel<IN_PLACE, true>, grid, kMoveThreads, 0, s, p);
+  else launch_dependent(kv_move_kernel<IN_PLACE, false>, grid, kMoveThreads, 0, s, p);
   return cudaGetLastError();
 }
 

@@ -490,15 +490,15 @@ def attention_shared_prefix(q, k, v, cu_seqlens, cu_groups, scale):
 
 
 def paged_decode_shared(*args):
-    _count(4)
+    _count(2)                                    # (a third one makes the plan of many rows)
     return ext().paged_decode_shared(*args)
 
 
 def paged_decode_scored(*args):
-    _count(3)
+    _count(2)
     return ext().paged_decode_scored(*args)
 
 
 def kv_evict(*args):
-    _count(3)
+    _count(2)
     return ext().kv_evict(*args)
