@@ -70,6 +70,13 @@ class RLConfig:
     kv_cache_dtype: str = "fp8"                 # sampler KV pages: fp8 (e4m3 + per-token scales: half the bytes of the HBM-bound
                                                 # decode attention, 1.6x faster, 2x capacity) | bf16.  Old log-probs are always
                                                 # recomputed by the bf16 training engine, so this only shapes the samples.
+    shared_decode: bool = False                 # sampler: attention reads the prompt pages that samples share once for all of them; pays for long
+                                                # prompts of many samples (32 x 16 rows of 2000 + 128 bf16 tokens 106 -> 62 us a layer, 128 x 8 of
+                                                # 200 + 800 144 -> 164)
+    kv_budget: int = 0                          # sampler: most cached tokens of a row between two evictions, 0: all of them.  Tokens that
+                                                # little attention went to are given up; as kv_cache_dtype, it only shapes the samples
+    kv_sinks: int = 4                           # of them, the row's first
+    kv_recent: Optional[int] = None             # and its newest (None: a quarter of the budget)
     sampler: str = "auto"                       # auto | native | torch
     kv_block_size: int = 16
 
@@ -93,6 +100,8 @@ class RLConfig:
     token_budget_fwd: int = 22 * 2316           # padded-token budget of a no-grad forward (:534)
     token_budget_train: int = 4 * 2316          # r1 micro-bucket budget (grpo_r1_trainer.py:700)
     train_samples_per_prompt: int = 1           # GRPO/RLOO keep 1 random of N (grpo_trainer.py:504)
+    share_prompts: bool = False                 # log-prob passes and micro-steps compute the query of rows that share one once
+                                                # (Qwen2 models; on CUDA bf16, heads of 128); rows of a query are put together
     stats_include_padding: bool = False         # parity: entropy/approxkl over padded positions
     grpo_std_eps: float = 0.0
     num_sample_generations: int = 0

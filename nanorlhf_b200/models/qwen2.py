@@ -127,7 +127,7 @@ class Qwen2Attention(nn.Module):
         self.v_proj = Linear(d, cfg.num_key_value_heads * hd, bias=cfg.attention_bias)
         self.o_proj = Linear(cfg.num_attention_heads * hd, d, bias=False)
 
-    def forward(self, x, cos, sin, cu_seqlens, max_seqlen):
+    def forward(self, x, cos, sin, cu_seqlens, max_seqlen, cu_groups=None):
         cfg = self.cfg
         T = x.shape[0]
         from .lora import lora_group_forward
@@ -137,7 +137,10 @@ class Qwen2Attention(nn.Module):
         v = v.view(T, cfg.num_key_value_heads, cfg.head_dim)
         q = ops.apply_rope(q, cos, sin)
         k = ops.apply_rope(k, cos, sin)
-        o = ops.attention_varlen(q, k, v, cu_seqlens, max_seqlen, causal=True)
+        if cu_groups is not None:                      # sequences that continue the first one of their group (build_logprob_plan)
+            o = ops.attention_shared_prefix(q, k, v, cu_seqlens, cu_groups, max_seqlen)
+        else:
+            o = ops.attention_varlen(q, k, v, cu_seqlens, max_seqlen, causal=True)
         return self.o_proj(o.reshape(T, -1))
 
 
@@ -173,9 +176,9 @@ class Qwen2DecoderLayer(nn.Module):
         self.input_layernorm = RMSNorm(cfg.hidden_size, cfg.rms_norm_eps)
         self.post_attention_layernorm = RMSNorm(cfg.hidden_size, cfg.rms_norm_eps)
 
-    def forward(self, h, cos, sin, cu_seqlens, max_seqlen):
+    def forward(self, h, cos, sin, cu_seqlens, max_seqlen, cu_groups=None):
         from .lora import plain_module
-        a = self.self_attn(self.input_layernorm(h), cos, sin, cu_seqlens, max_seqlen)
+        a = self.self_attn(self.input_layernorm(h), cos, sin, cu_seqlens, max_seqlen, cu_groups)
         norm = self.post_attention_layernorm
         if (ops.direct_calls() and ops.use_native(h) and h.dim() == 2 and plain_module(norm, RMSNorm)
                 and h.dtype == a.dtype == norm.weight.dtype == torch.bfloat16):
@@ -195,8 +198,9 @@ class Qwen2Model(nn.Module):
         self.norm = RMSNorm(cfg.hidden_size, cfg.rms_norm_eps)
         self.gradient_checkpointing = False
 
-    def forward(self, input_ids, cu_seqlens, position_ids, max_seqlen=None):
-        """input_ids/position_ids: [T] packed; cu_seqlens: [S+1] int32.  Returns hidden [T, d]."""
+    def forward(self, input_ids, cu_seqlens, position_ids, max_seqlen=None, cu_groups=None):
+        """input_ids/position_ids: [T] packed; cu_seqlens: [S+1] int32; cu_groups: groups of sequences whose first is the
+        prefix of its others (``ops.attention_shared_prefix``).  Returns hidden [T, d]."""
         h = self.embed_tokens(input_ids)
         cos, sin = ops.ref.rope_cos_sin(position_ids, self.cfg.head_dim, self.cfg.rope_theta)
         ckpt = self.gradient_checkpointing and self.training and torch.is_grad_enabled()
@@ -206,10 +210,10 @@ class Qwen2Model(nn.Module):
             h = h.detach().requires_grad_(True)
         for layer in self.layers:
             if ckpt:
-                h = torch.utils.checkpoint.checkpoint(layer, h, cos, sin, cu_seqlens, max_seqlen,
+                h = torch.utils.checkpoint.checkpoint(layer, h, cos, sin, cu_seqlens, max_seqlen, cu_groups,
                                                       use_reentrant=False)
             else:
-                h = layer(h, cos, sin, cu_seqlens, max_seqlen)
+                h = layer(h, cos, sin, cu_seqlens, max_seqlen, cu_groups)
         return self.norm(h)
 
 
@@ -320,8 +324,8 @@ class Qwen2ForCausalLM(Qwen2PreTrained):
         if self.lm_head.weight is self.model.embed_tokens.weight:
             self.lm_head.weight = nn.Parameter(self.model.embed_tokens.weight.detach().clone())
 
-    def hidden_states(self, input_ids, cu_seqlens, position_ids, max_seqlen=None):
-        return self.model(input_ids, cu_seqlens, position_ids, max_seqlen)
+    def hidden_states(self, input_ids, cu_seqlens, position_ids, max_seqlen=None, cu_groups=None):
+        return self.model(input_ids, cu_seqlens, position_ids, max_seqlen, cu_groups)
 
     def logits(self, hidden):
         """Materialised logits -- API-edge / tests / CPU sampler only; never on the hot path."""
@@ -355,8 +359,8 @@ class Qwen2ForSequenceClassification(Qwen2PreTrained):
         self.model = Qwen2Model(cfg)
         self.score = nn.Linear(cfg.hidden_size, cfg.num_labels, bias=False)
 
-    def hidden_states(self, input_ids, cu_seqlens, position_ids, max_seqlen=None):
-        return self.model(input_ids, cu_seqlens, position_ids, max_seqlen)
+    def hidden_states(self, input_ids, cu_seqlens, position_ids, max_seqlen=None, cu_groups=None):
+        return self.model(input_ids, cu_seqlens, position_ids, max_seqlen, cu_groups)
 
     def values(self, hidden):
         return self.score(hidden).squeeze(-1).float()
@@ -411,14 +415,56 @@ def forward(model, query_responses: torch.Tensor, pad_token_id: int):
     return (out.view(B, L, -1),)
 
 
-def build_logprob_plan(query_responses: torch.Tensor, context_length: int, pad_token_id: int) -> dict:
+def _pack_shared(query_responses: torch.Tensor, context_length: int, pad_token_id: int):
+    """``pack_padded`` for rows of which several answer one query: (ids, cu, pos, max_seqlen, flat_index, cu_groups), or None if all queries differ.
+
+    Rows of one query become a group (rows are packed by query, whatever their order): its first sequence is the query but for
+    its last column, once; the others are each row's last query column and response.  So every position that predicts a token of
+    a response, or whose value counts, is in the sequence of its own row.
+    """
+    B, L = query_responses.shape
+    cut = context_length - 1
+    if B < 2 or cut < 1:
+        return None
+    dev = query_responses.device
+    prompt, sizes = torch.unique(query_responses[:, :context_length], dim=0, return_inverse=True, return_counts=True)[1:]
+    G = sizes.numel()
+    if G == B:
+        return None
+    order = torch.argsort(prompt, stable=True)
+    prompt = prompt[order]
+    mask = (query_responses != pad_token_id)[order]
+    first = torch.ones(B, dtype=torch.bool, device=dev)
+    first[1:] = prompt[1:] != prompt[:-1]
+    alone = sizes[prompt] == 1
+    shared, lens = mask[:, :cut].sum(1), mask.sum(1)
+    # a row gives one sequence, and the first row of a query with several also the one that they share, before its own
+    each = torch.stack([shared, torch.where(alone, lens, lens - shared)], 1)
+    there = torch.stack([first & ~alone, torch.ones_like(first)], 1)
+    seq = each[there]
+    cu = torch.zeros(seq.numel() + 1, dtype=torch.int32, device=dev)
+    cu[1:] = seq.cumsum(0)
+    cu_groups = torch.zeros(G + 1, dtype=torch.int32, device=dev)
+    cu_groups[1:] = (sizes + (sizes > 1)).cumsum(0)
+    packed = mask.clone()
+    packed[:, :cut] &= first[:, None]
+    at = packed.view(-1).nonzero(as_tuple=False).squeeze(1)
+    flat_index = order[at // L] * L + at % L
+    ids = query_responses.reshape(-1)[flat_index]
+    pos = (mask.long().cumsum(1) - 1).reshape(-1)[at]
+    return ids, cu, pos, int(lens.max().item()), flat_index, cu_groups
+
+
+def build_logprob_plan(query_responses: torch.Tensor, context_length: int, pad_token_id: int, share_prompts: bool = False) -> dict:
     """Host-synchronising part of ``response_logprobs``: packing indices and the (source row -> response slot) map.
 
     ``src[i]`` is the packed position whose hidden state predicts ``targets[i]``; the result lands in
-    slot ``(r[i], c[i])`` of the [B, T_r] output.
+    slot ``(r[i], c[i])`` of the [B, T_r] output.  With ``share_prompts`` the query of rows that have the same one is packed
+    once, and ``cu_groups`` says which sequences continue it (None: no two rows have the same).
     """
     B, L = query_responses.shape
-    ids, cu, pos, mx, flat = pack_padded(query_responses, pad_token_id)
+    shared = _pack_shared(query_responses, context_length, pad_token_id) if share_prompts else None
+    ids, cu, pos, mx, flat, cu_groups = shared or pack_padded(query_responses, pad_token_id) + (None,)
     # packed token at flat position (b, l) predicts target (b, l+1); needed when l+1 >= ctx
     col = flat % L
     row = flat // L
@@ -430,7 +476,14 @@ def build_logprob_plan(query_responses: torch.Tensor, context_length: int, pad_t
     src = pred.nonzero(as_tuple=False).squeeze(1)
     targets = query_responses.reshape(-1)[flat[src] + 1]
     return {"ids": ids, "cu": cu, "pos": pos, "max_seqlen": mx, "flat": flat, "col": col, "row": row, "src": src,
-            "targets": targets, "r": row[src], "c": col[src] + 1 - context_length}
+            "targets": targets, "r": row[src], "c": col[src] + 1 - context_length, "cu_groups": cu_groups}
+
+
+def planned_hidden_states(lm, plan: dict, max_seqlen=None):
+    """Hidden states [T, d] of a plan's packed tokens."""
+    args = (plan["ids"], plan["cu"], plan["pos"], max_seqlen or plan["max_seqlen"])
+    groups = plan.get("cu_groups")
+    return lm.hidden_states(*args) if groups is None else lm.hidden_states(*args, cu_groups=groups)
 
 
 def planned_response_logprobs(lm, plan: dict, B: int, T_r: int, temperature: float, want_entropy: bool,
@@ -439,7 +492,7 @@ def planned_response_logprobs(lm, plan: dict, B: int, T_r: int, temperature: flo
     extra ``src`` entries must carry ``r == B`` (a dump row that is sliced off)."""
     dev = plan["ids"].device
     if hidden is None:
-        hidden = lm.hidden_states(plan["ids"], plan["cu"], plan["pos"], max_seqlen or plan["max_seqlen"])
+        hidden = planned_hidden_states(lm, plan, max_seqlen)
     logp, ent = lm.token_logprobs(hidden.index_select(0, plan["src"]), plan["targets"], temperature, want_entropy)
     out_lp = torch.full((B + 1, T_r), invalid_value, dtype=torch.float32, device=dev)
     out_lp = out_lp.index_put((plan["r"], plan["c"]), logp)[:B]
@@ -451,7 +504,7 @@ def planned_response_logprobs(lm, plan: dict, B: int, T_r: int, temperature: flo
 
 def response_logprobs(lm, query_responses: torch.Tensor, context_length: int, pad_token_id: int,
                       temperature: float, want_entropy: bool = False, invalid_value: float = 1.0,
-                      value_model=None):
+                      value_model=None, share_prompts: bool = False):
     """Per-token log-probs of the response part, [B, T_r], via the fused lm-head op.
 
     Position j of the result is log p(response[j] | everything before), i.e. the reference's
@@ -461,19 +514,19 @@ def response_logprobs(lm, query_responses: torch.Tensor, context_length: int, pa
     If ``value_model`` is given also returns values [B, T_r] aligned the same way (PPO
     ``get_reward(...)[0][:, ctx-1:-1]``, PPO/ppo_trainer.py:630-634): values[j] is the critic's
     output at column ctx-1+j, so values[seq_len+1] is the value of the post-EOS state.
+    ``share_prompts``: rows with the same query compute it once (on CUDA bf16, heads of 128).
     Returns (logp, entropy[, values]).
     """
     B, L = query_responses.shape
     T_r = L - context_length
     dev = query_responses.device
-    plan = build_logprob_plan(query_responses, context_length, pad_token_id)
+    plan = build_logprob_plan(query_responses, context_length, pad_token_id, share_prompts)
     out_lp, out_ent, hidden = planned_response_logprobs(lm, plan, B, T_r, temperature, want_entropy, invalid_value)
     result = [out_lp, out_ent]
     if value_model is not None:
         col, row = plan["col"], plan["row"]
-        ids, cu, pos, mx = plan["ids"], plan["cu"], plan["pos"], plan["max_seqlen"]
         vsel = ((col >= context_length - 1) & (col <= L - 2)).nonzero(as_tuple=False).squeeze(1)
-        vhidden = hidden if value_model is lm else value_model.hidden_states(ids, cu, pos, mx)
+        vhidden = hidden if value_model is lm else planned_hidden_states(value_model, plan)
         vals = value_model.values(vhidden[vsel])
         out_v = torch.zeros((B, T_r), dtype=torch.float32, device=dev)
         out_v = out_v.index_put((row[vsel], col[vsel] + 1 - context_length), vals)
@@ -482,12 +535,13 @@ def response_logprobs(lm, query_responses: torch.Tensor, context_length: int, pa
 
 
 @torch.no_grad()
-def response_top_logprobs(lm, query_responses: torch.Tensor, context_length: int, pad_token_id: int, k: int, temperature: float = 1.0):
+def response_top_logprobs(lm, query_responses: torch.Tensor, context_length: int, pad_token_id: int, k: int, temperature: float = 1.0,
+                          share_prompts: bool = False):
     """A teacher's view of the response part: (logp [B, T_r, k], idx [B, T_r, k]), entry j of which are its k most probable tokens for position j of the response,
-    given everything before.  Slots that ``response_logprobs`` calls invalid have idx -1 and logp -inf."""
+    given everything before.  Slots that ``response_logprobs`` calls invalid have idx -1 and logp -inf.  ``share_prompts`` as there."""
     B, L = query_responses.shape
-    plan = build_logprob_plan(query_responses, context_length, pad_token_id)
-    hidden = lm.hidden_states(plan["ids"], plan["cu"], plan["pos"], plan["max_seqlen"])
+    plan = build_logprob_plan(query_responses, context_length, pad_token_id, share_prompts)
+    hidden = planned_hidden_states(lm, plan)
     logp, idx = lm.top_logprobs(hidden.index_select(0, plan["src"]), k, temperature)
     out_lp = logp.new_full((B, L - context_length, k), -math.inf)
     out_idx = idx.new_full((B, L - context_length, k), -1)
@@ -495,15 +549,17 @@ def response_top_logprobs(lm, query_responses: torch.Tensor, context_length: int
 
 
 def response_distill_loss(lm, query_responses: torch.Tensor, context_length: int, pad_token_id: int, top_logp: torch.Tensor, top_idx: torch.Tensor,
-                          weights: Optional[torch.Tensor] = None, temperature: float = 1.0, beta: float = 0.0, tail: bool = True):
+                          weights: Optional[torch.Tensor] = None, temperature: float = 1.0, beta: float = 0.0, tail: bool = True,
+                          share_prompts: bool = False):
     """Divergence of ``lm`` from a teacher's ``response_top_logprobs`` over the response part: (sum of weights * token losses, token losses [B, T_r]).
-    ``weights`` [B, T_r]: share of every slot (None: the mean over the valid ones); invalid slots do not count whatever they say.  Only the loss has a gradient."""
+    ``weights`` [B, T_r]: share of every slot (None: the mean over the valid ones); invalid slots do not count whatever they say.  Only the loss has a gradient.
+    ``share_prompts`` as in ``response_logprobs``."""
     B, L = query_responses.shape
     T_r = L - context_length
     if tuple(top_idx.shape[:2]) != (B, T_r) or (weights is not None and tuple(weights.shape) != (B, T_r)):
         raise ValueError(f"response_distill_loss: the teacher's entries and the weights must be [{B}, {T_r}, ...], got {tuple(top_idx.shape)}")
-    plan = build_logprob_plan(query_responses, context_length, pad_token_id)
-    hidden = lm.hidden_states(plan["ids"], plan["cu"], plan["pos"], plan["max_seqlen"])
+    plan = build_logprob_plan(query_responses, context_length, pad_token_id, share_prompts)
+    hidden = planned_hidden_states(lm, plan)
     r, c = plan["r"], plan["c"]
     loss, token = lm.distill_loss(hidden.index_select(0, plan["src"]), top_logp[r, c], top_idx[r, c], None if weights is None else weights[r, c], temperature, beta, tail)
     return loss, token.new_zeros(B, T_r).index_put((r, c), token)

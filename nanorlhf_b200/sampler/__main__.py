@@ -2,6 +2,7 @@
 
     python -m nanorlhf_b200.sampler --model DIR --prompt-ids 5,17,3 [--prompt-ids ...] [--n 1] [--max-tokens 32]
                                     [--temperature 0] [--top-p 1.0] [--top-k 0] [--min-p 0] [--seed 0] [--dtype bfloat16|float32] [--eos -1]
+                                    [--shared-decode | --kv-budget 0 [--kv-sinks 4] [--kv-recent N]]
 
 The model class and its engine (whole-prompt paged-KV engine or the step engine of hybrid decoders) are chosen by
 ``config.json``.  Prints one JSON line per sample: {"prompt": i, "sample": j, "tokens": [...]}.
@@ -25,6 +26,10 @@ def main() -> int:
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
     ap.add_argument("--eos", type=int, default=-1, help="stop token id (-1: none)")
     ap.add_argument("--pad", type=int, default=0)
+    ap.add_argument("--shared-decode", action="store_true", help="read the prompt pages that samples share once for all of them")
+    ap.add_argument("--kv-budget", type=int, default=0, help="most cached tokens of a sample between two evictions (0: all)")
+    ap.add_argument("--kv-sinks", type=int, default=4, help="first tokens that an eviction keeps")
+    ap.add_argument("--kv-recent", type=int, default=None, help="newest tokens that it keeps (a quarter of the budget)")
     a = ap.parse_args()
     import torch
     from ..csrc.build import build
@@ -40,7 +45,8 @@ def main() -> int:
     prompts = [[int(t) for t in p.split(",")] for p in a.prompt_ids]
     kw = {"rollout_dtype": a.dtype} if sampler_kind(model) == "hybrid" else {}
     out = generate(a.n, model, _Tok, prompts, a.temperature, a.max_tokens, top_p=a.top_p, seed=a.seed, backend="native",
-                   eos_token_id=a.eos, top_k=a.top_k, min_p=a.min_p, **kw).tolist()
+                   eos_token_id=a.eos, top_k=a.top_k, min_p=a.min_p,
+                   shared_decode=a.shared_decode, kv_budget=a.kv_budget, kv_sinks=a.kv_sinks, kv_recent=a.kv_recent, **kw).tolist()
     for i in range(len(prompts)):
         for j in range(a.n):
             print(json.dumps({"prompt": i, "sample": j, "tokens": out[i * a.n + j]}))

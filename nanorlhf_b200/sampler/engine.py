@@ -82,11 +82,27 @@ def release_native_engine(model):
         eng.release()
 
 
+def check_cache_options(shared_decode: bool, kv_budget: int, kv_sinks: int, kv_recent: Optional[int]) -> int:
+    """what ``generate`` is told about the cache; returns kv_recent (None: a quarter of the budget)"""
+    if kv_budget != int(kv_budget) or kv_budget < 0:
+        raise ValueError(f"kv_budget must be 0 (all tokens stay) or a positive whole number, got {kv_budget}")
+    recent = int(kv_budget) // 4 if kv_recent is None else kv_recent
+    if kv_budget and (kv_sinks < 0 or recent < 0 or kv_sinks + recent > kv_budget):
+        raise ValueError(f"kv_sinks and kv_recent must not be negative nor together over kv_budget, got {kv_sinks}, {recent} and {kv_budget}")
+    if kv_budget and shared_decode:
+        raise ValueError("a bounded cache has pages of its own for every sample; shared_decode does not go with kv_budget")
+    return recent
+
+
 def generate(n: int, model, tokenizer, prompts: Union[torch.Tensor, Sequence[Sequence[int]]], temperature: float,
              max_tokens: int, top_p: float = 0.95, seed: Optional[int] = None, backend: str = "auto",
-             eos_token_id: Optional[int] = None, rollout_dtype: str = "bf16", top_k: int = 0, min_p: float = 0.0, **engine_kw) -> torch.Tensor:
+             eos_token_id: Optional[int] = None, rollout_dtype: str = "bf16", top_k: int = 0, min_p: float = 0.0,
+             shared_decode: bool = False, kv_budget: int = 0, kv_sinks: int = 4, kv_recent: Optional[int] = None, **engine_kw) -> torch.Tensor:
+    """``shared_decode``: the decode attention reads the prompt pages that samples share once for all of them.  ``kv_budget`` (0: off) bounds
+    the cached tokens of a row, by ``kv_sinks`` and ``kv_recent`` as ``ops.kv_evict`` says; both on the whole-prompt engine only."""
     if top_k < 0 or top_k != int(top_k) or not 0.0 <= min_p <= 1.0:
         raise ValueError(f"top_k must be 0 (off) or a positive whole number and min_p between 0 (off) and 1, got {top_k} and {min_p}")
+    check_cache_options(shared_decode, kv_budget, kv_sinks, kv_recent)
     pad_id = tokenizer.pad_token_id
     eos_id = tokenizer.eos_token_id if eos_token_id is None else eos_token_id
     if isinstance(prompts, torch.Tensor):
@@ -94,10 +110,16 @@ def generate(n: int, model, tokenizer, prompts: Union[torch.Tensor, Sequence[Seq
     if seed is None:
         seed = next_rollout_seed()
     which = _pick_backend(model, backend)
+    cache_kw = {}
+    if shared_decode or kv_budget:
+        from ..models.registry import sampler_kind
+        if sampler_kind(model) == "hybrid" or (kv_budget and which != "native"):
+            raise ValueError("shared_decode and kv_budget are the whole-prompt paged-KV engine's; this model or backend has another")
+        cache_kw = dict(shared_decode=shared_decode, kv_budget=int(kv_budget), kv_sinks=kv_sinks, kv_recent=kv_recent)
     if which == "native":
         eng = get_native_engine(model, rollout_dtype=rollout_dtype, **engine_kw)
         eng.sync_weights()
-        return eng.generate(prompts, n, temperature, top_p, max_tokens, eos_id, pad_id, seed, top_k, min_p)
+        return eng.generate(prompts, n, temperature, top_p, max_tokens, eos_id, pad_id, seed, top_k, min_p, **cache_kw)
     return torch_generate(model, prompts, n, temperature, top_p, max_tokens, eos_id, pad_id, seed, top_k=top_k, min_p=min_p)
 
 

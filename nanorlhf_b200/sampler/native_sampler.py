@@ -10,7 +10,11 @@
   bucket; the host only looks at the ``finished`` flags every ``sync_every`` steps;
 * sampling semantics of the reference's ``vllm_generate``: temperature, top-p 0.95 (and, where asked for, min-p and top-k in front of it), n samples per
   prompt, seeded, stop at EOS (kept), right-pad with pad_id, prompt-major / sample-minor order
-  (GRPO/grpo_trainer.py:122-166); temperature 0 = greedy (ReMax baseline / eval).
+  (GRPO/grpo_trainer.py:122-166); temperature 0 = greedy (ReMax baseline / eval);
+* two other forms of the decode attention, each for one ``generate``: over the prompt pages that the samples of a prompt share, read
+  once for all of them (``shared_decode``), or over a cache of at most ``kv_budget`` tokens and ``sync_every`` new ones a
+  row, out of which every ``sync_every`` steps the tokens go that the steps so far looked at least (``kv_sinks`` first and
+  ``kv_recent`` newest ones stay).
 """
 from __future__ import annotations
 
@@ -20,8 +24,9 @@ from typing import Dict, List, Optional, Sequence
 import torch
 
 from ..models.lora import LoraLinear
-from ..ops import gemm as _gemm, native, reference as ref
+from ..ops import gemm as _gemm, kv_evict, native, paged_decode_scored, paged_decode_shared, reference as ref
 from ..ops.attention import attention_varlen
+from .engine import check_cache_options
 
 
 def _unwrap(model):
@@ -224,7 +229,13 @@ class NativeSampler:
         fp8 = self.kv_dtype == "fp8"
         native.ext().rope_kv_write(qkv, cos, sin, self.k_cache[li], self.v_cache[li], self.k_scale[li] if fp8 else None,
                                    self.v_scale[li] if fp8 else None, st["slot"], Hq, Hkv)
-        if self.kv_dtype == "fp8":
+        kw = dict(k_scale=self.k_scale[li] if fp8 else None, v_scale=self.v_scale[li] if fp8 else None, scale=1.0 / math.sqrt(D))
+        pages = (self.k_cache[li], self.v_cache[li], st["block_tables"], st["ctx_lens"])
+        if st["mode"][0] == "shared":
+            att = paged_decode_shared(q, *pages, st["cu_groups"], st["shared_lens"], st["mode"][1], **kw)
+        elif st["mode"][0] == "scored":
+            att = paged_decode_scored(q, *pages, st[f"scores{li}"], **kw)[0]
+        elif fp8:
             native._count()
             att = native.ext().paged_decode_fp8(q, self.k_cache[li], self.v_cache[li], self.k_scale[li], self.v_scale[li],
                                                 st["block_tables"], st["ctx_lens"], 1.0 / math.sqrt(D), st["splits"])
@@ -245,21 +256,23 @@ class NativeSampler:
     # prefill
     # ------------------------------------------------------------------------------------------
     @torch.no_grad()
-    def _prefill(self, sched, groups: List[int], prompts: Dict[int, Sequence[int]]):
+    def _prefill(self, sched, groups: List[int], prompts: Dict[int, Sequence[int]], once: bool = False):
         """Run the prompts of ``groups`` through the model, writing KV pages; returns last-token logits
-        [len(groups), V]."""
+        [len(groups), V].  ``once``: groups that follow one another with the very same prompt compute it once."""
         cfg, dev = self.cfg, self.device
         ids, pos, cu, slot, src = [], [], [0], [], []
-        off = 0
+        row, last_prompt = [], None
         for g in groups:
-            p = list(prompts[g])
-            ids += p
-            pos += list(range(len(p)))
-            cu.append(cu[-1] + len(p))
+            p = prompts[g]
+            if not (once and p is last_prompt):
+                ids += list(p)
+                pos += list(range(len(p)))
+                cu.append(cu[-1] + len(p))
+                last_prompt = p
+            row.append(len(cu) - 2)
             tok, sl = sched.prefill_slots(g)
-            src += [off + t for t in tok]
+            src += [cu[-2] + t for t in tok]
             slot += sl
-            off += len(p)
         ids_t = torch.tensor(ids, dtype=torch.long, device=dev)
         pos_t = torch.tensor(pos, dtype=torch.long, device=dev)
         cu_t = torch.tensor(cu, dtype=torch.int32, device=dev)
@@ -271,18 +284,20 @@ class NativeSampler:
         for li in range(cfg.num_hidden_layers):
             x, res = self._layer_prefill(li, x, res, cos, sin, cu_t, max_len, slot_t, src_t)
         last = cu_t[1:].long() - 1
+        if len(row) != last.numel():
+            last = last[torch.tensor(row, device=dev)]
         self.stats["prefill_tokens"] += len(ids)
         return self._final_logits(x[last].contiguous(), res[last].contiguous())
 
     # ------------------------------------------------------------------------------------------
     # decode
     # ------------------------------------------------------------------------------------------
-    def _alloc_state(self, S: int, max_blocks: int, max_tokens: int, pad_id: int = 0):
+    def _alloc_state(self, S: int, max_blocks: int, max_tokens: int, pad_id: int = 0, mode: tuple = ("plain", 0)):
         """Batch state of ``S`` rows.  States are pooled per shape: the decode CUDA graph of a bucket is captured
         against these exact tensors, so a batch that shrinks (compaction) or grows (admission) back into a bucket it
         has used before replays the existing graph instead of capturing a new one."""
         dev = self.device
-        key = (S, max_blocks, max_tokens)
+        key = (S, max_blocks, max_tokens, mode)
         st = self._state_pool.get(key)
         if st is None:
             i32 = dict(dtype=torch.int32, device=dev)
@@ -292,29 +307,64 @@ class NativeSampler:
                 "slot": torch.zeros(S, **i32), "finished": torch.ones(S, dtype=torch.bool, device=dev),
                 "gen_count": torch.zeros(S, **i32), "row_ids": torch.zeros(S, **i32),
                 "out": torch.full((S, max_tokens + 1), pad_id, dtype=torch.int32, device=dev),
-                "rows": torch.arange(S, device=dev), "splits": 1,
+                "rows": torch.arange(S, device=dev), "splits": 1, "mode": mode,
             }
+            if mode[0] == "shared":
+                st["cu_groups"], st["shared_lens"] = torch.zeros(S + 1, **i32), torch.zeros(S, **i32)
+            if mode[0] == "scored":
+                for name in self._score_names():
+                    st[name] = torch.zeros(S, self.cfg.num_key_value_heads, max_blocks * self.PAGE, device=dev)
             if len(self._state_pool) >= 8:
                 old = next(iter(self._state_pool))
                 self._state_pool.pop(old)
-                self._graphs = {k: v for k, v in self._graphs.items() if v[1] is not None and (k[0], k[1], k[7]) != old}
+                self._graphs = {k: v for k, v in self._graphs.items() if v[1] is not None and (k[0], k[1], k[7], k[-1]) != old}
             self._state_pool[key] = st
         else:
             for k, fill in (("tokens", 0), ("positions", 0), ("ctx_lens", 1), ("slot", 0), ("gen_count", 0), ("row_ids", 0)):
                 st[k].fill_(fill)
             st["finished"].fill_(True)
             st["out"].fill_(pad_id)
+            if mode[0] == "scored":
+                for name in self._score_names():
+                    st[name].zero_()
         return st
+
+    def _score_names(self):
+        return [f"scores{li}" for li in range(self.cfg.num_hidden_layers)]
+
+    def _share_pages(self, st, running: List[int], n: int, prompt_lens: List[int]):
+        """Groups of the batch rows: the samples of a prompt stand side by side, and share its full pages."""
+        cu, shared = [0], []
+        for i, sid in enumerate(running):
+            if i == 0 or sid // n != running[i - 1] // n:
+                cu.append(i)
+                shared.append(prompt_lens[sid // n] // self.PAGE * self.PAGE)
+            cu[-1] = i + 1
+        S, G = st["S"], len(shared)
+        shared = [t if cu[g + 1] - cu[g] > 1 else 0 for g, t in enumerate(shared)]           # a row alone is a plain one
+        st["cu_groups"].copy_(torch.tensor(cu + [cu[-1]] * (S - G), dtype=torch.int32))
+        st["shared_lens"].copy_(torch.tensor(shared + [0] * (S - G), dtype=torch.int32))
+
+    def _evict(self, st, keep: int, sinks: int, recent: int):
+        """Rows of more than ``keep`` cached tokens go back to ``keep``; every layer and kv head chooses its own."""
+        fp8, lens = self.kv_dtype == "fp8", None
+        for li, name in enumerate(self._score_names()):
+            _, scores, lens = kv_evict(self.k_cache[li], self.v_cache[li], st["block_tables"], st["ctx_lens"], st[name], keep, sinks, recent,
+                                       k_scale=self.k_scale[li] if fp8 else None, v_scale=self.v_scale[li] if fp8 else None)
+            st[name][:, :, :keep].copy_(scores[:, :, :st[name].shape[2]])
+        st["ctx_lens"].copy_(lens)
+        self.stats["evictions"] = self.stats.get("evictions", 0) + 1
 
     def _decode_step(self, st, temperature, top_p, seed, eos_id, pad_id, max_tokens):
         """One token for every row of the batch; pure device work (graph-capturable)."""
         cfg = self.cfg
         PAGE = self.PAGE
         pos = st["positions"]
-        # slot of the token being fed (position = ctx_len - 1)
-        page = torch.div(pos, PAGE, rounding_mode="floor").long()
+        # slot of the token being fed: its position, unless tokens in front of it have gone
+        at = st["ctx_lens"] - 1 if st["mode"][0] == "scored" else pos
+        page = torch.div(at, PAGE, rounding_mode="floor").long()
         blk = st["block_tables"].gather(1, page[:, None]).squeeze(1)
-        st["slot"].copy_(blk * PAGE + (pos % PAGE))
+        st["slot"].copy_(blk * PAGE + (at % PAGE))
         cos, sin = ref.rope_cos_sin(pos, cfg.head_dim, cfg.rope_theta)
         x, res = self._embed(st["tokens"]), None
         for li in range(cfg.num_hidden_layers):
@@ -339,7 +389,7 @@ class NativeSampler:
         """Run up to ``steps`` decode iterations through a CUDA graph (one graph per batch bucket and
         sampling configuration)."""
         key = (st["S"], st["block_tables"].shape[1], float(temperature), float(top_p), int(seed), eos_id, pad_id,
-               max_tokens, st["splits"], self._filters)
+               max_tokens, st["splits"], self._filters, st["mode"])
         if not self.use_cuda_graph:
             for _ in range(steps):
                 self._decode_step(st, temperature, top_p, seed, eos_id, pad_id, max_tokens)
@@ -377,8 +427,10 @@ class NativeSampler:
     # ------------------------------------------------------------------------------------------
     @torch.no_grad()
     def generate(self, prompts: Sequence[Sequence[int]], n: int, temperature: float, top_p: float, max_tokens: int,
-                 eos_id: Optional[int], pad_id: int, seed: int, top_k: int = 0, min_p: float = 0.0) -> torch.Tensor:
+                 eos_id: Optional[int], pad_id: int, seed: int, top_k: int = 0, min_p: float = 0.0,
+                 shared_decode: bool = False, kv_budget: int = 0, kv_sinks: int = 4, kv_recent: Optional[int] = None) -> torch.Tensor:
         from .. import _C
+        kv_recent = check_cache_options(shared_decode, kv_budget, kv_sinks, kv_recent)
         self._filters = (int(top_k), float(min_p))
         dev, PAGE = self.device, self.PAGE
         was_training = self.lm.training
@@ -387,14 +439,20 @@ class NativeSampler:
         total = P * n
         out = torch.full((total, max_tokens), pad_id, dtype=torch.long, device=dev)
         max_prompt = max(len(p) for p in prompts)
-        per_seq_blocks = (max_prompt + max_tokens + PAGE - 1) // PAGE + 1
-        need = sum((len(p) // PAGE) + n * ((len(p) + max_tokens + PAGE - 1) // PAGE - len(p) // PAGE) for p in prompts)
+        evicts = 0 < kv_budget < max_prompt + max_tokens
+        # a bounded cache: pages of its own for every sample, for the prompt or the budget and what comes until the next eviction
+        most = [min(len(p) + max_tokens, max(len(p) + 1, kv_budget) + self.sync_every) if evicts else len(p) + max_tokens for p in prompts]
+        mode = ("scored", 0) if evicts else ("shared", n) if shared_decode and n > 1 else ("plain", 0)
+        per_seq_blocks = (max(most) + PAGE - 1) // PAGE + 1
+        need = sum(n * ((m + PAGE - 1) // PAGE) for m in most) if evicts else sum((len(p) // PAGE) + n * ((len(p) + max_tokens + PAGE - 1) // PAGE - len(p) // PAGE) for p in prompts)
         self._ensure_kv(need + 8)
         sched = _C.Scheduler(self.num_blocks - 1, PAGE, self.max_num_seqs, True)   # last page = scratch for padding rows
         gid_to_prompt = {}
-        for i, p in enumerate(prompts):
-            gid = sched.add_request(len(p), n, max_tokens)
-            gid_to_prompt[gid] = p
+        per_request = 1 if evicts else n             # samples of a request
+        for p, m in zip(prompts, most):
+            for _ in range(n // per_request):
+                gid = sched.add_request(len(p), per_request, m - len(p))
+                gid_to_prompt[gid] = p
         scratch_block = self.num_blocks - 1
         running: List[int] = []          # seq ids in batch-row order
         st = None
@@ -411,7 +469,7 @@ class NativeSampler:
                         chunk.append(g)
                         tok_count += len(gid_to_prompt[g])
                     if chunk and (g is None or tok_count >= self.prefill_token_budget):
-                        logits_parts.append((list(chunk), self._prefill(sched, chunk, gid_to_prompt)))
+                        logits_parts.append((list(chunk), self._prefill(sched, chunk, gid_to_prompt, evicts)))
                         chunk, tok_count = [], 0
                 # ---- (re)build the batch state: surviving rows + new rows ----
                 keep_rows = []
@@ -423,7 +481,7 @@ class NativeSampler:
                 new_running = [running[i] for i in keep_rows]
                 old_state = st
                 old_keep = {k: old_state[k][torch.tensor(keep_rows, device=dev)] for k in
-                            ("tokens", "positions", "ctx_lens", "finished", "gen_count", "out")} if keep_rows else None
+                            ["tokens", "positions", "ctx_lens", "finished", "gen_count", "out"] + (self._score_names() if evicts else [])} if keep_rows else None
                 for groups, _ in logits_parts:
                     for g in groups:
                         new_running += sched.group_seqs(g)
@@ -433,7 +491,7 @@ class NativeSampler:
                         raise RuntimeError("KV pool too small: a waiting request group cannot be admitted into an empty batch")
                     break
                 S = max(128, (S_real + 127) // 128 * 128) if self.use_cuda_graph else S_real
-                st = self._alloc_state(S, per_seq_blocks, max_tokens, pad_id)
+                st = self._alloc_state(S, per_seq_blocks, max_tokens, pad_id, mode)
                 st["block_tables"].fill_(scratch_block)
                 bt = torch.from_numpy(sched.block_tables(new_running, per_seq_blocks, scratch_block))     # built by the C++ scheduler
                 st["block_tables"][:S_real].copy_(bt.to(dev))
@@ -445,12 +503,12 @@ class NativeSampler:
                 # first token of every new sequence: sample from the prompt's last-position logits
                 r0 = nk
                 for groups, logits in logits_parts:
-                    rep = torch.arange(len(groups), device=dev).repeat_interleave(n)
-                    cnt = len(groups) * n
+                    rep = torch.arange(len(groups), device=dev).repeat_interleave(per_request)
+                    cnt = len(groups) * per_request
                     rows = slice(r0, r0 + cnt)
                     lg = logits[rep]
                     tok = native.sample_tokens(lg, temperature, top_p, seed, st["row_ids"][rows], st["gen_count"][rows], *self._filters)
-                    plen = torch.tensor([len(gid_to_prompt[g]) for g in groups], dtype=torch.int32, device=dev).repeat_interleave(n)
+                    plen = torch.tensor([len(gid_to_prompt[g]) for g in groups], dtype=torch.int32, device=dev).repeat_interleave(per_request)
                     st["out"][rows, 0] = tok
                     st["tokens"][rows] = tok
                     st["positions"][rows] = plen
@@ -462,6 +520,8 @@ class NativeSampler:
                     st["finished"][rows] = done
                     r0 += cnt
                 running = new_running
+                if mode[0] == "shared":
+                    self._share_pages(st, running, n, [len(p) for p in prompts])
                 avg_ctx = float(st["ctx_lens"][:S_real].float().mean()) + max_tokens / 2
                 st["splits"] = 1 if S_real * self.cfg.num_key_value_heads >= 296 else int(min(8, max(1, math.ceil(
                     296 / max(1, S_real * self.cfg.num_key_value_heads)))))
@@ -469,6 +529,8 @@ class NativeSampler:
                 break
             # ---- decode until the next sync point ----
             self._run_decode(st, self.sync_every, temperature, top_p, seed, eos_id, pad_id, max_tokens)
+            if evicts:
+                self._evict(st, kv_budget, kv_sinks, kv_recent)
             self.stats["decode_steps"] += self.sync_every
             self.stats["row_steps"] += self.sync_every * st["S"]
             fin = st["finished"][:len(running)]

@@ -16,7 +16,7 @@ from ..models.qwen2 import response_logprobs
 from ..parallel.optimizer import build_param_groups
 from ..sampler import engine as sampler_engine
 from ..utils import INVALID_LOGPROB, masked_whiten
-from ..utils.batching import create_batches, strip_common_padding
+from ..utils.batching import strip_common_padding
 from .base import RLTrainer
 
 
@@ -112,13 +112,14 @@ class SparseGRPOTrainer(GRPOTrainer):
             mini = order[step * mini_size:(step + 1) * mini_size]
             self.optimizer.zero_grad()
             if len(mini) > 0:
-                buckets = create_batches([lens[i] for i in mini], a.token_budget_train, mode="packed")
+                buckets = self._packed_batches(batch["query_responses"][torch.as_tensor(mini, device=self.device)], ctx, [lens[i] for i in mini], a.token_budget_train)
                 n_tok_total = float(sum(int((~batch["padding_mask"][mini[j]]).sum()) for b in buckets for j in b))
                 for b in buckets:
                     inds = torch.as_tensor([mini[j] for j in b], device=self.device)
                     mb = {k: (v[inds] if isinstance(v, torch.Tensor) and v.dim() > 0 and v.shape[0] == n_local else v)
                           for k, v in batch.items()}
-                    out = response_logprobs(self.policy, mb["query_responses"], ctx, pad, a.temperature, want_entropy=True)
+                    out = response_logprobs(self.policy, mb["query_responses"], ctx, pad, a.temperature, want_entropy=True,
+                                            share_prompts=a.share_prompts)
                     mb["new_logprobs"] = torch.masked_fill(out[0], mb["padding_mask"], INVALID_LOGPROB)
                     loss, st = self.micro_loss(mb)
                     if self.loss_agg == "token":
@@ -194,7 +195,7 @@ class RemaxTrainer(RLTrainer):
         out["baseline_responses"] = sampler_engine.generate(
             1, self.model, self.tokenizer, queries, 0.0, a.response_length, top_p=1.0, seed=0,
             backend=a.sampler, rollout_dtype=a.rollout_dtype, kv_block_size=a.kv_block_size,
-                                            kv_cache_dtype=a.kv_cache_dtype)
+                                            kv_cache_dtype=a.kv_cache_dtype, **self._cache_kw())
         return out
 
     def post_score(self, queries, rollout, scores):

@@ -40,7 +40,7 @@ from ..runtime.offload import TieringEngine
 from ..sampler import engine as sampler_engine
 from ..utils import (INVALID_LOGPROB, disable_dropout_in_model, exact_div, masked_whiten, response_masks,
                      scatter_terminal_reward, truncate_response)
-from ..utils.batching import create_batches
+from ..utils.batching import create_batches, create_prompt_batches
 from ..utils.callbacks import (DEFAULT_CALLBACKS, CallbackHandler, OnlineTrainerState, ProgressCallback,
                                TrainerControl)
 from ..utils.data import DataCollatorWithPadding, PromptLoader
@@ -214,8 +214,12 @@ class RLTrainer:
                                             a.temperature, a.response_length, top_p=a.top_p,
                                             seed=seed + self.comm.rank * 7919, backend=a.sampler,
                                             rollout_dtype=a.rollout_dtype, kv_block_size=a.kv_block_size,
-                                            kv_cache_dtype=a.kv_cache_dtype, top_k=a.top_k, min_p=a.min_p, **self._weight_sync_kw())
+                                            kv_cache_dtype=a.kv_cache_dtype, top_k=a.top_k, min_p=a.min_p, **self._cache_kw(), **self._weight_sync_kw())
         return {"responses": responses}
+
+    def _cache_kw(self) -> dict:
+        a = self.args
+        return dict(shared_decode=a.shared_decode, kv_budget=a.kv_budget, kv_sinks=a.kv_sinks, kv_recent=a.kv_recent)
 
     def _weight_sync_kw(self) -> dict:
         """``weight_sync="sharded"`` (the default; needs fused DP on CUDA): the sampler arena refresh is K-BC across ranks."""
@@ -277,6 +281,17 @@ class RLTrainer:
         st["pg_loss"] = loss.detach()
         return loss, st
 
+    def _prompt_ids(self, query_responses, ctx) -> list:
+        """a number for the query of every row, the same for rows that have the same one"""
+        return torch.unique(query_responses[:, :ctx], dim=0, return_inverse=True)[1].tolist()
+
+    def _packed_batches(self, query_responses, ctx, lens, budget):
+        """rows in batches of at most ``budget`` real tokens; with ``share_prompts`` those of one query together, which counts once"""
+        if not self.args.share_prompts or len(lens) == 0:
+            return create_batches(lens, budget, mode="packed")
+        shared = (query_responses[:, :max(ctx - 1, 0)] != self.tokenizer.pad_token_id).sum(1).tolist()
+        return create_prompt_batches(lens, shared, self._prompt_ids(query_responses, ctx), budget)
+
     # ---- phase 4: no-grad logprob pass in token-budget chunks ----------------------------------
     @torch.no_grad()
     def logprob_pass(self, queries, responses):
@@ -286,7 +301,7 @@ class RLTrainer:
         qr = torch.cat([queries, responses], 1)
         lens = (qr != pad).sum(1).tolist()
         # packed layout => the budget is on real tokens, not on padded rectangles
-        chunks = create_batches(lens, a.token_budget_fwd, mode="packed")
+        chunks = self._packed_batches(qr, ctx, lens, a.token_budget_fwd)
         B, T_r = responses.shape
         lp = torch.empty(B, T_r, dtype=torch.float32, device=self.device)
         rlp = torch.empty_like(lp)
@@ -295,11 +310,13 @@ class RLTrainer:
         for idx in chunks:
             ii = torch.as_tensor(idx, device=self.device)
             out = response_logprobs(self.policy, qr[ii], ctx, pad, a.temperature, want_entropy=False,
-                                    value_model=self.model.value_model if self.uses_value_model else None)
+                                    value_model=self.model.value_model if self.uses_value_model else None,
+                                    share_prompts=a.share_prompts)
             lp[ii] = out[0]
             if self.uses_value_model:
                 vals[ii] = out[2]
-            rlp[ii] = response_logprobs(self.ref_policy, qr[ii], ctx, pad, a.temperature, want_entropy=False)[0]
+            rlp[ii] = response_logprobs(self.ref_policy, qr[ii], ctx, pad, a.temperature, want_entropy=False,
+                                        share_prompts=a.share_prompts)[0]
         return qr, lp, rlp, vals
 
     # ---- the update --------------------------------------------------------------------------
@@ -516,10 +533,13 @@ class RLTrainer:
         rows = {}
         self.ckpt_writer.wait_snapshot()          # an in-flight checkpoint has finished READING the parameters / moments
         self.policy.train()
+        prompts = np.asarray(self._prompt_ids(batch["query_responses"], ctx)) if a.share_prompts else None
         for ep in range(a.num_ppo_epochs):
             b_inds = self._np_rng.permutation(n_local)
             for mi, mb_start in enumerate(range(0, n_local, lmb)):
                 mini = b_inds[mb_start:mb_start + lmb]
+                if prompts is not None:                   # the same rows in the step, those of a query in the same micro-steps
+                    mini = mini[np.argsort(prompts[mini], kind="stable")]
                 self.optimizer.zero_grad()
                 for gi, mc_start in enumerate(range(0, len(mini), a.per_device_train_batch_size)):
                     inds = torch.as_tensor(mini[mc_start:mc_start + a.per_device_train_batch_size], device=self.device)
@@ -534,7 +554,8 @@ class RLTrainer:
                                                             # from backward hooks; earlier micro-steps do not reduce = no_sync)
                     out = response_logprobs(self.policy, mb["query_responses"], ctx, pad, a.temperature,
                                             want_entropy=True,
-                                            value_model=self.model.value_model if self.uses_value_model else None)
+                                            value_model=self.model.value_model if self.uses_value_model else None,
+                                            share_prompts=a.share_prompts)
                     new_lp = torch.masked_fill(out[0], mb["padding_mask"], INVALID_LOGPROB)
                     mb["new_logprobs"] = new_lp
                     if self.uses_value_model:

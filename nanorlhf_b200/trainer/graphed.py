@@ -8,6 +8,8 @@ once per shape bucket and replayed:
 * packed tokens are padded to a multiple of ``TOKEN_BUCKET`` with one dummy sequence of pad tokens,
   response rows to a multiple of ``ROW_BUCKET`` with entries that land in a dump row -- neither
   reaches the loss, so gradients are unchanged;
+* with ``share_prompts`` the number of sequences depends on how many rows have the same query: sequences and groups are
+  padded with empty ones to the most that the rows can make;
 * gradients accumulate in place into the optimizer's flat buffer (static addresses), the
   per-micro-step statistics come back through one static vector;
 * all graphs share one memory pool (they are replayed strictly one after another).
@@ -23,7 +25,7 @@ from typing import Dict, Optional
 
 import torch
 
-from ..models.qwen2 import build_logprob_plan, planned_response_logprobs
+from ..models.qwen2 import build_logprob_plan, planned_hidden_states, planned_response_logprobs
 from ..utils import INVALID_LOGPROB
 
 TOKEN_BUCKET = 256
@@ -61,7 +63,7 @@ class GraphedMicroStep:
         mb["new_logprobs"] = torch.masked_fill(out_lp, mb["padding_mask"], INVALID_LOGPROB)
         if t.uses_value_model:                               # PPO: the critic's forward / backward rides in the same graph
             vm = t.model.value_model
-            vh = hidden if vm is t.policy else vm.hidden_states(plan["ids"], plan["cu"], plan["pos"], L)
+            vh = hidden if vm is t.policy else planned_hidden_states(vm, plan, L)
             vals = vm.values(vh.index_select(0, plan["vsel"]))
             out_v = torch.zeros((B + 1, T_r), dtype=torch.float32, device=vals.device)
             mb["vpred"] = out_v.index_put((plan["vr"], plan["vc"]), vals.float())[:B]     # padded entries land in dump row B
@@ -88,9 +90,11 @@ class GraphedMicroStep:
         pos[:T] = plan["pos"]
         if T_b > T:
             pos[T:] = torch.arange(T_b - T, device=dev, dtype=pos.dtype)
-        cu = torch.empty(B + 2, dtype=torch.int32, device=dev)
-        cu[:B + 1] = plan["cu"]
-        cu[B + 1] = T_b                                      # dummy sequence (possibly empty)
+        S, groups = plan["cu"].numel() - 1, plan.get("cu_groups")
+        most = B if groups is None else B + B // 2           # a query of two rows or more is a sequence of its own
+        cu = torch.full((most + 2,), T, dtype=torch.int32, device=dev)
+        cu[:S + 1] = plan["cu"]
+        cu[most + 1] = T_b                                   # dummy sequence (possibly empty)
         src = torch.zeros(R_b, dtype=plan["src"].dtype, device=dev)
         src[:R] = plan["src"]
         tg = torch.zeros(R_b, dtype=plan["targets"].dtype, device=dev)
@@ -99,7 +103,11 @@ class GraphedMicroStep:
         r[:R] = plan["r"]
         c = torch.zeros(R_b, dtype=plan["c"].dtype, device=dev)
         c[:R] = plan["c"]
-        return {"ids": ids, "cu": cu, "pos": pos, "src": src, "targets": tg, "r": r, "c": c}
+        out = {"ids": ids, "cu": cu, "pos": pos, "src": src, "targets": tg, "r": r, "c": c}
+        if groups is not None:                               # the padding is in no group
+            out["cu_groups"] = torch.full((B + 1,), S, dtype=torch.int32, device=dev)
+            out["cu_groups"][:groups.numel()] = groups
+        return out
 
     # ---- public ----------------------------------------------------------------------------------------
     def __call__(self, mb: dict, ctx: int, pad_id: int) -> torch.Tensor:
@@ -108,12 +116,12 @@ class GraphedMicroStep:
         qr = mb["query_responses"]
         B, L = qr.shape
         T_r = L - ctx
-        plan = build_logprob_plan(qr, ctx, pad_id)
+        plan = build_logprob_plan(qr, ctx, pad_id, self.t.args.share_prompts)
         T_b = _round_up(plan["ids"].numel(), TOKEN_BUCKET)
         R_b = _round_up(max(plan["src"].numel(), 1), ROW_BUCKET)
         tens = {k: v for k, v in mb.items() if isinstance(v, torch.Tensor) and k != "query_responses"}
         accum = int(getattr(self.t, "_accum_steps", self.t.args.gradient_accumulation_steps))
-        key = (T_b, R_b, B, L, accum, tuple(sorted((k, tuple(v.shape), str(v.dtype)) for k, v in tens.items())))
+        key = (T_b, R_b, B, L, accum, plan["cu_groups"] is not None, tuple(sorted((k, tuple(v.shape), str(v.dtype)) for k, v in tens.items())))
         padded = self._pad_plan(plan, B, pad_id, T_b, R_b)
         if self.t.uses_value_model:
             # value positions (columns ctx-1 .. L-2 of every real token, models/qwen2.py response_logprobs), padded to a bucket

@@ -34,6 +34,36 @@ def create_batches(lengths: Sequence[int], max_batch_memory_size: int, mode: str
     return batches
 
 
+def create_prompt_batches(lengths: Sequence[int], shared: Sequence[int], prompts: Sequence[int], max_batch_memory_size: int) -> List[List[int]]:
+    """``create_batches`` in packed mode for rows that share prompts: rows of one prompt stay together if a batch has room for them.
+
+    ``lengths[i]`` tokens has row i, of which the first ``shared[i]`` count once for all rows of ``prompts[i]`` in a batch.
+    Prompts come in the order of their longest row."""
+    rows = {}
+    for i, p in enumerate(prompts):
+        rows.setdefault(p, []).append(i)
+    batches: List[List[int]] = []
+    cur: List[int] = []
+    cur_sum = 0
+    for p in sorted(rows, key=lambda p: (max(int(lengths[i]) for i in rows[p]), p)):
+        own = sorted(rows[p], key=lambda i: (int(lengths[i]), i))
+        prefix = int(shared[own[0]])
+        if cur and cur_sum + prefix + sum(int(lengths[i]) - prefix for i in own) > max_batch_memory_size:
+            batches.append(cur)
+            cur, cur_sum = [], 0
+        cur_sum += prefix
+        for n, i in enumerate(own):
+            L = int(lengths[i]) - prefix
+            if n > 0 and cur_sum + L > max_batch_memory_size:
+                batches.append(cur)
+                cur, cur_sum = [], prefix
+            cur.append(i)
+            cur_sum += L
+    if cur:
+        batches.append(cur)
+    return batches
+
+
 def strip_common_padding(queries, responses, pad_token_id: int):
     """Drop all-pad leading query columns and all-pad trailing response columns
     (sparse-GRPO de-padding, grpo_r1_trainer.py:572-584)."""
