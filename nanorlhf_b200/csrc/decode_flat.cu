@@ -6,7 +6,7 @@
 // The pages of all rows and kv heads, one behind the other, are dealt to the warps of the chip in equal runs: no block is longer than another, none starts
 // again for every row, and few long contexts are cut as finely as many short ones.
 //   decode_plan   (one block) adds up the rows' pages and finds where every warp's run begins; few rows without prefixes' runs do without it: every block of
-//                 decode_flat makes the plan (4 rows of 330 tokens 10.1 -> 7.4 us, 64 rows of a 100-token prefix 17.9 -> 17.8)
+//                 decode_flat makes the plan (4 rows of 330 tokens 10.1 -> 7.4 us)
 //   decode_flat   the first blocks walk the prefixes (decode_prefix.cuh), then all of them the rows: a warp walks a run through its own ring of pages (cp.async);
 //                 of every row that it meets it leaves a part.  Run w and row-head r meet in part w + r: along the runs one of the two grows by one at a time
 //   decode_join   a warp a row and head joins the parts, the prefix's too, in their order; with scores, further blocks form the weights from the scores that the
@@ -519,6 +519,9 @@ __global__ void __launch_bounds__(kFlatWarps * 32, FlatSizes<FP8>::kBlocks) deco
 
 // ---- parts to results, scores to weights ---------------------------------------------------------------------------------------------
 
+constexpr int kJoinU = 4;                // parts in flight
+constexpr int kJoinWarps = 8;
+
 struct FlatParts {
   const float2* ml;                      // of the first part of a row
   const float4* o;
@@ -537,54 +540,77 @@ NRL_DEVICE FlatParts prefix_parts(const FlatParams& p, int g, int s, int h, int 
   const long at = prefix_part_row(p, first, h, group.w, row) + static_cast<long>(kPrefixRows) * c0;
   return {reinterpret_cast<const float2*>(p.prefix_ml) + at, reinterpret_cast<const float4*>(p.prefix_o) + at * 32, (a + group.y - 1) / run - c0 + 1};
 }
-// a lane has four elements; a row's parts lie 8 rows apart, a prefix's 64
-template <bool PREFIX, int kJoinU>
-NRL_DEVICE void join_parts(const FlatParts& x, int lane, float& M, float& L, float4& acc) {
-  for (int i0 = 0; i0 < x.n; i0 += kJoinU) {
+NRL_DEVICE void join_part(float2 e, float4 o, float& M, float& L, float4& acc) {
+  if (e.x == -INFINITY) return;
+  const float top = fmaxf(M, e.x), a = exp2f(M - top), b = exp2f(e.x - top);          // 2^-inf = 0
+  L = L * a + e.y * b;
+  acc.x = acc.x * a + o.x * b; acc.y = acc.y * a + o.y * b; acc.z = acc.z * a + o.z * b; acc.w = acc.w * a + o.w * b;
+  M = top;
+}
+// Parts `from`, `from` + STEP, ...; a lane has four elements; a row's parts lie 8 rows apart, a prefix's 64
+template <bool PREFIX, int STEP>
+NRL_DEVICE void join_parts(const FlatParts& x, int from, int lane, float& M, float& L, float4& acc) {
+  for (int i0 = from; i0 < x.n; i0 += kJoinU * STEP) {
     float2 e[kJoinU];
     float4 o[kJoinU];
 #pragma unroll
     for (int u = 0; u < kJoinU; ++u) {
-      const bool ok = i0 + u < x.n;
-      const long at = (i0 + u) * (PREFIX ? static_cast<long>(kPrefixRows) : 8L);
+      const bool ok = i0 + u * STEP < x.n;
+      const long at = (i0 + u * STEP) * (PREFIX ? static_cast<long>(kPrefixRows) : 8L);
       e[u] = ok ? x.ml[at] : make_float2(-INFINITY, 0.f);
       o[u] = ok ? x.o[at * 32 + lane] : make_float4(0.f, 0.f, 0.f, 0.f);
     }
 #pragma unroll
-    for (int u = 0; u < kJoinU; ++u) {
-      if (e[u].x == -INFINITY) continue;
-      const float top = fmaxf(M, e[u].x), a = exp2f(M - top), b = exp2f(e[u].x - top);          // 2^-inf = 0
-      L = L * a + e[u].y * b;
-      acc.x = acc.x * a + o[u].x * b; acc.y = acc.y * a + o[u].y * b; acc.z = acc.z * a + o[u].z * b; acc.w = acc.w * a + o[u].w * b;
-      M = top;
-    }
+    for (int u = 0; u < kJoinU; ++u) join_part(e[u], o[u], M, L, acc);
   }
 }
+NRL_DEVICE void join_store(const FlatParams& p, int s, int head, int lane, float L, float4 acc) {
+  const float f = L > 0.f ? 1.f / L : 0.f;
+  uint2 v;
+  v.x = pack_bf16x2(acc.x * f, acc.y * f);
+  v.y = pack_bf16x2(acc.z * f, acc.w * f);
+  *reinterpret_cast<uint2*>(p.out + (static_cast<long>(s) * p.Hq + head) * kFlatD + lane * 4) = v;
+}
 
-// grid: rows x (kv heads x, with scores, chunks of tokens); a warp a query head for the results, which the first chunk's blocks form.
-// U parts in flight: 8 for the many parts of few rows (8 rows of 30 k tokens 55 -> 53 us, 4 of 330 7.4 -> 6.8), else 4 (253 rows of 2 k tokens 71, with 8 73)
-template <bool SCORES, int U>
-__global__ void __launch_bounds__(256) decode_join_kernel(const FlatParams p) {
+// Many rows: grid rows x (kv heads x, with scores, chunks of tokens), a warp a query head for the results, which the first chunk's blocks form.
+// NEAR, few rows of many parts: rows x (query heads, whose parts are dealt to eight warps; then the chunks).  8 rows of 30 k tokens with scores 53 -> 47 us, 32 rows of
+// 556 fp8 tokens 12.7 -> 10.8.
+template <bool SCORES, bool NEAR>
+__global__ void __launch_bounds__(kJoinWarps * 32) decode_join_kernel(const FlatParams p) {
   pdl_wait();
   pdl_launch_dependents();
-  const int s = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = blockIdx.y % p.Hkv, chunk = blockIdx.y / p.Hkv;
+  const int s = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (NEAR && static_cast<int>(blockIdx.y) < p.Hq) {
+    __shared__ float2 part_ml[kJoinWarps];
+    __shared__ float4 part_o[kJoinWarps][32];
+    const int head = blockIdx.y;
+    float M = -INFINITY, L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    join_parts<false, kJoinWarps>(flat_parts(p, p.rows[s], s, head / p.G, head % p.G), warp, lane, M, L, acc);
+    if (lane == 0) part_ml[warp] = make_float2(M, L);
+    part_o[warp][lane] = acc;
+    __syncthreads();
+    if (warp > 0) return;
+#pragma unroll
+    for (int w = 1; w < kJoinWarps; ++w) join_part(part_ml[w], part_o[w][lane], M, L, acc);
+    join_store(p, s, head, lane, L, acc);
+    return;
+  }
+  const int y = blockIdx.y - (NEAR ? p.Hq : 0), h = y % p.Hkv, chunk = y / p.Hkv;
   const int ctx = flat_context(p, s), t0 = chunk * p.chunk, n = SCORES ? min(min(ctx, p.max_tokens), t0 + p.chunk) : 0;
-  if (chunk > 0 && t0 >= n) return;
+  if ((NEAR || chunk > 0) && t0 >= n) return;
   const int4 row = p.rows[s];
   __shared__ float top[8], inv[8];
   if (warp < p.G) {
     const FlatParts own = flat_parts(p, row, s, h, warp);
     float M = -INFINITY, L = 0.f;
-    if (chunk == 0) {
+    if (!NEAR && chunk == 0) {
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (!SCORES && row.w > 0 && p.prefix_runs > 0) join_parts<true, U>(prefix_parts(p, row.w - 1, s, h, warp), lane, M, L, acc);
-      join_parts<false, U>(own, lane, M, L, acc);
-      const float f = L > 0.f ? 1.f / L : 0.f;
-      uint2 v;
-      v.x = pack_bf16x2(acc.x * f, acc.y * f);
-      v.y = pack_bf16x2(acc.z * f, acc.w * f);
-      *reinterpret_cast<uint2*>(p.out + (static_cast<long>(s) * p.Hq + h * p.G + warp) * kFlatD + lane * 4) = v;
+      if (!SCORES && row.w > 0 && p.prefix_runs > 0) join_parts<true, 1>(prefix_parts(p, row.w - 1, s, h, warp), 0, lane, M, L, acc);
+      join_parts<false, 1>(own, 0, lane, M, L, acc);
+      join_store(p, s, h * p.G + warp, lane, L, acc);
     } else {
+#pragma unroll 8
       for (int i = lane; i < own.n; i += 32) {
         const float2 e = own.ml[i * 8];
         const float m = fmaxf(M, e.x);
@@ -663,9 +689,8 @@ cudaError_t launch_flat(const FlatParams& p, cudaStream_t s) {
 
 template <bool SCORES>
 cudaError_t launch_join(const FlatParams& p, int chunks, int threads, cudaStream_t s) {
-  const dim3 grid(p.S, p.Hkv * chunks);
-  if (p.near) launch_dependent(decode_join_kernel<SCORES, 8>, grid, threads, 0, s, p);
-  else launch_dependent(decode_join_kernel<SCORES, 4>, grid, threads, 0, s, p);
+  if (p.near) launch_dependent(decode_join_kernel<SCORES, true>, dim3(p.S, p.Hq + (SCORES ? p.Hkv * chunks : 0)), kJoinWarps * 32, 0, s, p);
+  else launch_dependent(decode_join_kernel<SCORES, false>, dim3(p.S, p.Hkv * chunks), threads, 0, s, p);
   return cudaGetLastError();
 }
 
@@ -682,8 +707,9 @@ struct Pieces {
 };
 
 // Runs: as many as warps (prefixes: blocks) fit the chip, or as the longest contexts that the tables allow could fill.
-// Where those contexts are few bytes, rows walk their prefixes themselves: the prefixes' kernel takes 8 us, in which decode_flat reads 40 MB.
-constexpr long kPrefixBytes = 40L << 20;
+// Where those contexts are few bytes, rows walk their prefixes themselves: with prefixes' runs, of whatever size, a call takes 17 us, in which others read 100 MB
+// (16 groups of 8 rows, 100 + 100 bf16 tokens, 17 us with, 14 without; 16 of 4 rows, 1000 + 100, 20 and 17).
+constexpr long kPrefixBytes = 100L << 20;
 // A prefix's step of 64 tokens takes a block as long as this many pages of rows: blocks that begin with prefixes are as many SMs' worth as their share of the work.
 // Rows of 12 heads, 2 kv heads, all on one block an SM, two, three: bf16 64 x 8 of 512 + 256 tokens 48, 51, 58 us, 32 x 16 of 2000 + 128 77, 61, 75;
 // fp8 42, 42, 43 and 90, 67, 57; 13 x 16 of 28 heads, 4100 + 560 tokens 116, 86, 89.

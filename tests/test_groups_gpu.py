@@ -238,9 +238,9 @@ BATCHES = {
 
 
 def widen(st):
-    """Page tables of 50 MB of pages and more: prefixes are attended to for all rows of a group, instead of by each row."""
+    """Page tables of 110 MB of pages and more: prefixes are attended to for all rows of a group, instead of by each row."""
     S, width = st["tables"].shape
-    more = 50_000_000 // (S * st["k"].shape[1] * 4096) + 1
+    more = 110_000_000 // (S * st["k"].shape[1] * 4096) + 1
     st["tables"] = torch.cat([st["tables"], torch.full((S, more), st["k"].shape[0] - 1, dtype=torch.int32, device=DEV)], 1)
 
 
@@ -290,14 +290,16 @@ def test_rows_of_no_group_are_plain(fp8, wide):
     assert torch.equal(a[2:], c[2:]) and torch.equal(c, d)
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("fp8", [False, True])
-def test_many_groups_and_long_prefixes(fp8):
+def test_many_groups_and_long_prefixes(fp8, wide):
     """More groups and rows than decode_plan has threads, runs that meet several tiles, groups of more than one tile of query rows."""
     few = [(300 + 16 * i, [320 + 16 * i + j for j in range(33)]) for i in range(3)] + [(1500, [1501 + j for j in range(70)])]
     many = [(16 * (i % 5), [16 * (i % 5) + 1 + i % 3] * (1 + i % 2)) for i in range(1100)]
     for seed, groups in ((70, few), (71, many)):
         st = shared_batch(seed, groups, 2, fp8)
-        widen(st)
+        if wide:
+            widen(st)
         S = st["context"].numel()
         q = torch.randn(S, 12, 128, generator=gen(seed), device=DEV).to(torch.bfloat16)
         out = ops.paged_decode_shared(q, st["k"], st["v"], st["tables"], st["context"], st["cu"], st["shared"], max_group=70, k_scale=st["ks"], v_scale=st["vs"])
@@ -342,7 +344,8 @@ def test_decode_over_shared_pages_in_two_graphs(fp8):
 # ---- scores ----------------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("heads,kv", [(12, 2), (7, 1), (16, 2), (4, 4)])
-@pytest.mark.parametrize("contexts", [[1], [0, 1, 2, 16, 17], [129, 33, 77], [600 + 13 * i for i in range(50)], [5000, 64]])
+@pytest.mark.parametrize("contexts", [[1], [0, 1, 2, 16, 17], [129, 33, 77], [600 + 13 * i for i in range(50)], [5000, 64], [7 * i % 90 for i in range(129)]],
+                         ids=lambda c: f"{len(c)}x{max(c)}")
 def test_decode_with_scores(contexts, heads, kv, fp8):
     st = shared_batch(21, [(0, [c]) for c in contexts], kv, fp8)
     S, L = len(contexts), max(contexts) + 3
