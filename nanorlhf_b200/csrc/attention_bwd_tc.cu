@@ -95,21 +95,25 @@ NRL_DEVICE void bwd_chunk(const uint32_t (&sv)[16], const uint32_t (&dv)[16], ui
 }
 
 // Half a warp per pair, sixteen bytes per lane, two pairs in flight: 12 011 tokens x 28 heads 51 -> 29 us (8 bytes per lane, one pair per warp before)
-// GROUPS: the gradients of rows behind the last sequence are cleared
+// GROUPS: the gradients of rows behind the last sequence are cleared, and O comes with the part that bf16 has no room for: a rounded O puts an error of up to 2^-9 of
+// its terms into every row's delta, which all keys of the row share (error of dQ and dK 2.7e-3 of their norm, with the rest 2.4e-3).  The rest is e5m2, off by 2^-3 of
+// itself at most: 1 byte beside 4 that are read anyway (as bf16 the same error, and 40 us more of a micro-step's 700)
 template <bool GROUPS>
-__global__ void attn_bwd_delta_tc_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ dout,
+__global__ void attn_bwd_delta_tc_kernel(const __nv_bfloat16* __restrict__ o, const uint8_t* __restrict__ rest, const __nv_bfloat16* __restrict__ dout,
                                          float* __restrict__ delta, long o_stride_t, int total, unsigned Hq, unsigned pairs, const AttnBwdParams p) {
   pdl_wait();
   pdl_launch_dependents();
   const int sub = threadIdx.x & 15;
   const unsigned first = (blockIdx.x * (blockDim.x >> 4) + (threadIdx.x >> 4)) * 2;
   uint4 a[2], b[2];
+  uint2 c[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const unsigned idx = min(first + u, pairs - 1), t = idx / Hq, h = idx - t * Hq;
     const long off = t * o_stride_t + h * 128 + sub * 8;
     a[u] = *reinterpret_cast<const uint4*>(o + off);
     b[u] = *reinterpret_cast<const uint4*>(dout + off);
+    if (GROUPS) c[u] = t < static_cast<unsigned>(p.seqs.cu[p.seqs.num]) ? *reinterpret_cast<const uint2*>(rest + idx * 128l + sub * 8) : make_uint2(0, 0);
   }
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -119,6 +123,16 @@ __global__ void attn_bwd_delta_tc_kernel(const __nv_bfloat16* __restrict__ o, co
     for (int e = 0; e < 4; ++e) {
       const float2 x = unpack_bf16x2(aw[e]), y = unpack_bf16x2(bw[e]);
       acc = fmaf(x.x, y.x, fmaf(x.y, y.y, acc));
+    }
+    if (GROUPS) {
+      float more = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>((e < 2 ? c[u].x : c[u].y) >> (e & 1) * 16), __NV_E5M2);
+        const float2 x = __half22float2(__half2(h)), y = unpack_bf16x2(bw[e]);
+        more = fmaf(x.x, y.x, fmaf(x.y, y.y, more));
+      }
+      acc = fmaf(more, 1.f / kAttnRest, acc);
     }
 #pragma unroll
     for (int m = 8; m > 0; m >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, m);
@@ -542,7 +556,7 @@ namespace nrl {
 namespace {
 
 template <bool GROUPS>
-cudaError_t attn_bwd_tc(const CUtensorMap* maps, const void* o, const void* dout, const float* lse,
+cudaError_t attn_bwd_tc(const CUtensorMap* maps, const void* o, const void* rest, const void* dout, const float* lse,
                         float* delta, void* dq, void* dk, void* dv, long o_stride_t, long dq_stride_t,
                         long dkv_stride_t, const AttnSeqs& seqs, int total, int Hq, int Hkv,
                         float scale, cudaStream_t s) {
@@ -558,8 +572,8 @@ cudaError_t attn_bwd_tc(const CUtensorMap* maps, const void* o, const void* dout
   p.dq_stride_t = dq_stride_t; p.dkv_stride_t = dkv_stride_t;
   p.total_tokens = total; p.Hq = Hq; p.G = Hq / Hkv;
   p.scale = scale; p.scale_log2 = scale * 1.4426950408889634f;
-  launch_dependent(attn_bwd_delta_tc_kernel<GROUPS>, (pairs + 31) / 32, 256, 0, s, static_cast<const __nv_bfloat16*>(o), static_cast<const __nv_bfloat16*>(dout), delta,
-                   o_stride_t, total, static_cast<unsigned>(Hq), pairs, p);
+  launch_dependent(attn_bwd_delta_tc_kernel<GROUPS>, (pairs + 31) / 32, 256, 0, s, static_cast<const __nv_bfloat16*>(o), static_cast<const uint8_t*>(rest),
+                   static_cast<const __nv_bfloat16*>(dout), delta, o_stride_t, total, static_cast<unsigned>(Hq), pairs, p);
   const unsigned most = total / 128 + seqs.num, grid_kv = most * Hkv, grid_q = most * Hq;
   launch_dependent(attn_bwd_tc_kernel<GROUPS>, grid_kv + grid_q, kBwdThreads, smem, s, maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], maps[6], maps[7], p,
                    grid_kv);
@@ -573,13 +587,13 @@ extern "C" cudaError_t nrl_attn_bwd_tc(const CUtensorMap* maps, const void* o, c
                                        float* delta, void* dq, void* dk, void* dv, long o_stride_t, long dq_stride_t,
                                        long dkv_stride_t, const int* cu, int num_seqs, int total, int Hq, int Hkv,
                                        float scale, cudaStream_t s) {
-  return nrl::attn_bwd_tc<false>(maps, o, dout, lse, delta, dq, dk, dv, o_stride_t, dq_stride_t, dkv_stride_t, {cu, nullptr, num_seqs}, total, Hq, Hkv, scale, s);
+  return nrl::attn_bwd_tc<false>(maps, o, nullptr, dout, lse, delta, dq, dk, dv, o_stride_t, dq_stride_t, dkv_stride_t, {cu, nullptr, num_seqs}, total, Hq, Hkv, scale, s);
 }
 
 // table: attention_groups.cu
-extern "C" cudaError_t nrl_attn_groups_bwd_tc(const CUtensorMap* maps, const void* o, const void* dout, const float* lse, float* delta, void* dq, void* dk,
-                                              void* dv, long o_stride_t, long dq_stride_t, long dkv_stride_t, const int* cu, const int* table, int num_seqs,
+extern "C" cudaError_t nrl_attn_groups_bwd_tc(const CUtensorMap* maps, const void* o, const void* rest, const void* dout, const float* lse, float* delta, void* dq,
+                                              void* dk, void* dv, long o_stride_t, long dq_stride_t, long dkv_stride_t, const int* cu, const int* table, int num_seqs,
                                               int total, int Hq, int Hkv, float scale, cudaStream_t s) {
-  return nrl::attn_bwd_tc<true>(maps, o, dout, lse, delta, dq, dk, dv, o_stride_t, dq_stride_t, dkv_stride_t, {cu, reinterpret_cast<const int4*>(table), num_seqs},
+  return nrl::attn_bwd_tc<true>(maps, o, rest, dout, lse, delta, dq, dk, dv, o_stride_t, dq_stride_t, dkv_stride_t, {cu, reinterpret_cast<const int4*>(table), num_seqs},
                                 total, Hq, Hkv, scale, s);
 }

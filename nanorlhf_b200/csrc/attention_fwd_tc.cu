@@ -29,6 +29,7 @@ struct AttnTcParams {
   AttnSeqs seqs;
   __nv_bfloat16* out;
   float* lse;                 // [Hq, T_total]
+  uint8_t* rest;              // GROUPS: [T_total, Hq, 128] what of the result bf16 has no room for, e5m2 of kAttnRest times it (null: not asked for)
   long o_stride_t;
   int total_tokens, Hq, G;
   float scale_log2;
@@ -41,6 +42,13 @@ struct AttnTcSmem {
   static constexpr int kTab = kBar + 256;                        // two items: head (-1: none left), q0, first token, length, prefix's first token, its length
   static constexpr int kTotal = kTab + 2 * 32;
 };
+
+// two elements, times f
+NRL_DEVICE uint32_t attn_rest(const uint32_t* x, float f) {
+  const float a = __uint_as_float(x[0]) * f, b = __uint_as_float(x[1]) * f;
+  const float2 kept = unpack_bf16x2(pack_bf16x2(a, b));
+  return __nv_cvt_float2_to_fp8x2(make_float2((a - kept.x) * kAttnRest, (b - kept.y) * kAttnRest), __NV_SATFINITE, __NV_E5M2);
+}
 
 template <bool GROUPS>
 struct AttnItem {
@@ -298,6 +306,12 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         tmem_ld_32x32b_x32(t_o + c * 32, ov);
         tmem_ld_wait();
         if (!row_ok) continue;
+        if (GROUPS && p.rest != nullptr) {
+          uint32_t rest[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) rest[i] = attn_rest(ov + 4 * i, inv) | attn_rest(ov + 4 * i + 2, inv) << 16;
+          stg_v8(p.rest + (t * p.Hq + it.head) * kAtD + c * 32, rest);
+        }
 #pragma unroll
         for (int i = 0; i < 16; ++i) ov[i] = pack_bf16x2(__uint_as_float(ov[2 * i]) * inv, __uint_as_float(ov[2 * i + 1]) * inv);
         stg_v8(orow + c * 32, ov);
@@ -323,11 +337,11 @@ namespace nrl {
 namespace {
 
 template <bool GROUPS>
-cudaError_t attn_fwd_tc(const CUtensorMap* tmQ, const CUtensorMap* tmK, const CUtensorMap* tmV, void* out, float* lse, long o_stride_t, const AttnSeqs& seqs,
+cudaError_t attn_fwd_tc(const CUtensorMap* tmQ, const CUtensorMap* tmK, const CUtensorMap* tmV, void* out, void* rest, float* lse, long o_stride_t, const AttnSeqs& seqs,
                         int total, int Hq, int Hkv, float scale, int num_sms, cudaStream_t s) {
   if (total == 0) return cudaSuccess;
   AttnTcParams p;
-  p.seqs = seqs; p.out = static_cast<__nv_bfloat16*>(out); p.lse = lse; p.o_stride_t = o_stride_t;
+  p.seqs = seqs; p.out = static_cast<__nv_bfloat16*>(out); p.lse = lse; p.rest = static_cast<uint8_t*>(rest); p.o_stride_t = o_stride_t;
   p.total_tokens = total; p.Hq = Hq; p.G = Hq / Hkv;
   p.scale_log2 = scale * 1.4426950408889634f;
   static PerDevice<bool> configured;
@@ -344,12 +358,12 @@ cudaError_t attn_fwd_tc(const CUtensorMap* tmQ, const CUtensorMap* tmK, const CU
 extern "C" cudaError_t nrl_attn_fwd_tc(const CUtensorMap* tmQ, const CUtensorMap* tmK, const CUtensorMap* tmV, void* out,
                                        float* lse, long o_stride_t, const int* cu, int num_seqs, int total, int Hq, int Hkv,
                                        float scale, int num_sms, cudaStream_t s) {
-  return nrl::attn_fwd_tc<false>(tmQ, tmK, tmV, out, lse, o_stride_t, {cu, nullptr, num_seqs}, total, Hq, Hkv, scale, num_sms, s);
+  return nrl::attn_fwd_tc<false>(tmQ, tmK, tmV, out, nullptr, lse, o_stride_t, {cu, nullptr, num_seqs}, total, Hq, Hkv, scale, num_sms, s);
 }
 
 // table: attention_groups.cu
-extern "C" cudaError_t nrl_attn_groups_fwd_tc(const CUtensorMap* tmQ, const CUtensorMap* tmK, const CUtensorMap* tmV, void* out, float* lse, long o_stride_t,
-                                              const int* cu, const int* table, int num_seqs, int total, int Hq, int Hkv, float scale, int num_sms,
+extern "C" cudaError_t nrl_attn_groups_fwd_tc(const CUtensorMap* tmQ, const CUtensorMap* tmK, const CUtensorMap* tmV, void* out, void* rest, float* lse,
+                                              long o_stride_t, const int* cu, const int* table, int num_seqs, int total, int Hq, int Hkv, float scale, int num_sms,
                                               cudaStream_t s) {
-  return nrl::attn_fwd_tc<true>(tmQ, tmK, tmV, out, lse, o_stride_t, {cu, reinterpret_cast<const int4*>(table), num_seqs}, total, Hq, Hkv, scale, num_sms, s);
+  return nrl::attn_fwd_tc<true>(tmQ, tmK, tmV, out, rest, lse, o_stride_t, {cu, reinterpret_cast<const int4*>(table), num_seqs}, total, Hq, Hkv, scale, num_sms, s);
 }

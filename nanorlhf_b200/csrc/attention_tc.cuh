@@ -3,7 +3,11 @@
 #pragma once
 #include "common.cuh"
 
+#include <cuda_fp8.h>
+
 namespace nrl {
+
+constexpr float kAttnRest = 1024.f;        // of what a result's rounding to bf16 left: e5m2 ends at 2^-16, the rest of an element of 2^-17 begins there
 
 // D[tmem] (+)= A[tmem] * B[smem desc]: A is [128 lanes][K] bf16, two elements per 32-bit column
 NRL_DEVICE void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {

@@ -61,26 +61,26 @@ CUtensorMap map_of(const torch::Tensor& t, int box_rows) {
   return nrl::make_tma_2d(t.data_ptr(), t.size(0), static_cast<uint64_t>(t.size(1)) * 128, row_stride(t) * 2, box_rows, 64, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2);
 }
 
-// (out, lse [Hq, T], table of the sequences for the backward); q, k, v as head_rows gives them
-std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> attn_groups_fwd(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
-                                                                        const torch::Tensor& cu_seqlens, const torch::Tensor& cu_groups, double scale) {
+// (out, what bf16 had no room for of it, lse [Hq, T], table of the sequences: for the backward, without which the second is not formed); q, k, v as head_rows gives them
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> attn_groups_fwd(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
+                                                                        const torch::Tensor& cu_seqlens, const torch::Tensor& cu_groups, double scale, bool train) {
   const char* what = "attention_shared_prefix";
   c10::cuda::CUDAGuard guard(q.device());
   const int T = q.size(0), Hq = q.size(1), Hkv = k.size(1), n = cu_seqlens.numel() - 1;
   torch::Tensor out = torch::empty({T, Hq, 128}, q.options()), lse = torch::empty({Hq, T}, q.options().dtype(torch::kFloat32));
-  torch::Tensor table = torch::empty({n, 8}, cu_seqlens.options());
-  if (T == 0) return {out, lse, table};
+  torch::Tensor table = torch::empty({n, 8}, cu_seqlens.options()), rest = train ? torch::empty({T, Hq, 128}, q.options().dtype(torch::kUInt8)) : torch::Tensor();
+  if (T == 0) return {out, rest, lse, table};
   const CUtensorMap mq = map_of(q, 128), mk = map_of(k, 128), mv = map_of(v, 128);
   check(nrl_attn_group_table(cu_seqlens.data_ptr<int>(), cu_groups.data_ptr<int>(), table.data_ptr<int>(), n, cu_groups.numel() - 1, out.data_ptr(), T, Hq, cur_stream()),
         what);
-  check(nrl_attn_groups_fwd_tc(&mq, &mk, &mv, out.data_ptr(), lse.data_ptr<float>(), out.stride(0), cu_seqlens.data_ptr<int>(), table.data_ptr<int>(), n, T, Hq, Hkv,
+  check(nrl_attn_groups_fwd_tc(&mq, &mk, &mv, out.data_ptr(), train ? rest.data_ptr() : nullptr, lse.data_ptr<float>(), out.stride(0), cu_seqlens.data_ptr<int>(), table.data_ptr<int>(), n, T, Hq, Hkv,
                                static_cast<float>(scale), num_sms(), cur_stream()), what);
-  return {out, lse, table};
+  return {out, rest, lse, table};
 }
 
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> attn_groups_bwd(const torch::Tensor& grad, const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
-                                                                        const torch::Tensor& o, const torch::Tensor& lse, const torch::Tensor& cu_seqlens,
-                                                                        const torch::Tensor& table, double scale) {
+                                                                        const torch::Tensor& o, const torch::Tensor& rest, const torch::Tensor& lse,
+                                                                        const torch::Tensor& cu_seqlens, const torch::Tensor& table, double scale) {
   const char* what = "attention_shared_prefix backward";
   const torch::Tensor dout = grad.contiguous();
   TORCH_CHECK(dout.sizes() == o.sizes() && dout.device() == q.device() && dout.scalar_type() == torch::kBFloat16, what, ": the gradient must be like the result");
@@ -90,7 +90,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> attn_groups_bwd(const to
   if (T == 0) return {dq, dk, dv};
   torch::Tensor delta = torch::empty({Hq, T}, q.options().dtype(torch::kFloat32));
   const CUtensorMap maps[8] = {map_of(q, 64), map_of(dout, 64), map_of(k, 128), map_of(v, 128), map_of(q, 128), map_of(dout, 128), map_of(k, 64), map_of(v, 64)};
-  check(nrl_attn_groups_bwd_tc(maps, o.data_ptr(), dout.data_ptr(), lse.data_ptr<float>(), delta.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+  check(nrl_attn_groups_bwd_tc(maps, o.data_ptr(), rest.data_ptr(), dout.data_ptr(), lse.data_ptr<float>(), delta.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                o.stride(0), dq.stride(0), dk.stride(0), cu_seqlens.data_ptr<int>(), table.data_ptr<int>(), n, T, Hq, Hkv, static_cast<float>(scale),
                                cur_stream()), what);
   return {dq, dk, dv};
@@ -110,14 +110,14 @@ torch::Tensor refuse_second(const torch::Tensor& grad) {
 struct AttnGroupsFn : torch::autograd::Function<AttnGroupsFn> {
   static torch::Tensor forward(torch::autograd::AutogradContext* ctx, torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor cu_seqlens, torch::Tensor cu_groups,
                                double scale) {
-    auto [out, lse, table] = attn_groups_fwd(q, k, v, cu_seqlens, cu_groups, scale);
-    ctx->save_for_backward({q, k, v, out, lse, cu_seqlens, table});
+    auto [out, rest, lse, table] = attn_groups_fwd(q, k, v, cu_seqlens, cu_groups, scale, true);
+    ctx->save_for_backward({q, k, v, out, rest, lse, cu_seqlens, table});
     ctx->saved_data["scale"] = scale;
     return out;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
     const auto s = ctx->get_saved_variables();
-    auto [dq, dk, dv] = attn_groups_bwd(g[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6], ctx->saved_data["scale"].toDouble());
+    auto [dq, dk, dv] = attn_groups_bwd(g[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], ctx->saved_data["scale"].toDouble());
     return {refuse_second(dq), refuse_second(dk), refuse_second(dv), {}, {}, {}};
   }
 };
@@ -135,7 +135,7 @@ torch::Tensor attention_shared_prefix(const torch::Tensor& q_in, const torch::Te
                                       const torch::Tensor& cu_groups_in, const c10::optional<double>& scale_in) {
   auto [q, k, v, cu_seqlens, cu_groups, scale] = packed_arguments(q_in, k_in, v_in, cu_seqlens_in, cu_groups_in, scale_in);
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad())) return AttnGroupsFn::apply(q, k, v, cu_seqlens, cu_groups, scale);
-  return std::get<0>(attn_groups_fwd(q, k, v, cu_seqlens, cu_groups, scale));
+  return std::get<0>(attn_groups_fwd(q, k, v, cu_seqlens, cu_groups, scale, false));
 }
 
 // ---- pages -----------------------------------------------------------------------------------------------------------------------------

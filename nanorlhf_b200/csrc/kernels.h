@@ -87,9 +87,9 @@ cudaError_t nrl_attn_bwd_tc(const CUtensorMap* maps, const void* o, const void* 
 // groups of sequences that continue a prefix (attention_groups.cu): table [num_seqs, 8] ints, formed from cu_seqlens and cu_groups [num_groups + 1]; rows behind
 // the last sequence are 0 in `out` and in the gradients
 cudaError_t nrl_attn_group_table(const int* cu, const int* cu_groups, int* table, int num_seqs, int num_groups, void* out, int total, int Hq, cudaStream_t s);
-cudaError_t nrl_attn_groups_fwd_tc(const CUtensorMap* tmQ, const CUtensorMap* tmK, const CUtensorMap* tmV, void* out, float* lse, long o_stride_t, const int* cu,
-                                   const int* table, int num_seqs, int total, int Hq, int Hkv, float scale, int num_sms, cudaStream_t s);
-cudaError_t nrl_attn_groups_bwd_tc(const CUtensorMap* maps, const void* o, const void* dout, const float* lse, float* delta, void* dq, void* dk, void* dv,
+cudaError_t nrl_attn_groups_fwd_tc(const CUtensorMap* tmQ, const CUtensorMap* tmK, const CUtensorMap* tmV, void* out, void* rest, float* lse, long o_stride_t,
+                                   const int* cu, const int* table, int num_seqs, int total, int Hq, int Hkv, float scale, int num_sms, cudaStream_t s);
+cudaError_t nrl_attn_groups_bwd_tc(const CUtensorMap* maps, const void* o, const void* rest, const void* dout, const float* lse, float* delta, void* dq, void* dk, void* dv,
                                    long o_stride_t, long dq_stride_t, long dkv_stride_t, const int* cu, const int* table, int num_seqs, int total, int Hq,
                                    int Hkv, float scale, cudaStream_t s);
 }

@@ -471,8 +471,8 @@ class _RecordedSharedPrefixFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, cu_seqlens, cu_groups, scale):
-        o, lse, table = ext().attn_groups_fwd(q, k, v, cu_seqlens, cu_groups, scale)
-        ctx.save_for_backward(q, k, v, o, lse, cu_seqlens, table)
+        o, rest, lse, table = ext().attn_groups_fwd(q, k, v, cu_seqlens, cu_groups, scale, True)
+        ctx.save_for_backward(q, k, v, o, rest, lse, cu_seqlens, table)
         ctx.scale = scale
         return o
 

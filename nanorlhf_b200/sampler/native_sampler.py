@@ -346,13 +346,14 @@ class NativeSampler:
         st["shared_lens"].copy_(torch.tensor(shared + [0] * (S - G), dtype=torch.int32))
 
     def _evict(self, st, keep: int, sinks: int, recent: int):
-        """Rows of more than ``keep`` cached tokens go back to ``keep``; every layer and kv head chooses its own."""
-        fp8, lens = self.kv_dtype == "fp8", None
+        """Rows of more than ``keep`` cached tokens go back to ``keep``; every layer and kv head chooses its own.  The token that is
+        fed next counts among ctx_lens already, but is not cached yet: it comes behind what is kept."""
+        fp8, lens, cached = self.kv_dtype == "fp8", None, st["ctx_lens"] - 1
         for li, name in enumerate(self._score_names()):
-            _, scores, lens = kv_evict(self.k_cache[li], self.v_cache[li], st["block_tables"], st["ctx_lens"], st[name], keep, sinks, recent,
+            _, scores, lens = kv_evict(self.k_cache[li], self.v_cache[li], st["block_tables"], cached, st[name], keep, sinks, recent,
                                        k_scale=self.k_scale[li] if fp8 else None, v_scale=self.v_scale[li] if fp8 else None)
             st[name][:, :, :keep].copy_(scores[:, :, :st[name].shape[2]])
-        st["ctx_lens"].copy_(lens)
+        st["ctx_lens"].copy_(lens + 1)
         self.stats["evictions"] = self.stats.get("evictions", 0) + 1
 
     def _decode_step(self, st, temperature, top_p, seed, eos_id, pad_id, max_tokens):

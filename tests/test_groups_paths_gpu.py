@@ -67,7 +67,7 @@ def test_samples_over_a_bounded_cache(fp8, graph):
     longest = torch.tensor([len(p) + 40 <= 24 + 8 for p in prompts]).repeat_interleave(2)
     assert not torch.equal(narrow[~longest], wide[~longest])                                   # 16 tokens and more of 64 have gone
     st = next(v for k, v in eng._state_pool.items() if v["mode"][0] == "scored" and v["scores0"].shape[2] < 104 + 16)
-    assert int(st["ctx_lens"].max()) <= 24 and int(st["positions"].max()) == 64 + 40 - 2
+    assert int(st["ctx_lens"].max()) == 24 + 1 and int(st["positions"].max()) == 64 + 40 - 2
 
 
 def test_a_bounded_cache_keeps_what_is_looked_at():
@@ -98,6 +98,26 @@ def test_a_bounded_cache_keeps_what_is_looked_at():
         lens = lens + 1
         assert lens.tolist() == [budget + 1] * S
         assert all(t in kept[s, h].tolist() for t in [0, 1, 2, 3] + special for s in range(S) for h in range(Hkv))
+
+
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+def test_the_token_that_is_fed_next_is_not_cached_yet(fp8):
+    """it stands behind the kept ones whatever its place in the scores holds, and its place in the cache is free"""
+    eng = _engine(fp8)
+    eng.generate(_prompts((40,)), 1, 0.0, 1.0, 9, None, PAD, 1, kv_budget=47)
+    st = next(v for v in eng._state_pool.values() if v["mode"][0] == "scored")
+    st["ctx_lens"].fill_(1)
+    st["ctx_lens"][0] = 41
+    st["block_tables"][0, :3] = torch.tensor([2, 0, 1])
+    for li in range(eng.cfg.num_hidden_layers):
+        st[f"scores{li}"][0] = torch.arange(st[f"scores{li}"].shape[2], device="cuda").float()
+        st[f"scores{li}"][0, :, 40] = -1.0
+    k = eng.k_cache[0].clone()
+    eng._evict(st, 16, 0, 0)
+    assert st["ctx_lens"][0] == 17 and (st["ctx_lens"][1:] == 1).all()
+    row = lambda x, t: x[st["block_tables"][0, t // 16].long(), :, t % 16]                               # noqa: E731
+    for j in range(16):                                                                                  # tokens 24 to 39 of the forty
+        assert torch.equal(row(eng.k_cache[0], j), row(k, 24 + j)) and (st["scores1"][0, :, j] == 24 + j).all()
 
 
 def test_evicted_rows_are_moved_with_their_scores():
