@@ -799,5 +799,6 @@ extern "C" cudaError_t nrl_paged_decode_scored(const DecodeCall* c, const float*
   p.wide = (reinterpret_cast<uintptr_t>(scores_in) | reinterpret_cast<uintptr_t>(scores_out)) % 16 == 0 && (in_row | in_head | out_row | out_head) % 4 == 0;
   // tokens a block: rows' contexts whole where there are rows enough for the chip
   p.chunk = static_cast<long>(c->S) * c->Hkv >= 2L * num_sms ? 4096 : 1024;
+  while ((p.max_tokens - 1) / p.chunk + 1 > 32768 / c->Hkv) p.chunk *= 2;                       // (a grid's second dimension ends at 65 535)
   return launch_join<true>(p, (p.max_tokens + p.chunk - 1) / p.chunk, 256, s);
 }

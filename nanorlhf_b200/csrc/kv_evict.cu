@@ -188,14 +188,15 @@ __global__ void __launch_bounds__(WARPS * 32) kv_select_kernel(const EvictCall p
 constexpr int kMoveThreads = 256;
 constexpr int kMoveUnits = 8;             // pieces a thread holds
 constexpr int kMovePieces = 4;            // pieces of a token that a block moves (64 bytes)
-constexpr int kMoveRange = kMoveThreads / kMovePieces * kMoveUnits;   // places at a time
+constexpr int kMoveRange = kMoveThreads / kMovePieces * kMoveUnits;   // places of a block, where sources and targets are apart; of fewer row-heads than fill the chip fewer:
+constexpr int kMoveLeast = 64;            // a span of transposed values follows another, and 2 rows of 24 k fp8 tokens, 628 kept, took 193 us with 512 places a block
 constexpr int kSpanPages = 16;            // of transposed values at a time: their tokens are as many as the threads
 constexpr int kSpanRow = 5;               // words from an element's row to the next
 
 struct MoveParams {
   EvictCall e;
   const int* out_tables;
-  int out_blocks, key_slices;             // grid.y: kv heads x ranges of places; grid.z: slices of keys, then of values (fp8: the scales), then the scores
+  int out_blocks, key_slices, range;             // grid.y: kv heads x ranges of places; grid.z: slices of keys, then of values (fp8: the scales), then the scores
 };
 
 // where token t of a row lies: its place among all tokens (below 2^31: checked on the host)
@@ -326,7 +327,7 @@ NRL_DEVICE MoveRow move_row(const MoveParams& p) {
   const EvictCall& e = p.e;
   const int seq = blockIdx.x, kvh = blockIdx.y % e.Hkv, range = blockIdx.y / e.Hkv, n = min(e.context_lens[seq], e.max_tokens), count = max(0, min(n, e.keep));
   const long row = static_cast<long>(seq) * e.Hkv + kvh;
-  const int j0 = IN_PLACE ? 0 : range * kMoveRange, j1 = IN_PLACE ? (n > e.keep ? count : 0) : min(count, j0 + kMoveRange);
+  const int j0 = IN_PLACE ? 0 : range * p.range, j1 = IN_PLACE ? (n > e.keep ? count : 0) : min(count, j0 + p.range);
   return {e.block_tables + static_cast<long>(seq) * e.max_blocks, p.out_tables + static_cast<long>(seq) * p.out_blocks, e.kept + row * e.keep, row, kvh, j0, j1};
 }
 
@@ -336,19 +337,22 @@ __global__ void __launch_bounds__(kMoveThreads, IN_PLACE ? 2 : 4) kv_move_kernel
   pdl_wait();
   pdl_launch_dependents();
   const EvictCall& e = p.e;
-  const MoveRow m = move_row<IN_PLACE>(p);
   const int z = static_cast<int>(blockIdx.z) - (FP8 ? 1 : 0), last = FP8 ? p.key_slices + 2 : 2 * p.key_slices;
   if (z == last) {
-    float* to = e.kept_scores + m.row * e.keep;
-    const float* sc = e.scores + static_cast<long>(blockIdx.x) * e.score_row + m.kvh * e.score_head;
-    const int j0 = IN_PLACE ? 0 : blockIdx.y / e.Hkv * kMoveRange, j1 = IN_PLACE || (blockIdx.y / e.Hkv + 1) * e.Hkv == gridDim.y ? e.keep : min(e.keep, j0 + kMoveRange);
+    const int kvh = blockIdx.y % e.Hkv;
+    const long row = static_cast<long>(blockIdx.x) * e.Hkv + kvh;
+    const int* kept = e.kept + row * e.keep;
+    float* to = e.kept_scores + row * e.keep;
+    const float* sc = e.scores + static_cast<long>(blockIdx.x) * e.score_row + kvh * e.score_head;
+    const int j0 = IN_PLACE ? 0 : blockIdx.y / e.Hkv * p.range, j1 = IN_PLACE || (blockIdx.y / e.Hkv + 1) * e.Hkv == gridDim.y ? e.keep : min(e.keep, j0 + p.range);
 #pragma unroll 4
     for (int j = j0 + threadIdx.x; j < j1; j += kMoveThreads) {
-      const int t = m.kept[j];
+      const int t = kept[j];
       to[j] = t >= 0 ? sc[t] : 0.f;
     }
     return;
   }
+  const MoveRow m = move_row<IN_PLACE>(p);
   if (m.j0 >= m.j1) return;
   if constexpr (FP8) {
     if (z < 0) {
@@ -376,15 +380,19 @@ cudaError_t launch_select(const EvictCall& c, int cluster, int tokens, cudaStrea
   static PerDevice<bool> configured;
   const cudaError_t e = allow_smem(configured, kv_select_kernel<WARPS>, kSelTokens * 4);
   if (e != cudaSuccess) return e;
-  launch_dependent_clusters(kv_select_kernel<WARPS>, dim3(c.S * cluster, c.Hkv), WARPS * 32, tokens * 4, s, cluster, c, cluster);
+  const dim3 grid(c.S * cluster, c.Hkv);
+  launch_dependent_clusters(kv_select_kernel<WARPS>, grid, WARPS * 32, tokens * 4, s, cluster, c, cluster);       // (one block a cluster: 60 us where a plain launch takes 64)
   return cudaGetLastError();
 }
 
 template <bool IN_PLACE>
-cudaError_t launch_moves(const MoveParams& p, cudaStream_t s) {
+cudaError_t launch_moves(MoveParams p, int num_sms, cudaStream_t s) {
   const EvictCall& c = p.e;
   const bool fp8 = c.k_scale != nullptr;
-  const int places = c.keep < c.max_tokens ? c.keep : c.max_tokens, ranges = IN_PLACE ? 1 : (places + kMoveRange - 1) / kMoveRange;
+  const int places = c.keep < c.max_tokens ? c.keep : c.max_tokens;
+  p.range = kMoveRange;
+  while (!IN_PLACE && p.range > kMoveLeast && static_cast<long>(c.S) * c.Hkv * ((places + p.range - 1) / p.range) < 2L * num_sms) p.range /= 2;
+  const int ranges = IN_PLACE ? 1 : (places + p.range - 1) / p.range;
   const dim3 grid(c.S, c.Hkv * ranges, (fp8 ? p.key_slices + 3 : 2 * p.key_slices) + 1);
   if (fp8) launch_dependent(kv_move_kernel<IN_PLACE, true>, grid, kMoveThreads, 0, s, p);
   else launch_dependent(kv_move_kernel<IN_PLACE, false>, grid, kMoveThreads, 0, s, p);
@@ -408,5 +416,5 @@ extern "C" cudaError_t nrl_kv_evict(const EvictCall* c, int num_sms, cudaStream_
   p.out_tables = c->out_tables != nullptr ? c->out_tables : c->block_tables;
   p.out_blocks = c->out_tables != nullptr ? c->out_blocks : c->max_blocks;
   p.key_slices = (c->k_scale != nullptr ? 8 : 16) / kMovePieces;
-  return c->out_tables != nullptr ? launch_moves<false>(p, s) : launch_moves<true>(p, s);
+  return c->out_tables != nullptr ? launch_moves<false>(p, num_sms, s) : launch_moves<true>(p, num_sms, s);
 }
