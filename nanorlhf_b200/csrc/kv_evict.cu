@@ -187,9 +187,13 @@ __global__ void __launch_bounds__(WARPS * 32) kv_select_kernel(const EvictCall p
 // ---- tokens' rows: 16-byte pieces of keys (and of bf16 values), and their scales ---------------------------------------------------------------------
 constexpr int kMoveThreads = 256;
 constexpr int kMoveUnits = 8;             // pieces a thread holds
-constexpr int kMovePieces = 4;            // pieces of a token that a block moves (64 bytes)
-constexpr int kMoveRange = kMoveThreads / kMovePieces * kMoveUnits;   // places of a block, where sources and targets are apart; of fewer row-heads than fill the chip fewer:
-constexpr int kMoveLeast = 64;            // a span of transposed values follows another, and 2 rows of 24 k fp8 tokens, 628 kept, took 193 us with 512 places a block
+// 16-byte pieces of a token that a block moves.  In place a block has all places of a row, and a slice of 64 bytes: more blocks.  Where sources and targets are apart it
+// has whole rows and a range of places: of slices, indices were looked up once for each (253 fp8 rows 60.7 -> 57.2 us, 8 of 30 k bf16 tokens 70 -> 60).
+__host__ __device__ constexpr int move_pieces(bool in_place, bool fp8) { return in_place ? 4 : fp8 ? 8 : 16; }
+// Places of a block.  253 fp8 rows take 67 us with 128 (spans of transposed values meet too few), 57 with 256, 61 with 512.  Of fewer row-heads than fill the chip fewer:
+// one span of transposed values follows another, and 2 rows of 24 k fp8 tokens, 628 kept, took 193 us with 512 places a block, 47 with 64.
+__host__ __device__ constexpr int move_range(bool fp8) { return fp8 ? 256 : 128; }
+constexpr int kMoveLeast = 64;
 constexpr int kSpanPages = 16;            // of transposed values at a time: their tokens are as many as the threads
 constexpr int kSpanRow = 5;               // words from an element's row to the next
 
@@ -365,7 +369,7 @@ __global__ void __launch_bounds__(kMoveThreads, IN_PLACE ? 2 : 4) kv_move_kernel
   if (FP8 && !keys)
     move_rows<IN_PLACE, float, 1>(z == p.key_slices ? e.k_scale : e.v_scale, 1, 0, m.from, m.to, m.kept, m.j0, m.j1, e.Hkv, m.kvh);
   else
-    move_rows<IN_PLACE, uint4, kMovePieces>(static_cast<uint4*>(keys ? e.k_cache : e.v_cache), FP8 ? 8 : 16, keys ? z : z - p.key_slices, m.from, m.to, m.kept, m.j0, m.j1,
+    move_rows<IN_PLACE, uint4, move_pieces(IN_PLACE, FP8)>(static_cast<uint4*>(keys ? e.k_cache : e.v_cache), FP8 ? 8 : 16, keys ? z : z - p.key_slices, m.from, m.to, m.kept, m.j0, m.j1,
                                             e.Hkv, m.kvh);
 }
 
@@ -390,8 +394,10 @@ cudaError_t launch_moves(MoveParams p, int num_sms, cudaStream_t s) {
   const EvictCall& c = p.e;
   const bool fp8 = c.k_scale != nullptr;
   const int places = c.keep < c.max_tokens ? c.keep : c.max_tokens;
-  p.range = kMoveRange;
+  p.range = move_range(fp8);
+  p.key_slices = (fp8 ? 8 : 16) / move_pieces(IN_PLACE, fp8);
   while (!IN_PLACE && p.range > kMoveLeast && static_cast<long>(c.S) * c.Hkv * ((places + p.range - 1) / p.range) < 2L * num_sms) p.range /= 2;
+  while (static_cast<long>(c.Hkv) * ((places + p.range - 1) / p.range) > 65535) p.range *= 2;          // (a grid's second dimension)
   const int ranges = IN_PLACE ? 1 : (places + p.range - 1) / p.range;
   const dim3 grid(c.S, c.Hkv * ranges, (fp8 ? p.key_slices + 3 : 2 * p.key_slices) + 1);
   if (fp8) launch_dependent(kv_move_kernel<IN_PLACE, true>, grid, kMoveThreads, 0, s, p);
@@ -415,6 +421,5 @@ extern "C" cudaError_t nrl_kv_evict(const EvictCall* c, int num_sms, cudaStream_
   p.e = *c;
   p.out_tables = c->out_tables != nullptr ? c->out_tables : c->block_tables;
   p.out_blocks = c->out_tables != nullptr ? c->out_blocks : c->max_blocks;
-  p.key_slices = (c->k_scale != nullptr ? 8 : 16) / kMovePieces;
   return c->out_tables != nullptr ? launch_moves<false>(p, num_sms, s) : launch_moves<true>(p, num_sms, s);
 }
