@@ -7,11 +7,11 @@
 // counted again, word by word of 32, and indices and a bit a token are written in order.  Bound by latency, up to eleven rounds of a barrier (and one of the cluster).
 // (Counts of digits by atomics in shared memory meet: a score's highest bits are a few exponents, and 3750 tokens a block took 120 us with eight bits a round, 20 with eleven;
 // seven votes a word and round 20.)
-// kv_move: a block per (row, kv head, slice of a token's keys or values), and per range of places where sources and targets are apart.  In place, token j of what
-// is kept comes from a place >= j, so that a block that reads a range of places before it writes them, ranges in order and the next one on its way, may move it;
-// other slices' bytes are not touched.
-// Values of fp8 pages lie transposed, and their blocks come first, for they take longest (in a launch in front of the others' 69 us, in one 60).  Sixteen pages at a time go through shared memory, rows of 16 bytes 20 apart (no bank
-// conflicts), and a thread puts together an element's bytes of a whole page.
+// kv_move: in place a block per (row, kv head, 64 bytes of a token's keys or values): token j of what is kept comes from a place >= j, so that a block that reads a range
+// of places before it writes them, ranges in order and the next one on its way, may move it; other slices' bytes are not touched.  Where sources and targets are
+// apart a block per (row, kv head, range of places, keys or values).
+// Values of fp8 pages lie transposed, and their blocks come first, for they take longest (in a launch in front of the others' 69 us, in one 60).  Sixteen pages at a
+// time go through shared memory, rows of 16 bytes 20 apart (no bank conflicts), and a thread puts together an element's bytes of a whole page.
 #include "common.cuh"
 #include "group_kernels.h"
 #include "launch.h"
