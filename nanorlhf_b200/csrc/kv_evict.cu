@@ -17,6 +17,8 @@
 #include "launch.h"
 #include "per_device.h"
 
+#include <climits>
+
 namespace nrl {
 
 constexpr int kSelTokens = 48 * 1024;     // of a block, in shared memory; kSelCluster times as many of a row at the most (checked on the host)
@@ -255,6 +257,7 @@ NRL_DEVICE void move_transposed(uint4* v, long step, const int* from, const int*
   __shared__ uint32_t left[2][128 * kSpanRow];                        // places of a page that is not full yet: read by one span, written by it for the next
   __shared__ __align__(16) uint32_t place[kMoveThreads + 16];         // of the span's kept tokens, from the first place of their page on: the byte of element 0
   const int tid = threadIdx.x, d = tid & 127, warp_half = tid >> 7;
+  __shared__ int ahead[2];                                            // the page of the first kept token behind the span, as far as the threads have looked
   const int last = kept[j1 - 1] >> 4;
   int page = kept[j0] >> 4, j = j0, turn = 0;
   uint4 cur[kMoveUnits];
@@ -266,7 +269,9 @@ NRL_DEVICE void move_transposed(uint4* v, long step, const int* from, const int*
     }
   };
   read(page);
-  for (; j < j1; page += kSpanPages, turn ^= 1) {
+  if (tid < 2) ahead[tid] = INT_MAX;
+  __syncthreads();
+  while (j < j1) {
     const int t = j + tid < j1 ? kept[j + tid] : -1;
     const bool here = t >= 0 && (t >> 4) < page + kSpanPages;
 #pragma unroll
@@ -275,8 +280,11 @@ NRL_DEVICE void move_transposed(uint4* v, long step, const int* from, const int*
       w[0] = cur[u].x; w[1] = cur[u].y; w[2] = cur[u].z; w[3] = cur[u].w;
     }
     if (here) place[(j & 15) + tid] = ((t >> 4) - page) * 128 * kSpanRow * 4 + (t & 15);
+    const int warp_ahead = __reduce_min_sync(0xffffffffu, t >= 0 && !here ? t >> 4 : INT_MAX);
+    if ((tid & 31) == 0 && warp_ahead != INT_MAX) atomicMin(&ahead[turn], warp_ahead);
     const int to_j = j + __syncthreads_count(here);                   // places [j, to_j) come from this span
-    if (to_j < j1) read(page + kSpanPages);
+    const int next = ahead[turn] != INT_MAX ? ahead[turn] : page + kSpanPages;         // (pages between that keep nothing are passed over)
+    if (to_j < j1) read(next);
     const uint8_t* bytes = reinterpret_cast<const uint8_t*>(span) + d * kSpanRow * 4;
     for (int pg = (j >> 4) + warp_half; pg * 16 < to_j; pg += 2) {
       uint32_t word[4];
@@ -317,6 +325,9 @@ NRL_DEVICE void move_transposed(uint4* v, long step, const int* from, const int*
       }
     }
     j = to_j;
+    page = next;
+    if (tid == 0) ahead[turn ^ 1] = INT_MAX;
+    turn ^= 1;
     __syncthreads();                                                  // `left` is written, span and places are read
   }
 }
