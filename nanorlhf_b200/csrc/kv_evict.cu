@@ -41,7 +41,8 @@ NRL_DEVICE void evict_cluster_sync() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// WARPS: 4 for up to 2048 tokens a block, where sums over more warps cost more than their share of the words saves
+// WARPS: 4 for up to 2048 tokens a block, 8 for up to 3840, else 16: sums over more warps cost more than their share of the words saves (3752 tokens a block: 60 us of a
+// call with 16 warps, 58 with 8, 69 with 4; 4096: 27 with 16, 29 with 8, 34 with 4)
 template <int WARPS>
 __global__ void __launch_bounds__(WARPS * 32) kv_select_kernel(const EvictCall p, const int cluster) {
   constexpr int kSelWarps = WARPS, kSelThreads = WARPS * 32;
@@ -426,7 +427,7 @@ extern "C" cudaError_t nrl_kv_evict(const EvictCall* c, int num_sms, cudaStream_
                                    c->max_tokens > static_cast<long>(cluster) * kSelTokens)) cluster *= 2;
   const int tokens = ((c->max_tokens + 31) / 32 + cluster - 1) / cluster * 32;
   if (tokens > kSelTokens) return cudaErrorInvalidValue;
-  cudaError_t e = tokens <= 2048 ? launch_select<4>(*c, cluster, tokens, s) : launch_select<16>(*c, cluster, tokens, s);
+  cudaError_t e = tokens <= 2048 ? launch_select<4>(*c, cluster, tokens, s) : tokens <= 3840 ? launch_select<8>(*c, cluster, tokens, s) : launch_select<16>(*c, cluster, tokens, s);
   if (e != cudaSuccess) return e;
   MoveParams p;
   p.e = *c;
