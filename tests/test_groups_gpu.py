@@ -318,6 +318,24 @@ def test_many_groups_and_long_prefixes(fp8, wide):
 
 
 @pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("rows", [127, 128, 129])
+def test_around_the_rows_for_which_every_block_plans(rows, fp8):
+    groups = [(33, [34 + i % 40 for i in range(rows - 60)]), (0, [i % 5 for i in range(20)]), (100, [90 + i for i in range(40)])]
+    st = shared_batch(75, groups, 2, fp8)
+    q = torch.randn(rows, 12, 128, generator=gen(75), device=DEV).to(torch.bfloat16)
+    out = ops.paged_decode_shared(q, st["k"], st["v"], st["tables"], st["context"], st["cu"], st["shared"], k_scale=st["ks"], v_scale=st["vs"])
+    row = 0
+    for shared, ctxs in groups:
+        first = row
+        for c in ctxs:
+            n = min(shared, c)
+            parts = zip(oracle.page_rows(st, st["tables"][first], n), (x[:, n:] for x in oracle.page_rows(st, st["tables"][row], c)))
+            want, bound, _, _ = oracle.decode_row(q[row], *(torch.cat(x, 1) for x in parts), SCALE, fp8)
+            within(out[row], want, bound, f"row {row}")
+            row += 1
+
+
+@pytest.mark.parametrize("fp8", [False, True])
 def test_decode_over_shared_pages_in_two_graphs(fp8):
     """Two captured calls of other batches, replayed in turn and with other inputs."""
     calls = []
@@ -440,10 +458,11 @@ def test_evict_by_several_blocks_a_row(contexts, keep):
     evict_both(st, random_scores(38, len(contexts), 1, max(contexts)), keep, 16, 100)
 
 
+@pytest.mark.parametrize("keep", [61, 700])
 @pytest.mark.parametrize("apart", [False, True])
-def test_evict_from_far_apart(apart):
-    """What is kept lies many pages apart: values of fp8 pages that wait for a page to be full, over spans without any."""
-    n, keep = 4000, 61
+def test_evict_from_far_apart(apart, keep):
+    """What is kept lies many pages apart: values of fp8 pages that wait for a page to be full, over spans without any; and by several blocks a row."""
+    n = 4000
     st = shared_batch(39, [(0, [n])], 2, True)
     scores = torch.zeros(1, 2, n, device=DEV)
     scores[0, 0, 5::97], scores[0, 1, [3, 4, 1000, 3990]] = 1.0, 2.0
@@ -451,8 +470,8 @@ def test_evict_from_far_apart(apart):
     if apart:
         m = st["k"].shape[0]
         for name in ("k", "v", "ks", "vs"):
-            st[name] = torch.cat([st[name], torch.zeros_like(st[name][:4])])
-        to = torch.arange(m, m + 4, device=DEV).int()[None]
+            st[name] = torch.cat([st[name], torch.zeros_like(st[name][:44])])
+        to = torch.arange(m, m + 44, device=DEV).int()[None]
     evict_both(st, scores, keep, 0, 3, to)
 
 
