@@ -33,11 +33,13 @@ double scale_of(const c10::optional<double>& scale, const char* what) {
   TORCH_CHECK_VALUE(!scale.has_value() || std::isfinite(*scale), what, ": scale must be finite, got ", *scale);
   return scale.value_or(0.08838834764831845);                         // 1 / sqrt(128)
 }
-// [rows, heads, 128] whose heads lie side by side and whose rows start on 16 bytes: a view of a projection stays one
+// A copy where the first element is not on 16 bytes: `contiguous` leaves a contiguous slice of a buffer where it is
+torch::Tensor on_16(const torch::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone(at::MemoryFormat::Contiguous); }
+// [rows, heads, 128] whose heads lie side by side and whose rows start on 16 bytes: a view of a projection stays one, rows that are one row repeated do not
 torch::Tensor head_rows(const torch::Tensor& t) {
-  const bool ok = t.stride(2) == 1 && (t.stride(1) == 128 || t.size(1) == 1) && (t.size(0) <= 1 || t.stride(0) % 8 == 0) &&
-                  reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-  return ok || t.numel() == 0 ? t : t.contiguous();
+  if (t.numel() == 0) return t;
+  const bool laid = t.stride(2) == 1 && (t.stride(1) == 128 || t.size(1) == 1) && (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) > 0));
+  return on_16(laid ? t : t.contiguous());
 }
 int64_t row_stride(const torch::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1) * 128; }
 
@@ -82,7 +84,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> attn_groups_bwd(const to
                                                                         const torch::Tensor& o, const torch::Tensor& rest, const torch::Tensor& lse,
                                                                         const torch::Tensor& cu_seqlens, const torch::Tensor& table, double scale) {
   const char* what = "attention_shared_prefix backward";
-  const torch::Tensor dout = grad.contiguous();
+  const torch::Tensor dout = on_16(grad.contiguous());
   TORCH_CHECK(dout.sizes() == o.sizes() && dout.device() == q.device() && dout.scalar_type() == torch::kBFloat16, what, ": the gradient must be like the result");
   c10::cuda::CUDAGuard guard(q.device());
   const int T = q.size(0), Hq = q.size(1), Hkv = k.size(1), n = cu_seqlens.numel() - 1;

@@ -1,0 +1,67 @@
+"""Attention over shared prefixes, decode attention over pages with scores and eviction: calls at the borders of what their documentation allows."""
+import math
+
+import pytest
+import torch
+
+import groups_oracle as oracle
+from nanorlhf_b200 import ops
+from nanorlhf_b200.ops import native
+from tests.test_groups_gpu import DEV, SCALE, gen, offsets, packed_inputs, shared_batch, within
+
+pytestmark = pytest.mark.gpu
+
+
+def offset(x):
+    """the same numbers, contiguous, in a buffer of which they begin at the second element"""
+    return torch.cat([x.new_zeros(1), x.reshape(-1)])[1:].view(x.shape)
+
+
+# ---- where inputs lie ----------------------------------------------------------------------------------------------------------------------
+def test_packed_inputs_that_do_not_start_on_16_bytes():
+    groups = [[33, 20, 70], [5]]
+    q, k, v, dout, cu, cg = packed_inputs(groups, 4, 2, 101)
+    # first what the kernels are handed, without a launch
+    for x in native.ext().attn_groups_arguments(offset(q), offset(k), offset(v), cu, cg, None)[:3]:
+        assert x.data_ptr() % 16 == 0
+    results = []
+    for place in (lambda x: x.contiguous(), offset):
+        leaves = [place(x).detach().requires_grad_() for x in (q, k, v)]
+        out = ops.attention_shared_prefix(*leaves, cu, cg)
+        results.append((out.detach(), *torch.autograd.grad(out, leaves, place(dout))))
+    assert all(x.data_ptr() % 16 for x in leaves)
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+def test_packed_inputs_of_one_row_repeated():
+    """expanded rows, and a gradient that is one (of a sum)"""
+    groups = [[33, 20]]
+    q, k, v, _, cu, cg = packed_inputs(groups, 4, 2, 102)
+    q, k, v = (x[:1].expand(53, -1, -1) for x in (q, k, v))
+    dout = torch.ones(1, 1, 1, dtype=torch.bfloat16, device=DEV).expand(53, 4, 128)
+    for x in native.ext().attn_groups_arguments(q, k, v, cu, cg, None)[:3]:
+        assert x.stride(0) > 0
+    results = []
+    for place in (lambda x: x.contiguous(), lambda x: x):
+        leaves = [place(x).detach().requires_grad_() for x in (q, k, v)]
+        out = ops.attention_shared_prefix(*leaves, cu, cg)
+        results.append((out.detach(), *torch.autograd.grad(out, leaves, place(dout))))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_decode_queries_that_do_not_start_on_16_bytes(fp8):
+    st = shared_batch(103, [(100, [133, 101, 117]), (0, [33])], 2, fp8)
+    q = torch.randn(4, 12, 128, generator=gen(103), device=DEV).to(torch.bfloat16)
+    kw = {"k_scale": st["ks"], "v_scale": st["vs"]}
+    args, rows = (st["k"], st["v"], st["tables"], st["context"]), []
+    for x in (q, offset(q), q[:1].expand(4, -1, -1), q[:1].expand(4, -1, -1).contiguous()):
+        scores = torch.zeros(4, 2, 133, device=DEV)
+        out, _ = ops.paged_decode_scored(x, *args, scores, **kw)
+        rows.append((ops.paged_decode_shared(x, *args, st["cu"], st["shared"], **kw), out, scores))
+    bits = lambda x: x.view(torch.int16 if x.dtype == torch.bfloat16 else torch.int32)  # noqa: E731
+    for i in (0, 2):
+        for a, b in zip(rows[i], rows[i + 1]):
+            assert torch.equal(bits(a), bits(b))              # (the scored rows' own copies of shared tokens are NaN)
