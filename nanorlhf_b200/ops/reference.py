@@ -93,7 +93,8 @@ def attention_shared_prefix(q, k, v, cu_seqlens, cu_groups, scale: Optional[floa
         hidden = torch.ones(n, n, dtype=torch.bool, device=q.device).triu(1)
         att = att.masked_fill(torch.cat([hidden.new_zeros(n, extra), hidden], 1), float("-inf"))
         rows.append(torch.matmul(att.softmax(-1), vs).transpose(0, 1))
-    return torch.cat(rows + [q.new_zeros(q.shape[0] - cs[-1], *q.shape[1:])]).to(dtype)
+    nothing = q[:0].sum() + k[:0].sum() + v[:0].sum()    # 0, of which all three have a gradient where no sequence looks at them
+    return torch.cat(rows + [q.new_zeros(q.shape[0] - cs[-1], *q.shape[1:]) + nothing]).to(dtype)
 
 
 def _page_tokens(k_cache, v_cache, table, n, k_scale=None, v_scale=None):
