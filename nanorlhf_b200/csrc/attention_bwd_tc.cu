@@ -60,10 +60,13 @@ NRL_DEVICE bool bwd_locate(const AttnSeqs& seqs, int rank, int* info, int& block
     }
     const int src = found ? attn_nth_of<GROUPS, KEYS, 128>(seqs, lo, rank - above, lane) : 0;
     if (lane == 0) {
-      const AttnSeq q = attn_seq<GROUPS>(seqs, src);
-      const AttnLevels l = attn_levels<GROUPS, KEYS, 128>(seqs, src);
-      info[0] = found; info[1] = KEYS ? l.top - 1 - lo : lo - (l.top - l.blocks); info[2] = q.start; info[3] = q.len;
-      if (GROUPS) { info[4] = q.prefix_start; info[5] = q.prefix_len; info[6] = q.seen_by; }
+      info[0] = found;
+      if (found) {                                             // (there may be no sequence to look at)
+        const AttnSeq q = attn_seq<GROUPS>(seqs, src);
+        const AttnLevels l = attn_levels<GROUPS, KEYS, 128>(seqs, src);
+        info[1] = KEYS ? l.top - 1 - lo : lo - (l.top - l.blocks); info[2] = q.start; info[3] = q.len;
+        if (GROUPS) { info[4] = q.prefix_start; info[5] = q.prefix_len; info[6] = q.seen_by; }
+      }
     }
   }
   __syncthreads();
@@ -574,6 +577,7 @@ cudaError_t attn_bwd_tc(const CUtensorMap* maps, const void* o, const void* rest
   p.scale = scale; p.scale_log2 = scale * 1.4426950408889634f;
   launch_dependent(attn_bwd_delta_tc_kernel<GROUPS>, (pairs + 31) / 32, 256, 0, s, static_cast<const __nv_bfloat16*>(o), static_cast<const uint8_t*>(rest),
                    static_cast<const __nv_bfloat16*>(dout), delta, o_stride_t, total, static_cast<unsigned>(Hq), pairs, p);
+  if (GROUPS && seqs.num == 0) return cudaGetLastError();                      // all rows have been cleared
   const unsigned most = total / 128 + seqs.num, grid_kv = most * Hkv, grid_q = most * Hq;
   launch_dependent(attn_bwd_tc_kernel<GROUPS>, grid_kv + grid_q, kBwdThreads, smem, s, maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], maps[6], maps[7], p,
                    grid_kv);

@@ -339,7 +339,7 @@ namespace {
 template <bool GROUPS>
 cudaError_t attn_fwd_tc(const CUtensorMap* tmQ, const CUtensorMap* tmK, const CUtensorMap* tmV, void* out, void* rest, float* lse, long o_stride_t, const AttnSeqs& seqs,
                         int total, int Hq, int Hkv, float scale, int num_sms, cudaStream_t s) {
-  if (total == 0) return cudaSuccess;
+  if (total == 0 || (GROUPS && seqs.num == 0)) return cudaSuccess;             // (rows of no sequence have been cleared: attention_groups.cu)
   AttnTcParams p;
   p.seqs = seqs; p.out = static_cast<__nv_bfloat16*>(out); p.lse = lse; p.rest = static_cast<uint8_t*>(rest); p.o_stride_t = o_stride_t;
   p.total_tokens = total; p.Hq = Hq; p.G = Hq / Hkv;

@@ -65,3 +65,19 @@ def test_decode_queries_that_do_not_start_on_16_bytes(fp8):
     for i in (0, 2):
         for a, b in zip(rows[i], rows[i + 1]):
             assert torch.equal(bits(a), bits(b))              # (the scored rows' own copies of shared tokens are NaN)
+
+
+@pytest.mark.parametrize("rows", [5, 300])
+@pytest.mark.parametrize("groups", [0, 2])
+def test_rows_without_any_sequence(rows, groups):
+    """they are behind the last one: 0, and so are their gradients"""
+    q, k, v, dout, cu, _ = packed_inputs([[rows]], 4, 2, 104)
+    cu, cg = cu[:1].contiguous(), torch.zeros(groups + 1, dtype=torch.int32, device=DEV)
+    junk = torch.full((50, 1024, 128), float("nan"), device=DEV)             # what the allocator hands out next is not zero
+    del junk
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    out = ops.attention_shared_prefix(*leaves, cu, cg)
+    for x in (out, *torch.autograd.grad(out, leaves, dout)):
+        assert torch.equal(x, torch.zeros_like(x))
+    with torch.no_grad():
+        assert torch.equal(ops.attention_shared_prefix(q, k, v, cu, cg), torch.zeros_like(q))
