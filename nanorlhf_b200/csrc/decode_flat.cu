@@ -136,9 +136,15 @@ __global__ void __launch_bounds__(kPlanThreads) decode_plan_kernel(const FlatPar
   pdl_wait();
   pdl_launch_dependents();
   __shared__ int warp_sums[32];
-  __shared__ int cu_near[kPlanThreads + 1], from_near[kPlanThreads];
+  __shared__ int cu_near[kPlanThreads + 1], from_near[kPlanThreads], longest_near[kPlanThreads];
   const int tid = threadIdx.x;
   const int* cu = p.cu_groups;
+  // of every group the longest context: no page of the prefix behind it is anybody's, whatever the table says of it
+  const bool prefixes = p.prefix_runs > 0, near = p.n_groups <= kPlanThreads;
+  if (prefixes) {
+    for (int g = tid; g < p.n_groups; g += kPlanThreads) (near ? longest_near[g] : p.groups[g].z) = 0;
+    __syncthreads();
+  }
   if (p.n_groups > 0 && p.n_groups <= kPlanThreads) {
     for (int i = tid; i <= p.n_groups; i += kPlanThreads) cu_near[i] = p.cu_groups[i];
     cu = cu_near;
@@ -158,6 +164,7 @@ __global__ void __launch_bounds__(kPlanThreads) decode_plan_kernel(const FlatPar
           const int shared = p.shared[g];
           prefix = shared > 0 ? g + 1 : 0;
           first = max(0, min(shared, ctx));
+          if (prefixes) atomicMax(near ? &longest_near[g] : &p.groups[g].z, ctx);
         }
       }
       n = flat_pages(p, ctx, first);
@@ -178,14 +185,14 @@ __global__ void __launch_bounds__(kPlanThreads) decode_plan_kernel(const FlatPar
   __syncthreads();
   for (int g0 = 0; g0 < p.n_groups; g0 += kPlanThreads) {
     const int g = g0 + tid;
-    int rows = 0, tiles = 0, steps = 0;
+    int rows = 0, steps = 0, tokens = 0;
     if (g < p.n_groups && group_ok(g)) {
       rows = (cu[g + 1] - cu[g]) * p.G;
-      tiles = (rows + kPrefixRows - 1) / kPrefixRows;
-      steps = (max(0, min(p.shared[g], p.max_blocks * 16)) + kPrefixKeys - 1) / kPrefixKeys;
+      tokens = max(0, min(p.shared[g], near ? longest_near[g] : __ldcg(&p.groups[g].z)));
+      steps = (tokens + kPrefixKeys - 1) / kPrefixKeys;
     }
-    off = before + plan_scan(steps * tiles * p.Hkv, warp_sums, all);
-    if (g < p.n_groups) p.groups[g] = make_int4(off, steps, tiles, rows);
+    off = before + plan_scan(steps * prefix_tiles(rows) * p.Hkv, warp_sums, all);
+    if (g < p.n_groups) p.groups[g] = make_int4(off, steps, tokens, rows);
     from_near[tid] = off;
     before += all;
   }
@@ -536,9 +543,9 @@ NRL_DEVICE FlatParts flat_parts(const FlatParams& p, int4 row, int s, int h, int
 // and of the prefix's, one a run
 NRL_DEVICE FlatParts prefix_parts(const FlatParams& p, int g, int s, int h, int r) {
   const int4 group = p.groups[g];
-  const int first = p.cu_groups[g], row = (s - first) * p.G + r, run = p.groups[p.n_groups].y, a = group.x + (h * group.z + row / kPrefixRows) * group.y, c0 = a / run;
+  const int first = p.cu_groups[g], row = (s - first) * p.G + r, run = p.groups[p.n_groups].y, a = group.x + (h * prefix_tiles(group.w) + row / kPrefixRows) * group.y, c0 = a / run;
   const long at = prefix_part_row(p, first, h, group.w, row) + static_cast<long>(kPrefixRows) * c0;
-  return {reinterpret_cast<const float2*>(p.prefix_ml) + at, reinterpret_cast<const float4*>(p.prefix_o) + at * 32, (a + group.y - 1) / run - c0 + 1};
+  return {reinterpret_cast<const float2*>(p.prefix_ml) + at, reinterpret_cast<const float4*>(p.prefix_o) + at * 32, group.y > 0 ? (a + group.y - 1) / run - c0 + 1 : 0};
 }
 NRL_DEVICE void join_part(float2 e, float4 o, float& M, float& L, float4& acc) {
   if (e.x == -INFINITY) return;

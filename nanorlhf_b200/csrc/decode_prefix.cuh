@@ -36,7 +36,7 @@ struct PreSmem {
 struct PreWalk {
   int g, h, tile, step, n;
   int first, rows;                                 // the group's first row; query rows of a kv head
-  int shared, tiles, steps;                        // tokens; the group's tiles and steps
+  int shared, tiles, steps;                        // tokens that any row sees; the group's tiles and steps
   int left, at;                                    // steps of the run from this segment on; kv head x tiles + tile
   NRL_DEVICE PreWalk(const FlatParams& p, int run) {
     const int4 all = p.groups[p.n_groups], start = p.prefix_starts[run];               // all steps, steps a run
@@ -48,8 +48,8 @@ struct PreWalk {
     const int4 x = p.groups[group];
     g = group; step = from;
     first = p.cu_groups[g];
-    shared = min(p.shared[g], p.max_blocks * 16);
-    steps = x.y; tiles = x.z; rows = x.w;
+    steps = x.y; shared = x.z; rows = x.w;
+    tiles = prefix_tiles(rows);
     h = at / tiles; tile = at - h * tiles;
     n = min(left, steps - step);
   }

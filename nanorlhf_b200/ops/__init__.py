@@ -312,6 +312,7 @@ def paged_decode_shared(q, k_cache, v_cache, block_tables, context_lens, cu_grou
     ``k_scale`` and ``v_scale`` [blocks, Hkv, 16] the e4m3 pages of the sampler).  Group g has rows cu_groups[g] .. cu_groups[g + 1] (int32), ``max_group`` of them at
     most (a host number; None: S), and shares its first shared_lens[g] tokens: they are read from the pages of its first row, whatever the tables of its others say of
     whole pages among them.  A row sees its first context_lens tokens, the shared ones among them; with none its result is 0; rows of no group are plain.
+    What is shared ends with the longest row of the group: nothing behind it is read.  A non-finite shared value may reach rows of the group that end before it.
     No gradient."""
     if use_native(k_cache):
         return _nat().paged_decode_shared(q, k_cache, v_cache, block_tables, context_lens, cu_groups, shared_lens, max_group, k_scale, v_scale, scale)

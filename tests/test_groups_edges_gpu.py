@@ -7,7 +7,7 @@ import torch
 import groups_oracle as oracle
 from nanorlhf_b200 import ops
 from nanorlhf_b200.ops import native
-from tests.test_groups_gpu import DEV, SCALE, gen, offsets, packed_inputs, shared_batch, within
+from tests.test_groups_gpu import DEV, SCALE, fill, gen, offsets, packed_inputs, pages_of, shared_batch, widen, within
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +81,49 @@ def test_rows_without_any_sequence(rows, groups):
         assert torch.equal(x, torch.zeros_like(x))
     with torch.no_grad():
         assert torch.equal(ops.attention_shared_prefix(q, k, v, cu, cg), torch.zeros_like(q))
+
+
+# ---- shared pages --------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("groups", [[(200, [50, 0, 33, 64]), (70, [0, 0]), (64, [100])], [(200, [65 + i % 40 for i in range(40)])],
+                                    [(40 + 100 * (i % 3), [(7 * i) % 60, i % 5]) for i in range(1100)]], ids=["short", "one", "many"])
+def test_shared_tokens_behind_all_contexts_are_nobodys(groups, fp8, wide):
+    """Rows that all end inside what they share: tables need not say anything of the pages behind, and places behind the longest row hold anything."""
+    kv, heads, width = 2, 12, 13
+    rows, blocks = [], 1
+    for shared, ctxs in groups:
+        n = (max(ctxs) + 15) // 16
+        first = list(range(blocks, blocks + n))
+        blocks += n
+        for c in ctxs:
+            whole = first[:shared // 16]
+            own = max(0, (c + 15) // 16 - len(whole))
+            rows.append((whole if c else []) + list(range(blocks, blocks + own)))
+            blocks += own
+        rows[len(rows) - len(ctxs)] = first                    # the first row's pages hold what anybody sees of the prefix
+    st, g = pages_of(105, blocks, kv, fp8), gen(105)           # (page 0, of NaN, stands for what tables hold behind)
+    at = 0
+    for shared, ctxs in groups:
+        fill(st, g, rows[at], 0, max(ctxs))
+        for i, c in enumerate(ctxs):
+            if i:
+                fill(st, g, rows[at + i], shared, c)
+        at += len(ctxs)
+    st["tables"] = torch.tensor([r + [0] * (width - len(r)) for r in rows], dtype=torch.int32, device=DEV)
+    st["context"] = torch.tensor([c for _, cs in groups for c in cs], dtype=torch.int32, device=DEV)
+    cu, shared_lens = offsets([len(cs) for _, cs in groups]), torch.tensor([n for n, _ in groups], dtype=torch.int32, device=DEV)
+    if wide:
+        widen(st)
+    q = torch.randn(len(rows), heads, 128, generator=gen(106), device=DEV).to(torch.bfloat16)
+    out = ops.paged_decode_shared(q, st["k"], st["v"], st["tables"], st["context"], cu, shared_lens, k_scale=st["ks"], v_scale=st["vs"])
+    row = 0
+    for i, (shared, ctxs) in enumerate(groups):
+        first = row
+        for c in ctxs:
+            if len(groups) < 10 or i % 37 < 2:
+                n = min(shared, c)
+                parts = zip(oracle.page_rows(st, st["tables"][first], n), (x[:, n:] for x in oracle.page_rows(st, st["tables"][row], c)))
+                want, bound, _, _ = oracle.decode_row(q[row], *(torch.cat(x, 1) for x in parts), SCALE, fp8)
+                within(out[row], want, bound, f"row {row}")
+            row += 1
