@@ -2,6 +2,7 @@
 #include "bindings_groups.h"
 
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -58,6 +59,9 @@ void check_packed(const torch::Tensor& q, const torch::Tensor& k, const torch::T
   TORCH_CHECK_TYPE(q.is_cuda() && q.scalar_type() == torch::kBFloat16 && q.size(2) == 128, what, ": on CUDA bf16 and a head size of 128 are needed, got ", q.scalar_type(),
                    " and ", q.size(2));
   TORCH_CHECK_VALUE(q.size(0) * q.size(1) <= kIntMax, what, ": too many rows");
+  // the kernels would leave a tangent behind, whether autograd records or not
+  for (const torch::Tensor* t : {&q, &k, &v})
+    TORCH_CHECK(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t->_fw_grad(0).defined(), what, ": there is no forward-mode derivative");
 }
 CUtensorMap map_of(const torch::Tensor& t, int box_rows) {
   return nrl::make_tma_2d(t.data_ptr(), t.size(0), static_cast<uint64_t>(t.size(1)) * 128, row_stride(t) * 2, box_rows, 64, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2);

@@ -271,7 +271,8 @@ def attention_shared_prefix(q, k, v, cu_seqlens, cu_groups, max_seqlen=None, sca
     """Causal attention of packed groups: ``q`` [T, Hq, D], ``k`` and ``v`` [T, Hkv, D], sequence s in rows cu_seqlens[s] .. cu_seqlens[s + 1], group g of the sequences
     cu_groups[g] .. cu_groups[g + 1] (int32).  The first sequence of a group is the *prefix* of its others: their rows see all of it, then their own sequence up to
     themselves, as if the prefix stood in front of each of them; it is computed once.  Lengths may be 0.  A sequence of no group, and one that is its group's only
-    one, is plain (``attention_varlen``).  Rows behind the last sequence are 0, and so are their gradients.  Differentiable once in q, k and v.
+    one, is plain (``attention_varlen``).  Rows behind the last sequence are 0, and so are their gradients.  Differentiable once in q, k and v (on CUDA
+    in reverse mode: a tangent is refused).
     On CUDA bf16 and D = 128; q, k and v may be views of a projection.  ``max_seqlen`` is not needed.  A non-finite value in one sequence may reach the ones packed
     beside it."""
     if use_native(q):

@@ -83,6 +83,23 @@ def test_rows_without_any_sequence(rows, groups):
         assert torch.equal(ops.attention_shared_prefix(q, k, v, cu, cg), torch.zeros_like(q))
 
 
+@pytest.mark.parametrize("recorded", [False, True])
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_a_tangent_is_refused(which, recorded):
+    """... and not lost; inputs without one go through"""
+    import torch.autograd.forward_ad as fwd
+    *qkv, _, cu, cg = packed_inputs([[4, 4]], 2, 1, 107)
+    qkv = [x.contiguous().requires_grad_(recorded) for x in qkv]
+    plain = ops.attention_shared_prefix(*qkv, cu, cg)
+    with fwd.dual_level():
+        assert torch.equal(ops.attention_shared_prefix(*qkv, cu, cg), plain)
+        qkv[which] = fwd.make_dual(qkv[which], torch.ones_like(qkv[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.attention_shared_prefix(*qkv, cu, cg)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            ops.attention_shared_prefix(*qkv, cu, cg)
+
+
 # ---- shared pages --------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("fp8", [False, True])
