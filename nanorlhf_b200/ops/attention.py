@@ -59,6 +59,7 @@ def attention_varlen(q, k, v, cu_seqlens, max_seqlen=None, causal=True, scale=No
     if impl == "native":
         cu = cu_seqlens.to(torch.int32)
         needs_grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+        needs_grad = needs_grad or torch.autograd.forward_ad._current_level >= 0         # (a tangent is refused there, and not left behind)
         if not needs_grad and _USE_TC and q.shape[-1] == 128:
             # inference (rollout prefill, log-prob passes): the TMA maps take strided q/k/v views as they are
             from . import native

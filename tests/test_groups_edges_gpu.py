@@ -100,6 +100,18 @@ def test_a_tangent_is_refused(which, recorded):
             ops.attention_shared_prefix(*qkv, cu, cg)
 
 
+@pytest.mark.parametrize("recorded", [False, True])
+def test_a_tangent_is_refused_by_plain_packed_attention(recorded):
+    import torch.autograd.forward_ad as fwd
+    *qkv, _, cu, _ = packed_inputs([[4], [5]], 2, 1, 108)
+    qkv = [x.contiguous().requires_grad_(recorded) for x in qkv]
+    plain = ops.attention_varlen(*qkv, cu, 5)
+    with fwd.dual_level():
+        assert torch.equal(ops.attention_varlen(*qkv, cu, 5), plain)
+        with pytest.raises(RuntimeError):
+            ops.attention_varlen(fwd.make_dual(qkv[0], torch.ones_like(qkv[0])), *qkv[1:], cu, 5)
+
+
 # ---- shared pages --------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("fp8", [False, True])
