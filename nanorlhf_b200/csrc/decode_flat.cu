@@ -547,8 +547,10 @@ NRL_DEVICE FlatParts prefix_parts(const FlatParams& p, int g, int s, int h, int 
   const long at = prefix_part_row(p, first, h, group.w, row) + static_cast<long>(kPrefixRows) * c0;
   return {reinterpret_cast<const float2*>(p.prefix_ml) + at, reinterpret_cast<const float4*>(p.prefix_o) + at * 32, group.y > 0 ? (a + group.y - 1) / run - c0 + 1 : 0};
 }
+// A part that has seen nothing has maximum -inf and sum 0; one that has seen nothing but NaN has sum NaN, as the maximum passes them over
+NRL_DEVICE bool nothing_seen(float2 e) { return e.x == -INFINITY && e.y == 0.f; }
 NRL_DEVICE void join_part(float2 e, float4 o, float& M, float& L, float4& acc) {
-  if (e.x == -INFINITY) return;
+  if (nothing_seen(e)) return;
   const float top = fmaxf(M, e.x), a = exp2f(M - top), b = exp2f(e.x - top);          // 2^-inf = 0
   L = L * a + e.y * b;
   acc.x = acc.x * a + o.x * b; acc.y = acc.y * a + o.y * b; acc.z = acc.z * a + o.z * b; acc.w = acc.w * a + o.w * b;
@@ -572,7 +574,7 @@ NRL_DEVICE void join_parts(const FlatParts& x, int from, int lane, float& M, flo
   }
 }
 NRL_DEVICE void join_store(const FlatParams& p, int s, int head, int lane, float L, float4 acc) {
-  const float f = L > 0.f ? 1.f / L : 0.f;
+  const float f = L == 0.f ? 0.f : 1.f / L;
   uint2 v;
   v.x = pack_bf16x2(acc.x * f, acc.y * f);
   v.y = pack_bf16x2(acc.z * f, acc.w * f);
@@ -620,18 +622,18 @@ __global__ void __launch_bounds__(kJoinWarps * 32) decode_join_kernel(const Flat
 #pragma unroll 8
       for (int i = lane; i < own.n; i += 32) {
         const float2 e = own.ml[i * 8];
+        if (nothing_seen(e)) continue;
         const float m = fmaxf(M, e.x);
-        if (m == -INFINITY) continue;
         L = L * exp2f(M - m) + e.y * exp2f(e.x - m);
         M = m;
       }
       const float all = warp_max(M);
-      L = warp_sum(M == -INFINITY ? 0.f : L * exp2f(M - all));
+      L = warp_sum(L == 0.f ? 0.f : L * exp2f(M - all));
       M = all;
     }
     if (SCORES && lane == 0) {
       top[warp] = M == -INFINITY ? 0.f : M;
-      inv[warp] = L > 0.f ? 1.f / L : 0.f;
+      inv[warp] = L == 0.f ? 0.f : 1.f / L;
     }
   }
   if (!SCORES) return;

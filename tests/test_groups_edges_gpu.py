@@ -156,3 +156,34 @@ def test_shared_tokens_behind_all_contexts_are_nobodys(groups, fp8, wide):
                 want, bound, _, _ = oracle.decode_row(q[row], *(torch.cat(x, 1) for x in parts), SCALE, fp8)
                 within(out[row], want, bound, f"row {row}")
             row += 1
+
+
+# ---- what is not a number ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_a_query_that_is_not_a_number_has_no_result_that_is_one(fp8, wide):
+    """One head of some rows, of one token and of many, behind a shared prefix and alone; the other heads and rows are as without it."""
+    st = shared_batch(109, [(100, [133, 101, 117]), (0, [33, 1, 0, 2000])], 2, fp8)
+    if wide:
+        widen(st)
+    q = torch.randn(7, 12, 128, generator=gen(109), device=DEV).to(torch.bfloat16)
+    bad = q.clone()
+    rows, heads = [0, 3, 4, 5, 6], [0, 5, 7, 8, 11]
+    bad[rows, heads, 17] = float("nan")
+    kw = {"k_scale": st["ks"], "v_scale": st["vs"]}
+    args = (st["k"], st["v"], st["tables"], st["context"])
+    good, out = (ops.paged_decode_shared(x, *args, st["cu"], st["shared"], **kw) for x in (q, bad))
+    for r, h in zip(rows, heads):
+        want = torch.zeros_like if r == 5 else lambda x: torch.full_like(x, float("nan"))           # (row 5 sees nothing)
+        assert torch.equal(out[r, h].isnan(), want(out[r, h]).isnan()), (r, h)
+        good[r, h] = out[r, h] = 0
+    assert torch.equal(good, out)
+    alone = [3, 4, 5, 6]                                                      # (the others' own pages do not hold what they share)
+    args = (st["k"], st["v"], st["tables"][alone].contiguous(), st["context"][alone].contiguous())
+    (good, sums), (out, spoilt) = (ops.paged_decode_scored(x[alone].contiguous(), *args, torch.zeros(4, 2, 2000, device=DEV), **kw) for x in (q, bad))
+    for r, h in zip(range(4), heads[1:]):
+        n = int(st["context"][alone[r]])
+        assert out[r, h].isnan().all() or n == 0
+        assert spoilt[r, h // 6, :n].isnan().all() and torch.equal(spoilt[r, 1 - h // 6], sums[r, 1 - h // 6]) and (spoilt[r, :, n:] == 0).all()
+        good[r, h] = out[r, h] = 0
+    assert torch.equal(good, out)
