@@ -29,7 +29,6 @@ constexpr int kFlatD = 128;
 constexpr int kPlanThreads = 1024;
 constexpr int kNearRows = kFlatWarps * 32;
 constexpr int kPrefixLeast = 2;                   // steps of the prefixes a run
-constexpr float kFlatScale = 1024.f;              // of fp8 weights, which are f16 (2^10: small ones stay normal)
 
 template <bool FP8>
 struct FlatSizes {
@@ -337,7 +336,7 @@ __global__ void __launch_bounds__(kFlatWarps * 32, FlatSizes<FP8>::kBlocks) deco
 
     uint32_t qa0[8], qa2[8];                                           // row g: query head g of the kv head
     float o[16][4];
-    float m_run = 0.f, l_run = 0.f;
+    float m_run = 0.f, l_run = 0.f, factor = 1.f;                    // of weights, and of what they have summed
     auto enter = [&]() {                                               // a row-head's queries, nothing seen
       const bool real = g < p.G;
       const __nv_bfloat16* qrow = p.q + here.s * p.q_stride_s + (here.h * p.G + (real ? g : 0)) * kFlatD;
@@ -357,8 +356,10 @@ __global__ void __launch_bounds__(kFlatWarps * 32, FlatSizes<FP8>::kBlocks) deco
       for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
       m_run = -INFINITY;
       l_run = 0.f;
+      factor = FP8 ? __uint_as_float(kMostFactor) : 1.f;
     };
     auto leave = [&]() {                                               // its part
+      const float f = FP8 ? inverse_factor(factor) : 1.f;
       float l = l_run;
       l += __shfl_xor_sync(0xffffffffu, l, 1);
       l += __shfl_xor_sync(0xffffffffu, l, 2);
@@ -367,7 +368,7 @@ __global__ void __launch_bounds__(kFlatWarps * 32, FlatSizes<FP8>::kBlocks) deco
         float* dst = p.part_o + part * kFlatD + t4 * 2;
 #pragma unroll
         for (int nd = 0; nd < 16; ++nd)
-          *reinterpret_cast<float2*>(dst + nd * 8) = make_float2(o[nd][0] * (FP8 ? 1.f / kFlatScale : 1.f), o[nd][1] * (FP8 ? 1.f / kFlatScale : 1.f));
+          *reinterpret_cast<float2*>(dst + nd * 8) = make_float2(o[nd][0] * f, o[nd][1] * f);
         if (t4 == 0) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(m_run, l);
       }
     };
@@ -458,19 +459,27 @@ __global__ void __launch_bounds__(kFlatWarps * 32, FlatSizes<FP8>::kBlocks) deco
       const float m_new = fmaxf(m_run, top), m_sub = m_new == -INFINITY ? 0.f : m_new;
       const float corr = exp2f(m_run - m_sub);                         // 0 while nothing has been seen
       uint32_t pa[U][2];
-      float sum = 0.f;
+      float sum = 0.f, corr_o = corr;
+      if constexpr (FP8) {
+        float most = 0.f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) most = fmaxf(most, fmaxf(fmaxf(vscale[u][0], vscale[u][1]), fmaxf(vscale[u][2], vscale[u][3])));
+        const float before = inverse_factor(factor);
+        factor = shrink_factor(factor, most);
+        corr_o = corr * (factor * before);
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const float p0 = exp2f(s[u][j][0] - m_sub), p1 = exp2f(s[u][j][1] - m_sub);
           sum += p0 + p1;
-          pa[u][j] = FP8 ? pack_f16x2(p0 * (vscale[u][2 * j] * kFlatScale), p1 * (vscale[u][2 * j + 1] * kFlatScale)) : pack_bf16x2(p0, p1);
+          pa[u][j] = FP8 ? pack_f16x2(p0 * (vscale[u][2 * j] * factor), p1 * (vscale[u][2 * j + 1] * factor)) : pack_bf16x2(p0, p1);
         }
       l_run = l_run * corr + sum;
       m_run = m_new;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) { o[i][0] *= corr; o[i][1] *= corr; }
+      for (int i = 0; i < 16; ++i) { o[i][0] *= corr_o; o[i][1] *= corr_o; }
       // ---- O += P V ----
 #pragma unroll
       for (int u = 0; u < U; ++u) {

@@ -21,7 +21,6 @@ namespace nrl {
 constexpr int kPreWarps = kPrefixRows / 16;
 constexpr int kPreStages = 3;
 constexpr int kPreStep = kPrefixKeys / 16;        // pages a step
-constexpr float kPreScale = 1024.f;               // of fp8 weights, which are f16 (2^10: small ones stay normal)
 
 template <bool FP8>
 struct PreSmem {
@@ -170,7 +169,7 @@ NRL_DEVICE void decode_prefix_run(const FlatParams& p, uint8_t* smem, int run) {
     float o[16][4];
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f}, factor = FP8 ? __uint_as_float(kMostFactor) : 1.f;          // (of weights, and of o)
 
     for (int step = w.step; step < w.step + w.n; ++step, ++n_out) {
       cp_async_wait<1>();
@@ -248,8 +247,7 @@ NRL_DEVICE void decode_prefix_run(const FlatParams& p, uint8_t* smem, int run) {
           const uint4 kr = lds128(sb + t4 * 16), vr = lds128(sb + 64 + t4 * 16);
           ksc[0] = __uint_as_float(kr.x) * p.scale_log2; ksc[1] = __uint_as_float(kr.y) * p.scale_log2;
           ksc[2] = __uint_as_float(kr.z) * p.scale_log2; ksc[3] = __uint_as_float(kr.w) * p.scale_log2;
-          vsc[u][0] = __uint_as_float(vr.x) * kPreScale; vsc[u][1] = __uint_as_float(vr.y) * kPreScale;
-          vsc[u][2] = __uint_as_float(vr.z) * kPreScale; vsc[u][3] = __uint_as_float(vr.w) * kPreScale;
+          vsc[u][0] = __uint_as_float(vr.x); vsc[u][1] = __uint_as_float(vr.y); vsc[u][2] = __uint_as_float(vr.z); vsc[u][3] = __uint_as_float(vr.w);
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -272,6 +270,22 @@ NRL_DEVICE void decode_prefix_run(const FlatParams& p, uint8_t* smem, int run) {
         corr[i] = exp2f(m_run[i] - m_sub[i]);                          // 0 while nothing has been seen
         m_run[i] = m_new;
       }
+      if constexpr (FP8) {
+        float most = 0.f;
+#pragma unroll
+        for (int u = 0; u < L::kPages; ++u) most = fmaxf(most, fmaxf(fmaxf(vsc[u][0], vsc[u][1]), fmaxf(vsc[u][2], vsc[u][3])));
+        const float before = inverse_factor(factor);
+        factor = shrink_factor(factor, most);
+#pragma unroll
+        for (int u = 0; u < L::kPages; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) vsc[u][i] *= factor;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          l_run[i] *= corr[i];
+          corr[i] *= factor * before;
+        }
+      }
       uint32_t pa[L::kPages][4];
 #pragma unroll
       for (int u = 0; u < L::kPages; ++u)
@@ -284,7 +298,7 @@ NRL_DEVICE void decode_prefix_run(const FlatParams& p, uint8_t* smem, int run) {
             pa[u][2 * j + i] = FP8 ? pack_f16x2(p0 * vsc[u][2 * j], p1 * vsc[u][2 * j + 1]) : pack_bf16x2(p0, p1);
           }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) l_run[i] = l_run[i] * corr[i] + sum[i];
+      for (int i = 0; i < 2; ++i) l_run[i] = FP8 ? l_run[i] + sum[i] : l_run[i] * corr[i] + sum[i];
       if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) { o[i][0] *= corr[0]; o[i][1] *= corr[0]; o[i][2] *= corr[1]; o[i][3] *= corr[1]; }
@@ -320,9 +334,10 @@ NRL_DEVICE void decode_prefix_run(const FlatParams& p, uint8_t* smem, int run) {
       if (!real[i]) continue;
       const long at = prefix_part_row(p, w.first, w.h, w.rows, w.tile * kPrefixRows + warp * 16 + g + i * 8) + static_cast<long>(kPrefixRows) * run;
       float* dst = p.prefix_o + at * 128 + t4 * 2;
+      const float f = FP8 ? inverse_factor(factor) : 1.f;
 #pragma unroll
       for (int nd = 0; nd < 16; ++nd)
-        *reinterpret_cast<float2*>(dst + nd * 8) = make_float2(o[nd][2 * i] * (FP8 ? 1.f / kPreScale : 1.f), o[nd][2 * i + 1] * (FP8 ? 1.f / kPreScale : 1.f));
+        *reinterpret_cast<float2*>(dst + nd * 8) = make_float2(o[nd][2 * i] * f, o[nd][2 * i + 1] * f);
       if (t4 == 0) *reinterpret_cast<float2*>(p.prefix_ml + at * 2) = make_float2(m_run[i], l_run[i]);
     }
   }

@@ -34,6 +34,18 @@ NRL_DEVICE uint4 lds128(uint32_t addr) {
 // (or 4..7) of an even and an odd row, which are all eight chunks' banks.
 NRL_DEVICE int k_sigma(int r) { return (r & 1) << 2; }
 
+// Weights of fp8 values are f16, a value's scale riding in its weight, and all times a power of two that makes the largest weight of the largest scale so far 2^13 to 2^14,
+// whatever scales there are.  A weight is off by 2^-11 of itself, or by 2^-25, 2^-38 of the largest, where it is denormal.
+// (Times a constant 2^10, scales of 2.2e-5, of values up to 0.01, made weights under 2.7e-3 denormal: one of 6e-6 is 2.3 steps there, and all of a long tail of them were
+// off by a seventh to the same side.)
+constexpr uint32_t kMostFactor = 0x78800000u;                        // 2^114: for scales of 2^-100 and less
+// the factor, shrunk to a step's scales, of which each lane has some (a whole warp)
+NRL_DEVICE float shrink_factor(float factor, float scale) {
+  const uint32_t top = min((__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(scale))) + 0x7fffffu) & 0x7f800000u, 0x7e800000u);      // a power of two at or above
+  return fminf(factor, __uint_as_float(min(0x86000000u - top, kMostFactor)));
+}
+NRL_DEVICE float inverse_factor(float factor) { return __uint_as_float(0x7f000000u - __float_as_uint(factor)); }
+
 // a page's values V^T [128][16] in shared memory: tokens outside [from, to) become 0 (a whole warp; synchronised before and after)
 NRL_DEVICE void fp8_clear_values(uint8_t* vt, int from, int to, int lane) {
   uint32_t keep[4];

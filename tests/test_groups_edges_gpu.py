@@ -187,3 +187,37 @@ def test_a_query_that_is_not_a_number_has_no_result_that_is_one(fp8, wide):
         assert spoilt[r, h // 6, :n].isnan().all() and torch.equal(spoilt[r, 1 - h // 6], sums[r, 1 - h // 6]) and (spoilt[r, :, n:] == 0).all()
         good[r, h] = out[r, h] = 0
     assert torch.equal(good, out)
+
+
+# ---- small values --------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("amax", [1e-2, 1e-6, 3e4])
+@pytest.mark.parametrize("rows,shared", [(100, 0), (300, 0), (40, 1500)])
+def test_tails_of_small_weights_over_fp8_values(rows, shared, amax):
+    """A key in 97 has all the weight and a value of 0; the others' weights are 6e-6 of it, and the result is their sum.  Few and many rows, and a shared prefix."""
+    n, kv, heads, group = 1570, 2, 12, 6
+    pages = (n + 15) // 16
+    k, v = torch.zeros(pages, kv, 16, 128, device=DEV), torch.rand(pages, kv, 16, 128, generator=gen(110), device=DEV) * amax
+    at = torch.arange(5, n, 97, device=DEV)
+    k[at // 16, :, at % 16], v[at // 16, :, at % 16] = 1.0, 0.0
+    vs = (v.amax(-1) / 448.0).clamp_(min=amax / 448.0)
+    st = {"k": (k * 448.0).to(torch.float8_e4m3fn).view(torch.uint8), "ks": torch.full((pages, kv, 16), 1.0 / 448.0, device=DEV), "vs": vs,
+          "v": (v / vs[..., None]).to(torch.float8_e4m3fn).transpose(2, 3).contiguous().view(torch.uint8)}
+    table = torch.arange(pages, dtype=torch.int32, device=DEV)
+    st["tables"], st["context"] = table.expand(rows, -1).contiguous(), torch.tensor([n - i % 60 for i in range(rows)], dtype=torch.int32, device=DEV)
+    if shared:
+        widen(st)
+    # a key's score: 12.02 = -log(6e-6) above the others'
+    q = torch.full((rows, heads, 128), 12.02 * math.sqrt(128) / 128, device=DEV).to(torch.bfloat16)
+    kw = {"k_scale": st["ks"], "v_scale": st["vs"]}
+    cu, lens = offsets([rows]), torch.tensor([shared], dtype=torch.int32, device=DEV)
+    args = (q, st["k"], st["v"], st["tables"], st["context"])
+    outs = [ops.paged_decode_shared(*args, cu, lens, **kw), ops.paged_decode_scored(*args, torch.zeros(rows, kv, n, device=DEV), **kw)[0]]
+    for r in range(0, rows, 13):
+        c = int(st["context"][r])
+        keys, values = oracle.page_rows(st, table, c)
+        p = torch.softmax(q[r].double().view(kv, group, 128) @ keys.transpose(1, 2) * SCALE, -1)
+        want = (p @ values).flatten(0, 1)
+        # weights in f16: 2^-11 of each, and of the largest value 2^-37 for one that is denormal beside the run's largest; a score of 12 in float32
+        bound = (oracle.F16 + oracle.F32) * (p @ values.abs()).flatten(0, 1) + c * 2.0 ** -37 * values.abs().max() * p.max()
+        for out in outs:
+            within(out[r], want, bound, f"row {r}")
