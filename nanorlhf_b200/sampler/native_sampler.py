@@ -466,12 +466,14 @@ class NativeSampler:
                 new_seq, first_tok_logits_rows, chunk, tok_count = [], [], [], 0
                 logits_parts = []
                 for g in admitted + [None]:
-                    if g is not None:
-                        chunk.append(g)
-                        tok_count += len(gid_to_prompt[g])
-                    if chunk and (g is None or tok_count >= self.prefill_token_budget):
+                    # (of a bounded cache every sample is a request: those of one prompt stay in one chunk, which computes it once)
+                    again = evicts and g is not None and bool(chunk) and gid_to_prompt[g] is gid_to_prompt[chunk[-1]]
+                    if chunk and (g is None or (tok_count >= self.prefill_token_budget and not again)):
                         logits_parts.append((list(chunk), self._prefill(sched, chunk, gid_to_prompt, evicts)))
                         chunk, tok_count = [], 0
+                    if g is not None:
+                        chunk.append(g)
+                        tok_count += 0 if again else len(gid_to_prompt[g])
                 # ---- (re)build the batch state: surviving rows + new rows ----
                 keep_rows = []
                 if st is not None:

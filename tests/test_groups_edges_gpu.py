@@ -221,3 +221,20 @@ def test_tails_of_small_weights_over_fp8_values(rows, shared, amax):
         bound = (oracle.F16 + oracle.F32) * (p @ values.abs()).flatten(0, 1) + c * 2.0 ** -37 * values.abs().max() * p.max()
         for out in outs:
             within(out[r], want, bound, f"row {r}")
+
+
+# ---- a bounded cache's prefill -------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("budget", [1, 100, 250, 32768])
+def test_a_bounded_cache_computes_every_prompt_once(budget):
+    """... however many samples it has, in however many chunks the prompts are computed; and chunks are no smaller for the samples"""
+    from tests.test_groups_paths_gpu import PAD, _engine, _prompts
+    eng, prompts, chunks = _engine(), _prompts((40, 65, 18, 33, 90, 7)), []
+    whole = eng.generate(prompts, 8, 0.9, 0.95, 16, None, PAD, 3, kv_budget=30)
+    prefill, tokens = eng._prefill, sum(map(len, prompts))
+    assert eng.stats["prefill_tokens"] == tokens
+    eng.prefill_token_budget = budget
+    eng._prefill = lambda sched, groups, *a: (chunks.append(len(groups)), prefill(sched, groups, *a))[1]
+    out = eng.generate(prompts, 8, 0.9, 0.95, 16, None, PAD, 3, kv_budget=30)
+    assert eng.stats["prefill_tokens"] == 2 * tokens
+    assert chunks == {1: [8] * 6, 100: [16, 24, 8], 250: [48], 32768: [48]}[budget]
+    assert torch.equal(out[:, 0], whole[:, 0])
