@@ -62,6 +62,13 @@ class PolicyAndValueWrapper(nn.Module):
         return self.policy(*a, **kw)
 
 
+def check_share_prompts(models, native: bool):
+    """``RLConfig.share_prompts`` is refused before anything has run: the kernels of ``ops.attention_shared_prefix`` have heads of 128; plain packing takes others."""
+    for m in models:
+        if native and m is not None and m.config.head_dim != 128:
+            raise ValueError(f"share_prompts needs models with heads of 128 on CUDA, got {type(m).__name__} with {m.config.head_dim}")
+
+
 class RLTrainer:
     algo_name = "rl"
     samples_per_prompt_field: Optional[str] = None    # e.g. "grpo_sample_N"
@@ -102,6 +109,8 @@ class RLTrainer:
                 disable_dropout_in_model(m)
         if args.logprob_top_p_consistent and (args.top_k > 0 or args.min_p > 0.0):
             raise ValueError("logprob_top_p_consistent scores with the nucleus alone; it does not go with top_k or min_p")
+        if args.share_prompts:
+            check_share_prompts((policy, ref_policy, value_model if self.uses_value_model else None), ops.use_native(torch.empty(0, device=self.device)))
         if args.logprob_top_p_consistent and args.top_p < 1.0:
             # experimental: policy and reference log-probs under the truncated softmax the sampler draws from
             for m in (policy, ref_policy):

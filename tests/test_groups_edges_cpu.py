@@ -14,3 +14,20 @@ def test_rows_without_any_sequence(groups):
     out = ops.attention_shared_prefix(*leaves, cu[:1], ints(*[0] * (groups + 1)))
     for x in (out, *torch.autograd.grad(out, leaves, dout)):
         assert torch.equal(x, torch.zeros_like(x))
+
+
+def test_share_prompts_is_refused_when_a_trainer_is_built():
+    """... for models whose heads the kernels do not take; the CPU form takes all"""
+    from nanorlhf_b200.models.lora import LoraConfig, get_peft_model
+    from nanorlhf_b200.models.qwen2 import Qwen2Config, Qwen2ForCausalLM, Qwen2ForSequenceClassification
+    from nanorlhf_b200.trainer.base import check_share_prompts
+    made = lambda cls, dim: cls.from_config(Qwen2Config(vocab_size=64, hidden_size=64, intermediate_size=64, num_hidden_layers=1, num_attention_heads=2,  # noqa: E731
+                                                        num_key_value_heads=1, head_dim=dim), torch.float32, "cpu", seed=1)
+    narrow, wide = made(Qwen2ForCausalLM, 64), made(Qwen2ForCausalLM, 128)
+    critic = Qwen2ForSequenceClassification.from_causal_lm(narrow)
+    adapted = get_peft_model(made(Qwen2ForCausalLM, 64), LoraConfig(r=2, lora_alpha=4))
+    for models in ((narrow, wide, None), (wide, narrow, None), (wide, wide, critic), (adapted, wide, None)):
+        check_share_prompts(models, False)
+        with pytest.raises(ValueError, match="share_prompts"):
+            check_share_prompts(models, True)
+    check_share_prompts((wide, wide, None), True)

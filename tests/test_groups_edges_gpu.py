@@ -238,3 +238,16 @@ def test_a_bounded_cache_computes_every_prompt_once(budget):
     assert eng.stats["prefill_tokens"] == 2 * tokens
     assert chunks == {1: [8] * 6, 100: [16, 24, 8], 250: [48], 32768: [48]}[budget]
     assert torch.equal(out[:, 0], whole[:, 0])
+
+
+@pytest.mark.parametrize("algo", ["grpo", "ppo"])
+def test_trainers_look_at_heads_when_they_are_built(algo, tmp_path, monkeypatch):
+    from nanorlhf_b200.models.qwen2 import Qwen2Config
+    from nanorlhf_b200.trainer import GRPOTrainer, PPOTrainer
+    from tests.test_trainers_gpu import _setup
+    cls, extra = (PPOTrainer, {"policy_learning_rate": 1e-4, "value_learning_rate": 2e-4}) if algo == "ppo" else (GRPOTrainer, {"grpo_sample_N": 4})
+    _setup(tmp_path, cls, extra, share_prompts=True)
+    monkeypatch.setattr(Qwen2Config, "__post_init__", lambda self: setattr(self, "head_dim", 64), raising=False)
+    _setup(tmp_path, cls, extra)
+    with pytest.raises(ValueError, match="share_prompts"):
+        _setup(tmp_path, cls, extra, share_prompts=True)
