@@ -1,6 +1,7 @@
 // Tensors in, launches out: attention over shared prefixes, decode attention with scores, eviction.
 #include "bindings_groups.h"
 
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -248,6 +249,8 @@ std::tuple<torch::Tensor, torch::Tensor> paged_decode_scored(const torch::Tensor
     check_scores(into, k, c.S, what, "out_scores");
     TORCH_CHECK_VALUE(into.sizes() == scores.sizes(), what, ": out_scores must be like scores, got ", into.sizes(), " and ", scores.sizes());
   }
+  TORCH_CHECK_VALUE(at::has_internal_overlap(into) != at::MemOverlap::Yes, what, ": ", out_scores.has_value() ? "out_scores" : "scores",
+                    " must not be expanded: they are written to");
   TORCH_CHECK_VALUE(std::isfinite(decay), what, ": decay must be finite, got ", decay);
   if (t.empty()) return {t.out, into};
   const int64_t raws = 16LL * c.max_blocks * c.S * c.Hq;

@@ -350,6 +350,9 @@ def paged_decode_scored(q, k_cache, v_cache, block_tables, context_lens, scores,
         _check_scores(what, out_scores, k_cache, q.shape[0], "out_scores")
         if out_scores.shape != scores.shape:
             raise ValueError(f"{what}: out_scores must be like scores, got {tuple(out_scores.shape)} and {tuple(scores.shape)}")
+    into = "scores" if out_scores is None else "out_scores"
+    if any(stride == 0 and size > 1 for stride, size in zip((out_scores if out_scores is not None else scores).stride(), scores.shape)):
+        raise ValueError(f"{what}: {into} must not be expanded: they are written to")
     if not math.isfinite(decay):
         raise ValueError(f"{what}: decay must be finite, got {decay}")
     return ref.paged_decode_scored(q, k_cache, v_cache, block_tables, context_lens, scores, decay, k_scale, v_scale, _scale_of(what, scale, q), out_scores)

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from groups_refusals import ints, packed
+from groups_refusals import ints, packed, pool
 from nanorlhf_b200 import ops
 
 
@@ -31,3 +31,24 @@ def test_share_prompts_is_refused_when_a_trainer_is_built():
         with pytest.raises(ValueError, match="share_prompts"):
             check_share_prompts(models, True)
     check_share_prompts((wide, wide, None), True)
+
+
+def expanded_scores_are_refused(device):
+    """... where they are written to: rows or heads that are one"""
+    st = {n: None if x is None else x.to(device) for n, x in pool().items()}
+    tables, context = torch.tensor([[0, 1, 2], [3, 4, 5]], dtype=torch.int32, device=device), ints(40, 6).to(device)
+    q = torch.ones(2, 4, 128, dtype=torch.bfloat16, device=device)
+    call = lambda scores, into: ops.paged_decode_scored(q, st["k"], st["v"], tables, context, scores, out_scores=into)  # noqa: E731
+    full = torch.rand(1, 2, 48, device=device).expand(2, -1, -1).contiguous()
+    for x in (full[:1].expand(2, -1, -1), full[:, :1].expand(-1, 2, -1)):
+        for scores, into in ((x, None), (full, x)):
+            with pytest.raises(ValueError, match="expanded"):
+                call(scores, into)
+    # read, they may be
+    want = call(full, torch.zeros_like(full))
+    for a, b in zip(want, call(full[:1].expand(2, -1, -1), torch.zeros_like(full))):
+        assert torch.equal(a, b)
+
+
+def test_expanded_scores():
+    expanded_scores_are_refused("cpu")

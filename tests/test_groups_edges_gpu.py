@@ -251,3 +251,8 @@ def test_trainers_look_at_heads_when_they_are_built(algo, tmp_path, monkeypatch)
     _setup(tmp_path, cls, extra)
     with pytest.raises(ValueError, match="share_prompts"):
         _setup(tmp_path, cls, extra, share_prompts=True)
+
+
+def test_expanded_scores():
+    from test_groups_edges_cpu import expanded_scores_are_refused
+    expanded_scores_are_refused(DEV)
