@@ -366,8 +366,9 @@ def kv_evict(k_cache, v_cache, block_tables, context_lens, scores, keep: int, si
     the row: within its pages, or into those of ``out_tables`` [S, pages], where rows of fewer tokens are copied too.  kept[s, h, j] is where the token of place j was, -1 (score 0) behind the
     last.  Places that nothing moves to stay as they are.  Pages that are written to must be one row's alone and, with ``out_tables``, no row's source; no context may
     be longer than L.  Rotated keys keep their rotation: positions go on from where they were, lengths from the new ones."""
-    if int(keep) != keep:
-        raise ValueError(f"kv_evict: keep must be a whole number, got {keep}")
+    for name, x in (("keep", keep), ("sinks", sinks), ("recent", recent)):
+        if not math.isfinite(x) or int(x) != x:
+            raise ValueError(f"kv_evict: {name} must be a whole number, got {x}")
     if use_native(k_cache):
         return _nat().kv_evict(k_cache, v_cache, block_tables, context_lens, scores, int(keep), int(sinks), int(recent), k_scale, v_scale, out_tables)
     what = "kv_evict"

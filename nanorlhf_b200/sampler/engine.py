@@ -13,6 +13,7 @@ strings -> ids) and exposes ``top_p`` / ``top_k`` / ``min_p`` / ``seed`` (``ops.
 """
 from __future__ import annotations
 
+import math
 import random
 from typing import List, Optional, Sequence, Union
 
@@ -84,9 +85,11 @@ def release_native_engine(model):
 
 def check_cache_options(shared_decode: bool, kv_budget: int, kv_sinks: int, kv_recent: Optional[int]) -> int:
     """what ``generate`` is told about the cache; returns kv_recent (None: a quarter of the budget)"""
-    if kv_budget != int(kv_budget) or kv_budget < 0:
+    if not math.isfinite(kv_budget) or kv_budget != int(kv_budget) or kv_budget < 0:
         raise ValueError(f"kv_budget must be 0 (all tokens stay) or a positive whole number, got {kv_budget}")
     recent = int(kv_budget) // 4 if kv_recent is None else kv_recent
+    if kv_budget and not all(math.isfinite(x) and int(x) == x for x in (kv_sinks, recent)):
+        raise ValueError(f"kv_sinks and kv_recent must be whole numbers, got {kv_sinks} and {recent}")
     if kv_budget and (kv_sinks < 0 or recent < 0 or kv_sinks + recent > kv_budget):
         raise ValueError(f"kv_sinks and kv_recent must not be negative nor together over kv_budget, got {kv_sinks}, {recent} and {kv_budget}")
     if kv_budget and shared_decode:

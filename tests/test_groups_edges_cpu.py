@@ -52,3 +52,18 @@ def expanded_scores_are_refused(device):
 
 def test_expanded_scores():
     expanded_scores_are_refused("cpu")
+
+
+@pytest.mark.parametrize("kw", [{"keep": float("inf")}, {"keep": 8.5}, {"sinks": 1.5}, {"recent": 2.5}, {"recent": float("nan")}])
+def test_evict_counts_in_whole_numbers(kw):
+    st = pool()
+    with pytest.raises(ValueError, match="whole number"):
+        ops.kv_evict(st["k"], st["v"], torch.tensor([[0, 1, 2]], dtype=torch.int32), ints(40), torch.rand(1, 2, 40), **{"keep": 10, **kw})
+
+
+@pytest.mark.parametrize("args", [(float("inf"), 4, None), (20.5, 4, None), (20, 1.5, None), (20, 4, 2.5), (20, 4, float("nan"))])
+def test_a_bounded_cache_counts_in_whole_numbers(args):
+    from nanorlhf_b200.sampler.engine import check_cache_options
+    with pytest.raises(ValueError, match="whole number"):
+        check_cache_options(False, *args)
+    assert check_cache_options(False, 20.0, 4.0, None) == 5
