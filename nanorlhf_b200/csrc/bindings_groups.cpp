@@ -136,7 +136,10 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, torch::Te
                                                                                                                const c10::optional<double>& scale) {
   const char* what = "attention_shared_prefix";
   check_packed(q, k, v, cu_seqlens, cu_groups, what);
-  return {head_rows(q), head_rows(k), head_rows(v), cu_seqlens.contiguous(), cu_groups.contiguous(), scale_of(scale, what)};
+  // masked scores are -inf in front of the scale: times 0 or less they would not stay it
+  const double by = scale_of(scale, what);
+  TORCH_CHECK_VALUE(by >= 1e-37 && by <= 1e37, what, ": scale must be positive, from 1e-37 to 1e37, got ", by);
+  return {head_rows(q), head_rows(k), head_rows(v), cu_seqlens.contiguous(), cu_groups.contiguous(), by};
 }
 torch::Tensor attention_shared_prefix(const torch::Tensor& q_in, const torch::Tensor& k_in, const torch::Tensor& v_in, const torch::Tensor& cu_seqlens_in,
                                       const torch::Tensor& cu_groups_in, const c10::optional<double>& scale_in) {

@@ -273,7 +273,7 @@ def attention_shared_prefix(q, k, v, cu_seqlens, cu_groups, max_seqlen=None, sca
     themselves, as if the prefix stood in front of each of them; it is computed once.  Lengths may be 0.  A sequence of no group, and one that is its group's only
     one, is plain (``attention_varlen``).  Rows behind the last sequence are 0, and so are their gradients.  Differentiable once in q, k and v (on CUDA
     in reverse mode: a tangent is refused).
-    On CUDA bf16 and D = 128; q, k and v may be views of a projection.  ``max_seqlen`` is not needed.  A non-finite value in one sequence may reach the ones packed
+    On CUDA bf16 and D = 128; q, k and v may be views of a projection.  ``max_seqlen`` is not needed; ``scale`` is positive.  A non-finite value in one sequence may reach the ones packed
     beside it."""
     if use_native(q):
         return _nat().attention_shared_prefix(q, k, v, cu_seqlens, cu_groups, scale)          # (checked there, with the same errors)
@@ -285,7 +285,10 @@ def attention_shared_prefix(q, k, v, cu_seqlens, cu_groups, max_seqlen=None, sca
     if cu_seqlens.dim() != 1 or cu_groups.dim() != 1 or cu_seqlens.numel() < 1 or cu_groups.numel() < 1:
         raise ValueError(f"{what}: cu_seqlens [sequences + 1] and cu_groups [groups + 1] are needed, got {tuple(cu_seqlens.shape)} and {tuple(cu_groups.shape)}")
     _check_int32(what, q, cu_seqlens=cu_seqlens, cu_groups=cu_groups)
-    return ref.attention_shared_prefix(q, k, v, cu_seqlens, cu_groups, _scale_of(what, scale, q))
+    scale = _scale_of(what, scale, q)
+    if not 1e-37 <= scale <= 1e37:
+        raise ValueError(f"{what}: scale must be positive, from 1e-37 to 1e37, got {scale}")
+    return ref.attention_shared_prefix(q, k, v, cu_seqlens, cu_groups, scale)
 
 
 def _check_pages(what, q, k_cache, v_cache, block_tables, context_lens, k_scale, v_scale):

@@ -67,3 +67,22 @@ def test_a_bounded_cache_counts_in_whole_numbers(args):
     with pytest.raises(ValueError, match="whole number"):
         check_cache_options(False, *args)
     assert check_cache_options(False, 20.0, 4.0, None) == 5
+
+
+def scales_of_packed_attention(device, dtype):
+    """masked scores would not stay masked times 0 or less; small and large ones are taken"""
+    q, k, v, _, cu, cg = (x.to(device) for x in packed([[3, 4]], 4, 2))
+    q, k, v = (x.to(dtype) for x in (q, k, v))
+    for bad in (0.0, -0.0, -0.1, 1e-40, 1e38, float("inf")):
+        with pytest.raises(ValueError, match="scale"):
+            ops.attention_shared_prefix(q, k, v, cu, cg, scale=bad)
+    # so small that all scores are alike: means of the values up to a row (bf16: weights of 2^-8, the result's rounding)
+    out = ops.attention_shared_prefix(q, k, v, cu, cg, scale=1e-37).float()
+    seen = [list(range(i + 1)) for i in range(7)]
+    for i, rows in enumerate(seen):
+        want = v[rows].float().mean(0).repeat_interleave(2, 0)
+        assert (out[i] - want).abs().max() <= (2 * 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -20) * v.float().abs().max()
+
+
+def test_scales_of_packed_attention():
+    scales_of_packed_attention("cpu", torch.float32)

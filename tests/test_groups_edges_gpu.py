@@ -256,3 +256,35 @@ def test_trainers_look_at_heads_when_they_are_built(algo, tmp_path, monkeypatch)
 def test_expanded_scores():
     from test_groups_edges_cpu import expanded_scores_are_refused
     expanded_scores_are_refused(DEV)
+
+
+def test_scales_of_packed_attention():
+    from test_groups_edges_cpu import scales_of_packed_attention
+    scales_of_packed_attention(DEV, torch.bfloat16)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("scale", [0.0, -0.05, 3.0])
+def test_scales_of_decode(scale, fp8):
+    """there the mask comes behind the scale: none of these is refused"""
+    groups = [(40, [50, 41, 77]), (0, [33, 0, 200])]
+    st = shared_batch(111, groups, 2, fp8)
+    q = torch.randn(6, 12, 128, generator=gen(111), device=DEV).to(torch.bfloat16)
+    kw = {"k_scale": st["ks"], "v_scale": st["vs"], "scale": scale}
+    args, sums = (st["k"], st["v"], st["tables"], st["context"]), torch.zeros(6, 2, 200, device=DEV)
+    shared, scored = ops.paged_decode_shared(q, *args, st["cu"], st["shared"], **kw), ops.paged_decode_scored(q, *args, sums, **kw)[0]
+    row = 0
+    for n_shared, ctxs in groups:
+        first = row
+        for c in ctxs:
+            n = min(n_shared, c)
+            parts = zip(oracle.page_rows(st, st["tables"][first], n), (x[:, n:] for x in oracle.page_rows(st, st["tables"][row], c)))
+            keys, values = (torch.cat(x, 1) for x in parts)
+            want, bound, w, _ = oracle.decode_row(q[row], keys, values, scale, fp8)
+            # scores up to 3 * 60 * sqrt(128) are off by 2^-24 of what they sum, 128 * 2^-24 at the worst, and so are their exponentials
+            worst = 0.0 if c == 0 else (q[row].double().abs().view(2, 6, 128) @ keys.abs().transpose(1, 2)).amax() * abs(scale) * 128 * 2.0 ** -24
+            bound = bound + (0.0 if c == 0 else worst * values.abs().amax())
+            within(shared[row], want, bound, f"row {row}")
+            if n_shared == 0:
+                within(scored[row], want, bound, f"scored row {row}")
+            row += 1
