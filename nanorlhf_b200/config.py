@@ -73,8 +73,9 @@ class RLConfig:
     shared_decode: bool = False                 # sampler: attention reads the prompt pages that samples share once for all of them; pays for long
                                                 # prompts of many samples (32 x 16 rows of 2000 + 128 bf16 tokens 106 -> 62 us a layer, 128 x 8 of
                                                 # 200 + 800 144 -> 164)
-    kv_budget: int = 0                          # sampler: most cached tokens of a row between two evictions, 0: all of them.  Tokens that
-                                                # little attention went to are given up; as kv_cache_dtype, it only shapes the samples
+    kv_budget: int = 0                          # sampler: cached tokens that a row goes back to, every 64 steps, 0: all of them stay.  In between it
+                                                # holds up to 64 more, or its whole prompt and 64.  Tokens that little attention went to are given
+                                                # up; as kv_cache_dtype, it only shapes the samples
     kv_sinks: int = 4                           # of them, the row's first
     kv_recent: Optional[int] = None             # and its newest (None: a quarter of the budget)
     sampler: str = "auto"                       # auto | native | torch

@@ -1,5 +1,4 @@
-// Python bindings of the kernels around many samples of one prompt and a cache of bounded size (attention_groups.cu, decode_prefix.cu, decode_scored.cu,
-// kv_evict.cu).
+// Python bindings of the kernels around many samples of one prompt and a cache of bounded size (attention_groups.cu, decode_flat.cu, kv_evict.cu).
 #pragma once
 #include <pybind11/pybind11.h>
 

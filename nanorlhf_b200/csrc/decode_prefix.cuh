@@ -6,7 +6,7 @@
 //
 // Block = 4 warps of 16 rows; 4 pages a step through shared memory (cp.async, three stages), mma.sync m16n8k16.  fp8 pages are dequantised on the operand fragments as in
 // attention_decode_fp8.cu.  Bound by the latency of a step (fp8, 96 rows: 2 warps a scheduler, of which one issues in 31 % of the cycles, the tensor pipe 25 %): so an
-// fp8 warp holds the scores of two pages at a time and its queries in shared memory, in 167 registers, for three blocks an SM (32 x 2 x 2000 tokens of 96 rows 46 -> 41 us).
+// fp8 warp holds the scores of two pages at a time and its queries in shared memory, in 168 registers, for three blocks an SM (32 x 2 x 2000 tokens of 96 rows 46 -> 41 us).
 // Pages turned into f16 tiles once for the block, in place of once for every warp, took as long: what it saves in conversions it waits at one more barrier.
 // On tcgen05, tiles of 128 rows against blocks of 128 keys with two streams of scores and a warpgroup each for their softmax, 13 groups x 4 kv heads x 4096 fp8
 // tokens of 112 rows took 44 us and 64 x 2 x 390 bf16 tokens of 48 rows 21: a tile of few rows costs the tensor pipe as much as a full one, and fp8 pages' way

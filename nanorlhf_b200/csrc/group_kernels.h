@@ -1,5 +1,5 @@
 // Launch API of the kernels around many samples of one prompt and a cache of bounded size: decode attention behind a shared prefix and with scores
-// (decode_prefix.cu, decode_flat.cu), eviction (kv_evict.cu).  Pages have 16 tokens, heads 128 elements.
+// (decode_flat.cu, decode_prefix.cuh), eviction (kv_evict.cu).  Pages have 16 tokens, heads 128 elements.
 #pragma once
 #include <cuda_runtime.h>
 

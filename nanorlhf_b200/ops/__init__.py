@@ -273,8 +273,8 @@ def attention_shared_prefix(q, k, v, cu_seqlens, cu_groups, max_seqlen=None, sca
     themselves, as if the prefix stood in front of each of them; it is computed once.  Lengths may be 0.  A sequence of no group, and one that is its group's only
     one, is plain (``attention_varlen``).  Rows behind the last sequence are 0, and so are their gradients.  Differentiable once in q, k and v (on CUDA
     in reverse mode: a tangent is refused).
-    On CUDA bf16 and D = 128; q, k and v may be views of a projection.  ``max_seqlen`` is not needed; ``scale`` is positive.  A non-finite value in one sequence may reach the ones packed
-    beside it."""
+    On CUDA bf16 and D = 128; q, k and v may be views of a projection.  ``max_seqlen`` is not needed; ``scale`` is positive.  A non-finite value in one sequence, or
+    behind the last one, may reach the ones packed beside it."""
     if use_native(q):
         return _nat().attention_shared_prefix(q, k, v, cu_seqlens, cu_groups, scale)          # (checked there, with the same errors)
     what = "attention_shared_prefix"

@@ -27,7 +27,7 @@ def main() -> int:
     ap.add_argument("--eos", type=int, default=-1, help="stop token id (-1: none)")
     ap.add_argument("--pad", type=int, default=0)
     ap.add_argument("--shared-decode", action="store_true", help="read the prompt pages that samples share once for all of them")
-    ap.add_argument("--kv-budget", type=int, default=0, help="most cached tokens of a sample between two evictions (0: all)")
+    ap.add_argument("--kv-budget", type=int, default=0, help="cached tokens that a sample goes back to every 64 steps (0: all stay)")
     ap.add_argument("--kv-sinks", type=int, default=4, help="first tokens that an eviction keeps")
     ap.add_argument("--kv-recent", type=int, default=None, help="newest tokens that it keeps (a quarter of the budget)")
     a = ap.parse_args()

@@ -102,7 +102,8 @@ def generate(n: int, model, tokenizer, prompts: Union[torch.Tensor, Sequence[Seq
              eos_token_id: Optional[int] = None, rollout_dtype: str = "bf16", top_k: int = 0, min_p: float = 0.0,
              shared_decode: bool = False, kv_budget: int = 0, kv_sinks: int = 4, kv_recent: Optional[int] = None, **engine_kw) -> torch.Tensor:
     """``shared_decode``: the decode attention reads the prompt pages that samples share once for all of them.  ``kv_budget`` (0: off) bounds
-    the cached tokens of a row, by ``kv_sinks`` and ``kv_recent`` as ``ops.kv_evict`` says; both on the whole-prompt engine only."""
+    the cached tokens of a row: every ``sync_every`` steps (64) it goes back to so many, by ``kv_sinks`` and ``kv_recent`` as ``ops.kv_evict`` says, and holds up to
+    max(prompt + 1, ``kv_budget``) + ``sync_every`` in between.  Both on the whole-prompt engine only."""
     if top_k < 0 or top_k != int(top_k) or not 0.0 <= min_p <= 1.0:
         raise ValueError(f"top_k must be 0 (off) or a positive whole number and min_p between 0 (off) and 1, got {top_k} and {min_p}")
     check_cache_options(shared_decode, kv_budget, kv_sinks, kv_recent)

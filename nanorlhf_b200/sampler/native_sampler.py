@@ -12,7 +12,7 @@
   prompt, seeded, stop at EOS (kept), right-pad with pad_id, prompt-major / sample-minor order
   (GRPO/grpo_trainer.py:122-166); temperature 0 = greedy (ReMax baseline / eval);
 * two other forms of the decode attention, each for one ``generate``: over the prompt pages that the samples of a prompt share, read
-  once for all of them (``shared_decode``), or over a cache of at most ``kv_budget`` tokens and ``sync_every`` new ones a
+  once for all of them (``shared_decode``), or over a cache of at most ``kv_budget`` tokens (at first the prompt) and ``sync_every`` new ones a
   row, out of which every ``sync_every`` steps the tokens go that the steps so far looked at least (``kv_sinks`` first and
   ``kv_recent`` newest ones stay).
 """
