@@ -11,7 +11,7 @@
 //                 of every row that it meets it leaves a part.  Run w and row-head r meet in part w + r: along the runs one of the two grows by one at a time
 //   decode_join   a warp a row and head joins the parts, the prefix's too, in their order; with scores, further blocks form the weights from the scores that the
 //                 walk left in scratch memory (4 G bytes a token beside the 512 or 264 of its keys and values; what fits L2 is not read from memory again)
-// The arithmetic is that of attention_decode.cu and attention_decode_fp8.cu.  Bound by memory.
+// The arithmetic is that of attention_decode.cu and attention_decode_fp8.cu, but for the factor of fp8 weights (fp8_fragments.cuh).  Bound by memory.
 #include "common.cuh"
 #include "decode_prefix.cuh"
 #include "decode_runs.cuh"
