@@ -126,8 +126,9 @@ def paged_decode_shared(q, k_cache, v_cache, block_tables, context_lens, cu_grou
     for r, n in enumerate(context_lens.tolist()):
         first, common = head.get(r, (r, 0))
         common = min(common, n)
+        own = common // 16                                       # where the row's own table begins to count
         parts = [_page_tokens(k_cache, v_cache, block_tables[first], common, k_scale, v_scale),
-                 tuple(x[:, common:] for x in _page_tokens(k_cache, v_cache, block_tables[r], n, k_scale, v_scale))]
+                 tuple(x[:, common - own * 16:] for x in _page_tokens(k_cache, v_cache, block_tables[r][own:], n - own * 16 if n > common else 0, k_scale, v_scale))]
         out[r] = _decode_row(q[r], *(torch.cat(x, 1) for x in zip(*parts)), scale)[0]
     return out
 

@@ -86,3 +86,28 @@ def scales_of_packed_attention(device, dtype):
 
 def test_scales_of_packed_attention():
     scales_of_packed_attention("cpu", torch.float32)
+
+
+def tables_of_shared_pages(device, wide=False, nobody=-1):
+    """Rows behind the first, and ones that end inside what is shared: their tables need not name whole pages of it.  Entries that do not count are
+    `nobody`; -1 is the page in front of the cache, of NaN."""
+    for fp8 in (False, True):
+        whole = {n: None if x is None else torch.cat([torch.full_like(x[:1], 0x7F if x.dtype == torch.uint8 else float("nan")), x]).to(device) for n, x in pool(fp8=fp8).items()}
+        st = {n: None if x is None else x[1:] for n, x in whole.items()}                    # (page -1 lies in the same memory)
+        full = torch.tensor([[0, 1, 2, 3], [0, 1, 4, 5], [0, 1, 2, 3], [0, 1, 2, 3], [0, 1, 2, 3], [0, 1, 6, 7]], dtype=torch.int32)
+        context, cu, shared = ints(60, 64, 20, 0, 40, 41), ints(0, 6), ints(40)
+        sparse = full.clone()
+        sparse[1:, :2] = nobody
+        sparse[2:5] = nobody                                                                 # they end inside
+        sparse[5, 3] = nobody                                                                # 41 tokens: three pages
+        if wide:
+            full, sparse = (torch.cat([x, torch.full((6, 3000), -1, dtype=torch.int32)], 1) for x in (full, sparse))
+        q = torch.randn(6, 12, 128, generator=torch.Generator().manual_seed(6)).to(torch.bfloat16).to(device)
+        a, b = (ops.paged_decode_shared(q, st["k"], st["v"], t.to(device), context.to(device), cu.to(device), shared.to(device), k_scale=st["ks"], v_scale=st["vs"])
+                for t in (full, sparse))
+        assert torch.equal(a, b) and a.isfinite().all()
+
+
+def test_tables_of_shared_pages():
+    tables_of_shared_pages("cpu")
+    tables_of_shared_pages("cpu", nobody=1_000_000)
