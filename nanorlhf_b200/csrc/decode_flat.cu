@@ -87,8 +87,9 @@ NRL_DEVICE void plan_starts(int4* starts, int owners, int total, int run, From f
   }
 }
 
-NRL_DEVICE int flat_pages(const FlatParams& p, int ctx, int first) {     // that a row walks itself
-  return (ctx + 15) / 16 - first / 16 + (p.prefix_runs == 0 ? (first + 15) / 16 : 0);
+// Pages that a row walks itself.  A row that ends inside the shared tokens has none of its own: its table may say anything of the page where it ends.
+NRL_DEVICE int flat_pages(const FlatParams& p, int ctx, int first) {
+  return (ctx > first ? (ctx + 15) / 16 - first / 16 : 0) + (p.prefix_runs == 0 ? (first + 15) / 16 : 0);
 }
 // The plan of few rows and no prefixes' runs, by every block for itself, a thread a row: no kernel in front.
 NRL_DEVICE const int4* plan_near(const FlatParams& p) {

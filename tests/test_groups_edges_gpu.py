@@ -288,3 +288,9 @@ def test_scales_of_decode(scale, fp8):
             if n_shared == 0:
                 within(scored[row], want, bound, f"scored row {row}")
             row += 1
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_tables_of_shared_pages(wide):
+    from test_groups_edges_cpu import tables_of_shared_pages
+    tables_of_shared_pages(DEV, wide)
